@@ -299,7 +299,7 @@ def _plan(tables, rows, new, tokens, P):
     total = need.cumsum(0)
     head, tail = counters[0], counters[1]
     granted = fits & ((need == 0) | (total <= tail - head))
-    taken = torch.where(granted, total, 0).amax()
+    taken = torch.where(granted & (need > 0), total, 0).amax()
     first = total - need
     after = torch.where(granted, want, old)
     cu = torch.cat([end.new_zeros(1), end]).clamp(max=tokens)
