@@ -374,6 +374,194 @@ int sq_format_decode(const sq_format_pool *pool, const void *slots, int32_t slot
 int sq_format_step(const sq_format_pool *pool, const sq_step_args *args, void *stream);
 
 /*
+ * Keys and values of softmax-attention layers, held in 8 bits in pages.
+ *
+ * A page holds page_tokens tokens of every KV head: per head the keys
+ * [page_tokens, dim], then the values [page_tokens, dim], one byte each;
+ * after all heads, per head two floats, the peaks of its keys and values.
+ * The peak of a (page, head) is the largest magnitude among the tokens that
+ * the page holds (at least 2^-60); a value x is held as
+ *   SQ_KV_INT8  rint(x / peak * 127) + 128, and stands for code * peak / 127
+ *   SQ_KV_FP8   e4m3(x / peak * 448), and stands for code * peak / 448.
+ * A block that is given an infinity or NaN has that peak and reads as NaN.
+ * page_bytes is a multiple of 16 and data 16-byte aligned; page 0 is the
+ * padding page, which no request holds.  dim is 64, 128 or 256; page_tokens
+ * a multiple of 64 with page_tokens * dim <= 32768.
+ */
+enum {
+    SQ_KV_INT8 = 0,
+    SQ_KV_FP8 = 1
+};
+
+typedef struct sq_kv_cache {
+    uint8_t *data;
+    int64_t page_bytes;   /* >= heads * (2 * page_tokens * dim + 8) */
+    int64_t num_pages;
+    int32_t heads;
+    int32_t dim;
+    int32_t page_tokens;
+    int32_t storage;      /* SQ_KV_* */
+} sq_kv_cache;
+
+/*
+ * Block tables of up to `requests` requests.
+ *   table       [requests, width] page of each block of page_tokens tokens
+ *   lens        [requests] tokens held
+ *   free_pages  [capacity] ring of free pages: entry i mod capacity for i in
+ *               [counters[0], counters[1])
+ */
+typedef struct sq_kv_tables {
+    int32_t *table;
+    int32_t *lens;
+    int32_t *free_pages;
+    int64_t *counters;
+    int64_t requests;
+    int64_t capacity;
+    int32_t width;
+    int32_t page_tokens;
+} sq_kv_tables;
+
+/*
+ * How one kind of attention layer splits its work, filled by sq_kv_plan.
+ * One unit is `rows` query rows (token-major, the heads of a group inside a
+ * token) against a range of keys; units of one set of rows that was cut are
+ * joined by a merge.  With tokens, batch, G = q_heads / kv_heads and
+ * s = slots / kv_heads (rounded down where a count is meant):
+ *   max_units    >= ceil(tokens * G / rows) + batch + 1 + s
+ *   max_merges   >= s
+ *   max_partials >= 2 * slots / kv_heads
+ */
+typedef struct sq_kv_schedule {
+    int32_t *units;       /* [max_units, 8] */
+    int32_t *merges;      /* [max_merges, 8] */
+    int32_t max_units;
+    int32_t max_merges;
+    int32_t max_partials;
+    int32_t q_heads;
+    int32_t kv_heads;
+    int32_t rows;         /* 16, 32, 64 or 128 */
+    int32_t causal;
+    int32_t window;       /* 0: none; else the last `window` keys (causal only) */
+    int32_t slots;        /* workgroups that the device holds at once */
+    int32_t min_tiles;    /* least 64-key tiles of a part, at least 1 */
+    int32_t merge_rows;   /* most rows of a unit: min(rows, max_count * G) */
+    int32_t reserved;
+} sq_kv_schedule;
+
+#define SQ_KV_MAX_REQUESTS 4096
+#define SQ_KV_MAX_SCHEDULES 4
+
+/*
+ * New tokens of `batch` requests, in packed rows (request after request):
+ *   rows      [batch] rows of the tables, distinct; counts [batch] new tokens
+ *   cu        [batch + 1] first packed row of each request, at most `tokens`
+ *   slots     [tokens] page * page_tokens + offset, -1 where there is none
+ *   positions [tokens] position within the request, -1 where there is none
+ *   lens      [batch] tokens held afterwards
+ *   granted   [batch] 0 where the request's tokens find no room: the table's
+ *             row is too short, it has more than max_count of them, its
+ *             packed rows pass `tokens`, the tables' row does not exist, or the free pages run out (pages are given in request
+ *             order; from the first request that they do not cover, none that
+ *             needs a page gets one)
+ *   pages     [max_tiles] the pages that new tokens fall into, request by
+ *             request in block order, 0 past the last; filled [max_tiles] the
+ *             tokens that each holds afterwards; tiles [max_tiles, 2] its
+ *             first new offset and the packed row that goes there
+ *   counters  [2] the tables' counters afterwards
+ * max_tiles >= min(tokens, tokens / page_tokens + 2 * batch).
+ */
+typedef struct sq_kv_plan_args {
+    const void *rows;
+    const void *counts;
+    int32_t *cu;
+    int64_t *slots;
+    int32_t *positions;
+    int32_t *lens;
+    uint8_t *granted;
+    int32_t *pages;
+    int32_t *filled;
+    int32_t *tiles;
+    int64_t *counters;
+    int64_t tokens;
+    int32_t batch;
+    int32_t max_tiles;
+    int32_t rows_dtype;    /* SQ_I32 or SQ_I64 */
+    int32_t counts_dtype;
+    int32_t n_schedules;
+    int32_t max_count;     /* most new tokens of a request */
+    sq_kv_schedule schedules[SQ_KV_MAX_SCHEDULES];
+} sq_kv_plan_args;
+
+/*
+ * Fills a plan from the tables and writes the new blocks' pages into the
+ * table; lens and counters stay (a plan that is not committed can be made
+ * again).  sq_kv_commit takes the plan's lengths and pages into the tables.
+ * sq_kv_release gives the pages of n rows back to the ring and empties them;
+ * entries that name a row a second time, or none, are passed over.
+ */
+int sq_kv_plan(const sq_kv_tables *tables, const sq_kv_plan_args *plan, void *stream);
+int sq_kv_commit(const sq_kv_tables *tables, const sq_kv_plan_args *plan, void *stream);
+int sq_kv_release(const sq_kv_tables *tables, const void *rows, int32_t rows_dtype, int64_t n, void *stream);
+
+/*
+ * Quantises the plan's new keys and values into their pages.  k and v are
+ * [tokens, heads, dim] (SQ_BF16 or SQ_F16) with element strides per token and
+ * head, multiples of 8, 16-byte aligned.  A block that starts with a new
+ * token starts afresh; one that holds tokens already keeps the larger peak,
+ * and its codes are brought to it.
+ */
+typedef struct sq_kv_append_args {
+    const void *k;
+    const void *v;
+    const int32_t *pages;
+    const int32_t *filled;
+    const int32_t *tiles;
+    int64_t tokens;
+    int64_t k_stride;
+    int64_t k_head_stride;
+    int64_t v_stride;
+    int64_t v_head_stride;
+    int32_t max_tiles;
+    int32_t dtype;
+} sq_kv_append_args;
+
+int sq_kv_append(const sq_kv_cache *cache, const sq_kv_append_args *args, void *stream);
+
+/*
+ * Pages as dense keys and values [n, page_tokens, heads, dim] of out_dtype,
+ * zero past the first filled[i] tokens (filled NULL: all are taken) and for
+ * pages that the cache does not have.
+ */
+int sq_kv_decode(const sq_kv_cache *cache, const int32_t *pages, const int32_t *filled, int64_t n, void *k, void *v,
+                 int32_t out_dtype, void *stream);
+
+/*
+ * out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the keys that
+ * the plan's schedule lets token t see; zero where it sees none (padding rows
+ * and requests that were not granted among them).
+ *   q    [tokens, q_heads, dim], dtype SQ_BF16 or SQ_F16, strides multiples
+ *        of 8, 16-byte aligned; out contiguous, same dtype
+ *   workspace  max_partials * kv_heads * rows * (dim + 2) floats
+ */
+typedef struct sq_kv_attend_args {
+    const void *q;
+    void *out;
+    float *workspace;
+    const int32_t *table;
+    int64_t requests;
+    int64_t tokens;
+    int64_t q_stride;
+    int64_t q_head_stride;
+    int32_t width;
+    int32_t dtype;
+    float scale;
+    int32_t reserved;
+    sq_kv_schedule schedule;
+} sq_kv_attend_args;
+
+int sq_kv_attend(const sq_kv_cache *cache, const sq_kv_attend_args *args, void *stream);
+
+/*
  * Flags for sq_pool.flags, computed from host copies of bits [H*K],
  * head_meta [H*4] and columns [H].  Returns a non-negative flag set, or a
  * negative SQ_E* code.  Host-only; no device access.

@@ -74,6 +74,50 @@ class FormatPool(ctypes.Structure):
                 ("flags", ctypes.c_int32)]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [("data", _P), ("page_bytes", ctypes.c_int64), ("num_pages", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32),
+                ("storage", ctypes.c_int32)]
+
+
+class KVTables(ctypes.Structure):
+    _fields_ = [("table", _P), ("lens", _P), ("free_pages", _P), ("counters", _P), ("requests", ctypes.c_int64),
+                ("capacity", ctypes.c_int64), ("width", ctypes.c_int32), ("page_tokens", ctypes.c_int32)]
+
+
+class KVSchedule(ctypes.Structure):
+    _fields_ = [("units", _P), ("merges", _P), ("max_units", ctypes.c_int32), ("max_merges", ctypes.c_int32),
+                ("max_partials", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("rows", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("slots", ctypes.c_int32), ("min_tiles", ctypes.c_int32), ("merge_rows", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+KV_INT8, KV_FP8 = 0, 1
+KV_MAX_REQUESTS, KV_MAX_SCHEDULES = 4096, 4
+
+
+class KVPlan(ctypes.Structure):
+    _fields_ = [("rows", _P), ("counts", _P), ("cu", _P), ("slots", _P), ("positions", _P), ("lens", _P),
+                ("granted", _P), ("pages", _P), ("filled", _P), ("tiles", _P), ("counters", _P),
+                ("tokens", ctypes.c_int64), ("batch", ctypes.c_int32), ("max_tiles", ctypes.c_int32),
+                ("rows_dtype", ctypes.c_int32), ("counts_dtype", ctypes.c_int32), ("n_schedules", ctypes.c_int32),
+                ("max_count", ctypes.c_int32), ("schedules", KVSchedule * KV_MAX_SCHEDULES)]
+
+
+class KVAppend(ctypes.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("pages", _P), ("filled", _P), ("tiles", _P), ("tokens", ctypes.c_int64),
+                ("k_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("v_head_stride", ctypes.c_int64), ("max_tiles", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class KVAttend(ctypes.Structure):
+    _fields_ = [("q", _P), ("out", _P), ("workspace", _P), ("table", _P), ("requests", ctypes.c_int64),
+                ("tokens", ctypes.c_int64), ("q_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("width", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("reserved", ctypes.c_int32), ("schedule", KVSchedule)]
+
+
 FMT_FP32, FMT_SYMMETRIC, FMT_DSQ = 0, 1, 2
 FMT_ROWS_CONTIGUOUS = 1
 
@@ -83,7 +127,8 @@ EXPORTS = ("sq_abi_version", "sq_last_error", "sq_encode", "sq_decode_dense", "s
            "sq_prefill_plan", "sq_prefill_split",
            "sq_format_encode", "sq_format_decode", "sq_format_step", "sq_copy_slots_static", "sq_copy_slots_direct",
            "sq_event_create", "sq_event_destroy", "sq_event_record", "sq_event_wait", "sq_event_query",
-           "sq_event_synchronize")
+           "sq_event_synchronize", "sq_kv_plan", "sq_kv_commit", "sq_kv_release", "sq_kv_append", "sq_kv_decode",
+           "sq_kv_attend")
 COPY_STATIC_BYTES = 16 << 20
 COPY_DIRECT_PAGES = 256
 
@@ -132,6 +177,12 @@ def lib():
     L.sq_stream_capture_id.argtypes = [_P, PP(ctypes.c_int32), PP(ctypes.c_uint64)]
     L.sq_create_cu_stream.argtypes = [ctypes.c_int32, ctypes.c_int32, PP(_P), PP(ctypes.c_int32),
                                       PP(ctypes.c_int32)]
+    L.sq_kv_plan.argtypes = [PP(KVTables), PP(KVPlan), _P]
+    L.sq_kv_commit.argtypes = [PP(KVTables), PP(KVPlan), _P]
+    L.sq_kv_release.argtypes = [PP(KVTables), _P, ctypes.c_int32, ctypes.c_int64, _P]
+    L.sq_kv_append.argtypes = [PP(KVCache), PP(KVAppend), _P]
+    L.sq_kv_decode.argtypes = [PP(KVCache), _P, _P, ctypes.c_int64, _P, _P, ctypes.c_int32, _P]
+    L.sq_kv_attend.argtypes = [PP(KVCache), PP(KVAttend), _P]
     for name in EXPORTS:
         if name not in ("sq_last_error",):
             getattr(L, name).restype = ctypes.c_int

@@ -1,0 +1,1125 @@
+// MI355X (gfx950) kernels for keys and values held in 8 bits in pages: block
+// tables and slot maps from request lengths, the quantising write and its
+// read-back, and attention over the pages.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <utility>
+
+#include "internal.h"
+#include "stepquant_hip.h"
+
+// every fused multiply-add is written out, so that codes round as defined
+#pragma clang fp contract(off)
+
+namespace {
+
+typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_v __attribute__((ext_vector_type(8)));
+typedef float f32x4_v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
+
+constexpr float kFloor = 8.673617379884035e-19f;  // 2^-60, the least peak of a block
+constexpr int kTile = 64;                         // keys of one attention tile
+
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// eight 16-bit elements as floats
+__device__ __forceinline__ void widen8(u32x4_v w, int dtype, float x[8]) {
+  if (dtype == SQ_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[2 * i] = bf_lo(w[i]), x[2 * i + 1] = bf_hi(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t pair = w[i];  // (bit_cast of a vector's element takes the vector's first)
+      const half2_v h = __builtin_bit_cast(half2_v, pair);
+      x[2 * i] = (float)h[0], x[2 * i + 1] = (float)h[1];
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+__device__ __forceinline__ uint32_t f16_bits(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+
+__device__ __forceinline__ int64_t load_index(const void *p, int dtype, int64_t i) {
+  return dtype == SQ_I64 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
+}
+
+// ------------------------------------------------------------ block tables
+//
+// Every workgroup scans the requests for itself (they are few) and then
+// serves its share of the tokens and pages, so a plan is one launch; the
+// last workgroups lay out the attention layers' work.
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanItems = SQ_KV_MAX_REQUESTS / kPlanThreads;
+constexpr int kPlanShare = 1024;  // tokens (and page entries) of one workgroup
+
+struct PlanDev {
+  sq_kv_tables t;
+  sq_kv_plan_args p;
+  int share_blocks;
+};
+
+// Inclusive prefix sums over the workgroup, and the total.
+template <int NT>
+__device__ int64_t block_scan(int64_t x, int64_t *total, int64_t *waves) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; w++) {
+    if (w < wave) before += waves[w];
+    all += waves[w];
+  }
+  *total = all;
+  return x + before;
+}
+
+// First index whose entry exceeds x (n when none does).
+__device__ __forceinline__ int upper_bound(const int32_t *a, int n, int x) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] > x) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// What a workgroup knows of the requests, [batch] each, in LDS.
+struct PlanLds {
+  int32_t *end;    // end of the request's packed rows, at most `tokens`
+  int32_t *old;    // tokens held; -1: not granted
+  int32_t *tiles;  // end of its page entries (then: of its sets of query rows)
+  int32_t *first;  // first of its new pages among those of the plan
+  int32_t *row;
+};
+
+// One attention layer's units: sets of `rows` query rows, the longest key
+// ranges of a request first, each cut into near-equal parts of at most
+// `chunk` key tiles.  chunk is the work that each of the device's slots has
+// when it is spread evenly, so a set is cut only where it would outlast the
+// others.
+__device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, int64_t *waves) {
+  const int tid = threadIdx.x, B = p.batch, G = s.q_heads / s.kv_heads, tokens = (int)p.tokens;
+  const int NB = B + 1;  // the last: packed rows past every request's
+  auto row_count = [&](int b) { return (b < B ? L.end[b] : tokens) - (b ? L.end[b - 1] : 0); };
+  int64_t sum = 0, total;
+  const int items = (NB + kPlanThreads - 1) / kPlanThreads;
+  for (int i = 0; i < items; i++) {
+    const int b = tid * items + i;
+    if (b < NB) sum += ((int64_t)row_count(b) * G + s.rows - 1) / s.rows;
+  }
+  int64_t at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
+  for (int i = 0; i < items; i++) {
+    const int b = tid * items + i;
+    if (b < NB) L.tiles[b] = (int32_t)(at += ((int64_t)row_count(b) * G + s.rows - 1) / s.rows);
+  }
+  __syncthreads();
+  const int sets = (int)total;
+  struct Set {
+    int b, f0, rows, kv0, kv1, n;
+  };
+  auto find = [&](int e) {
+    Set r;
+    r.b = upper_bound(L.tiles, NB, e);
+    const int i = L.tiles[r.b] - 1 - e;  // the request's last rows first
+    const int all = row_count(r.b) * G;
+    r.f0 = i * s.rows;
+    r.rows = min(s.rows, all - r.f0);
+    r.kv0 = r.kv1 = r.n = 0;
+    const int old = r.b < B ? L.old[r.b] : -1;
+    if (old >= 0) {
+      const int held = old + row_count(r.b);
+      r.kv1 = s.causal ? old + (r.f0 + r.rows - 1) / G + 1 : held;
+      if (s.window > 0) r.kv0 = max(0, old + r.f0 / G - s.window + 1) & ~(kTile - 1);
+      r.n = (r.kv1 - r.kv0 + kTile - 1) / kTile;
+    }
+    return r;
+  };
+  sum = 0;
+  for (int e = tid; e < sets; e += kPlanThreads) sum += find(e).n;
+  block_scan<kPlanThreads>(sum, &total, waves);
+  const int64_t chunk = max((int64_t)s.min_tiles, (total * s.kv_heads + s.slots - 1) / s.slots);
+  int units = 0, parts = 0, merges = 0;
+  for (int e0 = 0; e0 < sets; e0 += kPlanThreads) {
+    const int e = e0 + tid;
+    Set r = {};
+    int k = 0;
+    if (e < sets) {
+      r = find(e);
+      k = max(1, (int)((r.n + chunk - 1) / chunk));
+    }
+    const int cut = k > 1;
+    // three sums in one: units and parts stay below 2^24, merges below 2^16
+    const int64_t mine = (int64_t)k | (int64_t)(cut ? k : 0) << 24 | (int64_t)cut << 48;
+    const int64_t upto = block_scan<kPlanThreads>(mine, &total, waves) - mine;
+    const int u = units + (int)(upto & 0xffffff), q = parts + (int)(upto >> 24 & 0xffffff), m = merges + (int)(upto >> 48);
+    const int q0 = e < sets && r.b ? L.end[r.b - 1] : 0;
+    for (int j = 0; j < k; j++) {
+      if (u + j >= s.max_units) break;
+      int32_t *o = s.units + 8 * (int64_t)(u + j);
+      const int t0 = (int)((int64_t)r.n * j / k), t1 = (int)((int64_t)r.n * (j + 1) / k);
+      o[0] = r.b < B ? L.row[r.b] : 0;
+      o[1] = q0;
+      o[2] = r.f0;
+      o[3] = r.rows;
+      o[4] = r.b < B ? L.old[r.b] : 0;
+      o[5] = r.kv0 + t0 * kTile;
+      o[6] = min(r.kv1, r.kv0 + t1 * kTile);
+      o[7] = cut ? q + j : -1;
+    }
+    if (cut && m < s.max_merges) {
+      int32_t *o = s.merges + 8 * (int64_t)m;
+      o[0] = q0;
+      o[1] = r.f0;
+      o[2] = r.rows;
+      o[3] = q;
+      o[4] = k;
+    }
+    units += (int)(total & 0xffffff), parts += (int)(total >> 24 & 0xffffff), merges += (int)(total >> 48);
+  }
+  for (int u = units + tid; u < s.max_units; u += kPlanThreads) s.units[8 * (int64_t)u + 3] = 0;
+  for (int m = merges + tid; m < s.max_merges; m += kPlanThreads) s.merges[8 * (int64_t)m + 2] = 0;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanDev d) {
+  extern __shared__ int32_t lds[];
+  __shared__ int64_t waves[kPlanThreads / 64];
+  const sq_kv_tables &t = d.t;
+  const sq_kv_plan_args &p = d.p;
+  const int tid = threadIdx.x, B = p.batch, P = t.page_tokens;
+  PlanLds L;
+  L.end = lds;
+  L.old = L.end + B + 1;
+  L.tiles = L.old + B + 1;
+  L.first = L.tiles + B + 1;
+  L.row = L.first + B + 1;
+  const int items = (B + kPlanThreads - 1) / kPlanThreads;
+  const int64_t head = t.counters[0], tail = t.counters[1];
+  const int64_t room = tail - head;
+  int row[kPlanItems], old[kPlanItems], cnt[kPlanItems];
+  int64_t sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < kPlanItems; i++) {
+    const int b = tid * items + i;
+    row[i] = -1, old[i] = -1, cnt[i] = 0;
+    if (i < items && b < B) {
+      const int64_t r = load_index(p.rows, p.rows_dtype, b), n = load_index(p.counts, p.counts_dtype, b);
+      // more than `tokens` rows never fit: the sums stay within 64 bits
+      cnt[i] = (int)(n < 0 ? 0 : n > p.tokens + 1 ? p.tokens + 1 : n);
+      if (r >= 0 && r < t.requests) {
+        row[i] = (int)r;
+        old[i] = t.lens[r];
+      }
+      sum += cnt[i];
+    }
+  }
+  int64_t at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
+  int64_t need[kPlanItems];
+  bool fits[kPlanItems];
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanItems; i++) {
+    const int b = tid * items + i;
+    need[i] = 0, fits[i] = false;
+    if (i < items && b < B) {
+      at += cnt[i];
+      L.end[b] = (int32_t)min(at, p.tokens);
+      const int64_t want = (int64_t)old[i] + cnt[i], blocks = (want + P - 1) / P;
+      fits[i] = old[i] >= 0 && cnt[i] <= p.max_count && blocks <= t.width && at <= p.tokens && want <= 0x7fffffff;
+      if (fits[i]) need[i] = blocks - (old[i] + (int64_t)P - 1) / P;
+      sum += need[i];
+    }
+  }
+  at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
+  int64_t taken = 0;
+  int touched[kPlanItems];
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanItems; i++) {
+    const int b = tid * items + i;
+    touched[i] = 0;
+    if (i < items && b < B) {
+      const int64_t first = at;
+      at += need[i];
+      const bool ok = fits[i] && (need[i] == 0 || at <= room);
+      if (ok && need[i]) taken = at;
+      L.row[b] = row[i];
+      L.first[b] = ok ? (int32_t)min(first, (int64_t)0x7fffffff) : 0;
+      L.old[b] = ok ? old[i] : -1;
+      if (ok && cnt[i]) touched[i] = (int)((old[i] + (int64_t)cnt[i] + P - 1) / P - old[i] / P);
+      sum += touched[i];
+      if (blockIdx.x == 0) {
+        p.lens[b] = row[i] < 0 ? 0 : ok ? old[i] + cnt[i] : old[i];
+        p.granted[b] = ok;
+      }
+    }
+  }
+  at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
+#pragma unroll
+  for (int i = 0; i < kPlanItems; i++) {
+    const int b = tid * items + i;
+    if (i < items && b < B) L.tiles[b] = (int32_t)(at += touched[i]);
+  }
+  const int n_tiles = (int)total;
+  __syncthreads();
+  if ((int)blockIdx.x >= d.share_blocks) {
+    plan_schedule(p.schedules[blockIdx.x - d.share_blocks], p, L, waves);
+    return;
+  }
+  if (blockIdx.x == 0) {
+    // the pages taken: those of the last request that needed and got one
+    block_scan<kPlanThreads>(0, &total, waves);
+    int64_t best = taken;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) best = max(best, (int64_t)__shfl_xor(best, k, 64));
+    if ((tid & 63) == 0) waves[tid >> 6] = best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kPlanThreads / 64; w++) best = max(best, waves[w]);
+      p.counters[0] = head + best;
+      p.counters[1] = tail;
+      p.cu[0] = 0;
+    }
+    for (int b = tid; b < B; b += kPlanThreads) p.cu[b + 1] = L.end[b];
+  }
+  const int64_t h0 = head % t.capacity;
+  // the page of a request's block: its own, or the ring's entry that it gets
+  auto page_of = [&](int b, int block) {
+    const int had = (int)((L.old[b] + (int64_t)P - 1) / P);
+    if (block < had) return t.table[(int64_t)L.row[b] * t.width + block];
+    int64_t i = h0 + L.first[b] + (block - had);
+    if (i >= t.capacity) i -= t.capacity;
+    return t.free_pages[i];
+  };
+  const int from = blockIdx.x * kPlanShare, upto = from + kPlanShare;
+  for (int i = from + tid; i < upto && i < p.tokens; i += kPlanThreads) {
+    const int b = upper_bound(L.end, B, i);
+    int64_t slot = -1;
+    int pos = -1;
+    if (b < B && L.old[b] >= 0) {
+      pos = L.old[b] + i - (b ? L.end[b - 1] : 0);
+      slot = (int64_t)page_of(b, pos / P) * P + pos % P;
+    }
+    p.slots[i] = slot;
+    p.positions[i] = pos;
+  }
+  for (int i = from + tid; i < upto && i < p.max_tiles; i += kPlanThreads) {
+    int page = 0, filled = 0, start = 0, token = 0;
+    if (i < n_tiles) {
+      const int b = upper_bound(L.tiles, B, i);
+      const int old = L.old[b], base = b ? L.end[b - 1] : 0;
+      const int block = old / P + i - (b ? L.tiles[b - 1] : 0);
+      page = page_of(b, block);
+      if (block >= (int)((old + (int64_t)P - 1) / P)) t.table[(int64_t)L.row[b] * t.width + block] = page;
+      start = max(0, old - block * P);
+      token = base + max(0, block * P - old);
+      filled = (int)min((int64_t)P, (int64_t)old + L.end[b] - base - (int64_t)block * P);
+    }
+    p.pages[i] = page;
+    p.filled[i] = filled;
+    p.tiles[2 * (int64_t)i] = start;
+    p.tiles[2 * (int64_t)i + 1] = token;
+  }
+}
+
+__global__ __launch_bounds__(256) void kv_commit_kernel(PlanDev d) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b == 0) d.t.counters[0] = d.p.counters[0];
+  if (b >= d.p.batch) return;
+  const int64_t r = load_index(d.p.rows, d.p.rows_dtype, b);
+  if (r >= 0 && r < d.t.requests) d.t.lens[r] = d.p.lens[b];
+}
+
+// One workgroup: pages go back in the order of the rows and their blocks.
+__global__ __launch_bounds__(kPlanThreads) void kv_release_kernel(sq_kv_tables t, const void *rows, int rows_dtype, int n) {
+  extern __shared__ int32_t lds[];
+  __shared__ int64_t waves[kPlanThreads / 64];
+  int32_t *end = lds, *row = lds + n;
+  const int tid = threadIdx.x, items = (n + kPlanThreads - 1) / kPlanThreads;
+  const int64_t tail = t.counters[1];
+  int64_t sum = 0, total;
+  for (int i = 0; i < items; i++) {
+    const int b = tid * items + i;
+    if (b >= n) break;
+    const int64_t r = load_index(rows, rows_dtype, b);
+    // the exchange leaves a row's pages to one of the entries that name it
+    const int len = r >= 0 && r < t.requests ? atomicExch(&t.lens[r], 0) : 0;
+    row[b] = (int)(r >= 0 && r < t.requests ? r : 0);
+    end[b] = len > 0 ? (int)min(((int64_t)len + t.page_tokens - 1) / t.page_tokens, (int64_t)t.width) : 0;
+    sum += end[b];
+  }
+  int64_t at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
+  for (int i = 0; i < items; i++) {
+    const int b = tid * items + i;
+    if (b < n) end[b] = (int32_t)(at += end[b]);
+  }
+  __syncthreads();
+  const int64_t t0 = tail % t.capacity;
+  for (int64_t i = tid; i < total; i += kPlanThreads) {
+    const int b = upper_bound(end, n, (int)i);
+    int32_t *entry = t.table + (int64_t)row[b] * t.width + (i - (b ? end[b - 1] : 0));
+    t.free_pages[(t0 + i) % t.capacity] = *entry;
+    *entry = 0;
+  }
+  if (tid == 0) t.counters[1] = tail + total;
+}
+
+// ------------------------------------------------------------ codes
+
+// x / d rounded to nearest for a divisor of at most 11 significant bits, from
+// its rounded reciprocal: one correction with the exact residual (as in the
+// packed pages' fit; x and the quotient of normal size, which they are
+// wherever the code is not 0).
+__device__ __forceinline__ float quotient(float x, float d, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, d, x), inv, q);
+}
+
+// four values, each at most `top` in magnitude, as one word of codes
+template <bool FP8>
+__device__ __forceinline__ uint32_t code4(const float y[4]) {
+  if (FP8) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  }
+  // 1.5 * 2^23 + 128: the sum's low byte is rint(y) + 128
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) u[i] = __float_as_uint(y[i] + 12583040.f);
+  const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400), b = __builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400);
+  return a | b << 16;
+}
+
+template <bool FP8>
+__device__ __forceinline__ void decode4(uint32_t w, float x[4]) {
+  if (FP8) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = (float)(int)(w >> 8 * i & 255) - 128.f;
+  }
+}
+
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// One workgroup per (page entry, head, keys or values); a thread holds N
+// groups of 8 adjacent dims, so the new values are read once.
+template <bool FP8, int N>
+__global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_append_args a, int log_dim) {
+  __shared__ uint32_t peaks[4];
+  const int tid = threadIdx.x, tile = blockIdx.x, h = blockIdx.y, part = blockIdx.z;
+  const int64_t page = a.pages[tile];
+  const int start = a.tiles[2 * (int64_t)tile], token = a.tiles[2 * (int64_t)tile + 1], filled = a.filled[tile];
+  if (page <= 0 || page >= c.num_pages) return;
+  if (start < 0 || start >= filled || filled > c.page_tokens || token < 0 || token + (int64_t)filled - start > a.tokens)
+    return;
+  const float top = FP8 ? 448.f : 127.f;
+  const uint16_t *src = (const uint16_t *)(part ? a.v : a.k) + h * (part ? a.v_head_stride : a.k_head_stride);
+  const int64_t stride = part ? a.v_stride : a.k_stride;
+  uint8_t *base = c.data + page * c.page_bytes + ((int64_t)(2 * h + part) * c.page_tokens << log_dim);
+  float *peak_at = (float *)(c.data + page * c.page_bytes + (2 * (int64_t)c.heads * c.page_tokens << log_dim)) + 2 * h + part;
+  const int from = start << (log_dim - 3), upto = filled << (log_dim - 3);
+  u32x4_v x[N];
+  uint32_t most = 0;  // magnitudes as bits: their order, and NaN above all
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int g = from + i * 256 + tid;
+    if (g < upto) {
+      const int e = g << 3, t = e >> log_dim;
+      x[i] = *(const u32x4_v *)(src + (int64_t)(token + t - start) * stride + (e & ((1 << log_dim) - 1)));
+#pragma unroll
+      for (int k = 0; k < 4; k++) most = max(most, max(x[i][k] & 0x7fffu, x[i][k] >> 16 & 0x7fffu));
+    }
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, k, 64));
+  if ((tid & 63) == 0) peaks[tid >> 6] = most;
+  const float before = start ? *peak_at : kFloor;
+  __syncthreads();
+  most = max(max(peaks[0], peaks[1]), max(peaks[2], peaks[3]));
+  const float fresh = a.dtype == SQ_BF16 ? bf_lo(most) : (float)__builtin_bit_cast(_Float16, (uint16_t)most);
+  // the larger of the two, as magnitudes' bits, so that NaN stays
+  const float peak = __uint_as_float(max(max(__float_as_uint(fresh), __float_as_uint(before) & 0x7fffffffu),
+                                         __float_as_uint(kFloor)));
+  const float inv = 1.f / peak;
+  const bool good = finite(peak);
+  if (tid == 0) *peak_at = peak;
+  const uint32_t zero = FP8 ? 0u : 0x80808080u;
+  if (peak != before) {
+    for (int g = tid; g < from; g += 256) {
+      uint2 w = *(const uint2 *)(base + 8 * (int64_t)g);
+      float y[8];
+      decode4<FP8>(w.x, y);
+      decode4<FP8>(w.y, y + 4);
+#pragma unroll
+      for (int k = 0; k < 8; k++) y[k] = quotient(y[k] * before, peak, inv);
+      w.x = good ? code4<FP8>(y) : zero;
+      w.y = good ? code4<FP8>(y + 4) : zero;
+      *(uint2 *)(base + 8 * (int64_t)g) = w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int g = from + i * 256 + tid;
+    if (g < upto) {
+      float y[8];
+      widen8(x[i], a.dtype, y);
+#pragma unroll
+      for (int k = 0; k < 8; k++) y[k] = quotient(y[k], peak, inv) * top;
+      *(uint2 *)(base + 8 * (int64_t)g) = make_uint2(good ? code4<FP8>(y) : zero, good ? code4<FP8>(y + 4) : zero);
+    }
+  }
+}
+
+template <bool FP8>
+__global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int32_t *pages, const int32_t *filled, void *k,
+                                                        void *v, int dtype, int log_dim) {
+  const int tid = threadIdx.x, h = blockIdx.y, part = blockIdx.z;
+  const int64_t n = blockIdx.x;
+  const int64_t page = pages[n];
+  const bool there = page > 0 && page < c.num_pages;
+  const int held = there ? filled ? filled[n] : c.page_tokens : 0;
+  const uint8_t *at = c.data + (there ? page : 0) * c.page_bytes;
+  const uint8_t *base = at + ((int64_t)(2 * h + part) * c.page_tokens << log_dim);
+  const float scale = ((const float *)(at + (2 * (int64_t)c.heads * c.page_tokens << log_dim)))[2 * h + part] / (FP8 ? 448.f : 127.f);
+  void *out = part ? v : k;
+  const int groups = c.page_tokens << (log_dim - 3);
+  for (int g = tid; g < groups; g += 256) {
+    const int t = g >> (log_dim - 3), d = (g << 3) & ((1 << log_dim) - 1);
+    float x[8] = {};
+    if (t < held) {
+      const uint2 w = *(const uint2 *)(base + 8 * (int64_t)g);
+      decode4<FP8>(w.x, x);
+      decode4<FP8>(w.y, x + 4);
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] *= scale;
+    }
+    const int64_t o = (((n * c.page_tokens + t) * c.heads + h) << log_dim) + d;
+    if (dtype == SQ_F32) {
+      *(float4 *)((float *)out + o) = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4 *)((float *)out + o + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      u32x4_v w;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        w[i] = dtype == SQ_BF16 ? bf16_bits(x[2 * i]) | bf16_bits(x[2 * i + 1]) << 16
+                                : f16_bits(x[2 * i]) | f16_bits(x[2 * i + 1]) << 16;
+      *(u32x4_v *)((uint16_t *)out + o) = w;
+    }
+  }
+}
+
+// ------------------------------------------------------------ attention
+//
+// A unit's keys go by tiles of 64.  S^T = K Q^T and O^T = V^T P^T run as
+// 16x16x32 half-precision products: a query row is a column, so a lane holds
+// scores and outputs of one row only, and the rounded probabilities of one
+// product are the operand of the next without leaving their registers.
+// Codes of at most 8 bits are exact as halves, and so are queries: a row is
+// brought near 2^14 by a power of two first, where bfloat16's 8 bits fit.
+
+struct AttendDev {
+  sq_kv_cache c;
+  const uint16_t *q;
+  uint16_t *out;
+  float *ws;
+  const int32_t *table;
+  const int32_t *units;
+  const int32_t *merges;
+  int64_t requests, tokens, q_stride, q_head_stride;
+  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials;
+  float scale;
+};
+
+__device__ __forceinline__ float reduce_max4(float x) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float reduce_sum4(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ uint32_t half2_bits(half2_v h) { return __builtin_bit_cast(uint32_t, h); }
+
+// two keys' codes (bytes 2 i and 2 i + 1 of w) as halves
+template <bool FP8, int I>
+__device__ __forceinline__ uint32_t key2(uint32_t w) {
+  if (FP8) return half2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, I));
+  // 0x64uu is 1024 + u
+  const uint32_t m = __builtin_amdgcn_perm(0x64646464u, w, I ? 0x04030402 : 0x04010400);
+  return half2_bits(__builtin_bit_cast(half2_v, m) - (half2_v){(_Float16)1152.f, (_Float16)1152.f});
+}
+
+// One dim of eight tokens (byte E of each w) as halves; int8 codes come out
+// 2^-10 of their size: a byte is the half u 2^-24, and one fused product
+// makes it (u - 128) 2^-10.
+template <bool FP8, int E>
+__device__ __forceinline__ half8_v value8(const uint32_t w[8]) {
+  uint32_t o[4];
+  if (FP8) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t m = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x0c0c0000 | (4 + E) << 8 | E);
+      o[i] = half2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)m, 1.f, false));
+    }
+  } else {
+    const half2_v mul = {(_Float16)16384.f, (_Float16)16384.f}, add = {(_Float16)-.125f, (_Float16)-.125f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t m = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x0c000c00 | (4 + E) << 16 | E);
+      o[i] = half2_bits(__builtin_elementwise_fma(__builtin_bit_cast(half2_v, m), mul, add));
+    }
+  }
+  return __builtin_bit_cast(half8_v, *(u32x4_v *)o);
+}
+
+template <typename F, int... E>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, E...>) {
+  (f(std::integral_constant<int, E>{}), ...);
+}
+
+template <int D>
+struct alignas(D / 16) Bytes {  // a lane's bytes of one token's values
+  uint32_t w[D / 64];
+};
+
+// Units of up to 16 RT rows: the four waves take a unit's tiles in turn and
+// are joined at its end; keys and values go from memory to registers.
+template <int D, int RT, bool FP8>
+__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendDev a) {
+  extern __shared__ float smem[];
+  constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int h = blockIdx.x % a.kv_heads;
+  const int32_t *u = a.units + 8 * (int64_t)(blockIdx.x / a.kv_heads);
+  const int row = u[0], q0 = u[1], f0 = u[2], rows = u[3], pos0 = u[4], kv0 = u[5], part = u[7];
+  // a row of the table that does not exist holds no keys
+  const int kv1 = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
+  const int G = a.q_heads / a.kv_heads;
+  if (rows <= 0 || rows > 16 * RT || q0 < 0 || f0 < 0 || q0 + (int64_t)(f0 + rows - 1) / G >= a.tokens) return;
+  // queries
+  half8_v qf[RT][KS];
+  float mult[RT], m[RT], l[RT];
+  int hi[RT], lo[RT];
+  f32x4_v o[RT][DT];
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    const int f = f0 + 16 * r + c;
+    const bool live = 16 * r + c < rows;
+    const int t = live ? f / G : 0, head = h * G + (live ? f - t * G : 0);
+    const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 16 * g;
+    u32x4_v w[D / 64][2];
+#pragma unroll
+    for (int s = 0; s < D / 64; s++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) w[s][k] = live ? *(const u32x4_v *)(src + 64 * s + 8 * k) : (u32x4_v){0, 0, 0, 0};
+    float unit = 1.f;
+    if (a.dtype == SQ_BF16) {
+      float most = 0;
+#pragma unroll
+      for (int s = 0; s < D / 64; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][k][i])), fabsf(bf_hi(w[s][k][i]))));
+      most = reduce_max4(most);
+      // 2^(14 - e) brings the row's largest, in [2^e, 2^(e+1)), below 2^15
+      const int e = (int)(__float_as_uint(most) >> 23) - 127;
+      const bool plain = e > -100 && e < 100;
+      const float shift = plain ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 1.f;
+      unit = plain ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 1.f;
+#pragma unroll
+      for (int s = 0; s < D / 64; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            w[s][k][i] = f16_bits(bf_lo(w[s][k][i]) * shift) | f16_bits(bf_hi(w[s][k][i]) * shift) << 16;
+    }
+#pragma unroll
+    for (int s = 0; s < KS; s++) qf[r][s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
+    mult[r] = a.scale * 1.4426950408889634f * unit * (FP8 ? 1.f / 448.f : 1.f / 127.f);
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    hi[r] = live ? (a.causal ? pos0 + t + 1 : kv1) : kv1;
+    lo[r] = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
+#pragma unroll
+    for (int e = 0; e < DT; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
+  }
+  // tiles that every row sees whole need no mask: below the first row's last
+  // key and from the last row's first one on
+  const int all_hi = min(kv1, a.causal ? pos0 + f0 / G + 1 : kv1);
+  const int all_lo = a.window > 0 ? pos0 + (f0 + rows - 1) / G - a.window + 1 : 0;
+  const int P = a.c.page_tokens, per = P / kTile, log_per = 31 - __clz(per);
+  const bool pow2 = (per & (per - 1)) == 0;
+  const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
+  const int n = (kv1 - kv0 + kTile - 1) / kTile;
+  const int32_t *entries = a.table + (int64_t)row * a.width;
+  auto entry_of = [&](int tile) { return pow2 ? tile >> log_per : tile / per; };
+  int ids = 0;
+  Bytes<D> vf[2][8];
+  u32x4_v kf[4][D / 64];
+  int page = 0;
+  const uint8_t *tile_at = nullptr;
+  // page and tile of step i; the lanes hold the pages of 64 steps
+  auto locate = [&](int i) {
+    const int tile = kv0 / kTile + i;
+    const int p = __builtin_amdgcn_readlane(ids, (i >> 2) & 63);
+    page = p > 0 && p < a.c.num_pages ? p : 0;
+    tile_at = a.c.data + page * a.c.page_bytes;
+    return tile_at + ((int64_t)(2 * h) * P + (tile - entry_of(tile) * per) * kTile) * D;
+  };
+  auto fetch_ids = [&](int i) {
+    const int mine = i + 4 * lane;
+    ids = mine < n ? entries[entry_of(kv0 / kTile + mine)] : 0;
+  };
+  auto load_keys = [&](const uint8_t *at) {
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int s = 0; s < D / 64; s++) kf[t][s] = *(const u32x4_v *)(at + (16 * t + c) * D + 64 * s + 16 * g);
+  };
+  const uint8_t *at = nullptr;
+  if (wave < n) {
+    fetch_ids(wave);
+    at = locate(wave);
+    load_keys(at);
+  }
+  for (int i = wave; i < n; i += 4) {
+    const float2 peak = *(const float2 *)(tile_at + peaks_at);
+    const int first = kv0 + i * kTile;
+    const bool known = page != 0;
+    {
+      const uint8_t *vat = at + (int64_t)P * D;
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          vf[s][j] = *(const Bytes<D> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
+    }
+    f32x4_v s[RT][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int r = 0; r < RT; r++) s[r][t] = (f32x4_v){0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        u32x4_v w;
+        const uint32_t w0 = kf[t][k / 2][2 * (k & 1)], w1 = kf[t][k / 2][2 * (k & 1) + 1];
+        w[0] = key2<FP8, 0>(w0), w[1] = key2<FP8, 1>(w0), w[2] = key2<FP8, 0>(w1), w[3] = key2<FP8, 1>(w1);
+        const half8_v kh = __builtin_bit_cast(half8_v, w);
+#pragma unroll
+        for (int r = 0; r < RT; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[r][k], s[r][t], 0, 0, 0);
+      }
+    }
+    if (i + 4 < n) {
+      if ((((i + 4) >> 2) & 63) == 0) fetch_ids(i + 4);
+      at = locate(i + 4);
+      load_keys(at);
+    }
+    const bool whole = known && first + kTile <= all_hi && first >= all_lo;
+    half8_v pf[RT][2];
+    float alpha[RT], sv[RT];
+    bool same = true;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      const float f = mult[r] * peak.x;
+      float best = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          float x = s[r][t][k] * f;
+          if (!whole) {
+            const int j = first + 16 * t + 4 * g + k;
+            x = known && j < hi[r] && j >= lo[r] && j < kv1 ? x : -INFINITY;
+          }
+          s[r][t][k] = x;
+          best = fmaxf(best, x);
+        }
+      best = fmaxf(reduce_max4(best), m[r]);
+      const float base = best == -INFINITY ? 0.f : best;
+      alpha[r] = __builtin_amdgcn_exp2f(m[r] - base);
+      same = same && m[r] == best;
+      m[r] = best;
+      float sum = 0;
+      uint32_t w[2][4];
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          p[k] = __builtin_amdgcn_exp2f(s[r][t][k] - base);
+          sum += p[k];
+        }
+        w[t >> 1][2 * (t & 1)] = f16_bits(p[0]) | f16_bits(p[1]) << 16;
+        w[t >> 1][2 * (t & 1) + 1] = f16_bits(p[2]) | f16_bits(p[3]) << 16;
+      }
+      l[r] = fmaf(l[r], alpha[r], sum);
+      pf[r][0] = __builtin_bit_cast(half8_v, *(u32x4_v *)w[0]);
+      pf[r][1] = __builtin_bit_cast(half8_v, *(u32x4_v *)w[1]);
+      // a row that sees none of the tile takes nothing from it, whatever its peak
+      const bool some = whole || (known && first < min(hi[r], kv1) && first + kTile > lo[r]);
+      sv[r] = some ? peak.y * (FP8 ? 1.f / 448.f : 1024.f / 127.f) : 0.f;
+    }
+    const bool keep = __all(same);
+    auto value = [&](auto E) {
+      constexpr int e = decltype(E)::value;
+      half8_v v[2];
+#pragma unroll
+      for (int s2 = 0; s2 < 2; s2++) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = vf[s2][j].w[e / 4];
+        v[s2] = value8<FP8, e & 3>(w);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        f32x4_v x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], pf[r][0], (f32x4_v){0, 0, 0, 0}, 0, 0, 0);
+        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], pf[r][1], x, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float was = keep ? o[r][e][k] : o[r][e][k] * alpha[r];
+          o[r][e][k] = fmaf(x[k], sv[r], was);
+        }
+      }
+    };
+    each(value, std::make_integer_sequence<int, DT>{});
+  }
+  // the four waves' shares of each row, joined through LDS
+  float *so = smem;                  // [4][16][LDO]
+  float *sm = smem + 4 * 16 * LDO;   // [4][16] maxima, then sums
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    const float sum = reduce_sum4(l[r]);
+    if (r) __syncthreads();
+    if (g == 0) {
+      sm[16 * wave + c] = m[r];
+      sm[64 + 16 * wave + c] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
+#pragma unroll
+      for (int e = 0; e < DT; e += 4)
+        *(f32x4_v *)(dst + e) = (f32x4_v){o[r][e][k], o[r][e + 1][k], o[r][e + 2][k], o[r][e + 3][k]};
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * (D / 4); i += 256) {
+      const int j = i / (D / 4), d = 4 * (i % (D / 4));
+      if (16 * r + j >= rows) continue;
+      float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float sum2 = 0;
+      f32x4_v x = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
+        sum2 = fmaf(sm[64 + 16 * w + j], f, sum2);
+        x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
+      }
+      const int f = f0 + 16 * r + j;
+      if (part < 0) {
+        const float inv = sum2 == 0.f ? 0.f : 1.f / sum2;
+        x *= inv;
+        const int t = f / G, head = h * G + f - t * G;
+        uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + d;
+        uint2 w;
+        if (a.dtype == SQ_BF16) {
+          w.x = bf16_bits(x[0]) | bf16_bits(x[1]) << 16;
+          w.y = bf16_bits(x[2]) | bf16_bits(x[3]) << 16;
+        } else {
+          w.x = f16_bits(x[0]) | f16_bits(x[1]) << 16;
+          w.y = f16_bits(x[2]) | f16_bits(x[3]) << 16;
+        }
+        *(uint2 *)dst = w;
+      } else {
+        const int64_t slot = ((int64_t)part * a.kv_heads + h) * (16 * RT) + 16 * r + j;
+        *(f32x4_v *)(a.ws + slot * D + d) = x;
+        if (d == 0) {
+          float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * (16 * RT) * D + 2 * slot;
+          ml[0] = mm;
+          ml[1] = sum2;
+        }
+      }
+    }
+  }
+}
+
+// Joins the parts of one query row: one workgroup per (merge, head, row).
+template <int D>
+__global__ __launch_bounds__(256) void kv_merge_kernel(AttendDev a, int R) {
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ f32x4_v part_o[GROUPS][LANES];
+  __shared__ float part_l[GROUPS];
+  const int tid = threadIdx.x, j = blockIdx.y, h = blockIdx.x % a.kv_heads;
+  const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.kv_heads);
+  const int rows = u[2];
+  if (j >= rows) return;
+  const int q0 = u[0], f = u[1] + j, p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
+  const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * R + j, step = (int64_t)a.kv_heads * R;
+  const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * R * D;
+  float mm = -INFINITY;
+  for (int i = 0; i < n; i++) mm = fmaxf(mm, ml[2 * (slot0 + i * step)]);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  const int lane = tid % LANES, grp = tid / LANES;
+  f32x4_v x = {0, 0, 0, 0};
+  float sum = 0;
+  for (int i = grp; i < n; i += GROUPS) {
+    const int64_t s = slot0 + i * step;
+    const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base);
+    sum += ml[2 * s + 1] * w;
+    x += *(const f32x4_v *)(a.ws + s * D + 4 * lane) * w;
+  }
+  part_o[grp][lane] = x;
+  if (lane == 0) part_l[grp] = sum;
+  __syncthreads();
+  if (grp) return;
+  sum = 0;
+  x = (f32x4_v){0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < GROUPS; i++) {
+    x += part_o[i][lane];
+    sum += part_l[i];
+  }
+  x *= sum == 0.f ? 0.f : 1.f / sum;
+  const int t = f / G, head = h * G + f - t * G;
+  uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane;
+  uint2 w;
+  if (a.dtype == SQ_BF16) {
+    w.x = bf16_bits(x[0]) | bf16_bits(x[1]) << 16;
+    w.y = bf16_bits(x[2]) | bf16_bits(x[3]) << 16;
+  } else {
+    w.x = f16_bits(x[0]) | f16_bits(x[1]) << 16;
+    w.y = f16_bits(x[2]) | f16_bits(x[3]) << 16;
+  }
+  *(uint2 *)dst = w;
+}
+
+// ------------------------------------------------------------ host side
+
+int fail(int code, const char *msg) { return sq_internal_fail(code, msg); }
+
+bool index_type(int32_t dtype) { return dtype == SQ_I32 || dtype == SQ_I64; }
+
+int check_cache(const sq_kv_cache *c) {
+  if (!c || !c->data || ((uintptr_t)c->data & 15)) return fail(SQ_EINVAL, "kv cache: null or misaligned pages");
+  if (c->dim != 64 && c->dim != 128 && c->dim != 256) return fail(SQ_ESHAPE, "kv cache: dim must be 64, 128 or 256");
+  if (c->heads <= 0 || c->heads > 4096) return fail(SQ_ESHAPE, "kv cache: heads must be in [1, 4096]");
+  if (c->page_tokens <= 0 || c->page_tokens % kTile || c->page_tokens * (int64_t)c->dim > 32768)
+    return fail(SQ_ESHAPE, "kv cache: page_tokens must be a multiple of 64 with page_tokens * dim <= 32768");
+  if (c->storage != SQ_KV_INT8 && c->storage != SQ_KV_FP8) return fail(SQ_ESTORAGE, "kv cache: unknown storage");
+  if (c->num_pages <= 0 || c->num_pages > 0x7fffffff || c->page_bytes % 16 ||
+      c->page_bytes < (int64_t)c->heads * (2 * (int64_t)c->page_tokens * c->dim + 8))
+    return fail(SQ_EINVAL, "kv cache: page count or page bytes");
+  return 0;
+}
+
+int check_tables(const sq_kv_tables *t) {
+  if (!t || !t->table || !t->lens || !t->free_pages || !t->counters) return fail(SQ_EINVAL, "kv tables: null pointer");
+  if (t->requests <= 0 || t->requests > 0x7fffffff || t->width <= 0 || t->capacity <= 0 || t->capacity > 0x7fffffff)
+    return fail(SQ_EINVAL, "kv tables: sizes must be positive 32-bit numbers");
+  if (t->page_tokens <= 0) return fail(SQ_ESHAPE, "kv tables: page_tokens must be positive");
+  return 0;
+}
+
+int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
+  if (!s->units || s->max_units <= 0 || (s->max_merges > 0 && !s->merges) || s->max_merges < 0)
+    return fail(SQ_EINVAL, "kv schedule: null pointer or negative size");
+  if (s->kv_heads <= 0 || s->q_heads <= 0 || s->q_heads % s->kv_heads)
+    return fail(SQ_ESHAPE, "kv schedule: q_heads must be a positive multiple of kv_heads");
+  if (s->rows != 16 && s->rows != 32 && s->rows != 64 && s->rows != 128) return fail(SQ_ESHAPE, "kv schedule: rows");
+  if (s->window < 0 || (s->window > 0 && !s->causal))
+    return fail(SQ_EINVAL, "kv schedule: a window is non-negative and needs causal attention");
+  if (s->slots <= 0 || s->slots > 1 << 16) return fail(SQ_EINVAL, "kv schedule: slots must be in [1, 65536]");
+  if (s->min_tiles <= 0 || s->merge_rows <= 0 || s->merge_rows > s->rows) return fail(SQ_EINVAL, "kv schedule: min_tiles or merge_rows");
+  const int64_t G = s->q_heads / s->kv_heads;
+  if (tokens * G > 0x3fffffff) return fail(SQ_EINVAL, "kv schedule: tokens * heads of a group too large");
+  const int64_t sets = (tokens * G + s->rows - 1) / s->rows + batch + 1;
+  if (sets + s->slots / s->kv_heads > s->max_units || s->slots / s->kv_heads > s->max_merges ||
+      2 * s->slots / s->kv_heads > s->max_partials || s->max_units >= 1 << 24)
+    return fail(SQ_EINVAL, "kv schedule: room for units, merges or partials");
+  if ((int64_t)s->max_units * s->kv_heads > 0x7fffffff) return fail(SQ_EINVAL, "kv schedule: units * heads too large");
+  return 0;
+}
+
+int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
+  const int rc = check_tables(t);
+  if (rc) return rc;
+  if (!p || !p->rows || !p->counts || !p->cu || !p->slots || !p->positions || !p->lens || !p->granted || !p->pages ||
+      !p->filled || !p->tiles || !p->counters)
+    return fail(SQ_EINVAL, "kv plan: null pointer");
+  if (!index_type(p->rows_dtype) || !index_type(p->counts_dtype)) return fail(SQ_EINVAL, "kv plan: rows and counts are int32 or int64");
+  if (p->batch <= 0 || p->batch > SQ_KV_MAX_REQUESTS) return fail(SQ_EINVAL, "kv plan: batch must be in [1, 4096]");
+  if (p->max_count < 0) return fail(SQ_EINVAL, "kv plan: negative max_count");
+  if (p->tokens < 0 || p->tokens > 0x3fffffff) return fail(SQ_EINVAL, "kv plan: tokens must be in [0, 2^30)");
+  int64_t tiles = p->tokens / t->page_tokens + 2 * (int64_t)p->batch;
+  if (tiles > p->tokens) tiles = p->tokens;
+  if (p->max_tiles < tiles) return fail(SQ_EINVAL, "kv plan: room for page entries");
+  if (p->n_schedules < 0 || p->n_schedules > SQ_KV_MAX_SCHEDULES) return fail(SQ_EINVAL, "kv plan: number of schedules");
+  for (int i = 0; i < p->n_schedules; i++) {
+    const sq_kv_schedule &s = p->schedules[i];
+    const int e = check_schedule(&s, p->tokens, p->batch);
+    if (e) return e;
+    const int64_t most = (int64_t)p->max_count * (s.q_heads / s.kv_heads);
+    if (s.merge_rows < (most < s.rows ? most : s.rows)) return fail(SQ_EINVAL, "kv plan: merge_rows below max_count's");
+  }
+  return 0;
+}
+
+template <typename F>
+int dynamic_lds(F kernel, size_t bytes, const char *what) {
+  if (bytes <= 65536) return 0;
+  const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? 0 : fail((int)e, what);
+}
+
+int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
+
+template <int D, bool FP8>
+int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
+  const dim3 grid((unsigned)(s.max_units * s.kv_heads));
+  const size_t lds = (4 * 16 * (D + 4) + 128) * sizeof(float);
+  auto go = [&](auto kernel) {
+    const int rc = dynamic_lds(kernel, lds, "kv attend: LDS attribute");
+    if (rc) return rc;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, d);
+    return sq_internal_launched("kv_attend_kernel");
+  };
+  int rc;
+  if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>);
+  else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>);
+  else if constexpr (D <= 128) rc = s.rows == 64 ? go(kv_attend_kernel<D, 4, FP8>) : fail(SQ_ESHAPE, "kv attend: rows");
+  else rc = fail(SQ_ESHAPE, "kv attend: rows");
+  if (rc || !s.max_merges) return rc;
+  hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), (unsigned)s.merge_rows), dim3(256), 0, st,
+                     d, s.rows);
+  return sq_internal_launched("kv_merge_kernel");
+}
+
+}  // namespace
+
+extern "C" {
+
+int sq_kv_plan(const sq_kv_tables *t, const sq_kv_plan_args *p, void *stream) {
+  const int rc = check_plan(t, p);
+  if (rc) return rc;
+  PlanDev d = {*t, *p, 0};
+  const int64_t share = p->tokens > p->max_tiles ? p->tokens : p->max_tiles;
+  d.share_blocks = (int)((share + kPlanShare - 1) / kPlanShare);
+  if (d.share_blocks < 1) d.share_blocks = 1;
+  const size_t lds = 5 * sizeof(int32_t) * (size_t)(p->batch + 1);
+  const int e = dynamic_lds(kv_plan_kernel, lds, "kv plan: LDS attribute");
+  if (e) return e;
+  hipLaunchKernelGGL(kv_plan_kernel, dim3((unsigned)(d.share_blocks + p->n_schedules)), dim3(kPlanThreads), lds,
+                     (hipStream_t)stream, d);
+  return sq_internal_launched("kv_plan_kernel");
+}
+
+int sq_kv_commit(const sq_kv_tables *t, const sq_kv_plan_args *p, void *stream) {
+  const int rc = check_plan(t, p);
+  if (rc) return rc;
+  PlanDev d = {*t, *p, 0};
+  hipLaunchKernelGGL(kv_commit_kernel, dim3((unsigned)((p->batch + 255) / 256)), dim3(256), 0, (hipStream_t)stream, d);
+  return sq_internal_launched("kv_commit_kernel");
+}
+
+int sq_kv_release(const sq_kv_tables *t, const void *rows, int32_t rows_dtype, int64_t n, void *stream) {
+  const int rc = check_tables(t);
+  if (rc) return rc;
+  if (n == 0) return 0;
+  if (!rows || !index_type(rows_dtype) || n < 0 || n > SQ_KV_MAX_REQUESTS)
+    return fail(SQ_EINVAL, "kv release: rows must be int32 or int64, at most 4096 of them");
+  hipLaunchKernelGGL(kv_release_kernel, dim3(1), dim3(kPlanThreads), 2 * sizeof(int32_t) * (size_t)n, (hipStream_t)stream, *t,
+                     rows, rows_dtype, (int)n);
+  return sq_internal_launched("kv_release_kernel");
+}
+
+int sq_kv_append(const sq_kv_cache *c, const sq_kv_append_args *a, void *stream) {
+  const int rc = check_cache(c);
+  if (rc) return rc;
+  if (!a) return fail(SQ_EINVAL, "kv append: null arguments");
+  if (a->max_tiles == 0) return 0;
+  if (!a->k || !a->v || !a->pages || !a->filled || !a->tiles || a->max_tiles < 0) return fail(SQ_EINVAL, "kv append: null pointer");
+  if (a->dtype != SQ_BF16 && a->dtype != SQ_F16) return fail(SQ_EINVAL, "kv append: keys and values are bf16 or fp16");
+  if ((a->k_stride | a->k_head_stride | a->v_stride | a->v_head_stride) & 7 || (((uintptr_t)a->k | (uintptr_t)a->v) & 15))
+    return fail(SQ_EINVAL, "kv append: strides must be multiples of 8 and starts 16-byte aligned");
+  if (a->k_stride < 0 || a->k_head_stride < 0 || a->v_stride < 0 || a->v_head_stride < 0)
+    return fail(SQ_EINVAL, "kv append: negative stride");
+  const int n = c->page_tokens * c->dim / 2048;
+  const dim3 grid((unsigned)a->max_tiles, (unsigned)c->heads, 2);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, *a, log2_of(c->dim));
+    return sq_internal_launched("kv_append_kernel");
+  };
+  if (c->storage == SQ_KV_FP8)
+    return n <= 2 ? go(kv_append_kernel<true, 2>) : n <= 4 ? go(kv_append_kernel<true, 4>)
+           : n <= 8 ? go(kv_append_kernel<true, 8>) : go(kv_append_kernel<true, 16>);
+  return n <= 2 ? go(kv_append_kernel<false, 2>) : n <= 4 ? go(kv_append_kernel<false, 4>)
+         : n <= 8 ? go(kv_append_kernel<false, 8>) : go(kv_append_kernel<false, 16>);
+}
+
+int sq_kv_decode(const sq_kv_cache *c, const int32_t *pages, const int32_t *filled, int64_t n, void *k, void *v,
+                 int32_t out_dtype, void *stream) {
+  const int rc = check_cache(c);
+  if (rc) return rc;
+  if (n == 0) return 0;
+  if (!pages || !k || !v || n < 0 || n > 0x7fffffff) return fail(SQ_EINVAL, "kv decode: null pointer or page count");
+  if (out_dtype != SQ_F32 && out_dtype != SQ_BF16 && out_dtype != SQ_F16) return fail(SQ_EINVAL, "kv decode: output dtype");
+  const dim3 grid((unsigned)n, (unsigned)c->heads, 2);
+  if (c->storage == SQ_KV_FP8)
+    hipLaunchKernelGGL(kv_decode_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, *c, pages, filled, k, v, out_dtype,
+                       log2_of(c->dim));
+  else
+    hipLaunchKernelGGL(kv_decode_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, *c, pages, filled, k, v, out_dtype,
+                       log2_of(c->dim));
+  return sq_internal_launched("kv_decode_kernel");
+}
+
+int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  if (!a) return fail(SQ_EINVAL, "kv attend: null arguments");
+  if (a->tokens == 0) return 0;
+  if (!a->q || !a->out || !a->table || a->tokens < 0 || a->requests <= 0 || a->width <= 0)
+    return fail(SQ_EINVAL, "kv attend: null pointer or size");
+  if (a->dtype != SQ_BF16 && a->dtype != SQ_F16) return fail(SQ_EINVAL, "kv attend: queries are bf16 or fp16");
+  if ((a->q_stride | a->q_head_stride) & 7 || ((uintptr_t)a->q & 15) || ((uintptr_t)a->out & 15))
+    return fail(SQ_EINVAL, "kv attend: strides must be multiples of 8 and starts 16-byte aligned");
+  if (a->q_stride < 0 || a->q_head_stride < 0) return fail(SQ_EINVAL, "kv attend: negative stride");
+  rc = check_schedule(&a->schedule, a->tokens, 1);
+  if (rc) return rc;
+  if (a->schedule.kv_heads != c->heads) return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads");
+  if (a->schedule.max_merges && !a->workspace) return fail(SQ_EINVAL, "kv attend: null workspace");
+  const sq_kv_schedule &s = a->schedule;
+  const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges,
+                       a->requests, a->tokens, a->q_stride, a->q_head_stride, a->width, a->dtype, s.q_heads, s.kv_heads,
+                       s.causal, s.window, s.max_partials, a->scale};
+  const bool fp8 = c->storage == SQ_KV_FP8;
+  hipStream_t st = (hipStream_t)stream;
+  if (c->dim == 64) return fp8 ? launch_attend<64, true>(d, s, st) : launch_attend<64, false>(d, s, st);
+  if (c->dim == 128) return fp8 ? launch_attend<128, true>(d, s, st) : launch_attend<128, false>(d, s, st);
+  return fp8 ? launch_attend<256, true>(d, s, st) : launch_attend<256, false>(d, s, st);
+}
+
+}  // extern "C"

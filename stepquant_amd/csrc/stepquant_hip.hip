@@ -25,6 +25,7 @@
 
 #include <mutex>
 
+#include "internal.h"
 #include "stepquant_hip.h"
 
 namespace {
@@ -6700,6 +6701,9 @@ int launch_copy(const sq_pool *pool, const void *src, const void *dst, int32_t s
 }
 
 }  // namespace
+
+int sq_internal_fail(int code, const char *msg) { return fail(code, msg); }
+int sq_internal_launched(const char *what) { return check_launch(what); }
 
 extern "C" {
 

@@ -1,0 +1,343 @@
+"""Attention over keys and values held in 8 bits in pages, on one MI355X GPU.
+
+The softmax-attention layers between the recurrent layers that the state
+pools serve (no reference counterpart: the reference leaves them to its host
+engine).  Three pieces, used in turn by one model step:
+
+* ``BlockTables`` gives requests their pages.  ``plan`` turns the number of
+  new tokens of each request into block tables, slot maps and the attention
+  layers' split of work, on the GPU, without reading anything back;
+  ``commit`` takes the plan over; ``release`` returns requests' pages.
+* ``KVCache`` holds one layer's keys and values: ``append`` quantises the
+  plan's new tokens into their pages, ``decode`` gives pages back dense.
+* ``KVCache.attend`` is attention of the plan's new tokens over everything
+  that their requests hold.
+
+A block of ``page_tokens`` tokens shares one peak per KV head for its keys and
+one for its values.  ``int8`` codes stand for code * peak / 127, ``fp8`` codes
+(e4m3) for code * peak / 448; a token that raises the peak of a block that
+already holds tokens brings their codes to it (one more rounding).  A block
+that is given an infinity or a NaN reads as NaN.
+
+All calls are asynchronous on the current stream and can be captured in HIP
+graphs (``plan`` with device tensors, ``tokens`` and ``max_new``).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _native as N
+from .pool import PackedStatePool
+
+_STORAGE = {"int8": N.KV_INT8, "fp8": N.KV_FP8}
+_HALVES = {torch.bfloat16: N.BF16, torch.float16: N.F16}
+TILE = 64  # keys of one attention tile
+
+
+def _device(device):
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError("the KV cache requires a GPU (cuda) device")
+    return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+
+
+class KVPlan:
+    """New tokens of a batch of requests, as ``BlockTables.plan`` lays them out.
+
+    ``cu`` [B + 1] first packed row of each request; ``slots`` [tokens]
+    page * page_tokens + offset (-1: none); ``positions`` [tokens] position in
+    the request (-1: none); ``lens`` [B] tokens held afterwards; ``granted``
+    [B] whether the request's tokens found room; ``pages`` the pages that new
+    tokens fall into (0 past the last) and ``filled`` the tokens that each then
+    holds.  ``lens_before`` are not kept: a plan is committed once.
+    """
+
+    __slots__ = ("rows", "counts", "cu", "slots", "positions", "lens", "granted", "pages", "filled", "tiles",
+                 "counters", "tokens", "tables", "schedules", "_args", "_units")
+
+
+class BlockTables:
+    """Pages of up to ``requests`` requests of up to ``max_blocks`` blocks.
+
+    ``table`` [requests, max_blocks], ``lens`` [requests], ``free`` (a ring of
+    page numbers) and ``counters`` (pages taken from it and given to it so far)
+    live on the GPU.  Page 0 is the padding page and is never given out.
+    """
+
+    def __init__(self, requests, pages, max_blocks, *, page_tokens=64, device="cuda"):
+        if requests <= 0 or max_blocks <= 0 or pages < 2:
+            raise ValueError("block tables need requests, blocks and at least 2 pages")
+        if page_tokens <= 0 or page_tokens % TILE:
+            raise ValueError(f"page_tokens must be a positive multiple of {TILE}")
+        if max(requests, pages) > 0x7fffffff or max_blocks * page_tokens > 0x7fffffff:
+            raise ValueError("requests, pages and tokens of a request must be 32-bit numbers")
+        self.device = _device(device)
+        self.requests, self.pages, self.max_blocks, self.page_tokens = requests, pages, max_blocks, page_tokens
+        dev = self.device
+        self.table = torch.zeros((requests, max_blocks), dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.free = torch.arange(1, pages, dtype=torch.int32, device=dev)
+        self.counters = torch.tensor([0, pages - 1], dtype=torch.int64, device=dev)
+        self._desc = N.KVTables(table=self.table.data_ptr(), lens=self.lens.data_ptr(),
+                                free_pages=self.free.data_ptr(), counters=self.counters.data_ptr(),
+                                requests=requests, capacity=pages - 1, width=max_blocks, page_tokens=page_tokens)
+        self._cus = torch.cuda.get_device_properties(dev).multi_processor_count
+
+    def _index(self, x, what):
+        if not isinstance(x, torch.Tensor):
+            x = torch.as_tensor(x)
+        if x.dim() != 1 or x.dtype not in N.INTS:
+            raise ValueError(f"{what} must be one-dimensional int32 or int64")
+        return x.to(self.device).contiguous()
+
+    def plan(self, new, rows=None, *, tokens=None, max_new=None, heads=None, causal=True, window=0):
+        """Room for ``new[b]`` tokens of the request in row ``rows[b]`` (default: row b).
+
+        ``new`` and ``rows`` are lists or int32/int64 tensors, ``rows``
+        distinct.  ``tokens`` is the number of packed rows (at least
+        ``sum(new)``; rows past it are padding) and ``max_new`` the most new
+        tokens of a request; both default to those of ``new`` where that is on
+        the host and are required where it is on the GPU.  ``heads``
+        (query heads, KV heads) also lays out the work of ``attend``: with
+        ``causal`` each token sees its request's tokens up to itself, else all
+        of them; ``window`` > 0 leaves it the last ``window`` of those.  A
+        tuple of windows lays out several kinds of layers.
+
+        Requests that find no room (``granted`` 0) keep their length; their
+        tokens have no slot and their attention is zero.
+        """
+        if isinstance(new, torch.Tensor) and new.device.type == "cuda":
+            if tokens is None or max_new is None:
+                raise ValueError("counts on the GPU need tokens and max_new")
+        else:
+            host = [int(x) for x in new]
+            if any(x < 0 for x in host):
+                raise ValueError("new tokens cannot be negative")
+            tokens = sum(host) if tokens is None else tokens
+            max_new = max(host, default=0) if max_new is None else max_new
+            new = torch.tensor(host, dtype=torch.int64)
+        counts = self._index(new, "new")
+        batch = counts.numel()
+        if rows is None:
+            rows = torch.arange(batch, device=self.device)
+        rows = self._index(rows, "rows")
+        if rows.numel() != batch:
+            raise ValueError("new and rows must have the same length")
+        if not 0 < batch <= N.KV_MAX_REQUESTS:
+            raise ValueError(f"a plan takes 1 to {N.KV_MAX_REQUESTS} requests")
+        tokens, max_new = int(tokens), int(max_new)
+        if tokens < 0 or max_new < 0:
+            raise ValueError("tokens and max_new cannot be negative")
+        windows = tuple(window) if isinstance(window, (tuple, list)) else (window,)
+        if len(windows) > N.KV_MAX_SCHEDULES:
+            raise ValueError(f"a plan takes at most {N.KV_MAX_SCHEDULES} windows")
+        if any(windows) and not causal:
+            raise ValueError("a window needs causal attention")
+        dev = self.device
+        most = min(tokens, tokens // self.page_tokens + 2 * batch)
+        p = KVPlan()
+        p.tables, p.rows, p.counts, p.tokens = self, rows, counts, tokens
+        empty = torch.empty
+        p.cu = empty(batch + 1, dtype=torch.int32, device=dev)
+        p.slots = empty(tokens, dtype=torch.int64, device=dev)
+        p.positions = empty(tokens, dtype=torch.int32, device=dev)
+        p.lens = empty(batch, dtype=torch.int32, device=dev)
+        p.granted = empty(batch, dtype=torch.bool, device=dev)
+        p.pages = empty(most, dtype=torch.int32, device=dev)
+        p.filled = empty(most, dtype=torch.int32, device=dev)
+        p.tiles = empty((most, 2), dtype=torch.int32, device=dev)
+        p.counters = empty(2, dtype=torch.int64, device=dev)
+        # empty tensors have no address of their own
+        some = lambda t: t.data_ptr() or p.counters.data_ptr()
+        p._args = args = N.KVPlan(
+            rows=rows.data_ptr(), counts=counts.data_ptr(), cu=p.cu.data_ptr(), slots=some(p.slots),
+            positions=some(p.positions), lens=p.lens.data_ptr(), granted=p.granted.data_ptr(), pages=some(p.pages),
+            filled=some(p.filled), tiles=some(p.tiles), counters=p.counters.data_ptr(), tokens=tokens, batch=batch,
+            max_tiles=most, rows_dtype=N.INTS[rows.dtype], counts_dtype=N.INTS[counts.dtype],
+            max_count=min(max_new, 0x7fffffff))
+        p.schedules, p._units = {}, []
+        if heads is not None and tokens:
+            for i, w in enumerate(windows):
+                p.schedules[int(w)] = self._schedule(args.schedules[i], p, int(heads[0]), int(heads[1]), bool(causal),
+                                                     int(w), max_new, batch)
+            args.n_schedules = len(windows)
+        N.check(N.lib().sq_kv_plan(self._desc, args, N.stream_handle()), "kv plan")
+        return p
+
+    def _schedule(self, s, plan, q_heads, kv_heads, causal, window, max_new, batch):
+        if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
+            raise ValueError("query heads must be a positive multiple of KV heads")
+        if window < 0:
+            raise ValueError("a window cannot be negative")
+        group = q_heads // kv_heads
+        rows = 16 if max_new * group <= 16 else 32
+        slots = 2 * self._cus
+        s.q_heads, s.kv_heads, s.rows, s.causal, s.window = q_heads, kv_heads, rows, causal, window
+        s.slots, s.min_tiles = slots, 8
+        s.merge_rows = max(1, min(rows, max_new * group))
+        s.max_merges = slots // kv_heads
+        s.max_partials = 2 * slots // kv_heads
+        s.max_units = -(-plan.tokens * group // rows) + batch + 1 + slots // kv_heads
+        work = torch.empty((s.max_units + s.max_merges, 8), dtype=torch.int32, device=self.device)
+        plan._units.append(work)
+        s.units = work.data_ptr()
+        s.merges = s.units + 32 * s.max_units
+        return s
+
+    def commit(self, plan):
+        """Takes a plan's lengths and pages over; plans made before it are void."""
+        if plan.tables is not self:
+            raise ValueError("the plan is of other block tables")
+        N.check(N.lib().sq_kv_commit(self._desc, plan._args, N.stream_handle()), "kv commit")
+
+    def release(self, rows):
+        """Gives the pages of the requests in ``rows`` back; their rows are empty afterwards."""
+        rows = self._index(rows, "rows")
+        if rows.numel() > N.KV_MAX_REQUESTS:
+            raise ValueError(f"at most {N.KV_MAX_REQUESTS} rows at once")
+        if rows.numel():
+            N.check(N.lib().sq_kv_release(self._desc, N.ptr(rows), N.dtype_code(rows), rows.numel(),
+                                          N.stream_handle()), "kv release")
+
+
+class KVCache:
+    """One attention layer's keys and values in ``pages`` pages of ``page_tokens`` tokens.
+
+    ``data`` [pages, page_bytes] uint8: per head the keys' and the values'
+    codes [page_tokens, head_dim], then per head their two fp32 peaks.
+    ``head_dim`` is 64, 128 or 256 and ``page_tokens`` a multiple of 64, with
+    at most 32,768 values of a head in a page.
+    """
+
+    def __init__(self, pages, kv_heads, head_dim, *, page_tokens=64, storage="int8", device="cuda"):
+        if storage not in _STORAGE:
+            raise ValueError("KV storage must be int8 or fp8")
+        if head_dim not in (64, 128, 256):
+            raise ValueError("head_dim must be 64, 128 or 256")
+        if page_tokens <= 0 or page_tokens % TILE or page_tokens * head_dim > 32768:
+            raise ValueError(f"page_tokens must be a positive multiple of {TILE} with page_tokens * head_dim <= 32768")
+        if not 0 < kv_heads <= 4096 or not 0 < pages <= 0x7fffffff:
+            raise ValueError("pages and kv_heads must be positive, kv_heads at most 4096")
+        self.device = _device(device)
+        self.pages, self.heads, self.dim, self.page_tokens, self.storage = pages, kv_heads, head_dim, page_tokens, storage
+        codes = 2 * kv_heads * page_tokens * head_dim
+        # whole 128-byte lines, so that every token's row starts on one
+        self.page_bytes = -(-(codes + 8 * kv_heads) // 128) * 128
+        self.data = torch.zeros((pages, self.page_bytes), dtype=torch.uint8, device=self.device)
+        self._kv = N.KVCache(data=self.data.data_ptr(), page_bytes=self.page_bytes, num_pages=pages, heads=kv_heads,
+                             dim=head_dim, page_tokens=page_tokens, storage=_STORAGE[storage])
+        # page copies read only these
+        self._desc = N.Pool(data=self.data.data_ptr(), page_bytes=self.page_bytes, num_slots=pages)
+
+    @property
+    def nbytes(self):
+        return self.data.numel()
+
+    def wait(self):
+        """Writes are made on the caller's stream: nothing to wait for."""
+
+    def copy(self, source, destination):
+        """Copies whole pages (a shared prefix's part-filled page before it is written)."""
+        PackedStatePool.copy(self, source, destination)
+
+    def _rows(self, x, heads, tokens, what):
+        """[tokens, heads, dim] with rows that the kernels take: bf16 or fp16,
+        heads contiguous inside, strides of whole 16 bytes."""
+        if x.dtype not in _HALVES:
+            raise ValueError(f"{what} must be bf16 or fp16")
+        if x.device != self.device:
+            raise ValueError(f"{what} must be on the cache's device")
+        if x.dim() == 2 and x.shape[1] == heads * self.dim:
+            x = x.unflatten(1, (heads, self.dim))
+        if x.shape != (tokens, heads, self.dim):
+            raise ValueError(f"{what} must be [{tokens}, {heads}, {self.dim}], the plan's tokens")
+        s0, s1, s2 = x.stride()
+        if s2 != 1 or s0 % 8 or s1 % 8 or s0 < 0 or s1 < 0 or x.data_ptr() % 16:
+            x = x.contiguous()
+        return x
+
+    def _check_plan(self, plan):
+        tables = plan.tables
+        if tables.page_tokens != self.page_tokens or tables.device != self.device:
+            raise ValueError("the plan's block tables have other pages than the cache")
+
+    def append(self, k, v, plan):
+        """Quantises the plan's new keys and values [tokens, kv_heads, head_dim]
+        (or [tokens, kv_heads * head_dim]; bf16 or fp16) into their pages.
+
+        Pages shared by several requests are only ever whole: a part-filled
+        page belongs to one request (``copy`` it first).
+        """
+        self._check_plan(plan)
+        k = self._rows(k, self.heads, plan.tokens, "keys")
+        v = self._rows(v, self.heads, plan.tokens, "values")
+        if k.dtype != v.dtype:
+            raise ValueError("keys and values must have one dtype")
+        if not plan.tokens:
+            return
+        a = N.KVAppend(k=k.data_ptr(), v=v.data_ptr(), pages=plan.pages.data_ptr(), filled=plan.filled.data_ptr(),
+                       tiles=plan.tiles.data_ptr(), tokens=plan.tokens, k_stride=k.stride(0), k_head_stride=k.stride(1),
+                       v_stride=v.stride(0), v_head_stride=v.stride(1), max_tiles=plan.pages.numel(),
+                       dtype=_HALVES[k.dtype])
+        N.check(N.lib().sq_kv_append(self._kv, a, N.stream_handle()), "kv append")
+
+    def decode(self, pages, filled=None, *, dtype=torch.float32):
+        """Keys and values [n, page_tokens, kv_heads, head_dim] of ``pages``,
+        zero past the first ``filled`` tokens of each (default: all are taken)
+        and for pages that the cache does not have (page 0 among them)."""
+        if dtype not in N.FLOATS:
+            raise ValueError("dense keys and values are fp32, bf16 or fp16")
+        index = lambda x: torch.as_tensor(x).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
+        pages = index(pages)
+        n = pages.numel()
+        if filled is not None:
+            filled = index(filled)
+            if filled.numel() != n:
+                raise ValueError("pages and filled must have the same length")
+        shape = (n, self.page_tokens, self.heads, self.dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty(shape, dtype=dtype, device=self.device)
+        if n:
+            N.check(N.lib().sq_kv_decode(self._kv, N.ptr(pages), N.ptr(filled), n, N.ptr(k), N.ptr(v), N.FLOATS[dtype],
+                                         N.stream_handle()), "kv decode")
+        return k, v
+
+    def attend(self, q, plan, *, scale=None, window=None, out=None):
+        """Attention of the plan's new tokens over all that their requests hold.
+
+        ``q`` is [tokens, q_heads, head_dim] (or [tokens, q_heads * head_dim]),
+        bf16 or fp16, after ``append`` of the same plan; the result has its
+        shape (three-dimensional) and dtype.  ``scale`` defaults to
+        ``head_dim ** -0.5``; ``window`` picks one of the plan's windows
+        (default: the first).  Tokens that see no key get zero.
+        """
+        self._check_plan(plan)
+        if not plan.schedules:
+            if plan.tokens:
+                raise ValueError("the plan was made without heads")
+            return q.new_empty(q.shape if out is None else out.shape) if out is None else out
+        if window is None:
+            s = next(iter(plan.schedules.values()))
+        elif window in plan.schedules:
+            s = plan.schedules[window]
+        else:
+            raise ValueError(f"the plan was made without the window {window}")
+        if s.kv_heads != self.heads:
+            raise ValueError(f"the plan was made for {s.kv_heads} KV heads")
+        q = self._rows(q, s.q_heads, plan.tokens, "queries")
+        shape = (plan.tokens, s.q_heads, self.dim)
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise ValueError("out must be contiguous and like the queries")
+        ws = torch.empty(s.max_partials * s.kv_heads * s.rows * (self.dim + 2), dtype=torch.float32, device=self.device)
+        t = plan.tables
+        a = N.KVAttend(q=q.data_ptr(), out=out.data_ptr(), workspace=ws.data_ptr() or out.data_ptr(),
+                       table=t.table.data_ptr(), requests=t.requests, tokens=plan.tokens, q_stride=q.stride(0),
+                       q_head_stride=q.stride(1), width=t.max_blocks, dtype=_HALVES[q.dtype],
+                       scale=self.dim ** -.5 if scale is None else float(scale), schedule=s)
+        N.check(N.lib().sq_kv_attend(self._kv, a, N.stream_handle()), "kv attend")
+        return out
