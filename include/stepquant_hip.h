@@ -439,7 +439,7 @@ typedef struct sq_kv_schedule {
     int32_t max_partials;
     int32_t q_heads;
     int32_t kv_heads;
-    int32_t rows;         /* 16, 32, 64 or 128 */
+    int32_t rows;         /* 16, 32, 128 or 256 */
     int32_t causal;
     int32_t window;       /* 0: none; else the last `window` keys (causal only) */
     int32_t slots;        /* workgroups that the device holds at once */

@@ -540,20 +540,28 @@ struct AttendDev {
   const int32_t *units;
   const int32_t *merges;
   int64_t requests, tokens, q_stride, q_head_stride;
-  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials;
+  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials, unit_rows;
   float scale;
 };
 
-__device__ __forceinline__ float reduce_max4(float x) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float reduce_max2(float x) {  // over the lanes l and l ^ 32
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+__device__ __forceinline__ float reduce_sum2(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+__device__ __forceinline__ float reduce_max4(float x) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+  x = reduce_max2(x);
   auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 __device__ __forceinline__ float reduce_sum4(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  x = reduce_sum2(x);
   auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
@@ -569,27 +577,41 @@ __device__ __forceinline__ uint32_t key2(uint32_t w) {
   return half2_bits(__builtin_bit_cast(half2_v, m) - (half2_v){(_Float16)1152.f, (_Float16)1152.f});
 }
 
-// One dim of eight tokens (byte E of each w) as halves; int8 codes come out
+// One dim (byte E) of two tokens, or of eight, as halves; int8 codes come out
 // 2^-10 of their size: a byte is the half u 2^-24, and one fused product
 // makes it (u - 128) 2^-10.
 template <bool FP8, int E>
-__device__ __forceinline__ half8_v value8(const uint32_t w[8]) {
-  uint32_t o[4];
+__device__ __forceinline__ uint32_t value2(uint32_t w0, uint32_t w1) {
   if (FP8) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t m = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x0c0c0000 | (4 + E) << 8 | E);
-      o[i] = half2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)m, 1.f, false));
-    }
-  } else {
-    const half2_v mul = {(_Float16)16384.f, (_Float16)16384.f}, add = {(_Float16)-.125f, (_Float16)-.125f};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t m = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x0c000c00 | (4 + E) << 16 | E);
-      o[i] = half2_bits(__builtin_elementwise_fma(__builtin_bit_cast(half2_v, m), mul, add));
-    }
+    const uint32_t m = __builtin_amdgcn_perm(w1, w0, 0x0c0c0000 | (4 + E) << 8 | E);
+    return half2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)m, 1.f, false));
   }
-  return __builtin_bit_cast(half8_v, *(u32x4_v *)o);
+  const half2_v mul = {(_Float16)16384.f, (_Float16)16384.f}, add = {(_Float16)-.125f, (_Float16)-.125f};
+  const uint32_t m = __builtin_amdgcn_perm(w1, w0, 0x0c000c00 | (4 + E) << 16 | E);
+  return half2_bits(__builtin_elementwise_fma(__builtin_bit_cast(half2_v, m), mul, add));
+}
+
+template <bool FP8, int E>
+__device__ __forceinline__ half8_v value8(const uint32_t w[8]) {
+  u32x4_v o;
+#pragma unroll
+  for (int i = 0; i < 4; i++) o[i] = value2<FP8, E>(w[2 * i], w[2 * i + 1]);
+  return __builtin_bit_cast(half8_v, o);
+}
+
+// a code's share of the value that it stands for, beside its block's peak
+template <bool FP8>
+constexpr float kKeyUnit = FP8 ? 1.f / 448.f : 1.f / 127.f;
+template <bool FP8>
+constexpr float kValueUnit = FP8 ? 1.f / 448.f : 1024.f / 127.f;
+
+// The power of two that brings a bfloat16 row with this largest magnitude, in
+// [2^e, 2^(e+1)), below 2^15, and its inverse.
+__device__ __forceinline__ void row_shift(float most, float *shift, float *unit) {
+  const int e = (int)(__float_as_uint(most) >> 23) - 127;
+  const bool usual = e > -100 && e < 100;
+  *shift = usual ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 1.f;
+  *unit = usual ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 1.f;
 }
 
 template <typename F, int... E>
@@ -597,10 +619,29 @@ __device__ __forceinline__ void each(F f, std::integer_sequence<int, E...>) {
   (f(std::integral_constant<int, E>{}), ...);
 }
 
-template <int D>
-struct alignas(D / 16) Bytes {  // a lane's bytes of one token's values
-  uint32_t w[D / 64];
+template <int N>
+struct alignas(N) Bytes {  // a lane's N bytes of one token's values
+  uint32_t w[N / 4];
+  __device__ __forceinline__ uint32_t word(int i) const { return w[i]; }
 };
+template <>
+struct Bytes<2> {
+  uint16_t w;
+  __device__ __forceinline__ uint32_t word(int) const { return w; }
+};
+
+// N values of one row's output as halves of its type
+template <int N>
+__device__ __forceinline__ void store_row(uint16_t *dst, int dtype, const float *x) {
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; i++)
+    w[i] = dtype == SQ_BF16 ? bf16_bits(x[2 * i]) | bf16_bits(x[2 * i + 1]) << 16
+                            : f16_bits(x[2 * i]) | f16_bits(x[2 * i + 1]) << 16;
+  if constexpr (N == 2) *(uint32_t *)dst = w[0];
+  else if constexpr (N == 4) *(uint2 *)dst = make_uint2(w[0], w[1]);
+  else *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // Units of up to 16 RT rows: the four waves take a unit's tiles in turn and
 // are joined at its end; keys and values go from memory to registers.
@@ -643,11 +684,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
           for (int i = 0; i < 4; i++)
             most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][k][i])), fabsf(bf_hi(w[s][k][i]))));
       most = reduce_max4(most);
-      // 2^(14 - e) brings the row's largest, in [2^e, 2^(e+1)), below 2^15
-      const int e = (int)(__float_as_uint(most) >> 23) - 127;
-      const bool plain = e > -100 && e < 100;
-      const float shift = plain ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 1.f;
-      unit = plain ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 1.f;
+      float shift;
+      row_shift(most, &shift, &unit);
 #pragma unroll
       for (int s = 0; s < D / 64; s++)
 #pragma unroll
@@ -658,7 +696,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
     }
 #pragma unroll
     for (int s = 0; s < KS; s++) qf[r][s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
-    mult[r] = a.scale * 1.4426950408889634f * unit * (FP8 ? 1.f / 448.f : 1.f / 127.f);
+    mult[r] = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
     m[r] = -INFINITY;
     l[r] = 0.f;
     hi[r] = live ? (a.causal ? pos0 + t + 1 : kv1) : kv1;
@@ -677,7 +715,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   const int32_t *entries = a.table + (int64_t)row * a.width;
   auto entry_of = [&](int tile) { return pow2 ? tile >> log_per : tile / per; };
   int ids = 0;
-  Bytes<D> vf[2][8];
+  Bytes<D / 16> vf[2][8];
   u32x4_v kf[4][D / 64];
   int page = 0;
   const uint8_t *tile_at = nullptr;
@@ -715,7 +753,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
       for (int s = 0; s < 2; s++)
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          vf[s][j] = *(const Bytes<D> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
+          vf[s][j] = *(const Bytes<D / 16> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
     }
     f32x4_v s[RT][4];
 #pragma unroll
@@ -780,7 +818,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
       pf[r][1] = __builtin_bit_cast(half8_v, *(u32x4_v *)w[1]);
       // a row that sees none of the tile takes nothing from it, whatever its peak
       const bool some = whole || (known && first < min(hi[r], kv1) && first + kTile > lo[r]);
-      sv[r] = some ? peak.y * (FP8 ? 1.f / 448.f : 1024.f / 127.f) : 0.f;
+      sv[r] = some ? peak.y * kValueUnit<FP8> : 0.f;
     }
     const bool keep = __all(same);
     auto value = [&](auto E) {
@@ -844,15 +882,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
         x *= inv;
         const int t = f / G, head = h * G + f - t * G;
         uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + d;
-        uint2 w;
-        if (a.dtype == SQ_BF16) {
-          w.x = bf16_bits(x[0]) | bf16_bits(x[1]) << 16;
-          w.y = bf16_bits(x[2]) | bf16_bits(x[3]) << 16;
-        } else {
-          w.x = f16_bits(x[0]) | f16_bits(x[1]) << 16;
-          w.y = f16_bits(x[2]) | f16_bits(x[3]) << 16;
-        }
-        *(uint2 *)dst = w;
+        store_row<4>(dst, a.dtype, (const float *)&x);
       } else {
         const int64_t slot = ((int64_t)part * a.kv_heads + h) * (16 * RT) + 16 * r + j;
         *(f32x4_v *)(a.ws + slot * D + d) = x;
@@ -866,54 +896,344 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   }
 }
 
-// Joins the parts of one query row: one workgroup per (merge, head, row).
+typedef float f32x16_v __attribute__((ext_vector_type(16)));
+
+// A thread's share of a tile, as it is in the page.
+template <int D, int NW>
+struct TileCodes {
+  static constexpr int KN = D / 16 > NW ? D / 16 / NW : 1, VN = 8 / NW;
+  u32x4_v k[KN];
+  Bytes<D / 32> v[VN][4];
+};
+
+// Units of up to 32 NW rows, 32 a wave.  A tile is converted to halves once
+// for the workgroup, into LDS, in the order in which the 32x32x16 products
+// take it.  With AHEAD the products with the next tile's keys are issued
+// before this tile's softmax, which they do not depend on.
+//
+// O is kept in units of a row's largest value peak so far, so that a
+// probability times its block's peak in that unit (at most 2^8) is the half
+// that enters the product; the maximum that scores are taken from is raised
+// only when it is passed by more than 2^8.
+template <int D, int NW, bool FP8, bool AHEAD>
+__global__ __launch_bounds__(64 * NW, NW == 4 && D == 256 ? 1 : 2) void kv_attend_rows_kernel(AttendDev a) {
+  extern __shared__ uint4 tiles[];
+  constexpr int KS = D / 16, DT = D / 32, KB = 64 * D / 8;  // k steps, dim tiles, uint4 of a tile
+  typedef TileCodes<D, NW> Codes;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hl = lane >> 5;
+  const int h = blockIdx.x % a.kv_heads;
+  const int32_t *u = a.units + 8 * (int64_t)(blockIdx.x / a.kv_heads);
+  const int row = u[0], q0 = u[1], at_row = 32 * NW * blockIdx.y, f0 = u[2] + at_row, rows = min(u[3] - at_row, 32 * NW);
+  const int pos0 = u[4], kv0 = u[5], part = u[7];
+  const int G = a.q_heads / a.kv_heads;
+  int kv1 = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
+  if (a.causal) kv1 = min(kv1, pos0 + (f0 + rows - 1) / G + 1);  // (the unit's last rows may be another workgroup's)
+  if (rows <= 0 || u[3] > a.unit_rows || q0 < 0 || f0 < 0 || q0 + (int64_t)(f0 + rows - 1) / G >= a.tokens) return;
+  const int P = a.c.page_tokens, per = P / kTile, tile0 = kv0 / kTile, n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
+  const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
+  const int32_t *entries = a.table + (int64_t)row * a.width;
+
+  const int mine = 32 * wave + c;
+  const bool live = mine < rows;
+  const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
+  half8_v qf[KS];
+  float mult;
+  {
+    const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 8 * hl;
+    u32x4_v w[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) w[s] = live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0};
+    float unit = 1.f;
+    if (a.dtype == SQ_BF16) {
+      float most = 0, shift;
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][i])), fabsf(bf_hi(w[s][i]))));
+      row_shift(reduce_max2(most), &shift, &unit);
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[s][i] = f16_bits(bf_lo(w[s][i]) * shift) | f16_bits(bf_hi(w[s][i]) * shift) << 16;
+    }
+    // scores keep their order when they are scaled: the sign goes to the query
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s] ^ flip);
+    mult = fabsf(a.scale) * 1.4426950408889634f * unit * kKeyUnit<FP8>;
+  }
+  // what the row sees, and what every row of the wave sees whole
+  const int hi = live && a.causal ? min(kv1, pos0 + t + 1) : kv1;
+  const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
+  const int all_hi = min(kv1, a.causal ? pos0 + (f0 + 32 * wave) / G + 1 : kv1);
+  const int all_lo = a.window > 0 ? pos0 + (f0 + min(rows, 32 * wave + 32) - 1) / G - a.window + 1 : 0;
+  f32x16_v o[DT];
+#pragma unroll
+  for (int e = 0; e < DT; e++)
+#pragma unroll
+    for (int k = 0; k < 16; k++) o[e][k] = 0.f;
+  float m = -INFINITY, l = 0.f, ref = 0.f;
+
+  int ids = 0;  // the lanes hold the pages of 64 tiles
+  struct Place {
+    int page;
+    const uint8_t *at;
+    float2 peak;
+  };
+  auto locate = [&](int i) {
+    if ((i & 63) == 0) ids = i + lane < n ? entries[(tile0 + i + lane) / per] : 0;
+    const int p = __builtin_amdgcn_readlane(ids, i & 63);
+    Place x;
+    x.page = p > 0 && p < a.c.num_pages ? p : 0;
+    const uint8_t *base = a.c.data + x.page * a.c.page_bytes;
+    x.at = base + ((int64_t)(2 * h) * P + (tile0 + i) % per * kTile) * D;
+    x.peak = *(const float2 *)(base + peaks_at);
+    return x;
+  };
+  auto load_keys = [&](Codes &x, const uint8_t *at) {
+    if (KS >= NW || wave < KS)
+#pragma unroll
+      for (int k = 0; k < Codes::KN; k++) x.k[k] = *(const u32x4_v *)(at + 16 * (tid + 64 * NW * k));
+  };
+  auto load_values = [&](Codes &x, const uint8_t *at) {
+#pragma unroll
+    for (int r = 0; r < Codes::VN; r++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int w = wave + NW * r, token = 16 * (w >> 1) + 8 * hl + 4 * (w & 1) + k;
+        x.v[r][k] = *(const Bytes<D / 32> *)(at + (int64_t)P * D + token * D + c * DT);
+      }
+  };
+  // keys: [32 tokens][16 dims][half of them][token, permuted by the step] of
+  // eight dims; the permutation spreads a wave's writes over the banks
+  auto put_keys = [&](const Codes &x, uint4 *dst) {
+    if (KS >= NW || wave < KS)
+#pragma unroll
+      for (int k = 0; k < Codes::KN; k++) {
+        const int i = tid + 64 * NW * k, token = i / KS, s = i % KS;
+        uint4 *at = dst + ((token >> 5) * KS + s) * 64 + ((token & 31) ^ (s & 7));
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const uint32_t w0 = x.k[k][2 * b], w1 = x.k[k][2 * b + 1];
+          at[32 * b] = make_uint4(key2<FP8, 0>(w0), key2<FP8, 1>(w0), key2<FP8, 0>(w1), key2<FP8, 1>(w1));
+        }
+      }
+  };
+  // values: [dim tile e][16 tokens][half][r] of the eight tokens of a product's
+  // lane, for dim r D / 32 + e
+  auto put_values = [&](const Codes &x, uint4 *dst) {
+#pragma unroll
+    for (int r = 0; r < Codes::VN; r++) {
+      const int w = wave + NW * r;
+      uint2 *at = (uint2 *)(dst + ((w >> 1) * 64 + 32 * (w & 1) + c)) + hl;
+      auto one = [&](auto E) {
+        constexpr int e = decltype(E)::value;
+        uint32_t b[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) b[k] = x.v[r][k].word(e / 4);
+        at[512 * e] = make_uint2(value2<FP8, e & 3>(b[0], b[1]), value2<FP8, e & 3>(b[2], b[3]));
+      };
+      each(one, std::make_integer_sequence<int, DT>{});
+    }
+  };
+  uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
+  auto scores = [&](const uint4 *src, f32x16_v s[2]) {
+#pragma unroll
+    for (int tt = 0; tt < 2; tt++) {
+#pragma unroll
+      for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const uint4 w = src[(tt * KS + k) * 64 + 32 * hl + (c ^ (k & 7))];
+        s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), qf[k], s[tt], 0, 0, 0);
+      }
+    }
+  };
+
+  f32x16_v s[2], next[2];
+  Codes codes;
+  Place here = {}, there = {}, beyond = {};
+  if (n > 0) {
+    here = locate(0);
+    load_keys(codes, here.at);
+    load_values(codes, here.at);
+    put_keys(codes, kb);
+    put_values(codes, vb);
+    if (n > 1) {
+      there = locate(1);
+      if (AHEAD) {
+        load_keys(codes, there.at);
+        put_keys(codes, kb + KB);
+      }
+    }
+    __syncthreads();
+    if (AHEAD) scores(kb, s);
+  }
+  for (int i = 0; i < n; i++) {
+    const int first = kv0 + i * kTile;
+    if (i + 1 < n) {
+      load_values(codes, there.at);
+      if (!AHEAD) load_keys(codes, there.at);
+    }
+    if (i + 2 < n) {
+      beyond = locate(i + 2);
+      if (AHEAD) load_keys(codes, beyond.at);
+    }
+    if (AHEAD) {
+      if (i + 1 < n) scores(kb + ((i + 1) & 1) * KB, next);
+    } else {
+      scores(kb + (i & 1) * KB, s);
+    }
+    const bool known = here.page != 0, whole = known && first + kTile <= all_hi && first >= all_lo;
+    uint32_t seen = ~0u;
+    if (!whole) {
+      seen = 0;
+#pragma unroll
+      for (int k = 0; k < 32; k++) {
+        const int j = first + 32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hl + (k & 3);
+        const bool yes = known && j < hi && j >= lo;
+        seen |= (uint32_t)yes << k;
+        s[k >> 4][k & 15] = yes ? s[k >> 4][k & 15] : -INFINITY;
+      }
+    }
+    float best = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int k = 1; k < 16; k++) best = fmaxf(best, fmaxf(s[0][k], s[1][k]));
+    best = reduce_max2(best);
+    // a tile that the row does not see takes no part in it, whatever its peaks
+    const bool some = whole || (known && first < hi && first + kTile > lo);
+    const float f = some ? mult * here.peak.x : 1.f;
+    best = some ? best * f : -INFINITY;
+    const float high = some ? fmaxf(ref, here.peak.y) : ref;
+    if (__any(best > m + 8.f || high > ref)) {
+      const float raised = fmaxf(m, best);
+      const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
+      const float shrink = high > ref ? ref / high * was : was;
+      m = raised;
+      ref = high;
+      l *= was;
+#pragma unroll
+      for (int e = 0; e < DT; e++)
+#pragma unroll
+        for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    const float size = some ? here.peak.y / ref : 1.f;
+    const float off = __builtin_amdgcn_logf(size) - base;
+    float sum = 0;
+    half8_v pf[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      u32x4_v w;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float p[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const int at = 8 * j + 2 * k + b;
+          p[b] = __builtin_amdgcn_exp2f(fmaf(s[at >> 4][at & 15], f, off));
+          if (!whole) p[b] = seen >> at & 1 ? p[b] : 0.f;
+          sum += p[b];
+        }
+        w[k] = f16_bits(p[0]) | f16_bits(p[1]) << 16;
+      }
+      pf[j] = __builtin_bit_cast(half8_v, w);
+    }
+    l += sum / size;
+    const uint4 *src = vb + (i & 1) * KB;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int e = 0; e < DT; e++) {
+        const uint4 w = src[(4 * e + j) * 64 + lane];
+        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), pf[j], o[e], 0, 0, 0);
+      }
+    if (i + 1 < n) {
+      put_values(codes, vb + ((i + 1) & 1) * KB);
+      if (!AHEAD) put_keys(codes, kb + ((i + 1) & 1) * KB);
+      if (AHEAD && i + 2 < n) put_keys(codes, kb + (i & 1) * KB);
+      __syncthreads();
+    }
+    here = there;
+    there = beyond;
+    if (AHEAD) s[0] = next[0], s[1] = next[1];
+  }
+  l = reduce_sum2(l);
+  if (!live) return;
+  const float unit = ref * kValueUnit<FP8>;
+  if (part < 0) {
+    const float f = l == 0.f ? 0.f : unit / l;
+    uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      float x[DT];
+#pragma unroll
+      for (int e = 0; e < DT; e++) x[e] = o[e][k] * f;
+      store_row<DT>(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT, a.dtype, x);
+    }
+  } else {
+    const int64_t slot = ((int64_t)part * a.kv_heads + h) * a.unit_rows + at_row + mine;
+    float *dst = a.ws + slot * D;
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+#pragma unroll
+      for (int e = 0; e < DT; e += 2)
+        *(float2 *)(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT + e) = make_float2(o[e][k] * unit, o[e + 1][k] * unit);
+    if (hl == 0) {
+      float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
+      ml[0] = m;
+      ml[1] = l;
+    }
+  }
+}
+
+// Joins the parts of query rows: one workgroup per (merge, head) and row, or
+// per 16th row.
 template <int D>
-__global__ __launch_bounds__(256) void kv_merge_kernel(AttendDev a, int R) {
+__global__ __launch_bounds__(256) void kv_merge_kernel(AttendDev a) {
   constexpr int LANES = D / 4, GROUPS = 256 / LANES;
   __shared__ f32x4_v part_o[GROUPS][LANES];
-  __shared__ float part_l[GROUPS];
-  const int tid = threadIdx.x, j = blockIdx.y, h = blockIdx.x % a.kv_heads;
+  __shared__ float part_l[GROUPS], part_m[GROUPS];
+  const int tid = threadIdx.x, h = blockIdx.x % a.kv_heads;
   const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.kv_heads);
-  const int rows = u[2];
-  if (j >= rows) return;
-  const int q0 = u[0], f = u[1] + j, p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
-  const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * R + j, step = (int64_t)a.kv_heads * R;
-  const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * R * D;
-  float mm = -INFINITY;
-  for (int i = 0; i < n; i++) mm = fmaxf(mm, ml[2 * (slot0 + i * step)]);
-  const float base = mm == -INFINITY ? 0.f : mm;
+  const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
   const int lane = tid % LANES, grp = tid / LANES;
-  f32x4_v x = {0, 0, 0, 0};
-  float sum = 0;
-  for (int i = grp; i < n; i += GROUPS) {
-    const int64_t s = slot0 + i * step;
-    const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base);
-    sum += ml[2 * s + 1] * w;
-    x += *(const f32x4_v *)(a.ws + s * D + 4 * lane) * w;
-  }
-  part_o[grp][lane] = x;
-  if (lane == 0) part_l[grp] = sum;
-  __syncthreads();
-  if (grp) return;
-  sum = 0;
-  x = (f32x4_v){0, 0, 0, 0};
+  const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D;
+  for (int j = blockIdx.y; j < rows; j += gridDim.y) {
+    const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * a.unit_rows + j, step = (int64_t)a.kv_heads * a.unit_rows;
+    // every group of lanes joins its parts as they come, then the groups
+    f32x4_v x = {0, 0, 0, 0};
+    float sum = 0, mm = -INFINITY;
+    for (int i = grp; i < n; i += GROUPS) {
+      const int64_t s = slot0 + i * step;
+      const float2 part = *(const float2 *)(ml + 2 * s);
+      const float high = fmaxf(mm, part.x), base = high == -INFINITY ? 0.f : high;
+      const float was = __builtin_amdgcn_exp2f(mm - base), w = __builtin_amdgcn_exp2f(part.x - base);
+      mm = high;
+      sum = fmaf(sum, was, part.y * w);
+      x = x * was + *(const f32x4_v *)(a.ws + s * D + 4 * lane) * w;
+    }
+    part_o[grp][lane] = x;
+    if (lane == 0) part_l[grp] = sum, part_m[grp] = mm;
+    __syncthreads();
+    if (grp == 0) {
 #pragma unroll
-  for (int i = 0; i < GROUPS; i++) {
-    x += part_o[i][lane];
-    sum += part_l[i];
+      for (int i = 0; i < GROUPS; i++) mm = fmaxf(mm, part_m[i]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      sum = 0;
+      x = (f32x4_v){0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < GROUPS; i++) {
+        const float w = __builtin_amdgcn_exp2f(part_m[i] - base);
+        x += part_o[i][lane] * w;
+        sum = fmaf(part_l[i], w, sum);
+      }
+      x *= sum == 0.f ? 0.f : 1.f / sum;
+      const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
+      store_row<4>(a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane, a.dtype, (const float *)&x);
+    }
+    __syncthreads();
   }
-  x *= sum == 0.f ? 0.f : 1.f / sum;
-  const int t = f / G, head = h * G + f - t * G;
-  uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane;
-  uint2 w;
-  if (a.dtype == SQ_BF16) {
-    w.x = bf16_bits(x[0]) | bf16_bits(x[1]) << 16;
-    w.y = bf16_bits(x[2]) | bf16_bits(x[3]) << 16;
-  } else {
-    w.x = f16_bits(x[0]) | f16_bits(x[1]) << 16;
-    w.y = f16_bits(x[2]) | f16_bits(x[3]) << 16;
-  }
-  *(uint2 *)dst = w;
 }
 
 // ------------------------------------------------------------ host side
@@ -948,7 +1268,7 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
     return fail(SQ_EINVAL, "kv schedule: null pointer or negative size");
   if (s->kv_heads <= 0 || s->q_heads <= 0 || s->q_heads % s->kv_heads)
     return fail(SQ_ESHAPE, "kv schedule: q_heads must be a positive multiple of kv_heads");
-  if (s->rows != 16 && s->rows != 32 && s->rows != 64 && s->rows != 128) return fail(SQ_ESHAPE, "kv schedule: rows");
+  if (s->rows != 16 && s->rows != 32 && s->rows != 128 && s->rows != 256) return fail(SQ_ESHAPE, "kv schedule: rows");
   if (s->window < 0 || (s->window > 0 && !s->causal))
     return fail(SQ_EINVAL, "kv schedule: a window is non-negative and needs causal attention");
   if (s->slots <= 0 || s->slots > 1 << 16) return fail(SQ_EINVAL, "kv schedule: slots must be in [1, 65536]");
@@ -998,22 +1318,21 @@ int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 template <int D, bool FP8>
 int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
-  const dim3 grid((unsigned)(s.max_units * s.kv_heads));
-  const size_t lds = (4 * 16 * (D + 4) + 128) * sizeof(float);
-  auto go = [&](auto kernel) {
+  auto go = [&](auto kernel, int threads, size_t lds, int blocks = 1) {
     const int rc = dynamic_lds(kernel, lds, "kv attend: LDS attribute");
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, d);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_units * s.kv_heads), (unsigned)blocks), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
+  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 4 * 64 * D * sizeof(uint16_t);
   int rc;
-  if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>);
-  else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>);
-  else if constexpr (D <= 128) rc = s.rows == 64 ? go(kv_attend_kernel<D, 4, FP8>) : fail(SQ_ESHAPE, "kv attend: rows");
-  else rc = fail(SQ_ESHAPE, "kv attend: rows");
+  if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 256, joined);
+  else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 256, joined);
+  else if (s.rows == 128 || D == 256) rc = go(kv_attend_rows_kernel<D, 4, FP8, true>, 256, staged, s.rows / 128);
+  else if constexpr (D != 256) rc = go(kv_attend_rows_kernel<D, 8, FP8, true>, 512, staged);
   if (rc || !s.max_merges) return rc;
-  hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), (unsigned)s.merge_rows), dim3(256), 0, st,
-                     d, s.rows);
+  const unsigned rows = s.merge_rows < 16 ? s.merge_rows : 16;
+  hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), rows), dim3(256), 0, st, d);
   return sq_internal_launched("kv_merge_kernel");
 }
 
@@ -1107,6 +1426,7 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   if ((a->q_stride | a->q_head_stride) & 7 || ((uintptr_t)a->q & 15) || ((uintptr_t)a->out & 15))
     return fail(SQ_EINVAL, "kv attend: strides must be multiples of 8 and starts 16-byte aligned");
   if (a->q_stride < 0 || a->q_head_stride < 0) return fail(SQ_EINVAL, "kv attend: negative stride");
+  if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(SQ_EINVAL, "kv attend: scale must be finite");
   rc = check_schedule(&a->schedule, a->tokens, 1);
   if (rc) return rc;
   if (a->schedule.kv_heads != c->heads) return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads");
@@ -1114,7 +1434,7 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   const sq_kv_schedule &s = a->schedule;
   const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges,
                        a->requests, a->tokens, a->q_stride, a->q_head_stride, a->width, a->dtype, s.q_heads, s.kv_heads,
-                       s.causal, s.window, s.max_partials, a->scale};
+                       s.causal, s.window, s.max_partials, s.rows, a->scale};
   const bool fp8 = c->storage == SQ_KV_FP8;
   hipStream_t st = (hipStream_t)stream;
   if (c->dim == 64) return fp8 ? launch_attend<64, true>(d, s, st) : launch_attend<64, false>(d, s, st);

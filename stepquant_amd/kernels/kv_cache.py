@@ -172,8 +172,9 @@ class BlockTables:
         if window < 0:
             raise ValueError("a window cannot be negative")
         group = q_heads // kv_heads
-        rows = 16 if max_new * group <= 16 else 32
-        slots = 2 * self._cus
+        most = max_new * group
+        rows = 16 if most <= 16 else 32 if most <= 32 else 128 if most <= 128 else 256
+        slots = self._cus if rows == 256 else 2 * self._cus
         s.q_heads, s.kv_heads, s.rows, s.causal, s.window = q_heads, kv_heads, rows, causal, window
         s.slots, s.min_tiles = slots, 8
         s.merge_rows = max(1, min(rows, max_new * group))
