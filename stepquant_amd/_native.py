@@ -234,6 +234,29 @@ def step_entry(name: str):
     return fn
 
 
+# the KV cache's argument blocks in the order of their structures' fields, as above
+KV_SCHEDULE = struct.Struct("=2Q12i")
+KV_PLAN = struct.Struct(f"=11Qq6i{KV_MAX_SCHEDULES * KV_SCHEDULE.size}s")
+KV_APPEND = struct.Struct("=5Q5q2i")
+KV_ATTEND = struct.Struct(f"=4Q4q2ifi{KV_SCHEDULE.size}s")
+_I32, _I64 = ctypes.c_int32, ctypes.c_int64
+_KV_ENTRIES = {"sq_kv_plan": [_P, ctypes.c_char_p, _P], "sq_kv_commit": [_P, ctypes.c_char_p, _P],
+               "sq_kv_append": [_P, ctypes.c_char_p, _P], "sq_kv_attend": [_P, ctypes.c_char_p, _P],
+               "sq_kv_decode": [_P, _P, _P, _I64, _P, _P, _I32, _P]}
+
+
+def kv_entry(name: str):
+    """A KV entry point taking the address of its tables or cache and a packed
+    argument block (``sq_kv_decode``: plain arguments)."""
+    fn = _step_entries.get(name)
+    if fn is None:
+        fn = lib()[name]
+        fn.restype = ctypes.c_int
+        fn.argtypes = _KV_ENTRIES[name]
+        _step_entries[name] = fn  # with its prototype, as in step_entry
+    return fn
+
+
 def raw_stream() -> int:
     """The current stream of the current device as a number."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())

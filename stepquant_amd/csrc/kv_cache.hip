@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "internal.h"
@@ -1307,29 +1308,40 @@ int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
   return 0;
 }
 
-template <typename F>
-int dynamic_lds(F kernel, size_t bytes, const char *what) {
+// Raises a kernel's limit of dynamic LDS, once per kernel (each with an id of
+// its own) and device, to 128 KiB, the most that one takes.
+std::atomic<uint64_t> g_raised[16];
+
+int dynamic_lds(const void *kernel, int id, size_t bytes, const char *what) {
   if (bytes <= 65536) return 0;
-  const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? 0 : fail((int)e, what);
+  int dev = -1;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail((int)e, what);
+  const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
+  if (g_raised[id].load(std::memory_order_relaxed) & bit) return 0;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+  if (e != hipSuccess) return fail((int)e, what);
+  g_raised[id].fetch_or(bit, std::memory_order_relaxed);
+  return 0;
 }
 
 int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 template <int D, bool FP8>
 int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
-  auto go = [&](auto kernel, int threads, size_t lds, int blocks = 1) {
-    const int rc = dynamic_lds(kernel, lds, "kv attend: LDS attribute");
+  auto go = [&](auto kernel, int id, int threads, size_t lds, int blocks = 1) {
+    const int rc = dynamic_lds((const void *)kernel, 2 * id + FP8, lds, "kv attend: LDS attribute");
     if (rc) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_units * s.kv_heads), (unsigned)blocks), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
+  static_assert(D <= 256, "ids of kernels with more than 64 KiB: one dim has them");
   constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 4 * 64 * D * sizeof(uint16_t);
   int rc;
-  if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 256, joined);
-  else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 256, joined);
-  else if (s.rows == 128 || D == 256) rc = go(kv_attend_rows_kernel<D, 4, FP8, true>, 256, staged, s.rows / 128);
-  else if constexpr (D != 256) rc = go(kv_attend_rows_kernel<D, 8, FP8, true>, 512, staged);
+  if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
+  else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
+  else if (s.rows == 128 || D == 256) rc = go(kv_attend_rows_kernel<D, 4, FP8, true>, 3, 256, staged, s.rows / 128);
+  else if constexpr (D != 256) rc = go(kv_attend_rows_kernel<D, 8, FP8, true>, 4, 512, staged);
   if (rc || !s.max_merges) return rc;
   const unsigned rows = s.merge_rows < 16 ? s.merge_rows : 16;
   hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), rows), dim3(256), 0, st, d);
@@ -1348,7 +1360,7 @@ int sq_kv_plan(const sq_kv_tables *t, const sq_kv_plan_args *p, void *stream) {
   d.share_blocks = (int)((share + kPlanShare - 1) / kPlanShare);
   if (d.share_blocks < 1) d.share_blocks = 1;
   const size_t lds = 5 * sizeof(int32_t) * (size_t)(p->batch + 1);
-  const int e = dynamic_lds(kv_plan_kernel, lds, "kv plan: LDS attribute");
+  const int e = dynamic_lds((const void *)kv_plan_kernel, 0, lds, "kv plan: LDS attribute");
   if (e) return e;
   hipLaunchKernelGGL(kv_plan_kernel, dim3((unsigned)(d.share_blocks + p->n_schedules)), dim3(kPlanThreads), lds,
                      (hipStream_t)stream, d);

@@ -51,11 +51,36 @@ class KVPlan:
     the request (-1: none); ``lens`` [B] tokens held afterwards; ``granted``
     [B] whether the request's tokens found room; ``pages`` the pages that new
     tokens fall into (0 past the last) and ``filled`` the tokens that each then
-    holds.  ``lens_before`` are not kept: a plan is committed once.
+    holds; ``counters`` the tables' counters afterwards.
     """
 
-    __slots__ = ("rows", "counts", "cu", "slots", "positions", "lens", "granted", "pages", "filled", "tiles",
-                 "counters", "tokens", "tables", "schedules", "_args", "_units")
+    __slots__ = ("tables", "rows", "counts", "tokens", "batch", "max_tiles", "schedules", "_args", "_ints", "_longs",
+                 "_sizes", "_append", "_views")
+
+    def _view(self, i):
+        # views are made when they are asked for: a step's kernels need none
+        views = self._views
+        if views is None:
+            counters, slots = self._longs.split((2, self.tokens))
+            views = self._ints.split_with_sizes(self._sizes)
+            self._views = views = (views[0], slots, *views[1:3], views[3].view(torch.bool)[:self.batch], *views[4:6],
+                                   counters)
+        return views[i]
+
+    cu = property(lambda self: self._view(0))
+    slots = property(lambda self: self._view(1))
+    positions = property(lambda self: self._view(2))
+    lens = property(lambda self: self._view(3))
+    granted = property(lambda self: self._view(4))
+    pages = property(lambda self: self._view(5))
+    filled = property(lambda self: self._view(6))
+    counters = property(lambda self: self._view(7))
+
+
+class _Schedule:
+    """One kind of attention layer's split of a plan (``sq_kv_schedule``)."""
+
+    __slots__ = ("packed", "q_heads", "kv_heads", "floats")
 
 
 class BlockTables:
@@ -83,6 +108,7 @@ class BlockTables:
         self._desc = N.KVTables(table=self.table.data_ptr(), lens=self.lens.data_ptr(),
                                 free_pages=self.free.data_ptr(), counters=self.counters.data_ptr(),
                                 requests=requests, capacity=pages - 1, width=max_blocks, page_tokens=page_tokens)
+        self._at = ctypes.addressof(self._desc)
         self._cus = torch.cuda.get_device_properties(dev).multi_processor_count
 
     def _index(self, x, what):
@@ -90,7 +116,7 @@ class BlockTables:
             x = torch.as_tensor(x)
         if x.dim() != 1 or x.dtype not in N.INTS:
             raise ValueError(f"{what} must be one-dimensional int32 or int64")
-        return x.to(self.device).contiguous()
+        return x if x.device == self.device and x.is_contiguous() else x.to(self.device).contiguous()
 
     def plan(self, new, rows=None, *, tokens=None, max_new=None, heads=None, causal=True, window=0):
         """Room for ``new[b]`` tokens of the request in row ``rows[b]`` (default: row b).
@@ -108,7 +134,7 @@ class BlockTables:
         Requests that find no room (``granted`` 0) keep their length; their
         tokens have no slot and their attention is zero.
         """
-        if isinstance(new, torch.Tensor) and new.device.type == "cuda":
+        if isinstance(new, torch.Tensor) and new.is_cuda:
             if tokens is None or max_new is None:
                 raise ValueError("counts on the GPU need tokens and max_new")
         else:
@@ -127,71 +153,75 @@ class BlockTables:
             raise ValueError("new and rows must have the same length")
         if not 0 < batch <= N.KV_MAX_REQUESTS:
             raise ValueError(f"a plan takes 1 to {N.KV_MAX_REQUESTS} requests")
-        tokens, max_new = int(tokens), int(max_new)
+        tokens, max_new = int(tokens), min(int(max_new), 0x7fffffff)
         if tokens < 0 or max_new < 0:
             raise ValueError("tokens and max_new cannot be negative")
         windows = tuple(window) if isinstance(window, (tuple, list)) else (window,)
-        if len(windows) > N.KV_MAX_SCHEDULES:
-            raise ValueError(f"a plan takes at most {N.KV_MAX_SCHEDULES} windows")
+        if len(windows) > N.KV_MAX_SCHEDULES or len(set(windows)) < len(windows):
+            raise ValueError(f"a plan takes at most {N.KV_MAX_SCHEDULES} windows, each once")
         if any(windows) and not causal:
             raise ValueError("a window needs causal attention")
-        dev = self.device
+        if heads is None:
+            windows = ()
+        else:
+            shape = self._shape(int(heads[0]), int(heads[1]), tokens, batch, max_new)
+            if not tokens:
+                windows = ()
         most = min(tokens, tokens // self.page_tokens + 2 * batch)
         p = KVPlan()
-        p.tables, p.rows, p.counts, p.tokens = self, rows, counts, tokens
-        empty = torch.empty
-        p.cu = empty(batch + 1, dtype=torch.int32, device=dev)
-        p.slots = empty(tokens, dtype=torch.int64, device=dev)
-        p.positions = empty(tokens, dtype=torch.int32, device=dev)
-        p.lens = empty(batch, dtype=torch.int32, device=dev)
-        p.granted = empty(batch, dtype=torch.bool, device=dev)
-        p.pages = empty(most, dtype=torch.int32, device=dev)
-        p.filled = empty(most, dtype=torch.int32, device=dev)
-        p.tiles = empty((most, 2), dtype=torch.int32, device=dev)
-        p.counters = empty(2, dtype=torch.int64, device=dev)
-        # empty tensors have no address of their own
-        some = lambda t: t.data_ptr() or p.counters.data_ptr()
-        p._args = args = N.KVPlan(
-            rows=rows.data_ptr(), counts=counts.data_ptr(), cu=p.cu.data_ptr(), slots=some(p.slots),
-            positions=some(p.positions), lens=p.lens.data_ptr(), granted=p.granted.data_ptr(), pages=some(p.pages),
-            filled=some(p.filled), tiles=some(p.tiles), counters=p.counters.data_ptr(), tokens=tokens, batch=batch,
-            max_tiles=most, rows_dtype=N.INTS[rows.dtype], counts_dtype=N.INTS[counts.dtype],
-            max_count=min(max_new, 0x7fffffff))
-        p.schedules, p._units = {}, []
-        if heads is not None and tokens:
-            for i, w in enumerate(windows):
-                p.schedules[int(w)] = self._schedule(args.schedules[i], p, int(heads[0]), int(heads[1]), bool(causal),
-                                                     int(w), max_new, batch)
-            args.n_schedules = len(windows)
-        N.check(N.lib().sq_kv_plan(self._desc, args, N.stream_handle()), "kv plan")
+        p.tables, p.rows, p.counts, p.tokens, p.batch, p.max_tiles, p._views = self, rows, counts, tokens, batch, most, None
+        flags = -(-batch // 4)
+        sizes = [batch + 1, tokens, batch, flags, most, most, 2 * most]
+        if windows:
+            max_units, max_merges, max_partials, q_heads, kv_heads, unit_rows, slots, merge_rows = shape
+            sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
+            sizes += [8 * (max_units + max_merges)] * len(windows)
+        p._sizes = sizes
+        p._ints = ints = torch.empty(sum(sizes), dtype=torch.int32, device=self.device)
+        p._longs = longs = torch.empty(2 + tokens, dtype=torch.int64, device=self.device)
+        at, base = [], ints.data_ptr()
+        for n in sizes:
+            at.append(base)
+            base += 4 * n
+        counters = longs.data_ptr()
+        p.schedules, packed = {}, b""
+        for w, units in zip(windows, at[7:]):
+            s = _Schedule()
+            s.packed = N.KV_SCHEDULE.pack(units, units + 32 * max_units, max_units, max_merges, max_partials, q_heads,
+                                          kv_heads, unit_rows, bool(causal), int(w), slots, self.min_tiles, merge_rows, 0)
+            s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, max_partials * kv_heads * unit_rows
+            p.schedules[int(w)] = s
+            packed += s.packed
+        p._append = (at[4], at[5], at[6])
+        p._args = args = N.KV_PLAN.pack(
+            rows.data_ptr(), counts.data_ptr(), at[0], counters + 16, at[1], at[2], at[3], at[4], at[5], at[6], counters,
+            tokens, batch, most, N.INTS[rows.dtype], N.INTS[counts.dtype], len(windows), max_new,
+            packed.ljust(N.KV_MAX_SCHEDULES * N.KV_SCHEDULE.size, b"\0"))
+        rc = N.kv_entry("sq_kv_plan")(self._at, args, N.raw_stream())
+        if rc:
+            N.check(rc, "kv plan")
         return p
 
-    def _schedule(self, s, plan, q_heads, kv_heads, causal, window, max_new, batch):
+    min_tiles = 8  # least 64-key tiles of a part
+
+    def _shape(self, q_heads, kv_heads, tokens, batch, max_new):
         if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
             raise ValueError("query heads must be a positive multiple of KV heads")
-        if window < 0:
-            raise ValueError("a window cannot be negative")
         group = q_heads // kv_heads
         most = max_new * group
         rows = 16 if most <= 16 else 32 if most <= 32 else 128 if most <= 128 else 256
         slots = self._cus if rows == 256 else 2 * self._cus
-        s.q_heads, s.kv_heads, s.rows, s.causal, s.window = q_heads, kv_heads, rows, causal, window
-        s.slots, s.min_tiles = slots, 8
-        s.merge_rows = max(1, min(rows, max_new * group))
-        s.max_merges = slots // kv_heads
-        s.max_partials = 2 * slots // kv_heads
-        s.max_units = -(-plan.tokens * group // rows) + batch + 1 + slots // kv_heads
-        work = torch.empty((s.max_units + s.max_merges, 8), dtype=torch.int32, device=self.device)
-        plan._units.append(work)
-        s.units = work.data_ptr()
-        s.merges = s.units + 32 * s.max_units
-        return s
+        merges = slots // kv_heads
+        return (-(-tokens * group // rows) + batch + 1 + merges, merges, 2 * slots // kv_heads, q_heads, kv_heads, rows,
+                slots, max(1, min(rows, most)))
 
     def commit(self, plan):
         """Takes a plan's lengths and pages over; plans made before it are void."""
         if plan.tables is not self:
             raise ValueError("the plan is of other block tables")
-        N.check(N.lib().sq_kv_commit(self._desc, plan._args, N.stream_handle()), "kv commit")
+        rc = N.kv_entry("sq_kv_commit")(self._at, plan._args, N.raw_stream())
+        if rc:
+            N.check(rc, "kv commit")
 
     def release(self, rows):
         """Gives the pages of the requests in ``rows`` back; their rows are empty afterwards."""
@@ -229,6 +259,7 @@ class KVCache:
         self.data = torch.zeros((pages, self.page_bytes), dtype=torch.uint8, device=self.device)
         self._kv = N.KVCache(data=self.data.data_ptr(), page_bytes=self.page_bytes, num_pages=pages, heads=kv_heads,
                              dim=head_dim, page_tokens=page_tokens, storage=_STORAGE[storage])
+        self._at = ctypes.addressof(self._kv)
         # page copies read only these
         self._desc = N.Pool(data=self.data.data_ptr(), page_bytes=self.page_bytes, num_slots=pages)
 
@@ -255,7 +286,7 @@ class KVCache:
         if x.shape != (tokens, heads, self.dim):
             raise ValueError(f"{what} must be [{tokens}, {heads}, {self.dim}], the plan's tokens")
         s0, s1, s2 = x.stride()
-        if s2 != 1 or s0 % 8 or s1 % 8 or s0 < 0 or s1 < 0 or x.data_ptr() % 16:
+        if s2 != 1 or (s0 | s1) % 8 or s0 < 0 or s1 < 0 or x.data_ptr() % 16:
             x = x.contiguous()
         return x
 
@@ -278,11 +309,12 @@ class KVCache:
             raise ValueError("keys and values must have one dtype")
         if not plan.tokens:
             return
-        a = N.KVAppend(k=k.data_ptr(), v=v.data_ptr(), pages=plan.pages.data_ptr(), filled=plan.filled.data_ptr(),
-                       tiles=plan.tiles.data_ptr(), tokens=plan.tokens, k_stride=k.stride(0), k_head_stride=k.stride(1),
-                       v_stride=v.stride(0), v_head_stride=v.stride(1), max_tiles=plan.pages.numel(),
-                       dtype=_HALVES[k.dtype])
-        N.check(N.lib().sq_kv_append(self._kv, a, N.stream_handle()), "kv append")
+        (ks, kh, _), (vs, vh, _) = k.stride(), v.stride()
+        args = N.KV_APPEND.pack(k.data_ptr(), v.data_ptr(), *plan._append, plan.tokens, ks, kh, vs, vh, plan.max_tiles,
+                                _HALVES[k.dtype])
+        rc = N.kv_entry("sq_kv_append")(self._at, args, N.raw_stream())
+        if rc:
+            N.check(rc, "kv append")
 
     def decode(self, pages, filled=None, *, dtype=torch.float32):
         """Keys and values [n, page_tokens, kv_heads, head_dim] of ``pages``,
@@ -290,20 +322,27 @@ class KVCache:
         and for pages that the cache does not have (page 0 among them)."""
         if dtype not in N.FLOATS:
             raise ValueError("dense keys and values are fp32, bf16 or fp16")
-        index = lambda x: torch.as_tensor(x).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
-        pages = index(pages)
+        pages = self._numbers(pages)
         n = pages.numel()
         if filled is not None:
-            filled = index(filled)
+            filled = self._numbers(filled)
             if filled.numel() != n:
                 raise ValueError("pages and filled must have the same length")
         shape = (n, self.page_tokens, self.heads, self.dim)
         k = torch.empty(shape, dtype=dtype, device=self.device)
         v = torch.empty(shape, dtype=dtype, device=self.device)
         if n:
-            N.check(N.lib().sq_kv_decode(self._kv, N.ptr(pages), N.ptr(filled), n, N.ptr(k), N.ptr(v), N.FLOATS[dtype],
-                                         N.stream_handle()), "kv decode")
+            rc = N.kv_entry("sq_kv_decode")(self._at, pages.data_ptr(), 0 if filled is None else filled.data_ptr(), n,
+                                            k.data_ptr(), v.data_ptr(), N.FLOATS[dtype], N.raw_stream())
+            if rc:
+                N.check(rc, "kv decode")
         return k, v
+
+    def _numbers(self, x):
+        if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.dim() == 1 and x.device == self.device \
+                and x.is_contiguous():
+            return x
+        return torch.as_tensor(x).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
 
     def attend(self, q, plan, *, scale=None, window=None, out=None):
         """Attention of the plan's new tokens over all that their requests hold.
@@ -315,30 +354,32 @@ class KVCache:
         (default: the first).  Tokens that see no key get zero.
         """
         self._check_plan(plan)
-        if not plan.schedules:
-            if plan.tokens:
-                raise ValueError("the plan was made without heads")
-            return q.new_empty(q.shape if out is None else out.shape) if out is None else out
+        schedules = plan.schedules
+        if not schedules and plan.tokens:
+            raise ValueError("the plan was made without heads")
+        if not plan.tokens:
+            return torch.empty_like(q) if out is None else out
         if window is None:
-            s = next(iter(plan.schedules.values()))
-        elif window in plan.schedules:
-            s = plan.schedules[window]
+            s = next(iter(schedules.values()))
+        elif window in schedules:
+            s = schedules[window]
         else:
             raise ValueError(f"the plan was made without the window {window}")
         if s.kv_heads != self.heads:
             raise ValueError(f"the plan was made for {s.kv_heads} KV heads")
         q = self._rows(q, s.q_heads, plan.tokens, "queries")
-        shape = (plan.tokens, s.q_heads, self.dim)
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
-        elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
+            out = torch.empty((plan.tokens, s.q_heads, self.dim), dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
                 or out.data_ptr() % 16:
             raise ValueError("out must be contiguous and like the queries")
-        ws = torch.empty(s.max_partials * s.kv_heads * s.rows * (self.dim + 2), dtype=torch.float32, device=self.device)
+        ws = torch.empty(s.floats * (self.dim + 2), dtype=torch.float32, device=self.device)
         t = plan.tables
-        a = N.KVAttend(q=q.data_ptr(), out=out.data_ptr(), workspace=ws.data_ptr() or out.data_ptr(),
-                       table=t.table.data_ptr(), requests=t.requests, tokens=plan.tokens, q_stride=q.stride(0),
-                       q_head_stride=q.stride(1), width=t.max_blocks, dtype=_HALVES[q.dtype],
-                       scale=self.dim ** -.5 if scale is None else float(scale), schedule=s)
-        N.check(N.lib().sq_kv_attend(self._kv, a, N.stream_handle()), "kv attend")
+        qs, qh, _ = q.stride()
+        args = N.KV_ATTEND.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr(), t.table.data_ptr(), t.requests, plan.tokens,
+                                qs, qh, t.max_blocks, _HALVES[q.dtype], self.dim ** -.5 if scale is None else scale, 0,
+                                s.packed)
+        rc = N.kv_entry("sq_kv_attend")(self._at, args, N.raw_stream())
+        if rc:
+            N.check(rc, "kv attend")
         return out
