@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 #include <utility>
 
 #include "internal.h"
@@ -15,8 +16,10 @@
 
 namespace {
 
+typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_v __attribute__((ext_vector_type(8)));
+typedef float f32x2_v __attribute__((ext_vector_type(2)));
 typedef float f32x4_v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
 
@@ -633,12 +636,16 @@ struct Bytes<2> {
 
 // N values of one row's output as halves of its type
 template <int N>
-__device__ __forceinline__ void store_row(uint16_t *dst, int dtype, const float *x) {
+__device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float *x) {
   uint32_t w[N / 2];
 #pragma unroll
-  for (int i = 0; i < N / 2; i++)
-    w[i] = dtype == SQ_BF16 ? bf16_bits(x[2 * i]) | bf16_bits(x[2 * i + 1]) << 16
-                            : f16_bits(x[2 * i]) | f16_bits(x[2 * i + 1]) << 16;
+  for (int i = 0; i < N / 2; i++) {
+    const f32x2_v y = {x[2 * i], x[2 * i + 1]};
+    // both are computed: a branch for every pair costs more
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, bf16x2_v));
+    const uint32_t h = half2_bits(__builtin_convertvector(y, half2_v));
+    w[i] = bf16 ? b : h;
+  }
   if constexpr (N == 2) *(uint32_t *)dst = w[0];
   else if constexpr (N == 4) *(uint2 *)dst = make_uint2(w[0], w[1]);
   else *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
@@ -883,7 +890,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
         x *= inv;
         const int t = f / G, head = h * G + f - t * G;
         uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + d;
-        store_row<4>(dst, a.dtype, (const float *)&x);
+        store_row<4>(dst, a.dtype == SQ_BF16, (const float *)&x);
       } else {
         const int64_t slot = ((int64_t)part * a.kv_heads + h) * (16 * RT) + 16 * r + j;
         *(f32x4_v *)(a.ws + slot * D + d) = x;
@@ -899,291 +906,313 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
 
 typedef float f32x16_v __attribute__((ext_vector_type(16)));
 
-// A thread's share of a tile, as it is in the page.
-template <int D, int NW>
-struct TileCodes {
-  static constexpr int KN = D / 16 > NW ? D / 16 / NW : 1, VN = 8 / NW;
-  u32x4_v k[KN];
-  Bytes<D / 32> v[VN][4];
-};
-
-// Units of up to 32 NW rows, 32 a wave.  A tile is converted to halves once
-// for the workgroup, into LDS, in the order in which the 32x32x16 products
-// take it.  With AHEAD the products with the next tile's keys are issued
-// before this tile's softmax, which they do not depend on.
+// Units of up to 256 rows: 8 waves of 32 rows (of 256 dims: 128 rows at a time,
+// each wave half of their outputs' dims).
+// A tile is converted to halves once for the workgroup, into LDS, in the order
+// in which the 32x32x16 products take it.
+//
+// Two waves share a SIMD, one of each half of the workgroup, and the halves
+// run half a tile apart: while one issues its products (this tile's values,
+// the next tile's keys: 32 of 32 cycles each at 128 dims), the other one's
+// vector instructions (softmax, conversion of a later tile) have the SIMD.  A
+// barrier ends each half.
 //
 // O is kept in units of a row's largest value peak so far, so that a
 // probability times its block's peak in that unit (at most 2^8) is the half
 // that enters the product; the maximum that scores are taken from is raised
 // only when it is passed by more than 2^8.
-template <int D, int NW, bool FP8, bool AHEAD>
-__global__ __launch_bounds__(64 * NW, NW == 4 && D == 256 ? 1 : 2) void kv_attend_rows_kernel(AttendDev a) {
+template <int D, bool FP8>
+__global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   extern __shared__ uint4 tiles[];
-  constexpr int KS = D / 16, DT = D / 32, KB = 64 * D / 8;  // k steps, dim tiles, uint4 of a tile
-  typedef TileCodes<D, NW> Codes;
+  constexpr int KS = D / 16, DT = D / 32;                   // k steps and dim tiles
+  constexpr int KF = 65, KB = 2 * KS * KF, VB = 4 * DT * 64;  // uint4 of a step's keys, of a tile's keys and values
+  constexpr int OT = D == 256 ? DT / 2 : DT;                // a wave's dim tiles
+  constexpr int WR = D == 256 ? 128 : 256;                  // rows of the workgroup at a time
+  constexpr int KN = KS > 8 ? KS / 8 : 1;                   // 16-byte groups of keys of a thread
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hl = lane >> 5;
+  const int late = wave >> 2, e0 = D == 256 ? late * OT : 0;
   const int h = blockIdx.x % a.kv_heads;
   const int32_t *u = a.units + 8 * (int64_t)(blockIdx.x / a.kv_heads);
-  const int row = u[0], q0 = u[1], at_row = 32 * NW * blockIdx.y, f0 = u[2] + at_row, rows = min(u[3] - at_row, 32 * NW);
-  const int pos0 = u[4], kv0 = u[5], part = u[7];
+  const int row = u[0], q0 = u[1], pos0 = u[4], kv0 = u[5], part = u[7];
   const int G = a.q_heads / a.kv_heads;
-  int kv1 = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
-  if (a.causal) kv1 = min(kv1, pos0 + (f0 + rows - 1) / G + 1);  // (the unit's last rows may be another workgroup's)
-  if (rows <= 0 || u[3] > a.unit_rows || q0 < 0 || f0 < 0 || q0 + (int64_t)(f0 + rows - 1) / G >= a.tokens) return;
-  const int P = a.c.page_tokens, per = P / kTile, tile0 = kv0 / kTile, n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
+  if (u[3] <= 0 || u[3] > a.unit_rows || q0 < 0 || u[2] < 0 || q0 + (int64_t)(u[2] + u[3] - 1) / G >= a.tokens) return;
+  const int end = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
+  const int P = a.c.page_tokens, per = P / kTile, tile0 = kv0 / kTile;
   const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
   const int32_t *entries = a.table + (int64_t)row * a.width;
+  uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
 
-  const int mine = 32 * wave + c;
-  const bool live = mine < rows;
-  const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
-  half8_v qf[KS];
-  float mult;
-  {
-    const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 8 * hl;
-    u32x4_v w[KS];
+  for (int turn = 0; turn < u[3]; turn += WR) {
+    const int f0 = u[2] + turn, rows = min(u[3] - turn, WR);
+    // (the unit's last rows may be of another turn)
+    const int kv1 = a.causal ? min(end, pos0 + (f0 + rows - 1) / G + 1) : end;
+    const int n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
+    const int first_row = 32 * (D == 256 ? wave & 3 : wave), mine = first_row + c;
+    const bool live = mine < rows;
+    const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
+    half8_v qf[KS];
+    float mult;
+    {
+      const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 8 * hl;
+      u32x4_v w[KS];
 #pragma unroll
-    for (int s = 0; s < KS; s++) w[s] = live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0};
-    float unit = 1.f;
-    if (a.dtype == SQ_BF16) {
-      float most = 0, shift;
+      for (int s = 0; s < KS; s++) w[s] = live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0};
+      float unit = 1.f;
+      if (a.dtype == SQ_BF16) {
+        float most = 0, shift;
 #pragma unroll
-      for (int s = 0; s < KS; s++)
+        for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][i])), fabsf(bf_hi(w[s][i]))));
-      row_shift(reduce_max2(most), &shift, &unit);
+          for (int i = 0; i < 4; i++) most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][i])), fabsf(bf_hi(w[s][i]))));
+        row_shift(reduce_max2(most), &shift, &unit);
 #pragma unroll
-      for (int s = 0; s < KS; s++)
+        for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[s][i] = f16_bits(bf_lo(w[s][i]) * shift) | f16_bits(bf_hi(w[s][i]) * shift) << 16;
+          for (int i = 0; i < 4; i++) w[s][i] = f16_bits(bf_lo(w[s][i]) * shift) | f16_bits(bf_hi(w[s][i]) * shift) << 16;
+      }
+      // scores keep their order when they are scaled: the sign goes to the query
+      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s] ^ flip);
+      mult = fabsf(a.scale) * 1.4426950408889634f * unit * kKeyUnit<FP8>;
     }
-    // scores keep their order when they are scaled: the sign goes to the query
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    // what the row sees, and what every row of the wave sees whole
+    const int hi = live && a.causal ? min(kv1, pos0 + t + 1) : kv1;
+    const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
+    const int all_hi = min(kv1, a.causal ? pos0 + (f0 + first_row) / G + 1 : kv1);
+    const int all_lo = a.window > 0 ? pos0 + (f0 + max(1, min(rows, first_row + 32)) - 1) / G - a.window + 1 : 0;
+    f32x16_v o[OT], s[2];
+    half8_v pf[4];
 #pragma unroll
-    for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s] ^ flip);
-    mult = fabsf(a.scale) * 1.4426950408889634f * unit * kKeyUnit<FP8>;
-  }
-  // what the row sees, and what every row of the wave sees whole
-  const int hi = live && a.causal ? min(kv1, pos0 + t + 1) : kv1;
-  const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
-  const int all_hi = min(kv1, a.causal ? pos0 + (f0 + 32 * wave) / G + 1 : kv1);
-  const int all_lo = a.window > 0 ? pos0 + (f0 + min(rows, 32 * wave + 32) - 1) / G - a.window + 1 : 0;
-  f32x16_v o[DT];
+    for (int e = 0; e < OT; e++)
 #pragma unroll
-  for (int e = 0; e < DT; e++)
-#pragma unroll
-    for (int k = 0; k < 16; k++) o[e][k] = 0.f;
-  float m = -INFINITY, l = 0.f, ref = 0.f;
+      for (int k = 0; k < 16; k++) o[e][k] = 0.f;
+    float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
 
-  int ids = 0;  // the lanes hold the pages of 64 tiles
-  struct Place {
-    int page;
-    const uint8_t *at;
-    float2 peak;
-  };
-  auto locate = [&](int i) {
-    if ((i & 63) == 0) ids = i + lane < n ? entries[(tile0 + i + lane) / per] : 0;
-    const int p = __builtin_amdgcn_readlane(ids, i & 63);
-    Place x;
-    x.page = p > 0 && p < a.c.num_pages ? p : 0;
-    const uint8_t *base = a.c.data + x.page * a.c.page_bytes;
-    x.at = base + ((int64_t)(2 * h) * P + (tile0 + i) % per * kTile) * D;
-    x.peak = *(const float2 *)(base + peaks_at);
-    return x;
-  };
-  auto load_keys = [&](Codes &x, const uint8_t *at) {
-    if (KS >= NW || wave < KS)
+    // The tiles in order; past the last one the last again, so that loads ahead
+    // need no branch.
+    struct Walk {
+      int block, sub, left, id;
+    };
+    auto begin = [&](Walk &w) {
+      w.block = tile0 / per, w.sub = tile0 - w.block * per, w.left = n;
+      w.id = entries[w.block];
+    };
+    auto page_at = [&](Walk &w, bool &known) {  // and a step on; the next page's number is loaded a step ahead
+      const int page = __builtin_amdgcn_readfirstlane(w.id);
+      known = page > 0 && page < a.c.num_pages;
+      const uint8_t *at = a.c.data + (known ? page : 0) * a.c.page_bytes;
+      w.left--;
+      const bool more = w.left > 0, next = w.sub + 1 == per;
+      w.sub = more ? next ? 0 : w.sub + 1 : w.sub;
+      w.block += more && next;
+      w.id = entries[w.block];
+      return at;
+    };
+    u32x4_v ck[KN];
+    Bytes<D / 32> cv[4];
+    auto load_keys = [&](const uint8_t *at) {
+      if (KS >= 8 || wave < KS)
 #pragma unroll
-      for (int k = 0; k < Codes::KN; k++) x.k[k] = *(const u32x4_v *)(at + 16 * (tid + 64 * NW * k));
-  };
-  auto load_values = [&](Codes &x, const uint8_t *at) {
+        for (int k = 0; k < KN; k++) ck[k] = *(const u32x4_v *)(at + 16 * (tid + 512 * k));
+    };
+    const int vtoken = 16 * (wave >> 1) + 8 * hl + 4 * (wave & 1);
+    auto load_values = [&](const uint8_t *at) {
 #pragma unroll
-    for (int r = 0; r < Codes::VN; r++)
+      for (int k = 0; k < 4; k++) cv[k] = *(const Bytes<D / 32> *)(at + (int64_t)P * D + (vtoken + k) * D + c * DT);
+    };
+    // keys: [32 tokens][16 dims][half of them][token] of eight dims; steps lie
+    // 65 groups apart, so that a wave's writes, 8 of a token's, fall on
+    // different banks
+    auto put_keys = [&](uint4 *dst) {
+      if (KS >= 8 || wave < KS)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int w = wave + NW * r, token = 16 * (w >> 1) + 8 * hl + 4 * (w & 1) + k;
-        x.v[r][k] = *(const Bytes<D / 32> *)(at + (int64_t)P * D + token * D + c * DT);
-      }
-  };
-  // keys: [32 tokens][16 dims][half of them][token, permuted by the step] of
-  // eight dims; the permutation spreads a wave's writes over the banks
-  auto put_keys = [&](const Codes &x, uint4 *dst) {
-    if (KS >= NW || wave < KS)
+        for (int k = 0; k < KN; k++) {
+          const int i = tid + 512 * k, token = i / KS, st = i % KS;
+          uint4 *at = dst + ((token >> 5) * KS + st) * KF + (token & 31);
 #pragma unroll
-      for (int k = 0; k < Codes::KN; k++) {
-        const int i = tid + 64 * NW * k, token = i / KS, s = i % KS;
-        uint4 *at = dst + ((token >> 5) * KS + s) * 64 + ((token & 31) ^ (s & 7));
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const uint32_t w0 = x.k[k][2 * b], w1 = x.k[k][2 * b + 1];
-          at[32 * b] = make_uint4(key2<FP8, 0>(w0), key2<FP8, 1>(w0), key2<FP8, 0>(w1), key2<FP8, 1>(w1));
+          for (int b = 0; b < 2; b++) {
+            const uint32_t w0 = ck[k][2 * b], w1 = ck[k][2 * b + 1];
+            at[32 * b] = make_uint4(key2<FP8, 0>(w0), key2<FP8, 1>(w0), key2<FP8, 0>(w1), key2<FP8, 1>(w1));
+          }
         }
-      }
-  };
-  // values: [dim tile e][16 tokens][half][r] of the eight tokens of a product's
-  // lane, for dim r D / 32 + e
-  auto put_values = [&](const Codes &x, uint4 *dst) {
-#pragma unroll
-    for (int r = 0; r < Codes::VN; r++) {
-      const int w = wave + NW * r;
-      uint2 *at = (uint2 *)(dst + ((w >> 1) * 64 + 32 * (w & 1) + c)) + hl;
+    };
+    // values: [dim tile e][16 tokens][half][r] of the eight tokens of a
+    // product's lane, for dim r D / 32 + e
+    auto put_values = [&](uint4 *dst) {
+      uint2 *at = (uint2 *)(dst + ((wave >> 1) * 64 + 32 * (wave & 1) + c)) + hl;
       auto one = [&](auto E) {
         constexpr int e = decltype(E)::value;
         uint32_t b[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) b[k] = x.v[r][k].word(e / 4);
+        for (int k = 0; k < 4; k++) b[k] = cv[k].word(e / 4);
         at[512 * e] = make_uint2(value2<FP8, e & 3>(b[0], b[1]), value2<FP8, e & 3>(b[2], b[3]));
       };
       each(one, std::make_integer_sequence<int, DT>{});
-    }
-  };
-  uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
-  auto scores = [&](const uint4 *src, f32x16_v s[2]) {
+    };
+    auto scores = [&](const uint4 *src) {
 #pragma unroll
-    for (int tt = 0; tt < 2; tt++) {
+      for (int tt = 0; tt < 2; tt++)
 #pragma unroll
-      for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
+        for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        const uint4 w = src[(tt * KS + k) * 64 + 32 * hl + (c ^ (k & 7))];
-        s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), qf[k], s[tt], 0, 0, 0);
-      }
-    }
-  };
-
-  f32x16_v s[2], next[2];
-  Codes codes;
-  Place here = {}, there = {}, beyond = {};
-  if (n > 0) {
-    here = locate(0);
-    load_keys(codes, here.at);
-    load_values(codes, here.at);
-    put_keys(codes, kb);
-    put_values(codes, vb);
-    if (n > 1) {
-      there = locate(1);
-      if (AHEAD) {
-        load_keys(codes, there.at);
-        put_keys(codes, kb + KB);
-      }
-    }
-    __syncthreads();
-    if (AHEAD) scores(kb, s);
-  }
-  for (int i = 0; i < n; i++) {
-    const int first = kv0 + i * kTile;
-    if (i + 1 < n) {
-      load_values(codes, there.at);
-      if (!AHEAD) load_keys(codes, there.at);
-    }
-    if (i + 2 < n) {
-      beyond = locate(i + 2);
-      if (AHEAD) load_keys(codes, beyond.at);
-    }
-    if (AHEAD) {
-      if (i + 1 < n) scores(kb + ((i + 1) & 1) * KB, next);
-    } else {
-      scores(kb + (i & 1) * KB, s);
-    }
-    const bool known = here.page != 0, whole = known && first + kTile <= all_hi && first >= all_lo;
-    uint32_t seen = ~0u;
-    if (!whole) {
-      seen = 0;
+      for (int k = 0; k < KS; k++)
 #pragma unroll
-      for (int k = 0; k < 32; k++) {
-        const int j = first + 32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hl + (k & 3);
-        const bool yes = known && j < hi && j >= lo;
-        seen |= (uint32_t)yes << k;
-        s[k >> 4][k & 15] = yes ? s[k >> 4][k & 15] : -INFINITY;
-      }
-    }
-    float best = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-    for (int k = 1; k < 16; k++) best = fmaxf(best, fmaxf(s[0][k], s[1][k]));
-    best = reduce_max2(best);
-    // a tile that the row does not see takes no part in it, whatever its peaks
-    const bool some = whole || (known && first < hi && first + kTile > lo);
-    const float f = some ? mult * here.peak.x : 1.f;
-    best = some ? best * f : -INFINITY;
-    const float high = some ? fmaxf(ref, here.peak.y) : ref;
-    if (__any(best > m + 8.f || high > ref)) {
-      const float raised = fmaxf(m, best);
-      const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
-      const float shrink = high > ref ? ref / high * was : was;
-      m = raised;
-      ref = high;
-      l *= was;
-#pragma unroll
-      for (int e = 0; e < DT; e++)
-#pragma unroll
-        for (int k = 0; k < 16; k++) o[e][k] *= shrink;
-    }
-    const float base = m == -INFINITY ? 0.f : m;
-    const float size = some ? here.peak.y / ref : 1.f;
-    const float off = __builtin_amdgcn_logf(size) - base;
-    float sum = 0;
-    half8_v pf[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      u32x4_v w;
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        float p[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const int at = 8 * j + 2 * k + b;
-          p[b] = __builtin_amdgcn_exp2f(fmaf(s[at >> 4][at & 15], f, off));
-          if (!whole) p[b] = seen >> at & 1 ? p[b] : 0.f;
-          sum += p[b];
+        for (int tt = 0; tt < 2; tt++) {
+          const uint4 w = src[(tt * KS + k) * KF + lane];
+          s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), qf[k], s[tt], 0, 0, 0);
         }
-        w[k] = f16_bits(p[0]) | f16_bits(p[1]) << 16;
-      }
-      pf[j] = __builtin_bit_cast(half8_v, w);
-    }
-    l += sum / size;
-    const uint4 *src = vb + (i & 1) * KB;
+    };
+    auto outputs = [&](const uint4 *src) {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+      for (int j = 0; j < 4; j++)
 #pragma unroll
-      for (int e = 0; e < DT; e++) {
-        const uint4 w = src[(4 * e + j) * 64 + lane];
-        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), pf[j], o[e], 0, 0, 0);
+        for (int e = 0; e < OT; e++) {
+          const uint4 w = src[(4 * (e0 + e) + j) * 64 + lane];
+          o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), pf[j], o[e], 0, 0, 0);
+        }
+    };
+    auto softmax = [&](int i, bool known, float2 peak) {
+      const int first = kv0 + i * kTile;
+      bool some = true;
+      if (!(known && first + kTile <= all_hi && first >= all_lo)) {  // some row does not see all of the tile
+        const int above = known ? hi - first - 4 * hl : 0, below = lo - first - 4 * hl;
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+          const int j = 32 * (k >> 4) + 8 * (k >> 2 & 3) + (k & 3);
+          s[k >> 4][k & 15] = j < above && j >= below ? s[k >> 4][k & 15] : -INFINITY;
+        }
+        some = known && first < hi && first + kTile > lo;
       }
-    if (i + 1 < n) {
-      put_values(codes, vb + ((i + 1) & 1) * KB);
-      if (!AHEAD) put_keys(codes, kb + ((i + 1) & 1) * KB);
-      if (AHEAD && i + 2 < n) put_keys(codes, kb + (i & 1) * KB);
+      float best = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int k = 1; k < 16; k++) best = fmaxf(fmaxf(best, s[0][k]), s[1][k]);
+      best = reduce_max2(best);
+      // a tile that the row does not see takes no part in it, whatever its
+      // peaks; a factor of 0 would make NaN of the scores that are masked
+      float f = mult * peak.x;
+      f = !some ? 1.f : f == 0.f ? 1e-37f : f;
+      best *= f;
+      const float high = some ? fmaxf(ref, peak.y) : ref;
+      if (__any(best > m + 8.f || high > ref)) {
+        const float raised = fmaxf(m, best);
+        const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
+        const float shrink = high > ref ? ref / high * was : was;
+        m = raised;
+        ref = high;
+        log_ref = ref > 0.f ? __builtin_amdgcn_logf(ref) : 0.f;
+        l *= was;
+#pragma unroll
+        for (int e = 0; e < OT; e++)
+#pragma unroll
+          for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      const float size = some ? __builtin_amdgcn_logf(peak.y) - log_ref : 0.f;
+      const float off = size - base;
+      float sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        u32x4_v w;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          float p[2];
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            const int at = 8 * j + 2 * k + b;
+            p[b] = __builtin_amdgcn_exp2f(fmaf(s[at >> 4][at & 15], f, off));
+            sum += p[b];
+          }
+          w[k] = half2_bits(__builtin_convertvector((f32x2_v){p[0], p[1]}, half2_v));
+        }
+        pf[j] = __builtin_bit_cast(half8_v, w);
+      }
+      l = fmaf(sum, __builtin_amdgcn_exp2f(-size), l);
+    };
+
+    if (n > 0) {
+      // Step j of the loop needs values j and keys j + 1.  The early waves put
+      // their share of them there in step j, the late ones, whose step j begins
+      // half a step later, in step j - 1.
+      Walk w, peaks;
+      begin(w);
+      begin(peaks);
+      bool known, unused;
+      const uint8_t *at = page_at(peaks, known);
+      float2 peak = *(const float2 *)(at + peaks_at);
+      const int sub0 = w.sub;
+      at = page_at(w, unused) + ((int64_t)(2 * h) * P + sub0 * kTile) * D;
+      auto next_tile = [&]() {
+        const int sub = w.sub;
+        bool k;
+        return page_at(w, k) + ((int64_t)(2 * h) * P + sub * kTile) * D;
+      };
+      load_keys(at);
+      put_keys(kb);
+      const uint8_t *keys = next_tile();
+      load_values(at);
+      load_keys(keys);
+      if (late) {
+        put_values(vb);
+        put_keys(kb + KB);
+        at = keys;
+        keys = next_tile();
+        load_values(at);
+        load_keys(keys);
+      }
       __syncthreads();
+      if (late) __syncthreads();
+      scores(kb);
+      __syncthreads();
+      for (int i = 0; i < n; i++) {
+        bool next_known;
+        const uint8_t *base = page_at(peaks, next_known);
+        const float2 next_peak = *(const float2 *)(base + peaks_at);
+        softmax(i, known, peak);
+        known = next_known, peak = next_peak;
+        // (past the last tile: into buffers that nothing reads)
+        put_values(vb + ((i + late) & 1) * VB);
+        put_keys(kb + ((i + late + 1) & 1) * KB);
+        at = keys;
+        keys = next_tile();
+        load_values(at);
+        load_keys(keys);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        outputs(vb + (i & 1) * VB);
+        scores(kb + ((i + 1) & 1) * KB);
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+      }
+      if (!late) __syncthreads();
+      __syncthreads();  // the next turn writes where the last products read
     }
-    here = there;
-    there = beyond;
-    if (AHEAD) s[0] = next[0], s[1] = next[1];
-  }
-  l = reduce_sum2(l);
-  if (!live) return;
-  const float unit = ref * kValueUnit<FP8>;
-  if (part < 0) {
-    const float f = l == 0.f ? 0.f : unit / l;
-    uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D;
+    l = reduce_sum2(l);
+    if (!live) continue;
+    const float unit = ref * kValueUnit<FP8>;
+    if (part < 0) {
+      const float f = l == 0.f ? 0.f : unit / l;
+      uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + e0;
 #pragma unroll
-    for (int k = 0; k < 16; k++) {
-      float x[DT];
+      for (int k = 0; k < 16; k++) {
+        float x[OT];
 #pragma unroll
-      for (int e = 0; e < DT; e++) x[e] = o[e][k] * f;
-      store_row<DT>(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT, a.dtype, x);
-    }
-  } else {
-    const int64_t slot = ((int64_t)part * a.kv_heads + h) * a.unit_rows + at_row + mine;
-    float *dst = a.ws + slot * D;
+        for (int e = 0; e < OT; e++) x[e] = o[e][k] * f;
+        store_row<OT>(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT, a.dtype == SQ_BF16, x);
+      }
+    } else {
+      const int64_t slot = ((int64_t)part * a.kv_heads + h) * a.unit_rows + turn + mine;
+      float *dst = a.ws + slot * D + e0;
 #pragma unroll
-    for (int k = 0; k < 16; k++)
+      for (int k = 0; k < 16; k++)
 #pragma unroll
-      for (int e = 0; e < DT; e += 2)
-        *(float2 *)(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT + e) = make_float2(o[e][k] * unit, o[e + 1][k] * unit);
-    if (hl == 0) {
-      float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
-      ml[0] = m;
-      ml[1] = l;
+        for (int e = 0; e < OT; e += 2)
+          *(float2 *)(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT + e) = make_float2(o[e][k] * unit, o[e + 1][k] * unit);
+      if (hl == 0 && e0 == 0) {
+        float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
+        ml[0] = m;
+        ml[1] = l;
+      }
     }
   }
 }
@@ -1231,7 +1260,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(AttendDev a) {
       }
       x *= sum == 0.f ? 0.f : 1.f / sum;
       const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
-      store_row<4>(a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane, a.dtype, (const float *)&x);
+      store_row<4>(a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane, a.dtype == SQ_BF16, (const float *)&x);
     }
     __syncthreads();
   }
@@ -1309,7 +1338,7 @@ int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
 }
 
 // Raises a kernel's limit of dynamic LDS, once per kernel (each with an id of
-// its own) and device, to 128 KiB, the most that one takes.
+// its own) and device, to 136 KiB, more than the most that one takes.
 std::atomic<uint64_t> g_raised[16];
 
 int dynamic_lds(const void *kernel, int id, size_t bytes, const char *what) {
@@ -1319,7 +1348,7 @@ int dynamic_lds(const void *kernel, int id, size_t bytes, const char *what) {
   if (e != hipSuccess) return fail((int)e, what);
   const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
   if (g_raised[id].load(std::memory_order_relaxed) & bit) return 0;
-  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024);
   if (e != hipSuccess) return fail((int)e, what);
   g_raised[id].fetch_or(bit, std::memory_order_relaxed);
   return 0;
@@ -1329,19 +1358,18 @@ int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 template <int D, bool FP8>
 int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
-  auto go = [&](auto kernel, int id, int threads, size_t lds, int blocks = 1) {
+  auto go = [&](auto kernel, int id, int threads, size_t lds) {
     const int rc = dynamic_lds((const void *)kernel, 2 * id + FP8, lds, "kv attend: LDS attribute");
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_units * s.kv_heads), (unsigned)blocks), dim3(threads), lds, st, d);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_units * s.kv_heads)), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
   static_assert(D <= 256, "ids of kernels with more than 64 KiB: one dim has them");
-  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 4 * 64 * D * sizeof(uint16_t);
+  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64);
   int rc;
   if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
   else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
-  else if (s.rows == 128 || D == 256) rc = go(kv_attend_rows_kernel<D, 4, FP8, true>, 3, 256, staged, s.rows / 128);
-  else if constexpr (D != 256) rc = go(kv_attend_rows_kernel<D, 8, FP8, true>, 4, 512, staged);
+  else rc = go(kv_attend_rows_kernel<D, FP8>, 3, 512, staged);
   if (rc || !s.max_merges) return rc;
   const unsigned rows = s.merge_rows < 16 ? s.merge_rows : 16;
   hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), rows), dim3(256), 0, st, d);
