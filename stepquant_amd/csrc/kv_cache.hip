@@ -941,6 +941,10 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
   const int32_t *entries = a.table + (int64_t)row * a.width;
   uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
+  // the peaks of two tiles, and whether their pages exist
+  float4 *const peaks = (float4 *)(vb + 2 * VB);
+  const int pages = (int)a.c.num_pages, first_key = 2 * h * P * D;
+  const uint32_t page_bytes = (uint32_t)a.c.page_bytes;
 
   for (int turn = 0; turn < u[3]; turn += WR) {
     const int f0 = u[2] + turn, rows = min(u[3] - turn, WR);
@@ -990,23 +994,20 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
     float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
 
     // The tiles in order; past the last one the last again, so that loads ahead
-    // need no branch.
-    struct Walk {
-      int block, sub, left, id;
-    };
-    auto begin = [&](Walk &w) {
-      w.block = tile0 / per, w.sub = tile0 - w.block * per, w.left = n;
-      w.id = entries[w.block];
-    };
-    auto page_at = [&](Walk &w, bool &known) {  // and a step on; the next page's number is loaded a step ahead
-      const int page = __builtin_amdgcn_readfirstlane(w.id);
-      known = page > 0 && page < a.c.num_pages;
-      const uint8_t *at = a.c.data + (known ? page : 0) * a.c.page_bytes;
-      w.left--;
-      const bool more = w.left > 0, next = w.sub + 1 == per;
-      w.sub = more ? next ? 0 : w.sub + 1 : w.sub;
-      w.block += more && next;
-      w.id = entries[w.block];
+    // need no branch.  A page's number is loaded a tile before it is used.
+    int block = tile0 / per, sub = tile0 - block * per, left = n, id = n > 0 ? entries[block] : 0;
+    bool known;
+    const uint8_t *base;  // of the page of the tile
+    auto next_tile = [&]() {
+      const int page = __builtin_amdgcn_readfirstlane(id);
+      known = page > 0 && page < pages;
+      base = a.c.data + (uint64_t)(uint32_t)(known ? page : 0) * page_bytes;
+      const uint8_t *at = base + first_key + sub * (kTile * D);
+      left--;
+      const bool more = left > 0, turned = sub + 1 == per;
+      sub = more ? turned ? 0 : sub + 1 : sub;
+      block = __builtin_amdgcn_readfirstlane(block + (more && turned));
+      id = entries[block];
       return at;
     };
     u32x4_v ck[KN];
@@ -1050,37 +1051,52 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       };
       each(one, std::make_integer_sequence<int, DT>{});
     };
-    auto scores = [&](const uint4 *src) {
+    // Outputs with one tile's values (with VALUES), then scores with another
+    // one's keys; the operands are read DEEP products ahead.
+    auto products = [&](auto VALUES, const uint4 *values, const uint4 *keys) {
+      constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + 2 * KS, DEEP = 8;
 #pragma unroll
       for (int tt = 0; tt < 2; tt++)
 #pragma unroll
         for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
+      uint4 w[DEEP];
+      auto read = [&](int i) {
+        const int k = (i - NV) >> 1, tt = (i - NV) & 1;
+        return i < NV ? values[(4 * (e0 + i % OT) + i / OT) * 64 + lane] : keys[(tt * KS + k) * KF + lane];
+      };
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+      for (int i = 0; i < DEEP; i++) w[i] = read(i);
 #pragma unroll
-        for (int tt = 0; tt < 2; tt++) {
-          const uint4 w = src[(tt * KS + k) * KF + lane];
-          s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), qf[k], s[tt], 0, 0, 0);
-        }
+      for (int i = 0; i < N; i++) {
+        const half8_v x = __builtin_bit_cast(half8_v, w[i % DEEP]);
+        if (i < NV) o[i % OT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[i / OT], o[i % OT], 0, 0, 0);
+        else s[(i - NV) & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - NV) >> 1], s[(i - NV) & 1], 0, 0, 0);
+        if (i + DEEP < N) w[i % DEEP] = read(i + DEEP);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, DEEP, 0);  // LDS reads
+#pragma unroll
+      for (int i = 0; i < N - DEEP; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, DEEP, 0);
     };
-    auto outputs = [&](const uint4 *src) {
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int e = 0; e < OT; e++) {
-          const uint4 w = src[(4 * (e0 + e) + j) * 64 + lane];
-          o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, w), pf[j], o[e], 0, 0, 0);
-        }
-    };
-    auto softmax = [&](int i, bool known, float2 peak) {
+    auto softmax = [&](int i) {
+      const float4 peak = peaks[i & 1];
       const int first = kv0 + i * kTile;
+      const bool known = __builtin_amdgcn_readfirstlane(__float_as_uint(peak.z)) != 0;
       bool some = true;
       if (!(known && first + kTile <= all_hi && first >= all_lo)) {  // some row does not see all of the tile
         const int above = known ? hi - first - 4 * hl : 0, below = lo - first - 4 * hl;
 #pragma unroll
         for (int k = 0; k < 32; k++) {
           const int j = 32 * (k >> 4) + 8 * (k >> 2 & 3) + (k & 3);
-          s[k >> 4][k & 15] = j < above && j >= below ? s[k >> 4][k & 15] : -INFINITY;
+          // all ones where below <= j < above; as conditions, 64 of them would
+          // spill the loop's scalar registers
+          int seen = ((j - above) & (below - 1 - j)) >> 31;
+          asm("" : "+v"(seen));
+          const float x = s[k >> 4][k & 15];
+          s[k >> 4][k & 15] = __uint_as_float((__float_as_uint(x) & seen) | (0xff800000u & ~seen));
         }
         some = known && first < hi && first + kTile > lo;
       }
@@ -1134,53 +1150,44 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       // Step j of the loop needs values j and keys j + 1.  The early waves put
       // their share of them there in step j, the late ones, whose step j begins
       // half a step later, in step j - 1.
-      Walk w, peaks;
-      begin(w);
-      begin(peaks);
-      bool known, unused;
-      const uint8_t *at = page_at(peaks, known);
-      float2 peak = *(const float2 *)(at + peaks_at);
-      const int sub0 = w.sub;
-      at = page_at(w, unused) + ((int64_t)(2 * h) * P + sub0 * kTile) * D;
-      auto next_tile = [&]() {
-        const int sub = w.sub;
-        bool k;
-        return page_at(w, k) + ((int64_t)(2 * h) * P + sub * kTile) * D;
+      const uint8_t *at = next_tile();
+      // (values and keys that a thread holds on their way to LDS; with the keys
+      // their tile's peaks)
+      float4 peak;
+      auto load = [&](const uint8_t *values, const uint8_t *keys) {
+        if (values) load_values(values);
+        load_keys(keys);
+        const float2 x = *(const float2 *)(base + peaks_at);
+        peak = make_float4(x.x, x.y, known ? 1.f : 0.f, 0.f);
       };
-      load_keys(at);
+      load(nullptr, at);
       put_keys(kb);
+      if (tid == 0) peaks[0] = peak;
       const uint8_t *keys = next_tile();
-      load_values(at);
-      load_keys(keys);
+      load(at, keys);
       if (late) {
         put_values(vb);
         put_keys(kb + KB);
         at = keys;
         keys = next_tile();
-        load_values(at);
-        load_keys(keys);
+        load(at, keys);
       }
       __syncthreads();
       if (late) __syncthreads();
-      scores(kb);
+      products(std::false_type{}, vb, kb);
       __syncthreads();
       for (int i = 0; i < n; i++) {
-        bool next_known;
-        const uint8_t *base = page_at(peaks, next_known);
-        const float2 next_peak = *(const float2 *)(base + peaks_at);
-        softmax(i, known, peak);
-        known = next_known, peak = next_peak;
+        softmax(i);
         // (past the last tile: into buffers that nothing reads)
         put_values(vb + ((i + late) & 1) * VB);
         put_keys(kb + ((i + late + 1) & 1) * KB);
+        if (tid == 0) peaks[(i + 1) & 1] = peak;
         at = keys;
         keys = next_tile();
-        load_values(at);
-        load_keys(keys);
+        load(at, keys);
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
-        outputs(vb + (i & 1) * VB);
-        scores(kb + ((i + 1) & 1) * KB);
+        products(std::true_type{}, vb + (i & 1) * VB, kb + ((i + 1) & 1) * KB);
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
       }
@@ -1279,7 +1286,7 @@ int check_cache(const sq_kv_cache *c) {
   if (c->page_tokens <= 0 || c->page_tokens % kTile || c->page_tokens * (int64_t)c->dim > 32768)
     return fail(SQ_ESHAPE, "kv cache: page_tokens must be a multiple of 64 with page_tokens * dim <= 32768");
   if (c->storage != SQ_KV_INT8 && c->storage != SQ_KV_FP8) return fail(SQ_ESTORAGE, "kv cache: unknown storage");
-  if (c->num_pages <= 0 || c->num_pages > 0x7fffffff || c->page_bytes % 16 ||
+  if (c->num_pages <= 0 || c->num_pages > 0x7fffffff || c->page_bytes % 16 || c->page_bytes > 0x7fffffff ||
       c->page_bytes < (int64_t)c->heads * (2 * (int64_t)c->page_tokens * c->dim + 8))
     return fail(SQ_EINVAL, "kv cache: page count or page bytes");
   return 0;
@@ -1365,7 +1372,7 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
     return sq_internal_launched("kv_attend_kernel");
   };
   static_assert(D <= 256, "ids of kernels with more than 64 KiB: one dim has them");
-  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64);
+  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1);
   int rc;
   if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
   else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
