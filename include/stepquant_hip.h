@@ -424,26 +424,32 @@ typedef struct sq_kv_tables {
 /*
  * How one kind of attention layer splits its work, filled by sq_kv_plan.
  * One unit is `rows` query rows (token-major, the heads of a group inside a
- * token) against a range of keys; units of one set of rows that was cut are
- * joined by a merge.  With tokens, batch, G = q_heads / kv_heads and
- * s = slots / kv_heads (rounded down where a count is meant):
- *   max_units    >= ceil(tokens * G / rows) + batch + 1 + s
+ * token) against a range of keys; a worker (one workgroup for each KV head)
+ * takes units starts[w] to starts[w + 1] - 1.  Units of rows whose keys were
+ * cut between workers are joined by a merge.  With tokens, batch,
+ * G = q_heads / kv_heads, sets = ceil(tokens * G / rows) + batch + 1 and
+ * s = max(1, slots / kv_heads):
+ *   max_workers  >= max(sets, s), and starts holds max_workers + 1
+ *   max_units    >= sets + s
  *   max_merges   >= s
- *   max_partials >= 2 * slots / kv_heads
+ *   max_partials >= 2 * s
  */
 typedef struct sq_kv_schedule {
     int32_t *units;       /* [max_units, 8] */
     int32_t *merges;      /* [max_merges, 8] */
+    int32_t *starts;      /* [max_workers + 1] */
     int32_t max_units;
     int32_t max_merges;
+    int32_t max_workers;
     int32_t max_partials;
     int32_t q_heads;
     int32_t kv_heads;
-    int32_t rows;         /* 16, 32, 128 or 256 */
+    int32_t rows;         /* 16, 32 or 256 */
     int32_t causal;
     int32_t window;       /* 0: none; else the last `window` keys (causal only) */
-    int32_t slots;        /* workgroups that the device holds at once */
-    int32_t min_tiles;    /* least 64-key tiles of a part, at least 1 */
+    int32_t slots;        /* workgroups that the device holds at once, at most 4096 */
+    int32_t min_tiles;    /* least 64-key tiles of a worker, at least 1 */
+    int32_t cut_tiles;    /* what a cut costs, in tiles of work */
     int32_t merge_rows;   /* most rows of a unit: min(rows, max_count * G) */
     int32_t reserved;
 } sq_kv_schedule;

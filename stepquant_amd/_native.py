@@ -86,11 +86,9 @@ class KVTables(ctypes.Structure):
 
 
 class KVSchedule(ctypes.Structure):
-    _fields_ = [("units", _P), ("merges", _P), ("max_units", ctypes.c_int32), ("max_merges", ctypes.c_int32),
-                ("max_partials", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
-                ("rows", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
-                ("slots", ctypes.c_int32), ("min_tiles", ctypes.c_int32), ("merge_rows", ctypes.c_int32),
-                ("reserved", ctypes.c_int32)]
+    _fields_ = [("units", _P), ("merges", _P), ("starts", _P)] + [(n, ctypes.c_int32) for n in (
+        "max_units", "max_merges", "max_workers", "max_partials", "q_heads", "kv_heads", "rows", "causal", "window",
+        "slots", "min_tiles", "cut_tiles", "merge_rows", "reserved")]
 
 
 KV_INT8, KV_FP8 = 0, 1
@@ -235,7 +233,7 @@ def step_entry(name: str):
 
 
 # the KV cache's argument blocks in the order of their structures' fields, as above
-KV_SCHEDULE = struct.Struct("=2Q12i")
+KV_SCHEDULE = struct.Struct("=3Q14i")
 KV_PLAN = struct.Struct(f"=11Qq6i{KV_MAX_SCHEDULES * KV_SCHEDULE.size}s")
 KV_APPEND = struct.Struct("=5Q5q2i")
 KV_ATTEND = struct.Struct(f"=4Q4q2ifi{KV_SCHEDULE.size}s")

@@ -59,6 +59,7 @@ __device__ __forceinline__ int64_t load_index(const void *p, int dtype, int64_t 
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanItems = SQ_KV_MAX_REQUESTS / kPlanThreads;
+constexpr int kMaxSlots = 4096;
 constexpr int kPlanShare = 1024;  // tokens (and page entries) of one workgroup
 
 struct PlanDev {
@@ -109,12 +110,17 @@ struct PlanLds {
   int32_t *row;
 };
 
-// One attention layer's units: sets of `rows` query rows, the longest key
-// ranges of a request first, each cut into near-equal parts of at most
-// `chunk` key tiles.  chunk is the work that each of the device's slots has
-// when it is spread evenly, so a set is cut only where it would outlast the
-// others.
+// One attention layer's units: sets of `rows` query rows with the tiles of
+// keys that they see, the longest of a request first.
+//
+// Either every set is a worker of its own, and the device takes them as its
+// slots come free: then the last ones to start, the short ones, decide how
+// unevenly it ends.  Or the sets' tiles, one after the other, are dealt out in
+// equal shares, one for each slot, and sets that lie across a border are cut
+// there.  The second costs `cut_tiles` a worker (partial results to write, to
+// read and to join) and is taken where it ends sooner by that count.
 __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, int64_t *waves) {
+  __shared__ int32_t starts[kMaxSlots + 1];
   const int tid = threadIdx.x, B = p.batch, G = s.q_heads / s.kv_heads, tokens = (int)p.tokens;
   const int NB = B + 1;  // the last: packed rows past every request's
   auto row_count = [&](int b) { return (b < B ? L.end[b] : tokens) - (b ? L.end[b - 1] : 0); };
@@ -151,19 +157,46 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
     }
     return r;
   };
+  int most = 0, least = 0x7fffffff;
   sum = 0;
-  for (int e = tid; e < sets; e += kPlanThreads) sum += find(e).n;
-  block_scan<kPlanThreads>(sum, &total, waves);
-  const int64_t chunk = max((int64_t)s.min_tiles, (total * s.kv_heads + s.slots - 1) / s.slots);
+  for (int e = tid; e < sets; e += kPlanThreads) {
+    const int n = find(e).n;
+    sum += n;
+    most = max(most, n);
+    least = min(least, n);
+  }
+  int64_t tiles;
+  block_scan<kPlanThreads>(sum, &tiles, waves);
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    most = max(most, __shfl_xor(most, k, 64));
+    least = min(least, __shfl_xor(least, k, 64));
+  }
+  __syncthreads();
+  if ((tid & 63) == 0) waves[tid >> 6] = (int64_t)most << 32 | (uint32_t)least;
+  __syncthreads();
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    most = max(most, (int)(waves[w] >> 32));
+    least = min(least, (int)(uint32_t)waves[w]);
+  }
+  const int64_t slots = max(1, s.slots / s.kv_heads);
+  const int64_t workers = max((int64_t)1, min(slots, tiles / s.min_tiles)), share = (tiles + workers - 1) / workers;
+  // tiles until the last slot is done, either way
+  const int64_t whole = sets <= slots ? most : max((int64_t)most, (tiles + slots - 1) / slots + least);
+  const bool dealt = share + s.cut_tiles < whole;
+  if (dealt)
+    for (int w = tid; w <= workers; w += kPlanThreads) starts[w] = 0x7fffffff;
   int units = 0, parts = 0, merges = 0;
+  int64_t before = 0;  // tiles of the sets before
   for (int e0 = 0; e0 < sets; e0 += kPlanThreads) {
     const int e = e0 + tid;
     Set r = {};
-    int k = 0;
-    if (e < sets) {
-      r = find(e);
-      k = max(1, (int)((r.n + chunk - 1) / chunk));
-    }
+    if (e < sets) r = find(e);
+    const int64_t a = before + block_scan<kPlanThreads>(r.n, &total, waves) - r.n;
+    before += total;
+    // worker w has the tiles from w tiles / workers (rounded down) on
+    auto worker_of = [&](int64_t tile) { return (int)min(workers - 1, ((tile + 1) * workers - 1) / max((int64_t)1, tiles)); };
+    const int w0 = dealt ? worker_of(a) : 0, k = e >= sets ? 0 : dealt && r.n ? worker_of(a + r.n - 1) - w0 + 1 : 1;
     const int cut = k > 1;
     // three sums in one: units and parts stay below 2^24, merges below 2^16
     const int64_t mine = (int64_t)k | (int64_t)(cut ? k : 0) << 24 | (int64_t)cut << 48;
@@ -173,7 +206,8 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
     for (int j = 0; j < k; j++) {
       if (u + j >= s.max_units) break;
       int32_t *o = s.units + 8 * (int64_t)(u + j);
-      const int t0 = (int)((int64_t)r.n * j / k), t1 = (int)((int64_t)r.n * (j + 1) / k);
+      const int64_t border0 = (w0 + j) * tiles / workers, border1 = (w0 + j + 1) * tiles / workers;
+      const int t0 = j ? (int)(border0 - a) : 0, t1 = j + 1 < k ? (int)(border1 - a) : r.n;
       o[0] = r.b < B ? L.row[r.b] : 0;
       o[1] = q0;
       o[2] = r.f0;
@@ -182,6 +216,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
       o[5] = r.kv0 + t0 * kTile;
       o[6] = min(r.kv1, r.kv0 + t1 * kTile);
       o[7] = cut ? q + j : -1;
+      if (dealt) atomicMin(&starts[w0 + j], u + j);
     }
     if (cut && m < s.max_merges) {
       int32_t *o = s.merges + 8 * (int64_t)m;
@@ -193,7 +228,9 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
     }
     units += (int)(total & 0xffffff), parts += (int)(total >> 24 & 0xffffff), merges += (int)(total >> 48);
   }
-  for (int u = units + tid; u < s.max_units; u += kPlanThreads) s.units[8 * (int64_t)u + 3] = 0;
+  __syncthreads();
+  for (int w = tid; w <= s.max_workers; w += kPlanThreads)
+    s.starts[w] = dealt ? w < workers ? min(units, starts[w]) : units : min(units, w);
   for (int m = merges + tid; m < s.max_merges; m += kPlanThreads) s.merges[8 * (int64_t)m + 2] = 0;
 }
 
@@ -543,8 +580,9 @@ struct AttendDev {
   const int32_t *table;
   const int32_t *units;
   const int32_t *merges;
+  const int32_t *starts;
   int64_t requests, tokens, q_stride, q_head_stride;
-  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials, unit_rows;
+  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials, max_units, unit_rows;
   float scale;
 };
 
@@ -658,13 +696,14 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   extern __shared__ float smem[];
   constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % a.kv_heads;
-  const int32_t *u = a.units + 8 * (int64_t)(blockIdx.x / a.kv_heads);
+  const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
+  const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
+  for (int unit_at = unit0; unit_at < unit1; unit_at++) {
+  const int32_t *u = a.units + 8 * (int64_t)unit_at;
   const int row = u[0], q0 = u[1], f0 = u[2], rows = u[3], pos0 = u[4], kv0 = u[5], part = u[7];
   // a row of the table that does not exist holds no keys
   const int kv1 = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
-  const int G = a.q_heads / a.kv_heads;
-  if (rows <= 0 || rows > 16 * RT || q0 < 0 || f0 < 0 || q0 + (int64_t)(f0 + rows - 1) / G >= a.tokens) return;
+  if (rows <= 0 || rows > 16 * RT || q0 < 0 || f0 < 0 || q0 + (int64_t)(f0 + rows - 1) / G >= a.tokens) continue;
   // queries
   half8_v qf[RT][KS];
   float mult[RT], m[RT], l[RT];
@@ -902,6 +941,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
       }
     }
   }
+  __syncthreads();  // before the next unit's shares
+  }
 }
 
 typedef float f32x16_v __attribute__((ext_vector_type(16)));
@@ -931,11 +972,12 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   constexpr int KN = KS > 8 ? KS / 8 : 1;                   // 16-byte groups of keys of a thread
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hl = lane >> 5;
   const int late = wave >> 2, e0 = D == 256 ? late * OT : 0;
-  const int h = blockIdx.x % a.kv_heads;
-  const int32_t *u = a.units + 8 * (int64_t)(blockIdx.x / a.kv_heads);
+  const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
+  const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
+  for (int unit_at = unit0; unit_at < unit1; unit_at++) {
+  const int32_t *u = a.units + 8 * (int64_t)unit_at;
   const int row = u[0], q0 = u[1], pos0 = u[4], kv0 = u[5], part = u[7];
-  const int G = a.q_heads / a.kv_heads;
-  if (u[3] <= 0 || u[3] > a.unit_rows || q0 < 0 || u[2] < 0 || q0 + (int64_t)(u[2] + u[3] - 1) / G >= a.tokens) return;
+  if (u[3] <= 0 || u[3] > a.unit_rows || q0 < 0 || u[2] < 0 || q0 + (int64_t)(u[2] + u[3] - 1) / G >= a.tokens) continue;
   const int end = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
   const int P = a.c.page_tokens, per = P / kTile, tile0 = kv0 / kTile;
   const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
@@ -1222,6 +1264,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       }
     }
   }
+  }
 }
 
 // Joins the parts of query rows: one workgroup per (merge, head) and row, or
@@ -1301,22 +1344,24 @@ int check_tables(const sq_kv_tables *t) {
 }
 
 int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
-  if (!s->units || s->max_units <= 0 || (s->max_merges > 0 && !s->merges) || s->max_merges < 0)
-    return fail(SQ_EINVAL, "kv schedule: null pointer or negative size");
+  if (!s->units || !s->merges || !s->starts) return fail(SQ_EINVAL, "kv schedule: null pointer");
   if (s->kv_heads <= 0 || s->q_heads <= 0 || s->q_heads % s->kv_heads)
     return fail(SQ_ESHAPE, "kv schedule: q_heads must be a positive multiple of kv_heads");
-  if (s->rows != 16 && s->rows != 32 && s->rows != 128 && s->rows != 256) return fail(SQ_ESHAPE, "kv schedule: rows");
+  if (s->rows != 16 && s->rows != 32 && s->rows != 256) return fail(SQ_ESHAPE, "kv schedule: rows");
   if (s->window < 0 || (s->window > 0 && !s->causal))
     return fail(SQ_EINVAL, "kv schedule: a window is non-negative and needs causal attention");
-  if (s->slots <= 0 || s->slots > 1 << 16) return fail(SQ_EINVAL, "kv schedule: slots must be in [1, 65536]");
-  if (s->min_tiles <= 0 || s->merge_rows <= 0 || s->merge_rows > s->rows) return fail(SQ_EINVAL, "kv schedule: min_tiles or merge_rows");
+  if (s->slots <= 0 || s->slots > kMaxSlots) return fail(SQ_EINVAL, "kv schedule: slots must be in [1, 4096]");
+  if (s->min_tiles <= 0 || s->cut_tiles < 0 || s->merge_rows <= 0 || s->merge_rows > s->rows)
+    return fail(SQ_EINVAL, "kv schedule: min_tiles, cut_tiles or merge_rows");
   const int64_t G = s->q_heads / s->kv_heads;
   if (tokens * G > 0x3fffffff) return fail(SQ_EINVAL, "kv schedule: tokens * heads of a group too large");
   const int64_t sets = (tokens * G + s->rows - 1) / s->rows + batch + 1;
-  if (sets + s->slots / s->kv_heads > s->max_units || s->slots / s->kv_heads > s->max_merges ||
-      2 * s->slots / s->kv_heads > s->max_partials || s->max_units >= 1 << 24)
-    return fail(SQ_EINVAL, "kv schedule: room for units, merges or partials");
-  if ((int64_t)s->max_units * s->kv_heads > 0x7fffffff) return fail(SQ_EINVAL, "kv schedule: units * heads too large");
+  const int64_t slots = s->slots / s->kv_heads > 1 ? s->slots / s->kv_heads : 1;
+  if (s->max_workers < (sets > slots ? sets : slots) || s->max_units < sets + slots || s->max_merges < slots ||
+      s->max_partials < 2 * slots || s->max_units >= 1 << 24)
+    return fail(SQ_EINVAL, "kv schedule: room for workers, units, merges or partials");
+  if ((int64_t)s->max_workers * s->kv_heads > 0x7fffffff || (int64_t)s->max_merges * s->kv_heads > 0x7fffffff)
+    return fail(SQ_EINVAL, "kv schedule: workers * heads too large");
   return 0;
 }
 
@@ -1368,7 +1413,7 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
   auto go = [&](auto kernel, int id, int threads, size_t lds) {
     const int rc = dynamic_lds((const void *)kernel, 2 * id + FP8, lds, "kv attend: LDS attribute");
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_units * s.kv_heads)), dim3(threads), lds, st, d);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_workers * s.kv_heads)), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
   static_assert(D <= 256, "ids of kernels with more than 64 KiB: one dim has them");
@@ -1377,7 +1422,7 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
   if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
   else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
   else rc = go(kv_attend_rows_kernel<D, FP8>, 3, 512, staged);
-  if (rc || !s.max_merges) return rc;
+  if (rc) return rc;
   const unsigned rows = s.merge_rows < 16 ? s.merge_rows : 16;
   hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), rows), dim3(256), 0, st, d);
   return sq_internal_launched("kv_merge_kernel");
@@ -1477,11 +1522,11 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   rc = check_schedule(&a->schedule, a->tokens, 1);
   if (rc) return rc;
   if (a->schedule.kv_heads != c->heads) return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads");
-  if (a->schedule.max_merges && !a->workspace) return fail(SQ_EINVAL, "kv attend: null workspace");
+  if (!a->workspace) return fail(SQ_EINVAL, "kv attend: null workspace");
   const sq_kv_schedule &s = a->schedule;
-  const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges,
+  const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges, s.starts,
                        a->requests, a->tokens, a->q_stride, a->q_head_stride, a->width, a->dtype, s.q_heads, s.kv_heads,
-                       s.causal, s.window, s.max_partials, s.rows, a->scale};
+                       s.causal, s.window, s.max_partials, s.max_units, s.rows, a->scale};
   const bool fp8 = c->storage == SQ_KV_FP8;
   hipStream_t st = (hipStream_t)stream;
   if (c->dim == 64) return fp8 ? launch_attend<64, true>(d, s, st) : launch_attend<64, false>(d, s, st);

@@ -173,9 +173,10 @@ class BlockTables:
         flags = -(-batch // 4)
         sizes = [batch + 1, tokens, batch, flags, most, most, 2 * most]
         if windows:
-            max_units, max_merges, max_partials, q_heads, kv_heads, unit_rows, slots, merge_rows = shape
+            sets, cuts, q_heads, kv_heads, unit_rows, slots, merge_rows = shape
+            workers = max(sets, cuts)
             sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
-            sizes += [8 * (max_units + max_merges)] * len(windows)
+            sizes += [8 * (sets + 2 * cuts) + (workers + 8) // 8 * 8] * len(windows)
         p._sizes = sizes
         p._ints = ints = torch.empty(sum(sizes), dtype=torch.int32, device=self.device)
         p._longs = longs = torch.empty(2 + tokens, dtype=torch.int64, device=self.device)
@@ -187,9 +188,11 @@ class BlockTables:
         p.schedules, packed = {}, b""
         for w, units in zip(windows, at[7:]):
             s = _Schedule()
-            s.packed = N.KV_SCHEDULE.pack(units, units + 32 * max_units, max_units, max_merges, max_partials, q_heads,
-                                          kv_heads, unit_rows, bool(causal), int(w), slots, self.min_tiles, merge_rows, 0)
-            s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, max_partials * kv_heads * unit_rows
+            merges = units + 32 * (sets + cuts)
+            s.packed = N.KV_SCHEDULE.pack(units, merges, merges + 32 * cuts, sets + cuts, cuts, workers, 2 * cuts, q_heads,
+                                          kv_heads, unit_rows, bool(causal), int(w), slots, self.min_tiles,
+                                          self.cut_tiles[unit_rows], merge_rows, 0)
+            s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, 2 * cuts * kv_heads * unit_rows
             p.schedules[int(w)] = s
             packed += s.packed
         p._append = (at[4], at[5], at[6])
@@ -202,18 +205,18 @@ class BlockTables:
             N.check(rc, "kv plan")
         return p
 
-    min_tiles = 8  # least 64-key tiles of a part
+    min_tiles = 8  # least 64-key tiles of a workgroup where a set of rows is cut
+    cut_tiles = {16: 4, 32: 4, 256: 16}  # what its partial results cost, in tiles
 
     def _shape(self, q_heads, kv_heads, tokens, batch, max_new):
         if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
             raise ValueError("query heads must be a positive multiple of KV heads")
         group = q_heads // kv_heads
         most = max_new * group
-        rows = 16 if most <= 16 else 32 if most <= 32 else 128 if most <= 128 else 256
+        rows = 16 if most <= 16 else 32 if most <= 32 else 256
         slots = self._cus if rows == 256 else 2 * self._cus
-        merges = slots // kv_heads
-        return (-(-tokens * group // rows) + batch + 1 + merges, merges, 2 * slots // kv_heads, q_heads, kv_heads, rows,
-                slots, max(1, min(rows, most)))
+        return (-(-tokens * group // rows) + batch + 1, max(1, slots // kv_heads), q_heads, kv_heads, rows, slots,
+                max(1, min(rows, most)))
 
     def commit(self, plan):
         """Takes a plan's lengths and pages over; plans made before it are void."""

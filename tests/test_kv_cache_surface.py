@@ -45,8 +45,8 @@ def _tables(**kw):
 
 
 def _schedule(**kw):
-    a = dict(units=16, merges=16, max_units=4 + 2 + 1 + 256, max_merges=256, max_partials=512, q_heads=8, kv_heads=2,
-             rows=16, causal=1, window=0, slots=512, min_tiles=1, merge_rows=16)
+    a = dict(units=16, merges=16, starts=16, max_units=4 + 2 + 1 + 256, max_merges=256, max_workers=256, max_partials=512,
+             q_heads=8, kv_heads=2, rows=16, causal=1, window=0, slots=512, min_tiles=1, merge_rows=16)
     return N.KVSchedule(**{**a, **kw})
 
 
@@ -76,7 +76,8 @@ def test_caches_are_checked_before_any_launch(cache, code):
     ({}, dict(batch=4097), {}), ({}, dict(tokens=-1), {}), ({}, dict(max_tiles=3), {}), ({}, dict(n_schedules=5), {}),
     ({}, dict(max_count=-1), {}), ({}, {}, dict(units=None)), ({}, {}, dict(q_heads=7)), ({}, {}, dict(rows=48)),
     ({}, {}, dict(window=3, causal=0)), ({}, {}, dict(window=-1)), ({}, {}, dict(slots=0)), ({}, {}, dict(max_units=262)),
-    ({}, {}, dict(max_merges=255)), ({}, {}, dict(max_partials=511)), ({}, {}, dict(min_tiles=0)),
+    ({}, {}, dict(max_merges=255)), ({}, {}, dict(max_partials=511)), ({}, {}, dict(max_workers=255)),
+    ({}, {}, dict(slots=4097)), ({}, {}, dict(starts=None)), ({}, {}, dict(cut_tiles=-1)), ({}, {}, dict(min_tiles=0)),
     ({}, {}, dict(merge_rows=15)), ({}, {}, dict(merge_rows=17))])
 def test_plans_are_checked_before_any_launch(tables, plan, schedule):
     rc = N.lib().sq_kv_plan(_tables(**tables), _plan(_schedule(**schedule), **plan), None)
