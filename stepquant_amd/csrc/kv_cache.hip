@@ -690,258 +690,273 @@ __device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float 
 }
 
 // Units of up to 16 RT rows: the four waves take a unit's tiles in turn and
-// are joined at its end; keys and values go from memory to registers.
+// are joined at its end; keys and values go from memory to registers.  The
+// next tile's keys are under way during a tile's softmax, and the next unit's
+// first ones while the waves are joined.  Tiles of 256 dims are taken by
+// halves, which keeps a lane within 256 registers and two waves on a SIMD.
 template <int D, int RT, bool FP8>
 __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendDev a) {
   extern __shared__ float smem[];
   constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
+  constexpr int NT = D == 256 ? 2 : 4, STEP = 16 * NT;  // 16-key groups and keys of a step
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
   const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
-  for (int unit_at = unit0; unit_at < unit1; unit_at++) {
-  const int32_t *u = a.units + 8 * (int64_t)unit_at;
-  const int row = u[0], q0 = u[1], f0 = u[2], rows = u[3], pos0 = u[4], kv0 = u[5], part = u[7];
-  // a row of the table that does not exist holds no keys
-  const int kv1 = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
-  if (rows <= 0 || rows > 16 * RT || q0 < 0 || f0 < 0 || q0 + (int64_t)(f0 + rows - 1) / G >= a.tokens) continue;
-  // queries
-  half8_v qf[RT][KS];
-  float mult[RT], m[RT], l[RT];
-  int hi[RT], lo[RT];
-  f32x4_v o[RT][DT];
-#pragma unroll
-  for (int r = 0; r < RT; r++) {
-    const int f = f0 + 16 * r + c;
-    const bool live = 16 * r + c < rows;
-    const int t = live ? f / G : 0, head = h * G + (live ? f - t * G : 0);
-    const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 16 * g;
-    u32x4_v w[D / 64][2];
-#pragma unroll
-    for (int s = 0; s < D / 64; s++)
-#pragma unroll
-      for (int k = 0; k < 2; k++) w[s][k] = live ? *(const u32x4_v *)(src + 64 * s + 8 * k) : (u32x4_v){0, 0, 0, 0};
-    float unit = 1.f;
-    if (a.dtype == SQ_BF16) {
-      float most = 0;
-#pragma unroll
-      for (int s = 0; s < D / 64; s++)
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][k][i])), fabsf(bf_hi(w[s][k][i]))));
-      most = reduce_max4(most);
-      float shift;
-      row_shift(most, &shift, &unit);
-#pragma unroll
-      for (int s = 0; s < D / 64; s++)
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            w[s][k][i] = f16_bits(bf_lo(w[s][k][i]) * shift) | f16_bits(bf_hi(w[s][k][i]) * shift) << 16;
-    }
-#pragma unroll
-    for (int s = 0; s < KS; s++) qf[r][s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
-    mult[r] = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-    hi[r] = live ? (a.causal ? pos0 + t + 1 : kv1) : kv1;
-    lo[r] = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
-#pragma unroll
-    for (int e = 0; e < DT; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
-  }
-  // tiles that every row sees whole need no mask: below the first row's last
-  // key and from the last row's first one on
-  const int all_hi = min(kv1, a.causal ? pos0 + f0 / G + 1 : kv1);
-  const int all_lo = a.window > 0 ? pos0 + (f0 + rows - 1) / G - a.window + 1 : 0;
-  const int P = a.c.page_tokens, per = P / kTile, log_per = 31 - __clz(per);
+  if (unit0 >= unit1) return;
+  const int P = a.c.page_tokens, per = P / STEP, log_per = 31 - __clz(per);
   const bool pow2 = (per & (per - 1)) == 0;
   const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
-  const int n = (kv1 - kv0 + kTile - 1) / kTile;
-  const int32_t *entries = a.table + (int64_t)row * a.width;
-  auto entry_of = [&](int tile) { return pow2 ? tile >> log_per : tile / per; };
-  int ids = 0;
-  Bytes<D / 16> vf[2][8];
-  u32x4_v kf[4][D / 64];
-  int page = 0;
-  const uint8_t *tile_at = nullptr;
-  // page and tile of step i; the lanes hold the pages of 64 steps
-  auto locate = [&](int i) {
-    const int tile = kv0 / kTile + i;
+  auto entry_of = [&](int step) { return pow2 ? step >> log_per : step / per; };
+
+  struct Unit {
+    int row, q0, f0, rows, pos0, kv0, kv1, part, n;
+  };
+  auto read_unit = [&](int i) {
+    const int32_t *u = a.units + 8 * (int64_t)i;
+    Unit x = {u[0], u[1], u[2], u[3], u[4], u[5], u[6], u[7], 0};
+    if (x.rows <= 0 || x.rows > 16 * RT || x.q0 < 0 || x.f0 < 0 || x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
+      x.rows = 0;
+    // a row of the table that does not exist holds no keys
+    const bool held = x.rows > 0 && x.row >= 0 && x.row < a.requests;
+    x.kv1 = held ? (int)min((int64_t)x.kv1, (int64_t)a.width * P) : 0;
+    x.n = max(0, (x.kv1 - x.kv0 + STEP - 1) / STEP);
+    return x;
+  };
+
+  Bytes<D / 16> vf[NT / 2][8];
+  u32x4_v kf[NT][D / 64];
+  int ids = 0, page = 0;
+  const uint8_t *page_at = nullptr, *at = nullptr;
+  // the lanes hold the pages of 64 of the wave's steps
+  auto fetch_ids = [&](const Unit &u, int i) {
+    const int mine = i + 4 * lane;
+    ids = mine < u.n ? a.table[(int64_t)u.row * a.width + entry_of(u.kv0 / STEP + mine)] : 0;
+  };
+  auto open = [&](const Unit &u, int i) {  // step i of a unit: its page, and its keys on their way
+    const int step = u.kv0 / STEP + i;
     const int p = __builtin_amdgcn_readlane(ids, (i >> 2) & 63);
     page = p > 0 && p < a.c.num_pages ? p : 0;
-    tile_at = a.c.data + page * a.c.page_bytes;
-    return tile_at + ((int64_t)(2 * h) * P + (tile - entry_of(tile) * per) * kTile) * D;
-  };
-  auto fetch_ids = [&](int i) {
-    const int mine = i + 4 * lane;
-    ids = mine < n ? entries[entry_of(kv0 / kTile + mine)] : 0;
-  };
-  auto load_keys = [&](const uint8_t *at) {
+    page_at = a.c.data + page * a.c.page_bytes;
+    at = page_at + ((int64_t)(2 * h) * P + (step - entry_of(step) * per) * STEP) * D;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int s = 0; s < D / 64; s++) kf[t][s] = *(const u32x4_v *)(at + (16 * t + c) * D + 64 * s + 16 * g);
   };
-  const uint8_t *at = nullptr;
-  if (wave < n) {
-    fetch_ids(wave);
-    at = locate(wave);
-    load_keys(at);
-  }
-  for (int i = wave; i < n; i += 4) {
-    const float2 peak = *(const float2 *)(tile_at + peaks_at);
-    const int first = kv0 + i * kTile;
-    const bool known = page != 0;
-    {
-      const uint8_t *vat = at + (int64_t)P * D;
-#pragma unroll
-      for (int s = 0; s < 2; s++)
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          vf[s][j] = *(const Bytes<D / 16> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
+  auto begin = [&](const Unit &u) {
+    if (wave < u.n) {
+      fetch_ids(u, wave);
+      open(u, wave);
     }
-    f32x4_v s[RT][4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-#pragma unroll
-      for (int r = 0; r < RT; r++) s[r][t] = (f32x4_v){0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < KS; k++) {
-        u32x4_v w;
-        const uint32_t w0 = kf[t][k / 2][2 * (k & 1)], w1 = kf[t][k / 2][2 * (k & 1) + 1];
-        w[0] = key2<FP8, 0>(w0), w[1] = key2<FP8, 1>(w0), w[2] = key2<FP8, 0>(w1), w[3] = key2<FP8, 1>(w1);
-        const half8_v kh = __builtin_bit_cast(half8_v, w);
-#pragma unroll
-        for (int r = 0; r < RT; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[r][k], s[r][t], 0, 0, 0);
-      }
-    }
-    if (i + 4 < n) {
-      if ((((i + 4) >> 2) & 63) == 0) fetch_ids(i + 4);
-      at = locate(i + 4);
-      load_keys(at);
-    }
-    const bool whole = known && first + kTile <= all_hi && first >= all_lo;
-    half8_v pf[RT][2];
-    float alpha[RT], sv[RT];
-    bool same = true;
+  };
+
+  Unit u = read_unit(unit0);
+  begin(u);
+  for (int unit_at = unit0; unit_at < unit1; unit_at++) {
+    const Unit following = read_unit(min(unit_at + 1, unit1 - 1));
+    // queries
+    half8_v qf[RT][KS];
+    float mult[RT], m[RT], l[RT];
+    int hi[RT], lo[RT];
+    f32x4_v o[RT][DT];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const float f = mult[r] * peak.x;
-      float best = -INFINITY;
+      const int f = u.f0 + 16 * r + c;
+      const bool live = 16 * r + c < u.rows;
+      const int t = live ? f / G : 0, head = h * G + (live ? f - t * G : 0);
+      const uint16_t *src = a.q + (int64_t)(u.q0 + t) * a.q_stride + head * a.q_head_stride + 16 * g;
+      u32x4_v w[D / 64][2];
 #pragma unroll
-      for (int t = 0; t < 4; t++)
+      for (int s = 0; s < D / 64; s++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          float x = s[r][t][k] * f;
-          if (!whole) {
-            const int j = first + 16 * t + 4 * g + k;
-            x = known && j < hi[r] && j >= lo[r] && j < kv1 ? x : -INFINITY;
-          }
-          s[r][t][k] = x;
-          best = fmaxf(best, x);
-        }
-      best = fmaxf(reduce_max4(best), m[r]);
-      const float base = best == -INFINITY ? 0.f : best;
-      alpha[r] = __builtin_amdgcn_exp2f(m[r] - base);
-      same = same && m[r] == best;
-      m[r] = best;
-      float sum = 0;
-      uint32_t w[2][4];
+        for (int k = 0; k < 2; k++) w[s][k] = live ? *(const u32x4_v *)(src + 64 * s + 8 * k) : (u32x4_v){0, 0, 0, 0};
+      float unit = 1.f;
+      if (a.dtype == SQ_BF16) {
+        float most = 0;
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        float p[4];
+        for (int s = 0; s < D / 64; s++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          p[k] = __builtin_amdgcn_exp2f(s[r][t][k] - base);
-          sum += p[k];
-        }
-        w[t >> 1][2 * (t & 1)] = f16_bits(p[0]) | f16_bits(p[1]) << 16;
-        w[t >> 1][2 * (t & 1) + 1] = f16_bits(p[2]) | f16_bits(p[3]) << 16;
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][k][i])), fabsf(bf_hi(w[s][k][i]))));
+        most = reduce_max4(most);
+        float shift;
+        row_shift(most, &shift, &unit);
+#pragma unroll
+        for (int s = 0; s < D / 64; s++)
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              w[s][k][i] = f16_bits(bf_lo(w[s][k][i]) * shift) | f16_bits(bf_hi(w[s][k][i]) * shift) << 16;
       }
-      l[r] = fmaf(l[r], alpha[r], sum);
-      pf[r][0] = __builtin_bit_cast(half8_v, *(u32x4_v *)w[0]);
-      pf[r][1] = __builtin_bit_cast(half8_v, *(u32x4_v *)w[1]);
-      // a row that sees none of the tile takes nothing from it, whatever its peak
-      const bool some = whole || (known && first < min(hi[r], kv1) && first + kTile > lo[r]);
-      sv[r] = some ? peak.y * kValueUnit<FP8> : 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[r][s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
+      mult[r] = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+      hi[r] = live && a.causal ? min(u.kv1, u.pos0 + t + 1) : u.kv1;
+      lo[r] = live && a.window > 0 ? u.pos0 + t - a.window + 1 : 0;
+#pragma unroll
+      for (int e = 0; e < DT; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
     }
-    const bool keep = __all(same);
-    auto value = [&](auto E) {
-      constexpr int e = decltype(E)::value;
-      half8_v v[2];
+    // steps that every row sees whole need no mask: below the first row's last
+    // key and from the last row's first one on
+    const int all_hi = min(u.kv1, a.causal ? u.pos0 + u.f0 / G + 1 : u.kv1);
+    const int all_lo = a.window > 0 ? u.pos0 + (u.f0 + u.rows - 1) / G - a.window + 1 : 0;
+    for (int i = wave; i < u.n; i += 4) {
+      const float2 peak = *(const float2 *)(page_at + peaks_at);
+      const int first = u.kv0 + i * STEP;
+      const bool known = page != 0;
+      {
+        const uint8_t *vat = at + (int64_t)P * D;
 #pragma unroll
-      for (int s2 = 0; s2 < 2; s2++) {
-        uint32_t w[8];
+        for (int s = 0; s < NT / 2; s++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = vf[s2][j].w[e / 4];
-        v[s2] = value8<FP8, e & 3>(w);
+          for (int j = 0; j < 8; j++)
+            vf[s][j] = *(const Bytes<D / 16> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
       }
+      f32x4_v s[RT][NT];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int r = 0; r < RT; r++) s[r][t] = (f32x4_v){0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          u32x4_v w;
+          const uint32_t w0 = kf[t][k / 2][2 * (k & 1)], w1 = kf[t][k / 2][2 * (k & 1) + 1];
+          w[0] = key2<FP8, 0>(w0), w[1] = key2<FP8, 1>(w0), w[2] = key2<FP8, 0>(w1), w[3] = key2<FP8, 1>(w1);
+          const half8_v kh = __builtin_bit_cast(half8_v, w);
+#pragma unroll
+          for (int r = 0; r < RT; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[r][k], s[r][t], 0, 0, 0);
+        }
+      }
+      if (i + 4 < u.n) {
+        if ((((i + 4) >> 2) & 63) == 0) fetch_ids(u, i + 4);
+        open(u, i + 4);
+      }
+      const bool whole = known && first + STEP <= all_hi && first >= all_lo;
+      half8_v pf[RT][NT / 2];
+      float alpha[RT], sv[RT];
+      bool same = true;
 #pragma unroll
       for (int r = 0; r < RT; r++) {
-        f32x4_v x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], pf[r][0], (f32x4_v){0, 0, 0, 0}, 0, 0, 0);
-        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], pf[r][1], x, 0, 0, 0);
+        const float f = mult[r] * peak.x;
+        float best = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float was = keep ? o[r][e][k] : o[r][e][k] * alpha[r];
-          o[r][e][k] = fmaf(x[k], sv[r], was);
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            float x = s[r][t][k] * f;
+            if (!whole) {
+              const int j = first + 16 * t + 4 * g + k;
+              x = known && j < hi[r] && j >= lo[r] ? x : -INFINITY;
+            }
+            s[r][t][k] = x;
+            best = fmaxf(best, x);
+          }
+        best = fmaxf(reduce_max4(best), m[r]);
+        const float base = best == -INFINITY ? 0.f : best;
+        alpha[r] = __builtin_amdgcn_exp2f(m[r] - base);
+        same = same && m[r] == best;
+        m[r] = best;
+        float sum = 0;
+        u32x4_v w[NT / 2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          float p[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            p[k] = __builtin_amdgcn_exp2f(s[r][t][k] - base);
+            sum += p[k];
+          }
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+            w[t >> 1][2 * (t & 1) + k] = half2_bits(__builtin_convertvector((f32x2_v){p[2 * k], p[2 * k + 1]}, half2_v));
+        }
+        l[r] = fmaf(l[r], alpha[r], sum);
+#pragma unroll
+        for (int t = 0; t < NT / 2; t++) pf[r][t] = __builtin_bit_cast(half8_v, w[t]);
+        // a row that sees none of the step takes nothing from it, whatever its peak
+        const bool some = whole || (known && first < hi[r] && first + STEP > lo[r]);
+        sv[r] = some ? peak.y * kValueUnit<FP8> : 0.f;
+      }
+      const bool keep = __all(same);
+      auto value = [&](auto E) {
+        constexpr int e = decltype(E)::value;
+        half8_v v[NT / 2];
+#pragma unroll
+        for (int s2 = 0; s2 < NT / 2; s2++) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) w[j] = vf[s2][j].w[e / 4];
+          v[s2] = value8<FP8, e & 3>(w);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          f32x4_v x = {0, 0, 0, 0};
+#pragma unroll
+          for (int s2 = 0; s2 < NT / 2; s2++) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s2], pf[r][s2], x, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float was = keep ? o[r][e][k] : o[r][e][k] * alpha[r];
+            o[r][e][k] = fmaf(x[k], sv[r], was);
+          }
+        }
+      };
+      each(value, std::make_integer_sequence<int, DT>{});
+    }
+    if (unit_at + 1 < unit1) begin(following);
+    // the four waves' shares of each row, joined through LDS
+    float *so = smem;                 // [4][16][LDO]
+    float *sm = smem + 4 * 16 * LDO;  // [4][16] maxima, then sums
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      const float sum = reduce_sum4(l[r]);
+      __syncthreads();  // (after the last unit's, or the last rows', readers)
+      if (g == 0) {
+        sm[16 * wave + c] = m[r];
+        sm[64 + 16 * wave + c] = sum;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
+#pragma unroll
+        for (int e = 0; e < DT; e += 4)
+          *(f32x4_v *)(dst + e) = (f32x4_v){o[r][e][k], o[r][e + 1][k], o[r][e + 2][k], o[r][e + 3][k]};
+      }
+      __syncthreads();
+      for (int i = tid; i < 16 * (D / 4); i += 256) {
+        const int j = i / (D / 4), d = 4 * (i % (D / 4));
+        if (16 * r + j >= u.rows) break;
+        float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
+        const float base = mm == -INFINITY ? 0.f : mm;
+        float all = 0;
+        f32x4_v x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
+          all = fmaf(sm[64 + 16 * w + j], f, all);
+          x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
+        }
+        const int f = u.f0 + 16 * r + j;
+        if (u.part < 0) {
+          x *= all == 0.f ? 0.f : 1.f / all;
+          const int t = f / G, head = h * G + f - t * G;
+          store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
+        } else {
+          const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * (16 * RT) + 16 * r + j;
+          *(f32x4_v *)(a.ws + slot * D + d) = x;
+          if (d == 0) {
+            float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * (16 * RT) * D + 2 * slot;
+            ml[0] = mm;
+            ml[1] = all;
+          }
         }
       }
-    };
-    each(value, std::make_integer_sequence<int, DT>{});
-  }
-  // the four waves' shares of each row, joined through LDS
-  float *so = smem;                  // [4][16][LDO]
-  float *sm = smem + 4 * 16 * LDO;   // [4][16] maxima, then sums
-#pragma unroll
-  for (int r = 0; r < RT; r++) {
-    const float sum = reduce_sum4(l[r]);
-    if (r) __syncthreads();
-    if (g == 0) {
-      sm[16 * wave + c] = m[r];
-      sm[64 + 16 * wave + c] = sum;
     }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
-#pragma unroll
-      for (int e = 0; e < DT; e += 4)
-        *(f32x4_v *)(dst + e) = (f32x4_v){o[r][e][k], o[r][e + 1][k], o[r][e + 2][k], o[r][e + 3][k]};
-    }
-    __syncthreads();
-    for (int i = tid; i < 16 * (D / 4); i += 256) {
-      const int j = i / (D / 4), d = 4 * (i % (D / 4));
-      if (16 * r + j >= rows) continue;
-      float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
-      const float base = mm == -INFINITY ? 0.f : mm;
-      float sum2 = 0;
-      f32x4_v x = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
-        sum2 = fmaf(sm[64 + 16 * w + j], f, sum2);
-        x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
-      }
-      const int f = f0 + 16 * r + j;
-      if (part < 0) {
-        const float inv = sum2 == 0.f ? 0.f : 1.f / sum2;
-        x *= inv;
-        const int t = f / G, head = h * G + f - t * G;
-        uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + d;
-        store_row<4>(dst, a.dtype == SQ_BF16, (const float *)&x);
-      } else {
-        const int64_t slot = ((int64_t)part * a.kv_heads + h) * (16 * RT) + 16 * r + j;
-        *(f32x4_v *)(a.ws + slot * D + d) = x;
-        if (d == 0) {
-          float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * (16 * RT) * D + 2 * slot;
-          ml[0] = mm;
-          ml[1] = sum2;
-        }
-      }
-    }
-  }
-  __syncthreads();  // before the next unit's shares
+    u = following;
   }
 }
 

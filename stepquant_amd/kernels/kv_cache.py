@@ -205,7 +205,7 @@ class BlockTables:
             N.check(rc, "kv plan")
         return p
 
-    min_tiles = 8  # least 64-key tiles of a workgroup where a set of rows is cut
+    min_tiles = 4  # least 64-key tiles of a workgroup where a set of rows is cut
     cut_tiles = {16: 4, 32: 4, 256: 16}  # what its partial results cost, in tiles
 
     def _shape(self, q_heads, kv_heads, tokens, batch, max_new):
