@@ -431,7 +431,7 @@ typedef struct sq_kv_tables {
  * s = max(1, slots / kv_heads):
  *   max_workers  >= max(sets, s), and starts holds max_workers + 1
  *   max_units    >= sets + s
- *   max_merges   >= s
+ *   max_merges   >= min(sets, s)
  *   max_partials >= 2 * s
  */
 typedef struct sq_kv_schedule {

@@ -701,6 +701,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   constexpr int NT = D == 256 ? 2 : 4, STEP = 16 * NT;  // 16-key groups and keys of a step
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
+  const int at_row = 16 * RT * blockIdx.y;  // of the unit's rows
   const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
   if (unit0 >= unit1) return;
   const int P = a.c.page_tokens, per = P / STEP, log_per = 31 - __clz(per);
@@ -713,8 +714,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   };
   auto read_unit = [&](int i) {
     const int32_t *u = a.units + 8 * (int64_t)i;
-    Unit x = {u[0], u[1], u[2], u[3], u[4], u[5], u[6], u[7], 0};
-    if (x.rows <= 0 || x.rows > 16 * RT || x.q0 < 0 || x.f0 < 0 || x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
+    Unit x = {u[0], u[1], u[2] + at_row, min(u[3] - at_row, 16 * RT), u[4], u[5], u[6], u[7], 0};
+    if (x.rows <= 0 || u[3] > a.unit_rows || x.q0 < 0 || x.f0 < 0 || x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
       x.rows = 0;
     // a row of the table that does not exist holds no keys
     const bool held = x.rows > 0 && x.row >= 0 && x.row < a.requests;
@@ -946,10 +947,10 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
           const int t = f / G, head = h * G + f - t * G;
           store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
         } else {
-          const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * (16 * RT) + 16 * r + j;
+          const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * a.unit_rows + at_row + 16 * r + j;
           *(f32x4_v *)(a.ws + slot * D + d) = x;
           if (d == 0) {
-            float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * (16 * RT) * D + 2 * slot;
+            float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
             ml[0] = mm;
             ml[1] = all;
           }
@@ -1013,7 +1014,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
     const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
     half8_v qf[KS];
     float mult;
-    {
+    auto read_queries = [&]() {
       const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 8 * hl;
       u32x4_v w[KS];
 #pragma unroll
@@ -1036,7 +1037,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
 #pragma unroll
       for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s] ^ flip);
       mult = fabsf(a.scale) * 1.4426950408889634f * unit * kKeyUnit<FP8>;
-    }
+    };
     // what the row sees, and what every row of the wave sees whole
     const int hi = live && a.causal ? min(kv1, pos0 + t + 1) : kv1;
     const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
@@ -1051,8 +1052,20 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
     float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
 
     // The tiles in order; past the last one the last again, so that loads ahead
-    // need no branch.  A page's number is loaded a tile before it is used.
-    int block = tile0 / per, sub = tile0 - block * per, left = n, id = n > 0 ? entries[block] : 0;
+    // need no branch.  A page's number is loaded two tiles before it is used.
+    const int block = tile0 / per;
+    int sub = tile0 - block * per, left = n, id = 0, id2 = 0, ahead = block, ahead_sub = sub, ahead_left = n;
+    auto next_id = [&]() {
+      ahead_left--;
+      const bool more = ahead_left > 0, turned = ahead_sub + 1 == per;
+      ahead_sub = more ? turned ? 0 : ahead_sub + 1 : ahead_sub;
+      ahead = __builtin_amdgcn_readfirstlane(ahead + (more && turned));
+      return entries[ahead];
+    };
+    if (n > 0) {
+      id = entries[block];
+      id2 = next_id();
+    }
     bool known;
     const uint8_t *base;  // of the page of the tile
     auto next_tile = [&]() {
@@ -1063,13 +1076,13 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       left--;
       const bool more = left > 0, turned = sub + 1 == per;
       sub = more ? turned ? 0 : sub + 1 : sub;
-      block = __builtin_amdgcn_readfirstlane(block + (more && turned));
-      id = entries[block];
+      id = id2;
+      id2 = next_id();
       return at;
     };
-    u32x4_v ck[KN];
+    u32x4_v ck[KN], ck0[KN];
     Bytes<D / 32> cv[4];
-    auto load_keys = [&](const uint8_t *at) {
+    auto load_keys = [&](u32x4_v *ck, const uint8_t *at) {
       if (KS >= 8 || wave < KS)
 #pragma unroll
         for (int k = 0; k < KN; k++) ck[k] = *(const u32x4_v *)(at + 16 * (tid + 512 * k));
@@ -1082,7 +1095,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
     // keys: [32 tokens][16 dims][half of them][token] of eight dims; steps lie
     // 65 groups apart, so that a wave's writes, 8 of a token's, fall on
     // different banks
-    auto put_keys = [&](uint4 *dst) {
+    auto put_keys = [&](const u32x4_v *ck, uint4 *dst) {
       if (KS >= 8 || wave < KS)
 #pragma unroll
         for (int k = 0; k < KN; k++) {
@@ -1109,9 +1122,9 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       each(one, std::make_integer_sequence<int, DT>{});
     };
     // Outputs with one tile's values (with VALUES), then scores with another
-    // one's keys; the operands are read DEEP products ahead.
+    // one's keys; the operands are read DEEP products ahead (8; 4 of 256 dims, where registers end).
     auto products = [&](auto VALUES, const uint4 *values, const uint4 *keys) {
-      constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + 2 * KS, DEEP = 8;
+      constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + 2 * KS, DEEP = D == 256 ? 4 : 8;
 #pragma unroll
       for (int tt = 0; tt < 2; tt++)
 #pragma unroll
@@ -1203,28 +1216,38 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       l = fmaf(sum, __builtin_amdgcn_exp2f(-size), l);
     };
 
+    float4 peak, peak0;
+    const uint8_t *at = nullptr, *keys = nullptr;
+    auto load_peak = [&]() {
+      const float2 x = *(const float2 *)(base + peaks_at);
+      peak = make_float4(x.x, x.y, known ? 1.f : 0.f, 0.f);
+    };
+    // the first tiles' loads go out before the queries', whose conversion they run under
+    if (n > 0) {
+      at = next_tile();
+      load_keys(ck0, at);
+      load_peak();
+      peak0 = peak;
+      load_values(at);
+      keys = next_tile();
+      load_keys(ck, keys);
+      load_peak();
+    }
+    read_queries();
     if (n > 0) {
       // Step j of the loop needs values j and keys j + 1.  The early waves put
       // their share of them there in step j, the late ones, whose step j begins
       // half a step later, in step j - 1.
-      const uint8_t *at = next_tile();
-      // (values and keys that a thread holds on their way to LDS; with the keys
-      // their tile's peaks)
-      float4 peak;
+      put_keys(ck0, kb);
+      if (tid == 0) peaks[0] = peak0;
       auto load = [&](const uint8_t *values, const uint8_t *keys) {
-        if (values) load_values(values);
-        load_keys(keys);
-        const float2 x = *(const float2 *)(base + peaks_at);
-        peak = make_float4(x.x, x.y, known ? 1.f : 0.f, 0.f);
+        load_values(values);
+        load_keys(ck, keys);
+        load_peak();
       };
-      load(nullptr, at);
-      put_keys(kb);
-      if (tid == 0) peaks[0] = peak;
-      const uint8_t *keys = next_tile();
-      load(at, keys);
       if (late) {
         put_values(vb);
-        put_keys(kb + KB);
+        put_keys(ck, kb + KB);
         at = keys;
         keys = next_tile();
         load(at, keys);
@@ -1237,7 +1260,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         softmax(i);
         // (past the last tile: into buffers that nothing reads)
         put_values(vb + ((i + late) & 1) * VB);
-        put_keys(kb + ((i + late + 1) & 1) * KB);
+        put_keys(ck, kb + ((i + late + 1) & 1) * KB);
         if (tid == 0) peaks[(i + 1) & 1] = peak;
         at = keys;
         keys = next_tile();
@@ -1252,28 +1275,57 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       __syncthreads();  // the next turn writes where the last products read
     }
     l = reduce_sum2(l);
-    if (!live) continue;
     const float unit = ref * kValueUnit<FP8>;
     if (part < 0) {
+      // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
+      constexpr int OD = 32 * OT, OW = OD * 2 + 8;  // a wave's dims of a row, and the bytes from row to row
       const float f = l == 0.f ? 0.f : unit / l;
-      uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + e0;
+      uint8_t *rows_at = (uint8_t *)tiles + wave * (32 * OW);
 #pragma unroll
       for (int k = 0; k < 16; k++) {
         float x[OT];
 #pragma unroll
         for (int e = 0; e < OT; e++) x[e] = o[e][k] * f;
-        store_row<OT>(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT, a.dtype == SQ_BF16, x);
+        store_row<OT>((uint16_t *)(rows_at + c * OW) + (8 * (k >> 2) + 4 * hl + (k & 3)) * OT, a.dtype == SQ_BF16, x);
       }
+      __builtin_amdgcn_wave_barrier();
+      if constexpr (D == 256) {
+        // the wave's dims are every other group of four: 8 bytes a lane
+        constexpr int LANES = OD / 4;
+#pragma unroll
+        for (int i = 0; i < 32 * LANES / 64; i++) {
+          const int r = (64 * i + lane) / LANES, d = (64 * i + lane) % LANES, f = f0 + first_row + r;
+          if (first_row + r < rows)
+            *(uint2 *)(a.out + ((int64_t)(q0 + f / G) * a.q_heads + h * G + f % G) * D + 8 * d + e0) =
+                *(const uint2 *)(rows_at + r * OW + 8 * d);
+        }
+      } else {
+        constexpr int LANES = OD / 8;
+#pragma unroll
+        for (int i = 0; i < 32 * LANES / 64; i++) {
+          const int r = (64 * i + lane) / LANES, d = (64 * i + lane) % LANES, f = f0 + first_row + r;
+          const uint2 *src = (const uint2 *)(rows_at + r * OW + 16 * d);  // (rows lie 8 bytes off a multiple of 16)
+          const uint2 x0 = src[0], x1 = src[1];
+          if (first_row + r < rows)
+            *(uint4 *)(a.out + ((int64_t)(q0 + f / G) * a.q_heads + h * G + f % G) * D + 8 * d) =
+                make_uint4(x0.x, x0.y, x1.x, x1.y);
+        }
+      }
+      __syncthreads();  // before the next unit's tiles
     } else {
-      const int64_t slot = ((int64_t)part * a.kv_heads + h) * a.unit_rows + turn + mine;
-      float *dst = a.ws + slot * D + e0;
+      // as the registers hold them: a wave writes 64 OT floats in a row
+      typedef float vec __attribute__((ext_vector_type(OT)));
+      const int64_t slot = (int64_t)part * a.kv_heads + h;
+      float *dst = a.ws + ((slot * (D == 256 ? 16 : 8) + turn / WR * 8 + wave) * (16 * 64) + lane) * OT;
 #pragma unroll
-      for (int k = 0; k < 16; k++)
+      for (int k = 0; k < 16; k++) {
+        vec x;
 #pragma unroll
-        for (int e = 0; e < OT; e += 2)
-          *(float2 *)(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT + e) = make_float2(o[e][k] * unit, o[e + 1][k] * unit);
-      if (hl == 0 && e0 == 0) {
-        float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
+        for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit;
+        *(vec *)(dst + k * 64 * OT) = x;
+      }
+      if (live && hl == 0 && e0 == 0) {
+        float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * (slot * a.unit_rows + turn + mine);
         ml[0] = m;
         ml[1] = l;
       }
@@ -1282,52 +1334,120 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   }
 }
 
-// Joins the parts of query rows: one workgroup per (merge, head) and row, or
-// per 16th row.
+// Joins the parts of query rows of units of up to 32: one workgroup per
+// (merge, head) and row; LANES lanes read a part, GROUPS parts at a time.
 template <int D>
-__global__ __launch_bounds__(256) void kv_merge_kernel(AttendDev a) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+__global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
+  constexpr int LANES = D / 4, GROUPS = 512 / LANES, AHEAD = 4;
   __shared__ f32x4_v part_o[GROUPS][LANES];
   __shared__ float part_l[GROUPS], part_m[GROUPS];
-  const int tid = threadIdx.x, h = blockIdx.x % a.kv_heads;
+  const int tid = threadIdx.x, h = blockIdx.x % a.kv_heads, j = blockIdx.y;
   const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.kv_heads);
   const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
+  if (j >= rows) return;
   const int lane = tid % LANES, grp = tid / LANES;
   const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D;
-  for (int j = blockIdx.y; j < rows; j += gridDim.y) {
-    const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * a.unit_rows + j, step = (int64_t)a.kv_heads * a.unit_rows;
-    // every group of lanes joins its parts as they come, then the groups
-    f32x4_v x = {0, 0, 0, 0};
-    float sum = 0, mm = -INFINITY;
-    for (int i = grp; i < n; i += GROUPS) {
-      const int64_t s = slot0 + i * step;
-      const float2 part = *(const float2 *)(ml + 2 * s);
-      const float high = fmaxf(mm, part.x), base = high == -INFINITY ? 0.f : high;
-      const float was = __builtin_amdgcn_exp2f(mm - base), w = __builtin_amdgcn_exp2f(part.x - base);
+  const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * a.unit_rows + j, step = (int64_t)a.kv_heads * a.unit_rows;
+  // every group of lanes joins its parts as they come, then the groups
+  f32x4_v x = {0, 0, 0, 0};
+  float sum = 0, mm = -INFINITY;
+#pragma unroll 1
+  for (int i0 = grp; i0 < n; i0 += AHEAD * GROUPS) {
+    float2 stat[AHEAD];
+    f32x4_v y[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {  // (past the end the last part again, with no weight)
+      const int64_t s = slot0 + min(i0 + k * GROUPS, n - 1) * step;
+      stat[k] = *(const float2 *)(ml + 2 * s);
+      y[k] = *(const f32x4_v *)(a.ws + s * D + 4 * lane);
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+      if (i0 + k * GROUPS >= n) break;
+      const float high = fmaxf(mm, stat[k].x), base = high == -INFINITY ? 0.f : high;
+      const float was = __builtin_amdgcn_exp2f(mm - base), w = __builtin_amdgcn_exp2f(stat[k].x - base);
       mm = high;
-      sum = fmaf(sum, was, part.y * w);
-      x = x * was + *(const f32x4_v *)(a.ws + s * D + 4 * lane) * w;
+      sum = fmaf(sum, was, stat[k].y * w);
+      x = x * was + y[k] * w;
     }
-    part_o[grp][lane] = x;
-    if (lane == 0) part_l[grp] = sum, part_m[grp] = mm;
-    __syncthreads();
-    if (grp == 0) {
+  }
+  part_o[grp][lane] = x;
+  if (lane == 0) part_l[grp] = sum, part_m[grp] = mm;
+  __syncthreads();
+  if (grp) return;
+  const int groups = min(GROUPS, n);
+#pragma unroll 1
+  for (int i = 1; i < groups; i++) mm = fmaxf(mm, part_m[i]);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  sum = 0;
+  x = (f32x4_v){0, 0, 0, 0};
+#pragma unroll 1
+  for (int i = 0; i < groups; i++) {
+    const float w = __builtin_amdgcn_exp2f(part_m[i] - base);
+    x += part_o[i][lane] * w;
+    sum = fmaf(part_l[i], w, sum);
+  }
+  x *= sum == 0.f ? 0.f : 1.f / sum;
+  const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
+  store_row<4>(a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane, a.dtype == SQ_BF16, (const float *)&x);
+}
+
+// Joins the parts of units of up to 256 rows, in the order in which a wave's
+// registers of kv_attend_rows_kernel went out: one workgroup per (merge, head)
+// and wave; its two halves take the parts in turn, two at a time.
+template <int D>
+__global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
+  constexpr int DT = D / 32, OT = D == 256 ? DT / 2 : DT, BLOCKS = D == 256 ? 16 : 8;
+  typedef float vec __attribute__((ext_vector_type(OT)));
+  __shared__ vec part_o[4][256];
+  __shared__ float2 part_s[256];
+  const int h = blockIdx.x % a.kv_heads, wave = blockIdx.y & 7, turn = blockIdx.y >> 3;
+  const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.kv_heads);
+  const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
+  const int tid = threadIdx.x & 255, half = threadIdx.x >> 8, lane = tid & 63, c = lane & 31, hl = lane >> 5, k0 = tid >> 6;
+  const int e0 = D == 256 ? (wave >> 2) * OT : 0;
+  const int first = D == 256 ? 128 * turn + 32 * (wave & 3) : 32 * wave, j = first + c;
+  if (first >= rows) return;
+  const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * (int64_t)min(j, rows - 1);
+  vec x[4];
 #pragma unroll
-      for (int i = 0; i < GROUPS; i++) mm = fmaxf(mm, part_m[i]);
-      const float base = mm == -INFINITY ? 0.f : mm;
-      sum = 0;
-      x = (f32x4_v){0, 0, 0, 0};
+  for (int i = 0; i < 4; i++) x[i] = (vec)(0.f);
+  float sum = 0, mm = -INFINITY;
+#pragma unroll 2
+  for (int i = half; i < n; i += 2) {
+    const int64_t slot = (int64_t)(p0 + i) * a.kv_heads + h;
+    const float2 stat = *(const float2 *)(ml + 2 * slot * a.unit_rows);
+    vec y[4];
 #pragma unroll
-      for (int i = 0; i < GROUPS; i++) {
-        const float w = __builtin_amdgcn_exp2f(part_m[i] - base);
-        x += part_o[i][lane] * w;
-        sum = fmaf(part_l[i], w, sum);
-      }
-      x *= sum == 0.f ? 0.f : 1.f / sum;
-      const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
-      store_row<4>(a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane, a.dtype == SQ_BF16, (const float *)&x);
-    }
-    __syncthreads();
+    for (int k = 0; k < 4; k++)
+      y[k] = *(const vec *)(a.ws + (((slot * BLOCKS + blockIdx.y) * 16 + k0 + 4 * k) * 64 + lane) * OT);
+    const float high = fmaxf(mm, stat.x), base = high == -INFINITY ? 0.f : high;
+    const float was = __builtin_amdgcn_exp2f(mm - base), w = __builtin_amdgcn_exp2f(stat.x - base);
+    mm = high;
+    sum = fmaf(sum, was, stat.y * w);
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[k] = x[k] * was + y[k] * w;
+  }
+  if (half) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) part_o[k][tid] = x[k];
+    part_s[tid] = make_float2(mm, sum);
+  }
+  __syncthreads();
+  if (half || j >= rows) return;
+  const float2 other = part_s[tid];
+  const float high = fmaxf(mm, other.x), base = high == -INFINITY ? 0.f : high;
+  float mine = __builtin_amdgcn_exp2f(mm - base), theirs = __builtin_amdgcn_exp2f(other.x - base);
+  sum = fmaf(sum, mine, other.y * theirs);
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  mine *= f, theirs *= f;
+  const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
+  uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + e0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int k = k0 + 4 * i;
+    x[i] = x[i] * mine + part_o[i][tid] * theirs;
+    store_row<OT>(dst + (8 * (k >> 2) + 4 * hl + (k & 3)) * DT, a.dtype == SQ_BF16, (const float *)&x[i]);
   }
 }
 
@@ -1372,7 +1492,7 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
   if (tokens * G > 0x3fffffff) return fail(SQ_EINVAL, "kv schedule: tokens * heads of a group too large");
   const int64_t sets = (tokens * G + s->rows - 1) / s->rows + batch + 1;
   const int64_t slots = s->slots / s->kv_heads > 1 ? s->slots / s->kv_heads : 1;
-  if (s->max_workers < (sets > slots ? sets : slots) || s->max_units < sets + slots || s->max_merges < slots ||
+  if (s->max_workers < (sets > slots ? sets : slots) || s->max_units < sets + slots || s->max_merges < (sets < slots ? sets : slots) ||
       s->max_partials < 2 * slots || s->max_units >= 1 << 24)
     return fail(SQ_EINVAL, "kv schedule: room for workers, units, merges or partials");
   if ((int64_t)s->max_workers * s->kv_heads > 0x7fffffff || (int64_t)s->max_merges * s->kv_heads > 0x7fffffff)
@@ -1425,21 +1545,27 @@ int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 template <int D, bool FP8>
 int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
-  auto go = [&](auto kernel, int id, int threads, size_t lds) {
+  auto go = [&](auto kernel, int id, int threads, size_t lds, int turns = 1) {
     const int rc = dynamic_lds((const void *)kernel, 2 * id + FP8, lds, "kv attend: LDS attribute");
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_workers * s.kv_heads)), dim3(threads), lds, st, d);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_workers * s.kv_heads), (unsigned)turns), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
-  static_assert(D <= 256, "ids of kernels with more than 64 KiB: one dim has them");
-  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float), staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1);
+  static_assert(D <= 256, "ids of kernels with more than 64 KiB");
+  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float);
+  // tiles and peaks; the outputs' way out
+  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1), rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
+  constexpr size_t many = staged > rows_out ? staged : rows_out;
   int rc;
   if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
+  // 32 rows of 256 dims do not fit a wave's registers twice on a SIMD: they go to two workgroups
+  else if constexpr (D == 256) rc = s.rows == 32 ? go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined, 2) : go(kv_attend_rows_kernel<D, FP8>, 3, 512, many);
   else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
-  else rc = go(kv_attend_rows_kernel<D, FP8>, 3, 512, staged);
+  else rc = go(kv_attend_rows_kernel<D, FP8>, 4, 512, many);
   if (rc) return rc;
-  const unsigned rows = s.merge_rows < 16 ? s.merge_rows : 16;
-  hipLaunchKernelGGL(kv_merge_kernel<D>, dim3((unsigned)(s.max_merges * s.kv_heads), rows), dim3(256), 0, st, d);
+  const unsigned merges = s.max_merges * s.kv_heads;
+  if (s.rows == 256) hipLaunchKernelGGL(kv_merge_rows_kernel<D>, dim3(merges, D == 256 ? 16 : 8), dim3(512), 0, st, d);
+  else hipLaunchKernelGGL(kv_merge_kernel<D>, dim3(merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
   return sq_internal_launched("kv_merge_kernel");
 }
 

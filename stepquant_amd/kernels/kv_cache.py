@@ -174,9 +174,9 @@ class BlockTables:
         sizes = [batch + 1, tokens, batch, flags, most, most, 2 * most]
         if windows:
             sets, cuts, q_heads, kv_heads, unit_rows, slots, merge_rows = shape
-            workers = max(sets, cuts)
+            workers, joins = max(sets, cuts), min(sets, cuts)
             sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
-            sizes += [8 * (sets + 2 * cuts) + (workers + 8) // 8 * 8] * len(windows)
+            sizes += [8 * (sets + cuts + joins) + (workers + 8) // 8 * 8] * len(windows)
         p._sizes = sizes
         p._ints = ints = torch.empty(sum(sizes), dtype=torch.int32, device=self.device)
         p._longs = longs = torch.empty(2 + tokens, dtype=torch.int64, device=self.device)
@@ -189,8 +189,8 @@ class BlockTables:
         for w, units in zip(windows, at[7:]):
             s = _Schedule()
             merges = units + 32 * (sets + cuts)
-            s.packed = N.KV_SCHEDULE.pack(units, merges, merges + 32 * cuts, sets + cuts, cuts, workers, 2 * cuts, q_heads,
-                                          kv_heads, unit_rows, bool(causal), int(w), slots, self.min_tiles,
+            s.packed = N.KV_SCHEDULE.pack(units, merges, merges + 32 * joins, sets + cuts, joins, workers, 2 * cuts, q_heads,
+                                          kv_heads, unit_rows, bool(causal), int(w), slots, self.min_tiles[unit_rows],
                                           self.cut_tiles[unit_rows], merge_rows, 0)
             s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, 2 * cuts * kv_heads * unit_rows
             p.schedules[int(w)] = s
@@ -205,7 +205,7 @@ class BlockTables:
             N.check(rc, "kv plan")
         return p
 
-    min_tiles = 4  # least 64-key tiles of a workgroup where a set of rows is cut
+    min_tiles = {16: 4, 32: 4, 256: 4}  # least 64-key tiles of a workgroup where a set of rows is cut
     cut_tiles = {16: 4, 32: 4, 256: 16}  # what its partial results cost, in tiles
 
     def _shape(self, q_heads, kv_heads, tokens, batch, max_new):

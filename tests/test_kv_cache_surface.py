@@ -76,7 +76,7 @@ def test_caches_are_checked_before_any_launch(cache, code):
     ({}, dict(batch=4097), {}), ({}, dict(tokens=-1), {}), ({}, dict(max_tiles=3), {}), ({}, dict(n_schedules=5), {}),
     ({}, dict(max_count=-1), {}), ({}, {}, dict(units=None)), ({}, {}, dict(q_heads=7)), ({}, {}, dict(rows=48)),
     ({}, {}, dict(window=3, causal=0)), ({}, {}, dict(window=-1)), ({}, {}, dict(slots=0)), ({}, {}, dict(max_units=262)),
-    ({}, {}, dict(max_merges=255)), ({}, {}, dict(max_partials=511)), ({}, {}, dict(max_workers=255)),
+    ({}, {}, dict(max_merges=6)), ({}, {}, dict(max_partials=511)), ({}, {}, dict(max_workers=255)),
     ({}, {}, dict(slots=4097)), ({}, {}, dict(starts=None)), ({}, {}, dict(cut_tiles=-1)), ({}, {}, dict(min_tiles=0)),
     ({}, {}, dict(merge_rows=15)), ({}, {}, dict(merge_rows=17))])
 def test_plans_are_checked_before_any_launch(tables, plan, schedule):
