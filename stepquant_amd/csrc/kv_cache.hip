@@ -58,7 +58,6 @@ __device__ __forceinline__ int64_t load_index(const void *p, int dtype, int64_t 
 // last workgroups lay out the attention layers' work.
 
 constexpr int kPlanThreads = 512;
-constexpr int kPlanItems = SQ_KV_MAX_REQUESTS / kPlanThreads;
 constexpr int kMaxSlots = 4096;
 constexpr int kPlanShare = 1024;  // tokens (and page entries) of one workgroup
 
@@ -68,26 +67,41 @@ struct PlanDev {
   int share_blocks;
 };
 
-// Inclusive prefix sums over the workgroup, and the total.
-template <int NT>
-__device__ int64_t block_scan(int64_t x, int64_t *total, int64_t *waves) {
+// Sums of the threads before, and of all.  They stop at 2^31 - 1, which no size
+// that fits reaches.  Every use calls one copy of the code.
+constexpr uint32_t kMost = 0x7fffffffu;
+
+struct Scan {
+  uint32_t before, all;
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {  // 0 where no lane is named
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+
+__device__ __attribute__((noinline)) Scan block_scan(uint32_t x) {
+  __shared__ uint32_t waves[kPlanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
+  // 16 lanes by shifts, then the ends of the rows of 16 over the rows behind
+  uint32_t y = min(x + dpp<0x111, 0xf>(x), kMost);
+  y = min(y + dpp<0x112, 0xf>(y), kMost);
+  y = min(y + dpp<0x114, 0xf>(y), kMost);
+  y = min(y + dpp<0x118, 0xf>(y), kMost);
+  y = min(y + dpp<0x142, 0xa>(y), kMost);
+  y = min(y + dpp<0x143, 0xc>(y), kMost);
   __syncthreads();
-  if (lane == 63) waves[wave] = x;
+  if (lane == 63) waves[wave] = y;
   __syncthreads();
-  int64_t before = 0, all = 0;
+  const uint32_t left = __shfl_up((int)y, 1, 64);
+  Scan r = {lane ? left : 0u, 0u};
 #pragma unroll
-  for (int w = 0; w < NT / 64; w++) {
-    if (w < wave) before += waves[w];
-    all += waves[w];
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    const uint32_t n = waves[w];
+    r.before = w < wave ? min(r.before + n, kMost) : r.before;
+    r.all = min(r.all + n, kMost);
   }
-  *total = all;
-  return x + before;
+  return r;
 }
 
 // First index whose entry exceeds x (n when none does).
@@ -99,6 +113,10 @@ __device__ __forceinline__ int upper_bound(const int32_t *a, int n, int x) {
     else lo = mid + 1;
   }
   return lo;
+}
+
+__device__ __forceinline__ uint32_t ring_at(int64_t i, int64_t capacity) {
+  return (uint64_t)i >> 32 ? (uint32_t)(i % capacity) : (uint32_t)i % (uint32_t)capacity;
 }
 
 // What a workgroup knows of the requests, [batch] each, in LDS.
@@ -119,95 +137,118 @@ struct PlanLds {
 // equal shares, one for each slot, and sets that lie across a border are cut
 // there.  The second costs `cut_tiles` a worker (partial results to write, to
 // read and to join) and is taken where it ends sooner by that count.
-__device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, int64_t *waves) {
-  __shared__ int32_t starts[kMaxSlots + 1];
-  const int tid = threadIdx.x, B = p.batch, G = s.q_heads / s.kv_heads, tokens = (int)p.tokens;
-  const int NB = B + 1;  // the last: packed rows past every request's
-  auto row_count = [&](int b) { return (b < B ? L.end[b] : tokens) - (b ? L.end[b - 1] : 0); };
-  int64_t sum = 0, total;
-  const int items = (NB + kPlanThreads - 1) / kPlanThreads;
-  for (int i = 0; i < items; i++) {
-    const int b = tid * items + i;
-    if (b < NB) sum += ((int64_t)row_count(b) * G + s.rows - 1) / s.rows;
+struct Set {  // query rows f0 to f0 + rows - 1 of request b, and the keys that they see
+  int b, f0, rows, kv0, kv1, n;
+};
+
+__device__ __forceinline__ int set_rows(const sq_kv_plan_args &p, const PlanLds &L, int b) {
+  return (b < p.batch ? L.end[b] : (int)p.tokens) - (b ? L.end[b - 1] : 0);
+}
+
+__device__ __forceinline__ Set find_set(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, int e) {
+  const int G = s.q_heads / s.kv_heads;
+  Set r;
+  r.b = upper_bound(L.tiles, p.batch + 1, e);
+  const int count = set_rows(p, L, r.b);
+  r.f0 = (L.tiles[r.b] - 1 - e) * s.rows;  // the request's last rows first
+  r.rows = min(s.rows, count * G - r.f0);
+  r.kv0 = r.kv1 = r.n = 0;
+  const int old = r.b < p.batch ? L.old[r.b] : -1;
+  if (old >= 0) {
+    r.kv1 = s.causal ? old + (r.f0 + r.rows - 1) / G + 1 : old + count;
+    if (s.window > 0) r.kv0 = max(0, old + r.f0 / G - s.window + 1) & ~(kTile - 1);
+    r.n = (r.kv1 - r.kv0 + kTile - 1) / kTile;
   }
-  int64_t at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
+  return r;
+}
+
+__device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, uint32_t *waves) {
+  __shared__ int32_t starts[kMaxSlots + 1];
+  const int tid = threadIdx.x, B = p.batch, G = s.q_heads / s.kv_heads;
+  const int NB = B + 1;  // the last: packed rows past every request's
+  uint32_t sum = 0;
+  const int items = (NB + kPlanThreads - 1) / kPlanThreads;
+#pragma unroll 1
   for (int i = 0; i < items; i++) {
     const int b = tid * items + i;
-    if (b < NB) L.tiles[b] = (int32_t)(at += ((int64_t)row_count(b) * G + s.rows - 1) / s.rows);
+    if (b < NB) sum += (uint32_t)(set_rows(p, L, b) * G + s.rows - 1) / s.rows;
+  }
+  Scan scan = block_scan(sum);
+  uint32_t at = scan.before;
+#pragma unroll 1
+  for (int i = 0; i < items; i++) {
+    const int b = tid * items + i;
+    if (b < NB) L.tiles[b] = (int32_t)(at += (uint32_t)(set_rows(p, L, b) * G + s.rows - 1) / s.rows);
   }
   __syncthreads();
-  const int sets = (int)total;
-  struct Set {
-    int b, f0, rows, kv0, kv1, n;
-  };
-  auto find = [&](int e) {
-    Set r;
-    r.b = upper_bound(L.tiles, NB, e);
-    const int i = L.tiles[r.b] - 1 - e;  // the request's last rows first
-    const int all = row_count(r.b) * G;
-    r.f0 = i * s.rows;
-    r.rows = min(s.rows, all - r.f0);
-    r.kv0 = r.kv1 = r.n = 0;
-    const int old = r.b < B ? L.old[r.b] : -1;
-    if (old >= 0) {
-      const int held = old + row_count(r.b);
-      r.kv1 = s.causal ? old + (r.f0 + r.rows - 1) / G + 1 : held;
-      if (s.window > 0) r.kv0 = max(0, old + r.f0 / G - s.window + 1) & ~(kTile - 1);
-      r.n = (r.kv1 - r.kv0 + kTile - 1) / kTile;
-    }
-    return r;
-  };
-  int most = 0, least = 0x7fffffff;
+  const int sets = (int)scan.all;
+  uint32_t most = 0, least = kMost;
   sum = 0;
+  Set own = {};  // the thread's last set: its only one where there are few
+#pragma unroll 1
   for (int e = tid; e < sets; e += kPlanThreads) {
-    const int n = find(e).n;
-    sum += n;
+    own = find_set(s, p, L, e);
+    const uint32_t n = own.n;
+    sum = min(sum + n, kMost);
     most = max(most, n);
     least = min(least, n);
   }
-  int64_t tiles;
-  block_scan<kPlanThreads>(sum, &tiles, waves);
+  const uint32_t tiles = block_scan(sum).all;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
-    most = max(most, __shfl_xor(most, k, 64));
-    least = min(least, __shfl_xor(least, k, 64));
+    most = max(most, (uint32_t)__shfl_xor((int)most, k, 64));
+    least = min(least, (uint32_t)__shfl_xor((int)least, k, 64));
   }
   __syncthreads();
-  if ((tid & 63) == 0) waves[tid >> 6] = (int64_t)most << 32 | (uint32_t)least;
+  if ((tid & 63) == 0) waves[tid >> 6] = most, waves[kPlanThreads / 64 + (tid >> 6)] = least;
   __syncthreads();
+#pragma unroll
   for (int w = 0; w < kPlanThreads / 64; w++) {
-    most = max(most, (int)(waves[w] >> 32));
-    least = min(least, (int)(uint32_t)waves[w]);
+    most = max(most, waves[w]);
+    least = min(least, waves[kPlanThreads / 64 + w]);
   }
-  const int64_t slots = max(1, s.slots / s.kv_heads);
-  const int64_t workers = max((int64_t)1, min(slots, tiles / s.min_tiles)), share = (tiles + workers - 1) / workers;
+  // worker w has the tiles from w * share on
+  const uint32_t slots = max(1, s.slots / s.kv_heads), share = max((uint32_t)s.min_tiles, (tiles + slots - 1) / slots);
   // tiles until the last slot is done, either way
-  const int64_t whole = sets <= slots ? most : max((int64_t)most, (tiles + slots - 1) / slots + least);
-  const bool dealt = share + s.cut_tiles < whole;
+  const uint32_t whole = (uint32_t)sets <= slots ? most : max(most, (tiles + slots - 1) / slots + least);
+  const bool dealt = share + s.cut_tiles < whole && tiles < kMost;
+  const int workers = dealt ? (int)((tiles + share - 1) / share) : sets;
   if (dealt)
-    for (int w = tid; w <= workers; w += kPlanThreads) starts[w] = 0x7fffffff;
-  int units = 0, parts = 0, merges = 0;
-  int64_t before = 0;  // tiles of the sets before
+    for (int w = tid; w < workers; w += kPlanThreads) starts[w] = (int)kMost;
+  uint32_t units = 0, parts = 0, merges = 0, before = 0;  // of the sets before; `before` counts their tiles
+#pragma unroll 1
   for (int e0 = 0; e0 < sets; e0 += kPlanThreads) {
     const int e = e0 + tid;
     Set r = {};
-    if (e < sets) r = find(e);
-    const int64_t a = before + block_scan<kPlanThreads>(r.n, &total, waves) - r.n;
-    before += total;
-    // worker w has the tiles from w tiles / workers (rounded down) on
-    auto worker_of = [&](int64_t tile) { return (int)min(workers - 1, ((tile + 1) * workers - 1) / max((int64_t)1, tiles)); };
-    const int w0 = dealt ? worker_of(a) : 0, k = e >= sets ? 0 : dealt && r.n ? worker_of(a + r.n - 1) - w0 + 1 : 1;
-    const int cut = k > 1;
-    // three sums in one: units and parts stay below 2^24, merges below 2^16
-    const int64_t mine = (int64_t)k | (int64_t)(cut ? k : 0) << 24 | (int64_t)cut << 48;
-    const int64_t upto = block_scan<kPlanThreads>(mine, &total, waves) - mine;
-    const int u = units + (int)(upto & 0xffffff), q = parts + (int)(upto >> 24 & 0xffffff), m = merges + (int)(upto >> 48);
+    if (e < sets) r = sets <= kPlanThreads ? own : find_set(s, p, L, e);
+    uint32_t a = 0;
+    int w0 = 0, k = e < sets;
+    if (dealt) {
+      scan = block_scan(r.n);
+      a = before + scan.before;
+      before += scan.all;
+      w0 = min(a / share, (uint32_t)workers - 1);
+      if (r.n) k = (int)((a + r.n - 1) / share) - w0 + 1;
+    }
+    const bool cut = k > 1;
+    scan = block_scan(k);
+    const uint32_t u = units + scan.before;
+    units += scan.all;
+    uint32_t q = 0, m = 0;
+    if (dealt) {
+      scan = block_scan(cut ? k : 0);
+      q = parts + scan.before;
+      parts += scan.all;
+      scan = block_scan(cut);
+      m = merges + scan.before;
+      merges += scan.all;
+    }
     const int q0 = e < sets && r.b ? L.end[r.b - 1] : 0;
+#pragma unroll 1
     for (int j = 0; j < k; j++) {
-      if (u + j >= s.max_units) break;
+      if (u + j >= (uint32_t)s.max_units) break;
       int32_t *o = s.units + 8 * (int64_t)(u + j);
-      const int64_t border0 = (w0 + j) * tiles / workers, border1 = (w0 + j + 1) * tiles / workers;
-      const int t0 = j ? (int)(border0 - a) : 0, t1 = j + 1 < k ? (int)(border1 - a) : r.n;
+      const int t0 = j ? (int)((w0 + j) * share - a) : 0, t1 = j + 1 < k ? (int)((w0 + j + 1) * share - a) : r.n;
       o[0] = r.b < B ? L.row[r.b] : 0;
       o[1] = q0;
       o[2] = r.f0;
@@ -215,10 +256,10 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
       o[4] = r.b < B ? L.old[r.b] : 0;
       o[5] = r.kv0 + t0 * kTile;
       o[6] = min(r.kv1, r.kv0 + t1 * kTile);
-      o[7] = cut ? q + j : -1;
-      if (dealt) atomicMin(&starts[w0 + j], u + j);
+      o[7] = cut ? (int)q + j : -1;
+      if (dealt) atomicMin(&starts[w0 + j], (int)u + j);
     }
-    if (cut && m < s.max_merges) {
+    if (cut && m < (uint32_t)s.max_merges) {
       int32_t *o = s.merges + 8 * (int64_t)m;
       o[0] = q0;
       o[1] = r.f0;
@@ -226,17 +267,18 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
       o[3] = q;
       o[4] = k;
     }
-    units += (int)(total & 0xffffff), parts += (int)(total >> 24 & 0xffffff), merges += (int)(total >> 48);
   }
   __syncthreads();
+#pragma unroll 1
   for (int w = tid; w <= s.max_workers; w += kPlanThreads)
-    s.starts[w] = dealt ? w < workers ? min(units, starts[w]) : units : min(units, w);
+    s.starts[w] = w < workers ? dealt ? min((int)units, starts[w]) : w : (int)units;
+#pragma unroll 1
   for (int m = merges + tid; m < s.max_merges; m += kPlanThreads) s.merges[8 * (int64_t)m + 2] = 0;
 }
 
 __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanDev d) {
   extern __shared__ int32_t lds[];
-  __shared__ int64_t waves[kPlanThreads / 64];
+  __shared__ uint32_t waves[2 * kPlanThreads / 64];
   const sq_kv_tables &t = d.t;
   const sq_kv_plan_args &p = d.p;
   const int tid = threadIdx.x, B = p.batch, P = t.page_tokens;
@@ -246,132 +288,125 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanDev d) {
   L.tiles = L.old + B + 1;
   L.first = L.tiles + B + 1;
   L.row = L.first + B + 1;
-  const int items = (B + kPlanThreads - 1) / kPlanThreads;
+  const int items = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(B, tid * items), b1 = min(B, b0 + items);
   const int64_t head = t.counters[0], tail = t.counters[1];
   const int64_t room = tail - head;
-  int row[kPlanItems], old[kPlanItems], cnt[kPlanItems];
-  int64_t sum = 0, total;
-#pragma unroll
-  for (int i = 0; i < kPlanItems; i++) {
-    const int b = tid * items + i;
-    row[i] = -1, old[i] = -1, cnt[i] = 0;
-    if (i < items && b < B) {
-      const int64_t r = load_index(p.rows, p.rows_dtype, b), n = load_index(p.counts, p.counts_dtype, b);
-      // more than `tokens` rows never fit: the sums stay within 64 bits
-      cnt[i] = (int)(n < 0 ? 0 : n > p.tokens + 1 ? p.tokens + 1 : n);
-      if (r >= 0 && r < t.requests) {
-        row[i] = (int)r;
-        old[i] = t.lens[r];
-      }
-      sum += cnt[i];
-    }
+  const int most = (int)min((int64_t)p.max_count, p.tokens);  // no request with more new tokens finds room
+  uint32_t sum = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; b++) {
+    const int64_t r = load_index(p.rows, p.rows_dtype, b), n = load_index(p.counts, p.counts_dtype, b);
+    const bool there = r >= 0 && r < t.requests;
+    L.row[b] = there ? (int)r : -1;
+    L.old[b] = there ? t.lens[r] : -1;
+    // (its rows count all the same; past 2^30 the sums stop counting)
+    const int count = (int)(n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : n);
+    L.first[b] = count;
+    sum = min(sum + count, kMost);
   }
-  int64_t at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
-  int64_t need[kPlanItems];
-  bool fits[kPlanItems];
+  Scan scan = block_scan(sum);
+  uint32_t at = scan.before;
   sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPlanItems; i++) {
-    const int b = tid * items + i;
-    need[i] = 0, fits[i] = false;
-    if (i < items && b < B) {
-      at += cnt[i];
-      L.end[b] = (int32_t)min(at, p.tokens);
-      const int64_t want = (int64_t)old[i] + cnt[i], blocks = (want + P - 1) / P;
-      fits[i] = old[i] >= 0 && cnt[i] <= p.max_count && blocks <= t.width && at <= p.tokens && want <= 0x7fffffff;
-      if (fits[i]) need[i] = blocks - (old[i] + (int64_t)P - 1) / P;
-      sum += need[i];
+#pragma unroll 1
+  for (int b = b0; b < b1; b++) {
+    const uint32_t count = L.first[b];
+    at = min(at + count, kMost);
+    const int old = L.old[b];
+    L.end[b] = (int)min((int64_t)at, p.tokens);
+    // pages for the new tokens; -1: the request does not fit
+    int need = -1;
+    if (old >= 0 && count <= (uint32_t)most && at <= p.tokens && old <= (int)kMost - (int)count) {
+      const uint32_t blocks = (old + count + P - 1) / P;
+      if (blocks <= (uint32_t)t.width) need = blocks - ((uint32_t)old + P - 1) / P;
     }
+    L.tiles[b] = need;
+    sum = min(sum + max(need, 0), kMost);
   }
-  at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
-  int64_t taken = 0;
-  int touched[kPlanItems];
+  scan = block_scan(sum);
+  at = scan.before;
+  uint32_t taken = 0;
   sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPlanItems; i++) {
-    const int b = tid * items + i;
-    touched[i] = 0;
-    if (i < items && b < B) {
-      const int64_t first = at;
-      at += need[i];
-      const bool ok = fits[i] && (need[i] == 0 || at <= room);
-      if (ok && need[i]) taken = at;
-      L.row[b] = row[i];
-      L.first[b] = ok ? (int32_t)min(first, (int64_t)0x7fffffff) : 0;
-      L.old[b] = ok ? old[i] : -1;
-      if (ok && cnt[i]) touched[i] = (int)((old[i] + (int64_t)cnt[i] + P - 1) / P - old[i] / P);
-      sum += touched[i];
-      if (blockIdx.x == 0) {
-        p.lens[b] = row[i] < 0 ? 0 : ok ? old[i] + cnt[i] : old[i];
-        p.granted[b] = ok;
-      }
+#pragma unroll 1
+  for (int b = b0; b < b1; b++) {
+    const int need = L.tiles[b], old = L.old[b], count = L.first[b];
+    const uint32_t first = at;
+    at = min(at + max(need, 0), kMost);
+    const bool ok = need == 0 || (need > 0 && at <= room);
+    if (ok && need) taken = at;
+    const int touched = ok && count ? ((uint32_t)old + count + P - 1) / P - old / P : 0;
+    if (blockIdx.x == 0) {
+      p.lens[b] = L.row[b] < 0 ? 0 : ok ? old + count : old;
+      p.granted[b] = ok;
     }
+    L.first[b] = ok ? (int)first : 0;
+    L.old[b] = ok ? old : -1;
+    L.tiles[b] = touched;
+    sum += touched;
   }
-  at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
-#pragma unroll
-  for (int i = 0; i < kPlanItems; i++) {
-    const int b = tid * items + i;
-    if (i < items && b < B) L.tiles[b] = (int32_t)(at += touched[i]);
-  }
-  const int n_tiles = (int)total;
+  scan = block_scan(sum);
+  at = scan.before;
+#pragma unroll 1
+  for (int b = b0; b < b1; b++) L.tiles[b] = (int)(at += L.tiles[b]);
+  const int n_tiles = (int)scan.all;
   __syncthreads();
   if ((int)blockIdx.x >= d.share_blocks) {
     plan_schedule(p.schedules[blockIdx.x - d.share_blocks], p, L, waves);
     return;
   }
   if (blockIdx.x == 0) {
-    // the pages taken: those of the last request that needed and got one
-    block_scan<kPlanThreads>(0, &total, waves);
-    int64_t best = taken;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) best = max(best, (int64_t)__shfl_xor(best, k, 64));
-    if ((tid & 63) == 0) waves[tid >> 6] = best;
+    // the pages taken: up to those of the last request that needed and got one
+#pragma unroll 1
+    for (int k = 1; k < 64; k <<= 1) taken = max(taken, (uint32_t)__shfl_xor((int)taken, k, 64));
+    __syncthreads();
+    if ((tid & 63) == 0) waves[tid >> 6] = taken;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 0; w < kPlanThreads / 64; w++) best = max(best, waves[w]);
-      p.counters[0] = head + best;
+#pragma unroll 1
+      for (int w = 0; w < kPlanThreads / 64; w++) taken = max(taken, waves[w]);
+      p.counters[0] = head + taken;
       p.counters[1] = tail;
       p.cu[0] = 0;
     }
     for (int b = tid; b < B; b += kPlanThreads) p.cu[b + 1] = L.end[b];
   }
-  const int64_t h0 = head % t.capacity;
+  const uint32_t h0 = ring_at(head, t.capacity);
   // the page of a request's block: its own, or the ring's entry that it gets
   auto page_of = [&](int b, int block) {
-    const int had = (int)((L.old[b] + (int64_t)P - 1) / P);
-    if (block < had) return t.table[(int64_t)L.row[b] * t.width + block];
-    int64_t i = h0 + L.first[b] + (block - had);
-    if (i >= t.capacity) i -= t.capacity;
-    return t.free_pages[i];
+    const int had = (int)(((uint32_t)L.old[b] + P - 1) / P);
+    uint32_t i = h0 + L.first[b] + (block - had);
+    if (i >= (uint32_t)t.capacity) i -= t.capacity;
+    return block < had ? t.table[(int64_t)L.row[b] * t.width + block] : t.free_pages[i];
   };
   const int from = blockIdx.x * kPlanShare, upto = from + kPlanShare;
+#pragma unroll 1
   for (int i = from + tid; i < upto && i < p.tokens; i += kPlanThreads) {
     const int b = upper_bound(L.end, B, i);
     int64_t slot = -1;
     int pos = -1;
     if (b < B && L.old[b] >= 0) {
       pos = L.old[b] + i - (b ? L.end[b - 1] : 0);
-      slot = (int64_t)page_of(b, pos / P) * P + pos % P;
+      const int block = (uint32_t)pos / P;
+      slot = (int64_t)page_of(b, block) * P + (pos - block * P);
     }
     p.slots[i] = slot;
     p.positions[i] = pos;
   }
+#pragma unroll 1
   for (int i = from + tid; i < upto && i < p.max_tiles; i += kPlanThreads) {
     int page = 0, filled = 0, start = 0, token = 0;
     if (i < n_tiles) {
       const int b = upper_bound(L.tiles, B, i);
       const int old = L.old[b], base = b ? L.end[b - 1] : 0;
-      const int block = old / P + i - (b ? L.tiles[b - 1] : 0);
+      const int block = (uint32_t)old / P + i - (b ? L.tiles[b - 1] : 0);
       page = page_of(b, block);
-      if (block >= (int)((old + (int64_t)P - 1) / P)) t.table[(int64_t)L.row[b] * t.width + block] = page;
+      if (block >= (int)(((uint32_t)old + P - 1) / P)) t.table[(int64_t)L.row[b] * t.width + block] = page;
       start = max(0, old - block * P);
       token = base + max(0, block * P - old);
-      filled = (int)min((int64_t)P, (int64_t)old + L.end[b] - base - (int64_t)block * P);
+      filled = min(P, old + L.end[b] - base - block * P);
     }
     p.pages[i] = page;
     p.filled[i] = filled;
-    p.tiles[2 * (int64_t)i] = start;
-    p.tiles[2 * (int64_t)i + 1] = token;
+    *(int2 *)(p.tiles + 2 * (int64_t)i) = make_int2(start, token);
   }
 }
 
@@ -386,32 +421,33 @@ __global__ __launch_bounds__(256) void kv_commit_kernel(PlanDev d) {
 // One workgroup: pages go back in the order of the rows and their blocks.
 __global__ __launch_bounds__(kPlanThreads) void kv_release_kernel(sq_kv_tables t, const void *rows, int rows_dtype, int n) {
   extern __shared__ int32_t lds[];
-  __shared__ int64_t waves[kPlanThreads / 64];
   int32_t *end = lds, *row = lds + n;
   const int tid = threadIdx.x, items = (n + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(n, tid * items), b1 = min(n, b0 + items);
   const int64_t tail = t.counters[1];
-  int64_t sum = 0, total;
-  for (int i = 0; i < items; i++) {
-    const int b = tid * items + i;
-    if (b >= n) break;
+  uint32_t sum = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; b++) {
     const int64_t r = load_index(rows, rows_dtype, b);
+    const bool there = r >= 0 && r < t.requests;
     // the exchange leaves a row's pages to one of the entries that name it
-    const int len = r >= 0 && r < t.requests ? atomicExch(&t.lens[r], 0) : 0;
-    row[b] = (int)(r >= 0 && r < t.requests ? r : 0);
-    end[b] = len > 0 ? (int)min(((int64_t)len + t.page_tokens - 1) / t.page_tokens, (int64_t)t.width) : 0;
-    sum += end[b];
+    const int len = there ? atomicExch(&t.lens[r], 0) : 0;
+    row[b] = there ? (int)r : 0;
+    end[b] = len > 0 ? (int)min(((uint32_t)len + t.page_tokens - 1) / t.page_tokens, (uint32_t)t.width) : 0;
+    sum = min(sum + end[b], kMost);
   }
-  int64_t at = block_scan<kPlanThreads>(sum, &total, waves) - sum;
-  for (int i = 0; i < items; i++) {
-    const int b = tid * items + i;
-    if (b < n) end[b] = (int32_t)(at += end[b]);
-  }
+  const Scan scan = block_scan(sum);
+  uint32_t at = scan.before;
+#pragma unroll 1
+  for (int b = b0; b < b1; b++) end[b] = (int32_t)(at += end[b]);
   __syncthreads();
-  const int64_t t0 = tail % t.capacity;
-  for (int64_t i = tid; i < total; i += kPlanThreads) {
-    const int b = upper_bound(end, n, (int)i);
+  const int64_t total = min((int64_t)scan.all, t.capacity);  // (more pages than there are: tables that were not filled here)
+  const uint32_t t0 = ring_at(tail, t.capacity);
+  for (int i = tid; i < total; i += kPlanThreads) {
+    const int b = upper_bound(end, n, i);
     int32_t *entry = t.table + (int64_t)row[b] * t.width + (i - (b ? end[b - 1] : 0));
-    t.free_pages[(t0 + i) % t.capacity] = *entry;
+    const uint32_t j = t0 + i;
+    t.free_pages[j >= (uint32_t)t.capacity ? j - t.capacity : j] = *entry;
     *entry = 0;
   }
   if (tid == 0) t.counters[1] = tail + total;
