@@ -1019,11 +1019,16 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   extern __shared__ uint4 tiles[];
   constexpr int KS = D / 16, DT = D / 32;                   // k steps and dim tiles
   constexpr int KF = 65, KB = 2 * KS * KF, VB = 4 * DT * 64;  // uint4 of a step's keys, of a tile's keys and values
-  constexpr int OT = D == 256 ? DT / 2 : DT;                // a wave's dim tiles
-  constexpr int WR = D == 256 ? 128 : 256;                  // rows of the workgroup at a time
+  // Of 256 dims, whose outputs would fill a wave's registers, two waves share 32
+  // rows: each takes the scores of half of a tile's keys and the outputs of
+  // half of the dims, and they pass each other their probabilities in LDS.
+  constexpr bool PAIRS = D == 256;
+  constexpr int ST = PAIRS ? 1 : 2;                         // a wave's groups of 32 keys of a tile
+  constexpr int OT = PAIRS ? DT / 2 : DT;                   // a wave's dim tiles
+  constexpr int WR = PAIRS ? 128 : 256;                     // rows of the workgroup at a time
   constexpr int KN = KS > 8 ? KS / 8 : 1;                   // 16-byte groups of keys of a thread
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hl = lane >> 5;
-  const int late = wave >> 2, e0 = D == 256 ? late * OT : 0;
+  const int late = wave >> 2, side = PAIRS ? wave & 1 : 0, e0 = side * OT;
   const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
   const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
@@ -1037,6 +1042,9 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
   // the peaks of two tiles, and whether their pages exist
   float4 *const peaks = (float4 *)(vb + 2 * VB);
+  // (pairs) probabilities of a wave, and its rows' maxima, then sums
+  uint4 *const passed = (uint4 *)(peaks + 2) + wave * 128, *const taken = (uint4 *)(peaks + 2) + (wave ^ 1) * 128;
+  float *const passed_m = (float *)(peaks + 2 + 8 * 128) + wave * 32, *const taken_m = (float *)(peaks + 2 + 8 * 128) + (wave ^ 1) * 32;
   const int pages = (int)a.c.num_pages, first_key = 2 * h * P * D;
   const uint32_t page_bytes = (uint32_t)a.c.page_bytes;
 
@@ -1045,7 +1053,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
     // (the unit's last rows may be of another turn)
     const int kv1 = a.causal ? min(end, pos0 + (f0 + rows - 1) / G + 1) : end;
     const int n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
-    const int first_row = 32 * (D == 256 ? wave & 3 : wave), mine = first_row + c;
+    const int first_row = 32 * (PAIRS ? wave >> 1 : wave), mine = first_row + c;
     const bool live = mine < rows;
     const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
     half8_v qf[KS];
@@ -1079,13 +1087,14 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
     const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
     const int all_hi = min(kv1, a.causal ? pos0 + (f0 + first_row) / G + 1 : kv1);
     const int all_lo = a.window > 0 ? pos0 + (f0 + max(1, min(rows, first_row + 32)) - 1) / G - a.window + 1 : 0;
-    f32x16_v o[OT], s[2];
-    half8_v pf[4];
+    f32x16_v o[OT], s[ST];
+    half8_v pf[2 * ST];
 #pragma unroll
     for (int e = 0; e < OT; e++)
 #pragma unroll
       for (int k = 0; k < 16; k++) o[e][k] = 0.f;
     float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
+    float om = -INFINITY, oref = 0.f;  // (pairs) what the outputs are in units of
 
     // The tiles in order; past the last one the last again, so that loads ahead
     // need no branch.  A page's number is loaded two tiles before it is used.
@@ -1158,25 +1167,54 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       each(one, std::make_integer_sequence<int, DT>{});
     };
     // Outputs with one tile's values (with VALUES), then scores with another
-    // one's keys; the operands are read DEEP products ahead (8; 4 of 256 dims, where registers end).
+    // one's keys; the operands are read DEEP products ahead.
     auto products = [&](auto VALUES, const uint4 *values, const uint4 *keys) {
-      constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + 2 * KS, DEEP = D == 256 ? 4 : 8;
+      constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + ST * KS, DEEP = 8;
+      half8_v pv[4];
+      if constexpr (!PAIRS) {
 #pragma unroll
-      for (int tt = 0; tt < 2; tt++)
+        for (int j = 0; j < 4; j++) pv[j] = pf[j];
+      } else if constexpr (NV > 0) {
+        // own probabilities and the other wave's, brought to one maximum: maxima
+        // are whole numbers here, so that the factors are powers of two
+        const uint4 w0 = taken[lane], w1 = taken[64 + lane];
+        const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
+        pv[0] = pf[0], pv[1] = pf[1];
+        pv[2] = __builtin_bit_cast(half8_v, w0), pv[3] = __builtin_bit_cast(half8_v, w1);
+        if (__any(m != theirs)) {
+          const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(m - base), f1 = (_Float16)__builtin_amdgcn_exp2f(theirs - base);
+          pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
+        }
+        if (__any(high > om || ref > oref)) {
+          float shrink = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - high);
+          if (ref > oref) shrink *= oref / ref;
+          om = high, oref = ref;
+#pragma unroll
+          for (int e = 0; e < OT; e++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+        }
+      }
+#pragma unroll
+      for (int tt = 0; tt < ST; tt++)
 #pragma unroll
         for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
       uint4 w[DEEP];
+      // (pairs: the wave's own half of the keys first)
+      const uint4 *const near = PAIRS ? values + (4 * e0 + 2 * side) * 64 + lane : values + lane;
+      const uint4 *const far = PAIRS ? values + (4 * e0 + 2 * (1 - side) - 2) * 64 + lane : near;
+      const uint4 *const key = keys + side * (KS * KF) + lane;
       auto read = [&](int i) {
-        const int k = (i - NV) >> 1, tt = (i - NV) & 1;
-        return i < NV ? values[(4 * (e0 + i % OT) + i / OT) * 64 + lane] : keys[(tt * KS + k) * KF + lane];
+        if (i < NV) return (i / OT < 2 ? near : far)[(4 * (i % OT) + i / OT) * 64];
+        return key[((i - NV) % ST * KS + (i - NV) / ST) * KF];
       };
 #pragma unroll
       for (int i = 0; i < DEEP; i++) w[i] = read(i);
 #pragma unroll
       for (int i = 0; i < N; i++) {
         const half8_v x = __builtin_bit_cast(half8_v, w[i % DEEP]);
-        if (i < NV) o[i % OT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[i / OT], o[i % OT], 0, 0, 0);
-        else s[(i - NV) & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - NV) >> 1], s[(i - NV) & 1], 0, 0, 0);
+        if (i < NV) o[i % OT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pv[i / OT], o[i % OT], 0, 0, 0);
+        else s[(i - NV) % ST] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - NV) / ST], s[(i - NV) % ST], 0, 0, 0);
         if (i + DEEP < N) w[i % DEEP] = read(i + DEEP);
       }
       __builtin_amdgcn_sched_group_barrier(0x100, DEEP, 0);  // LDS reads
@@ -1193,9 +1231,9 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       const bool known = __builtin_amdgcn_readfirstlane(__float_as_uint(peak.z)) != 0;
       bool some = true;
       if (!(known && first + kTile <= all_hi && first >= all_lo)) {  // some row does not see all of the tile
-        const int above = known ? hi - first - 4 * hl : 0, below = lo - first - 4 * hl;
+        const int mine = first + 32 * side + 4 * hl, above = known ? hi - mine : 0, below = lo - mine;
 #pragma unroll
-        for (int k = 0; k < 32; k++) {
+        for (int k = 0; k < 16 * ST; k++) {
           const int j = 32 * (k >> 4) + 8 * (k >> 2 & 3) + (k & 3);
           // all ones where below <= j < above; as conditions, 64 of them would
           // spill the loop's scalar registers
@@ -1206,9 +1244,9 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         }
         some = known && first < hi && first + kTile > lo;
       }
-      float best = fmaxf(s[0][0], s[1][0]);
+      float best = s[0][0];
 #pragma unroll
-      for (int k = 1; k < 16; k++) best = fmaxf(fmaxf(best, s[0][k]), s[1][k]);
+      for (int k = 1; k < 16 * ST; k++) best = fmaxf(best, s[k >> 4][k & 15]);
       best = reduce_max2(best);
       // a tile that the row does not see takes no part in it, whatever its
       // peaks; a factor of 0 would make NaN of the scores that are masked
@@ -1217,24 +1255,26 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       best *= f;
       const float high = some ? fmaxf(ref, peak.y) : ref;
       if (__any(best > m + 8.f || high > ref)) {
-        const float raised = fmaxf(m, best);
+        const float raised = fmaxf(m, PAIRS ? ceilf(best) : best);
         const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
         const float shrink = high > ref ? ref / high * was : was;
         m = raised;
         ref = high;
         log_ref = ref > 0.f ? __builtin_amdgcn_logf(ref) : 0.f;
         l *= was;
+        if constexpr (!PAIRS) {
 #pragma unroll
-        for (int e = 0; e < OT; e++)
+          for (int e = 0; e < OT; e++)
 #pragma unroll
-          for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+            for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+        }
       }
       const float base = m == -INFINITY ? 0.f : m;
       const float size = some ? __builtin_amdgcn_logf(peak.y) - log_ref : 0.f;
       const float off = size - base;
       float sum = 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < 2 * ST; j++) {
         u32x4_v w;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -1250,6 +1290,11 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         pf[j] = __builtin_bit_cast(half8_v, w);
       }
       l = fmaf(sum, __builtin_amdgcn_exp2f(-size), l);
+      if constexpr (PAIRS) {
+        passed[lane] = __builtin_bit_cast(uint4, pf[0]);
+        passed[64 + lane] = __builtin_bit_cast(uint4, pf[1]);
+        if (hl == 0) passed_m[c] = m;
+      }
     };
 
     float4 peak, peak0;
@@ -1311,6 +1356,18 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       __syncthreads();  // the next turn writes where the last products read
     }
     l = reduce_sum2(l);
+    if constexpr (PAIRS) {
+      // the two waves' sums, brought to one maximum (their last products are done)
+      if (hl == 0) {
+        passed_m[c] = m;
+        ((float *)passed)[c] = l;
+      }
+      __syncthreads();
+      const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
+      l = fmaf(l, __builtin_amdgcn_exp2f(m - base), ((float *)taken)[c] * __builtin_amdgcn_exp2f(theirs - base));
+      m = high;
+      __syncthreads();
+    }
     const float unit = ref * kValueUnit<FP8>;
     if (part < 0) {
       // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
@@ -1325,7 +1382,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         store_row<OT>((uint16_t *)(rows_at + c * OW) + (8 * (k >> 2) + 4 * hl + (k & 3)) * OT, a.dtype == SQ_BF16, x);
       }
       __builtin_amdgcn_wave_barrier();
-      if constexpr (D == 256) {
+      if constexpr (PAIRS) {
         // the wave's dims are every other group of four: 8 bytes a lane
         constexpr int LANES = OD / 4;
 #pragma unroll
@@ -1352,7 +1409,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       // as the registers hold them: a wave writes 64 OT floats in a row
       typedef float vec __attribute__((ext_vector_type(OT)));
       const int64_t slot = (int64_t)part * a.kv_heads + h;
-      float *dst = a.ws + ((slot * (D == 256 ? 16 : 8) + turn / WR * 8 + wave) * (16 * 64) + lane) * OT;
+      float *dst = a.ws + ((slot * (PAIRS ? 16 : 8) + turn / WR * 8 + wave) * (16 * 64) + lane) * OT;
 #pragma unroll
       for (int k = 0; k < 16; k++) {
         vec x;
@@ -1441,8 +1498,8 @@ __global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
   const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.kv_heads);
   const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
   const int tid = threadIdx.x & 255, half = threadIdx.x >> 8, lane = tid & 63, c = lane & 31, hl = lane >> 5, k0 = tid >> 6;
-  const int e0 = D == 256 ? (wave >> 2) * OT : 0;
-  const int first = D == 256 ? 128 * turn + 32 * (wave & 3) : 32 * wave, j = first + c;
+  const int e0 = D == 256 ? (wave & 1) * OT : 0;
+  const int first = D == 256 ? 128 * turn + 32 * (wave >> 1) : 32 * wave, j = first + c;
   if (first >= rows) return;
   const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * (int64_t)min(j, rows - 1);
   vec x[4];
@@ -1560,18 +1617,18 @@ int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
   return 0;
 }
 
-// Raises a kernel's limit of dynamic LDS, once per kernel (each with an id of
-// its own) and device, to 136 KiB, more than the most that one takes.
+// Raises a kernel's limit of dynamic LDS to the most that it takes, once per
+// kernel (each with an id of its own) and device.
 std::atomic<uint64_t> g_raised[16];
 
-int dynamic_lds(const void *kernel, int id, size_t bytes, const char *what) {
-  if (bytes <= 65536) return 0;
+int dynamic_lds(const void *kernel, int id, size_t most, const char *what) {
+  if (most <= 65536) return 0;
   int dev = -1;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return fail((int)e, what);
   const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
   if (g_raised[id].load(std::memory_order_relaxed) & bit) return 0;
-  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024);
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
   if (e != hipSuccess) return fail((int)e, what);
   g_raised[id].fetch_or(bit, std::memory_order_relaxed);
   return 0;
@@ -1590,7 +1647,7 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
   static_assert(D <= 256, "ids of kernels with more than 64 KiB");
   constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float);
   // tiles and peaks; the outputs' way out
-  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1), rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
+  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 128) : 0), rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
   constexpr size_t many = staged > rows_out ? staged : rows_out;
   int rc;
   if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
@@ -1617,7 +1674,7 @@ int sq_kv_plan(const sq_kv_tables *t, const sq_kv_plan_args *p, void *stream) {
   d.share_blocks = (int)((share + kPlanShare - 1) / kPlanShare);
   if (d.share_blocks < 1) d.share_blocks = 1;
   const size_t lds = 5 * sizeof(int32_t) * (size_t)(p->batch + 1);
-  const int e = dynamic_lds((const void *)kv_plan_kernel, 0, lds, "kv plan: LDS attribute");
+  const int e = dynamic_lds((const void *)kv_plan_kernel, 0, 5 * sizeof(int32_t) * (SQ_KV_MAX_REQUESTS + 1), "kv plan: LDS attribute");
   if (e) return e;
   hipLaunchKernelGGL(kv_plan_kernel, dim3((unsigned)(d.share_blocks + p->n_schedules)), dim3(kPlanThreads), lds,
                      (hipStream_t)stream, d);
