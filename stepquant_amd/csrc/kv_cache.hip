@@ -646,6 +646,15 @@ __device__ __forceinline__ float reduce_sum4(float x) {
 
 __device__ __forceinline__ uint32_t half2_bits(half2_v h) { return __builtin_bit_cast(uint32_t, h); }
 
+// Two probabilities as the halves that enter the products, their sum added in
+// 32 bits.  The sum is of the rounded ones, so that their rounding cancels
+// where one key has most of a row (5e-5 in place of 1e-4 of an output there).
+__device__ __forceinline__ uint32_t weigh2(float p0, float p1, float &sum) {
+  const half2_v h = __builtin_convertvector((f32x2_v){p0, p1}, half2_v);
+  sum = __builtin_amdgcn_fdot2(h, (half2_v){(_Float16)1.f, (_Float16)1.f}, sum, false);
+  return half2_bits(h);
+}
+
 // two keys' codes (bytes 2 i and 2 i + 1 of w) as halves
 template <bool FP8, int I>
 __device__ __forceinline__ uint32_t key2(uint32_t w) {
@@ -904,13 +913,9 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
         for (int t = 0; t < NT; t++) {
           float p[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            p[k] = __builtin_amdgcn_exp2f(s[r][t][k] - base);
-            sum += p[k];
-          }
+          for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(s[r][t][k] - base);
 #pragma unroll
-          for (int k = 0; k < 2; k++)
-            w[t >> 1][2 * (t & 1) + k] = half2_bits(__builtin_convertvector((f32x2_v){p[2 * k], p[2 * k + 1]}, half2_v));
+          for (int k = 0; k < 2; k++) w[t >> 1][2 * (t & 1) + k] = weigh2(p[2 * k], p[2 * k + 1], sum);
         }
         l[r] = fmaf(l[r], alpha[r], sum);
 #pragma unroll
@@ -1283,9 +1288,8 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
           for (int b = 0; b < 2; b++) {
             const int at = 8 * j + 2 * k + b;
             p[b] = __builtin_amdgcn_exp2f(fmaf(s[at >> 4][at & 15], f, off));
-            sum += p[b];
           }
-          w[k] = half2_bits(__builtin_convertvector((f32x2_v){p[0], p[1]}, half2_v));
+          w[k] = weigh2(p[0], p[1], sum);
         }
         pf[j] = __builtin_bit_cast(half8_v, w);
       }
