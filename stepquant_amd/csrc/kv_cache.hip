@@ -419,7 +419,8 @@ __global__ __launch_bounds__(256) void kv_commit_kernel(PlanDev d) {
 }
 
 // One workgroup: pages go back in the order of the rows and their blocks.
-__global__ __launch_bounds__(kPlanThreads) void kv_release_kernel(sq_kv_tables t, const void *rows, int rows_dtype, int n) {
+__global__ __launch_bounds__(kPlanThreads) void kv_release_kernel(sq_kv_tables t, const void *rows, int rows_dtype,
+                                                                  int n) {
   extern __shared__ int32_t lds[];
   int32_t *end = lds, *row = lds + n;
   const int tid = threadIdx.x, items = (n + kPlanThreads - 1) / kPlanThreads;
@@ -441,7 +442,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_release_kernel(sq_kv_tables t
 #pragma unroll 1
   for (int b = b0; b < b1; b++) end[b] = (int32_t)(at += end[b]);
   __syncthreads();
-  const int64_t total = min((int64_t)scan.all, t.capacity);  // (more pages than there are: tables that were not filled here)
+  // (more pages than there are: tables that were not filled here)
+  const int64_t total = min((int64_t)scan.all, t.capacity);
   const uint32_t t0 = ring_at(tail, t.capacity);
   for (int i = tid; i < total; i += kPlanThreads) {
     const int b = upper_bound(end, n, i);
@@ -507,7 +509,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
   const uint16_t *src = (const uint16_t *)(part ? a.v : a.k) + h * (part ? a.v_head_stride : a.k_head_stride);
   const int64_t stride = part ? a.v_stride : a.k_stride;
   uint8_t *base = c.data + page * c.page_bytes + ((int64_t)(2 * h + part) * c.page_tokens << log_dim);
-  float *peak_at = (float *)(c.data + page * c.page_bytes + (2 * (int64_t)c.heads * c.page_tokens << log_dim)) + 2 * h + part;
+  const int64_t peaks_at = 2 * (int64_t)c.heads * c.page_tokens << log_dim;
+  float *peak_at = (float *)(c.data + page * c.page_bytes + peaks_at) + 2 * h + part;
   const int from = start << (log_dim - 3), upto = filled << (log_dim - 3);
   u32x4_v x[N];
   uint32_t most = 0;  // magnitudes as bits: their order, and NaN above all
@@ -562,8 +565,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
 }
 
 template <bool FP8>
-__global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int32_t *pages, const int32_t *filled, void *k,
-                                                        void *v, int dtype, int log_dim) {
+__global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int32_t *pages, const int32_t *filled,
+                                                        void *k, void *v, int dtype, int log_dim) {
   const int tid = threadIdx.x, h = blockIdx.y, part = blockIdx.z;
   const int64_t n = blockIdx.x;
   const int64_t page = pages[n];
@@ -571,7 +574,8 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int
   const int held = there ? filled ? filled[n] : c.page_tokens : 0;
   const uint8_t *at = c.data + (there ? page : 0) * c.page_bytes;
   const uint8_t *base = at + ((int64_t)(2 * h + part) * c.page_tokens << log_dim);
-  const float scale = ((const float *)(at + (2 * (int64_t)c.heads * c.page_tokens << log_dim)))[2 * h + part] / (FP8 ? 448.f : 127.f);
+  const int64_t peaks_at = 2 * (int64_t)c.heads * c.page_tokens << log_dim;
+  const float scale = ((const float *)(at + peaks_at))[2 * h + part] / (FP8 ? 448.f : 127.f);
   void *out = part ? v : k;
   const int groups = c.page_tokens << (log_dim - 3);
   for (int g = tid; g < groups; g += 256) {
@@ -744,7 +748,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   extern __shared__ float smem[];
   constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
   constexpr int NT = D == 256 ? 2 : 4, STEP = 16 * NT;  // 16-key groups and keys of a step
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
   const int at_row = 16 * RT * blockIdx.y;  // of the unit's rows
   const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
@@ -760,7 +765,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   auto read_unit = [&](int i) {
     const int32_t *u = a.units + 8 * (int64_t)i;
     Unit x = {u[0], u[1], u[2] + at_row, min(u[3] - at_row, 16 * RT), u[4], u[5], u[6], u[7], 0};
-    if (x.rows <= 0 || u[3] > a.unit_rows || x.q0 < 0 || x.f0 < 0 || x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
+    if (x.rows <= 0 || u[3] > a.unit_rows || x.q0 < 0 || x.f0 < 0 ||
+        x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
       x.rows = 0;
     // a row of the table that does not exist holds no keys
     const bool held = x.rows > 0 && x.row >= 0 && x.row < a.requests;
@@ -1032,402 +1038,409 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   constexpr int OT = PAIRS ? DT / 2 : DT;                   // a wave's dim tiles
   constexpr int WR = PAIRS ? 128 : 256;                     // rows of the workgroup at a time
   constexpr int KN = KS > 8 ? KS / 8 : 1;                   // 16-byte groups of keys of a thread
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hl = lane >> 5;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 31, hl = lane >> 5;
   const int late = wave >> 2, side = PAIRS ? wave & 1 : 0, e0 = side * OT;
   const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
   const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
-  const int32_t *u = a.units + 8 * (int64_t)unit_at;
-  const int row = u[0], q0 = u[1], pos0 = u[4], kv0 = u[5], part = u[7];
-  if (u[3] <= 0 || u[3] > a.unit_rows || q0 < 0 || u[2] < 0 || q0 + (int64_t)(u[2] + u[3] - 1) / G >= a.tokens) continue;
-  const int end = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
-  const int P = a.c.page_tokens, per = P / kTile, tile0 = kv0 / kTile;
-  const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
-  const int32_t *entries = a.table + (int64_t)row * a.width;
-  uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
-  // the peaks of two tiles, and whether their pages exist
-  float4 *const peaks = (float4 *)(vb + 2 * VB);
-  // (pairs) probabilities of a wave, and its rows' maxima, then sums
-  uint4 *const passed = (uint4 *)(peaks + 2) + wave * 128, *const taken = (uint4 *)(peaks + 2) + (wave ^ 1) * 128;
-  float *const passed_m = (float *)(peaks + 2 + 8 * 128) + wave * 32, *const taken_m = (float *)(peaks + 2 + 8 * 128) + (wave ^ 1) * 32;
-  const int pages = (int)a.c.num_pages, first_key = 2 * h * P * D;
-  const uint32_t page_bytes = (uint32_t)a.c.page_bytes;
+    const int32_t *u = a.units + 8 * (int64_t)unit_at;
+    const int row = u[0], q0 = u[1], pos0 = u[4], kv0 = u[5], part = u[7];
+    if (u[3] <= 0 || u[3] > a.unit_rows || q0 < 0 || u[2] < 0 || q0 + (int64_t)(u[2] + u[3] - 1) / G >= a.tokens)
+      continue;
+    const int end = row >= 0 && row < a.requests ? (int)min((int64_t)u[6], (int64_t)a.width * a.c.page_tokens) : 0;
+    const int P = a.c.page_tokens, per = P / kTile, tile0 = kv0 / kTile;
+    const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
+    const int32_t *entries = a.table + (int64_t)row * a.width;
+    uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
+    // the peaks of two tiles, and whether their pages exist
+    float4 *const peaks = (float4 *)(vb + 2 * VB);
+    // (pairs) probabilities of a wave, and its rows' maxima, then sums
+    uint4 *const shared = (uint4 *)(peaks + 2), *const passed = shared + wave * 128, *const taken = shared + (wave ^ 1) * 128;
+    float *const shared_m = (float *)(shared + 8 * 128);
+    float *const passed_m = shared_m + wave * 32, *const taken_m = shared_m + (wave ^ 1) * 32;
+    const int pages = (int)a.c.num_pages, first_key = 2 * h * P * D;
+    const uint32_t page_bytes = (uint32_t)a.c.page_bytes;
 
-  for (int turn = 0; turn < u[3]; turn += WR) {
-    const int f0 = u[2] + turn, rows = min(u[3] - turn, WR);
-    // (the unit's last rows may be of another turn)
-    const int kv1 = a.causal ? min(end, pos0 + (f0 + rows - 1) / G + 1) : end;
-    const int n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
-    const int first_row = 32 * (PAIRS ? wave >> 1 : wave), mine = first_row + c;
-    const bool live = mine < rows;
-    const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
-    half8_v qf[KS];
-    float mult;
-    auto read_queries = [&]() {
-      const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 8 * hl;
-      u32x4_v w[KS];
+    for (int turn = 0; turn < u[3]; turn += WR) {
+      const int f0 = u[2] + turn, rows = min(u[3] - turn, WR);
+      // (the unit's last rows may be of another turn)
+      const int kv1 = a.causal ? min(end, pos0 + (f0 + rows - 1) / G + 1) : end;
+      const int n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
+      const int first_row = 32 * (PAIRS ? wave >> 1 : wave), mine = first_row + c;
+      const bool live = mine < rows;
+      const int t = live ? (f0 + mine) / G : 0, head = h * G + (live ? f0 + mine - t * G : 0);
+      half8_v qf[KS];
+      float mult;
+      auto read_queries = [&]() {
+        const uint16_t *src = a.q + (int64_t)(q0 + t) * a.q_stride + head * a.q_head_stride + 8 * hl;
+        u32x4_v w[KS];
 #pragma unroll
-      for (int s = 0; s < KS; s++) w[s] = live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0};
-      float unit = 1.f;
-      if (a.dtype == SQ_BF16) {
-        float most = 0, shift;
+        for (int s = 0; s < KS; s++) w[s] = live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0};
+        float unit = 1.f;
+        if (a.dtype == SQ_BF16) {
+          float most = 0, shift;
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+          for (int s = 0; s < KS; s++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][i])), fabsf(bf_hi(w[s][i]))));
-        row_shift(reduce_max2(most), &shift, &unit);
+            for (int i = 0; i < 4; i++) most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][i])), fabsf(bf_hi(w[s][i]))));
+          row_shift(reduce_max2(most), &shift, &unit);
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+          for (int s = 0; s < KS; s++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) w[s][i] = f16_bits(bf_lo(w[s][i]) * shift) | f16_bits(bf_hi(w[s][i]) * shift) << 16;
+            for (int i = 0; i < 4; i++)
+              w[s][i] = f16_bits(bf_lo(w[s][i]) * shift) | f16_bits(bf_hi(w[s][i]) * shift) << 16;
+        }
+        // scores keep their order when they are scaled: the sign goes to the query
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s] ^ flip);
+        mult = fabsf(a.scale) * 1.4426950408889634f * unit * kKeyUnit<FP8>;
+      };
+      // what the row sees, and what every row of the wave sees whole
+      const int hi = live && a.causal ? min(kv1, pos0 + t + 1) : kv1;
+      const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
+      const int all_hi = min(kv1, a.causal ? pos0 + (f0 + first_row) / G + 1 : kv1);
+      const int all_lo = a.window > 0 ? pos0 + (f0 + max(1, min(rows, first_row + 32)) - 1) / G - a.window + 1 : 0;
+      f32x16_v o[OT], s[ST];
+      half8_v pf[2 * ST];
+#pragma unroll
+      for (int e = 0; e < OT; e++)
+#pragma unroll
+        for (int k = 0; k < 16; k++) o[e][k] = 0.f;
+      float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
+      float om = -INFINITY, oref = 0.f;  // (pairs) what the outputs are in units of
+
+      // The tiles in order; past the last one the last again, so that loads ahead
+      // need no branch.  A page's number is loaded two tiles before it is used.
+      const int block = tile0 / per;
+      int sub = tile0 - block * per, left = n, id = 0, id2 = 0, ahead = block, ahead_sub = sub, ahead_left = n;
+      auto next_id = [&]() {
+        ahead_left--;
+        const bool more = ahead_left > 0, turned = ahead_sub + 1 == per;
+        ahead_sub = more ? turned ? 0 : ahead_sub + 1 : ahead_sub;
+        ahead = __builtin_amdgcn_readfirstlane(ahead + (more && turned));
+        return entries[ahead];
+      };
+      if (n > 0) {
+        id = entries[block];
+        id2 = next_id();
       }
-      // scores keep their order when they are scaled: the sign goes to the query
-      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+      bool known;
+      const uint8_t *base;  // of the page of the tile
+      auto next_tile = [&]() {
+        const int page = __builtin_amdgcn_readfirstlane(id);
+        known = page > 0 && page < pages;
+        base = a.c.data + (uint64_t)(uint32_t)(known ? page : 0) * page_bytes;
+        const uint8_t *at = base + first_key + sub * (kTile * D);
+        left--;
+        const bool more = left > 0, turned = sub + 1 == per;
+        sub = more ? turned ? 0 : sub + 1 : sub;
+        id = id2;
+        id2 = next_id();
+        return at;
+      };
+      u32x4_v ck[KN], ck0[KN];
+      Bytes<D / 32> cv[4];
+      auto load_keys = [&](u32x4_v *ck, const uint8_t *at) {
+        if (KS >= 8 || wave < KS)
 #pragma unroll
-      for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s] ^ flip);
-      mult = fabsf(a.scale) * 1.4426950408889634f * unit * kKeyUnit<FP8>;
-    };
-    // what the row sees, and what every row of the wave sees whole
-    const int hi = live && a.causal ? min(kv1, pos0 + t + 1) : kv1;
-    const int lo = live && a.window > 0 ? pos0 + t - a.window + 1 : 0;
-    const int all_hi = min(kv1, a.causal ? pos0 + (f0 + first_row) / G + 1 : kv1);
-    const int all_lo = a.window > 0 ? pos0 + (f0 + max(1, min(rows, first_row + 32)) - 1) / G - a.window + 1 : 0;
-    f32x16_v o[OT], s[ST];
-    half8_v pf[2 * ST];
+          for (int k = 0; k < KN; k++) ck[k] = *(const u32x4_v *)(at + 16 * (tid + 512 * k));
+      };
+      const int vtoken = 16 * (wave >> 1) + 8 * hl + 4 * (wave & 1);
+      auto load_values = [&](const uint8_t *at) {
 #pragma unroll
-    for (int e = 0; e < OT; e++)
+        for (int k = 0; k < 4; k++) cv[k] = *(const Bytes<D / 32> *)(at + (int64_t)P * D + (vtoken + k) * D + c * DT);
+      };
+      // keys: [32 tokens][16 dims][half of them][token] of eight dims; steps lie
+      // 65 groups apart, so that a wave's writes, 8 of a token's, fall on
+      // different banks
+      auto put_keys = [&](const u32x4_v *ck, uint4 *dst) {
+        if (KS >= 8 || wave < KS)
 #pragma unroll
-      for (int k = 0; k < 16; k++) o[e][k] = 0.f;
-    float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
-    float om = -INFINITY, oref = 0.f;  // (pairs) what the outputs are in units of
-
-    // The tiles in order; past the last one the last again, so that loads ahead
-    // need no branch.  A page's number is loaded two tiles before it is used.
-    const int block = tile0 / per;
-    int sub = tile0 - block * per, left = n, id = 0, id2 = 0, ahead = block, ahead_sub = sub, ahead_left = n;
-    auto next_id = [&]() {
-      ahead_left--;
-      const bool more = ahead_left > 0, turned = ahead_sub + 1 == per;
-      ahead_sub = more ? turned ? 0 : ahead_sub + 1 : ahead_sub;
-      ahead = __builtin_amdgcn_readfirstlane(ahead + (more && turned));
-      return entries[ahead];
-    };
-    if (n > 0) {
-      id = entries[block];
-      id2 = next_id();
-    }
-    bool known;
-    const uint8_t *base;  // of the page of the tile
-    auto next_tile = [&]() {
-      const int page = __builtin_amdgcn_readfirstlane(id);
-      known = page > 0 && page < pages;
-      base = a.c.data + (uint64_t)(uint32_t)(known ? page : 0) * page_bytes;
-      const uint8_t *at = base + first_key + sub * (kTile * D);
-      left--;
-      const bool more = left > 0, turned = sub + 1 == per;
-      sub = more ? turned ? 0 : sub + 1 : sub;
-      id = id2;
-      id2 = next_id();
-      return at;
-    };
-    u32x4_v ck[KN], ck0[KN];
-    Bytes<D / 32> cv[4];
-    auto load_keys = [&](u32x4_v *ck, const uint8_t *at) {
-      if (KS >= 8 || wave < KS)
+          for (int k = 0; k < KN; k++) {
+            const int i = tid + 512 * k, token = i / KS, st = i % KS;
+            uint4 *at = dst + ((token >> 5) * KS + st) * KF + (token & 31);
 #pragma unroll
-        for (int k = 0; k < KN; k++) ck[k] = *(const u32x4_v *)(at + 16 * (tid + 512 * k));
-    };
-    const int vtoken = 16 * (wave >> 1) + 8 * hl + 4 * (wave & 1);
-    auto load_values = [&](const uint8_t *at) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) cv[k] = *(const Bytes<D / 32> *)(at + (int64_t)P * D + (vtoken + k) * D + c * DT);
-    };
-    // keys: [32 tokens][16 dims][half of them][token] of eight dims; steps lie
-    // 65 groups apart, so that a wave's writes, 8 of a token's, fall on
-    // different banks
-    auto put_keys = [&](const u32x4_v *ck, uint4 *dst) {
-      if (KS >= 8 || wave < KS)
-#pragma unroll
-        for (int k = 0; k < KN; k++) {
-          const int i = tid + 512 * k, token = i / KS, st = i % KS;
-          uint4 *at = dst + ((token >> 5) * KS + st) * KF + (token & 31);
-#pragma unroll
-          for (int b = 0; b < 2; b++) {
-            const uint32_t w0 = ck[k][2 * b], w1 = ck[k][2 * b + 1];
-            at[32 * b] = make_uint4(key2<FP8, 0>(w0), key2<FP8, 1>(w0), key2<FP8, 0>(w1), key2<FP8, 1>(w1));
+            for (int b = 0; b < 2; b++) {
+              const uint32_t w0 = ck[k][2 * b], w1 = ck[k][2 * b + 1];
+              at[32 * b] = make_uint4(key2<FP8, 0>(w0), key2<FP8, 1>(w0), key2<FP8, 0>(w1), key2<FP8, 1>(w1));
+            }
           }
-        }
-    };
-    // values: [dim tile e][16 tokens][half][r] of the eight tokens of a
-    // product's lane, for dim r D / 32 + e
-    auto put_values = [&](uint4 *dst) {
-      uint2 *at = (uint2 *)(dst + ((wave >> 1) * 64 + 32 * (wave & 1) + c)) + hl;
-      auto one = [&](auto E) {
-        constexpr int e = decltype(E)::value;
-        uint32_t b[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) b[k] = cv[k].word(e / 4);
-        at[512 * e] = make_uint2(value2<FP8, e & 3>(b[0], b[1]), value2<FP8, e & 3>(b[2], b[3]));
       };
-      each(one, std::make_integer_sequence<int, DT>{});
-    };
-    // Outputs with one tile's values (with VALUES), then scores with another
-    // one's keys; the operands are read DEEP products ahead.
-    auto products = [&](auto VALUES, const uint4 *values, const uint4 *keys) {
-      constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + ST * KS, DEEP = 8;
-      half8_v pv[4];
-      if constexpr (!PAIRS) {
+      // values: [dim tile e][16 tokens][half][r] of the eight tokens of a
+      // product's lane, for dim r D / 32 + e
+      auto put_values = [&](uint4 *dst) {
+        uint2 *at = (uint2 *)(dst + ((wave >> 1) * 64 + 32 * (wave & 1) + c)) + hl;
+        auto one = [&](auto E) {
+          constexpr int e = decltype(E)::value;
+          uint32_t b[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) pv[j] = pf[j];
-      } else if constexpr (NV > 0) {
-        // own probabilities and the other wave's, brought to one maximum: maxima
-        // are whole numbers here, so that the factors are powers of two
-        const uint4 w0 = taken[lane], w1 = taken[64 + lane];
-        const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
-        pv[0] = pf[0], pv[1] = pf[1];
-        pv[2] = __builtin_bit_cast(half8_v, w0), pv[3] = __builtin_bit_cast(half8_v, w1);
-        if (__any(m != theirs)) {
-          const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(m - base), f1 = (_Float16)__builtin_amdgcn_exp2f(theirs - base);
-          pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
-        }
-        if (__any(high > om || ref > oref)) {
-          float shrink = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - high);
-          if (ref > oref) shrink *= oref / ref;
-          om = high, oref = ref;
-#pragma unroll
-          for (int e = 0; e < OT; e++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) o[e][k] *= shrink;
-        }
-      }
-#pragma unroll
-      for (int tt = 0; tt < ST; tt++)
-#pragma unroll
-        for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
-      uint4 w[DEEP];
-      // (pairs: the wave's own half of the keys first)
-      const uint4 *const near = PAIRS ? values + (4 * e0 + 2 * side) * 64 + lane : values + lane;
-      const uint4 *const far = PAIRS ? values + (4 * e0 + 2 * (1 - side) - 2) * 64 + lane : near;
-      const uint4 *const key = keys + side * (KS * KF) + lane;
-      auto read = [&](int i) {
-        if (i < NV) return (i / OT < 2 ? near : far)[(4 * (i % OT) + i / OT) * 64];
-        return key[((i - NV) % ST * KS + (i - NV) / ST) * KF];
+          for (int k = 0; k < 4; k++) b[k] = cv[k].word(e / 4);
+          at[512 * e] = make_uint2(value2<FP8, e & 3>(b[0], b[1]), value2<FP8, e & 3>(b[2], b[3]));
+        };
+        each(one, std::make_integer_sequence<int, DT>{});
       };
-#pragma unroll
-      for (int i = 0; i < DEEP; i++) w[i] = read(i);
-#pragma unroll
-      for (int i = 0; i < N; i++) {
-        const half8_v x = __builtin_bit_cast(half8_v, w[i % DEEP]);
-        if (i < NV) o[i % OT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pv[i / OT], o[i % OT], 0, 0, 0);
-        else s[(i - NV) % ST] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - NV) / ST], s[(i - NV) % ST], 0, 0, 0);
-        if (i + DEEP < N) w[i % DEEP] = read(i + DEEP);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x100, DEEP, 0);  // LDS reads
-#pragma unroll
-      for (int i = 0; i < N - DEEP; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x8, DEEP, 0);
-    };
-    auto softmax = [&](int i) {
-      const float4 peak = peaks[i & 1];
-      const int first = kv0 + i * kTile;
-      const bool known = __builtin_amdgcn_readfirstlane(__float_as_uint(peak.z)) != 0;
-      bool some = true;
-      if (!(known && first + kTile <= all_hi && first >= all_lo)) {  // some row does not see all of the tile
-        const int mine = first + 32 * side + 4 * hl, above = known ? hi - mine : 0, below = lo - mine;
-#pragma unroll
-        for (int k = 0; k < 16 * ST; k++) {
-          const int j = 32 * (k >> 4) + 8 * (k >> 2 & 3) + (k & 3);
-          // all ones where below <= j < above; as conditions, 64 of them would
-          // spill the loop's scalar registers
-          int seen = ((j - above) & (below - 1 - j)) >> 31;
-          asm("" : "+v"(seen));
-          const float x = s[k >> 4][k & 15];
-          s[k >> 4][k & 15] = __uint_as_float((__float_as_uint(x) & seen) | (0xff800000u & ~seen));
-        }
-        some = known && first < hi && first + kTile > lo;
-      }
-      float best = s[0][0];
-#pragma unroll
-      for (int k = 1; k < 16 * ST; k++) best = fmaxf(best, s[k >> 4][k & 15]);
-      best = reduce_max2(best);
-      // a tile that the row does not see takes no part in it, whatever its
-      // peaks; a factor of 0 would make NaN of the scores that are masked
-      float f = mult * peak.x;
-      f = !some ? 1.f : f == 0.f ? 1e-37f : f;
-      best *= f;
-      const float high = some ? fmaxf(ref, peak.y) : ref;
-      if (__any(best > m + 8.f || high > ref)) {
-        const float raised = fmaxf(m, PAIRS ? ceilf(best) : best);
-        const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
-        const float shrink = high > ref ? ref / high * was : was;
-        m = raised;
-        ref = high;
-        log_ref = ref > 0.f ? __builtin_amdgcn_logf(ref) : 0.f;
-        l *= was;
+      // Outputs with one tile's values (with VALUES), then scores with another
+      // one's keys; the operands are read DEEP products ahead.
+      auto products = [&](auto VALUES, const uint4 *values, const uint4 *keys) {
+        constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + ST * KS, DEEP = 8;
+        half8_v pv[4];
         if constexpr (!PAIRS) {
 #pragma unroll
-          for (int e = 0; e < OT; e++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) o[e][k] *= shrink;
-        }
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      const float size = some ? __builtin_amdgcn_logf(peak.y) - log_ref : 0.f;
-      const float off = size - base;
-      float sum = 0;
-#pragma unroll
-      for (int j = 0; j < 2 * ST; j++) {
-        u32x4_v w;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          float p[2];
-#pragma unroll
-          for (int b = 0; b < 2; b++) {
-            const int at = 8 * j + 2 * k + b;
-            p[b] = __builtin_amdgcn_exp2f(fmaf(s[at >> 4][at & 15], f, off));
+          for (int j = 0; j < 4; j++) pv[j] = pf[j];
+        } else if constexpr (NV > 0) {
+          // own probabilities and the other wave's, brought to one maximum: maxima
+          // are whole numbers here, so that the factors are powers of two
+          const uint4 w0 = taken[lane], w1 = taken[64 + lane];
+          const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
+          pv[0] = pf[0], pv[1] = pf[1];
+          pv[2] = __builtin_bit_cast(half8_v, w0), pv[3] = __builtin_bit_cast(half8_v, w1);
+          if (__any(m != theirs)) {
+            const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(m - base);
+            const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(theirs - base);
+            pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
           }
-          w[k] = weigh2(p[0], p[1], sum);
+          if (__any(high > om || ref > oref)) {
+            float shrink = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - high);
+            if (ref > oref) shrink *= oref / ref;
+            om = high, oref = ref;
+#pragma unroll
+            for (int e = 0; e < OT; e++)
+#pragma unroll
+              for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+          }
         }
-        pf[j] = __builtin_bit_cast(half8_v, w);
-      }
-      l = fmaf(sum, __builtin_amdgcn_exp2f(-size), l);
-      if constexpr (PAIRS) {
-        passed[lane] = __builtin_bit_cast(uint4, pf[0]);
-        passed[64 + lane] = __builtin_bit_cast(uint4, pf[1]);
-        if (hl == 0) passed_m[c] = m;
-      }
-    };
+#pragma unroll
+        for (int tt = 0; tt < ST; tt++)
+#pragma unroll
+          for (int k = 0; k < 16; k++) s[tt][k] = 0.f;
+        uint4 w[DEEP];
+        // (pairs: the wave's own half of the keys first)
+        const uint4 *const near = PAIRS ? values + (4 * e0 + 2 * side) * 64 + lane : values + lane;
+        const uint4 *const far = PAIRS ? values + (4 * e0 + 2 * (1 - side) - 2) * 64 + lane : near;
+        const uint4 *const key = keys + side * (KS * KF) + lane;
+        auto read = [&](int i) {
+          if (i < NV) return (i / OT < 2 ? near : far)[(4 * (i % OT) + i / OT) * 64];
+          return key[((i - NV) % ST * KS + (i - NV) / ST) * KF];
+        };
+#pragma unroll
+        for (int i = 0; i < DEEP; i++) w[i] = read(i);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          const half8_v x = __builtin_bit_cast(half8_v, w[i % DEEP]);
+          if (i < NV) o[i % OT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pv[i / OT], o[i % OT], 0, 0, 0);
+          else
+            s[(i - NV) % ST] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[(i - NV) / ST], s[(i - NV) % ST], 0, 0, 0);
+          if (i + DEEP < N) w[i % DEEP] = read(i + DEEP);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, DEEP, 0);  // LDS reads
+#pragma unroll
+        for (int i = 0; i < N - DEEP; i++) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, DEEP, 0);
+      };
+      auto softmax = [&](int i) {
+        const float4 peak = peaks[i & 1];
+        const int first = kv0 + i * kTile;
+        const bool known = __builtin_amdgcn_readfirstlane(__float_as_uint(peak.z)) != 0;
+        bool some = true;
+        if (!(known && first + kTile <= all_hi && first >= all_lo)) {  // some row does not see all of the tile
+          const int mine = first + 32 * side + 4 * hl, above = known ? hi - mine : 0, below = lo - mine;
+#pragma unroll
+          for (int k = 0; k < 16 * ST; k++) {
+            const int j = 32 * (k >> 4) + 8 * (k >> 2 & 3) + (k & 3);
+            // all ones where below <= j < above; as conditions, 64 of them would
+            // spill the loop's scalar registers
+            int seen = ((j - above) & (below - 1 - j)) >> 31;
+            asm("" : "+v"(seen));
+            const float x = s[k >> 4][k & 15];
+            s[k >> 4][k & 15] = __uint_as_float((__float_as_uint(x) & seen) | (0xff800000u & ~seen));
+          }
+          some = known && first < hi && first + kTile > lo;
+        }
+        float best = s[0][0];
+#pragma unroll
+        for (int k = 1; k < 16 * ST; k++) best = fmaxf(best, s[k >> 4][k & 15]);
+        best = reduce_max2(best);
+        // a tile that the row does not see takes no part in it, whatever its
+        // peaks; a factor of 0 would make NaN of the scores that are masked
+        float f = mult * peak.x;
+        f = !some ? 1.f : f == 0.f ? 1e-37f : f;
+        best *= f;
+        const float high = some ? fmaxf(ref, peak.y) : ref;
+        if (__any(best > m + 8.f || high > ref)) {
+          const float raised = fmaxf(m, PAIRS ? ceilf(best) : best);
+          const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
+          const float shrink = high > ref ? ref / high * was : was;
+          m = raised;
+          ref = high;
+          log_ref = ref > 0.f ? __builtin_amdgcn_logf(ref) : 0.f;
+          l *= was;
+          if constexpr (!PAIRS) {
+#pragma unroll
+            for (int e = 0; e < OT; e++)
+#pragma unroll
+              for (int k = 0; k < 16; k++) o[e][k] *= shrink;
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        const float size = some ? __builtin_amdgcn_logf(peak.y) - log_ref : 0.f;
+        const float off = size - base;
+        float sum = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * ST; j++) {
+          u32x4_v w;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            float p[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+              const int at = 8 * j + 2 * k + b;
+              p[b] = __builtin_amdgcn_exp2f(fmaf(s[at >> 4][at & 15], f, off));
+            }
+            w[k] = weigh2(p[0], p[1], sum);
+          }
+          pf[j] = __builtin_bit_cast(half8_v, w);
+        }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-size), l);
+        if constexpr (PAIRS) {
+          passed[lane] = __builtin_bit_cast(uint4, pf[0]);
+          passed[64 + lane] = __builtin_bit_cast(uint4, pf[1]);
+          if (hl == 0) passed_m[c] = m;
+        }
+      };
 
-    float4 peak, peak0;
-    const uint8_t *at = nullptr, *keys = nullptr;
-    auto load_peak = [&]() {
-      const float2 x = *(const float2 *)(base + peaks_at);
-      peak = make_float4(x.x, x.y, known ? 1.f : 0.f, 0.f);
-    };
-    // the first tiles' loads go out before the queries', whose conversion they run under
-    if (n > 0) {
-      at = next_tile();
-      load_keys(ck0, at);
-      load_peak();
-      peak0 = peak;
-      load_values(at);
-      keys = next_tile();
-      load_keys(ck, keys);
-      load_peak();
-    }
-    read_queries();
-    if (n > 0) {
-      // Step j of the loop needs values j and keys j + 1.  The early waves put
-      // their share of them there in step j, the late ones, whose step j begins
-      // half a step later, in step j - 1.
-      put_keys(ck0, kb);
-      if (tid == 0) peaks[0] = peak0;
-      auto load = [&](const uint8_t *values, const uint8_t *keys) {
-        load_values(values);
+      float4 peak, peak0;
+      const uint8_t *at = nullptr, *keys = nullptr;
+      auto load_peak = [&]() {
+        const float2 x = *(const float2 *)(base + peaks_at);
+        peak = make_float4(x.x, x.y, known ? 1.f : 0.f, 0.f);
+      };
+      // the first tiles' loads go out before the queries', whose conversion they run under
+      if (n > 0) {
+        at = next_tile();
+        load_keys(ck0, at);
+        load_peak();
+        peak0 = peak;
+        load_values(at);
+        keys = next_tile();
         load_keys(ck, keys);
         load_peak();
-      };
-      if (late) {
-        put_values(vb);
-        put_keys(ck, kb + KB);
-        at = keys;
-        keys = next_tile();
-        load(at, keys);
       }
-      __syncthreads();
-      if (late) __syncthreads();
-      products(std::false_type{}, vb, kb);
-      __syncthreads();
-      for (int i = 0; i < n; i++) {
-        softmax(i);
-        // (past the last tile: into buffers that nothing reads)
-        put_values(vb + ((i + late) & 1) * VB);
-        put_keys(ck, kb + ((i + late + 1) & 1) * KB);
-        if (tid == 0) peaks[(i + 1) & 1] = peak;
-        at = keys;
-        keys = next_tile();
-        load(at, keys);
+      read_queries();
+      if (n > 0) {
+        // Step j of the loop needs values j and keys j + 1.  The early waves put
+        // their share of them there in step j, the late ones, whose step j begins
+        // half a step later, in step j - 1.
+        put_keys(ck0, kb);
+        if (tid == 0) peaks[0] = peak0;
+        auto load = [&](const uint8_t *values, const uint8_t *keys) {
+          load_values(values);
+          load_keys(ck, keys);
+          load_peak();
+        };
+        if (late) {
+          put_values(vb);
+          put_keys(ck, kb + KB);
+          at = keys;
+          keys = next_tile();
+          load(at, keys);
+        }
         __syncthreads();
-        __builtin_amdgcn_sched_barrier(0);
-        products(std::true_type{}, vb + (i & 1) * VB, kb + ((i + 1) & 1) * KB);
-        __builtin_amdgcn_sched_barrier(0);
+        if (late) __syncthreads();
+        products(std::false_type{}, vb, kb);
         __syncthreads();
+        for (int i = 0; i < n; i++) {
+          softmax(i);
+          // (past the last tile: into buffers that nothing reads)
+          put_values(vb + ((i + late) & 1) * VB);
+          put_keys(ck, kb + ((i + late + 1) & 1) * KB);
+          if (tid == 0) peaks[(i + 1) & 1] = peak;
+          at = keys;
+          keys = next_tile();
+          load(at, keys);
+          __syncthreads();
+          __builtin_amdgcn_sched_barrier(0);
+          products(std::true_type{}, vb + (i & 1) * VB, kb + ((i + 1) & 1) * KB);
+          __builtin_amdgcn_sched_barrier(0);
+          __syncthreads();
+        }
+        if (!late) __syncthreads();
+        __syncthreads();  // the next turn writes where the last products read
       }
-      if (!late) __syncthreads();
-      __syncthreads();  // the next turn writes where the last products read
-    }
-    l = reduce_sum2(l);
-    if constexpr (PAIRS) {
-      // the two waves' sums, brought to one maximum (their last products are done)
-      if (hl == 0) {
-        passed_m[c] = m;
-        ((float *)passed)[c] = l;
-      }
-      __syncthreads();
-      const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
-      l = fmaf(l, __builtin_amdgcn_exp2f(m - base), ((float *)taken)[c] * __builtin_amdgcn_exp2f(theirs - base));
-      m = high;
-      __syncthreads();
-    }
-    const float unit = ref * kValueUnit<FP8>;
-    if (part < 0) {
-      // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
-      constexpr int OD = 32 * OT, OW = OD * 2 + 8;  // a wave's dims of a row, and the bytes from row to row
-      const float f = l == 0.f ? 0.f : unit / l;
-      uint8_t *rows_at = (uint8_t *)tiles + wave * (32 * OW);
-#pragma unroll
-      for (int k = 0; k < 16; k++) {
-        float x[OT];
-#pragma unroll
-        for (int e = 0; e < OT; e++) x[e] = o[e][k] * f;
-        store_row<OT>((uint16_t *)(rows_at + c * OW) + (8 * (k >> 2) + 4 * hl + (k & 3)) * OT, a.dtype == SQ_BF16, x);
-      }
-      __builtin_amdgcn_wave_barrier();
+      l = reduce_sum2(l);
       if constexpr (PAIRS) {
-        // the wave's dims are every other group of four: 8 bytes a lane
-        constexpr int LANES = OD / 4;
-#pragma unroll
-        for (int i = 0; i < 32 * LANES / 64; i++) {
-          const int r = (64 * i + lane) / LANES, d = (64 * i + lane) % LANES, f = f0 + first_row + r;
-          if (first_row + r < rows)
-            *(uint2 *)(a.out + ((int64_t)(q0 + f / G) * a.q_heads + h * G + f % G) * D + 8 * d + e0) =
-                *(const uint2 *)(rows_at + r * OW + 8 * d);
+        // the two waves' sums, brought to one maximum (their last products are done)
+        if (hl == 0) {
+          passed_m[c] = m;
+          ((float *)passed)[c] = l;
         }
+        __syncthreads();
+        const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
+        l = fmaf(l, __builtin_amdgcn_exp2f(m - base), ((float *)taken)[c] * __builtin_amdgcn_exp2f(theirs - base));
+        m = high;
+        __syncthreads();
+      }
+      const float unit = ref * kValueUnit<FP8>;
+      if (part < 0) {
+        // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
+        constexpr int OD = 32 * OT, OW = OD * 2 + 8;  // a wave's dims of a row, and the bytes from row to row
+        const float f = l == 0.f ? 0.f : unit / l;
+        uint8_t *rows_at = (uint8_t *)tiles + wave * (32 * OW);
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+          float x[OT];
+#pragma unroll
+          for (int e = 0; e < OT; e++) x[e] = o[e][k] * f;
+          store_row<OT>((uint16_t *)(rows_at + c * OW) + (8 * (k >> 2) + 4 * hl + (k & 3)) * OT, a.dtype == SQ_BF16, x);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (PAIRS) {
+          // the wave's dims are every other group of four: 8 bytes a lane
+          constexpr int LANES = OD / 4;
+#pragma unroll
+          for (int i = 0; i < 32 * LANES / 64; i++) {
+            const int r = (64 * i + lane) / LANES, d = (64 * i + lane) % LANES, f = f0 + first_row + r;
+            if (first_row + r < rows)
+              *(uint2 *)(a.out + ((int64_t)(q0 + f / G) * a.q_heads + h * G + f % G) * D + 8 * d + e0) =
+                  *(const uint2 *)(rows_at + r * OW + 8 * d);
+          }
+        } else {
+          constexpr int LANES = OD / 8;
+#pragma unroll
+          for (int i = 0; i < 32 * LANES / 64; i++) {
+            const int r = (64 * i + lane) / LANES, d = (64 * i + lane) % LANES, f = f0 + first_row + r;
+            const uint2 *src = (const uint2 *)(rows_at + r * OW + 16 * d);  // (rows lie 8 bytes off a multiple of 16)
+            const uint2 x0 = src[0], x1 = src[1];
+            if (first_row + r < rows)
+              *(uint4 *)(a.out + ((int64_t)(q0 + f / G) * a.q_heads + h * G + f % G) * D + 8 * d) =
+                  make_uint4(x0.x, x0.y, x1.x, x1.y);
+          }
+        }
+        __syncthreads();  // before the next unit's tiles
       } else {
-        constexpr int LANES = OD / 8;
+        // as the registers hold them: a wave writes 64 OT floats in a row
+        typedef float vec __attribute__((ext_vector_type(OT)));
+        const int64_t slot = (int64_t)part * a.kv_heads + h;
+        float *dst = a.ws + ((slot * (PAIRS ? 16 : 8) + turn / WR * 8 + wave) * (16 * 64) + lane) * OT;
 #pragma unroll
-        for (int i = 0; i < 32 * LANES / 64; i++) {
-          const int r = (64 * i + lane) / LANES, d = (64 * i + lane) % LANES, f = f0 + first_row + r;
-          const uint2 *src = (const uint2 *)(rows_at + r * OW + 16 * d);  // (rows lie 8 bytes off a multiple of 16)
-          const uint2 x0 = src[0], x1 = src[1];
-          if (first_row + r < rows)
-            *(uint4 *)(a.out + ((int64_t)(q0 + f / G) * a.q_heads + h * G + f % G) * D + 8 * d) =
-                make_uint4(x0.x, x0.y, x1.x, x1.y);
+        for (int k = 0; k < 16; k++) {
+          vec x;
+#pragma unroll
+          for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit;
+          *(vec *)(dst + k * 64 * OT) = x;
         }
-      }
-      __syncthreads();  // before the next unit's tiles
-    } else {
-      // as the registers hold them: a wave writes 64 OT floats in a row
-      typedef float vec __attribute__((ext_vector_type(OT)));
-      const int64_t slot = (int64_t)part * a.kv_heads + h;
-      float *dst = a.ws + ((slot * (PAIRS ? 16 : 8) + turn / WR * 8 + wave) * (16 * 64) + lane) * OT;
-#pragma unroll
-      for (int k = 0; k < 16; k++) {
-        vec x;
-#pragma unroll
-        for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit;
-        *(vec *)(dst + k * 64 * OT) = x;
-      }
-      if (live && hl == 0 && e0 == 0) {
-        float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * (slot * a.unit_rows + turn + mine);
-        ml[0] = m;
-        ml[1] = l;
+        if (live && hl == 0 && e0 == 0) {
+          float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D;
+          ml += 2 * (slot * a.unit_rows + turn + mine);
+          ml[0] = m;
+          ml[1] = l;
+        }
       }
     }
-  }
   }
 }
 
@@ -1501,7 +1514,8 @@ __global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
   const int h = blockIdx.x % a.kv_heads, wave = blockIdx.y & 7, turn = blockIdx.y >> 3;
   const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.kv_heads);
   const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
-  const int tid = threadIdx.x & 255, half = threadIdx.x >> 8, lane = tid & 63, c = lane & 31, hl = lane >> 5, k0 = tid >> 6;
+  const int tid = threadIdx.x & 255, half = threadIdx.x >> 8, k0 = tid >> 6;
+  const int lane = tid & 63, c = lane & 31, hl = lane >> 5;
   const int e0 = D == 256 ? (wave & 1) * OT : 0;
   const int first = D == 256 ? 128 * turn + 32 * (wave >> 1) : 32 * wave, j = first + c;
   if (first >= rows) return;
@@ -1589,10 +1603,12 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
   if (tokens * G > 0x3fffffff) return fail(SQ_EINVAL, "kv schedule: tokens * heads of a group too large");
   const int64_t sets = (tokens * G + s->rows - 1) / s->rows + batch + 1;
   const int64_t slots = s->slots / s->kv_heads > 1 ? s->slots / s->kv_heads : 1;
-  if (s->max_workers < (sets > slots ? sets : slots) || s->max_units < sets + slots || s->max_merges < (sets < slots ? sets : slots) ||
+  const int64_t larger = sets > slots ? sets : slots, smaller = sets < slots ? sets : slots;
+  if (s->max_workers < larger || s->max_units < sets + slots || s->max_merges < smaller ||
       s->max_partials < 2 * slots || s->max_units >= 1 << 24)
     return fail(SQ_EINVAL, "kv schedule: room for workers, units, merges or partials");
-  if ((int64_t)s->max_workers * s->kv_heads > 0x7fffffff || (int64_t)s->max_merges * s->kv_heads > 0x7fffffff)
+  // (a launch has fewer than 2^32 threads, 512 a workgroup)
+  if ((int64_t)s->max_workers * s->kv_heads >= 1 << 23 || (int64_t)s->max_merges * s->kv_heads >= 1 << 23)
     return fail(SQ_EINVAL, "kv schedule: workers * heads too large");
   return 0;
 }
@@ -1603,14 +1619,16 @@ int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
   if (!p || !p->rows || !p->counts || !p->cu || !p->slots || !p->positions || !p->lens || !p->granted || !p->pages ||
       !p->filled || !p->tiles || !p->counters)
     return fail(SQ_EINVAL, "kv plan: null pointer");
-  if (!index_type(p->rows_dtype) || !index_type(p->counts_dtype)) return fail(SQ_EINVAL, "kv plan: rows and counts are int32 or int64");
+  if (!index_type(p->rows_dtype) || !index_type(p->counts_dtype))
+    return fail(SQ_EINVAL, "kv plan: rows and counts are int32 or int64");
   if (p->batch <= 0 || p->batch > SQ_KV_MAX_REQUESTS) return fail(SQ_EINVAL, "kv plan: batch must be in [1, 4096]");
   if (p->max_count < 0) return fail(SQ_EINVAL, "kv plan: negative max_count");
   if (p->tokens < 0 || p->tokens > 0x3fffffff) return fail(SQ_EINVAL, "kv plan: tokens must be in [0, 2^30)");
   int64_t tiles = p->tokens / t->page_tokens + 2 * (int64_t)p->batch;
   if (tiles > p->tokens) tiles = p->tokens;
   if (p->max_tiles < tiles) return fail(SQ_EINVAL, "kv plan: room for page entries");
-  if (p->n_schedules < 0 || p->n_schedules > SQ_KV_MAX_SCHEDULES) return fail(SQ_EINVAL, "kv plan: number of schedules");
+  if (p->n_schedules < 0 || p->n_schedules > SQ_KV_MAX_SCHEDULES)
+    return fail(SQ_EINVAL, "kv plan: number of schedules");
   for (int i = 0; i < p->n_schedules; i++) {
     const sq_kv_schedule &s = p->schedules[i];
     const int e = check_schedule(&s, p->tokens, p->batch);
@@ -1645,18 +1663,21 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
   auto go = [&](auto kernel, int id, int threads, size_t lds, int turns = 1) {
     const int rc = dynamic_lds((const void *)kernel, 2 * id + FP8, lds, "kv attend: LDS attribute");
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.max_workers * s.kv_heads), (unsigned)turns), dim3(threads), lds, st, d);
+    const dim3 grid((unsigned)(s.max_workers * s.kv_heads), (unsigned)turns);
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
   static_assert(D <= 256, "ids of kernels with more than 64 KiB");
   constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float);
-  // tiles and peaks; the outputs' way out
-  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 128) : 0), rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
+  // tiles, peaks, and what the pairs of waves share; the outputs' way out
+  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 128) : 0);
+  constexpr size_t rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
   constexpr size_t many = staged > rows_out ? staged : rows_out;
   int rc;
   if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
   // 32 rows of 256 dims do not fit a wave's registers twice on a SIMD: they go to two workgroups
-  else if constexpr (D == 256) rc = s.rows == 32 ? go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined, 2) : go(kv_attend_rows_kernel<D, FP8>, 3, 512, many);
+  else if constexpr (D == 256)
+    rc = s.rows == 32 ? go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined, 2) : go(kv_attend_rows_kernel<D, FP8>, 3, 512, many);
   else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
   else rc = go(kv_attend_rows_kernel<D, FP8>, 4, 512, many);
   if (rc) return rc;
@@ -1678,7 +1699,8 @@ int sq_kv_plan(const sq_kv_tables *t, const sq_kv_plan_args *p, void *stream) {
   d.share_blocks = (int)((share + kPlanShare - 1) / kPlanShare);
   if (d.share_blocks < 1) d.share_blocks = 1;
   const size_t lds = 5 * sizeof(int32_t) * (size_t)(p->batch + 1);
-  const int e = dynamic_lds((const void *)kv_plan_kernel, 0, 5 * sizeof(int32_t) * (SQ_KV_MAX_REQUESTS + 1), "kv plan: LDS attribute");
+  const int e = dynamic_lds((const void *)kv_plan_kernel, 0, 5 * sizeof(int32_t) * (SQ_KV_MAX_REQUESTS + 1),
+                            "kv plan: LDS attribute");
   if (e) return e;
   hipLaunchKernelGGL(kv_plan_kernel, dim3((unsigned)(d.share_blocks + p->n_schedules)), dim3(kPlanThreads), lds,
                      (hipStream_t)stream, d);
@@ -1699,8 +1721,8 @@ int sq_kv_release(const sq_kv_tables *t, const void *rows, int32_t rows_dtype, i
   if (n == 0) return 0;
   if (!rows || !index_type(rows_dtype) || n < 0 || n > SQ_KV_MAX_REQUESTS)
     return fail(SQ_EINVAL, "kv release: rows must be int32 or int64, at most 4096 of them");
-  hipLaunchKernelGGL(kv_release_kernel, dim3(1), dim3(kPlanThreads), 2 * sizeof(int32_t) * (size_t)n, (hipStream_t)stream, *t,
-                     rows, rows_dtype, (int)n);
+  hipLaunchKernelGGL(kv_release_kernel, dim3(1), dim3(kPlanThreads), 2 * sizeof(int32_t) * (size_t)n, (hipStream_t)stream,
+                     *t, rows, rows_dtype, (int)n);
   return sq_internal_launched("kv_release_kernel");
 }
 
@@ -1709,7 +1731,8 @@ int sq_kv_append(const sq_kv_cache *c, const sq_kv_append_args *a, void *stream)
   if (rc) return rc;
   if (!a) return fail(SQ_EINVAL, "kv append: null arguments");
   if (a->max_tiles == 0) return 0;
-  if (!a->k || !a->v || !a->pages || !a->filled || !a->tiles || a->max_tiles < 0) return fail(SQ_EINVAL, "kv append: null pointer");
+  if (!a->k || !a->v || !a->pages || !a->filled || !a->tiles || a->max_tiles < 0)
+    return fail(SQ_EINVAL, "kv append: null pointer");
   if (a->dtype != SQ_BF16 && a->dtype != SQ_F16) return fail(SQ_EINVAL, "kv append: keys and values are bf16 or fp16");
   if ((a->k_stride | a->k_head_stride | a->v_stride | a->v_head_stride) & 7 || (((uintptr_t)a->k | (uintptr_t)a->v) & 15))
     return fail(SQ_EINVAL, "kv append: strides must be multiples of 8 and starts 16-byte aligned");
@@ -1733,8 +1756,9 @@ int sq_kv_decode(const sq_kv_cache *c, const int32_t *pages, const int32_t *fill
   const int rc = check_cache(c);
   if (rc) return rc;
   if (n == 0) return 0;
-  if (!pages || !k || !v || n < 0 || n > 0x7fffffff) return fail(SQ_EINVAL, "kv decode: null pointer or page count");
-  if (out_dtype != SQ_F32 && out_dtype != SQ_BF16 && out_dtype != SQ_F16) return fail(SQ_EINVAL, "kv decode: output dtype");
+  if (!pages || !k || !v || n < 0 || n >= 1 << 24) return fail(SQ_EINVAL, "kv decode: null pointer or page count");
+  if (out_dtype != SQ_F32 && out_dtype != SQ_BF16 && out_dtype != SQ_F16)
+    return fail(SQ_EINVAL, "kv decode: output dtype");
   const dim3 grid((unsigned)n, (unsigned)c->heads, 2);
   if (c->storage == SQ_KV_FP8)
     hipLaunchKernelGGL(kv_decode_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, *c, pages, filled, k, v, out_dtype,
@@ -1759,7 +1783,8 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(SQ_EINVAL, "kv attend: scale must be finite");
   rc = check_schedule(&a->schedule, a->tokens, 1);
   if (rc) return rc;
-  if (a->schedule.kv_heads != c->heads) return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads");
+  if (a->schedule.kv_heads != c->heads)
+    return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads");
   if (!a->workspace) return fail(SQ_EINVAL, "kv attend: null workspace");
   const sq_kv_schedule &s = a->schedule;
   const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges, s.starts,

@@ -352,6 +352,11 @@ CASES = [  # heads, KV heads, dim, page, storage, dtype, cached, new, padding, c
     (8, 2, 64, 64, "int8", "fp16", [300], [17], 0, True, 1),
     (4, 2, 128, 64, "int8", "bf16", [129, 0, 1], [30, 64, 2], 3, False, 0),
     (2, 2, 64, 256, "fp8", "bf16", [1025], [1], 0, False, 0),
+    (4, 1, 256, 64, "int8", "bf16", [500, 0], [40, 90], 1, True, 70),
+    (8, 2, 256, 64, "fp8", "bf16", [130, 1], [20, 50], 0, False, 0),
+    (32, 1, 256, 64, "int8", "fp16", [700, 31], [1, 1], 1, True, 0),
+    (3, 3, 128, 192, "int8", "bf16", [100], [37], 0, True, 0),
+    (40, 2, 128, 64, "fp8", "bf16", [257, 90], [1, 1], 0, True, 33),
 ]
 
 
@@ -394,6 +399,89 @@ def filled(old, new, Hq=8, H=2, D=128, P=64, storage="int8", seed=0, **kw):
     plan = tables.plan(new, heads=(Hq, H), **kw)
     cache.append(values(g, (plan.tokens, H, D), torch.bfloat16), values(g, (plan.tokens, H, D), torch.bfloat16), plan)
     return tables, cache, plan, values(g, (plan.tokens, Hq, D), torch.bfloat16)
+
+
+@pytest.mark.parametrize("Hq,H,D,storage,window", [(4, 2, 64, "int8", 0), (2, 1, 128, "fp8", 0), (8, 1, 64, "fp8", 50)])
+def test_many_requests_of_unequal_lengths(Hq, H, D, storage, window):
+    """More sets of rows than workgroups for them: shares with several sets, cut
+    at both ends."""
+    g = rng(Hq, H, D)
+    old = [int(x) for x in np.exp(g.uniform(0, np.log(900), 230))]
+    new = [int(x) for x in g.integers(1, 3, 230)]
+    print(f"case {Hq} over {H} heads of {D}, {sum(old)} tokens held", flush=True)
+    tables, cache, plan, q = filled(old, new, Hq=Hq, H=H, D=D, storage=storage, window=window)
+    check_attend(tables, cache, plan, list(range(230)), old, new, q, window=window)
+
+
+@pytest.mark.parametrize("Hq,H,D,old,new,causal", [(8, 1, 64, [0], [1100], True), (4, 2, 128, [900, 70], [333, 400], True),
+                                                   (2, 1, 256, [64], [520], False), (4, 1, 256, [333], [300], True)])
+def test_prompts_of_many_sets_of_rows(Hq, H, D, old, new, causal):
+    print(f"case {Hq} over {H} heads of {D}, {new} over {old}", flush=True)
+    tables, cache, plan, q = filled(old, new, Hq=Hq, H=H, D=D, causal=causal)
+    check_attend(tables, cache, plan, list(range(len(old))), old, new, q, causal=causal)
+
+
+@pytest.mark.parametrize("D,new", [(128, 1), (128, 5), (64, 40), (256, 30)])
+@pytest.mark.parametrize("scale", [-.1, 0., 3.])
+def test_scales_of_any_sign(D, new, scale):
+    old = [90]
+    tables, cache, plan, q = filled(old, [new], D=D, H=1, Hq=8)
+    out = cache.attend(q, plan, scale=scale)
+    codes, peaks = page_parts(cache)
+    parts = codes, peaks.astype(np.float64) / TOP["int8"]
+    x = q.double().cpu().numpy()
+    want, bound = attend_oracle(parts, tables.table.cpu().numpy()[0], 90 + new, 90, x, 0, new, scale, True, 0)
+    if scale <= 0:  # the oracle's bound takes the scale's size
+        bound = attend_oracle(parts, tables.table.cpu().numpy()[0], 90 + new, 90, x, 0, new, abs(scale), True, 0)[1]
+    err = np.abs(out.double().cpu().numpy() - want)
+    assert (err <= bound + np.abs(want) * 2. ** -8 * (1 + 2. ** -9) + 2. ** -25).all()
+
+
+def test_requests_come_and_go():
+    """Pages that were released serve other requests, whose blocks start afresh."""
+    g = rng(21)
+    tables, cache = BlockTables(4, 12, 6), KVCache(12, 2, 64)
+    held = [0, 0, 0, 0]
+    for step in range(14):
+        rows = g.permutation(4)[:int(g.integers(1, 5))].tolist()
+        new = [int(x) for x in g.integers(0, 120, len(rows))]
+        plan = tables.plan(new, rows, heads=(4, 2))
+        x = values(g, (plan.tokens, 2, 64), torch.bfloat16, 1.)
+        y = values(g, (plan.tokens, 2, 64), torch.bfloat16, 1.)
+        check_append(cache, x, y, plan)
+        ok = plan.granted.tolist()
+        q = values(g, (plan.tokens, 4, 64), torch.bfloat16)
+        out = cache.attend(q, plan)
+        at = 0
+        for r, n, good in zip(rows, new, ok):
+            if not good:
+                assert not out[at:at + n].any()
+            at += n
+        if all(ok) and plan.tokens:
+            check_attend(tables, cache, plan, rows, [held[r] for r in rows], new, q, out=out)
+        tables.commit(plan)
+        for r, n, good in zip(rows, new, ok):
+            held[r] += n if good else 0
+        assert tables.lens.tolist() == held
+        gone = [r for r in range(4) if held[r] and g.random() < (.9 if not all(ok) else .25)]
+        tables.release(gone) if gone else None
+        for r in gone:
+            held[r] = 0
+
+
+def test_rows_that_kernels_do_not_take_are_copied():
+    old, new = [100], [3]
+    tables, cache, plan, q = filled(old, new)
+    want = cache.attend(q, plan)
+    wide = torch.empty((3, 8, 130), dtype=q.dtype, device=dev())
+    wide[..., 1:129] = q
+    assert torch.equal(cache.attend(wide[..., 1:129], plan), want)
+    assert torch.equal(cache.attend(q.transpose(1, 2).contiguous().transpose(1, 2), plan), want)
+    k = values(rng(30), (3, 2, 128), torch.bfloat16)
+    cache.append(k, k, plan)
+    want = cache.data.clone()
+    cache.append(k.transpose(0, 1).contiguous().transpose(0, 1), k[:, :, :].clone().flatten(1), plan)
+    assert torch.equal(cache.data, want)
 
 
 def test_refused_requests_give_zero():
