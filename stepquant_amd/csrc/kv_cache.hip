@@ -1184,7 +1184,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       // Outputs with one tile's values (with VALUES), then scores with another
       // one's keys; the operands are read DEEP products ahead.
       auto products = [&](auto VALUES, const uint4 *values, const uint4 *keys) {
-        constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + ST * KS, DEEP = 8;
+        constexpr int NV = decltype(VALUES)::value ? 4 * OT : 0, N = NV + ST * KS, DEEP = 4;
         half8_v pv[4];
         if constexpr (!PAIRS) {
 #pragma unroll

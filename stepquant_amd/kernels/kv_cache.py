@@ -109,6 +109,7 @@ class BlockTables:
                                 free_pages=self.free.data_ptr(), counters=self.counters.data_ptr(),
                                 requests=requests, capacity=pages - 1, width=max_blocks, page_tokens=page_tokens)
         self._at = ctypes.addressof(self._desc)
+        self._layouts = {}
         self._cus = torch.cuda.get_device_properties(dev).multi_processor_count
 
     def _index(self, x, what):
@@ -161,62 +162,69 @@ class BlockTables:
             raise ValueError(f"a plan takes at most {N.KV_MAX_SCHEDULES} windows, each once")
         if any(windows) and not causal:
             raise ValueError("a window needs causal attention")
-        if heads is None:
-            windows = ()
-        else:
-            shape = self._shape(int(heads[0]), int(heads[1]), tokens, batch, max_new)
-            if not tokens:
-                windows = ()
-        most = min(tokens, tokens // self.page_tokens + 2 * batch)
+        heads = None if heads is None else tuple(heads)
+        key = (batch, tokens, max_new, heads, causal, windows)
+        layout = self._layouts.get(key)
+        if layout is None:
+            if len(self._layouts) >= 64:
+                self._layouts.clear()
+            layout = self._layouts[key] = self._layout(batch, tokens, max_new, heads, bool(causal), windows)
+        sizes, total, offsets, most, schedules = layout
         p = KVPlan()
         p.tables, p.rows, p.counts, p.tokens, p.batch, p.max_tiles, p._views = self, rows, counts, tokens, batch, most, None
-        flags = -(-batch // 4)
-        sizes = [batch + 1, tokens, batch, flags, most, most, 2 * most]
-        if windows:
-            sets, cuts, q_heads, kv_heads, unit_rows, slots, merge_rows = shape
-            workers, joins = max(sets, cuts), min(sets, cuts)
-            sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
-            sizes += [8 * (sets + cuts + joins) + (workers + 8) // 8 * 8] * len(windows)
         p._sizes = sizes
-        p._ints = ints = torch.empty(sum(sizes), dtype=torch.int32, device=self.device)
+        p._ints = ints = torch.empty(total, dtype=torch.int32, device=self.device)
         p._longs = longs = torch.empty(2 + tokens, dtype=torch.int64, device=self.device)
-        at, base = [], ints.data_ptr()
-        for n in sizes:
-            at.append(base)
-            base += 4 * n
-        counters = longs.data_ptr()
+        base, counters = ints.data_ptr(), longs.data_ptr()
+        cu, positions, lens, granted, pages, filled, tiles = (base + x for x in offsets)
         p.schedules, packed = {}, b""
-        for w, units in zip(windows, at[7:]):
+        for w, q_heads, kv_heads, floats, units, merges, starts, numbers in schedules:
             s = _Schedule()
-            merges = units + 32 * (sets + cuts)
-            s.packed = N.KV_SCHEDULE.pack(units, merges, merges + 32 * joins, sets + cuts, joins, workers, 2 * cuts, q_heads,
-                                          kv_heads, unit_rows, bool(causal), int(w), slots, self.min_tiles[unit_rows],
-                                          self.cut_tiles[unit_rows], merge_rows, 0)
-            s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, 2 * cuts * kv_heads * unit_rows
-            p.schedules[int(w)] = s
+            s.packed = N.KV_SCHEDULE.pack(base + units, base + merges, base + starts, *numbers)
+            s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, floats
+            p.schedules[w] = s
             packed += s.packed
-        p._append = (at[4], at[5], at[6])
+        p._append = (pages, filled, tiles)
         p._args = args = N.KV_PLAN.pack(
-            rows.data_ptr(), counts.data_ptr(), at[0], counters + 16, at[1], at[2], at[3], at[4], at[5], at[6], counters,
-            tokens, batch, most, N.INTS[rows.dtype], N.INTS[counts.dtype], len(windows), max_new,
+            rows.data_ptr(), counts.data_ptr(), cu, counters + 16, positions, lens, granted, pages, filled, tiles, counters,
+            tokens, batch, most, N.INTS[rows.dtype], N.INTS[counts.dtype], len(schedules), max_new,
             packed.ljust(N.KV_MAX_SCHEDULES * N.KV_SCHEDULE.size, b"\0"))
         rc = N.kv_entry("sq_kv_plan")(self._at, args, N.raw_stream())
         if rc:
             N.check(rc, "kv plan")
         return p
 
-    min_tiles = {16: 4, 32: 4, 256: 4}  # least 64-key tiles of a workgroup where a set of rows is cut
-    cut_tiles = {16: 4, 32: 4, 256: 16}  # what its partial results cost, in tiles
+    min_tiles = {16: 4, 32: 4, 256: 4}    # least 64-key tiles of a workgroup where a set of rows is cut
+    cut_tiles = {16: 4, 32: 4, 256: 16}   # what its partial results cost, in tiles
 
-    def _shape(self, q_heads, kv_heads, tokens, batch, max_new):
-        if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
-            raise ValueError("query heads must be a positive multiple of KV heads")
-        group = q_heads // kv_heads
-        most = max_new * group
-        rows = 16 if most <= 16 else 32 if most <= 32 else 256
-        slots = self._cus if rows == 256 else 2 * self._cus
-        return (-(-tokens * group // rows) + batch + 1, max(1, slots // kv_heads), q_heads, kv_heads, rows, slots,
-                max(1, min(rows, most)))
+    def _layout(self, batch, tokens, max_new, heads, causal, windows):
+        """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all
+        words, byte offsets of the first seven, page entries, per window what
+        ``sq_kv_schedule`` holds)."""
+        most = min(tokens, tokens // self.page_tokens + 2 * batch)
+        sizes = [batch + 1, tokens, batch, -(-batch // 4), most, most, 2 * most]
+        schedules = []
+        if heads is not None:
+            q_heads, kv_heads = (int(x) for x in heads)
+            if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
+                raise ValueError("query heads must be a positive multiple of KV heads")
+            group = q_heads // kv_heads
+            rows = max_new * group
+            rows = 16 if rows <= 16 else 32 if rows <= 32 else 256
+            slots = self._cus if rows == 256 else 2 * self._cus
+            sets, cuts = -(-tokens * group // rows) + batch + 1, max(1, slots // kv_heads)
+            workers, joins = max(sets, cuts), min(sets, cuts)
+            sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
+            for w in windows if tokens else ():
+                units = 4 * sum(sizes)
+                merges = units + 32 * (sets + cuts)
+                numbers = (sets + cuts, joins, workers, 2 * cuts, q_heads, kv_heads, rows, causal, int(w), slots,
+                           self.min_tiles[rows], self.cut_tiles[rows], max(1, min(rows, max_new * group)), 0)
+                schedules.append((int(w), q_heads, kv_heads, 2 * cuts * kv_heads * rows, units, merges,
+                                  merges + 32 * joins, numbers))
+                sizes.append(8 * (sets + cuts + joins) + (workers + 8) // 8 * 8)
+        offsets = [4 * sum(sizes[:i]) for i in range(7)]
+        return sizes, sum(sizes), offsets, most, schedules
 
     def commit(self, plan):
         """Takes a plan's lengths and pages over; plans made before it are void."""
