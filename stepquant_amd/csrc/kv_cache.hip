@@ -1112,32 +1112,23 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       float om = -INFINITY, oref = 0.f;  // (pairs) what the outputs are in units of
 
       // The tiles in order; past the last one the last again, so that loads ahead
-      // need no branch.  A page's number is loaded two tiles before it is used.
-      const int block = tile0 / per;
-      int sub = tile0 - block * per, left = n, id = 0, id2 = 0, ahead = block, ahead_sub = sub, ahead_left = n;
-      auto next_id = [&]() {
-        ahead_left--;
-        const bool more = ahead_left > 0, turned = ahead_sub + 1 == per;
-        ahead_sub = more ? turned ? 0 : ahead_sub + 1 : ahead_sub;
-        ahead = __builtin_amdgcn_readfirstlane(ahead + (more && turned));
-        return entries[ahead];
-      };
-      if (n > 0) {
-        id = entries[block];
-        id2 = next_id();
-      }
+      // need no branch.  The lanes hold where the pages of 64 tiles lie (all ones:
+      // a page that does not exist) and the tiles in them.
+      int ahead = 0;
+      uint32_t page_lo = 0, page_hi = 0, in_page = 0;
       bool known;
       const uint8_t *base;  // of the page of the tile
       auto next_tile = [&]() {
-        const int page = __builtin_amdgcn_readfirstlane(id);
-        known = page > 0 && page < pages;
-        base = a.c.data + (uint64_t)(uint32_t)(known ? page : 0) * page_bytes;
-        const uint8_t *at = base + first_key + sub * (kTile * D);
-        left--;
-        const bool more = left > 0, turned = sub + 1 == per;
-        sub = more ? turned ? 0 : sub + 1 : sub;
-        id = id2;
-        id2 = next_id();
+        if ((ahead & 63) == 0) {
+          const int tile = tile0 + min(ahead + lane, n - 1), block = tile / per, page = entries[block];
+          const uint64_t off = page > 0 && page < pages ? (uint64_t)(uint32_t)page * page_bytes : ~(uint64_t)0;
+          page_lo = (uint32_t)off, page_hi = (uint32_t)(off >> 32), in_page = (tile - block * per) * (kTile * D);
+        }
+        const uint32_t hi = __builtin_amdgcn_readlane(page_hi, ahead & 63), lo = __builtin_amdgcn_readlane(page_lo, ahead & 63);
+        known = hi != 0xffffffffu;
+        base = a.c.data + (known ? (uint64_t)hi << 32 | lo : 0);
+        const uint8_t *at = base + (uint32_t)(first_key + __builtin_amdgcn_readlane(in_page, ahead & 63));
+        ahead++;
         return at;
       };
       u32x4_v ck[KN], ck0[KN];
