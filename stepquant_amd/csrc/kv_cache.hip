@@ -80,6 +80,15 @@ __device__ __forceinline__ uint32_t dpp(uint32_t x) {  // 0 where no lane is nam
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
 
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {  // lane 63 holds the wave's
+  x = max(x, dpp<0x111, 0xf>(x));
+  x = max(x, dpp<0x112, 0xf>(x));
+  x = max(x, dpp<0x114, 0xf>(x));
+  x = max(x, dpp<0x118, 0xf>(x));
+  x = max(x, dpp<0x142, 0xa>(x));
+  return max(x, dpp<0x143, 0xc>(x));
+}
+
 __device__ __attribute__((noinline)) Scan block_scan(uint32_t x) {
   __shared__ uint32_t waves[kPlanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -162,8 +171,9 @@ __device__ __forceinline__ Set find_set(const sq_kv_schedule &s, const sq_kv_pla
   return r;
 }
 
-__device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, uint32_t *waves) {
+__device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L) {
   __shared__ int32_t starts[kMaxSlots + 1];
+  __shared__ uint32_t bounds[2];  // the most and the least tiles of a set
   const int tid = threadIdx.x, B = p.batch, G = s.q_heads / s.kv_heads;
   const int NB = B + 1;  // the last: packed rows past every request's
   uint32_t sum = 0;
@@ -173,6 +183,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
     const int b = tid * items + i;
     if (b < NB) sum += (uint32_t)(set_rows(p, L, b) * G + s.rows - 1) / s.rows;
   }
+  if (tid == 0) bounds[0] = 0, bounds[1] = kMost;
   Scan scan = block_scan(sum);
   uint32_t at = scan.before;
 #pragma unroll 1
@@ -193,20 +204,13 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
     most = max(most, n);
     least = min(least, n);
   }
-  const uint32_t tiles = block_scan(sum).all;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    most = max(most, (uint32_t)__shfl_xor((int)most, k, 64));
-    least = min(least, (uint32_t)__shfl_xor((int)least, k, 64));
+  most = wave_max(most), least = kMost - wave_max(kMost - least);
+  if ((tid & 63) == 63) {
+    atomicMax(&bounds[0], most);
+    atomicMin(&bounds[1], least);
   }
-  __syncthreads();
-  if ((tid & 63) == 0) waves[tid >> 6] = most, waves[kPlanThreads / 64 + (tid >> 6)] = least;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; w++) {
-    most = max(most, waves[w]);
-    least = min(least, waves[kPlanThreads / 64 + w]);
-  }
+  const uint32_t tiles = block_scan(sum).all;  // (its barriers stand behind the atomics, too)
+  most = bounds[0], least = bounds[1];
   // worker w has the tiles from w * share on
   const uint32_t slots = max(1, s.slots / s.kv_heads), share = max((uint32_t)s.min_tiles, (tiles + slots - 1) / slots);
   // tiles until the last slot is done, either way
@@ -215,13 +219,13 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   const int workers = dealt ? (int)((tiles + share - 1) / share) : sets;
   if (dealt)
     for (int w = tid; w < workers; w += kPlanThreads) starts[w] = (int)kMost;
-  uint32_t units = 0, parts = 0, merges = 0, before = 0;  // of the sets before; `before` counts their tiles
+  uint32_t units = 0, merges = 0, before = 0;  // of the sets before; `before` counts their tiles
 #pragma unroll 1
   for (int e0 = 0; e0 < sets; e0 += kPlanThreads) {
     const int e = e0 + tid;
     Set r = {};
     if (e < sets) r = sets <= kPlanThreads ? own : find_set(s, p, L, e);
-    uint32_t a = 0;
+    uint32_t a = 0, u = e, m = 0;
     int w0 = 0, k = e < sets;
     if (dealt) {
       scan = block_scan(r.n);
@@ -229,20 +233,13 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
       before += scan.all;
       w0 = min(a / share, (uint32_t)workers - 1);
       if (r.n) k = (int)((a + r.n - 1) / share) - w0 + 1;
+      // units and merges in one sum: fewer than 2^13 and 2^10 here
+      scan = block_scan(k | (uint32_t)(k > 1) << 16);
+      u = units + (scan.before & 0xffff), m = merges + (scan.before >> 16);
+      units += scan.all & 0xffff, merges += scan.all >> 16;
     }
     const bool cut = k > 1;
-    scan = block_scan(k);
-    const uint32_t u = units + scan.before;
-    units += scan.all;
-    uint32_t q = 0, m = 0;
-    if (dealt) {
-      scan = block_scan(cut ? k : 0);
-      q = parts + scan.before;
-      parts += scan.all;
-      scan = block_scan(cut);
-      m = merges + scan.before;
-      merges += scan.all;
-    }
+    const uint32_t q = u - (e - m);  // units of cut sets before: all but one for each other set
     const int q0 = e < sets && r.b ? L.end[r.b - 1] : 0;
 #pragma unroll 1
     for (int j = 0; j < k; j++) {
@@ -271,7 +268,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   __syncthreads();
 #pragma unroll 1
   for (int w = tid; w <= s.max_workers; w += kPlanThreads)
-    s.starts[w] = w < workers ? dealt ? min((int)units, starts[w]) : w : (int)units;
+    s.starts[w] = w < workers ? dealt ? min((int)units, starts[w]) : w : dealt ? (int)units : sets;
 #pragma unroll 1
   for (int m = merges + tid; m < s.max_merges; m += kPlanThreads) s.merges[8 * (int64_t)m + 2] = 0;
 }
@@ -350,7 +347,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanDev d) {
   const int n_tiles = (int)scan.all;
   __syncthreads();
   if ((int)blockIdx.x >= d.share_blocks) {
-    plan_schedule(p.schedules[blockIdx.x - d.share_blocks], p, L, waves);
+    plan_schedule(p.schedules[blockIdx.x - d.share_blocks], p, L);
     return;
   }
   if (blockIdx.x == 0) {
