@@ -24,6 +24,7 @@ typedef float f32x4_v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
 
 constexpr float kFloor = 8.673617379884035e-19f;  // 2^-60, the least peak of a block
+constexpr float kNone = -3e38f;                   // a row's largest score before it has seen a key
 constexpr int kTile = 64;                         // keys of one attention tile
 
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -1018,10 +1019,12 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // vector instructions (softmax, conversion of a later tile) have the SIMD.  A
 // barrier ends each half.
 //
-// O is kept in units of a row's largest value peak so far, so that a
-// probability times its block's peak in that unit (at most 2^8) is the half
-// that enters the product; the maximum that scores are taken from is raised
-// only when it is passed by more than 2^8.
+// A row's sum is kept in units of 2^m, m its largest score so far, and its
+// outputs in units of 2^om, om the largest score and log2 of the block's value
+// peak together: so what enters the products as halves is a probability times
+// its block's peak, whichever blocks the row's outputs come from.  Both are
+// raised only when one is passed by more than 2^8.  They start at a number below
+// every score, so that no difference of them needs care.
 template <int D, bool FP8>
 __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   extern __shared__ uint4 tiles[];
@@ -1105,8 +1108,8 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
       for (int e = 0; e < OT; e++)
 #pragma unroll
         for (int k = 0; k < 16; k++) o[e][k] = 0.f;
-      float m = -INFINITY, l = 0.f, ref = 0.f, log_ref = 0.f;
-      float om = -INFINITY, oref = 0.f;  // (pairs) what the outputs are in units of
+      float m = kNone, l = 0.f, om = kNone;
+      float both = kNone;  // (pairs) what the outputs are in units of: the larger of the two waves' om
 
       // The tiles in order; past the last one the last again, so that loads ahead
       // need no branch.  The lanes hold where the pages of 64 tiles lie (all ones:
@@ -1181,18 +1184,17 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
           // own probabilities and the other wave's, brought to one maximum: maxima
           // are whole numbers here, so that the factors are powers of two
           const uint4 w0 = taken[lane], w1 = taken[64 + lane];
-          const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
+          const float theirs = taken_m[c], high = fmaxf(om, theirs);
           pv[0] = pf[0], pv[1] = pf[1];
           pv[2] = __builtin_bit_cast(half8_v, w0), pv[3] = __builtin_bit_cast(half8_v, w1);
-          if (__any(m != theirs)) {
-            const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(m - base);
-            const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(theirs - base);
+          if (__any(om != theirs)) {
+            const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(om - high);
+            const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(theirs - high);
             pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
           }
-          if (__any(high > om || ref > oref)) {
-            float shrink = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - high);
-            if (ref > oref) shrink *= oref / ref;
-            om = high, oref = ref;
+          if (__any(high > both)) {
+            const float shrink = __builtin_amdgcn_exp2f(both - high);
+            both = high;
 #pragma unroll
             for (int e = 0; e < OT; e++)
 #pragma unroll
@@ -1258,25 +1260,27 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         float f = mult * peak.x;
         f = !some ? 1.f : f == 0.f ? 1e-37f : f;
         best *= f;
-        const float high = some ? fmaxf(ref, peak.y) : ref;
-        if (__any(best > m + 8.f || high > ref)) {
-          const float raised = fmaxf(m, PAIRS ? ceilf(best) : best);
-          const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
-          const float shrink = high > ref ? ref / high * was : was;
-          m = raised;
-          ref = high;
-          log_ref = ref > 0.f ? __builtin_amdgcn_logf(ref) : 0.f;
-          l *= was;
+        // the halves are the probabilities times 2^size
+        const float part = some ? __builtin_amdgcn_logf(peak.y) : 0.f;
+        float off = part - om, size = off + m;
+        if (__any(fmaxf(fmaxf(best - m, best + off), -size) > 8.f)) {
+          const float raised = fmaxf(m, best), top = fmaxf(om, PAIRS ? ceilf(best + part) : best + part);
+          const float shrink = __builtin_amdgcn_exp2f(om - top);
+          l *= __builtin_amdgcn_exp2f(m - raised);
+          m = raised, om = top;
           if constexpr (!PAIRS) {
 #pragma unroll
             for (int e = 0; e < OT; e++)
 #pragma unroll
               for (int k = 0; k < 16; k++) o[e][k] *= shrink;
           }
+          off = part - om, size = off + m;
+          if (__any(size < -8.f)) {  // small values: as halves, some of their probabilities would be missing in the sum
+#pragma unroll
+            for (int k = 0; k < 16 * ST; k++) l += __builtin_amdgcn_exp2f(fmaf(s[k >> 4][k & 15], f, -m));
+            size = -kNone;
+          }
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        const float size = some ? __builtin_amdgcn_logf(peak.y) - log_ref : 0.f;
-        const float off = size - base;
         float sum = 0;
 #pragma unroll
         for (int j = 0; j < 2 * ST; j++) {
@@ -1297,7 +1301,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         if constexpr (PAIRS) {
           passed[lane] = __builtin_bit_cast(uint4, pf[0]);
           passed[64 + lane] = __builtin_bit_cast(uint4, pf[1]);
-          if (hl == 0) passed_m[c] = m;
+          if (hl == 0) passed_m[c] = om;
         }
       };
 
@@ -1367,24 +1371,27 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
           ((float *)passed)[c] = l;
         }
         __syncthreads();
-        const float theirs = taken_m[c], high = fmaxf(m, theirs), base = high == -INFINITY ? 0.f : high;
-        l = fmaf(l, __builtin_amdgcn_exp2f(m - base), ((float *)taken)[c] * __builtin_amdgcn_exp2f(theirs - base));
+        const float theirs = taken_m[c], high = fmaxf(m, theirs);
+        l = fmaf(l, __builtin_amdgcn_exp2f(m - high), ((float *)taken)[c] * __builtin_amdgcn_exp2f(theirs - high));
         m = high;
+        om = both;
         __syncthreads();
       }
-      const float unit = ref * kValueUnit<FP8>;
+      // the outputs' unit beside the sum's, in two factors: 2^128 is in reach
+      const float root = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(.5f * (om - m)), unit = root * kValueUnit<FP8>;
       if (part < 0) {
         // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
         constexpr int OD = 32 * OT, OW = OD * 2 + 8;  // a wave's dims of a row, and the bytes from row to row
-        const float f = l == 0.f ? 0.f : unit / l;
+        const float f = l == 0.f ? 0.f : root / l;
         uint8_t *rows_at = (uint8_t *)tiles + wave * (32 * OW);
 #pragma unroll
         for (int k = 0; k < 16; k++) {
           float x[OT];
 #pragma unroll
-          for (int e = 0; e < OT; e++) x[e] = o[e][k] * f;
+          for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit * f;
           store_row<OT>((uint16_t *)(rows_at + c * OW) + (8 * (k >> 2) + 4 * hl + (k & 3)) * OT, a.dtype == SQ_BF16, x);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if constexpr (PAIRS) {
           // the wave's dims are every other group of four: 8 bytes a lane
@@ -1418,7 +1425,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         for (int k = 0; k < 16; k++) {
           vec x;
 #pragma unroll
-          for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit;
+          for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit * root;
           *(vec *)(dst + k * 64 * OT) = x;
         }
         if (live && hl == 0 && e0 == 0) {

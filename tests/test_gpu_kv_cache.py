@@ -484,6 +484,56 @@ def test_rows_that_kernels_do_not_take_are_copied():
     assert torch.equal(cache.data, want)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_values_of_very_different_sizes(D, new):
+    """Blocks of values of 0, 2^-30, 2^20 and between, each looked at by some rows:
+    none is lost beside another one's size, in the outputs or in the sums."""
+    Hq, sizes = 4, [2. ** -30, 1., 0., 2. ** 20, 2. ** -12, 2. ** -6]
+    print(f"case {new} new tokens of {D} dims", flush=True)
+    g = rng(41, D, new)
+    old = 64 * len(sizes)
+    tables, cache = make(1, 1, D, 64, "int8", old + new)
+    k, v = g.standard_normal((old + new, 1, D)) * .1, g.standard_normal((old + new, 1, D))
+    sharp = (40. * D ** .5) ** .5
+    for b, size in enumerate(sizes):
+        v[64 * b:64 * (b + 1)] *= size
+        k[64 * b:64 * (b + 1), :, b] += sharp
+    q = g.standard_normal((new, Hq, D)) * .1
+    for t in range(new):
+        for h in range(Hq):
+            # a block, two of them alike, or none
+            i = (t * Hq + h + D // 64) % 8
+            q[t, h, :6] += sharp * np.eye(6)[i % 6] if i < 6 else sharp / 2 * (i == 6) * np.array([0, 1, 1, 0, 0, 0])
+    x = [torch.tensor(a, dtype=torch.bfloat16, device=dev()) for a in (k, v, q)]
+    plan = tables.plan([old])
+    cache.append(x[0][:old], x[1][:old], plan)
+    tables.commit(plan)
+    plan = tables.plan([new], heads=(Hq, 1))
+    cache.append(x[0][old:], x[1][old:], plan)
+    got = cache.attend(x[2], plan).double().cpu().numpy()
+    codes, peaks = page_parts(cache)
+    unit = peaks.astype(np.float64) / 127.
+    ids = tables.table.cpu().numpy()[0]
+    keys, vals = ((codes[ids] * unit[ids][..., None, None]).transpose(2, 1, 0, 3, 4).reshape(2, -1, D))
+    peak = np.repeat(peaks[ids].reshape(len(ids), -1)[:, 1].astype(np.float64), 64)
+    queries = x[2].double().cpu().numpy()
+    for t in range(new):
+        n = old + t + 1
+        for h in range(Hq):
+            s = keys[:n] @ queries[t, h] * D ** -.5
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            want, size = p @ vals[:n], p @ np.abs(vals[:n])
+            ds = (D + 8) * 2. ** -24 * D ** -.5 * (np.abs(keys[:n]) @ np.abs(queries[t, h])).max()
+            # halves of weights and of the sum's terms (2^-17 of the largest at least), and
+            # of products too small for a half beside the row's largest product
+            tol = size * (2. ** -10 + n * 2. ** -17 + 2 * ds + (n + 64) * 2. ** -23) + n * 2. ** -24 * (p * peak[:n]).max()
+            tol += np.abs(want) * 2. ** -8 * (1 + 2. ** -9)
+            err = np.abs(got[t, h] - want)
+            assert (err <= tol).all(), (t, h, float((err / tol).max()))
+
+
 def test_refused_requests_give_zero():
     tables, cache = make(2, 2, 64, 64, "int8", 64)
     plan = tables.plan([3, 200, 5], [0, 1, 1], heads=(4, 2), causal=False)
