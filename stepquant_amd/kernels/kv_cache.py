@@ -25,6 +25,7 @@ graphs (``plan`` with device tensors, ``tokens`` and ``max_new``).
 from __future__ import annotations
 
 import ctypes
+from operator import index
 
 import torch
 
@@ -75,6 +76,11 @@ class KVPlan:
     pages = property(lambda self: self._view(5))
     filled = property(lambda self: self._view(6))
     counters = property(lambda self: self._view(7))
+
+    def record_stream(self, stream):
+        """The plan's memory is also used on ``stream`` (not only on the one it was made on)."""
+        for x in (self._ints, self._longs, self.rows, self.counts):
+            x.record_stream(stream)
 
 
 class _Schedule:
@@ -139,7 +145,11 @@ class BlockTables:
             if tokens is None or max_new is None:
                 raise ValueError("counts on the GPU need tokens and max_new")
         else:
-            host = [int(x) for x in new]
+            if isinstance(new, torch.Tensor):
+                if new.dim() != 1 or new.dtype not in N.INTS:
+                    raise ValueError("new must be one-dimensional int32 or int64")
+                new = new.tolist()
+            host = [index(x) for x in new]
             if any(x < 0 for x in host):
                 raise ValueError("new tokens cannot be negative")
             tokens = sum(host) if tokens is None else tokens
@@ -298,7 +308,7 @@ class KVCache:
             raise ValueError(f"{what} must be [{tokens}, {heads}, {self.dim}], the plan's tokens")
         s0, s1, s2 = x.stride()
         if s2 != 1 or (s0 | s1) % 8 or s0 < 0 or s1 < 0 or x.data_ptr() % 16:
-            x = x.contiguous()
+            x = x.clone(memory_format=torch.contiguous_format)
         return x
 
     def _check_plan(self, plan):
@@ -353,7 +363,11 @@ class KVCache:
         if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.dim() == 1 and x.device == self.device \
                 and x.is_contiguous():
             return x
-        return torch.as_tensor(x).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
+        x = torch.as_tensor(x)
+        if x.numel() and (x.is_floating_point() or x.is_complex() or x.dtype == torch.bool):
+            raise ValueError("pages and token counts must be integers")
+        # (numbers that 32 bits do not hold are of no page)
+        return x.clamp(-1, 0x7fffffff).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
 
     def attend(self, q, plan, *, scale=None, window=None, out=None):
         """Attention of the plan's new tokens over all that their requests hold.
@@ -369,7 +383,8 @@ class KVCache:
         if not schedules and plan.tokens:
             raise ValueError("the plan was made without heads")
         if not plan.tokens:
-            return torch.empty_like(q) if out is None else out
+            shape = (0, q.shape[-1] // self.dim, self.dim) if q.dim() == 2 else (0, *q.shape[1:])
+            return q.new_empty(shape) if out is None else out
         if window is None:
             s = next(iter(schedules.values()))
         elif window in schedules:

@@ -484,6 +484,47 @@ def test_rows_that_kernels_do_not_take_are_copied():
     assert torch.equal(cache.data, want)
 
 
+def test_starts_that_kernels_do_not_take_are_copied():
+    tables, cache, plan, q = filled([70], [3])
+    want = cache.attend(q, plan)
+    k = values(rng(31), (3, 2, 128), torch.bfloat16)
+    cache.append(k, k, plan)
+    data, want = cache.data.clone(), cache.attend(q, plan)
+
+    def moved(x):
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape)
+        return y.copy_(x)
+
+    assert moved(q).is_contiguous() and moved(q).data_ptr() % 16
+    assert torch.equal(cache.attend(moved(q), plan), want)
+    cache.append(moved(k), moved(k), plan)
+    assert torch.equal(cache.data, data)
+
+
+def test_plans_without_tokens():
+    tables, cache = make(2, 2, 128, 64, "int8", 64)
+    plan = tables.plan([0, 0], heads=(8, 2))
+    none = torch.empty((0, 8, 128), dtype=torch.bfloat16, device=dev())
+    cache.append(none[:, :2], none[:, :2], plan)
+    assert cache.attend(none, plan).shape == cache.attend(none.flatten(1), plan).shape == (0, 8, 128)
+    tables.commit(plan)
+    assert tables.lens.tolist() == [0, 0] and plan.granted.tolist() == [True, True]
+
+
+def test_a_plan_lives_on_for_another_stream():
+    tables, cache, plan, q = filled([130], [2])
+    want = cache.attend(q, plan)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = cache.attend(q, plan)
+    plan.record_stream(side)
+    del plan
+    tables.plan([5], heads=(8, 2))
+    side.synchronize()
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("new", [1, 5, 90])
 def test_values_of_very_different_sizes(D, new):
@@ -711,6 +752,12 @@ def test_refusals():
             tables.plan(**bad)
     with pytest.raises(ValueError):
         cache.decode([1], dtype=torch.int8)
+    with pytest.raises(ValueError, match="integers"):
+        cache.decode([1.5])
+    with pytest.raises(ValueError, match="int32 or int64"):
+        tables.plan(torch.tensor([1.]))
+    with pytest.raises(TypeError):
+        tables.plan([1.5])
     with pytest.raises(ValueError):
         cache.decode([1], [1, 2])
     with pytest.raises(ValueError):
