@@ -620,7 +620,7 @@ struct AttendDev {
   const int32_t *merges;
   const int32_t *starts;
   int64_t requests, tokens, q_stride, q_head_stride;
-  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials, max_units, unit_rows;
+  int32_t width, dtype, q_heads, kv_heads, causal, window, max_partials, max_units, max_workers, unit_rows;
   float scale;
 };
 
@@ -736,20 +736,25 @@ __device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float 
   else *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Units of up to 16 RT rows: the four waves take a unit's tiles in turn and
-// are joined at its end; keys and values go from memory to registers.  The
+// 16 rows of a unit: the four waves take its tiles in turn and are joined at
+// its end; keys and values go from memory to registers.  The
 // next tile's keys are under way during a tile's softmax, and the next unit's
 // first ones while the waves are joined.  Tiles of 256 dims are taken by
 // halves, which keeps a lane within 256 registers and two waves on a SIMD.
-template <int D, int RT, bool FP8>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendDev a) {
+template <int D, bool FP8>
+__global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendDev a) {
   extern __shared__ float smem[];
   constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
   constexpr int NT = D == 256 ? 2 : 4, STEP = 16 * NT;  // 16-key groups and keys of a step
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads, G = a.q_heads / a.kv_heads;
-  const int at_row = 16 * RT * blockIdx.y;  // of the unit's rows
+  // Units of 32 rows have two workgroups, which run side by side on one XCD (8
+  // apart, blocks go to the 8 in turn) so that its L2 gives one of them the keys.
+  const bool two = a.unit_rows == 32;
+  const uint32_t id = two ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x;
+  const int at_row = two ? 2 * (blockIdx.x & 8) : 0;
+  const int h = id % a.kv_heads, worker = id / a.kv_heads, G = a.q_heads / a.kv_heads;
+  if (worker >= a.max_workers) return;
   const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
   if (unit0 >= unit1) return;
   const int P = a.c.page_tokens, per = P / STEP, log_per = 31 - __clz(per);
@@ -762,7 +767,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   };
   auto read_unit = [&](int i) {
     const int32_t *u = a.units + 8 * (int64_t)i;
-    Unit x = {u[0], u[1], u[2] + at_row, min(u[3] - at_row, 16 * RT), u[4], u[5], u[6], u[7], 0};
+    Unit x = {u[0], u[1], u[2] + at_row, min(u[3] - at_row, 16), u[4], u[5], u[6], u[7], 0};
     if (x.rows <= 0 || u[3] > a.unit_rows || x.q0 < 0 || x.f0 < 0 ||
         x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
       x.rows = 0;
@@ -805,14 +810,13 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
     const Unit following = read_unit(min(unit_at + 1, unit1 - 1));
     // queries
-    half8_v qf[RT][KS];
-    float mult[RT], m[RT], l[RT];
-    int hi[RT], lo[RT];
-    f32x4_v o[RT][DT];
-#pragma unroll
-    for (int r = 0; r < RT; r++) {
-      const int f = u.f0 + 16 * r + c;
-      const bool live = 16 * r + c < u.rows;
+    half8_v qf[KS];
+    float mult, m = -INFINITY, l = 0.f;
+    int hi, lo;
+    f32x4_v o[DT];
+    {
+      const int f = u.f0 + c;
+      const bool live = c < u.rows;
       const int t = live ? f / G : 0, head = h * G + (live ? f - t * G : 0);
       const uint16_t *src = a.q + (int64_t)(u.q0 + t) * a.q_stride + head * a.q_head_stride + 16 * g;
       u32x4_v w[D / 64][2];
@@ -842,14 +846,12 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
               w[s][k][i] = f16_bits(bf_lo(w[s][k][i]) * shift) | f16_bits(bf_hi(w[s][k][i]) * shift) << 16;
       }
 #pragma unroll
-      for (int s = 0; s < KS; s++) qf[r][s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
-      mult[r] = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
-      m[r] = -INFINITY;
-      l[r] = 0.f;
-      hi[r] = live && a.causal ? min(u.kv1, u.pos0 + t + 1) : u.kv1;
-      lo[r] = live && a.window > 0 ? u.pos0 + t - a.window + 1 : 0;
+      for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
+      mult = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
+      hi = live && a.causal ? min(u.kv1, u.pos0 + t + 1) : u.kv1;
+      lo = live && a.window > 0 ? u.pos0 + t - a.window + 1 : 0;
 #pragma unroll
-      for (int e = 0; e < DT; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
+      for (int e = 0; e < DT; e++) o[e] = (f32x4_v){0, 0, 0, 0};
     }
     // steps that every row sees whole need no mask: below the first row's last
     // key and from the last row's first one on
@@ -867,19 +869,17 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
           for (int j = 0; j < 8; j++)
             vf[s][j] = *(const Bytes<D / 16> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
       }
-      f32x4_v s[RT][NT];
+      f32x4_v s[NT];
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-#pragma unroll
-        for (int r = 0; r < RT; r++) s[r][t] = (f32x4_v){0, 0, 0, 0};
+        s[t] = (f32x4_v){0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < KS; k++) {
           u32x4_v w;
           const uint32_t w0 = kf[t][k / 2][2 * (k & 1)], w1 = kf[t][k / 2][2 * (k & 1) + 1];
           w[0] = key2<FP8, 0>(w0), w[1] = key2<FP8, 1>(w0), w[2] = key2<FP8, 0>(w1), w[3] = key2<FP8, 1>(w1);
           const half8_v kh = __builtin_bit_cast(half8_v, w);
-#pragma unroll
-          for (int r = 0; r < RT; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[r][k], s[r][t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[k], s[t], 0, 0, 0);
         }
       }
       if (i + 4 < u.n) {
@@ -887,48 +887,42 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
         open(u, i + 4);
       }
       const bool whole = known && first + STEP <= all_hi && first >= all_lo;
-      half8_v pf[RT][NT / 2];
-      float alpha[RT], sv[RT];
-      bool same = true;
+      half8_v pf[NT / 2];
+      const float f = mult * peak.x;
+      float best = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const float f = mult[r] * peak.x;
-        float best = -INFINITY;
+      for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            float x = s[r][t][k] * f;
-            if (!whole) {
-              const int j = first + 16 * t + 4 * g + k;
-              x = known && j < hi[r] && j >= lo[r] ? x : -INFINITY;
-            }
-            s[r][t][k] = x;
-            best = fmaxf(best, x);
+        for (int k = 0; k < 4; k++) {
+          float x = s[t][k] * f;
+          if (!whole) {
+            const int j = first + 16 * t + 4 * g + k;
+            x = known && j < hi && j >= lo ? x : -INFINITY;
           }
-        best = fmaxf(reduce_max4(best), m[r]);
-        const float base = best == -INFINITY ? 0.f : best;
-        alpha[r] = __builtin_amdgcn_exp2f(m[r] - base);
-        same = same && m[r] == best;
-        m[r] = best;
-        float sum = 0;
-        u32x4_v w[NT / 2];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          float p[4];
-#pragma unroll
-          for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(s[r][t][k] - base);
-#pragma unroll
-          for (int k = 0; k < 2; k++) w[t >> 1][2 * (t & 1) + k] = weigh2(p[2 * k], p[2 * k + 1], sum);
+          s[t][k] = x;
+          best = fmaxf(best, x);
         }
-        l[r] = fmaf(l[r], alpha[r], sum);
+      best = fmaxf(reduce_max4(best), m);
+      const float base = best == -INFINITY ? 0.f : best;
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      const bool keep = __all(m == best);
+      m = best;
+      float sum = 0;
+      u32x4_v w[NT / 2];
 #pragma unroll
-        for (int t = 0; t < NT / 2; t++) pf[r][t] = __builtin_bit_cast(half8_v, w[t]);
-        // a row that sees none of the step takes nothing from it, whatever its peak
-        const bool some = whole || (known && first < hi[r] && first + STEP > lo[r]);
-        sv[r] = some ? peak.y * kValueUnit<FP8> : 0.f;
+      for (int t = 0; t < NT; t++) {
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(s[t][k] - base);
+#pragma unroll
+        for (int k = 0; k < 2; k++) w[t >> 1][2 * (t & 1) + k] = weigh2(p[2 * k], p[2 * k + 1], sum);
       }
-      const bool keep = __all(same);
+      l = fmaf(l, alpha, sum);
+#pragma unroll
+      for (int t = 0; t < NT / 2; t++) pf[t] = __builtin_bit_cast(half8_v, w[t]);
+      // a row that sees none of the step takes nothing from it, whatever its peak
+      const bool some = whole || (known && first < hi && first + STEP > lo);
+      const float sv = some ? peak.y * kValueUnit<FP8> : 0.f;
       auto value = [&](auto E) {
         constexpr int e = decltype(E)::value;
         half8_v v[NT / 2];
@@ -939,16 +933,13 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
           for (int j = 0; j < 8; j++) w[j] = vf[s2][j].w[e / 4];
           v[s2] = value8<FP8, e & 3>(w);
         }
+        f32x4_v x = {0, 0, 0, 0};
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-          f32x4_v x = {0, 0, 0, 0};
+        for (int s2 = 0; s2 < NT / 2; s2++) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s2], pf[s2], x, 0, 0, 0);
 #pragma unroll
-          for (int s2 = 0; s2 < NT / 2; s2++) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s2], pf[r][s2], x, 0, 0, 0);
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float was = keep ? o[r][e][k] : o[r][e][k] * alpha[r];
-            o[r][e][k] = fmaf(x[k], sv[r], was);
-          }
+        for (int k = 0; k < 4; k++) {
+          const float was = keep ? o[e][k] : o[e][k] * alpha;
+          o[e][k] = fmaf(x[k], sv, was);
         }
       };
       each(value, std::make_integer_sequence<int, DT>{});
@@ -957,48 +948,45 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void kv_attend_kernel(AttendD
     // the four waves' shares of each row, joined through LDS
     float *so = smem;                 // [4][16][LDO]
     float *sm = smem + 4 * 16 * LDO;  // [4][16] maxima, then sums
+    const float sum = reduce_sum4(l);
+    __syncthreads();  // (after the last unit's readers)
+    if (g == 0) {
+      sm[16 * wave + c] = m;
+      sm[64 + 16 * wave + c] = sum;
+    }
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-      const float sum = reduce_sum4(l[r]);
-      __syncthreads();  // (after the last unit's, or the last rows', readers)
-      if (g == 0) {
-        sm[16 * wave + c] = m[r];
-        sm[64 + 16 * wave + c] = sum;
+    for (int k = 0; k < 4; k++) {
+      float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
+#pragma unroll
+      for (int e = 0; e < DT; e += 4)
+        *(f32x4_v *)(dst + e) = (f32x4_v){o[e][k], o[e + 1][k], o[e + 2][k], o[e + 3][k]};
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * (D / 4); i += 256) {
+      const int j = i / (D / 4), d = 4 * (i % (D / 4));
+      if (j >= u.rows) break;
+      float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float all = 0;
+      f32x4_v x = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
+        all = fmaf(sm[64 + 16 * w + j], f, all);
+        x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
       }
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
-#pragma unroll
-        for (int e = 0; e < DT; e += 4)
-          *(f32x4_v *)(dst + e) = (f32x4_v){o[r][e][k], o[r][e + 1][k], o[r][e + 2][k], o[r][e + 3][k]};
-      }
-      __syncthreads();
-      for (int i = tid; i < 16 * (D / 4); i += 256) {
-        const int j = i / (D / 4), d = 4 * (i % (D / 4));
-        if (16 * r + j >= u.rows) break;
-        float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
-        const float base = mm == -INFINITY ? 0.f : mm;
-        float all = 0;
-        f32x4_v x = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-          const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
-          all = fmaf(sm[64 + 16 * w + j], f, all);
-          x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
-        }
-        const int f = u.f0 + 16 * r + j;
-        if (u.part < 0) {
-          x *= all == 0.f ? 0.f : 1.f / all;
-          const int t = f / G, head = h * G + f - t * G;
-          store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
-        } else {
-          const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * a.unit_rows + at_row + 16 * r + j;
-          *(f32x4_v *)(a.ws + slot * D + d) = x;
-          if (d == 0) {
-            float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
-            ml[0] = mm;
-            ml[1] = all;
-          }
+      const int f = u.f0 + j;
+      if (u.part < 0) {
+        x *= all == 0.f ? 0.f : 1.f / all;
+        const int t = f / G, head = h * G + f - t * G;
+        store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
+      } else {
+        const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * a.unit_rows + at_row + j;
+        *(f32x4_v *)(a.ws + slot * D + d) = x;
+        if (d == 0) {
+          float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
+          ml[0] = mm;
+          ml[1] = all;
         }
       }
     }
@@ -1655,26 +1643,22 @@ int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 template <int D, bool FP8>
 int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
-  auto go = [&](auto kernel, int id, int threads, size_t lds, int turns = 1) {
+  const unsigned blocks = s.max_workers * s.kv_heads;
+  auto go = [&](auto kernel, int id, unsigned grid, int threads, size_t lds) {
     const int rc = dynamic_lds((const void *)kernel, 2 * id + FP8, lds, "kv attend: LDS attribute");
     if (rc) return rc;
-    const dim3 grid((unsigned)(s.max_workers * s.kv_heads), (unsigned)turns);
-    hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, st, d);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
-  static_assert(D <= 256, "ids of kernels with more than 64 KiB");
   constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float);
   // tiles, peaks, and what the pairs of waves share; the outputs' way out
   constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 128) : 0);
   constexpr size_t rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
   constexpr size_t many = staged > rows_out ? staged : rows_out;
+  // (ids of kernels with more than 64 KiB: one of each kind needs one of 256 dims, the many rows' one of 128)
   int rc;
-  if (s.rows == 16) rc = go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined);
-  // 32 rows of 256 dims do not fit a wave's registers twice on a SIMD: they go to two workgroups
-  else if constexpr (D == 256)
-    rc = s.rows == 32 ? go(kv_attend_kernel<D, 1, FP8>, 1, 256, joined, 2) : go(kv_attend_rows_kernel<D, FP8>, 3, 512, many);
-  else if (s.rows == 32) rc = go(kv_attend_kernel<D, 2, FP8>, 2, 256, joined);
-  else rc = go(kv_attend_rows_kernel<D, FP8>, 4, 512, many);
+  if (s.rows == 256) rc = go(kv_attend_rows_kernel<D, FP8>, D == 256 ? 2 : 3, blocks, 512, many);
+  else rc = go(kv_attend_kernel<D, FP8>, 1, s.rows == 32 ? (blocks + 7) / 8 * 16 : blocks, 256, joined);
   if (rc) return rc;
   const unsigned merges = s.max_merges * s.kv_heads;
   if (s.rows == 256) hipLaunchKernelGGL(kv_merge_rows_kernel<D>, dim3(merges, D == 256 ? 16 : 8), dim3(512), 0, st, d);
@@ -1784,7 +1768,7 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   const sq_kv_schedule &s = a->schedule;
   const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges, s.starts,
                        a->requests, a->tokens, a->q_stride, a->q_head_stride, a->width, a->dtype, s.q_heads, s.kv_heads,
-                       s.causal, s.window, s.max_partials, s.max_units, s.rows, a->scale};
+                       s.causal, s.window, s.max_partials, s.max_units, s.max_workers, s.rows, a->scale};
   const bool fp8 = c->storage == SQ_KV_FP8;
   hipStream_t st = (hipStream_t)stream;
   if (c->dim == 64) return fp8 ? launch_attend<64, true>(d, s, st) : launch_attend<64, false>(d, s, st);

@@ -204,8 +204,20 @@ class BlockTables:
             N.check(rc, "kv plan")
         return p
 
-    min_tiles = {16: 4, 32: 4, 256: 4}    # least 64-key tiles of a workgroup where a set of rows is cut
-    cut_tiles = {16: 4, 32: 4, 256: 16}   # what its partial results cost, in tiles
+    # Rows of a set.  16: one workgroup.  32: two that read the same keys side by
+    # side (32 rows of 8 heads of 128 dims, 160 requests of 4096 tokens: 477 us in
+    # sets of 16, 318 so).  256: tiles that are converted once for 8 waves; that
+    # pays past 64 rows (64 rows of 4 requests of 4000: 39.8 us, 30.1 in sets of 32;
+    # of 160 requests 638 and 590; 96 rows of 160 requests 653 and 851).
+    # Slots, the workgroups that run at a time: two on a CU up to 32 rows (three
+    # would wait for one another: 64 requests of up to 8192, 116 us with two, 130
+    # with one, 131 with three), one of 256 rows.
+    # Least 64-key tiles of a workgroup where a set of rows is cut; 1 to 16 are alike.
+    min_tiles = {16: 4, 32: 4, 256: 4}
+    # What partial results cost, in tiles: 64 requests of up to 8192 take 116 us
+    # cut, 131 uncut; 160 of up to 4096 and 32 rows 223 us with 4 here, 210 with 16;
+    # a prompt of 8192 tokens 543 us uncut, 709 cut (with 0 here).
+    cut_tiles = {16: 4, 32: 16, 256: 16}
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows):
         """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all
@@ -220,8 +232,8 @@ class BlockTables:
                 raise ValueError("query heads must be a positive multiple of KV heads")
             group = q_heads // kv_heads
             rows = max_new * group
-            rows = 16 if rows <= 16 else 32 if rows <= 32 else 256
-            slots = self._cus if rows == 256 else 2 * self._cus
+            rows = 16 if rows <= 16 else 32 if rows <= 64 else 256
+            slots = 2 * self._cus if rows == 16 else self._cus
             sets, cuts = -(-tokens * group // rows) + batch + 1, max(1, slots // kv_heads)
             workers, joins = max(sets, cuts), min(sets, cuts)
             sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
