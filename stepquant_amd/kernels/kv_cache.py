@@ -216,8 +216,9 @@ class BlockTables:
     min_tiles = {16: 4, 32: 4, 256: 4}
     # What partial results cost, in tiles: 64 requests of up to 8192 take 116 us
     # cut, 131 uncut; 160 of up to 4096 and 32 rows 223 us with 4 here, 210 with 16;
-    # a prompt of 8192 tokens 543 us uncut, 709 cut (with 0 here).
-    cut_tiles = {16: 4, 32: 16, 256: 16}
+    # prompts of up to 2048 and 7 rows a token 77 us with 16,
+    # 58 with 24; a prompt of 8192 tokens 543 us uncut, 709 cut (with 0 here).
+    cut_tiles = {16: 4, 32: 16, 256: 24}
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows):
         """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all
