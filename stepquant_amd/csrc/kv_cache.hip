@@ -54,9 +54,17 @@ __device__ __forceinline__ int64_t load_index(const void *p, int dtype, int64_t 
 
 // ------------------------------------------------------------ block tables
 //
-// Every workgroup scans the requests for itself (they are few) and then
-// serves its share of the tokens and pages, so a plan is one launch; the
-// last workgroups lay out the attention layers' work.
+// Sums over the requests: the ends of their packed rows, of their new pages
+// and of the page entries that they touch; a request is granted if its pages
+// end within the free ones.  Every workgroup sums the requests for itself
+// (they are few) and then serves its share of the tokens and pages, so a plan
+// is one launch; the last workgroups lay out the attention layers' work.
+//
+// What bounds it is its chain of sums, each some 0.3 us with two barriers, and
+// the first loads (0.25 MB are written for 16,384 tokens): 9.0 us for 256
+// requests of one new token, 11.4 us for 48 prompts of up to 2731, commit 1.9.
+// Loops stay rolled and sums take 32 bits: 9 KB of code in place of 51, whose
+// fetching cost more than the branches (48 prompts 15.9 -> 13.2 us).
 
 constexpr int kPlanThreads = 512;
 constexpr int kMaxSlots = 4096;
@@ -492,8 +500,12 @@ __device__ __forceinline__ void decode4(uint32_t w, float x[4]) {
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// One workgroup per (page entry, head, keys or values); a thread holds N
-// groups of 8 adjacent dims, so the new values are read once.
+// One workgroup per (page entry, head, keys or values): it finds the peak of
+// its new values, brings the block's older codes to it where it grew, and
+// writes the new codes.  A thread holds N groups of 8 adjacent dims between
+// the two, so the new values are read once, 16 bytes a lane.  HBM bounds it:
+// 16,384 tokens of 8 heads of 128 dims, 101 MB, in 20.2 us (5.0 TB/s); 64
+// single tokens take 3.7 us, a launch and two loads one after the other.
 template <bool FP8, int N>
 __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_append_args a, int log_dim) {
   __shared__ uint32_t peaks[4];
@@ -562,6 +574,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
   }
 }
 
+// Codes times peak / top, 8 dims a lane; the same 16,384 tokens to bf16,
+// 101 MB, in 17.3 us (5.8 TB/s).
 template <bool FP8>
 __global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int32_t *pages, const int32_t *filled,
                                                         void *k, void *v, int dtype, int log_dim) {
@@ -608,7 +622,9 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int
 // scores and outputs of one row only, and the rounded probabilities of one
 // product are the operand of the next without leaving their registers.
 // Codes of at most 8 bits are exact as halves, and so are queries: a row is
-// brought near 2^14 by a power of two first, where bfloat16's 8 bits fit.
+// brought near 2^14 by a power of two first, where bfloat16's 8 bits fit.  So
+// scores are sums in 32 bits of exact products, times a block's peak; what is
+// rounded are the probabilities, to 11 bits, and the outputs.
 
 struct AttendDev {
   sq_kv_cache c;
@@ -737,10 +753,19 @@ __device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float 
 }
 
 // 16 rows of a unit: the four waves take its tiles in turn and are joined at
-// its end; keys and values go from memory to registers.  The
-// next tile's keys are under way during a tile's softmax, and the next unit's
-// first ones while the waves are joined.  Tiles of 256 dims are taken by
-// halves, which keeps a lane within 256 registers and two waves on a SIMD.
+// its end; keys and values go from memory to registers, in the order in which
+// a product's lanes hold them (keys 16 bytes of a token, values a token's
+// D / 16 bytes), so nothing passes LDS.  The next tile's keys are under way
+// during a tile's softmax, and the next unit's first ones while the waves are
+// joined.  Tiles of 256 dims are taken by halves, which keeps a lane within 256
+// registers and two waves on a SIMD.
+//
+// HBM bounds it where there is enough to read: 256 requests of 4096 tokens (8
+// heads of 128 dims, 2.16 GB) 356 us, 6.1 TB/s; 64 of up to 8192 (593 MB) 112
+// us; one of 131,072 (270 MB) 44 us.  A short one (1000 tokens of 2 heads of 256
+// dims) takes 10.8 us: loads of the schedule, the table, the pages and the
+// partial results one after the other.  Values fetched a tile ahead as well
+// cost 2 to 5% (registers), three or four workgroups on a CU 10 to 13%.
 template <int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendDev a) {
   extern __shared__ float smem[];
@@ -1006,6 +1031,19 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // the next tile's keys: 32 of 32 cycles each at 128 dims), the other one's
 // vector instructions (softmax, conversion of a later tile) have the SIMD.  A
 // barrier ends each half.
+//
+// LDS bounds the products (each reads one operand there, 128 bytes a cycle for
+// the four SIMDs, which is all that LDS gives; 64 rows a wave would halve that,
+// and need twice the registers), and the vector instructions of the other half
+// fill what is left.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims (550
+// GFLOP): 556 us, 990 TFLOP/s of the 1160 that a large library product reaches;
+// the products alone, without softmax and conversion, take 400 us.  256 dims 890
+// TFLOP/s, as tiles are converted for 128 rows, not 256; 64 dims 630, as scores
+// cost the same there and products half.  The halves half a tile apart took it
+// from 827 to 670 us, peaks by way of LDS and masks without conditions (no
+// scalar register spilled) to 579.  The order of products and LDS reads that the
+// groups below ask for takes 3% off; wave priorities change nothing, nor do 8
+// operands ahead in place of 4.
 //
 // A row's sum is kept in units of 2^m, m its largest score so far, and its
 // outputs in units of 2^om, om the largest score and log2 of the block's value
@@ -1427,8 +1465,9 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   }
 }
 
-// Joins the parts of query rows of units of up to 32: one workgroup per
-// (merge, head) and row; LANES lanes read a part, GROUPS parts at a time.
+// Joins the parts of query rows of units of up to 32, by their maxima: one
+// workgroup per (merge, head) and row; LANES lanes read a part, GROUPS parts at
+// a time.  3.9 to 5.0 us, most of them a launch's own; 6.7 us for 64 parts.
 template <int D>
 __global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
   constexpr int LANES = D / 4, GROUPS = 512 / LANES, AHEAD = 4;
@@ -1487,7 +1526,9 @@ __global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
 
 // Joins the parts of units of up to 256 rows, in the order in which a wave's
 // registers of kv_attend_rows_kernel went out: one workgroup per (merge, head)
-// and wave; its two halves take the parts in turn, two at a time.
+// and wave; its two halves take the parts in turn, two at a time.  19.6 us for
+// the parts of 4 chunks of 701 tokens, 16 heads over 2 of 256 dims (up to 67 MB, written
+// the kernel before).
 template <int D>
 __global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
   constexpr int DT = D / 32, OT = D == 256 ? DT / 2 : DT, BLOCKS = D == 256 ? 16 : 8;
