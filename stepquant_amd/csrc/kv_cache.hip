@@ -25,6 +25,7 @@ typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
 
 constexpr float kFloor = 8.673617379884035e-19f;  // 2^-60, the least peak of a block
 constexpr float kNone = -3e38f;                   // a row's largest score before it has seen a key
+constexpr float kLarge = 0x1p-17f;                // a score above 8 / this is large (in log2)
 constexpr int kTile = 64;                         // keys of one attention tile
 
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -1288,9 +1289,10 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
         best *= f;
         // the halves are the probabilities times 2^size
         const float part = some ? __builtin_amdgcn_logf(peak.y) : 0.f;
-        float off = part - om, size = off + m;
-        if (__any(fmaxf(fmaxf(best - m, best + off), -size) > 8.f)) {
-          const float raised = fmaxf(m, best), top = fmaxf(om, PAIRS ? ceilf(best + part) : best + part);
+        float off = part - om, size = part + (m - om);
+        const float raised = fmaxf(m, best), by = best - m;
+        if (__any(fmaxf(fmaxf(by, by + size), fmaxf(-size, fabsf(raised) * kLarge)) > 8.f)) {
+          const float top = fmaxf(om, PAIRS ? ceilf(best + part) : best + part);
           const float shrink = __builtin_amdgcn_exp2f(om - top);
           l *= __builtin_amdgcn_exp2f(m - raised);
           m = raised, om = top;
@@ -1300,10 +1302,18 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
 #pragma unroll
               for (int k = 0; k < 16; k++) o[e][k] *= shrink;
           }
-          off = part - om, size = off + m;
+          off = part - om, size = part + (m - om);
+          float less = m;
+          if (__any(fabsf(m) * kLarge > 8.f)) {
+            // scores of which 32 bits hold no fractions: rounded before the difference,
+            // as the maximum is, so that no weight exceeds what a half holds
+#pragma unroll
+            for (int k = 0; k < 16 * ST; k++) s[k >> 4][k & 15] = s[k >> 4][k & 15] * f - m;
+            f = 1.f, off = size, less = 0.f;
+          }
           if (__any(size < -8.f)) {  // small values: as halves, some of their probabilities would be missing in the sum
 #pragma unroll
-            for (int k = 0; k < 16 * ST; k++) l += __builtin_amdgcn_exp2f(fmaf(s[k >> 4][k & 15], f, -m));
+            for (int k = 0; k < 16 * ST; k++) l += __builtin_amdgcn_exp2f(fmaf(s[k >> 4][k & 15], f, -less));
             size = -kNone;
           }
         }

@@ -575,6 +575,40 @@ def test_values_of_very_different_sizes(D, new):
             assert (err <= tol).all(), (t, h, float((err / tol).max()))
 
 
+@pytest.mark.parametrize("D,new", [(64, 1), (64, 90), (128, 20), (128, 90), (256, 5), (256, 90)])
+def test_scores_beyond_fractions(D, new):
+    """Scores of 10^8 and more: the largest takes the row, nothing overflows."""
+    old, Hq = 300, 4
+    print(f"case {new} new tokens of {D} dims", flush=True)
+    g = rng(43, D, new)
+    tables, cache = make(1, 1, D, 64, "int8", old + new)
+    big = [torch.from_numpy(np.clip(2e4 * g.standard_normal((old + new, h, D)), -6e4, 6e4)).to(dev(), torch.float16)
+           for h in (1, Hq)]
+    v = values(g, (old + new, 1, D), torch.float16)
+    plan = tables.plan([old])
+    cache.append(big[0][:old], v[:old], plan)
+    tables.commit(plan)
+    plan = tables.plan([new], heads=(Hq, 1))
+    cache.append(big[0][old:], v[old:], plan)
+    q = big[1][old:]
+    got = cache.attend(q, plan).double().cpu().numpy()
+    codes, peaks = page_parts(cache)
+    ids = tables.table.cpu().numpy()[0]
+    x = (codes[ids] * (peaks.astype(np.float64) / 127.)[ids][..., None, None]).transpose(2, 1, 0, 3, 4).reshape(2, -1, D)
+    clear = 0
+    for t in range(new):
+        for h in range(Hq):
+            s = x[0][:old + t + 1] @ q[t, h].double().cpu().numpy() * D ** -.5
+            best, other = np.sort(s)[[-1, -2]]
+            assert np.abs(got[t, h]).max() <= np.abs(x[1]).max() * 1.001
+            # 32-bit sums of D products: a gap of twice their error leaves one key
+            if best - other > 2 * ((D + 8) * 2. ** -24 * np.abs(s).max() * D ** .5 + 100):
+                clear += 1
+                want = x[1][s.argmax()]
+                assert (np.abs(got[t, h] - want) <= np.abs(want) * 2. ** -10 + 2. ** -24).all(), (t, h)
+    assert clear >= new
+
+
 def test_refused_requests_give_zero():
     tables, cache = make(2, 2, 64, 64, "int8", 64)
     plan = tables.plan([3, 200, 5], [0, 1, 1], heads=(4, 2), causal=False)
