@@ -121,6 +121,7 @@ class BlockTables:
     def _index(self, x, what):
         if not isinstance(x, torch.Tensor):
             x = torch.as_tensor(x)
+            x = x if x.numel() else x.long()
         if x.dim() != 1 or x.dtype not in N.INTS:
             raise ValueError(f"{what} must be one-dimensional int32 or int64")
         return x if x.device == self.device and x.is_contiguous() else x.to(self.device).contiguous()
@@ -131,8 +132,9 @@ class BlockTables:
         ``new`` and ``rows`` are lists or int32/int64 tensors, ``rows``
         distinct.  ``tokens`` is the number of packed rows (at least
         ``sum(new)``; rows past it are padding) and ``max_new`` the most new
-        tokens of a request; both default to those of ``new`` where that is on
-        the host and are required where it is on the GPU.  ``heads``
+        tokens of a request (requests past either are refused); both default to
+        those of ``new`` where that is on the host and are required where it is
+        on the GPU.  ``heads``
         (query heads, KV heads) also lays out the work of ``attend``: with
         ``causal`` each token sees its request's tokens up to itself, else all
         of them; ``window`` > 0 leaves it the last ``window`` of those.  A
@@ -305,7 +307,7 @@ class KVCache:
         """Writes are made on the caller's stream: nothing to wait for."""
 
     def copy(self, source, destination):
-        """Copies whole pages (a shared prefix's part-filled page before it is written)."""
+        """Copies whole pages, codes and peaks (a request that starts as another one's copy)."""
         PackedStatePool.copy(self, source, destination)
 
     def _rows(self, x, heads, tokens, what):
@@ -333,8 +335,8 @@ class KVCache:
         """Quantises the plan's new keys and values [tokens, kv_heads, head_dim]
         (or [tokens, kv_heads * head_dim]; bf16 or fp16) into their pages.
 
-        Pages shared by several requests are only ever whole: a part-filled
-        page belongs to one request (``copy`` it first).
+        Every page belongs to one request, as ``BlockTables`` gives them out: two
+        requests that wrote to one page would race for its peaks.
         """
         self._check_plan(plan)
         k = self._rows(k, self.heads, plan.tokens, "keys")

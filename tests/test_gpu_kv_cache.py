@@ -509,6 +509,9 @@ def test_plans_without_tokens():
     assert cache.attend(none, plan).shape == cache.attend(none.flatten(1), plan).shape == (0, 8, 128)
     tables.commit(plan)
     assert tables.lens.tolist() == [0, 0] and plan.granted.tolist() == [True, True]
+    tables.release([])
+    assert cache.decode([])[0].shape == (0, 64, 2, 128)
+    assert tables.counters.tolist() == [0, tables.pages - 1]
 
 
 def test_a_plan_lives_on_for_another_stream():
