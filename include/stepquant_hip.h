@@ -424,8 +424,8 @@ typedef struct sq_kv_tables {
 /*
  * How one kind of attention layer splits its work, filled by sq_kv_plan.
  * One unit is `rows` query rows (token-major, the heads of a group inside a
- * token) against a range of keys; a worker (one workgroup for each KV head)
- * takes units starts[w] to starts[w + 1] - 1.  Units of rows whose keys were
+ * token) against a range of keys; a worker (one workgroup for each KV head,
+ * two where rows is 32) takes units starts[w] to starts[w + 1] - 1.  Units of rows whose keys were
  * cut between workers are joined by a merge.  With tokens, batch,
  * G = q_heads / kv_heads, sets = ceil(tokens * G / rows) + batch + 1 and
  * s = max(1, slots / kv_heads):
@@ -447,7 +447,7 @@ typedef struct sq_kv_schedule {
     int32_t rows;         /* 16, 32 or 256 */
     int32_t causal;
     int32_t window;       /* 0: none; else the last `window` keys (causal only) */
-    int32_t slots;        /* workgroups that the device holds at once, at most 4096 */
+    int32_t slots;        /* workers times KV heads that the device holds at once, at most 4096 */
     int32_t min_tiles;    /* least 64-key tiles of a worker, at least 1 */
     int32_t cut_tiles;    /* what a cut costs, in tiles of work */
     int32_t merge_rows;   /* most rows of a unit: min(rows, max_count * G) */
@@ -466,9 +466,10 @@ typedef struct sq_kv_schedule {
  *   lens      [batch] tokens held afterwards
  *   granted   [batch] 0 where the request's tokens find no room: the table's
  *             row is too short, it has more than max_count of them, its
- *             packed rows pass `tokens`, the tables' row does not exist, or the free pages run out (pages are given in request
- *             order; from the first request that they do not cover, none that
- *             needs a page gets one)
+ *             packed rows pass `tokens`, the tables' row does not exist, or
+ *             the free pages run out (pages are given in request order; from
+ *             the first request that they do not cover, none that needs a
+ *             page gets one)
  *   pages     [max_tiles] the pages that new tokens fall into, request by
  *             request in block order, 0 past the last; filled [max_tiles] the
  *             tokens that each holds afterwards; tiles [max_tiles, 2] its
