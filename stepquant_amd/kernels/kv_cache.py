@@ -214,8 +214,10 @@ class BlockTables:
     # Slots, the workgroups that run at a time: two on a CU up to 32 rows (three
     # would wait for one another: 64 requests of up to 8192, 116 us with two, 130
     # with one, 131 with three), one of 256 rows.
-    # Least 64-key tiles of a workgroup where a set of rows is cut; 1 to 16 are alike.
-    min_tiles = {16: 4, 32: 4, 256: 4}
+    # Least 64-key tiles of a workgroup where a set of rows is cut: two of 256 dims
+    # are a step for each of four waves (1 request of 1000 tokens 13.3 us with 2,
+    # 14.1 with 4, 16.7 with 8); other dims are alike from 1 to 8.
+    min_tiles = {16: 2, 32: 2, 256: 4}
     # What partial results cost, in tiles: 64 requests of up to 8192 take 116 us
     # cut, 131 uncut; 160 of up to 4096 and 32 rows 223 us with 4 here, 210 with 16;
     # prompts of up to 2048 and 7 rows a token 77 us with 16,
