@@ -1712,7 +1712,8 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
   else rc = go(kv_attend_kernel<D, FP8>, 1, s.rows == 32 ? (blocks + 7) / 8 * 16 : blocks, 256, joined);
   if (rc) return rc;
   const unsigned merges = s.max_merges * s.kv_heads;
-  if (s.rows == 256) hipLaunchKernelGGL(kv_merge_rows_kernel<D>, dim3(merges, D == 256 ? 16 : 8), dim3(512), 0, st, d);
+  const unsigned waves = (unsigned)(s.merge_rows + 31) / 32 * (D == 256 ? 2 : 1);  // of a unit that have rows
+  if (s.rows == 256) hipLaunchKernelGGL(kv_merge_rows_kernel<D>, dim3(merges, waves), dim3(512), 0, st, d);
   else hipLaunchKernelGGL(kv_merge_kernel<D>, dim3(merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
   return sq_internal_launched("kv_merge_kernel");
 }
