@@ -764,7 +764,7 @@ __device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float 
 // HBM bounds it where there is enough to read: 256 requests of 4096 tokens (8
 // heads of 128 dims, 2.16 GB) 356 us, 6.1 TB/s; 64 of up to 8192 (593 MB) 112
 // us; one of 131,072 (270 MB) 44 us.  A short one (1000 tokens of 2 heads of 256
-// dims) takes 10.8 us: loads of the schedule, the table, the pages and the
+// dims) takes 9.8 us: loads of the schedule, the table, the pages and the
 // partial results one after the other.  Values fetched a tile ahead as well
 // cost 2 to 5% (registers), three or four workgroups on a CU 10 to 13%.
 template <int D, bool FP8>
