@@ -766,7 +766,7 @@ __device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float 
 // us; one of 131,072 (270 MB) 44 us.  A short one (1000 tokens of 2 heads of 256
 // dims) takes 9.8 us: loads of the schedule, the table, the pages and the
 // partial results one after the other.  Values fetched a tile ahead as well
-// cost 2 to 5% (registers), three or four workgroups on a CU 10 to 13%.
+// cost 2 to 5% (registers), three workgroups on a CU 10 to 16%.
 template <int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendDev a) {
   extern __shared__ float smem[];
