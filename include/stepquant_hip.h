@@ -429,7 +429,7 @@ typedef struct sq_kv_tables {
  * cut between workers are joined by a merge.  With tokens, batch,
  * G = q_heads / kv_heads, sets = ceil(tokens * G / rows) + batch + 1 and
  * s = max(1, slots / kv_heads):
- *   max_workers  >= max(sets, s), and starts holds max_workers + 1
+ *   max_workers  >= max(sets, s), and starts holds max_workers + 2
  *   max_units    >= sets + s
  *   max_merges   >= min(sets, s)
  *   max_partials >= 2 * s
@@ -437,7 +437,7 @@ typedef struct sq_kv_tables {
 typedef struct sq_kv_schedule {
     int32_t *units;       /* [max_units, 8] */
     int32_t *merges;      /* [max_merges, 8] */
-    int32_t *starts;      /* [max_workers + 1] */
+    int32_t *starts;      /* [max_workers + 2]; the last: the rows of a unit */
     int32_t max_units;
     int32_t max_merges;
     int32_t max_workers;
@@ -451,7 +451,10 @@ typedef struct sq_kv_schedule {
     int32_t min_tiles;    /* least 64-key tiles of a worker, at least 1 */
     int32_t cut_tiles;    /* what a cut costs, in tiles of work */
     int32_t merge_rows;   /* most rows of a unit: min(rows, max_count * G) */
-    int32_t reserved;
+    int32_t few_work;     /* 0, or for 256 rows: a plan of at most so many query rows (of all
+                             heads) times tiles that they see takes 32 (sets as of 32) */
+    int32_t few_min_tiles;  /* min_tiles and cut_tiles then */
+    int32_t few_cut_tiles;
 } sq_kv_schedule;
 
 #define SQ_KV_MAX_REQUESTS 4096

@@ -88,7 +88,8 @@ class KVTables(ctypes.Structure):
 class KVSchedule(ctypes.Structure):
     _fields_ = [("units", _P), ("merges", _P), ("starts", _P)] + [(n, ctypes.c_int32) for n in (
         "max_units", "max_merges", "max_workers", "max_partials", "q_heads", "kv_heads", "rows", "causal", "window",
-        "slots", "min_tiles", "cut_tiles", "merge_rows", "reserved")]
+        "slots", "min_tiles", "cut_tiles", "merge_rows", "few_work",
+        "few_min_tiles", "few_cut_tiles")]
 
 
 KV_INT8, KV_FP8 = 0, 1
@@ -233,7 +234,7 @@ def step_entry(name: str):
 
 
 # the KV cache's argument blocks in the order of their structures' fields, as above
-KV_SCHEDULE = struct.Struct("=3Q14i")
+KV_SCHEDULE = struct.Struct("=3Q16i")
 KV_PLAN = struct.Struct(f"=11Qq6i{KV_MAX_SCHEDULES * KV_SCHEDULE.size}s")
 KV_APPEND = struct.Struct("=5Q5q2i")
 KV_ATTEND = struct.Struct(f"=4Q4q2ifi{KV_SCHEDULE.size}s")

@@ -164,13 +164,13 @@ __device__ __forceinline__ int set_rows(const sq_kv_plan_args &p, const PlanLds 
   return (b < p.batch ? L.end[b] : (int)p.tokens) - (b ? L.end[b - 1] : 0);
 }
 
-__device__ __forceinline__ Set find_set(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, int e) {
+__device__ __forceinline__ Set find_set(const sq_kv_schedule &s, const sq_kv_plan_args &p, const PlanLds &L, int rows, int e) {
   const int G = s.q_heads / s.kv_heads;
   Set r;
   r.b = upper_bound(L.tiles, p.batch + 1, e);
   const int count = set_rows(p, L, r.b);
-  r.f0 = (L.tiles[r.b] - 1 - e) * s.rows;  // the request's last rows first
-  r.rows = min(s.rows, count * G - r.f0);
+  r.f0 = (L.tiles[r.b] - 1 - e) * rows;  // the request's last rows first
+  r.rows = min(rows, count * G - r.f0);
   r.kv0 = r.kv1 = r.n = 0;
   const int old = r.b < p.batch ? L.old[r.b] : -1;
   if (old >= 0) {
@@ -188,18 +188,36 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   const int NB = B + 1;  // the last: packed rows past every request's
   uint32_t sum = 0;
   const int items = (NB + kPlanThreads - 1) / kPlanThreads;
+  Scan scan;
+  int rows = s.rows, min_tiles = s.min_tiles, cut_tiles = s.cut_tiles;
+  if (s.few_work > 0) {
+    // query rows times the tiles that they see, about: little work goes to sets of 32
+#pragma unroll 1
+    for (int i = 0; i < items; i++) {
+      const int b = tid * items + i;
+      if (b < B && L.old[b] >= 0) {
+        const int count = set_rows(p, L, b);
+        uint32_t keys = (uint32_t)L.old[b] + (s.causal ? count / 2 : count);
+        if (s.window > 0) keys = min(keys, (uint32_t)s.window);
+        sum = min(sum + (uint32_t)min((uint64_t)count * s.q_heads * (keys / kTile + 1), (uint64_t)kMost), kMost);
+      }
+    }
+    scan = block_scan(sum);
+    if (scan.all <= (uint32_t)s.few_work) rows = 32, min_tiles = s.few_min_tiles, cut_tiles = s.few_cut_tiles;
+    sum = 0;
+  }
 #pragma unroll 1
   for (int i = 0; i < items; i++) {
     const int b = tid * items + i;
-    if (b < NB) sum += (uint32_t)(set_rows(p, L, b) * G + s.rows - 1) / s.rows;
+    if (b < NB) sum += (uint32_t)(set_rows(p, L, b) * G + rows - 1) / rows;
   }
   if (tid == 0) bounds[0] = 0, bounds[1] = kMost;
-  Scan scan = block_scan(sum);
+  scan = block_scan(sum);
   uint32_t at = scan.before;
 #pragma unroll 1
   for (int i = 0; i < items; i++) {
     const int b = tid * items + i;
-    if (b < NB) L.tiles[b] = (int32_t)(at += (uint32_t)(set_rows(p, L, b) * G + s.rows - 1) / s.rows);
+    if (b < NB) L.tiles[b] = (int32_t)(at += (uint32_t)(set_rows(p, L, b) * G + rows - 1) / rows);
   }
   __syncthreads();
   const int sets = (int)scan.all;
@@ -208,7 +226,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   Set own = {};  // the thread's last set: its only one where there are few
 #pragma unroll 1
   for (int e = tid; e < sets; e += kPlanThreads) {
-    own = find_set(s, p, L, e);
+    own = find_set(s, p, L, rows, e);
     const uint32_t n = own.n;
     sum = min(sum + n, kMost);
     most = max(most, n);
@@ -222,10 +240,10 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   const uint32_t tiles = block_scan(sum).all;  // (its barriers stand behind the atomics, too)
   most = bounds[0], least = bounds[1];
   // worker w has the tiles from w * share on
-  const uint32_t slots = max(1, s.slots / s.kv_heads), share = max((uint32_t)s.min_tiles, (tiles + slots - 1) / slots);
+  const uint32_t slots = max(1, s.slots / s.kv_heads), share = max((uint32_t)min_tiles, (tiles + slots - 1) / slots);
   // tiles until the last slot is done, either way
   const uint32_t whole = (uint32_t)sets <= slots ? most : max(most, (tiles + slots - 1) / slots + least);
-  const bool dealt = share + s.cut_tiles < whole && tiles < kMost;
+  const bool dealt = share + cut_tiles < whole && tiles < kMost;
   const int workers = dealt ? (int)((tiles + share - 1) / share) : sets;
   if (dealt)
     for (int w = tid; w < workers; w += kPlanThreads) starts[w] = (int)kMost;
@@ -234,7 +252,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   for (int e0 = 0; e0 < sets; e0 += kPlanThreads) {
     const int e = e0 + tid;
     Set r = {};
-    if (e < sets) r = sets <= kPlanThreads ? own : find_set(s, p, L, e);
+    if (e < sets) r = sets <= kPlanThreads ? own : find_set(s, p, L, rows, e);
     uint32_t a = 0, u = e, m = 0;
     int w0 = 0, k = e < sets;
     if (dealt) {
@@ -279,6 +297,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
 #pragma unroll 1
   for (int w = tid; w <= s.max_workers; w += kPlanThreads)
     s.starts[w] = w < workers ? dealt ? min((int)units, starts[w]) : w : dealt ? (int)units : sets;
+  if (tid == 0) s.starts[s.max_workers + 1] = rows;
 #pragma unroll 1
   for (int m = merges + tid; m < s.max_merges; m += kPlanThreads) s.merges[8 * (int64_t)m + 2] = 0;
 }
@@ -753,273 +772,6 @@ __device__ __forceinline__ void store_row(uint16_t *dst, bool bf16, const float 
   else *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 16 rows of a unit: the four waves take its tiles in turn and are joined at
-// its end; keys and values go from memory to registers, in the order in which
-// a product's lanes hold them (keys 16 bytes of a token, values a token's
-// D / 16 bytes), so nothing passes LDS.  The next tile's keys are under way
-// during a tile's softmax, and the next unit's first ones while the waves are
-// joined.  Tiles of 256 dims are taken by halves, which keeps a lane within 256
-// registers and two waves on a SIMD.
-//
-// HBM bounds it where there is enough to read: 256 requests of 4096 tokens (8
-// heads of 128 dims, 2.16 GB) 356 us, 6.1 TB/s; 64 of up to 8192 (593 MB) 112
-// us; one of 131,072 (270 MB) 44 us.  A short one (1000 tokens of 2 heads of 256
-// dims) takes 9.8 us: loads of the schedule, the table, the pages and the
-// partial results one after the other.  Values fetched a tile ahead as well
-// cost 2 to 5% (registers), three workgroups on a CU 10 to 16%.
-template <int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendDev a) {
-  extern __shared__ float smem[];
-  constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
-  constexpr int NT = D == 256 ? 2 : 4, STEP = 16 * NT;  // 16-key groups and keys of a step
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-  // Units of 32 rows have two workgroups, which run side by side on one XCD (8
-  // apart, blocks go to the 8 in turn) so that its L2 gives one of them the keys.
-  const bool two = a.unit_rows == 32;
-  const uint32_t id = two ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x;
-  const int at_row = two ? 2 * (blockIdx.x & 8) : 0;
-  const int h = id % a.kv_heads, worker = id / a.kv_heads, G = a.q_heads / a.kv_heads;
-  if (worker >= a.max_workers) return;
-  const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
-  if (unit0 >= unit1) return;
-  const int P = a.c.page_tokens, per = P / STEP, log_per = 31 - __clz(per);
-  const bool pow2 = (per & (per - 1)) == 0;
-  const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
-  auto entry_of = [&](int step) { return pow2 ? step >> log_per : step / per; };
-
-  struct Unit {
-    int row, q0, f0, rows, pos0, kv0, kv1, part, n;
-  };
-  auto read_unit = [&](int i) {
-    const int32_t *u = a.units + 8 * (int64_t)i;
-    Unit x = {u[0], u[1], u[2] + at_row, min(u[3] - at_row, 16), u[4], u[5], u[6], u[7], 0};
-    if (x.rows <= 0 || u[3] > a.unit_rows || x.q0 < 0 || x.f0 < 0 ||
-        x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
-      x.rows = 0;
-    // a row of the table that does not exist holds no keys
-    const bool held = x.rows > 0 && x.row >= 0 && x.row < a.requests;
-    x.kv1 = held ? (int)min((int64_t)x.kv1, (int64_t)a.width * P) : 0;
-    x.n = max(0, (x.kv1 - x.kv0 + STEP - 1) / STEP);
-    return x;
-  };
-
-  Bytes<D / 16> vf[NT / 2][8];
-  u32x4_v kf[NT][D / 64];
-  int ids = 0, page = 0;
-  const uint8_t *page_at = nullptr, *at = nullptr;
-  // the lanes hold the pages of 64 of the wave's steps
-  auto fetch_ids = [&](const Unit &u, int i) {
-    const int mine = i + 4 * lane;
-    ids = mine < u.n ? a.table[(int64_t)u.row * a.width + entry_of(u.kv0 / STEP + mine)] : 0;
-  };
-  auto open = [&](const Unit &u, int i) {  // step i of a unit: its page, and its keys on their way
-    const int step = u.kv0 / STEP + i;
-    const int p = __builtin_amdgcn_readlane(ids, (i >> 2) & 63);
-    page = p > 0 && p < a.c.num_pages ? p : 0;
-    page_at = a.c.data + page * a.c.page_bytes;
-    at = page_at + ((int64_t)(2 * h) * P + (step - entry_of(step) * per) * STEP) * D;
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-      for (int s = 0; s < D / 64; s++) kf[t][s] = *(const u32x4_v *)(at + (16 * t + c) * D + 64 * s + 16 * g);
-  };
-  auto begin = [&](const Unit &u) {
-    if (wave < u.n) {
-      fetch_ids(u, wave);
-      open(u, wave);
-    }
-  };
-
-  Unit u = read_unit(unit0);
-  begin(u);
-  for (int unit_at = unit0; unit_at < unit1; unit_at++) {
-    const Unit following = read_unit(min(unit_at + 1, unit1 - 1));
-    // queries
-    half8_v qf[KS];
-    float mult, m = -INFINITY, l = 0.f;
-    int hi, lo;
-    f32x4_v o[DT];
-    {
-      const int f = u.f0 + c;
-      const bool live = c < u.rows;
-      const int t = live ? f / G : 0, head = h * G + (live ? f - t * G : 0);
-      const uint16_t *src = a.q + (int64_t)(u.q0 + t) * a.q_stride + head * a.q_head_stride + 16 * g;
-      u32x4_v w[D / 64][2];
-#pragma unroll
-      for (int s = 0; s < D / 64; s++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) w[s][k] = live ? *(const u32x4_v *)(src + 64 * s + 8 * k) : (u32x4_v){0, 0, 0, 0};
-      float unit = 1.f;
-      if (a.dtype == SQ_BF16) {
-        float most = 0;
-#pragma unroll
-        for (int s = 0; s < D / 64; s++)
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][k][i])), fabsf(bf_hi(w[s][k][i]))));
-        most = reduce_max4(most);
-        float shift;
-        row_shift(most, &shift, &unit);
-#pragma unroll
-        for (int s = 0; s < D / 64; s++)
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              w[s][k][i] = f16_bits(bf_lo(w[s][k][i]) * shift) | f16_bits(bf_hi(w[s][k][i]) * shift) << 16;
-      }
-#pragma unroll
-      for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
-      mult = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
-      hi = live && a.causal ? min(u.kv1, u.pos0 + t + 1) : u.kv1;
-      lo = live && a.window > 0 ? u.pos0 + t - a.window + 1 : 0;
-#pragma unroll
-      for (int e = 0; e < DT; e++) o[e] = (f32x4_v){0, 0, 0, 0};
-    }
-    // steps that every row sees whole need no mask: below the first row's last
-    // key and from the last row's first one on
-    const int all_hi = min(u.kv1, a.causal ? u.pos0 + u.f0 / G + 1 : u.kv1);
-    const int all_lo = a.window > 0 ? u.pos0 + (u.f0 + u.rows - 1) / G - a.window + 1 : 0;
-    for (int i = wave; i < u.n; i += 4) {
-      const float2 peak = *(const float2 *)(page_at + peaks_at);
-      const int first = u.kv0 + i * STEP;
-      const bool known = page != 0;
-      {
-        const uint8_t *vat = at + (int64_t)P * D;
-#pragma unroll
-        for (int s = 0; s < NT / 2; s++)
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-            vf[s][j] = *(const Bytes<D / 16> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
-      }
-      f32x4_v s[NT];
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        s[t] = (f32x4_v){0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-          u32x4_v w;
-          const uint32_t w0 = kf[t][k / 2][2 * (k & 1)], w1 = kf[t][k / 2][2 * (k & 1) + 1];
-          w[0] = key2<FP8, 0>(w0), w[1] = key2<FP8, 1>(w0), w[2] = key2<FP8, 0>(w1), w[3] = key2<FP8, 1>(w1);
-          const half8_v kh = __builtin_bit_cast(half8_v, w);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[k], s[t], 0, 0, 0);
-        }
-      }
-      if (i + 4 < u.n) {
-        if ((((i + 4) >> 2) & 63) == 0) fetch_ids(u, i + 4);
-        open(u, i + 4);
-      }
-      const bool whole = known && first + STEP <= all_hi && first >= all_lo;
-      half8_v pf[NT / 2];
-      const float f = mult * peak.x;
-      float best = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          float x = s[t][k] * f;
-          if (!whole) {
-            const int j = first + 16 * t + 4 * g + k;
-            x = known && j < hi && j >= lo ? x : -INFINITY;
-          }
-          s[t][k] = x;
-          best = fmaxf(best, x);
-        }
-      best = fmaxf(reduce_max4(best), m);
-      const float base = best == -INFINITY ? 0.f : best;
-      const float alpha = __builtin_amdgcn_exp2f(m - base);
-      const bool keep = __all(m == best);
-      m = best;
-      float sum = 0;
-      u32x4_v w[NT / 2];
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        float p[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(s[t][k] - base);
-#pragma unroll
-        for (int k = 0; k < 2; k++) w[t >> 1][2 * (t & 1) + k] = weigh2(p[2 * k], p[2 * k + 1], sum);
-      }
-      l = fmaf(l, alpha, sum);
-#pragma unroll
-      for (int t = 0; t < NT / 2; t++) pf[t] = __builtin_bit_cast(half8_v, w[t]);
-      // a row that sees none of the step takes nothing from it, whatever its peak
-      const bool some = whole || (known && first < hi && first + STEP > lo);
-      const float sv = some ? peak.y * kValueUnit<FP8> : 0.f;
-      auto value = [&](auto E) {
-        constexpr int e = decltype(E)::value;
-        half8_v v[NT / 2];
-#pragma unroll
-        for (int s2 = 0; s2 < NT / 2; s2++) {
-          uint32_t w[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) w[j] = vf[s2][j].w[e / 4];
-          v[s2] = value8<FP8, e & 3>(w);
-        }
-        f32x4_v x = {0, 0, 0, 0};
-#pragma unroll
-        for (int s2 = 0; s2 < NT / 2; s2++) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s2], pf[s2], x, 0, 0, 0);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float was = keep ? o[e][k] : o[e][k] * alpha;
-          o[e][k] = fmaf(x[k], sv, was);
-        }
-      };
-      each(value, std::make_integer_sequence<int, DT>{});
-    }
-    if (unit_at + 1 < unit1) begin(following);
-    // the four waves' shares of each row, joined through LDS
-    float *so = smem;                 // [4][16][LDO]
-    float *sm = smem + 4 * 16 * LDO;  // [4][16] maxima, then sums
-    const float sum = reduce_sum4(l);
-    __syncthreads();  // (after the last unit's readers)
-    if (g == 0) {
-      sm[16 * wave + c] = m;
-      sm[64 + 16 * wave + c] = sum;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
-#pragma unroll
-      for (int e = 0; e < DT; e += 4)
-        *(f32x4_v *)(dst + e) = (f32x4_v){o[e][k], o[e + 1][k], o[e + 2][k], o[e + 3][k]};
-    }
-    __syncthreads();
-    for (int i = tid; i < 16 * (D / 4); i += 256) {
-      const int j = i / (D / 4), d = 4 * (i % (D / 4));
-      if (j >= u.rows) break;
-      float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
-      const float base = mm == -INFINITY ? 0.f : mm;
-      float all = 0;
-      f32x4_v x = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
-        all = fmaf(sm[64 + 16 * w + j], f, all);
-        x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
-      }
-      const int f = u.f0 + j;
-      if (u.part < 0) {
-        x *= all == 0.f ? 0.f : 1.f / all;
-        const int t = f / G, head = h * G + f - t * G;
-        store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
-      } else {
-        const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * a.unit_rows + at_row + j;
-        *(f32x4_v *)(a.ws + slot * D + d) = x;
-        if (d == 0) {
-          float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D + 2 * slot;
-          ml[0] = mm;
-          ml[1] = all;
-        }
-      }
-    }
-    u = following;
-  }
-}
-
 typedef float f32x16_v __attribute__((ext_vector_type(16)));
 
 // Units of up to 256 rows: 8 waves of 32 rows (of 256 dims: 128 rows at a time,
@@ -1053,8 +805,7 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // raised only when one is passed by more than 2^8.  They start at a number below
 // every score, so that no difference of them needs care.
 template <int D, bool FP8>
-__global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
-  extern __shared__ uint4 tiles[];
+__device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
   constexpr int KS = D / 16, DT = D / 32;                   // k steps and dim tiles
   constexpr int KF = 65, KB = 2 * KS * KF, VB = 4 * DT * 64;  // uint4 of a step's keys, of a tile's keys and values
   // Of 256 dims, whose outputs would fill a wave's registers, two waves share 32
@@ -1475,11 +1226,296 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
   }
 }
 
+template <int D, bool FP8>
+__global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
+  extern __shared__ uint4 tiles[];
+  attend_many<D, FP8>(a, tiles);
+}
+
+// 16 rows of a unit: the four waves take its tiles in turn and are joined at
+// its end; keys and values go from memory to registers, in the order in which
+// a product's lanes hold them (keys 16 bytes of a token, values a token's
+// D / 16 bytes), so nothing passes LDS.  The next tile's keys are under way
+// during a tile's softmax, and the next unit's first ones while the waves are
+// joined.  Tiles of 256 dims are taken by halves, which keeps a lane within 256
+// registers and two waves on a SIMD.
+//
+// HBM bounds it where there is enough to read: 256 requests of 4096 tokens (8
+// heads of 128 dims, 2.16 GB) 356 us, 6.1 TB/s; 64 of up to 8192 (593 MB) 112
+// us; one of 131,072 (270 MB) 44 us.  A short one (1000 tokens of 2 heads of 256
+// dims) takes 9.8 us: loads of the schedule, the table, the pages and the
+// partial results one after the other.  Values fetched a tile ahead as well
+// cost 2 to 5% (registers), three workgroups on a CU 10 to 16%.
+//
+// EITHER: where the plan decides between units of 256 rows and of 32, which
+// have the halves of a workgroup of 512 then.
+template <int D>
+constexpr int kJoin = 4 * 16 * (D + 4) + 128;  // floats of LDS
+
+template <int D, bool FP8, bool EITHER>
+__global__ __launch_bounds__(EITHER ? 512 : 256, 2) void kv_attend_kernel(AttendDev a) {
+  extern __shared__ float floats[];
+  if (EITHER && a.starts[a.max_workers + 1] != 32) {
+    attend_many<D, FP8>(a, (uint4 *)floats);
+    return;
+  }
+  float *const smem = floats + (EITHER ? (threadIdx.x >> 8) * kJoin<D> : 0);
+  constexpr int KS = D / 32, DT = D / 16, LDO = D + 4;
+  constexpr int NT = D == 256 ? 2 : 4, STEP = 16 * NT;  // 16-key groups and keys of a step
+  const int tid = EITHER ? threadIdx.x & 255 : threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+  // Units of 32 rows have two workgroups, which run side by side on one XCD (8
+  // apart, blocks go to the 8 in turn) so that its L2 gives one of them the keys.
+  const int unit_rows = EITHER ? 32 : a.unit_rows;
+  const bool two = !EITHER && unit_rows == 32;
+  const uint32_t id = two ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x;
+  const int at_row = EITHER ? 16 * (threadIdx.x >> 8) : two ? 2 * (blockIdx.x & 8) : 0;
+  const int h = id % a.kv_heads, worker = id / a.kv_heads, G = a.q_heads / a.kv_heads;
+  if (worker >= a.max_workers) return;
+  const int unit0 = max(0, a.starts[worker]), unit1 = min(a.starts[worker + 1], a.max_units);
+  if (unit0 >= unit1) return;
+  const int P = a.c.page_tokens, per = P / STEP, log_per = 31 - __clz(per);
+  const bool pow2 = (per & (per - 1)) == 0;
+  const int64_t peaks_at = 2 * (int64_t)a.c.heads * P * D + 8 * h;
+  auto entry_of = [&](int step) { return pow2 ? step >> log_per : step / per; };
+
+  struct Unit {
+    int row, q0, f0, rows, pos0, kv0, kv1, part, n;
+  };
+  auto read_unit = [&](int i) {
+    const int32_t *u = a.units + 8 * (int64_t)i;
+    Unit x = {u[0], u[1], u[2] + at_row, min(u[3] - at_row, 16), u[4], u[5], u[6], u[7], 0};
+    if (x.rows <= 0 || u[3] > unit_rows || x.q0 < 0 || x.f0 < 0 ||
+        x.q0 + (int64_t)(x.f0 + x.rows - 1) / G >= a.tokens)
+      x.rows = 0;
+    // a row of the table that does not exist holds no keys
+    const bool held = x.rows > 0 && x.row >= 0 && x.row < a.requests;
+    x.kv1 = held ? (int)min((int64_t)x.kv1, (int64_t)a.width * P) : 0;
+    x.n = max(0, (x.kv1 - x.kv0 + STEP - 1) / STEP);
+    return x;
+  };
+
+  Bytes<D / 16> vf[NT / 2][8];
+  u32x4_v kf[NT][D / 64];
+  int ids = 0, page = 0;
+  const uint8_t *page_at = nullptr, *at = nullptr;
+  // the lanes hold the pages of 64 of the wave's steps
+  auto fetch_ids = [&](const Unit &u, int i) {
+    const int mine = i + 4 * lane;
+    ids = mine < u.n ? a.table[(int64_t)u.row * a.width + entry_of(u.kv0 / STEP + mine)] : 0;
+  };
+  auto open = [&](const Unit &u, int i) {  // step i of a unit: its page, and its keys on their way
+    const int step = u.kv0 / STEP + i;
+    const int p = __builtin_amdgcn_readlane(ids, (i >> 2) & 63);
+    page = p > 0 && p < a.c.num_pages ? p : 0;
+    page_at = a.c.data + page * a.c.page_bytes;
+    at = page_at + ((int64_t)(2 * h) * P + (step - entry_of(step) * per) * STEP) * D;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int s = 0; s < D / 64; s++) kf[t][s] = *(const u32x4_v *)(at + (16 * t + c) * D + 64 * s + 16 * g);
+  };
+  auto begin = [&](const Unit &u) {
+    if (wave < u.n) {
+      fetch_ids(u, wave);
+      open(u, wave);
+    }
+  };
+
+  Unit u = read_unit(unit0);
+  begin(u);
+  for (int unit_at = unit0; unit_at < unit1; unit_at++) {
+    const Unit following = read_unit(min(unit_at + 1, unit1 - 1));
+    // queries
+    half8_v qf[KS];
+    float mult, m = -INFINITY, l = 0.f;
+    int hi, lo;
+    f32x4_v o[DT];
+    {
+      const int f = u.f0 + c;
+      const bool live = c < u.rows;
+      const int t = live ? f / G : 0, head = h * G + (live ? f - t * G : 0);
+      const uint16_t *src = a.q + (int64_t)(u.q0 + t) * a.q_stride + head * a.q_head_stride + 16 * g;
+      u32x4_v w[D / 64][2];
+#pragma unroll
+      for (int s = 0; s < D / 64; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) w[s][k] = live ? *(const u32x4_v *)(src + 64 * s + 8 * k) : (u32x4_v){0, 0, 0, 0};
+      float unit = 1.f;
+      if (a.dtype == SQ_BF16) {
+        float most = 0;
+#pragma unroll
+        for (int s = 0; s < D / 64; s++)
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              most = fmaxf(most, fmaxf(fabsf(bf_lo(w[s][k][i])), fabsf(bf_hi(w[s][k][i]))));
+        most = reduce_max4(most);
+        float shift;
+        row_shift(most, &shift, &unit);
+#pragma unroll
+        for (int s = 0; s < D / 64; s++)
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              w[s][k][i] = f16_bits(bf_lo(w[s][k][i]) * shift) | f16_bits(bf_hi(w[s][k][i]) * shift) << 16;
+      }
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[s] = __builtin_bit_cast(half8_v, w[s / 2][s & 1]);
+      mult = a.scale * 1.4426950408889634f * unit * kKeyUnit<FP8>;
+      hi = live && a.causal ? min(u.kv1, u.pos0 + t + 1) : u.kv1;
+      lo = live && a.window > 0 ? u.pos0 + t - a.window + 1 : 0;
+#pragma unroll
+      for (int e = 0; e < DT; e++) o[e] = (f32x4_v){0, 0, 0, 0};
+    }
+    // steps that every row sees whole need no mask: below the first row's last
+    // key and from the last row's first one on
+    const int all_hi = min(u.kv1, a.causal ? u.pos0 + u.f0 / G + 1 : u.kv1);
+    const int all_lo = a.window > 0 ? u.pos0 + (u.f0 + u.rows - 1) / G - a.window + 1 : 0;
+    for (int i = wave; i < u.n; i += 4) {
+      const float2 peak = *(const float2 *)(page_at + peaks_at);
+      const int first = u.kv0 + i * STEP;
+      const bool known = page != 0;
+      {
+        const uint8_t *vat = at + (int64_t)P * D;
+#pragma unroll
+        for (int s = 0; s < NT / 2; s++)
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            vf[s][j] = *(const Bytes<D / 16> *)(vat + (32 * s + 16 * (j >> 2) + 4 * g + (j & 3)) * D + c * DT);
+      }
+      f32x4_v s[NT];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        s[t] = (f32x4_v){0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          u32x4_v w;
+          const uint32_t w0 = kf[t][k / 2][2 * (k & 1)], w1 = kf[t][k / 2][2 * (k & 1) + 1];
+          w[0] = key2<FP8, 0>(w0), w[1] = key2<FP8, 1>(w0), w[2] = key2<FP8, 0>(w1), w[3] = key2<FP8, 1>(w1);
+          const half8_v kh = __builtin_bit_cast(half8_v, w);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[k], s[t], 0, 0, 0);
+        }
+      }
+      if (i + 4 < u.n) {
+        if ((((i + 4) >> 2) & 63) == 0) fetch_ids(u, i + 4);
+        open(u, i + 4);
+      }
+      const bool whole = known && first + STEP <= all_hi && first >= all_lo;
+      half8_v pf[NT / 2];
+      const float f = mult * peak.x;
+      float best = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          float x = s[t][k] * f;
+          if (!whole) {
+            const int j = first + 16 * t + 4 * g + k;
+            x = known && j < hi && j >= lo ? x : -INFINITY;
+          }
+          s[t][k] = x;
+          best = fmaxf(best, x);
+        }
+      best = fmaxf(reduce_max4(best), m);
+      const float base = best == -INFINITY ? 0.f : best;
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      const bool keep = __all(m == best);
+      m = best;
+      float sum = 0;
+      u32x4_v w[NT / 2];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(s[t][k] - base);
+#pragma unroll
+        for (int k = 0; k < 2; k++) w[t >> 1][2 * (t & 1) + k] = weigh2(p[2 * k], p[2 * k + 1], sum);
+      }
+      l = fmaf(l, alpha, sum);
+#pragma unroll
+      for (int t = 0; t < NT / 2; t++) pf[t] = __builtin_bit_cast(half8_v, w[t]);
+      // a row that sees none of the step takes nothing from it, whatever its peak
+      const bool some = whole || (known && first < hi && first + STEP > lo);
+      const float sv = some ? peak.y * kValueUnit<FP8> : 0.f;
+      auto value = [&](auto E) {
+        constexpr int e = decltype(E)::value;
+        half8_v v[NT / 2];
+#pragma unroll
+        for (int s2 = 0; s2 < NT / 2; s2++) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) w[j] = vf[s2][j].w[e / 4];
+          v[s2] = value8<FP8, e & 3>(w);
+        }
+        f32x4_v x = {0, 0, 0, 0};
+#pragma unroll
+        for (int s2 = 0; s2 < NT / 2; s2++) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s2], pf[s2], x, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float was = keep ? o[e][k] : o[e][k] * alpha;
+          o[e][k] = fmaf(x[k], sv, was);
+        }
+      };
+      each(value, std::make_integer_sequence<int, DT>{});
+    }
+    if (unit_at + 1 < unit1) begin(following);
+    // the four waves' shares of each row, joined through LDS
+    float *so = smem;                 // [4][16][LDO]
+    float *sm = smem + 4 * 16 * LDO;  // [4][16] maxima, then sums
+    const float sum = reduce_sum4(l);
+    __syncthreads();  // (after the last unit's readers)
+    if (g == 0) {
+      sm[16 * wave + c] = m;
+      sm[64 + 16 * wave + c] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      float *dst = so + (16 * wave + c) * LDO + (4 * g + k) * DT;
+#pragma unroll
+      for (int e = 0; e < DT; e += 4)
+        *(f32x4_v *)(dst + e) = (f32x4_v){o[e][k], o[e + 1][k], o[e + 2][k], o[e + 3][k]};
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * (D / 4); i += 256) {
+      const int j = i / (D / 4), d = 4 * (i % (D / 4));
+      if (j >= u.rows) break;
+      float mm = fmaxf(fmaxf(sm[j], sm[16 + j]), fmaxf(sm[32 + j], sm[48 + j]));
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float all = 0;
+      f32x4_v x = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float f = __builtin_amdgcn_exp2f(sm[16 * w + j] - base);
+        all = fmaf(sm[64 + 16 * w + j], f, all);
+        x += *(const f32x4_v *)(so + (16 * w + j) * LDO + d) * f;
+      }
+      const int f = u.f0 + j;
+      if (u.part < 0) {
+        x *= all == 0.f ? 0.f : 1.f / all;
+        const int t = f / G, head = h * G + f - t * G;
+        store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
+      } else {
+        const int64_t slot = ((int64_t)u.part * a.kv_heads + h) * unit_rows + at_row + j;
+        *(f32x4_v *)(a.ws + slot * D + d) = x;
+        if (d == 0) {
+          float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * unit_rows * D + 2 * slot;
+          ml[0] = mm;
+          ml[1] = all;
+        }
+      }
+    }
+    u = following;
+  }
+}
+
 // Joins the parts of query rows of units of up to 32, by their maxima: one
 // workgroup per (merge, head) and row; LANES lanes read a part, GROUPS parts at
 // a time.  3.9 to 5.0 us, most of them a launch's own; 6.7 us for 64 parts.
 template <int D>
-__global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
+__device__ __forceinline__ void merge_few(const AttendDev &a, int unit_rows) {
   constexpr int LANES = D / 4, GROUPS = 512 / LANES, AHEAD = 4;
   __shared__ f32x4_v part_o[GROUPS][LANES];
   __shared__ float part_l[GROUPS], part_m[GROUPS];
@@ -1488,8 +1524,8 @@ __global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
   const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4], G = a.q_heads / a.kv_heads;
   if (j >= rows) return;
   const int lane = tid % LANES, grp = tid / LANES;
-  const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * a.unit_rows * D;
-  const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * a.unit_rows + j, step = (int64_t)a.kv_heads * a.unit_rows;
+  const float *ml = a.ws + (int64_t)a.max_partials * a.kv_heads * unit_rows * D;
+  const int64_t slot0 = ((int64_t)p0 * a.kv_heads + h) * unit_rows + j, step = (int64_t)a.kv_heads * unit_rows;
   // every group of lanes joins its parts as they come, then the groups
   f32x4_v x = {0, 0, 0, 0};
   float sum = 0, mm = -INFINITY;
@@ -1540,7 +1576,7 @@ __global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
 // the parts of 4 chunks of 701 tokens, 16 heads over 2 of 256 dims (up to 67 MB, written
 // the kernel before).
 template <int D>
-__global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
+__device__ __forceinline__ void merge_many(const AttendDev &a) {
   constexpr int DT = D / 32, OT = D == 256 ? DT / 2 : DT, BLOCKS = D == 256 ? 16 : 8;
   typedef float vec __attribute__((ext_vector_type(OT)));
   __shared__ vec part_o[4][256];
@@ -1596,6 +1632,22 @@ __global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
   }
 }
 
+template <int D>
+__global__ __launch_bounds__(512) void kv_merge_kernel(AttendDev a) {
+  merge_few<D>(a, a.unit_rows);
+}
+
+template <int D>
+__global__ __launch_bounds__(512) void kv_merge_rows_kernel(AttendDev a) {
+  merge_many<D>(a);
+}
+
+template <int D>
+__global__ __launch_bounds__(512) void kv_merge_either_kernel(AttendDev a) {
+  if (a.starts[a.max_workers + 1] == 32) merge_few<D>(a, 32);
+  else if (blockIdx.y < (D == 256 ? 16 : 8)) merge_many<D>(a);
+}
+
 // ------------------------------------------------------------ host side
 
 int fail(int code, const char *msg) { return sq_internal_fail(code, msg); }
@@ -1635,7 +1687,9 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
     return fail(SQ_EINVAL, "kv schedule: min_tiles, cut_tiles or merge_rows");
   const int64_t G = s->q_heads / s->kv_heads;
   if (tokens * G > 0x3fffffff) return fail(SQ_EINVAL, "kv schedule: tokens * heads of a group too large");
-  const int64_t sets = (tokens * G + s->rows - 1) / s->rows + batch + 1;
+  if (s->few_work < 0 || (s->few_work > 0 && (s->rows != 256 || s->few_min_tiles <= 0 || s->few_cut_tiles < 0)))
+    return fail(SQ_EINVAL, "kv schedule: few_work, few_min_tiles or few_cut_tiles");
+  const int64_t least = s->few_work > 0 ? 32 : s->rows, sets = (tokens * G + least - 1) / least + batch + 1;
   const int64_t slots = s->slots / s->kv_heads > 1 ? s->slots / s->kv_heads : 1;
   const int64_t larger = sets > slots ? sets : slots, smaller = sets < slots ? sets : slots;
   if (s->max_workers < larger || s->max_units < sets + slots || s->max_merges < smaller ||
@@ -1701,19 +1755,21 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, d);
     return sq_internal_launched("kv_attend_kernel");
   };
-  constexpr size_t joined = (4 * 16 * (D + 4) + 128) * sizeof(float);
+  constexpr size_t joined = kJoin<D> * sizeof(float);
   // tiles, peaks, and what the pairs of waves share; the outputs' way out
   constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 128) : 0);
   constexpr size_t rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
   constexpr size_t many = staged > rows_out ? staged : rows_out;
   // (ids of kernels with more than 64 KiB: one of each kind needs one of 256 dims, the many rows' one of 128)
   int rc;
-  if (s.rows == 256) rc = go(kv_attend_rows_kernel<D, FP8>, D == 256 ? 2 : 3, blocks, 512, many);
-  else rc = go(kv_attend_kernel<D, FP8>, 1, s.rows == 32 ? (blocks + 7) / 8 * 16 : blocks, 256, joined);
+  if (s.few_work > 0) rc = go(kv_attend_kernel<D, FP8, true>, 3 + D / 64, blocks, 512, many > 2 * joined ? many : 2 * joined);
+  else if (s.rows == 256) rc = go(kv_attend_rows_kernel<D, FP8>, D == 256 ? 2 : 3, blocks, 512, many);
+  else rc = go(kv_attend_kernel<D, FP8, false>, 1, s.rows == 32 ? (blocks + 7) / 8 * 16 : blocks, 256, joined);
   if (rc) return rc;
   const unsigned merges = s.max_merges * s.kv_heads;
   const unsigned waves = (unsigned)(s.merge_rows + 31) / 32 * (D == 256 ? 2 : 1);  // of a unit that have rows
-  if (s.rows == 256) hipLaunchKernelGGL(kv_merge_rows_kernel<D>, dim3(merges, waves), dim3(512), 0, st, d);
+  if (s.few_work > 0) hipLaunchKernelGGL(kv_merge_either_kernel<D>, dim3(merges, 32), dim3(512), 0, st, d);
+  else if (s.rows == 256) hipLaunchKernelGGL(kv_merge_rows_kernel<D>, dim3(merges, waves), dim3(512), 0, st, d);
   else hipLaunchKernelGGL(kv_merge_kernel<D>, dim3(merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
   return sq_internal_launched("kv_merge_kernel");
 }

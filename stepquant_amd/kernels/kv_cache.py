@@ -219,10 +219,19 @@ class BlockTables:
     # 14.1 with 4, 16.7 with 8); other dims are alike from 1 to 8.
     min_tiles = {16: 2, 32: 2, 256: 4}
     # What partial results cost, in tiles: 64 requests of up to 8192 take 116 us
-    # cut, 131 uncut; 160 of up to 4096 and 32 rows 223 us with 4 here, 210 with 16;
-    # prompts of up to 2048 and 7 rows a token 77 us with 16,
-    # 58 with 24; a prompt of 8192 tokens 543 us uncut, 709 cut (with 0 here).
-    cut_tiles = {16: 4, 32: 16, 256: 24}
+    # cut, 131 uncut; 160 of up to 4096 and 32 rows 223 us with 4 here, 210 with 8 to
+    # 16, but 64 tokens over 1000 (256 dims) 36 us with 16, 28 with 12; prompts of up
+    # to 2048 and 7 rows a token 77 us with 16, 58 with 24; a prompt of 8192 tokens
+    # 543 us uncut, 709 cut (with 0 here).
+    cut_tiles = {16: 4, 32: 12, 256: 24}
+    # A tile is 2 us of a set of 256, and its start and end 10 more; a short prompt
+    # ends sooner in sets of 32, all at a time (128 tokens of 32 heads over 500: 30 us
+    # in sets of 256, 21 so; 64 of 256 dims over 1000: 94 and 28; but 64 over 8000 of
+    # 128 dims 34 and 45).  So for up to `few_rows` query rows of all heads the plan
+    # kernel, which knows the lengths, decides: sets of 32 where rows times the tiles
+    # that they see are at most `few_work` (the two meet near 2^17 for 128 dims, 2^18
+    # for 64 and 2^18.5 for 256).
+    few_rows, few_work = 1 << 14, 3 << 16
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows):
         """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all
@@ -239,17 +248,19 @@ class BlockTables:
             rows = max_new * group
             rows = 16 if rows <= 16 else 32 if rows <= 64 else 256
             slots = 2 * self._cus if rows == 16 else self._cus
-            sets, cuts = -(-tokens * group // rows) + batch + 1, max(1, slots // kv_heads)
+            few = rows == 256 and tokens * q_heads <= self.few_rows
+            sets, cuts = -(-tokens * group // (32 if few else rows)) + batch + 1, max(1, slots // kv_heads)
             workers, joins = max(sets, cuts), min(sets, cuts)
             sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
             for w in windows if tokens else ():
                 units = 4 * sum(sizes)
                 merges = units + 32 * (sets + cuts)
                 numbers = (sets + cuts, joins, workers, 2 * cuts, q_heads, kv_heads, rows, causal, int(w), slots,
-                           self.min_tiles[rows], self.cut_tiles[rows], max(1, min(rows, max_new * group)), 0)
+                           self.min_tiles[rows], self.cut_tiles[rows], max(1, min(rows, max_new * group)),
+                           self.few_work if few else 0, self.min_tiles[32], self.cut_tiles[32])
                 schedules.append((int(w), q_heads, kv_heads, 2 * cuts * kv_heads * rows, units, merges,
                                   merges + 32 * joins, numbers))
-                sizes.append(8 * (sets + cuts + joins) + (workers + 8) // 8 * 8)
+                sizes.append(8 * (sets + cuts + joins) + (workers + 9) // 8 * 8)
         offsets = [4 * sum(sizes[:i]) for i in range(7)]
         return sizes, sum(sizes), offsets, most, schedules
 

@@ -390,6 +390,19 @@ def test_attention(case):
     assert torch.equal(got, cache.attend(q.flatten(1), plan))
 
 
+@pytest.fixture(params=[(0, 0), (1 << 14, 1)], ids=["256", "256-decided"])
+def sets_of_256(request, monkeypatch):
+    """Sets of 256 rows, which short prompts would not get: asked for, or as the plan decides."""
+    monkeypatch.setattr(BlockTables, "few_rows", request.param[0])
+    monkeypatch.setattr(BlockTables, "few_work", request.param[1])
+
+
+@pytest.mark.parametrize("case", [c for c in CASES if max(c[7]) * (c[0] // c[1]) > 64],
+                         ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_attention_in_sets_of_256(case, sets_of_256):
+    test_attention(case)
+
+
 def filled(old, new, Hq=8, H=2, D=128, P=64, storage="int8", seed=0, **kw):
     g = rng(seed, Hq, D)
     tables, cache = make(len(old), H, D, P, storage, max(o + n for o, n in zip(old, new)))
@@ -610,6 +623,56 @@ def test_scores_beyond_fractions(D, new):
                 want = x[1][s.argmax()]
                 assert (np.abs(got[t, h] - want) <= np.abs(want) * 2. ** -10 + 2. ** -24).all(), (t, h)
     assert clear >= new
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_sizes_and_scores_in_sets_of_256(D, sets_of_256):
+    test_values_of_very_different_sizes(D, 90)
+    test_scores_beyond_fractions(D, 90)
+    for scale in (-.1, 0., 3.):
+        test_scales_of_any_sign(D, 40, scale)
+
+
+@pytest.mark.parametrize("storage", ["int8", "fp8"])
+def test_a_bad_block_in_sets_of_256(storage, sets_of_256):
+    test_a_bad_block_reaches_only_rows_that_see_it(storage)
+
+
+def test_prompts_of_many_sets_in_sets_of_256(sets_of_256):
+    test_prompts_of_many_sets_of_rows(4, 2, 128, [900, 70], [333, 400], True)
+    test_prompts_of_many_sets_of_rows(2, 1, 256, [64], [520], False)
+
+
+def test_a_graph_follows_the_lengths():
+    """Chunks of 40 tokens, captured once: the plan takes sets of 32 rows while the
+    requests are short and of 256 when they have grown."""
+    H, Hq, D, n = 2, 16, 128, 40
+    g = rng(47)
+    tables, cache = make(1, H, D, 64, "int8", 18 * n + 1)
+    new, rows = torch.tensor([n], dtype=torch.int32, device=dev()), torch.zeros(1, dtype=torch.int32, device=dev())
+    q, k, v = (torch.empty((n, h, D), dtype=torch.bfloat16, device=dev()) for h in (Hq, H, H))
+    tables.few_work = n * Hq * 6  # (tiles of the chunk's middle: up to five)
+    warm = tables.plan(new, rows, tokens=n, max_new=n, heads=(Hq, H))
+    for t in (q, k, v):
+        t.zero_()
+    cache.append(k, v, warm)
+    cache.attend(q, warm)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            plan = tables.plan(new, rows, tokens=n, max_new=n, heads=(Hq, H))
+            cache.append(k, v, plan)
+            out = cache.attend(q, plan)
+            tables.commit(plan)
+    for i in range(18):
+        for t in (q, k, v):
+            t.copy_(values(g, t.shape, torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attend(tables, cache, plan, [0], [n * i], [n], q, out=out)
+    assert tables.lens.tolist() == [18 * n]
 
 
 def test_refused_requests_give_zero():

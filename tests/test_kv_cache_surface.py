@@ -78,7 +78,11 @@ def test_caches_are_checked_before_any_launch(cache, code):
     ({}, {}, dict(window=3, causal=0)), ({}, {}, dict(window=-1)), ({}, {}, dict(slots=0)), ({}, {}, dict(max_units=262)),
     ({}, {}, dict(max_merges=6)), ({}, {}, dict(max_partials=511)), ({}, {}, dict(max_workers=255)),
     ({}, {}, dict(slots=4097)), ({}, {}, dict(starts=None)), ({}, {}, dict(cut_tiles=-1)), ({}, {}, dict(min_tiles=0)),
-    ({}, {}, dict(merge_rows=15)), ({}, {}, dict(merge_rows=17))])
+    ({}, {}, dict(merge_rows=15)), ({}, {}, dict(merge_rows=17)), ({}, {}, dict(few_work=-1)),
+    ({}, {}, dict(few_work=9, few_min_tiles=1)), ({}, {}, dict(few_work=9, rows=256, few_min_tiles=0)),
+    ({}, {}, dict(few_work=9, rows=256, few_min_tiles=1, few_cut_tiles=-1)),
+    # (room for sets of 256 rows only)
+    ({}, {}, dict(few_work=9, rows=256, few_min_tiles=1, max_units=1 + 3 + 256))])
 def test_plans_are_checked_before_any_launch(tables, plan, schedule):
     rc = N.lib().sq_kv_plan(_tables(**tables), _plan(_schedule(**schedule), **plan), None)
     assert rc in (-22, -23) and b"kv " in N.lib().sq_last_error()
