@@ -569,13 +569,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
   if (tid == 0) *peak_at = peak;
   const uint32_t zero = FP8 ? 0u : 0x80808080u;
   if (peak != before) {
+    // both peaks 2^-32 of their size where a code times one would pass 32 bits
+    const float down = peak > 0x1p100f ? 0x1p-32f : 1.f, was = before * down, now = peak * down, inv_now = 1.f / now;
     for (int g = tid; g < from; g += 256) {
       uint2 w = *(const uint2 *)(base + 8 * (int64_t)g);
       float y[8];
       decode4<FP8>(w.x, y);
       decode4<FP8>(w.y, y + 4);
 #pragma unroll
-      for (int k = 0; k < 8; k++) y[k] = quotient(y[k] * before, peak, inv);
+      for (int k = 0; k < 8; k++) y[k] = quotient(y[k] * was, now, inv_now);
       w.x = good ? code4<FP8>(y) : zero;
       w.y = good ? code4<FP8>(y + 4) : zero;
       *(uint2 *)(base + 8 * (int64_t)g) = w;
