@@ -732,6 +732,11 @@ constexpr float kKeyUnit = FP8 ? 1.f / 448.f : 1.f / 127.f;
 template <bool FP8>
 constexpr float kValueUnit = FP8 ? 1.f / 448.f : 1024.f / 127.f;
 
+// Outputs that are sums over keys, not yet divided by the sum of weights, are
+// held 2^-40 of their size: as many of the largest values as a row can see stay
+// within 32 bits, and the least peak's stay normal numbers.
+constexpr float kRoom = 0x1p40f;
+
 // The power of two that brings a bfloat16 row with this largest magnitude, in
 // [2^e, 2^(e+1)), below 2^15, and its inverse.
 __device__ __forceinline__ void row_shift(float most, float *shift, float *unit) {
@@ -1214,7 +1219,7 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
         for (int k = 0; k < 16; k++) {
           vec x;
 #pragma unroll
-          for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit * root;
+          for (int e = 0; e < OT; e++) x[e] = o[e][k] * unit * (root / kRoom);
           *(vec *)(dst + k * 64 * OT) = x;
         }
         if (live && hl == 0 && e0 == 0) {
@@ -1441,7 +1446,7 @@ __global__ __launch_bounds__(EITHER ? 512 : 256, 2) void kv_attend_kernel(Attend
       for (int t = 0; t < NT / 2; t++) pf[t] = __builtin_bit_cast(half8_v, w[t]);
       // a row that sees none of the step takes nothing from it, whatever its peak
       const bool some = whole || (known && first < hi && first + STEP > lo);
-      const float sv = some ? peak.y * kValueUnit<FP8> : 0.f;
+      const float sv = some ? peak.y * (kValueUnit<FP8> / kRoom) : 0.f;
       auto value = [&](auto E) {
         constexpr int e = decltype(E)::value;
         half8_v v[NT / 2];
@@ -1496,7 +1501,7 @@ __global__ __launch_bounds__(EITHER ? 512 : 256, 2) void kv_attend_kernel(Attend
       }
       const int f = u.f0 + j;
       if (u.part < 0) {
-        x *= all == 0.f ? 0.f : 1.f / all;
+        x *= all == 0.f ? 0.f : kRoom / all;
         const int t = f / G, head = h * G + f - t * G;
         store_row<4>(a.out + ((int64_t)(u.q0 + t) * a.q_heads + head) * D + d, a.dtype == SQ_BF16, (const float *)&x);
       } else {
@@ -1567,7 +1572,7 @@ __device__ __forceinline__ void merge_few(const AttendDev &a, int unit_rows) {
     x += part_o[i][lane] * w;
     sum = fmaf(part_l[i], w, sum);
   }
-  x *= sum == 0.f ? 0.f : 1.f / sum;
+  x *= sum == 0.f ? 0.f : kRoom / sum;
   const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
   store_row<4>(a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + 4 * lane, a.dtype == SQ_BF16, (const float *)&x);
 }
@@ -1622,7 +1627,7 @@ __device__ __forceinline__ void merge_many(const AttendDev &a) {
   const float high = fmaxf(mm, other.x), base = high == -INFINITY ? 0.f : high;
   float mine = __builtin_amdgcn_exp2f(mm - base), theirs = __builtin_amdgcn_exp2f(other.x - base);
   sum = fmaf(sum, mine, other.y * theirs);
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  const float f = sum == 0.f ? 0.f : kRoom / sum;
   mine *= f, theirs *= f;
   const int t = (f0 + j) / G, head = h * G + f0 + j - t * G;
   uint16_t *dst = a.out + ((int64_t)(q0 + t) * a.q_heads + head) * D + e0;

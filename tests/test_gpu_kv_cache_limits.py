@@ -5,8 +5,9 @@ import numpy as np
 import pytest
 import torch
 
+from stepquant_amd.kernels.kv_cache import BlockTables
 from tests.helpers import dev
-from tests.test_gpu_kv_cache import check_append, make, rng
+from tests.test_gpu_kv_cache import TOP, check_append, make, page_parts, rng
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +28,76 @@ def test_large_blocks_grow(storage, sizes):
         tables.commit(plan)
     k, v = cache.decode(plan.pages, plan.filled)
     assert torch.isfinite(k).all() and torch.isfinite(v).all()
+
+
+# ---------------------------------------------------------------- attention
+@pytest.fixture(params=[(0, 0), (1 << 14, 1)], ids=["256", "256-decided"])
+def sets_of_256(request, monkeypatch):
+    """Sets of 256 rows, which short prompts would not get: asked for, or as the plan decides."""
+    monkeypatch.setattr(BlockTables, "few_rows", request.param[0])
+    monkeypatch.setattr(BlockTables, "few_work", request.param[1])
+
+
+def attended(k, v, q, storage="int8", workgroups=None):
+    """One request of one KV head: the first keys held, the others new beside ``q``
+    [new, heads, D].  (outputs, keys, values and their blocks' peaks as held, in 64 bits)"""
+    n, D = k.shape
+    new, Hq, _ = q.shape
+    tables, cache = make(1, 1, D, 64, storage, n)
+    if workgroups:  # few, so that each of them has many keys
+        tables._cus = workgroups
+    k, v = k.view(n, 1, D), v.view(n, 1, D)
+    first = tables.plan([n - new])
+    cache.append(k[:n - new], v[:n - new], first)
+    tables.commit(first)
+    plan = tables.plan([new], heads=(Hq, 1))
+    cache.append(k[n - new:], v[n - new:], plan)
+    got = cache.attend(q, plan).double().cpu().numpy()
+    codes, peaks = page_parts(cache)
+    ids = tables.table.cpu().numpy()[0, :-(-n // 64)]
+    peaks = peaks[ids, 0].astype(np.float64)
+    keys, vals = (codes[ids, 0] * (peaks / TOP[storage])[..., None, None]).transpose(1, 0, 2, 3).reshape(2, -1, D)[:, :n]
+    return got, keys, vals, np.repeat(peaks[:, 1], 64)[:n]
+
+
+def check_sums(got, keys, vals, peak, q):
+    """Halves of weights (2^-11) in the products and in the sums, 32-bit sums, one
+    rounding at the end.  A weight has all its bits down to 2^-21 of a row's
+    largest and is 0 below 2^-31 of it (of the largest weight times a block's peak
+    in the products)."""
+    new, Hq, D = q.shape
+    x, unit = q.double().cpu().numpy(), 2. ** -8 if q.dtype == torch.bfloat16 else 2. ** -11
+    worst = 0.
+    for t in range(new):
+        n = len(keys) - new + t + 1
+        s = x[t] @ keys[:n].T * D ** -.5
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        want, size = p @ vals[:n], p @ np.abs(vals[:n])
+        ds = (D + 8) * 2. ** -24 * D ** -.5 * (np.abs(x[t]) @ np.abs(keys[:n]).T).max(1)[:, None]
+        tol = size * (2. ** -10 + 2 * ds + (n / 16 + 64) * 2. ** -23) + np.abs(want) * unit * (1 + 2. ** -9)
+        tol += n * 2. ** -31 * ((p * peak[:n]).max(1)[:, None] + np.abs(want)) + 2. ** -25
+        worst = max(worst, float((np.abs(got[t] - want) / tol).max())) if np.isfinite(got[t]).all() else np.inf
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 90])
+@pytest.mark.parametrize("storage", ["int8", "fp8"])
+def test_values_near_the_largest(D, new, storage):
+    """Outputs are finite where values are, however many of them a row sums."""
+    print(f"case {new} new tokens of {D} dims, {storage}", flush=True)
+    g = rng(52, D, new)
+    n = 2000 + new
+    sign = np.where(g.random(D) < .5, -1., 1.)
+    k = torch.from_numpy(g.standard_normal((n, D)) * .1).to(dev(), torch.bfloat16)
+    v = torch.from_numpy(g.uniform(.3, 1, (n, D)) * sign * 3.3e38).to(dev(), torch.bfloat16)
+    q = torch.from_numpy(g.standard_normal((new, 4, D))).to(dev(), torch.bfloat16)
+    check_sums(*attended(k, v, q, storage), q)
+    check_sums(*attended(k, v, q, storage, workgroups=1), q)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("storage", ["int8", "fp8"])
+def test_values_near_the_largest_in_sets_of_256(D, storage, sets_of_256):
+    test_values_near_the_largest(D, 90, storage)
