@@ -1426,7 +1426,12 @@ __global__ __launch_bounds__(EITHER ? 512 : 256, 2) void kv_attend_kernel(Attend
           s[t][k] = x;
           best = fmaxf(best, x);
         }
-      best = fmaxf(reduce_max4(best), m);
+      // Weights are in units of 2^m, 15 below the row's largest score: a half then
+      // holds all bits of a weight down to 2^-29 of the row's largest, and some down
+      // to 2^-39.  (Scores past 2^20, of which 32 bits hold no fine fractions, as
+      // they are: the difference of 15 would be rounded, and 65504 passed.)
+      best = reduce_max4(best);
+      best = fmaxf(fabsf(best) < 0x1p20f ? best - 15.f : best, m);
       const float base = best == -INFINITY ? 0.f : best;
       const float alpha = __builtin_amdgcn_exp2f(m - base);
       const bool keep = __all(m == best);

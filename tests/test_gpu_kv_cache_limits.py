@@ -101,3 +101,20 @@ def test_values_near_the_largest(D, new, storage):
 @pytest.mark.parametrize("storage", ["int8", "fp8"])
 def test_values_near_the_largest_in_sets_of_256(D, storage, sets_of_256):
     test_values_near_the_largest(D, 90, storage)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 90])
+@pytest.mark.parametrize("depth,first", [(18, 128.), (18, 8.), (23, 0.), (26, 0.)])
+def test_many_small_weights_beside_a_large_one(D, new, depth, first):
+    """20,000 keys at 2^-depth of a row's first one, whose values are ``first``
+    times the others' or zero."""
+    print(f"case {new} new tokens of {D} dims, 2^-{depth}, {first}", flush=True)
+    g = rng(53, D, new, depth)
+    n = 20000 + new
+    k, v = g.standard_normal((n, D)) * .3, 1 + .3 * g.standard_normal((n, D))
+    k[0, 0], v[0] = depth * np.log(2.), first * (1 + .1 * g.standard_normal(D))
+    q = .02 * g.standard_normal((new, 4, D))
+    q[..., 0] = D ** .5 * g.uniform(1, 1.05, (new, 4))
+    k, v, q = (torch.from_numpy(a).to(dev(), torch.float16) for a in (k, v, q))
+    check_sums(*attended(k, v, q, workgroups=1), q)
