@@ -806,11 +806,12 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // operands ahead in place of 4.
 //
 // A row's sum is kept in units of 2^m, m its largest score so far, and its
-// outputs in units of 2^om, om the largest score and log2 of the block's value
+// outputs in units of 2^(m + gap), the largest score and log2 of the block's value
 // peak together: so what enters the products as halves is a probability times
-// its block's peak, whichever blocks the row's outputs come from.  Both are
-// raised only when one is passed by more than 2^8.  They start at a number below
-// every score, so that no difference of them needs care.
+// its block's peak, whichever blocks the row's outputs come from.  (The gap by
+// itself, as 32 bits do not hold it beside a score past 2^24.)  Both are
+// raised only when one is passed by more than 2^8.  m starts at a number below
+// every score, so that no difference of it needs care.
 template <int D, bool FP8>
 __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
   constexpr int KS = D / 16, DT = D / 32;                   // k steps and dim tiles
@@ -840,10 +841,10 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
     uint4 *const kb = tiles, *const vb = tiles + 2 * KB;
     // the peaks of two tiles, and whether their pages exist
     float4 *const peaks = (float4 *)(vb + 2 * VB);
-    // (pairs) probabilities of a wave, and its rows' maxima, then sums
+    // (pairs) probabilities of a wave, and its rows' units, then sums
     uint4 *const shared = (uint4 *)(peaks + 2), *const passed = shared + wave * 128, *const taken = shared + (wave ^ 1) * 128;
-    float *const shared_m = (float *)(shared + 8 * 128);
-    float *const passed_m = shared_m + wave * 32, *const taken_m = shared_m + (wave ^ 1) * 32;
+    float2 *const shared_m = (float2 *)(shared + 8 * 128);
+    float2 *const passed_m = shared_m + wave * 32, *const taken_m = shared_m + (wave ^ 1) * 32;
     const int pages = (int)a.c.num_pages, first_key = 2 * h * P * D;
     const uint32_t page_bytes = (uint32_t)a.c.page_bytes;
 
@@ -893,8 +894,8 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
       for (int e = 0; e < OT; e++)
 #pragma unroll
         for (int k = 0; k < 16; k++) o[e][k] = 0.f;
-      float m = kNone, l = 0.f, om = kNone;
-      float both = kNone;  // (pairs) what the outputs are in units of: the larger of the two waves' om
+      float m = kNone, l = 0.f, gap = 0.f;
+      float both = kNone, both_gap = 0.f;  // (pairs) m and gap of the outputs: the larger unit of the two waves'
 
       // The tiles in order; past the last one the last again, so that loads ahead
       // need no branch.  The lanes hold where the pages of 64 tiles lie (all ones:
@@ -966,20 +967,23 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
 #pragma unroll
           for (int j = 0; j < 4; j++) pv[j] = pf[j];
         } else if constexpr (NV > 0) {
-          // own probabilities and the other wave's, brought to one maximum: maxima
-          // are whole numbers here, so that the factors are powers of two
+          // own probabilities and the other wave's, brought to one unit: units are
+          // whole numbers here, so that the factors are powers of two
           const uint4 w0 = taken[lane], w1 = taken[64 + lane];
-          const float theirs = taken_m[c], high = fmaxf(om, theirs);
+          const float2 theirs = taken_m[c];
+          const float over = (theirs.x - m) + (theirs.y - gap);  // their unit above the own one
+          const float high = over > 0.f ? theirs.x : m, high_gap = over > 0.f ? theirs.y : gap;
+          const float rise = (high - both) + (high_gap - both_gap);
           pv[0] = pf[0], pv[1] = pf[1];
           pv[2] = __builtin_bit_cast(half8_v, w0), pv[3] = __builtin_bit_cast(half8_v, w1);
-          if (__any(om != theirs)) {
-            const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(om - high);
-            const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(theirs - high);
+          if (__any(over != 0.f)) {
+            const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(fminf(-over, 0.f));
+            const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(fminf(over, 0.f));
             pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
           }
-          if (__any(high > both)) {
-            const float shrink = __builtin_amdgcn_exp2f(both - high);
-            both = high;
+          if (__any(rise > 0.f)) {
+            const float shrink = __builtin_amdgcn_exp2f(fminf(-rise, 0.f));
+            if (rise > 0.f) both = high, both_gap = high_gap;
 #pragma unroll
             for (int e = 0; e < OT; e++)
 #pragma unroll
@@ -1047,20 +1051,21 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
         best *= f;
         // the halves are the probabilities times 2^size
         const float part = some ? __builtin_amdgcn_logf(peak.y) : 0.f;
-        float off = part - om, size = part + (m - om);
-        const float raised = fmaxf(m, best), by = best - m;
+        float size = part - gap, off = size - m;
+        const float raised = fmaxf(m, PAIRS ? ceilf(best) : best), by = best - m;
         if (__any(fmaxf(fmaxf(by, by + size), fmaxf(-size, fabsf(raised) * kLarge)) > 8.f)) {
-          const float top = fmaxf(om, PAIRS ? ceilf(best + part) : best + part);
-          const float shrink = __builtin_amdgcn_exp2f(om - top);
+          const float was = gap + (m - raised), wanted = (best - raised) + part;
+          gap = fmaxf(was, PAIRS ? ceilf(wanted) : wanted);
+          const float shrink = __builtin_amdgcn_exp2f(was - gap);
           l *= __builtin_amdgcn_exp2f(m - raised);
-          m = raised, om = top;
+          m = raised;
           if constexpr (!PAIRS) {
 #pragma unroll
             for (int e = 0; e < OT; e++)
 #pragma unroll
               for (int k = 0; k < 16; k++) o[e][k] *= shrink;
           }
-          off = part - om, size = part + (m - om);
+          size = part - gap, off = size - m;
           float less = m;
           if (__any(fabsf(m) * kLarge > 8.f)) {
             // scores of which 32 bits hold no fractions: rounded before the difference,
@@ -1095,7 +1100,7 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
         if constexpr (PAIRS) {
           passed[lane] = __builtin_bit_cast(uint4, pf[0]);
           passed[64 + lane] = __builtin_bit_cast(uint4, pf[1]);
-          if (hl == 0) passed_m[c] = om;
+          if (hl == 0) passed_m[c] = make_float2(m, gap);
         }
       };
 
@@ -1160,19 +1165,17 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
       l = reduce_sum2(l);
       if constexpr (PAIRS) {
         // the two waves' sums, brought to one maximum (their last products are done)
-        if (hl == 0) {
-          passed_m[c] = m;
-          ((float *)passed)[c] = l;
-        }
+        if (hl == 0) passed_m[c] = make_float2(m, l);
         __syncthreads();
-        const float theirs = taken_m[c], high = fmaxf(m, theirs);
-        l = fmaf(l, __builtin_amdgcn_exp2f(m - high), ((float *)taken)[c] * __builtin_amdgcn_exp2f(theirs - high));
+        const float2 theirs = taken_m[c];
+        const float high = fmaxf(m, theirs.x);
+        l = fmaf(l, __builtin_amdgcn_exp2f(m - high), theirs.y * __builtin_amdgcn_exp2f(theirs.x - high));
         m = high;
-        om = both;
+        gap = (both - high) + both_gap;
         __syncthreads();
       }
       // the outputs' unit beside the sum's, in two factors: 2^128 is in reach
-      const float root = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(.5f * (om - m)), unit = root * kValueUnit<FP8>;
+      const float root = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(.5f * gap), unit = root * kValueUnit<FP8>;
       if (part < 0) {
         // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
         constexpr int OD = 32 * OT, OW = OD * 2 + 8;  // a wave's dims of a row, and the bytes from row to row
@@ -1769,7 +1772,7 @@ int launch_attend(const AttendDev &d, const sq_kv_schedule &s, hipStream_t st) {
   };
   constexpr size_t joined = kJoin<D> * sizeof(float);
   // tiles, peaks, and what the pairs of waves share; the outputs' way out
-  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 128) : 0);
+  constexpr size_t staged = 2 * sizeof(uint4) * (2 * (D / 16) * 65 + 4 * (D / 32) * 64 + 1) + (D == 256 ? 8 * (2048 + 256) : 0);
   constexpr size_t rows_out = 256 * (D == 256 ? 264 : 2 * D + 8);
   constexpr size_t many = staged > rows_out ? staged : rows_out;
   // (ids of kernels with more than 64 KiB: one of each kind needs one of 256 dims, the many rows' one of 128)

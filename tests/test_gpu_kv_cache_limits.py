@@ -118,3 +118,42 @@ def test_many_small_weights_beside_a_large_one(D, new, depth, first):
     q[..., 0] = D ** .5 * g.uniform(1, 1.05, (new, 4))
     k, v, q = (torch.from_numpy(a).to(dev(), torch.float16) for a in (k, v, q))
     check_sums(*attended(k, v, q, workgroups=1), q)
+
+
+def check_winners(got, keys, vals, q):
+    """Rows whose largest score is clear of the second by more than their error."""
+    new, Hq, D = q.shape
+    x, clear = q.double().cpu().numpy(), 0
+    for t in range(new):
+        n = len(keys) - new + t + 1
+        for h in range(Hq):
+            s = keys[:n] @ x[t, h] * D ** -.5
+            other, best = np.sort(s)[-2:]
+            if best - other > 2 * ((D + 8) * 2. ** -24 * np.abs(s).max() * D ** .5 + 100):
+                clear += 1
+                want = vals[s.argmax()]
+                tol = np.abs(want) * (2. ** -8 * (1 + 2. ** -9) + 2. ** -10) + np.abs(want).max() * 2. ** -22
+                assert (np.abs(got[t, h] - want) <= tol).all(), (t, h, got[t, h][:4], want[:4])
+    assert clear >= new
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_scores_past_2_30_and_values_of_any_size(D, new):
+    """Where 32 bits hold no difference of 100 between scores, blocks' value
+    peaks still come out as they are."""
+    print(f"case {new} new tokens of {D} dims", flush=True)
+    g = rng(54, D, new)
+    n = 320 + new
+    sizes = np.repeat([2. ** 40, 2. ** -20, 2. ** 100, 1., 2. ** -50, 2. ** 17, 2. ** 10], 64)[:n]
+    k, q = 1e5 * g.standard_normal((n, D)), 1e5 * g.standard_normal((new, 4, D))
+    v = g.standard_normal((n, D)) * sizes[:, None]
+    k, v, q = (torch.from_numpy(a).to(dev(), torch.bfloat16) for a in (k, v, q))
+    got, keys, vals, _ = attended(k, v, q)
+    assert np.isfinite(got).all()
+    check_winners(got, keys, vals, q)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_past_2_30_in_sets_of_256(D, sets_of_256):
+    test_scores_past_2_30_and_values_of_any_size(D, 90)
