@@ -25,7 +25,7 @@ typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
 
 constexpr float kFloor = 8.673617379884035e-19f;  // 2^-60, the least peak of a block
 constexpr float kNone = -3e38f;                   // a row's largest score before it has seen a key
-constexpr float kLarge = 0x1p-17f;                // a score above 8 / this is large (in log2)
+constexpr float kLarge = 0x1p20f;                 // scores from here on (in log2) hold no fine fractions
 constexpr int kTile = 64;                         // keys of one attention tile
 
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -684,6 +684,13 @@ __device__ __forceinline__ float reduce_sum4(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The unit of a row's weights: `below` the largest score, so that more of the
+// small weights are halves.  Large scores as they are: the difference would be
+// rounded, and the largest weight pass what a half holds.
+__device__ __forceinline__ float weight_unit(float best, float below) {
+  return fabsf(best) < kLarge ? best - below : best;
+}
+
 __device__ __forceinline__ uint32_t half2_bits(half2_v h) { return __builtin_bit_cast(uint32_t, h); }
 
 // Two probabilities as the halves that enter the products, their sum added in
@@ -805,13 +812,20 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // groups below ask for takes 3% off; wave priorities change nothing, nor do 8
 // operands ahead in place of 4.
 //
-// A row's sum is kept in units of 2^m, m its largest score so far, and its
-// outputs in units of 2^(m + gap), the largest score and log2 of the block's value
-// peak together: so what enters the products as halves is a probability times
-// its block's peak, whichever blocks the row's outputs come from.  (The gap by
-// itself, as 32 bits do not hold it beside a score past 2^24.)  Both are
-// raised only when one is passed by more than 2^8.  m starts at a number below
-// every score, so that no difference of it needs care.
+// A row's sum is kept in units of 2^m, m kBias below its largest score, and its
+// outputs in units of 2^(m + gap), such that the largest score and log2 of the
+// block's value peak together make 2^kBias: so what enters the products as halves
+// is a probability times its block's peak, whichever blocks the row's outputs come
+// from.  (The gap by itself, as 32 bits do not hold it beside a score past 2^24.)
+// Both are raised only when a half or a weight would pass 2^kTop; so halves hold all
+// bits of a product down to 2^-24 of the row's largest and some down to 2^-34.
+// Where a block's values are smaller than others by more than 2^kSmall, the sum
+// takes its weights before they are halves: it has all bits of those down to 2^-20
+// of the largest.  (A prompt of 8192 tokens: 611 us with units raised at 2^8 above
+// the largest half, which leaves 3 bits less, 615 so, 622 with 11 for kBias.)  m
+// starts at a number below every score, so that no difference of it needs care.
+constexpr float kBias = 10.f, kTop = 15.f, kSmall = 4.f;
+
 template <int D, bool FP8>
 __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
   constexpr int KS = D / 16, DT = D / 32;                   // k steps and dim tiles
@@ -977,9 +991,18 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
           pv[0] = pf[0], pv[1] = pf[1];
           pv[2] = __builtin_bit_cast(half8_v, w0), pv[3] = __builtin_bit_cast(half8_v, w1);
           if (__any(over != 0.f)) {
-            const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(fminf(-over, 0.f));
-            const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(fminf(over, 0.f));
-            pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
+            auto scale = [&](float e0, float e1) {
+              const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(e0), f1 = (_Float16)__builtin_amdgcn_exp2f(e1);
+              pv[0] *= f0, pv[1] *= f0, pv[2] *= f1, pv[3] *= f1;
+            };
+            scale(fmaxf(fminf(-over, 0.f), -14.f), fmaxf(fminf(over, 0.f), -14.f));
+            // (in two factors where one would be too small for a half)
+            if (__any(fabsf(over) > 14.f)) scale(fminf(14.f - over, 0.f), fminf(14.f + over, 0.f));
+            // both go on with the larger unit, for weights and for outputs
+            const float top = fmaxf(m, theirs.x);
+            gap = over > 0.f ? theirs.y + (theirs.x - top) : gap + (m - top);
+            l *= __builtin_amdgcn_exp2f(m - top);
+            m = top;
           }
           if (__any(rise > 0.f)) {
             const float shrink = __builtin_amdgcn_exp2f(fminf(-rise, 0.f));
@@ -1052,10 +1075,12 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
         // the halves are the probabilities times 2^size
         const float part = some ? __builtin_amdgcn_logf(peak.y) : 0.f;
         float size = part - gap, off = size - m;
-        const float raised = fmaxf(m, PAIRS ? ceilf(best) : best), by = best - m;
-        if (__any(fmaxf(fmaxf(by, by + size), fmaxf(-size, fabsf(raised) * kLarge)) > 8.f)) {
-          const float was = gap + (m - raised), wanted = (best - raised) + part;
-          gap = fmaxf(was, PAIRS ? ceilf(wanted) : wanted);
+        const float by = best - m;
+        // (m of large scores, in units in which 2^20 passes kTop)
+        if (__any(fmaxf(fmaxf(by, by + size), fmaxf(size * (-kTop / kSmall), fabsf(fmaxf(m, best)) * 0x1p-16f)) > kTop)) {
+          const float unit = weight_unit(best, kBias), raised = fmaxf(m, PAIRS ? floorf(unit) : unit);
+          const float was = gap + (m - raised), wanted = (best - raised) + (part - kBias);
+          gap = fmaxf(was, PAIRS ? floorf(wanted) : wanted);
           const float shrink = __builtin_amdgcn_exp2f(was - gap);
           l *= __builtin_amdgcn_exp2f(m - raised);
           m = raised;
@@ -1067,14 +1092,14 @@ __device__ __forceinline__ void attend_many(const AttendDev &a, uint4 *tiles) {
           }
           size = part - gap, off = size - m;
           float less = m;
-          if (__any(fabsf(m) * kLarge > 8.f)) {
-            // scores of which 32 bits hold no fractions: rounded before the difference,
+          if (__any(fabsf(m) >= kLarge - kBias)) {
+            // scores of which 32 bits hold no fine fractions: rounded before the difference,
             // as the maximum is, so that no weight exceeds what a half holds
 #pragma unroll
             for (int k = 0; k < 16 * ST; k++) s[k >> 4][k & 15] = s[k >> 4][k & 15] * f - m;
             f = 1.f, off = size, less = 0.f;
           }
-          if (__any(size < -8.f)) {  // small values: as halves, some of their probabilities would be missing in the sum
+          if (__any(size < -kSmall)) {  // small values: as halves, some of their probabilities would be missing in the sum
 #pragma unroll
             for (int k = 0; k < 16 * ST; k++) l += __builtin_amdgcn_exp2f(fmaf(s[k >> 4][k & 15], f, -less));
             size = -kNone;
@@ -1431,10 +1456,8 @@ __global__ __launch_bounds__(EITHER ? 512 : 256, 2) void kv_attend_kernel(Attend
         }
       // Weights are in units of 2^m, 15 below the row's largest score: a half then
       // holds all bits of a weight down to 2^-29 of the row's largest, and some down
-      // to 2^-39.  (Scores past 2^20, of which 32 bits hold no fine fractions, as
-      // they are: the difference of 15 would be rounded, and 65504 passed.)
-      best = reduce_max4(best);
-      best = fmaxf(fabsf(best) < 0x1p20f ? best - 15.f : best, m);
+      // to 2^-39.
+      best = fmaxf(weight_unit(reduce_max4(best), 15.f), m);
       const float base = best == -INFINITY ? 0.f : best;
       const float alpha = __builtin_amdgcn_exp2f(m - base);
       const bool keep = __all(m == best);
