@@ -745,12 +745,13 @@ constexpr float kValueUnit = FP8 ? 1.f / 448.f : 1024.f / 127.f;
 constexpr float kRoom = 0x1p40f;
 
 // The power of two that brings a bfloat16 row with this largest magnitude, in
-// [2^e, 2^(e+1)), below 2^15, and its inverse.
+// [2^e, 2^(e+1)), below 2^15, and its inverse.  Rows below 2^-100 come less far:
+// still within a half's normal numbers, and the inverse times a scale within those
+// of 32 bits.  Rows with an infinity or a NaN stay as they are.
 __device__ __forceinline__ void row_shift(float most, float *shift, float *unit) {
-  const int e = (int)(__float_as_uint(most) >> 23) - 127;
-  const bool usual = e > -100 && e < 100;
-  *shift = usual ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 1.f;
-  *unit = usual ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 1.f;
+  const int e = max((int)(__float_as_uint(most) >> 23) - 127, -100);
+  *shift = e < 128 ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 1.f;
+  *unit = e < 128 ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 1.f;
 }
 
 template <typename F, int... E>

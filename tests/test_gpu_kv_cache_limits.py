@@ -186,3 +186,27 @@ def test_a_bad_block_of_any_head_size(D, bad, sets_of_256):
         for a, b in ((out[:64 * block], clean[:64 * block]), (out[:, 4:], clean[:, 4:])):
             torch.testing.assert_close(a, b, rtol=2. ** -7, atol=2. ** -9)
         cache.data.copy_(kept)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 90])
+@pytest.mark.parametrize("size,keys_size", [(1e32, 1e-30), (1e32, 1e-16), (3e38, 1e-17), (2. ** -108, 2. ** 108),
+                                            (2. ** -120, 2. ** 120), (2. ** -126, 1.)])
+def test_queries_of_any_size(D, new, size, keys_size):
+    print(f"case {new} new tokens of {D} dims, queries of {size}, keys of {keys_size}", flush=True)
+    g = rng(55, D, new)
+    n = 320 + new
+    k, q = g.standard_normal((n, D)) * keys_size, np.clip(g.standard_normal((new, 4, D)) / 4, -1, 1) * size
+    v = g.standard_normal((n, D))
+    k, v, q = (torch.from_numpy(a).to(dev(), torch.bfloat16) for a in (k, v, q))
+    got, keys, vals, peak = attended(k, v, q)
+    if size * keys_size > 2 and keys.any():  # (keys below 2^-60 are zero as held)
+        check_winners(got, keys, vals, q)
+    else:
+        check_sums(got, keys, vals, peak, q)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size,keys_size", [(1e32, 1e-30), (3e38, 1e-17), (2. ** -120, 2. ** 120)])
+def test_queries_of_any_size_in_sets_of_256(D, size, keys_size, sets_of_256):
+    test_queries_of_any_size(D, 90, size, keys_size)
