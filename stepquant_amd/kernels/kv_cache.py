@@ -288,7 +288,8 @@ class KVCache:
     ``data`` [pages, page_bytes] uint8: per head the keys' and the values'
     codes [page_tokens, head_dim], then per head their two fp32 peaks.
     ``head_dim`` is 64, 128 or 256 and ``page_tokens`` a multiple of 64, with
-    at most 32,768 values of a head in a page.
+    at most 32,768 values of a head in a page.  A plan's block tables have the
+    same ``page_tokens`` and no more pages.
     """
 
     def __init__(self, pages, kv_heads, head_dim, *, page_tokens=64, storage="int8", device="cuda"):
@@ -343,6 +344,8 @@ class KVCache:
         tables = plan.tables
         if tables.page_tokens != self.page_tokens or tables.device != self.device:
             raise ValueError("the plan's block tables have other pages than the cache")
+        if tables.pages > self.pages:
+            raise ValueError(f"the plan's block tables give out {tables.pages} pages, the cache has {self.pages}")
 
     def append(self, k, v, plan):
         """Quantises the plan's new keys and values [tokens, kv_heads, head_dim]

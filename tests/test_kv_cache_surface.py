@@ -136,3 +136,25 @@ def test_python_surface_refuses_without_a_device():
             BlockTables(*a, device="cpu")
     with pytest.raises(ValueError):
         BlockTables(1, 4, 1, page_tokens=32, device="cpu")
+
+
+def _host_objects(cache_pages=6, table_pages=6):
+    """A cache and a plan of tables without their device memory, for checks before any launch."""
+    from types import SimpleNamespace
+    from stepquant_amd.kernels.kv_cache import KVCache
+    cpu = torch.device("cpu")
+    cache = KVCache.__new__(KVCache)
+    cache.pages, cache.heads, cache.dim, cache.page_tokens, cache.device = cache_pages, 2, 128, 64, cpu
+    return cache, SimpleNamespace(tokens=3, schedules={}, tables=SimpleNamespace(pages=table_pages, page_tokens=64, device=cpu))
+
+
+def test_plans_of_more_pages_than_the_cache_has_are_refused():
+    """Their tokens would be left out of the cache without an error."""
+    cache, plan = _host_objects(cache_pages=5)
+    k = torch.zeros((3, 2, 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="6 pages, the cache has 5"):
+        cache.append(k, k, plan)
+    with pytest.raises(ValueError, match="6 pages, the cache has 5"):
+        cache.attend(k, plan)
+    cache, plan = _host_objects(cache_pages=7)
+    cache._check_plan(plan)
