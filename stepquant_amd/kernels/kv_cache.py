@@ -156,7 +156,7 @@ class BlockTables:
                 raise ValueError("new tokens cannot be negative")
             tokens = sum(host) if tokens is None else tokens
             max_new = max(host, default=0) if max_new is None else max_new
-            new = torch.tensor(host, dtype=torch.int64)
+            new = torch.tensor([min(x, 0x7fffffff) for x in host], dtype=torch.int64)
         counts = self._index(new, "new")
         batch = counts.numel()
         if rows is None:
@@ -169,6 +169,8 @@ class BlockTables:
         tokens, max_new = int(tokens), min(int(max_new), 0x7fffffff)
         if tokens < 0 or max_new < 0:
             raise ValueError("tokens and max_new cannot be negative")
+        if tokens > 0x3fffffff:
+            raise ValueError("a plan takes fewer than 2^30 tokens")
         windows = tuple(window) if isinstance(window, (tuple, list)) else (window,)
         if len(windows) > N.KV_MAX_SCHEDULES or len(set(windows)) < len(windows):
             raise ValueError(f"a plan takes at most {N.KV_MAX_SCHEDULES} windows, each once")
@@ -245,6 +247,10 @@ class BlockTables:
             if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
                 raise ValueError("query heads must be a positive multiple of KV heads")
             group = q_heads // kv_heads
+            if q_heads > 0x7fffffff or tokens * group > 0x3fffffff:
+                raise ValueError("heads, or tokens times the heads of a group, too many")
+            if not all(0 <= int(w) <= 0x7fffffff for w in windows):
+                raise ValueError("a window is a non-negative 32-bit number")
             rows = max_new * group
             rows = 16 if rows <= 16 else 32 if rows <= 64 else 256
             slots = 2 * self._cus if rows == 16 else self._cus
@@ -425,6 +431,9 @@ class KVCache:
         if s.kv_heads != self.heads:
             raise ValueError(f"the plan was made for {s.kv_heads} KV heads")
         q = self._rows(q, s.q_heads, plan.tokens, "queries")
+        scale = self.dim ** -.5 if scale is None else float(scale)
+        if not abs(scale) < 3e38:
+            raise ValueError("scale must be finite, below 3e38")
         if out is None:
             out = torch.empty((plan.tokens, s.q_heads, self.dim), dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
@@ -434,8 +443,7 @@ class KVCache:
         t = plan.tables
         qs, qh, _ = q.stride()
         args = N.KV_ATTEND.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr(), t.table.data_ptr(), t.requests, plan.tokens,
-                                qs, qh, t.max_blocks, _HALVES[q.dtype], self.dim ** -.5 if scale is None else scale, 0,
-                                s.packed)
+                                qs, qh, t.max_blocks, _HALVES[q.dtype], scale, 0, s.packed)
         rc = N.kv_entry("sq_kv_attend")(self._at, args, N.raw_stream())
         if rc:
             N.check(rc, "kv attend")

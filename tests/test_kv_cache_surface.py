@@ -158,3 +158,28 @@ def test_plans_of_more_pages_than_the_cache_has_are_refused():
         cache.attend(k, plan)
     cache, plan = _host_objects(cache_pages=7)
     cache._check_plan(plan)
+
+
+def _host_tables():
+    from stepquant_amd.kernels.kv_cache import BlockTables
+    tables = BlockTables.__new__(BlockTables)
+    tables.device, tables.page_tokens, tables._cus, tables._layouts = torch.device("cpu"), 64, 256, {}
+    return tables
+
+
+@pytest.mark.parametrize("kw", [
+    dict(window=1 << 31, heads=(8, 2)), dict(window=(0, 1 << 40), heads=(8, 2)), dict(window=-1, heads=(8, 2)),
+    dict(heads=(1 << 33, 1 << 32)), dict(heads=(1 << 30, 1)), dict(tokens=1 << 30), dict(tokens=1 << 70, max_new=1),
+    dict(rows=[1 << 70]), dict(new=[1 << 70]), dict(new=[1 << 40], rows=[0])], ids=str)
+def test_numbers_past_the_kernels_types_are_refused_by_plan(kw):
+    with pytest.raises(ValueError):
+        _host_tables().plan(**{**dict(new=[5]), **kw})
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, float("inf"), float("nan"), 3e38])
+def test_scales_past_32_bits_are_refused(scale):
+    from types import SimpleNamespace
+    cache, plan = _host_objects()
+    plan.schedules = {0: SimpleNamespace(q_heads=2, kv_heads=2, floats=4, packed=b"")}
+    with pytest.raises(ValueError, match="scale"):
+        cache.attend(torch.zeros((3, 2, 128), dtype=torch.bfloat16), plan, scale=scale)
