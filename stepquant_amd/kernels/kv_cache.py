@@ -404,7 +404,7 @@ class KVCache:
         if x.numel() and (x.is_floating_point() or x.is_complex() or x.dtype == torch.bool):
             raise ValueError("pages and token counts must be integers")
         # (numbers that 32 bits do not hold are of no page)
-        return x.clamp(-1, 0x7fffffff).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
+        return x.long().clamp(-1, 0x7fffffff).to(device=self.device, dtype=torch.int32).reshape(-1).contiguous()
 
     def attend(self, q, plan, *, scale=None, window=None, out=None):
         """Attention of the plan's new tokens over all that their requests hold.

@@ -183,3 +183,12 @@ def test_scales_past_32_bits_are_refused(scale):
     plan.schedules = {0: SimpleNamespace(q_heads=2, kv_heads=2, floats=4, packed=b"")}
     with pytest.raises(ValueError, match="scale"):
         cache.attend(torch.zeros((3, 2, 128), dtype=torch.bfloat16), plan, scale=scale)
+
+
+def test_pages_are_integers_of_any_width():
+    cache, _ = _host_objects()
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16):
+        assert cache._numbers(torch.tensor([1, 2, 100], dtype=dtype)).tolist() == [1, 2, 100]
+    assert cache._numbers([3, -7, 1 << 40]).tolist() == [3, -1, 0x7fffffff]
+    with pytest.raises(ValueError):
+        cache._numbers([1 << 70])
