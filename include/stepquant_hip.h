@@ -476,7 +476,8 @@ typedef struct sq_kv_schedule {
  *   pages     [max_tiles] the pages that new tokens fall into, request by
  *             request in block order, 0 past the last; filled [max_tiles] the
  *             tokens that each holds afterwards; tiles [max_tiles, 2] its
- *             first new offset and the packed row that goes there
+ *             first new offset and the packed row that goes there (8-byte
+ *             aligned)
  *   counters  [2] the tables' counters afterwards
  * max_tiles >= min(tokens, tokens / page_tokens + 2 * batch).
  */
@@ -540,7 +541,7 @@ int sq_kv_append(const sq_kv_cache *cache, const sq_kv_append_args *args, void *
 /*
  * Pages as dense keys and values [n, page_tokens, heads, dim] of out_dtype,
  * zero past the first filled[i] tokens (filled NULL: all are taken) and for
- * pages that the cache does not have.
+ * pages that the cache does not have.  k and v are 16-byte aligned.
  */
 int sq_kv_decode(const sq_kv_cache *cache, const int32_t *pages, const int32_t *filled, int64_t n, void *k, void *v,
                  int32_t out_dtype, void *stream);
@@ -551,7 +552,7 @@ int sq_kv_decode(const sq_kv_cache *cache, const int32_t *pages, const int32_t *
  * and requests that were not granted among them).
  *   q    [tokens, q_heads, dim], dtype SQ_BF16 or SQ_F16, strides multiples
  *        of 8, 16-byte aligned; out contiguous, same dtype
- *   workspace  max_partials * kv_heads * rows * (dim + 2) floats
+ *   workspace  max_partials * kv_heads * rows * (dim + 2) floats, 16-byte aligned
  */
 typedef struct sq_kv_attend_args {
     const void *q;

@@ -1746,6 +1746,7 @@ int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
   if (!p || !p->rows || !p->counts || !p->cu || !p->slots || !p->positions || !p->lens || !p->granted || !p->pages ||
       !p->filled || !p->tiles || !p->counters)
     return fail(SQ_EINVAL, "kv plan: null pointer");
+  if ((uintptr_t)p->tiles & 7) return fail(SQ_EINVAL, "kv plan: tiles must be 8-byte aligned");
   if (!index_type(p->rows_dtype) || !index_type(p->counts_dtype))
     return fail(SQ_EINVAL, "kv plan: rows and counts are int32 or int64");
   if (p->batch <= 0 || p->batch > SQ_KV_MAX_REQUESTS) return fail(SQ_EINVAL, "kv plan: batch must be in [1, 4096]");
@@ -1885,6 +1886,7 @@ int sq_kv_decode(const sq_kv_cache *c, const int32_t *pages, const int32_t *fill
   if (!pages || !k || !v || n < 0 || n >= 1 << 24) return fail(SQ_EINVAL, "kv decode: null pointer or page count");
   if (out_dtype != SQ_F32 && out_dtype != SQ_BF16 && out_dtype != SQ_F16)
     return fail(SQ_EINVAL, "kv decode: output dtype");
+  if (((uintptr_t)k | (uintptr_t)v) & 15) return fail(SQ_EINVAL, "kv decode: outputs must be 16-byte aligned");
   const dim3 grid((unsigned)n, (unsigned)c->heads, 2);
   if (c->storage == SQ_KV_FP8)
     hipLaunchKernelGGL(kv_decode_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, *c, pages, filled, k, v, out_dtype,
@@ -1911,7 +1913,8 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   if (rc) return rc;
   if (a->schedule.kv_heads != c->heads)
     return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads");
-  if (!a->workspace) return fail(SQ_EINVAL, "kv attend: null workspace");
+  if (!a->workspace || ((uintptr_t)a->workspace & 15))
+    return fail(SQ_EINVAL, "kv attend: null or misaligned workspace");
   const sq_kv_schedule &s = a->schedule;
   const AttendDev d = {*c, (const uint16_t *)a->q, (uint16_t *)a->out, a->workspace, a->table, s.units, s.merges, s.starts,
                        a->requests, a->tokens, a->q_stride, a->q_head_stride, a->width, a->dtype, s.q_heads, s.kv_heads,

@@ -64,7 +64,7 @@ class KVPlan:
         if views is None:
             counters, slots = self._longs.split((2, self.tokens))
             views = self._ints.split_with_sizes(self._sizes)
-            self._views = views = (views[0], slots, *views[1:3], views[3].view(torch.bool)[:self.batch], *views[4:6],
+            self._views = views = (views[1], slots, *views[2:4], views[4].view(torch.bool)[:self.batch], *views[5:7],
                                    counters)
         return views[i]
 
@@ -190,7 +190,7 @@ class BlockTables:
         p._ints = ints = torch.empty(total, dtype=torch.int32, device=self.device)
         p._longs = longs = torch.empty(2 + tokens, dtype=torch.int64, device=self.device)
         base, counters = ints.data_ptr(), longs.data_ptr()
-        cu, positions, lens, granted, pages, filled, tiles = (base + x for x in offsets)
+        tiles, cu, positions, lens, granted, pages, filled = (base + x for x in offsets)
         p.schedules, packed = {}, b""
         for w, q_heads, kv_heads, floats, units, merges, starts, numbers in schedules:
             s = _Schedule()
@@ -240,7 +240,8 @@ class BlockTables:
         words, byte offsets of the first seven, page entries, per window what
         ``sq_kv_schedule`` holds)."""
         most = min(tokens, tokens // self.page_tokens + 2 * batch)
-        sizes = [batch + 1, tokens, batch, -(-batch // 4), most, most, 2 * most]
+        # (page entries' pairs of words first, on a boundary of theirs)
+        sizes = [2 * most, batch + 1, tokens, batch, -(-batch // 4), most, most]
         schedules = []
         if heads is not None:
             q_heads, kv_heads = (int(x) for x in heads)
@@ -257,7 +258,7 @@ class BlockTables:
             few = rows == 256 and tokens * q_heads <= self.few_rows
             sets, cuts = -(-tokens * group // (32 if few else rows)) + batch + 1, max(1, slots // kv_heads)
             workers, joins = max(sets, cuts), min(sets, cuts)
-            sizes[6] += -sum(sizes) % 8  # units and merges start on a boundary of their 32 bytes
+            sizes.append(-sum(sizes) % 8)  # units and merges start on a boundary of their 32 bytes
             for w in windows if tokens else ():
                 units = 4 * sum(sizes)
                 merges = units + 32 * (sets + cuts)

@@ -192,3 +192,37 @@ def test_pages_are_integers_of_any_width():
     assert cache._numbers([3, -7, 1 << 40]).tolist() == [3, -1, 0x7fffffff]
     with pytest.raises(ValueError):
         cache._numbers([1 << 70])
+
+
+@pytest.mark.parametrize("new,tokens,heads", [([1], 1, (8, 2)), ([2], 2, None), ([5, 0, 0], 5, (4, 4)), ([90] * 3, 300, (8, 1)),
+                                              ([1] * 256, 256, (32, 8))])
+def test_parts_of_a_plan_start_on_their_boundaries(new, tokens, heads, monkeypatch):
+    calls, tables = [], _host_tables()
+    tables._at = 0
+    monkeypatch.setattr(N, "kv_entry", lambda name: lambda at, args, stream: calls.append(args) or 0)
+    monkeypatch.setattr(N, "raw_stream", lambda: 0)
+    plan = tables.plan(new, tokens=tokens, heads=heads, window=(0, 64))
+    a = N.KVPlan.from_buffer_copy(calls[0])
+    assert a.tiles % 8 == 0 and a.slots % 8 == 0 and a.counters % 8 == 0
+    spans = [(a.cu, len(new) + 1), (a.positions, tokens), (a.lens, len(new)), (a.granted, -(-len(new) // 4)),
+             (a.pages, a.max_tiles), (a.filled, a.max_tiles), (a.tiles, 2 * a.max_tiles)]
+    for s in a.schedules[:a.n_schedules]:
+        assert s.units % 32 == 0 and s.merges % 32 == 0
+        spans += [(s.units, 8 * s.max_units), (s.merges, 8 * s.max_merges), (s.starts, s.max_workers + 2)]
+    # each within the plan's memory, none over another one
+    spans = sorted((start, start + 4 * n) for start, n in spans)
+    assert all(x[1] <= y[0] for x, y in zip(spans, spans[1:]))
+    base = plan._ints.data_ptr()
+    assert spans[0][0] >= base and spans[-1][1] <= base + 4 * plan._ints.numel()
+    for name, at in (("cu", a.cu), ("positions", a.positions), ("lens", a.lens), ("granted", a.granted), ("pages", a.pages),
+                     ("filled", a.filled), ("slots", a.slots), ("counters", a.counters)):
+        assert getattr(plan, name).data_ptr() == at, name
+    assert plan.granted.numel() == len(new) and plan.pages.numel() == plan.filled.numel() == a.max_tiles
+
+
+def test_misaligned_outputs_are_refused():
+    L = N.lib()
+    assert L.sq_kv_plan(_tables(), _plan(tiles=20), None) == -22
+    assert L.sq_kv_decode(_cache(), 16, None, 1, 16, 24, N.F32, None) == -22
+    assert L.sq_kv_decode(_cache(), 16, None, 1, 20, 16, N.BF16, None) == -22
+    assert L.sq_kv_attend(_cache(), _attend(workspace=24), None) == -22
