@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from stepquant_amd import _native as N
 from stepquant_amd.kernels.kv_cache import BlockTables
 from tests.helpers import dev
 from tests.test_gpu_kv_cache import TOP, check_append, filled, make, page_parts, rng
@@ -163,6 +164,45 @@ def test_scores_past_2_30_in_sets_of_256(D, sets_of_256):
 @pytest.mark.parametrize("depth,first", [(18, 128.), (18, 8.), (23, 0.), (26, 0.)])
 def test_many_small_weights_in_sets_of_256(D, depth, first, sets_of_256):
     test_many_small_weights_beside_a_large_one(D, 90, depth, first)
+
+
+def unit_rows(plan, window=0):
+    """Rows of a unit as the plan kernel stored them."""
+    fields = N.KV_SCHEDULE.unpack(plan.schedules[window].packed)
+    return int(plan._ints[(fields[2] - plan._ints.data_ptr()) // 4 + fields[5] + 1])
+
+
+def test_the_plan_decides_by_its_lengths():
+    """One captured plan takes sets of 32 rows while a request is short, of 256 when it has grown."""
+    n, Hq, H = 40, 16, 2
+    tables = BlockTables(1, 20, 18)
+    tables.few_work = n * Hq * 6  # (five tiles up to the chunk's middle, and one)
+    new, rows = torch.tensor([n], dtype=torch.int32, device=dev()), torch.zeros(1, dtype=torch.int32, device=dev())
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        plan = tables.plan(new, rows, tokens=n, max_new=n, heads=(Hq, H))
+        tables.commit(plan)
+    seen = []
+    for i in range(18):
+        graph.replay()
+        torch.cuda.synchronize()
+        seen.append(unit_rows(plan))
+    assert seen == [32 if (n * i + n // 2) // 64 + 1 <= 6 else 256 for i in range(18)] and len(set(seen)) == 2
+
+
+def test_sets_of_256_are_those(sets_of_256):
+    """What the tests in sets of 256 rows run, whether asked for or decided."""
+    for Hq, D, new in ((8, 128, 90), (4, 256, 90), (4, 64, 90)):
+        assert unit_rows(filled([200], [new], Hq=Hq, H=1, D=D)[2]) == 256
+    assert unit_rows(filled([200], [new], Hq=4, H=1, D=64, window=50)[2], 50) == 256
+
+
+def test_row_counts_by_the_longest_request():
+    for Hq, H, new, rows in ((4, 4, [16, 1], 16), (8, 1, [2, 1], 16), (8, 1, [3], 32), (8, 1, [8, 2], 32), (8, 1, [9], 32),
+                             (8, 1, [2100], 256)):
+        print(f"case {Hq} over {H}, {new}", flush=True)
+        assert unit_rows(filled([0] * len(new), new, Hq=Hq, H=H)[2]) == rows
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
