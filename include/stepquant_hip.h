@@ -387,6 +387,9 @@ int sq_format_step(const sq_format_pool *pool, const sq_step_args *args, void *s
  * page_bytes is a multiple of 16 and data 16-byte aligned; page 0 is the
  * padding page, which no request holds.  dim is 64, 128 or 256; page_tokens
  * a multiple of 64 with page_tokens * dim <= 32768.
+ * Attention reads a block's tokens past those that a request holds, with a
+ * weight of 0: pages start with codes that stand for finite numbers (zeroed
+ * memory; no e4m3 NaN), which is all that appends write.
  */
 enum {
     SQ_KV_INT8 = 0,
@@ -506,9 +509,11 @@ typedef struct sq_kv_plan_args {
 /*
  * Fills a plan from the tables and writes the new blocks' pages into the
  * table; lens and counters stay (a plan that is not committed can be made
- * again).  sq_kv_commit takes the plan's lengths and pages into the tables.
+ * again).  sq_kv_commit takes the plan's lengths and pages into the tables,
+ * for the rows that `rows` holds then; plans made before it are void.
  * sq_kv_release gives the pages of n rows back to the ring and empties them;
- * entries that name a row a second time, or none, are passed over.
+ * entries that name a row a second time, or none, are passed over.  Plans made
+ * before it that name such a row are void.
  */
 int sq_kv_plan(const sq_kv_tables *tables, const sq_kv_plan_args *plan, void *stream);
 int sq_kv_commit(const sq_kv_tables *tables, const sq_kv_plan_args *plan, void *stream);

@@ -646,7 +646,9 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(sq_kv_cache c, const int
 // Codes of at most 8 bits are exact as halves, and so are queries: a row is
 // brought near 2^14 by a power of two first, where bfloat16's 8 bits fit.  So
 // scores are sums in 32 bits of exact products, times a block's peak; what is
-// rounded are the probabilities, to 11 bits, and the outputs.
+// rounded are the probabilities, to 11 bits, and the outputs.  (bfloat16 would
+// round them to 8.)  A half's exponents reach from 2^-24 to 2^15: the largest of a
+// row stand near the upper end, so that small ones keep their bits.
 
 struct AttendDev {
   sq_kv_cache c;
@@ -804,12 +806,12 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // the four SIMDs, which is all that LDS gives; 64 rows a wave would halve that,
 // and need twice the registers), and the vector instructions of the other half
 // fill what is left.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims (550
-// GFLOP): 556 us, 990 TFLOP/s of the 1160 that a large library product reaches;
-// the products alone, without softmax and conversion, take 400 us.  256 dims 890
-// TFLOP/s, as tiles are converted for 128 rows, not 256; 64 dims 630, as scores
-// cost the same there and products half.  The halves half a tile apart took it
-// from 827 to 670 us, peaks by way of LDS and masks without conditions (no
-// scalar register spilled) to 579.  The order of products and LDS reads that the
+// GFLOP): 566 to 581 us, 950 to 970 TFLOP/s of the 1130 that a large library product
+// reaches there; the products alone, without softmax and conversion, take 400 us.
+// 256 dims 860 TFLOP/s, as tiles are converted for 128 rows, not 256; 64 dims 635
+// (int8) and 665 (e4m3), as scores cost the same there and products half.  The
+// halves half a tile apart took 128 dims from 827 to 670 us, peaks by way of LDS and
+// masks without conditions (no scalar register spilled) to 579.  The order of products and LDS reads that the
 // groups below ask for takes 3% off; wave priorities change nothing, nor do 8
 // operands ahead in place of 4.
 //
@@ -1279,7 +1281,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_rows_kernel(AttendDev a) {
 // HBM bounds it where there is enough to read: 256 requests of 4096 tokens (8
 // heads of 128 dims, 2.16 GB) 356 us, 6.1 TB/s; 64 of up to 8192 (593 MB) 112
 // us; one of 131,072 (270 MB) 44 us.  A short one (1000 tokens of 2 heads of 256
-// dims) takes 9.8 us: loads of the schedule, the table, the pages and the
+// dims) takes 8.4 to 9.8 us: loads of the schedule, the table, the pages and the
 // partial results one after the other.  Values fetched a tile ahead as well
 // cost 2 to 5% (registers), three workgroups on a CU 10 to 16%.
 //

@@ -1,8 +1,8 @@
 """Attention over keys and values held in 8 bits in pages, on one MI355X GPU.
 
 The softmax-attention layers between the recurrent layers that the state
-pools serve (no reference counterpart: the reference leaves them to its host
-engine).  Three pieces, used in turn by one model step:
+pools serve, where keys and values have one head size of 64, 128 or 256 (no
+reference counterpart: the reference leaves them to its host engine).  Three pieces, used in turn by one model step:
 
 * ``BlockTables`` gives requests their pages.  ``plan`` turns the number of
   new tokens of each request into block tables, slot maps and the attention
@@ -231,8 +231,12 @@ class BlockTables:
     # in sets of 256, 21 so; 64 of 256 dims over 1000: 94 and 28; but 64 over 8000 of
     # 128 dims 34 and 45).  So for up to `few_rows` query rows of all heads the plan
     # kernel, which knows the lengths, decides: sets of 32 where rows times the tiles
-    # that they see are at most `few_work` (the two meet near 2^17 for 128 dims, 2^18
-    # for 64 and 2^18.5 for 256).
+    # that they see are at most `few_work`.  It is one number for every head size,
+    # which a plan is not told, and for sets of 256 cut or not, so near it the other
+    # side can be ahead.  At 2^17.3, sets of 32 and of 256: 32 heads of 64 dims, 64
+    # tokens 23.5 and 19.9 us, 256 tokens 20.4 and 40.8; of 128 dims 33.5 and 25.9,
+    # 29.3 and 47.6; 16 heads of 256 dims 52 and 74, 56 and 76.  At 2^18: 28 and 24, 27
+    # and 31; 41 and 33, 39 and 37; 67 and 65, 71 and 81.
     few_rows, few_work = 1 << 14, 3 << 16
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows):
@@ -272,7 +276,11 @@ class BlockTables:
         return sizes, sum(sizes), offsets, most, schedules
 
     def commit(self, plan):
-        """Takes a plan's lengths and pages over; plans made before it are void."""
+        """Takes a plan's lengths and pages over; plans made before it are void.
+
+        The plan's ``rows`` are read again: a tensor of the caller's stays as it
+        was for ``plan`` until then.
+        """
         if plan.tables is not self:
             raise ValueError("the plan is of other block tables")
         rc = N.kv_entry("sq_kv_commit")(self._at, plan._args, N.raw_stream())
@@ -280,7 +288,8 @@ class BlockTables:
             N.check(rc, "kv commit")
 
     def release(self, rows):
-        """Gives the pages of the requests in ``rows`` back; their rows are empty afterwards."""
+        """Gives the pages of the requests in ``rows`` back; their rows are empty
+        afterwards, and plans made before that name them are void."""
         rows = self._index(rows, "rows")
         if rows.numel() > N.KV_MAX_REQUESTS:
             raise ValueError(f"at most {N.KV_MAX_REQUESTS} rows at once")
