@@ -811,9 +811,9 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // 256 dims 860 TFLOP/s, as tiles are converted for 128 rows, not 256; 64 dims 635
 // (int8) and 665 (e4m3), as scores cost the same there and products half.  The
 // halves half a tile apart took 128 dims from 827 to 670 us, peaks by way of LDS and
-// masks without conditions (no scalar register spilled) to 579.  The order of products and LDS reads that the
-// groups below ask for takes 3% off; wave priorities change nothing, nor do 8
-// operands ahead in place of 4.
+// masks without conditions (no scalar register spilled) to 579.  The order of
+// products and LDS reads that the groups below ask for takes 3% off; wave priorities
+// change nothing, nor do 8 operands ahead in place of 4.
 //
 // A row's sum is kept in units of 2^m, m kBias below its largest score, and its
 // outputs in units of 2^(m + gap), such that the largest score and log2 of the
@@ -823,10 +823,11 @@ typedef float f32x16_v __attribute__((ext_vector_type(16)));
 // Both are raised only when a half or a weight would pass 2^kTop; so halves hold all
 // bits of a product down to 2^-24 of the row's largest and some down to 2^-34.
 // Where a block's values are smaller than others by more than 2^kSmall, the sum
-// takes its weights before they are halves: it has all bits of those down to 2^-20
-// of the largest.  (A prompt of 8192 tokens: 611 us with units raised at 2^8 above
-// the largest half, which leaves 3 bits less, 615 so, 622 with 11 for kBias.)  m
-// starts at a number below every score, so that no difference of it needs care.
+// takes its weights before they are halves; from the others it has all bits of
+// weights down to 2^-20 of the largest.  (A prompt of 8192 tokens: 611 us with the
+// largest half at 2^0 to 2^8, 615 so, 622 with 2^11 to 2^15: the narrower, the more
+// tiles raise the units.)  m starts at a number below every score, so that no
+// difference of it needs care.
 constexpr float kBias = 10.f, kTop = 15.f, kSmall = 4.f;
 
 template <int D, bool FP8>
