@@ -374,6 +374,45 @@ int sq_format_decode(const sq_format_pool *pool, const void *slots, int32_t slot
 int sq_format_step(const sq_format_pool *pool, const sq_step_args *args, void *stream);
 
 /*
+ * Rotary positions.  Pair i of a head's first `dim` dims, (i, i + dim / 2) or,
+ * interleaved, (2 i, 2 i + 1), turns by an angle of position * f_i:
+ *   a' = magnitude * (a cos - b sin),  b' = magnitude * (a sin + b cos)
+ *   turns   [dim / 2] f_i / (2 pi), turns a position, times 2^64 (modulo 2^64)
+ *   dim     a multiple of 16, at most 1024
+ */
+typedef struct sq_rotary {
+    const uint64_t *turns;
+    int32_t dim;
+    int32_t interleaved;
+    float magnitude;
+    int32_t reserved;
+} sq_rotary;
+
+/*
+ * Rows to turn: x and out [tokens, heads, head_dim] (SQ_F32, SQ_BF16 or SQ_F16,
+ * one type) with element strides per token and head of whole 16 bytes, 16-byte
+ * aligned; dims past the rotated ones are copied.  out may be x (with its
+ * strides), and does not overlap it otherwise.  positions [tokens] (SQ_I32 or
+ * SQ_I64): rows at negative ones are copied as they are.
+ */
+typedef struct sq_rotary_rows {
+    const void *x;
+    void *out;
+    const void *positions;
+    int64_t tokens;
+    int64_t x_stride;
+    int64_t x_head_stride;
+    int64_t out_stride;
+    int64_t out_head_stride;
+    int32_t heads;
+    int32_t head_dim;
+    int32_t dtype;
+    int32_t positions_dtype;
+} sq_rotary_rows;
+
+int sq_rotary_apply(const sq_rotary *rotary, const sq_rotary_rows *rows, void *stream);
+
+/*
  * Keys and values of softmax-attention layers, held in 8 bits in pages.
  *
  * A page holds page_tokens tokens of every KV head: per head the keys
@@ -542,6 +581,14 @@ typedef struct sq_kv_append_args {
 } sq_kv_append_args;
 
 int sq_kv_append(const sq_kv_cache *cache, const sq_kv_append_args *args, void *stream);
+
+/*
+ * The same with the keys turned on the way, before their peaks are taken:
+ * positions [tokens] are the plan's.  `rows` (NULL: none) are turned in the same
+ * launch, the tokens' queries as a rule.
+ */
+int sq_kv_append_rotary(const sq_kv_cache *cache, const sq_kv_append_args *args, const int32_t *positions,
+                        const sq_rotary *rotary, const sq_rotary_rows *rows, void *stream);
 
 /*
  * Pages as dense keys and values [n, page_tokens, heads, dim] of out_dtype,

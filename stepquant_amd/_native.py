@@ -117,6 +117,18 @@ class KVAttend(ctypes.Structure):
                 ("reserved", ctypes.c_int32), ("schedule", KVSchedule)]
 
 
+class Rotary(ctypes.Structure):
+    _fields_ = [("turns", _P), ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("magnitude", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
+class RotaryRows(ctypes.Structure):
+    _fields_ = [("x", _P), ("out", _P), ("positions", _P), ("tokens", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+                ("x_head_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("positions_dtype", ctypes.c_int32)]
+
+
 FMT_FP32, FMT_SYMMETRIC, FMT_DSQ = 0, 1, 2
 FMT_ROWS_CONTIGUOUS = 1
 
@@ -127,7 +139,7 @@ EXPORTS = ("sq_abi_version", "sq_last_error", "sq_encode", "sq_decode_dense", "s
            "sq_format_encode", "sq_format_decode", "sq_format_step", "sq_copy_slots_static", "sq_copy_slots_direct",
            "sq_event_create", "sq_event_destroy", "sq_event_record", "sq_event_wait", "sq_event_query",
            "sq_event_synchronize", "sq_kv_plan", "sq_kv_commit", "sq_kv_release", "sq_kv_append", "sq_kv_decode",
-           "sq_kv_attend")
+           "sq_kv_attend", "sq_rotary_apply", "sq_kv_append_rotary")
 COPY_STATIC_BYTES = 16 << 20
 COPY_DIRECT_PAGES = 256
 
@@ -182,6 +194,8 @@ def lib():
     L.sq_kv_append.argtypes = [PP(KVCache), PP(KVAppend), _P]
     L.sq_kv_decode.argtypes = [PP(KVCache), _P, _P, ctypes.c_int64, _P, _P, ctypes.c_int32, _P]
     L.sq_kv_attend.argtypes = [PP(KVCache), PP(KVAttend), _P]
+    L.sq_rotary_apply.argtypes = [PP(Rotary), PP(RotaryRows), _P]
+    L.sq_kv_append_rotary.argtypes = [PP(KVCache), PP(KVAppend), _P, PP(Rotary), PP(RotaryRows), _P]
     for name in EXPORTS:
         if name not in ("sq_last_error",):
             getattr(L, name).restype = ctypes.c_int
@@ -238,15 +252,18 @@ KV_SCHEDULE = struct.Struct("=3Q16i")
 KV_PLAN = struct.Struct(f"=11Qq6i{KV_MAX_SCHEDULES * KV_SCHEDULE.size}s")
 KV_APPEND = struct.Struct("=5Q5q2i")
 KV_ATTEND = struct.Struct(f"=4Q4q2ifi{KV_SCHEDULE.size}s")
+ROTARY_ROWS = struct.Struct("=3Q5q4i")
 _I32, _I64 = ctypes.c_int32, ctypes.c_int64
 _KV_ENTRIES = {"sq_kv_plan": [_P, ctypes.c_char_p, _P], "sq_kv_commit": [_P, ctypes.c_char_p, _P],
                "sq_kv_append": [_P, ctypes.c_char_p, _P], "sq_kv_attend": [_P, ctypes.c_char_p, _P],
+               "sq_rotary_apply": [_P, ctypes.c_char_p, _P],
+               "sq_kv_append_rotary": [_P, ctypes.c_char_p, _P, _P, ctypes.c_char_p, _P],
                "sq_kv_decode": [_P, _P, _P, _I64, _P, _P, _I32, _P]}
 
 
 def kv_entry(name: str):
-    """A KV entry point taking the address of its tables or cache and a packed
-    argument block (``sq_kv_decode``: plain arguments)."""
+    """A KV or rotary entry point taking the address of its tables, cache or
+    frequencies and a packed argument block (``sq_kv_decode``: plain arguments)."""
     fn = _step_entries.get(name)
     if fn is None:
         fn = lib()[name]

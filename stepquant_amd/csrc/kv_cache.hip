@@ -9,6 +9,7 @@
 #include <utility>
 
 #include "internal.h"
+#include "rotary.h"
 #include "stepquant_hip.h"
 
 // every fused multiply-add is written out, so that codes round as defined
@@ -520,6 +521,27 @@ __device__ __forceinline__ void decode4(uint32_t w, float x[4]) {
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
+// A block's older codes, in the first `groups` groups of 8, brought from one peak
+// to another.
+template <bool FP8>
+__device__ __forceinline__ void bring_codes(uint8_t *base, int groups, float before, float peak) {
+  const uint32_t zero = FP8 ? 0u : 0x80808080u;
+  const bool good = finite(peak);
+  // both peaks 2^-32 of their size where a code times one would pass 32 bits
+  const float down = peak > 0x1p100f ? 0x1p-32f : 1.f, was = before * down, now = peak * down, inv_now = 1.f / now;
+  for (int g = threadIdx.x; g < groups; g += 256) {
+    uint2 w = *(const uint2 *)(base + 8 * (int64_t)g);
+    float y[8];
+    decode4<FP8>(w.x, y);
+    decode4<FP8>(w.y, y + 4);
+#pragma unroll
+    for (int k = 0; k < 8; k++) y[k] = quotient(y[k] * was, now, inv_now);
+    w.x = good ? code4<FP8>(y) : zero;
+    w.y = good ? code4<FP8>(y + 4) : zero;
+    *(uint2 *)(base + 8 * (int64_t)g) = w;
+  }
+}
+
 // One workgroup per (page entry, head, keys or values): it finds the peak of
 // its new values, brings the block's older codes to it where it grew, and
 // writes the new codes.  A thread holds N groups of 8 adjacent dims between
@@ -568,21 +590,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
   const bool good = finite(peak);
   if (tid == 0) *peak_at = peak;
   const uint32_t zero = FP8 ? 0u : 0x80808080u;
-  if (peak != before) {
-    // both peaks 2^-32 of their size where a code times one would pass 32 bits
-    const float down = peak > 0x1p100f ? 0x1p-32f : 1.f, was = before * down, now = peak * down, inv_now = 1.f / now;
-    for (int g = tid; g < from; g += 256) {
-      uint2 w = *(const uint2 *)(base + 8 * (int64_t)g);
-      float y[8];
-      decode4<FP8>(w.x, y);
-      decode4<FP8>(w.y, y + 4);
-#pragma unroll
-      for (int k = 0; k < 8; k++) y[k] = quotient(y[k] * was, now, inv_now);
-      w.x = good ? code4<FP8>(y) : zero;
-      w.y = good ? code4<FP8>(y + 4) : zero;
-      *(uint2 *)(base + 8 * (int64_t)g) = w;
-    }
-  }
+  if (peak != before) bring_codes<FP8>(base, from, before, peak);
 #pragma unroll
   for (int i = 0; i < N; i++) {
     const int g = from + i * 256 + tid;
@@ -592,6 +600,92 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
 #pragma unroll
       for (int k = 0; k < 8; k++) y[k] = quotient(y[k], peak, inv) * top;
       *(uint2 *)(base + 8 * (int64_t)g) = make_uint2(good ? code4<FP8>(y) : zero, good ? code4<FP8>(y + 4) : zero);
+    }
+  }
+}
+
+// The same with the keys turned on the way, in 32 bits: they are rounded once, to
+// their codes (rounded to bfloat16 first, 3% of int8 codes would be others).  A
+// thread holds N pairs of groups of 8 dims, which are turned together.  The
+// workgroups from z = 2 on turn the queries of the same tokens.
+template <bool FP8, int N>
+__global__ __launch_bounds__(256) void kv_append_rotary_kernel(sq_kv_cache c, sq_kv_append_args a, int log_dim,
+                                                               const int32_t *positions, sq_rotary r, sq_rotary_rows q,
+                                                               int q_lanes) {
+  __shared__ uint32_t peaks[4];
+  const int tid = threadIdx.x, tile = blockIdx.x, h = blockIdx.y, part = blockIdx.z;
+  if (part >= 2) {
+    const uint32_t block = ((part - 2) * gridDim.y + h) * gridDim.x + tile;
+    rotary::rotate_rows<1>(r, q, q_lanes, block * 256 + tid);
+    return;
+  }
+  const int64_t page = a.pages[tile];
+  const int start = a.tiles[2 * (int64_t)tile], token = a.tiles[2 * (int64_t)tile + 1], filled = a.filled[tile];
+  if (page <= 0 || page >= c.num_pages) return;
+  if (start < 0 || start >= filled || filled > c.page_tokens || token < 0 || token + (int64_t)filled - start > a.tokens)
+    return;
+  const float top = FP8 ? 448.f : 127.f;
+  const uint16_t *src = (const uint16_t *)(part ? a.v : a.k) + h * (part ? a.v_head_stride : a.k_head_stride);
+  const int64_t stride = part ? a.v_stride : a.k_stride;
+  uint8_t *base = c.data + page * c.page_bytes + ((int64_t)(2 * h + part) * c.page_tokens << log_dim);
+  const int64_t peaks_at = 2 * (int64_t)c.heads * c.page_tokens << log_dim;
+  float *peak_at = (float *)(c.data + page * c.page_bytes + peaks_at) + 2 * h + part;
+  const int from = start << (log_dim - 4), upto = filled << (log_dim - 4);
+  const int item = tid & ((1 << (log_dim - 4)) - 1);  // the same in every step: 256 is a multiple of a token's items
+  const bool turned = !part && item < r.dim / 16;
+  int ga, gb;
+  rotary::groups(r, item, ga, gb);
+  u32x4_v x[N][2];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int g = from + i * 256 + tid;
+    if (g < upto) {
+      const uint16_t *at = src + (int64_t)(token + (g >> (log_dim - 4)) - start) * stride;
+      x[i][0] = *(const u32x4_v *)(at + 8 * ga);
+      x[i][1] = *(const u32x4_v *)(at + 8 * gb);
+    }
+  }
+  const int first = positions[token] - start;  // the position of the page's first token
+  float y[N][16];
+  uint32_t most = 0;  // magnitudes as bits: their order, and NaN above all
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int g = from + i * 256 + tid;
+    if (g < upto) {
+      widen8(x[i][0], a.dtype, y[i]);
+      widen8(x[i][1], a.dtype, y[i] + 8);
+      if (turned) {
+        rotary::Angles t;
+        t.at(r, item, (uint64_t)(first + (g >> (log_dim - 4))));
+        rotary::rotate(r.interleaved, t, y[i]);
+      }
+#pragma unroll
+      for (int k = 0; k < 16; k++) most = max(most, __float_as_uint(y[i][k]) & 0x7fffffffu);
+    }
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, k, 64));
+  if ((tid & 63) == 0) peaks[tid >> 6] = most;
+  const float before = start ? *peak_at : kFloor;
+  __syncthreads();
+  most = max(max(peaks[0], peaks[1]), max(peaks[2], peaks[3]));
+  const float peak = __uint_as_float(max(max(most, __float_as_uint(before) & 0x7fffffffu), __float_as_uint(kFloor)));
+  const float inv = 1.f / peak;
+  const bool good = finite(peak);
+  if (tid == 0) *peak_at = peak;
+  const uint32_t zero = FP8 ? 0u : 0x80808080u;
+  if (peak != before) bring_codes<FP8>(base, 2 * from, before, peak);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int g = from + i * 256 + tid;
+    if (g < upto) {
+#pragma unroll
+      for (int k = 0; k < 16; k++) y[i][k] = quotient(y[i][k], peak, inv) * top;
+      uint8_t *at = base + ((int64_t)(g >> (log_dim - 4)) << log_dim);
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        *(uint2 *)(at + 8 * (k ? gb : ga)) =
+            make_uint2(good ? code4<FP8>(y[i] + 8 * k) : zero, good ? code4<FP8>(y[i] + 8 * k + 4) : zero);
     }
   }
 }
@@ -1770,6 +1864,21 @@ int check_plan(const sq_kv_tables *t, const sq_kv_plan_args *p) {
   return 0;
 }
 
+int check_append(const sq_kv_cache *c, const sq_kv_append_args *a) {
+  const int rc = check_cache(c);
+  if (rc) return rc;
+  if (!a) return fail(SQ_EINVAL, "kv append: null arguments");
+  if (a->max_tiles == 0) return 0;
+  if (!a->k || !a->v || !a->pages || !a->filled || !a->tiles || a->max_tiles < 0)
+    return fail(SQ_EINVAL, "kv append: null pointer");
+  if (a->dtype != SQ_BF16 && a->dtype != SQ_F16) return fail(SQ_EINVAL, "kv append: keys and values are bf16 or fp16");
+  if ((a->k_stride | a->k_head_stride | a->v_stride | a->v_head_stride) & 7 || (((uintptr_t)a->k | (uintptr_t)a->v) & 15))
+    return fail(SQ_EINVAL, "kv append: strides must be multiples of 8 and starts 16-byte aligned");
+  if (a->k_stride < 0 || a->k_head_stride < 0 || a->v_stride < 0 || a->v_head_stride < 0)
+    return fail(SQ_EINVAL, "kv append: negative stride");
+  return 0;
+}
+
 // Raises a kernel's limit of dynamic LDS to the most that it takes, once per
 // kernel (each with an id of its own) and device.
 std::atomic<uint64_t> g_raised[16];
@@ -1857,17 +1966,8 @@ int sq_kv_release(const sq_kv_tables *t, const void *rows, int32_t rows_dtype, i
 }
 
 int sq_kv_append(const sq_kv_cache *c, const sq_kv_append_args *a, void *stream) {
-  const int rc = check_cache(c);
-  if (rc) return rc;
-  if (!a) return fail(SQ_EINVAL, "kv append: null arguments");
-  if (a->max_tiles == 0) return 0;
-  if (!a->k || !a->v || !a->pages || !a->filled || !a->tiles || a->max_tiles < 0)
-    return fail(SQ_EINVAL, "kv append: null pointer");
-  if (a->dtype != SQ_BF16 && a->dtype != SQ_F16) return fail(SQ_EINVAL, "kv append: keys and values are bf16 or fp16");
-  if ((a->k_stride | a->k_head_stride | a->v_stride | a->v_head_stride) & 7 || (((uintptr_t)a->k | (uintptr_t)a->v) & 15))
-    return fail(SQ_EINVAL, "kv append: strides must be multiples of 8 and starts 16-byte aligned");
-  if (a->k_stride < 0 || a->k_head_stride < 0 || a->v_stride < 0 || a->v_head_stride < 0)
-    return fail(SQ_EINVAL, "kv append: negative stride");
+  const int rc = check_append(c, a);
+  if (rc || a->max_tiles == 0) return rc;
   const int n = c->page_tokens * c->dim / 2048;
   const dim3 grid((unsigned)a->max_tiles, (unsigned)c->heads, 2);
   auto go = [&](auto kernel) {
@@ -1879,6 +1979,40 @@ int sq_kv_append(const sq_kv_cache *c, const sq_kv_append_args *a, void *stream)
            : n <= 8 ? go(kv_append_kernel<true, 8>) : go(kv_append_kernel<true, 16>);
   return n <= 2 ? go(kv_append_kernel<false, 2>) : n <= 4 ? go(kv_append_kernel<false, 4>)
          : n <= 8 ? go(kv_append_kernel<false, 8>) : go(kv_append_kernel<false, 16>);
+}
+
+int sq_kv_append_rotary(const sq_kv_cache *c, const sq_kv_append_args *a, const int32_t *positions, const sq_rotary *r,
+                        const sq_rotary_rows *rows, void *stream) {
+  int rc = check_append(c, a);
+  if (rc || a->max_tiles == 0) return rc;
+  rc = rotary::check(r);
+  if (rc) return rc;
+  if (!positions) return fail(SQ_EINVAL, "kv append: null positions");
+  if (r->dim > c->dim) return fail(SQ_ESHAPE, "kv append: the rotation turns more dims than a head has");
+  sq_rotary_rows q = {};
+  int lanes = 0;
+  int64_t z = 2;
+  if (rows && rows->tokens) {
+    rc = rotary::check_rows(r, rows);
+    if (rc) return rc;
+    q = *rows;
+    lanes = q.heads;
+    const int64_t threads = q.tokens * q.heads * (r->dim / 16), plane = (int64_t)a->max_tiles * c->heads;
+    if (threads >= (int64_t)1 << 31) return fail(SQ_EINVAL, "kv append: too many queries for one call");
+    z += ((threads + 255) / 256 + plane - 1) / plane;
+    if (z > 65535) return fail(SQ_EINVAL, "kv append: too many queries for one call");
+  }
+  const int n = c->page_tokens * c->dim / 4096;
+  const dim3 grid((unsigned)a->max_tiles, (unsigned)c->heads, (unsigned)z);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, *a, log2_of(c->dim), positions, *r, q, lanes);
+    return sq_internal_launched("kv_append_rotary_kernel");
+  };
+  if (c->storage == SQ_KV_FP8)
+    return n <= 1 ? go(kv_append_rotary_kernel<true, 1>) : n <= 2 ? go(kv_append_rotary_kernel<true, 2>)
+           : n <= 4 ? go(kv_append_rotary_kernel<true, 4>) : go(kv_append_rotary_kernel<true, 8>);
+  return n <= 1 ? go(kv_append_rotary_kernel<false, 1>) : n <= 2 ? go(kv_append_rotary_kernel<false, 2>)
+         : n <= 4 ? go(kv_append_rotary_kernel<false, 4>) : go(kv_append_rotary_kernel<false, 8>);
 }
 
 int sq_kv_decode(const sq_kv_cache *c, const int32_t *pages, const int32_t *filled, int64_t n, void *k, void *v,

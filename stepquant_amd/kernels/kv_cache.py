@@ -56,7 +56,7 @@ class KVPlan:
     """
 
     __slots__ = ("tables", "rows", "counts", "tokens", "batch", "max_tiles", "schedules", "_args", "_ints", "_longs",
-                 "_sizes", "_append", "_views")
+                 "_sizes", "_append", "_views", "_positions")
 
     def _view(self, i):
         # views are made when they are asked for: a step's kernels need none
@@ -199,6 +199,7 @@ class BlockTables:
             p.schedules[w] = s
             packed += s.packed
         p._append = (pages, filled, tiles)
+        p._positions = positions
         p._args = args = N.KV_PLAN.pack(
             rows.data_ptr(), counts.data_ptr(), cu, counters + 16, positions, lens, granted, pages, filled, tiles, counters,
             tokens, batch, most, N.INTS[rows.dtype], N.INTS[counts.dtype], len(schedules), max_new,
@@ -363,9 +364,15 @@ class KVCache:
         if tables.pages > self.pages:
             raise ValueError(f"the plan's block tables give out {tables.pages} pages, the cache has {self.pages}")
 
-    def append(self, k, v, plan):
+    def append(self, k, v, plan, *, rotary=None, q=None, out=None):
         """Quantises the plan's new keys and values [tokens, kv_heads, head_dim]
         (or [tokens, kv_heads * head_dim]; bf16 or fp16) into their pages.
+
+        ``rotary`` (a ``Rotary`` of at most ``head_dim`` dims) turns the keys to the
+        plan's positions on the way, in 32 bits; then ``q``, the same tokens'
+        queries [tokens, q_heads, head_dim] (or [tokens, q_heads * head_dim]), are turned in the
+        same launch and returned, in ``out`` where it is given (which may be ``q``).
+        Rows without a slot come back as they are.
 
         Every page belongs to one request, as ``BlockTables`` gives them out: two
         requests that wrote to one page would race for its peaks.
@@ -375,14 +382,32 @@ class KVCache:
         v = self._rows(v, self.heads, plan.tokens, "values")
         if k.dtype != v.dtype:
             raise ValueError("keys and values must have one dtype")
+        if rotary is None:
+            if q is not None or out is not None:
+                raise ValueError("queries are turned by a rotary")
+        elif rotary.device != self.device or rotary.dim > self.dim:
+            raise ValueError("the rotary is on another device, or turns more dims than a head has")
+        rows = None
+        if q is not None:
+            if q.dim() == 2 and q.shape[1] % self.dim == 0:
+                q = q.unflatten(1, (-1, self.dim))
+            if q.dim() != 3 or q.shape[0] != plan.tokens or q.shape[2] != self.dim:
+                raise ValueError(f"queries must be [{plan.tokens}, heads, {self.dim}], the plan's tokens")
+            rows, out = rotary._rows(q, plan._positions, N.I32, out)
+        elif out is not None:
+            raise ValueError("out is where queries go")
         if not plan.tokens:
-            return
+            return out
         (ks, kh, _), (vs, vh, _) = k.stride(), v.stride()
         args = N.KV_APPEND.pack(k.data_ptr(), v.data_ptr(), *plan._append, plan.tokens, ks, kh, vs, vh, plan.max_tiles,
                                 _HALVES[k.dtype])
-        rc = N.kv_entry("sq_kv_append")(self._at, args, N.raw_stream())
+        if rotary is None:
+            rc = N.kv_entry("sq_kv_append")(self._at, args, N.raw_stream())
+        else:
+            rc = N.kv_entry("sq_kv_append_rotary")(self._at, args, plan._positions, rotary._at, rows, N.raw_stream())
         if rc:
             N.check(rc, "kv append")
+        return out
 
     def decode(self, pages, filled=None, *, dtype=torch.float32):
         """Keys and values [n, page_tokens, kv_heads, head_dim] of ``pages``,
