@@ -486,7 +486,7 @@ typedef struct sq_kv_schedule {
     int32_t max_partials;
     int32_t q_heads;
     int32_t kv_heads;
-    int32_t rows;         /* 16, 32 or 256 */
+    int32_t rows;         /* 16, 32 or 256 (latent attention: see there) */
     int32_t causal;
     int32_t window;       /* 0: none; else the last `window` keys (causal only) */
     int32_t slots;        /* workers times KV heads that the device holds at once, at most 4096 */
@@ -623,6 +623,133 @@ typedef struct sq_kv_attend_args {
 } sq_kv_attend_args;
 
 int sq_kv_attend(const sq_kv_cache *cache, const sq_kv_attend_args *args, void *stream);
+
+/*
+ * Latent attention: a token's keys and values of all heads come from one shared
+ * vector, its latent, and one rope key.  A page holds page_tokens tokens, each
+ * its latent [latent] and its rope key [rope] one after the other, in 16 bits:
+ *   data   [num_pages, page_tokens, latent + rope], 16-byte aligned; page 0 is the
+ *          padding page, which no request holds
+ * latent is 256 or 512, rope 64; page_tokens a multiple of 64, at most 4096.
+ * Block tables and plans are those of the 8-bit cache.
+ */
+typedef struct sq_latent_cache {
+    void *data;
+    int64_t num_pages;
+    int32_t latent;
+    int32_t rope;
+    int32_t page_tokens;
+    int32_t dtype;        /* SQ_BF16 or SQ_F16 */
+} sq_latent_cache;
+
+/*
+ * Writes tokens' latents [tokens, latent] and rope keys [tokens, rope] (the
+ * cache's type, element strides per token that are multiples of 8, 16-byte
+ * aligned) to `slots`; -1 and slots that the cache does not have are passed
+ * over.  With `rotary` rope keys are turned to `positions` on the way; `rows`
+ * (NULL: none; the cache's type) are turned in the same launch, the tokens' queries as a rule.
+ */
+typedef struct sq_latent_append_args {
+    const void *latent;
+    const void *rope;
+    const int64_t *slots;
+    const int32_t *positions;
+    int64_t tokens;
+    int64_t latent_stride;
+    int64_t rope_stride;
+} sq_latent_append_args;
+
+int sq_latent_append(const sq_latent_cache *cache, const sq_latent_append_args *args, const sq_rotary *rotary,
+                     const sq_rotary_rows *rows, void *stream);
+
+/*
+ * The rows of requests, one request after the other: request b has lens[b] of
+ * them from starts[b] on, by row rows[b] of the table.  latent [rows_out, latent]
+ * and rope [rows_out, rope] are zero past the last; starts [batch + 1] end at
+ * rows_out where there are more.
+ */
+typedef struct sq_latent_gather_args {
+    const void *rows;
+    const int32_t *lens;
+    const int32_t *table;
+    void *latent;
+    void *rope;
+    int32_t *starts;
+    int64_t requests;
+    int64_t rows_out;
+    int32_t batch;
+    int32_t width;
+    int32_t rows_dtype;
+    int32_t reserved;
+} sq_latent_gather_args;
+
+int sq_latent_gather(const sq_latent_cache *cache, const sq_latent_gather_args *args, void *stream);
+
+/*
+ * Absorbed: out[t, h] = sum_j softmax_j(scale * (q[t, h] . c_j + q_rope[t, h] . r_j)) c_j
+ * over the latents c and rope keys r that the schedule lets token t see; zero
+ * where it sees none.
+ *   q, q_rope  [tokens, heads, latent] and [tokens, heads, rope], the cache's
+ *              type, strides multiples of 8, 16-byte aligned; out contiguous
+ *   workspace  max_partials * rows * (latent + 2) floats, 16-byte aligned
+ *   schedule   of one KV head (q_heads of them share it), rows 16, 32 or 64, no window
+ */
+typedef struct sq_latent_attend_args {
+    const void *q;
+    const void *q_rope;
+    void *out;
+    float *workspace;
+    const int32_t *table;
+    int64_t requests;
+    int64_t tokens;
+    int64_t q_stride;
+    int64_t q_head_stride;
+    int64_t rope_stride;
+    int64_t rope_head_stride;
+    int32_t width;
+    float scale;
+    sq_kv_schedule schedule;
+} sq_latent_attend_args;
+
+int sq_latent_attend(const sq_latent_cache *cache, const sq_latent_attend_args *args, void *stream);
+
+/*
+ * Expanded: out[t, h] = sum_j softmax_j(scale * (q[t, h] . [k[j, h], rope[j]])) v[j, h]
+ * over the keys of token t's request up to its own (causal) or all of them.
+ *   q          [tokens, heads, dim + 64]; k, v [rows, heads, dim]; rope
+ *              [rows, 64]; one type, SQ_BF16 or SQ_F16, strides multiples of 8,
+ *              16-byte aligned; out [tokens, heads, dim] contiguous; dim 64 or 128
+ *   cu         [batch + 1] the plan's first packed rows of queries
+ *   starts     [batch + 1] the requests' first rows of keys; request b has
+ *              starts[b + 1] - starts[b], at least what its tokens see (rows that
+ *              are not there are not seen)
+ *   schedule   of as many KV heads as query heads, rows 256, no window
+ */
+typedef struct sq_expanded_attend_args {
+    const void *q;
+    const void *k;
+    const void *v;
+    const void *rope;
+    void *out;
+    const int32_t *cu;
+    const int32_t *starts;
+    int64_t tokens;
+    int64_t rows;
+    int64_t q_stride;
+    int64_t q_head_stride;
+    int64_t k_stride;
+    int64_t k_head_stride;
+    int64_t v_stride;
+    int64_t v_head_stride;
+    int64_t rope_stride;
+    int32_t batch;
+    int32_t dim;
+    int32_t dtype;
+    float scale;
+    sq_kv_schedule schedule;
+} sq_expanded_attend_args;
+
+int sq_expanded_attend(const sq_expanded_attend_args *args, void *stream);
 
 /*
  * Flags for sq_pool.flags, computed from host copies of bits [H*K],

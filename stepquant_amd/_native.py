@@ -129,6 +129,38 @@ class RotaryRows(ctypes.Structure):
                 ("positions_dtype", ctypes.c_int32)]
 
 
+class LatentCache(ctypes.Structure):
+    _fields_ = [("data", _P), ("num_pages", ctypes.c_int64), ("latent", ctypes.c_int32), ("rope", ctypes.c_int32),
+                ("page_tokens", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class LatentAppend(ctypes.Structure):
+    _fields_ = [("latent", _P), ("rope", _P), ("slots", _P), ("positions", _P), ("tokens", ctypes.c_int64),
+                ("latent_stride", ctypes.c_int64), ("rope_stride", ctypes.c_int64)]
+
+
+class LatentGather(ctypes.Structure):
+    _fields_ = [("rows", _P), ("lens", _P), ("table", _P), ("latent", _P), ("rope", _P), ("starts", _P),
+                ("requests", ctypes.c_int64), ("rows_out", ctypes.c_int64), ("batch", ctypes.c_int32),
+                ("width", ctypes.c_int32), ("rows_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class LatentAttend(ctypes.Structure):
+    _fields_ = [("q", _P), ("q_rope", _P), ("out", _P), ("workspace", _P), ("table", _P), ("requests", ctypes.c_int64),
+                ("tokens", ctypes.c_int64), ("q_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("rope_stride", ctypes.c_int64), ("rope_head_stride", ctypes.c_int64), ("width", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("schedule", KVSchedule)]
+
+
+class ExpandedAttend(ctypes.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("rope", _P), ("out", _P), ("cu", _P), ("starts", _P),
+                ("tokens", ctypes.c_int64), ("rows", ctypes.c_int64), ("q_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("rope_stride", ctypes.c_int64),
+                ("batch", ctypes.c_int32), ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("schedule", KVSchedule)]
+
+
 FMT_FP32, FMT_SYMMETRIC, FMT_DSQ = 0, 1, 2
 FMT_ROWS_CONTIGUOUS = 1
 
@@ -139,7 +171,8 @@ EXPORTS = ("sq_abi_version", "sq_last_error", "sq_encode", "sq_decode_dense", "s
            "sq_format_encode", "sq_format_decode", "sq_format_step", "sq_copy_slots_static", "sq_copy_slots_direct",
            "sq_event_create", "sq_event_destroy", "sq_event_record", "sq_event_wait", "sq_event_query",
            "sq_event_synchronize", "sq_kv_plan", "sq_kv_commit", "sq_kv_release", "sq_kv_append", "sq_kv_decode",
-           "sq_kv_attend", "sq_rotary_apply", "sq_kv_append_rotary")
+           "sq_kv_attend", "sq_rotary_apply", "sq_kv_append_rotary", "sq_latent_append", "sq_latent_gather",
+           "sq_latent_attend", "sq_expanded_attend")
 COPY_STATIC_BYTES = 16 << 20
 COPY_DIRECT_PAGES = 256
 
@@ -196,6 +229,10 @@ def lib():
     L.sq_kv_attend.argtypes = [PP(KVCache), PP(KVAttend), _P]
     L.sq_rotary_apply.argtypes = [PP(Rotary), PP(RotaryRows), _P]
     L.sq_kv_append_rotary.argtypes = [PP(KVCache), PP(KVAppend), _P, PP(Rotary), PP(RotaryRows), _P]
+    L.sq_latent_append.argtypes = [PP(LatentCache), PP(LatentAppend), PP(Rotary), PP(RotaryRows), _P]
+    L.sq_latent_gather.argtypes = [PP(LatentCache), PP(LatentGather), _P]
+    L.sq_latent_attend.argtypes = [PP(LatentCache), PP(LatentAttend), _P]
+    L.sq_expanded_attend.argtypes = [PP(ExpandedAttend), _P]
     for name in EXPORTS:
         if name not in ("sq_last_error",):
             getattr(L, name).restype = ctypes.c_int
@@ -253,16 +290,23 @@ KV_PLAN = struct.Struct(f"=11Qq6i{KV_MAX_SCHEDULES * KV_SCHEDULE.size}s")
 KV_APPEND = struct.Struct("=5Q5q2i")
 KV_ATTEND = struct.Struct(f"=4Q4q2ifi{KV_SCHEDULE.size}s")
 ROTARY_ROWS = struct.Struct("=3Q5q4i")
+LATENT_APPEND = struct.Struct("=4Q3q")
+LATENT_GATHER = struct.Struct("=6Q2q4i")
+LATENT_ATTEND = struct.Struct(f"=5Q6qif{KV_SCHEDULE.size}s")
+EXPANDED_ATTEND = struct.Struct(f"=7Q9q3if{KV_SCHEDULE.size}s")
 _I32, _I64 = ctypes.c_int32, ctypes.c_int64
 _KV_ENTRIES = {"sq_kv_plan": [_P, ctypes.c_char_p, _P], "sq_kv_commit": [_P, ctypes.c_char_p, _P],
                "sq_kv_append": [_P, ctypes.c_char_p, _P], "sq_kv_attend": [_P, ctypes.c_char_p, _P],
                "sq_rotary_apply": [_P, ctypes.c_char_p, _P],
                "sq_kv_append_rotary": [_P, ctypes.c_char_p, _P, _P, ctypes.c_char_p, _P],
+               "sq_latent_append": [_P, ctypes.c_char_p, _P, ctypes.c_char_p, _P],
+               "sq_latent_gather": [_P, ctypes.c_char_p, _P], "sq_latent_attend": [_P, ctypes.c_char_p, _P],
+               "sq_expanded_attend": [ctypes.c_char_p, _P],
                "sq_kv_decode": [_P, _P, _P, _I64, _P, _P, _I32, _P]}
 
 
 def kv_entry(name: str):
-    """A KV or rotary entry point taking the address of its tables, cache or
+    """A KV, latent or rotary entry point taking the address of its tables, cache or
     frequencies and a packed argument block (``sq_kv_decode``: plain arguments)."""
     fn = _step_entries.get(name)
     if fn is None:

@@ -55,8 +55,9 @@ class KVPlan:
     holds; ``counters`` the tables' counters afterwards.
     """
 
-    __slots__ = ("tables", "rows", "counts", "tokens", "batch", "max_tiles", "schedules", "_args", "_ints", "_longs",
-                 "_sizes", "_append", "_views", "_positions")
+    __slots__ = ("tables", "rows", "counts", "tokens", "batch", "max_tiles", "schedules", "latent", "_args", "_ints", "_longs",
+                 "_sizes", "_append", "_views", "_positions", "_lens",
+                 "_cu", "_slots")
 
     def _view(self, i):
         # views are made when they are asked for: a step's kernels need none
@@ -126,7 +127,8 @@ class BlockTables:
             raise ValueError(f"{what} must be one-dimensional int32 or int64")
         return x if x.device == self.device and x.is_contiguous() else x.to(self.device).contiguous()
 
-    def plan(self, new, rows=None, *, tokens=None, max_new=None, heads=None, causal=True, window=0):
+    def plan(self, new, rows=None, *, tokens=None, max_new=None, heads=None, causal=True, window=0,
+             absorbed=None, expanded=None):
         """Room for ``new[b]`` tokens of the request in row ``rows[b]`` (default: row b).
 
         ``new`` and ``rows`` are lists or int32/int64 tensors, ``rows``
@@ -138,7 +140,9 @@ class BlockTables:
         (query heads, KV heads) also lays out the work of ``attend``: with
         ``causal`` each token sees its request's tokens up to itself, else all
         of them; ``window`` > 0 leaves it the last ``window`` of those.  A
-        tuple of windows lays out several kinds of layers.
+        tuple of windows lays out several kinds of layers.  ``absorbed`` and
+        ``expanded`` (numbers of query heads) lay out the work of latent attention
+        in either form, without windows; all together at most four kinds.
 
         Requests that find no room (``granted`` 0) keep their length; their
         tokens have no slot and their attention is zero.
@@ -177,12 +181,15 @@ class BlockTables:
         if any(windows) and not causal:
             raise ValueError("a window needs causal attention")
         heads = None if heads is None else tuple(heads)
-        key = (batch, tokens, max_new, heads, causal, windows)
+        if len(windows) * (heads is not None) + (absorbed is not None) + (expanded is not None) > N.KV_MAX_SCHEDULES:
+            raise ValueError(f"a plan takes at most {N.KV_MAX_SCHEDULES} kinds of layers")
+        key = (batch, tokens, max_new, heads, causal, windows, absorbed, expanded)
         layout = self._layouts.get(key)
         if layout is None:
             if len(self._layouts) >= 64:
                 self._layouts.clear()
-            layout = self._layouts[key] = self._layout(batch, tokens, max_new, heads, bool(causal), windows)
+            layout = self._layouts[key] = self._layout(batch, tokens, max_new, heads, bool(causal), windows, absorbed,
+                                                               expanded)
         sizes, total, offsets, most, schedules = layout
         p = KVPlan()
         p.tables, p.rows, p.counts, p.tokens, p.batch, p.max_tiles, p._views = self, rows, counts, tokens, batch, most, None
@@ -191,15 +198,15 @@ class BlockTables:
         p._longs = longs = torch.empty(2 + tokens, dtype=torch.int64, device=self.device)
         base, counters = ints.data_ptr(), longs.data_ptr()
         tiles, cu, positions, lens, granted, pages, filled = (base + x for x in offsets)
-        p.schedules, packed = {}, b""
+        p.schedules, p.latent, packed = {}, {}, b""
         for w, q_heads, kv_heads, floats, units, merges, starts, numbers in schedules:
             s = _Schedule()
             s.packed = N.KV_SCHEDULE.pack(base + units, base + merges, base + starts, *numbers)
             s.q_heads, s.kv_heads, s.floats = q_heads, kv_heads, floats
-            p.schedules[w] = s
+            (p.latent if isinstance(w, str) else p.schedules)[w] = s
             packed += s.packed
         p._append = (pages, filled, tiles)
-        p._positions = positions
+        p._positions, p._lens, p._cu, p._slots = positions, lens, cu, counters + 16
         p._args = args = N.KV_PLAN.pack(
             rows.data_ptr(), counts.data_ptr(), cu, counters + 16, positions, lens, granted, pages, filled, tiles, counters,
             tokens, batch, most, N.INTS[rows.dtype], N.INTS[counts.dtype], len(schedules), max_new,
@@ -240,14 +247,33 @@ class BlockTables:
     # and 31; 41 and 33, 39 and 37; 67 and 65, 71 and 81.
     few_rows, few_work = 1 << 14, 3 << 16
 
-    def _layout(self, batch, tokens, max_new, heads, causal, windows):
+    # Latent attention.  Absorbed, every head shares the one key: a set is rows of all heads.
+    latent_min_tiles, latent_cut_tiles = 2, 4
+
+    def _layout(self, batch, tokens, max_new, heads, causal, windows, absorbed=None, expanded=None):
         """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all
-        words, byte offsets of the first seven, page entries, per window what
-        ``sq_kv_schedule`` holds)."""
+        words, byte offsets of the first seven, page entries, per window or form of
+        latent attention what ``sq_kv_schedule`` holds)."""
         most = min(tokens, tokens // self.page_tokens + 2 * batch)
         # (page entries' pairs of words first, on a boundary of theirs)
         sizes = [2 * most, batch + 1, tokens, batch, -(-batch // 4), most, most]
         schedules = []
+
+        def add(key, window, q_heads, kv_heads, rows, slots, min_tiles, cut_tiles, few=False):
+            group = q_heads // kv_heads
+            sets, cuts = -(-tokens * group // (32 if few else rows)) + batch + 1, max(1, slots // kv_heads)
+            workers, joins = max(sets, cuts), min(sets, cuts)
+            if not schedules:
+                sizes.append(-sum(sizes) % 8)  # units and merges start on a boundary of their 32 bytes
+            units = 4 * sum(sizes)
+            merges = units + 32 * (sets + cuts)
+            numbers = (sets + cuts, joins, workers, 2 * cuts, q_heads, kv_heads, rows, causal, window, slots,
+                       min_tiles, cut_tiles, max(1, min(rows, max_new * group)),
+                       self.few_work if few else 0, self.min_tiles[32], self.cut_tiles[32])
+            schedules.append((key, q_heads, kv_heads, 2 * cuts * kv_heads * rows, units, merges, merges + 32 * joins,
+                              numbers))
+            sizes.append(8 * (sets + cuts + joins) + (workers + 9) // 8 * 8)
+
         if heads is not None:
             q_heads, kv_heads = (int(x) for x in heads)
             if q_heads <= 0 or kv_heads <= 0 or q_heads % kv_heads:
@@ -261,18 +287,21 @@ class BlockTables:
             rows = 16 if rows <= 16 else 32 if rows <= 64 else 256
             slots = 2 * self._cus if rows == 16 else self._cus
             few = rows == 256 and tokens * q_heads <= self.few_rows
-            sets, cuts = -(-tokens * group // (32 if few else rows)) + batch + 1, max(1, slots // kv_heads)
-            workers, joins = max(sets, cuts), min(sets, cuts)
-            sizes.append(-sum(sizes) % 8)  # units and merges start on a boundary of their 32 bytes
             for w in windows if tokens else ():
-                units = 4 * sum(sizes)
-                merges = units + 32 * (sets + cuts)
-                numbers = (sets + cuts, joins, workers, 2 * cuts, q_heads, kv_heads, rows, causal, int(w), slots,
-                           self.min_tiles[rows], self.cut_tiles[rows], max(1, min(rows, max_new * group)),
-                           self.few_work if few else 0, self.min_tiles[32], self.cut_tiles[32])
-                schedules.append((int(w), q_heads, kv_heads, 2 * cuts * kv_heads * rows, units, merges,
-                                  merges + 32 * joins, numbers))
-                sizes.append(8 * (sets + cuts + joins) + (workers + 9) // 8 * 8)
+                add(int(w), int(w), q_heads, kv_heads, rows, slots, self.min_tiles[rows], self.cut_tiles[rows], few)
+        for form, n in ("absorbed", absorbed), ("expanded", expanded):
+            if n is None:
+                continue
+            if not 0 < index(n) <= 4096 or tokens * n > 0x3fffffff:
+                raise ValueError(f"{form}: 1 to 4096 query heads, and fewer than 2^30 of all tokens")
+            if not tokens:
+                continue
+            if form == "absorbed":
+                rows = max_new * n
+                rows = 16 if rows <= 16 else 32 if rows <= 32 else 64
+                add(form, 0, n, 1, rows, self._cus, self.latent_min_tiles, self.latent_cut_tiles)
+            else:
+                add(form, 0, n, n, 256, self._cus, 1, 1 << 28)
         offsets = [4 * sum(sizes[:i]) for i in range(7)]
         return sizes, sum(sizes), offsets, most, schedules
 
