@@ -221,13 +221,21 @@ __global__ __launch_bounds__(256) void latent_gather_kernel(sq_latent_cache c, s
 // 64 lanes' groups side by side, so a lane asks for the group whose place it has.
 __device__ __forceinline__ int mix(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
 
-// 16 bytes a lane from memory to LDS at `lds` + 16 lane
-typedef const __attribute__((address_space(1))) void *global_t;
-__device__ __forceinline__ void to_lds(uint32_t lds, const void *lane_at) {
-  __builtin_amdgcn_global_load_lds((global_t)(uintptr_t)lane_at, (lds_t)(uintptr_t)lds, 16, 0, 0);
+// 16 bytes a lane from memory to LDS at `lds` + 16 lane.  The compiler does not
+// count these loads: it would wait for all of them before any write to LDS; the
+// waits are written out.  M0, which holds the place in LDS, has no other use in these kernels.
+__device__ __forceinline__ void to_lds(uint32_t lds, const uint8_t *base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-__device__ __forceinline__ void to_lds(uint32_t lds, const uint8_t *base, uint32_t offset) { to_lds(lds, base + offset); }
+__device__ __forceinline__ void to_lds(uint32_t lds, const void *lane_at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(lane_at) : "memory");
+}
+
+// a word that the whole wave reads and no kernel running beside writes, by the scalar cache
+__device__ __forceinline__ int uniform_word(const int32_t *p) {
+  return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p;
+}
 
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // until at most N are under way
@@ -248,8 +256,21 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 // Four consecutive rows' elements of one column, transposed: of 16 lanes, lane i
 // addresses row i / 4, columns 4 (i % 4) to 4 (i % 4) + 3, and lane j gets column j
 // of the four rows.
-__device__ __forceinline__ short4_v read_column(const uint8_t *p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_v *)(uintptr_t)(lds_t)p);
+__device__ __forceinline__ short4_v read_column(uint32_t lds) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_v *)lds);
+}
+
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(3))) T *from_lds(uint32_t lds) {
+  return (const __attribute__((address_space(3))) T *)lds;
+}
+
+// A value that the compiler takes for a new one: what is made from it is made where
+// it is used, and keeps no registers in loops around.
+template <typename T>
+__device__ __forceinline__ T anew(T x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // infinities and NaN of two halves as zero
@@ -291,7 +312,8 @@ struct Unit {
 
 __device__ __forceinline__ Unit read_unit(const AbsorbedDev &a, int i) {
   const int32_t *u = a.units + 8 * (int64_t)i;
-  Unit x = {u[0], u[1], u[2], u[3], u[4], u[5], u[6], u[7]};
+  const auto word = [&](int k) { return __builtin_amdgcn_readfirstlane(u[k]); };
+  Unit x = {word(0), word(1), word(2), word(3), word(4), word(5), word(6), word(7)};
   if (x.rows <= 0 || x.rows > a.unit_rows || x.q0 < 0 || x.f0 < 0 || x.kv0 < 0 ||
       x.q0 + (int64_t)(x.f0 + x.rows - 1) / a.heads >= a.tokens)
     x.rows = 0;
@@ -319,51 +341,44 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
   float *const peaks = (float *)(weights + R * PROW);    // [4][R] largest scores of 16 keys
   float *const sums = peaks + 4 * R;                     // [4][R]
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave & 3, rg = wave >> 2;
-  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int unit0 = max(0, a.starts[blockIdx.x]), unit1 = min(a.starts[blockIdx.x + 1], a.max_units);
+  const int lane = tid & 63;
+  const int unit0 = max(0, __builtin_amdgcn_readfirstlane(a.starts[blockIdx.x]));
+  const int unit1 = min(__builtin_amdgcn_readfirstlane(a.starts[blockIdx.x + 1]), a.max_units);
   if (unit0 >= unit1) return;
   const int G = a.heads, P = a.c.page_tokens;
   const uint32_t ring_at = lds_address(smem) + wave * (LOADS * 1024);
 
-  // the groups of a tile's 8 rows that a lane loads; a wave has 8 or 16 rows
-  uint32_t from[EIGHT];
-#pragma unroll
-  for (int i = 0; i < EIGHT; i++) {
-    const int n = 64 * i + lane, row = n / (KD / 8), at = n - row * (KD / 8);
-    from[i] = row * ROW + 16 * ((at & ~7) | ((at & 7) ^ mix(row)));
-  }
-  // where a lane's operands lie in a tile: keys by steps of 32 dims (even and odd), values by blocks of 16
-  // (4 of them are 128 bytes) and halves of 8 keys
-  const uint8_t *key_at[2], *value_at[4][2];
-#pragma unroll
-  for (int i = 0; i < 2; i++) key_at[i] = smem + (16 * kg + c) * ROW + 16 * ((4 * i + g) ^ mix(c & 7));
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int z = 0; z < 2; z++) {
-      const int row = 8 * g + 4 * z + (c >> 2), block = wave * DB + i;
-      value_at[i][z] = smem + row * ROW + 128 * (block >> 2) + 16 * ((2 * (block & 3) + (c >> 1 & 1)) ^ mix(row & 7)) + 8 * (c & 1);
-    }
-
+  const uint32_t tiles_at = lds_address(smem);
   Unit u = read_unit(a, unit0);
-  int n = 0, ids = 0;
+  int n = 0, page = 0, in_page = 0;  // of the tile that is loaded next
+  const int32_t *entry = a.table;
   auto load = [&](int i) {  // tile i, into its place of the ring
-    if ((i & 63) == 0) {    // the lanes hold the pages of 64 tiles
-      const int mine = i + lane;
-      ids = mine < n ? a.table[(int64_t)u.row * a.width + (u.kv0 + kTile * mine) / P] : 0;
-    }
-    const int first = u.kv0 + kTile * i, page = __builtin_amdgcn_readlane(ids, i & 63);
     const bool known = page > 0 && page < a.c.num_pages;
-    const uint8_t *base = (const uint8_t *)a.c.data + ((known ? (int64_t)page * P : 0) + first % P + wave * (kTile / NW)) * ROW;
+    const uint8_t *base = (const uint8_t *)a.c.data + ((known ? (int64_t)page * P : 0) + in_page + wave * (kTile / NW)) * ROW;
     const uint32_t to = ring_at + i % RING * TILE;
+    // a wave has 8 or 16 rows of the tile; the offsets of 8 rows' groups are made anew, too
+    const int from = anew(lane);
 #pragma unroll
-    for (int k = 0; k < LOADS; k++) to_lds(to + 1024 * k, base + k / EIGHT * (8 * ROW), from[k % EIGHT]);
+    for (int k = 0; k < EIGHT; k++) {
+      const int n = 64 * k + from, row = n / (KD / 8), at = n - row * (KD / 8);
+      const uint32_t offset = row * ROW + 16 * ((at & ~7) | ((at & 7) ^ mix(row)));
+#pragma unroll
+      for (int j = 0; j < LOADS / EIGHT; j++) to_lds(to + 1024 * (j * EIGHT + k), base + j * (8 * ROW), offset);
+    }
+    in_page += kTile;
+    if (in_page == P && i + 1 < n) in_page = 0, page = uniform_word(++entry);
     return known;
   };
   uint32_t known = 0;  // bit i % RING: tile i has a page
   auto begin = [&]() {
     n = max(0, (u.kv1 - u.kv0 + kTile - 1) / kTile);
     known = 0;
+    if (n) {
+      const int block = u.kv0 / P;
+      entry = a.table + (int64_t)u.row * a.width + block;
+      in_page = u.kv0 - block * P;
+      page = uniform_word(entry);
+    }
 #pragma unroll
     for (int i = 0; i < RING; i++)
       if (i < n && load(i)) known |= 1u << i;
@@ -374,13 +389,14 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
     int hi[NR];
     float l[NR], m[RT];
     f32x4_v o[RT][DB];
+    const int lane_q = anew(lane), cq = lane_q & 15, gq = lane_q >> 4;
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-      const int row = 16 * (rg * NR + r) + c, f = u.f0 + row;
+      const int row = 16 * (rg * NR + r) + cq, f = u.f0 + row;
       const bool live = row < u.rows;
       const int t = live ? f / G : 0, head = live ? f - t * G : 0;
-      const uint16_t *src = a.q + (u.q0 + t) * a.q_stride + head * a.q_head_stride + 8 * g;
-      const uint16_t *rope = a.rope + (u.q0 + t) * a.rope_stride + head * a.rope_head_stride + 8 * g;
+      const uint16_t *src = a.q + (u.q0 + t) * a.q_stride + head * a.q_head_stride + 8 * gq;
+      const uint16_t *rope = a.rope + (u.q0 + t) * a.rope_stride + head * a.rope_head_stride + 8 * gq;
 #pragma unroll
       for (int s = 0; s < KS; s++)
         q[r][s] = live ? *(const u32x4_v *)(s < W / 32 ? src + 32 * s : rope + 32 * s - W) : (u32x4_v){0, 0, 0, 0};
@@ -406,14 +422,20 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
 
     for (int i = 0; i < n; i++) {
       const int first = u.kv0 + kTile * i, at = i % RING * TILE;
+      constexpr int CHAINS = NR == 1 ? 2 : 1;
       f32x4_v s[NR][2];
 #pragma unroll
       for (int r = 0; r < NR; r++) s[r][0] = s[r][1] = (f32x4_v){0, 0, 0, 0};
+      // (a lane's offsets are made anew in each part of a tile: two waves on a SIMD
+      // leave no registers for them)
+      const int lane_k = anew(lane), c = lane_k & 15, g = lane_k >> 4;
+      // a lane's key: other steps of 32 dims flip bit 6, or lie 128 bytes on
+      const uint32_t keys = tiles_at + at + (16 * kg + c) * ROW + 16 * (g ^ mix(c & 7));
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        const u32x4_v w = *(const u32x4_v *)(key_at[k & 1] + at + 128 * (k >> 1));
+        const u32x4_v w = *from_lds<u32x4_v>((keys ^ 64 * (k & 1)) + 128 * (k >> 1));
 #pragma unroll
-        for (int r = 0; r < NR; r++) s[r][k & 1] = H::mul32(w, q[r][k], s[r][k & 1]);
+        for (int r = 0; r < NR; r++) s[r][k % CHAINS] = H::mul32(w, q[r][k], s[r][k % CHAINS]);
       }
       const bool there = known >> (i % RING) & 1, whole = there && first + kTile <= all_hi;
       float x[NR][4];
@@ -442,9 +464,10 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
           *p = w;
         }
       }
+      const int lane_p = anew(lane), cp = lane_p & 15, gp = lane_p >> 4;
 #pragma unroll
       for (int r = 0; r < RT; r++) {
-        const float *peak = peaks + 16 * r + c;
+        const float *peak = peaks + 16 * r + cp;
         const float best = fmaxf(fmaxf(peak[0], peak[R]), fmaxf(peak[2 * R], peak[3 * R]));
         if (__any(best - m[r] > kTop)) {
           const float raised = best - m[r] > kTop ? best - kBias : m[r], shrink = __builtin_amdgcn_exp2f(m[r] - raised);
@@ -464,20 +487,25 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
         for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(x[r][k] - unit);
         const uint2 w = make_uint2(H::pack(p[0], p[1]), H::pack(p[2], p[3]));
         l[r] += H::sum(w.x) + H::sum(w.y);
-        *(uint2 *)(weights + (16 * (rg * NR + r) + c) * PROW + 2 * (16 * kg + 4 * g)) = w;
+        *(uint2 *)(weights + (16 * (rg * NR + r) + cp) * PROW + 2 * (16 * kg + 4 * gp)) = w;
       }
       __syncthreads();
+      // a lane's four keys of the wave's first 16 dims: four blocks of 16 flip bits 5
+      // and 6, four keys on flip bit 4
+      const int lane_v = anew(lane), cv = lane_v & 15, gv = lane_v >> 4, row_v = 8 * gv + (cv >> 2);
+      const uint32_t values = tiles_at + at + row_v * ROW + 128 * (wave * DB >> 2) +
+                              16 * ((2 * (wave * DB & 3) + (cv >> 1 & 1)) ^ mix(row_v & 7)) + 8 * (cv & 1);
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         u32x4_v p[RT];
 #pragma unroll
-        for (int r = 0; r < RT; r++) p[r] = *(const u32x4_v *)(weights + (16 * r + c) * PROW + 64 * j + 16 * g);
+        for (int r = 0; r < RT; r++) p[r] = *(const u32x4_v *)(weights + (16 * r + cv) * PROW + 64 * j + 16 * gv);
 #pragma unroll
         for (int e = 0; e < DB; e++) {
           uint2 w[2];
 #pragma unroll
           for (int z = 0; z < 2; z++)
-            w[z] = __builtin_bit_cast(uint2, read_column(value_at[e & 3][z] + at + 128 * (e >> 2) + 32 * j * ROW));
+            w[z] = __builtin_bit_cast(uint2, read_column((values ^ (32 * (e & 3) + 16 * z)) + 128 * (e >> 2) + (32 * j + 4 * z) * ROW));
           const u32x4_v v = {w[0].x, w[0].y, w[1].x, w[1].y};
 #pragma unroll
           for (int r = 0; r < RT; r++) o[r][e] = H::mul32(v, p[r], o[r][e]);
@@ -492,6 +520,7 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
     }
     // the next unit's first tiles load while this one's outputs leave
     const Unit done = u;
+    const int lane_o = anew(lane), co = lane_o & 15, go = lane_o >> 4;
     if (unit_at + 1 < unit1) {
       u = read_unit(a, unit_at + 1);
       begin();
@@ -499,12 +528,12 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
 #pragma unroll
     for (int r = 0; r < NR; r++) {
       const float sum = sum4(l[r]);
-      if (g == 0) sums[kg * R + 16 * (rg * NR + r) + c] = sum;
+      if (go == 0) sums[kg * R + 16 * (rg * NR + r) + co] = sum;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const int row = 16 * r + c, d = wave * (W / NW) + 4 * g;
+      const int row = 16 * r + co, d = wave * (W / NW) + 4 * go;
       const float *part = sums + row;
       const float all = (part[0] + part[R]) + (part[2 * R] + part[3 * R]);
       if (row >= done.rows) continue;
@@ -517,7 +546,7 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
         const int64_t slot = (int64_t)done.part * a.unit_rows + row;
 #pragma unroll
         for (int e = 0; e < DB; e++) *(f32x4_v *)(a.ws + slot * W + d + 16 * e) = o[r][e];
-        if (wave == 0 && g == 0)
+        if (wave == 0 && go == 0)
           *(float2 *)(a.ws + (int64_t)a.max_partials * a.unit_rows * W + 2 * slot) = make_float2(m[r], all);
       }
     }
@@ -655,6 +684,7 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
       __syncthreads();
       if (i + 1 < n) load(i + 1);
       const uint8_t *keys = kt + (i & 1) * KTILE, *values = vt + (i & 1) * VTILE;
+      const uint32_t values_at = vt_at + (i & 1) * VTILE;
       if (!whole) {
         // Values that are not numbers would reach rows that do not see their key
         // (0 times infinity); they are taken out, and rows that do see the key are NaN.
@@ -724,7 +754,7 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
           for (int z = 0; z < 2; z++) {
             const int row = 16 * j + 8 * z + 4 * hl + (lane >> 2 & 3), col = 32 * e + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
             const int g = col / 8;
-            w[z] = __builtin_bit_cast(uint2, read_column(values + row * VROW + 16 * ((g & ~7) | ((g & 7) ^ mix(row & 7))) + 2 * (col & 7)));
+            w[z] = __builtin_bit_cast(uint2, read_column(values_at + row * VROW + 16 * ((g & ~7) | ((g & 7) ^ mix(row & 7))) + 2 * (col & 7)));
           }
           o[e] = H::mul((u32x4_v){w[0].x, w[0].y, w[1].x, w[1].y}, p[j], o[e]);
         }
