@@ -692,7 +692,7 @@ int sq_latent_gather(const sq_latent_cache *cache, const sq_latent_gather_args *
  *   q, q_rope  [tokens, heads, latent] and [tokens, heads, rope], the cache's
  *              type, strides multiples of 8, 16-byte aligned; out contiguous
  *   workspace  max_partials * rows * (latent + 2) floats, 16-byte aligned
- *   schedule   of one KV head (q_heads of them share it), rows 16, 32 or 64, no window
+ *   schedule   of one KV head (q_heads of them share it), rows 16, 32, 64 or 128, no window
  */
 typedef struct sq_latent_attend_args {
     const void *q;

@@ -1815,7 +1815,8 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
   if (!s->units || !s->merges || !s->starts) return fail(SQ_EINVAL, "kv schedule: null pointer");
   if (s->kv_heads <= 0 || s->q_heads <= 0 || s->q_heads % s->kv_heads)
     return fail(SQ_ESHAPE, "kv schedule: q_heads must be a positive multiple of kv_heads");
-  if (s->rows != 16 && s->rows != 32 && s->rows != 64 && s->rows != 256) return fail(SQ_ESHAPE, "kv schedule: rows");
+  if (s->rows != 16 && s->rows != 32 && s->rows != 64 && s->rows != 128 && s->rows != 256)
+    return fail(SQ_ESHAPE, "kv schedule: rows");
   if (s->window < 0 || (s->window > 0 && !s->causal))
     return fail(SQ_EINVAL, "kv schedule: a window is non-negative and needs causal attention");
   if (s->slots <= 0 || s->slots > kMaxSlots) return fail(SQ_EINVAL, "kv schedule: slots must be in [1, 4096]");
@@ -2050,7 +2051,7 @@ int sq_kv_attend(const sq_kv_cache *c, const sq_kv_attend_args *a, void *stream)
   if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(SQ_EINVAL, "kv attend: scale must be finite");
   rc = check_schedule(&a->schedule, a->tokens, 1);
   if (rc) return rc;
-  if (a->schedule.kv_heads != c->heads || a->schedule.rows == 64)
+  if (a->schedule.kv_heads != c->heads || a->schedule.rows == 64 || a->schedule.rows == 128)
     return fail(SQ_ESHAPE, "kv attend: the schedule is for another number of KV heads, or for latent attention");
   if (!a->workspace || ((uintptr_t)a->workspace & 15))
     return fail(SQ_EINVAL, "kv attend: null or misaligned workspace");

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "internal.h"
 #include "rotary.h"
@@ -101,6 +102,26 @@ __device__ __forceinline__ float sum4(float x) {
   x = sum2(x);
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+// over the 8 or 16 lanes of a row: the lane 1, 2, 7 - l and 15 - l away
+template <int LANES>
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, dpp<0xb1>(x));
+  x = fmaxf(x, dpp<0x4e>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  return LANES == 8 ? x : fmaxf(x, dpp<0x140>(x));
+}
+template <int LANES>
+__device__ __forceinline__ float row_sum(float x) {
+  x += dpp<0xb1>(x);
+  x += dpp<0x4e>(x);
+  x += dpp<0x141>(x);
+  return LANES == 8 ? x : x + dpp<0x140>(x);
 }
 
 // ------------------------------------------------------------ pages
@@ -228,6 +249,11 @@ __device__ __forceinline__ void to_lds(uint32_t lds, const uint8_t *base, uint32
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
+// the same, of what nothing else will read (64 requests of up to 8192: 8% faster)
+__device__ __forceinline__ void to_lds_once(uint32_t lds, const uint8_t *base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+
 __device__ __forceinline__ void to_lds(uint32_t lds, const void *lane_at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(lane_at) : "memory");
 }
@@ -273,6 +299,11 @@ __device__ __forceinline__ T anew(T x) {
   return x;
 }
 
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(3))) T *to_lds_at(uint32_t lds) {
+  return (__attribute__((address_space(3))) T *)lds;
+}
+
 // infinities and NaN of two halves as zero
 template <bool BF16>
 __device__ __forceinline__ uint32_t only_finite(uint32_t w) {
@@ -310,13 +341,15 @@ struct Unit {
   int row, q0, f0, rows, pos0, kv0, kv1, part;
 };
 
-__device__ __forceinline__ Unit read_unit(const AbsorbedDev &a, int i) {
+// rows at_row to at_row + most - 1 of a unit
+__device__ __forceinline__ Unit read_unit(const AbsorbedDev &a, int i, int at_row, int most) {
   const int32_t *u = a.units + 8 * (int64_t)i;
-  const auto word = [&](int k) { return __builtin_amdgcn_readfirstlane(u[k]); };
+  const auto word = [&](int k) { return uniform_word(u + k); };
   Unit x = {word(0), word(1), word(2), word(3), word(4), word(5), word(6), word(7)};
   if (x.rows <= 0 || x.rows > a.unit_rows || x.q0 < 0 || x.f0 < 0 || x.kv0 < 0 ||
       x.q0 + (int64_t)(x.f0 + x.rows - 1) / a.heads >= a.tokens)
     x.rows = 0;
+  x.f0 += at_row, x.rows = max(0, min(x.rows - at_row, most));
   x.kv0 &= ~(kTile - 1);  // (a tile lies within a page)
   // a row of the table that does not exist holds no keys
   const bool held = x.rows > 0 && x.row >= 0 && x.row < a.requests;
@@ -324,218 +357,315 @@ __device__ __forceinline__ Unit read_unit(const AbsorbedDev &a, int i) {
   return x;
 }
 
-// A workgroup has RG groups of four waves and units of up to 16 RG NR rows.  Of a
-// tile of 64 keys, in a ring of tiles in LDS, each wave of a group takes the
-// scores of 16 keys and of the group's NR times 16 rows; the weights pass through
-// LDS, and each wave of the workgroup takes the outputs of its own share of the
-// dims, for all rows.  So keys are read from LDS once for each group, values once, and
-// outputs need no joining.
-template <int W, int RG, int NR, bool BF16>
-__global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev a) {
+// A workgroup has RG groups of four waves and units of up to 16 RG NR rows; tiles of
+// 32 keys pass through a ring in LDS.  A tile goes through two steps, with a
+// barrier behind each:
+//
+//   products  outputs with the tile before, every wave for its own share of the
+//             dims and all rows (so outputs need no joining); then scores with this
+//             tile, every wave for 16 keys, the group's rows and half of the dims,
+//             which go to LDS as sums in 32 bits;
+//   softmax   by rows: 8 or 16 lanes have a row's 32 scores, and alone know its
+//             unit and its sum; rounded weights and what the row's outputs are
+//             to be multiplied by go to LDS.
+//
+// So keys are read from LDS once for each group and values once, and a wave holds half of
+// its rows' queries.  PAIR: units of 128 rows have two workgroups, which run side by side
+// on one XCD (8 apart, blocks go to the 8 in turn) so that its L2 gives one of
+// them the keys; others are read past the caches' later use.
+template <int W_, int RG_, int NR_, int RING_, bool PAIR_ = false>
+struct Absorbed {
+  static constexpr int W = W_, TK = 32, RG = RG_, NR = NR_, RING = RING_, NW = 4 * RG, threads = 64 * NW;
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int R = 16 * RG * NR, TILE = TK * 2 * (W + kRope);
+  static constexpr int SROW = 4 * TK + 16, PROW = 2 * TK + 16;  // bytes from row to row of scores and weights
+  static constexpr size_t lds = RING * TILE + R * (2 * SROW + PROW + 4);
+  static_assert(lds <= 163840, "LDS of a CU");
+};
+
+template <typename S, bool BF16>
+__global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(AbsorbedDev a) {
   typedef Half<BF16> H;
-  constexpr int KD = W + kRope, ROW = 2 * KD, TILE = kTile * ROW, RING = W == 512 ? 2 : 3;
-  constexpr int NW = 4 * RG, LOADS = TILE / 1024 / NW, EIGHT = KD / 64;  // loads of a wave's tile, of 8 rows
-  constexpr int KS = KD / 32, DB = W / NW / 16, RT = RG * NR, R = 16 * RT, PROW = 2 * kTile + 16;
-  extern __shared__ uint8_t smem[];
-  uint8_t *const weights = smem + RING * TILE;           // [R] rows of 64 weights
-  float *const peaks = (float *)(weights + R * PROW);    // [4][R] largest scores of 16 keys
-  float *const sums = peaks + 4 * R;                     // [4][R]
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave & 3, rg = wave >> 2;
-  const int lane = tid & 63;
-  const int unit0 = max(0, __builtin_amdgcn_readfirstlane(a.starts[blockIdx.x]));
-  const int unit1 = min(__builtin_amdgcn_readfirstlane(a.starts[blockIdx.x + 1]), a.max_units);
+  constexpr int W = S::W, TK = S::TK, RG = S::RG, NR = S::NR, NW = S::NW, RING = S::RING, TILE = S::TILE, R = S::R;
+  constexpr int KD = W + kRope, ROW = 2 * KD, KS = KD / 64, DB = W / NW / 16, RT = RG * NR;
+  constexpr int SROW = S::SROW, PROW = S::PROW;
+  constexpr int BLOCKS = TILE / 1024, MOST = (BLOCKS + NW - 1) / NW;  // loads of a tile, of a wave
+  constexpr int LANES = 64 * NW / R, KEYS = TK / LANES;               // of a row's softmax, and of a lane
+  extern __shared__ __attribute__((aligned(128))) uint8_t smem[];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int kg = wave & 1, dh = wave >> 1 & 1, rg = wave >> 2;
+  const int worker = S::PAIR ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x;
+  const int at_row = S::PAIR ? R * (blockIdx.x >> 3 & 1) : 0;
+  if (worker >= a.max_workers) return;
+  const int unit0 = max(0, uniform_word(a.starts + worker)), unit1 = min(uniform_word(a.starts + worker + 1), a.max_units);
   if (unit0 >= unit1) return;
   const int G = a.heads, P = a.c.page_tokens;
-  const uint32_t ring_at = lds_address(smem) + wave * (LOADS * 1024);
-
   const uint32_t tiles_at = lds_address(smem);
-  Unit u = read_unit(a, unit0);
-  int n = 0, page = 0, in_page = 0;  // of the tile that is loaded next
-  const int32_t *entry = a.table;
-  auto load = [&](int i) {  // tile i, into its place of the ring
-    const bool known = page > 0 && page < a.c.num_pages;
-    const uint8_t *base = (const uint8_t *)a.c.data + ((known ? (int64_t)page * P : 0) + in_page + wave * (kTile / NW)) * ROW;
-    const uint32_t to = ring_at + i % RING * TILE;
-    // a wave has 8 or 16 rows of the tile; the offsets of 8 rows' groups are made anew, too
-    const int from = anew(lane);
+  const uint32_t scores = tiles_at + RING * TILE;     // [2][R] rows of TK
+  const uint32_t weights = scores + 2 * R * SROW;     // [R] rows of TK
+  const uint32_t factors = weights + R * PROW;        // [R]
+  // Where a lane's operands lie.  Its key and first dims in a tile: other steps of
+  // 32 dims flip bit 6, or lie 128 bytes on.  Its four keys of the wave's first 16
+  // dims: four blocks of 16 flip bits 5 and 6, four keys on flip bit 4.
+  const int c = lane & 15, g = lane >> 4, token = 8 * g + (c >> 2);
+  static_assert(KS % 2 == 1, "the second half of the dims begins with an odd step");
+  const uint32_t key_at = tiles_at + (16 * kg + c) * ROW + 16 * (g ^ mix(c & 7)) + 64 * (KS - 1) * dh;
+  const uint32_t even_at = key_at ^ 64 * dh, odd_at = (key_at ^ 64 * (1 - dh)) + 128 * dh;
+  const uint32_t value_at = tiles_at + token * ROW + 128 * (wave * DB >> 2) +
+                            16 * ((2 * (wave * DB & 3) + (c >> 1 & 1)) ^ mix(token & 7)) + 8 * (c & 1);
+  const uint32_t score_to = scores + (dh * R + 16 * rg * NR + c) * SROW + 64 * kg + 16 * g;
+  const uint32_t weight_at = weights + c * PROW + 16 * g, factor_at = factors + 4 * c;
+  const int mine = tid / LANES, part = tid % LANES;   // the lane's row of the softmax, and its keys there
+  const uint32_t score_at = scores + mine * SROW + 4 * KEYS * part, weight_to = weights + mine * PROW + 2 * KEYS * part;
+  uint32_t from[MOST];  // the groups of a tile that a lane loads
 #pragma unroll
-    for (int k = 0; k < EIGHT; k++) {
-      const int n = 64 * k + from, row = n / (KD / 8), at = n - row * (KD / 8);
-      const uint32_t offset = row * ROW + 16 * ((at & ~7) | ((at & 7) ^ mix(row)));
-#pragma unroll
-      for (int j = 0; j < LOADS / EIGHT; j++) to_lds(to + 1024 * (j * EIGHT + k), base + j * (8 * ROW), offset);
-    }
-    in_page += kTile;
-    if (in_page == P && i + 1 < n) in_page = 0, page = uniform_word(++entry);
-    return known;
+  for (int k = 0; k < MOST; k++) {
+    const int n = min(64 * NW * k + tid, TILE / 16 - 1), row = n / (KD / 8), at = n - row * (KD / 8);
+    from[k] = row * ROW + 16 * ((at & ~7) | ((at & 7) ^ mix(row & 7)));
+  }
+  const bool more = wave < BLOCKS % NW;  // the wave has MOST loads of a tile, else one fewer
+
+  // the tile that is loaded next: its page, the tokens before it there
+  struct Place {
+    const int32_t *entry;
+    int page, in_page, n;
   };
-  uint32_t known = 0;  // bit i % RING: tile i has a page
-  auto begin = [&]() {
-    n = max(0, (u.kv1 - u.kv0 + kTile - 1) / kTile);
-    known = 0;
-    if (n) {
+  auto place = [&](const Unit &u) {
+    Place x = {a.table, 0, 0, max(0, (u.kv1 - u.kv0 + TK - 1) / TK)};
+    if (x.n) {
       const int block = u.kv0 / P;
-      entry = a.table + (int64_t)u.row * a.width + block;
-      in_page = u.kv0 - block * P;
-      page = uniform_word(entry);
+      x.entry += (int64_t)u.row * a.width + block;
+      x.in_page = u.kv0 - block * P;
+      x.page = uniform_word(x.entry);
     }
+    return x;
+  };
+  Unit u = read_unit(a, unit0, at_row, R);
+  Place next = place(u);
+  int n = 0, loaded = 0;  // tiles of the unit, and how many of them are on their way
+  uint32_t known = 0;     // bit i % RING: tile i has a page
+  auto load = [&]() {
+    const int i = loaded++;
+    const bool there = next.page > 0 && next.page < a.c.num_pages;
+    const uint8_t *base = (const uint8_t *)a.c.data + ((there ? (int64_t)next.page * P : 0) + next.in_page) * ROW;
+    const uint32_t bit = 1u << (i % RING), to = tiles_at + i % RING * TILE + 1024 * wave;
+    known = there ? known | bit : known & ~bit;
 #pragma unroll
-    for (int i = 0; i < RING; i++)
-      if (i < n && load(i)) known |= 1u << i;
+    for (int k = 0; k < MOST; k++) {
+      if (k == MOST - 1 && BLOCKS % NW && !more) break;
+      if constexpr (S::PAIR) to_lds(to + 1024 * NW * k, base, from[k]);
+      else to_lds_once(to + 1024 * NW * k, base, from[k]);
+    }
+    next.in_page += TK;
+    if (next.in_page == P && i + 1 < n) next.in_page = 0, next.page = uniform_word(++next.entry);
+  };
+  // until at most `tiles` of the tiles on their way are not there
+  auto wait_tiles = [&](int tiles) {
+    if (tiles >= RING - 2) {
+      if (BLOCKS % NW == 0 || more) wait_loads<(RING - 2) * MOST>();
+      else wait_loads<(RING - 2) * (MOST - 1)>();
+    } else {
+      wait_loads<0>();
+    }
+  };
+  auto begin = [&]() {
+    n = next.n, loaded = 0;
+#pragma unroll
+    for (int i = 0; i < RING - 1; i++)
+      if (i < n) load();
   };
   begin();
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
+    const Unit following = read_unit(a, min(unit_at + 1, unit1 - 1), at_row, R);
+    const Place after = place(following);
     u32x4_v q[NR][KS];
-    int hi[NR];
-    float l[NR], m[RT];
     f32x4_v o[RT][DB];
-    const int lane_q = anew(lane), cq = lane_q & 15, gq = lane_q >> 4;
+    {
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-      const int row = 16 * (rg * NR + r) + cq, f = u.f0 + row;
-      const bool live = row < u.rows;
-      const int t = live ? f / G : 0, head = live ? f - t * G : 0;
-      const uint16_t *src = a.q + (u.q0 + t) * a.q_stride + head * a.q_head_stride + 8 * gq;
-      const uint16_t *rope = a.rope + (u.q0 + t) * a.rope_stride + head * a.rope_head_stride + 8 * gq;
+      for (int r = 0; r < NR; r++) {
+        const int row = 16 * (rg * NR + r) + c, f = u.f0 + row;
+        const bool live = row < u.rows;
+        const int t = live ? f / G : 0, head = live ? f - t * G : 0;
+        const uint16_t *src = a.q + (u.q0 + t) * a.q_stride + head * a.q_head_stride + 8 * g;
+        const uint16_t *rope = a.rope + (u.q0 + t) * a.rope_stride + head * a.rope_head_stride + 8 * g;
 #pragma unroll
-      for (int s = 0; s < KS; s++)
-        q[r][s] = live ? *(const u32x4_v *)(s < W / 32 ? src + 32 * s : rope + 32 * s - W) : (u32x4_v){0, 0, 0, 0};
-      hi[r] = live ? a.causal ? min(u.kv1, u.pos0 + t + 1) : u.kv1 : 0;
-      l[r] = 0.f;
+        for (int s = 0; s < KS; s++) {
+          const int d = 32 * (KS * dh + s);
+          q[r][s] = live ? *(const u32x4_v *)(d < W ? src + d : rope + d - W) : (u32x4_v){0, 0, 0, 0};
+        }
+      }
     }
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-      m[r] = kNone;
+    for (int r = 0; r < RT; r++)
 #pragma unroll
       for (int e = 0; e < DB; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
-    }
-    // (their loads are waited for here, not by a wait for all loads in the loop)
+    // (the queries' loads are waited for here, not by a wait for all loads in the loop)
 #pragma unroll
     for (int r = 0; r < NR; r++)
 #pragma unroll
       for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[r][s]));
     const float mult = a.scale * kLog2e;
+    // the keys that the lane's row sees
+    const int hi = mine >= u.rows ? 0 : a.causal ? min(u.kv1, u.pos0 + (u.f0 + mine) / G + 1) : u.kv1;
     // keys that every row of the unit sees
     const int all_hi = u.rows <= 0 ? 0 : a.causal ? min(u.kv1, u.pos0 + u.f0 / G + 1) : u.kv1;
-    wait_ring<LOADS * (RING - 1)>(n >= RING);
-    __syncthreads();
+    float m = kNone, l = 0.f;
 
-    for (int i = 0; i < n; i++) {
-      const int first = u.kv0 + kTile * i, at = i % RING * TILE;
-      constexpr int CHAINS = NR == 1 ? 2 : 1;
-      f32x4_v s[NR][2];
+    // Outputs with tile i - 1 (OUT) and scores with tile i (IN), their products in turn;
+    // operands are read some products ahead.
+    auto products = [&](auto OUT, auto IN, int i) {
+      constexpr int NO = decltype(OUT)::value ? DB : 0, NI = decltype(IN)::value ? KS : 0, N = NO + NI;
+      constexpr int AHEAD_K = NI < 3 ? NI : 3, AHEAD_V = NO < 2 ? NO : 2;
+      const uint32_t even_keys = even_at + i % RING * TILE, odd_keys = odd_at + i % RING * TILE;
+      const uint32_t values = value_at + (i + RING - 1) % RING * TILE;
+      u32x4_v p[RT], kw[AHEAD_K + 1], vw[AHEAD_V + 1];
+      f32x4_v s[NR];
 #pragma unroll
-      for (int r = 0; r < NR; r++) s[r][0] = s[r][1] = (f32x4_v){0, 0, 0, 0};
-      // (a lane's offsets are made anew in each part of a tile: two waves on a SIMD
-      // leave no registers for them)
-      const int lane_k = anew(lane), c = lane_k & 15, g = lane_k >> 4;
-      // a lane's key: other steps of 32 dims flip bit 6, or lie 128 bytes on
-      const uint32_t keys = tiles_at + at + (16 * kg + c) * ROW + 16 * (g ^ mix(c & 7));
+      for (int r = 0; r < NR; r++) s[r] = (f32x4_v){0, 0, 0, 0};
+      auto read_key = [&](int k) {
+        return *from_lds<u32x4_v>((k & 1 ? odd_keys : even_keys) + 128 * (k >> 1));
+      };
+      auto read_value = [&](int e) {
+        uint2 w[2];
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        const u32x4_v w = *from_lds<u32x4_v>((keys ^ 64 * (k & 1)) + 128 * (k >> 1));
+        for (int z = 0; z < 2; z++)
+          w[z] = __builtin_bit_cast(uint2, read_column((values ^ (32 * (e & 3) + 16 * z)) + 128 * (e >> 2) + 4 * z * ROW));
+        return (u32x4_v){w[0].x, w[0].y, w[1].x, w[1].y};
+      };
+      if constexpr (NO > 0) {
+        float f[RT];
+        bool raised = false;
 #pragma unroll
-        for (int r = 0; r < NR; r++) s[r][k % CHAINS] = H::mul32(w, q[r][k], s[r][k % CHAINS]);
-      }
-      const bool there = known >> (i % RING) & 1, whole = there && first + kTile <= all_hi;
-      float x[NR][4];
-#pragma unroll
-      for (int r = 0; r < NR; r++) {
-        float best = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          x[r][k] = (s[r][0][k] + s[r][1][k]) * mult;
-          if (!whole) x[r][k] = there && first + 16 * kg + 4 * g + k < hi[r] ? x[r][k] : -INFINITY;
-          best = fmaxf(best, x[r][k]);
+        for (int r = 0; r < RT; r++) {
+          f[r] = *from_lds<float>(factor_at + 64 * r);
+          p[r] = *from_lds<u32x4_v>(weight_at + 16 * r * PROW);
+          raised |= f[r] != 1.f;
         }
-        best = max4(best);
-        if (g == 0) peaks[kg * R + 16 * (rg * NR + r) + c] = best;
+        if (__any(raised)) {
+#pragma unroll
+          for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int e = 0; e < DB; e++) o[r][e] *= f[r];
+        }
       }
-      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < AHEAD_K; k++) kw[k] = read_key(k);
+#pragma unroll
+      for (int e = 0; e < AHEAD_V; e++) vw[e] = read_value(e);
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const int e = NO ? j * NO / N : 0;  // products of outputs before this one
+        if (NO && (j + 1) * NO / N > e) {
+          if (e + AHEAD_V < NO) vw[(e + AHEAD_V) % (AHEAD_V + 1)] = read_value(e + AHEAD_V);
+#pragma unroll
+          for (int r = 0; r < RT; r++) o[r][e] = H::mul32(vw[e % (AHEAD_V + 1)], p[r], o[r][e]);
+        } else {
+          const int k = j - e;
+          if (k + AHEAD_K < NI) kw[(k + AHEAD_K) % (AHEAD_K + 1)] = read_key(k + AHEAD_K);
+#pragma unroll
+          for (int r = 0; r < NR; r++) s[r] = H::mul32(kw[k % (AHEAD_K + 1)], q[r][k], s[r]);
+        }
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, AHEAD_K + 2 * AHEAD_V, 0);  // LDS reads
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const int e = NO ? j * NO / N : 0;
+        if (NO && (j + 1) * NO / N > e) {
+          if (e + AHEAD_V < NO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x8, RT, 0);  // products
+        } else {
+          if (j - e + AHEAD_K < NI) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x8, NR, 0);
+        }
+      }
+      if constexpr (NI > 0) {
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+          *to_lds_at<f32x4_v>(score_to + 16 * r * SROW) = s[r];
+      }
+    };
+    auto softmax = [&](int i) {
+      const int first = u.kv0 + TK * i;
+      const bool there = known >> (i % RING) & 1, whole = there && first + TK <= all_hi;
+      typedef float vec __attribute__((ext_vector_type(KEYS)));
+      vec x = *from_lds<vec>(score_at) + *from_lds<vec>(score_at + R * SROW);
       if (!whole) {
         // What some row does not see has a weight of 0 there; infinities and NaN
         // would still reach its outputs.  (Rows that see them have them in their scores.)
-        const int r0 = there ? max(0, min(kTile, all_hi - first)) : 0;
-        for (int j = r0 * (KD / 8) + tid; j < kTile * (KD / 8); j += 256 * RG) {
-          u32x4_v *p = (u32x4_v *)(smem + at + 16 * j);
+        const int r0 = there ? max(0, min(TK, all_hi - first)) : 0;
+        for (int j = r0 * (KD / 8) + tid; j < TK * (KD / 8); j += 64 * NW) {
+          u32x4_v *p = (u32x4_v *)(smem + i % RING * TILE + 16 * j);
           u32x4_v w = *p;
 #pragma unroll
           for (int k = 0; k < 4; k++) w[k] = only_finite<BF16>(w[k]);
           *p = w;
         }
       }
-      const int lane_p = anew(lane), cp = lane_p & 15, gp = lane_p >> 4;
+      float best = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const float *peak = peaks + 16 * r + cp;
-        const float best = fmaxf(fmaxf(peak[0], peak[R]), fmaxf(peak[2 * R], peak[3 * R]));
-        if (__any(best - m[r] > kTop)) {
-          const float raised = best - m[r] > kTop ? best - kBias : m[r], shrink = __builtin_amdgcn_exp2f(m[r] - raised);
-          m[r] = raised;
-          if (r / NR == rg) l[r % NR] *= shrink;
-#pragma unroll
-          for (int e = 0; e < DB; e++) o[r][e] *= shrink;
-        }
+      for (int k = 0; k < KEYS; k++) {
+        x[k] *= mult;
+        if (!whole) x[k] = there && first + KEYS * part + k < hi ? x[k] : -INFINITY;
+        best = fmaxf(best, x[k]);
       }
-#pragma unroll
-      for (int r = 0; r < NR; r++) {
-        float unit = m[r];
-#pragma unroll
-        for (int k = 1; k < RG; k++) unit = rg == k ? m[k * NR + r] : unit;
-        float p[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) p[k] = __builtin_amdgcn_exp2f(x[r][k] - unit);
-        const uint2 w = make_uint2(H::pack(p[0], p[1]), H::pack(p[2], p[3]));
-        l[r] += H::sum(w.x) + H::sum(w.y);
-        *(uint2 *)(weights + (16 * (rg * NR + r) + cp) * PROW + 2 * (16 * kg + 4 * gp)) = w;
+      best = row_max<LANES>(best);
+      float factor = 1.f;
+      if (best - m > kTop) {
+        const float raised = best - kBias;
+        factor = __builtin_amdgcn_exp2f(m - raised);
+        m = raised;
+        l *= factor;
       }
+      uint32_t w[KEYS / 2];
+#pragma unroll
+      for (int k = 0; k < KEYS / 2; k++) {
+        w[k] = H::pack(__builtin_amdgcn_exp2f(x[2 * k] - m), __builtin_amdgcn_exp2f(x[2 * k + 1] - m));
+        l += H::sum(w[k]);
+      }
+      typedef uint32_t words __attribute__((ext_vector_type(2)));
+      if constexpr (KEYS == 4) *to_lds_at<words>(weight_to) = (words){w[0], w[1]};
+      else *to_lds_at<uint32_t>(weight_to) = w[0];
+      if (part == 0) *to_lds_at<float>(factors + 4 * mine) = factor;
+    };
+
+    if (n > 0) {
+      wait_tiles(loaded - 1);
       __syncthreads();
-      // a lane's four keys of the wave's first 16 dims: four blocks of 16 flip bits 5
-      // and 6, four keys on flip bit 4
-      const int lane_v = anew(lane), cv = lane_v & 15, gv = lane_v >> 4, row_v = 8 * gv + (cv >> 2);
-      const uint32_t values = tiles_at + at + row_v * ROW + 128 * (wave * DB >> 2) +
-                              16 * ((2 * (wave * DB & 3) + (cv >> 1 & 1)) ^ mix(row_v & 7)) + 8 * (cv & 1);
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        u32x4_v p[RT];
-#pragma unroll
-        for (int r = 0; r < RT; r++) p[r] = *(const u32x4_v *)(weights + (16 * r + cv) * PROW + 64 * j + 16 * gv);
-#pragma unroll
-        for (int e = 0; e < DB; e++) {
-          uint2 w[2];
-#pragma unroll
-          for (int z = 0; z < 2; z++)
-            w[z] = __builtin_bit_cast(uint2, read_column((values ^ (32 * (e & 3) + 16 * z)) + 128 * (e >> 2) + (32 * j + 4 * z) * ROW));
-          const u32x4_v v = {w[0].x, w[0].y, w[1].x, w[1].y};
-#pragma unroll
-          for (int r = 0; r < RT; r++) o[r][e] = H::mul32(v, p[r], o[r][e]);
-        }
-      }
-      if (i + 1 < n) wait_ring<LOADS * (RING - 2)>(i + RING <= n);
-      __syncthreads();
-      if (i + RING < n) {
-        const uint32_t bit = 1u << (i % RING);
-        known = load(i + RING) ? known | bit : known & ~bit;
+      products(std::false_type{}, std::true_type{}, 0);
+      for (int i = 0;;) {
+        __syncthreads();
+        if (loaded < n) load();  // where the tile before this one was
+        softmax(i);
+        const bool last = ++i == n;
+        if (!last) wait_tiles(loaded - 1 - i);
+        __syncthreads();
+        if (last) break;
+        products(std::true_type{}, std::true_type{}, i);
       }
     }
-    // the next unit's first tiles load while this one's outputs leave
+    // the next unit's first tiles load beside the last products
     const Unit done = u;
-    const int lane_o = anew(lane), co = lane_o & 15, go = lane_o >> 4;
+    const int last = n;
+    u = following, next = after;
     if (unit_at + 1 < unit1) {
-      u = read_unit(a, unit_at + 1);
+      // (not where the last tile is)
+      if (last > 0) products(std::true_type{}, std::false_type{}, last);
+      __syncthreads();
       begin();
+    } else if (last > 0) {
+      products(std::true_type{}, std::false_type{}, last);
     }
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-      const float sum = sum4(l[r]);
-      if (go == 0) sums[kg * R + 16 * (rg * NR + r) + co] = sum;
+    // rows' units and sums, by way of LDS
+    l = row_sum<LANES>(l);
+    if (part == 0) {
+      *to_lds_at<float>(scores + 4 * mine) = m;
+      *to_lds_at<float>(scores + 4 * (R + mine)) = l;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const int row = 16 * r + co, d = wave * (W / NW) + 4 * go;
-      const float *part = sums + row;
-      const float all = (part[0] + part[R]) + (part[2 * R] + part[3 * R]);
+      const int row = 16 * r + c, d = wave * (W / NW) + 4 * g;
+      const float unit = *from_lds<float>(scores + 4 * row), all = *from_lds<float>(scores + 4 * (R + row));
       if (row >= done.rows) continue;
       if (done.part < 0) {
         const float f = all == 0.f ? 0.f : 1.f / all;
@@ -543,13 +673,14 @@ __global__ __launch_bounds__(256 * RG, RG) void latent_attend_kernel(AbsorbedDev
 #pragma unroll
         for (int e = 0; e < DB; e++) store4<BF16>(dst + 16 * e, o[r][e] * f);
       } else {
-        const int64_t slot = (int64_t)done.part * a.unit_rows + row;
+        const int64_t slot = (int64_t)done.part * a.unit_rows + at_row + row;
 #pragma unroll
         for (int e = 0; e < DB; e++) *(f32x4_v *)(a.ws + slot * W + d + 16 * e) = o[r][e];
-        if (wave == 0 && go == 0)
-          *(float2 *)(a.ws + (int64_t)a.max_partials * a.unit_rows * W + 2 * slot) = make_float2(m[r], all);
+        if (wave == 0 && g == 0)
+          *(float2 *)(a.ws + (int64_t)a.max_partials * a.unit_rows * W + 2 * slot) = make_float2(unit, all);
       }
     }
+    __syncthreads();  // before the next unit's scores
   }
 }
 
@@ -788,7 +919,7 @@ int check_cache(const sq_latent_cache *c) {
   return 0;
 }
 
-std::atomic<uint64_t> g_raised[16];
+std::atomic<uint64_t> g_raised[20];
 
 // Raises a kernel's limit of dynamic LDS, once per kernel (each with an id of its own) and device.
 int dynamic_lds(const void *kernel, int id, size_t most, const char *what) {
@@ -806,18 +937,23 @@ int dynamic_lds(const void *kernel, int id, size_t most, const char *what) {
 
 template <int W, bool BF16>
 int launch_absorbed(const AbsorbedDev &d, const sq_kv_schedule &s, hipStream_t st) {
-  constexpr int id = 6 * (W == 512) + 3 * BF16;
-  const size_t lds = (W == 512 ? 2 : 3) * kTile * 2 * (W + kRope) + s.rows * (2 * kTile + 16 + 32);
-  constexpr size_t most = (W == 512 ? 2 : 3) * kTile * 2 * (W + kRope) + 64 * (2 * kTile + 16 + 32);
-  auto go = [&](auto kernel, int which, int threads) {
-    const int rc = dynamic_lds((const void *)kernel, id + which, most, "latent attend: LDS attribute");
+  constexpr int id = 8 * (W == 512) + 4 * BF16;
+  auto go = [&](auto kernel, int which, auto shape) {
+    typedef decltype(shape) S;
+    const int rc = dynamic_lds((const void *)kernel, id + which, S::lds, "latent attend: LDS attribute");
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)s.max_workers), dim3(threads), lds, st, d);
+    const unsigned grid = S::PAIR ? ((unsigned)s.max_workers + 7) / 8 * 16 : (unsigned)s.max_workers;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::threads), S::lds, st, d);
     return sq_internal_launched("latent_attend_kernel");
   };
-  const int rc = s.rows == 16 ? go(latent_attend_kernel<W, 1, 1, BF16>, 0, 256)
-                 : s.rows == 32 ? go(latent_attend_kernel<W, 2, 1, BF16>, 1, 512)
-                                : go(latent_attend_kernel<W, 2, 2, BF16>, 2, 512);
+  typedef Absorbed<W, 1, 1, 4> S16;
+  typedef Absorbed<W, 2, 1, 4> S32;
+  typedef Absorbed<W, 2, 2, W == 512 ? 3 : 4> S64;
+  typedef Absorbed<W, 2, 2, W == 512 ? 3 : 4, true> S128;
+  const int rc = s.rows == 16   ? go(latent_attend_kernel<S16, BF16>, 0, S16{})
+                 : s.rows == 32 ? go(latent_attend_kernel<S32, BF16>, 1, S32{})
+                 : s.rows == 64 ? go(latent_attend_kernel<S64, BF16>, 2, S64{})
+                                : go(latent_attend_kernel<S128, BF16>, 3, S128{});
   if (rc) return rc;
   hipLaunchKernelGGL((latent_merge_kernel<W, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
   return sq_internal_launched("latent_merge_kernel");
@@ -826,7 +962,7 @@ int launch_absorbed(const AbsorbedDev &d, const sq_kv_schedule &s, hipStream_t s
 template <int D, bool BF16>
 int launch_expanded(const ExpandedDev &d, hipStream_t st) {
   constexpr size_t lds = 2 * 64 * 2 * (2 * D + kRope);
-  const int rc = dynamic_lds((const void *)expanded_attend_kernel<D, BF16>, 12 + 2 * (D == 128) + BF16, lds, "expanded attention: LDS attribute");
+  const int rc = dynamic_lds((const void *)expanded_attend_kernel<D, BF16>, 16 + 2 * (D == 128) + BF16, lds, "expanded attention: LDS attribute");
   if (rc) return rc;
   hipLaunchKernelGGL((expanded_attend_kernel<D, BF16>), dim3((unsigned)d.max_workers * d.heads), dim3(512), lds, st, d);
   return sq_internal_launched("expanded_attend_kernel");
@@ -906,7 +1042,7 @@ int sq_latent_attend(const sq_latent_cache *c, const sq_latent_attend_args *a, v
   const sq_kv_schedule &s = a->schedule;
   rc = sq_internal_check_schedule(&s, a->tokens, 1);
   if (rc) return rc;
-  if (s.kv_heads != 1 || s.window || s.few_work || (s.rows != 16 && s.rows != 32 && s.rows != 64))
+  if (s.kv_heads != 1 || s.window || s.few_work || (s.rows != 16 && s.rows != 32 && s.rows != 64 && s.rows != 128))
     return fail(SQ_ESHAPE, "latent attend: the schedule is for another kind of attention");
   if (!a->workspace || ((uintptr_t)a->workspace & 15)) return fail(SQ_EINVAL, "latent attend: null or misaligned workspace");
   const AbsorbedDev d = {*c, (const uint16_t *)a->q, (const uint16_t *)a->q_rope, (uint16_t *)a->out, a->workspace, a->table,

@@ -298,8 +298,9 @@ class BlockTables:
                 continue
             if form == "absorbed":
                 rows = max_new * n
-                rows = 16 if rows <= 16 else 32 if rows <= 32 else 64
-                add(form, 0, n, 1, rows, self._cus, self.latent_min_tiles, self.latent_cut_tiles)
+                rows = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
+                # (one workgroup on a CU; sets of 128 have two)
+                add(form, 0, n, 1, rows, self._cus // (2 if rows == 128 else 1), self.latent_min_tiles, self.latent_cut_tiles)
             else:
                 add(form, 0, n, n, 256, self._cus, 1, 1 << 28)
         offsets = [4 * sum(sizes[:i]) for i in range(7)]
