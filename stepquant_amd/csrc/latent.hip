@@ -235,11 +235,25 @@ __global__ __launch_bounds__(256) void latent_gather_kernel(sq_latent_cache c, s
 
 // ------------------------------------------------------------ tiles in LDS
 //
-// Rows of 16-byte groups lie one after the other, each row's groups of eight
-// exchanged by an exclusive or with `mix` of the row: 16 bytes of one group of 8
-// consecutive rows, and 32 of 4 consecutive rows (the transposing load of the
-// values), then fall on all banks.  The load that goes from memory to LDS puts
-// 64 lanes' groups side by side, so a lane asks for the group whose place it has.
+// LDS has 64 banks, 256 bytes.  A wave reads 16 bytes a lane in four cycles, of the
+// lanes 0-3, 12-15, 20-23 and 24-27, of 4-11, 16-19 and 28-31, and of the same 32 on;
+// the transposing load of 8 bytes a lane takes lanes 0-31 and 32-63.  (Taken from the
+// counters of conflicts of single reads.)  Rows of 16-byte groups lie one after
+// the other, and a row's groups are exchanged by an exclusive or, so that neither kind of
+// read meets a bank twice: 16 rows at four adjacent groups as lanes 16 g + row,
+// and 32 bytes of the rows 0-3 and 8-11, or 4-7 and 12-15.  The load from memory
+// to LDS puts 64 lanes' groups side by side, so a lane asks for the group whose place it has.
+
+// Cached tiles: rows are an odd number of 128 bytes long, the last 128 of them the rope key.
+template <int W>
+__device__ __forceinline__ int place_of(int row, int at) {
+  return at ^ (row & 3) << 1 ^ (at < W / 8 ? ((row >> 3 ^ row) & 1) << 3 : 0);
+}
+
+// rows of 32 scores (128 bytes) and of 32 weights (64)
+__device__ __forceinline__ int score_place(int row, int at) { return at ^ (row & 2) ^ (row >> 1 & 4); }
+__device__ __forceinline__ int weight_place(int row, int at) { return at ^ (row >> 2 & 2); }
+
 __device__ __forceinline__ int mix(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
 
 // 16 bytes a lane from memory to LDS at `lds` + 16 lane.  The compiler does not
@@ -357,29 +371,27 @@ __device__ __forceinline__ Unit read_unit(const AbsorbedDev &a, int i, int at_ro
   return x;
 }
 
-// A workgroup has RG groups of four waves and units of up to 16 RG NR rows; tiles of
-// 32 keys pass through a ring in LDS.  A tile goes through two steps, with a
-// barrier behind each:
+// Tiles of 32 keys pass through a ring in LDS, for one or two groups of four waves
+// with up to 16 NR rows each.  A group takes a tile through two steps:
 //
-//   products  outputs with the tile before, every wave for its own share of the
-//             dims and all rows (so outputs need no joining); then scores with this
-//             tile, every wave for 16 keys, the group's rows and half of the dims,
-//             which go to LDS as sums in 32 bits;
+//   products  outputs with the tile before, every wave for a quarter of the dims
+//             (so outputs need no joining); then scores with this tile, every
+//             wave for 16 keys and half of the dims, as sums in 32 bits;
 //   softmax   by rows: 8 or 16 lanes have a row's 32 scores, and alone know its
 //             unit and its sum; rounded weights and what the row's outputs are
 //             to be multiplied by go to LDS.
 //
-// So keys are read from LDS once for each group and values once, and a wave holds half of
-// its rows' queries.  PAIR: units of 128 rows have two workgroups, which run side by side
-// on one XCD (8 apart, blocks go to the 8 in turn) so that its L2 gives one of
-// them the keys; others are read past the caches' later use.
-template <int W_, int RG_, int NR_, int RING_, bool PAIR_ = false>
+// Two groups run a step apart, so that one's products have the matrix cores while
+// the other waits for scores and exponentials; a barrier ends each step.  The
+// late group loads.  PAIR: units of 128 rows have two workgroups, which run
+// side by side on one XCD (8 apart, blocks go to the 8 in turn) so that its L2 gives one
+// of them the keys; others are read past the caches' later use.
+template <int W_, int RG_, int NR_, bool PAIR_ = false>
 struct Absorbed {
-  static constexpr int W = W_, TK = 32, RG = RG_, NR = NR_, RING = RING_, NW = 4 * RG, threads = 64 * NW;
-  static constexpr bool PAIR = PAIR_;
-  static constexpr int R = 16 * RG * NR, TILE = TK * 2 * (W + kRope);
-  static constexpr int SROW = 4 * TK + 16, PROW = 2 * TK + 16;  // bytes from row to row of scores and weights
-  static constexpr size_t lds = RING * TILE + R * (2 * SROW + PROW + 4);
+  static constexpr int W = W_, TK = 32, RG = RG_, NR = NR_, NW = 4 * RG, threads = 64 * NW, RING = W == 512 ? 4 : 6;
+  static constexpr bool PAIR = PAIR_, HALVES = NR == 1;  // two waves share 16 rows' scores: half of the dims each
+  static constexpr int R = 16 * RG * NR, TILE = TK * 2 * (W + kRope), SROW = 4 * TK, PROW = 2 * TK;
+  static constexpr size_t lds = RING * TILE + R * ((HALVES ? 2 : 1) * SROW + PROW + 4);
   static_assert(lds <= 163840, "LDS of a CU");
 };
 
@@ -387,13 +399,14 @@ template <typename S, bool BF16>
 __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(AbsorbedDev a) {
   typedef Half<BF16> H;
   constexpr int W = S::W, TK = S::TK, RG = S::RG, NR = S::NR, NW = S::NW, RING = S::RING, TILE = S::TILE, R = S::R;
-  constexpr int KD = W + kRope, ROW = 2 * KD, KS = KD / 64, DB = W / NW / 16, RT = RG * NR;
+  constexpr int KD = W + kRope, ROW = 2 * KD, KS = KD / (S::HALVES ? 64 : 32), DB = W / 64;
   constexpr int SROW = S::SROW, PROW = S::PROW;
-  constexpr int BLOCKS = TILE / 1024, MOST = (BLOCKS + NW - 1) / NW;  // loads of a tile, of a wave
-  constexpr int LANES = 64 * NW / R, KEYS = TK / LANES;               // of a row's softmax, and of a lane
+  constexpr int LOADS = TILE / 4096;                           // of a tile, of a wave of the group that loads
+  constexpr int LANES = 256 / (16 * NR), KEYS = TK / LANES;    // of a row's softmax, and of a lane
   extern __shared__ __attribute__((aligned(128))) uint8_t smem[];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int kg = wave & 1, dh = wave >> 1 & 1, rg = wave >> 2;
+  const int rg = wave >> 2, share = wave & 3, kg = wave & 1, half = wave >> 1 & 1;
+  const bool late = RG == 2 && rg == 1, loads = rg == RG - 1;
   const int worker = S::PAIR ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x;
   const int at_row = S::PAIR ? R * (blockIdx.x >> 3 & 1) : 0;
   if (worker >= a.max_workers) return;
@@ -401,29 +414,35 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   if (unit0 >= unit1) return;
   const int G = a.heads, P = a.c.page_tokens;
   const uint32_t tiles_at = lds_address(smem);
-  const uint32_t scores = tiles_at + RING * TILE;     // [2][R] rows of TK
-  const uint32_t weights = scores + 2 * R * SROW;     // [R] rows of TK
-  const uint32_t factors = weights + R * PROW;        // [R]
-  // Where a lane's operands lie.  Its key and first dims in a tile: other steps of
-  // 32 dims flip bit 6, or lie 128 bytes on.  Its four keys of the wave's first 16
-  // dims: four blocks of 16 flip bits 5 and 6, four keys on flip bit 4.
+  const uint32_t scores = tiles_at + RING * TILE;  // [HALVES ? 2 : 1][R] rows of TK
+  const uint32_t weights = scores + (S::HALVES ? 2 : 1) * R * SROW;  // [R] rows of TK
+  const uint32_t factors = weights + R * PROW;     // [R]
+  // Where a lane's operands lie: its key's steps of 32 dims (four of them 256 bytes;
+  // the last two may be the rope key's), and its four keys of the wave's 16 dims of
+  // every 64 (two of them 256 bytes, and four keys on a constant way).
   const int c = lane & 15, g = lane >> 4, token = 8 * g + (c >> 2);
-  static_assert(KS % 2 == 1, "the second half of the dims begins with an odd step");
-  const uint32_t key_at = tiles_at + (16 * kg + c) * ROW + 16 * (g ^ mix(c & 7)) + 64 * (KS - 1) * dh;
-  const uint32_t even_at = key_at ^ 64 * dh, odd_at = (key_at ^ 64 * (1 - dh)) + 128 * dh;
-  const uint32_t value_at = tiles_at + token * ROW + 128 * (wave * DB >> 2) +
-                            16 * ((2 * (wave * DB & 3) + (c >> 1 & 1)) ^ mix(token & 7)) + 8 * (c & 1);
-  const uint32_t score_to = scores + (dh * R + 16 * rg * NR + c) * SROW + 64 * kg + 16 * g;
-  const uint32_t weight_at = weights + c * PROW + 16 * g, factor_at = factors + 4 * c;
-  const int mine = tid / LANES, part = tid % LANES;   // the lane's row of the softmax, and its keys there
-  const uint32_t score_at = scores + mine * SROW + 4 * KEYS * part, weight_to = weights + mine * PROW + 2 * KEYS * part;
-  uint32_t from[MOST];  // the groups of a tile that a lane loads
+  const int step0 = S::HALVES ? KS * half : 0;
+  auto key_step = [&](int k) {
+    const int row = 16 * kg + c;
+    return tiles_at + row * ROW + 16 * place_of<W>(row, 4 * (step0 + k) + g);
+  };
+  const uint32_t key_at[4] = {key_step(0), key_step(1), key_step(2), key_step(3)};
+  const uint32_t last_at[2] = {key_step(KS - 2), key_step(KS - 1)};
+  auto four_keys = [&](int e) { return tiles_at + token * ROW + 16 * place_of<W>(token, 8 * e + 2 * share + (c >> 1 & 1)) + 8 * (c & 1); };
+  const uint32_t value_at[2] = {four_keys(0), four_keys(1)};
+  uint32_t from[LOADS];  // the groups of a tile's eight rows that a lane loads
 #pragma unroll
-  for (int k = 0; k < MOST; k++) {
-    const int n = min(64 * NW * k + tid, TILE / 16 - 1), row = n / (KD / 8), at = n - row * (KD / 8);
-    from[k] = row * ROW + 16 * ((at & ~7) | ((at & 7) ^ mix(row & 7)));
+  for (int k = 0; k < LOADS; k++) {
+    const int n = 64 * k + lane, row = n / (KD / 8), at = n - row * (KD / 8);
+    from[k] = (row + 8 * share) * ROW + 16 * place_of<W>(row + 8 * share, at);
   }
-  const bool more = wave < BLOCKS % NW;  // the wave has MOST loads of a tile, else one fewer
+  const int row0 = 16 * NR * rg, q_row = row0 + (S::HALVES ? 0 : 16 * half) + c;  // of the group; of the lane's scores
+  const uint32_t score_to = scores + ((S::HALVES ? R * half : 0) + q_row) * SROW + 16 * score_place(c, 4 * kg + g);
+  const uint32_t weight_at = weights + (row0 + c) * PROW + 16 * weight_place(c, g), factor_at = factors + 4 * (row0 + c);
+  // the lane's row of the softmax, and its keys there
+  const int mine = row0 + (tid & 255) / LANES, part = tid % LANES;
+  const uint32_t score_at = scores + mine * SROW + 16 * score_place(mine, KEYS * part / 4) + 4 * (KEYS * part % 4);
+  const uint32_t weight_to = weights + mine * PROW + 16 * weight_place(mine, KEYS * part / 8) + 2 * (KEYS * part % 8);
 
   // the tile that is loaded next: its page, the tokens before it there
   struct Place {
@@ -443,33 +462,35 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   Unit u = read_unit(a, unit0, at_row, R);
   Place next = place(u);
   int n = 0, loaded = 0;  // tiles of the unit, and how many of them are on their way
-  uint32_t known = 0;     // bit i % RING: tile i has a page
+  uint32_t known = 0;     // bit i % 32: tile i has a page
+  uint32_t load_slot = 0; // where the next tile goes
+  auto after_slot = [&](uint32_t slot) { return slot + TILE == RING * TILE ? 0u : slot + TILE; };
   auto load = [&]() {
     const int i = loaded++;
     const bool there = next.page > 0 && next.page < a.c.num_pages;
-    const uint8_t *base = (const uint8_t *)a.c.data + ((there ? (int64_t)next.page * P : 0) + next.in_page) * ROW;
-    const uint32_t bit = 1u << (i % RING), to = tiles_at + i % RING * TILE + 1024 * wave;
-    known = there ? known | bit : known & ~bit;
+    known = known & ~(1u << (i & 31)) | (uint32_t)there << (i & 31);
+    if (loads) {
+      const uint8_t *base = (const uint8_t *)a.c.data + ((there ? (int64_t)next.page * P : 0) + next.in_page) * ROW;
+      const uint32_t to = tiles_at + load_slot + TILE / 4 * share;
 #pragma unroll
-    for (int k = 0; k < MOST; k++) {
-      if (k == MOST - 1 && BLOCKS % NW && !more) break;
-      if constexpr (S::PAIR) to_lds(to + 1024 * NW * k, base, from[k]);
-      else to_lds_once(to + 1024 * NW * k, base, from[k]);
+      for (int k = 0; k < LOADS; k++) {
+        if constexpr (S::PAIR) to_lds(to + 1024 * k, base, from[k]);
+        else to_lds_once(to + 1024 * k, base, from[k]);
+      }
     }
+    load_slot = after_slot(load_slot);
     next.in_page += TK;
     if (next.in_page == P && i + 1 < n) next.in_page = 0, next.page = uniform_word(++next.entry);
   };
-  // until at most `tiles` of the tiles on their way are not there
-  auto wait_tiles = [&](int tiles) {
-    if (tiles >= RING - 2) {
-      if (BLOCKS % NW == 0 || more) wait_loads<(RING - 2) * MOST>();
-      else wait_loads<(RING - 2) * (MOST - 1)>();
-    } else {
-      wait_loads<0>();
-    }
+  // until tile i is there, with MOST tiles behind it on their way as a rule
+  auto wait_tile = [&](auto MOST, int i) {
+    constexpr int most = decltype(MOST)::value;
+    if (!loads) return;
+    if (loaded - 1 - i >= most) wait_loads<most * LOADS>();
+    else wait_loads<0>();
   };
   auto begin = [&]() {
-    n = next.n, loaded = 0;
+    n = next.n, loaded = 0, load_slot = 0;
 #pragma unroll
     for (int i = 0; i < RING - 1; i++)
       if (i < n) load();
@@ -478,72 +499,61 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
     const Unit following = read_unit(a, min(unit_at + 1, unit1 - 1), at_row, R);
     const Place after = place(following);
-    u32x4_v q[NR][KS];
-    f32x4_v o[RT][DB];
+    u32x4_v q[KS];
+    f32x4_v o[NR][DB];
     {
+      const int fresh = anew(lane), row = q_row - c + (fresh & 15), f = u.f0 + row;
+      const bool live = row < u.rows;
+      const int t = live ? f / G : 0, head = live ? f - t * G : 0, d0 = 32 * step0 + 8 * (fresh >> 4);
+      const uint16_t *src = a.q + (u.q0 + t) * a.q_stride + head * a.q_head_stride;
+      const uint16_t *rope = a.rope + (u.q0 + t) * a.rope_stride + head * a.rope_head_stride;
 #pragma unroll
-      for (int r = 0; r < NR; r++) {
-        const int row = 16 * (rg * NR + r) + c, f = u.f0 + row;
-        const bool live = row < u.rows;
-        const int t = live ? f / G : 0, head = live ? f - t * G : 0;
-        const uint16_t *src = a.q + (u.q0 + t) * a.q_stride + head * a.q_head_stride + 8 * g;
-        const uint16_t *rope = a.rope + (u.q0 + t) * a.rope_stride + head * a.rope_head_stride + 8 * g;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-          const int d = 32 * (KS * dh + s);
-          q[r][s] = live ? *(const u32x4_v *)(d < W ? src + d : rope + d - W) : (u32x4_v){0, 0, 0, 0};
-        }
+      for (int s = 0; s < KS; s++) {
+        const int d = d0 + 32 * s;
+        q[s] = live ? *(const u32x4_v *)(32 * (step0 + s) < W ? src + d : rope + d - W) : (u32x4_v){0, 0, 0, 0};
       }
     }
 #pragma unroll
-    for (int r = 0; r < RT; r++)
+    for (int r = 0; r < NR; r++)
 #pragma unroll
       for (int e = 0; e < DB; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
     // (the queries' loads are waited for here, not by a wait for all loads in the loop)
 #pragma unroll
-    for (int r = 0; r < NR; r++)
-#pragma unroll
-      for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[r][s]));
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     const float mult = a.scale * kLog2e;
-    // the keys that the lane's row sees
+    // the keys that the lane's row sees, and those that every row of the unit sees
     const int hi = mine >= u.rows ? 0 : a.causal ? min(u.kv1, u.pos0 + (u.f0 + mine) / G + 1) : u.kv1;
-    // keys that every row of the unit sees
     const int all_hi = u.rows <= 0 ? 0 : a.causal ? min(u.kv1, u.pos0 + u.f0 / G + 1) : u.kv1;
     float m = kNone, l = 0.f;
+    auto whole = [&](int i) { return (known >> (i & 31) & 1) && u.kv0 + TK * (i + 1) <= all_hi; };
 
-    // Outputs with tile i - 1 (OUT) and scores with tile i (IN), their products in turn;
+    // Outputs with the tile at `values` (OUT) and scores with the one at `keys` (IN), their products in turn;
     // operands are read some products ahead.
-    auto products = [&](auto OUT, auto IN, int i) {
+    auto products = [&](auto OUT, auto IN, uint32_t values, uint32_t keys) {
       constexpr int NO = decltype(OUT)::value ? DB : 0, NI = decltype(IN)::value ? KS : 0, N = NO + NI;
-      constexpr int AHEAD_K = NI < 3 ? NI : 3, AHEAD_V = NO < 2 ? NO : 2;
-      const uint32_t even_keys = even_at + i % RING * TILE, odd_keys = odd_at + i % RING * TILE;
-      const uint32_t values = value_at + (i + RING - 1) % RING * TILE;
-      u32x4_v p[RT], kw[AHEAD_K + 1], vw[AHEAD_V + 1];
-      f32x4_v s[NR];
-#pragma unroll
-      for (int r = 0; r < NR; r++) s[r] = (f32x4_v){0, 0, 0, 0};
-      auto read_key = [&](int k) {
-        return *from_lds<u32x4_v>((k & 1 ? odd_keys : even_keys) + 128 * (k >> 1));
-      };
+      constexpr int AHEAD_K = NI < 4 ? NI : 4, AHEAD_V = NO < 2 ? NO : 2;
+      u32x4_v p[NR], kw[AHEAD_K + 1], vw[AHEAD_V + 1];
+      f32x4_v s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      auto read_key = [&](int k) { return *from_lds<u32x4_v>(k < KS - 2 ? key_at[k & 3] + keys + 256 * (k >> 2) : last_at[k - KS + 2] + keys); };
       auto read_value = [&](int e) {
         uint2 w[2];
 #pragma unroll
         for (int z = 0; z < 2; z++)
-          w[z] = __builtin_bit_cast(uint2, read_column((values ^ (32 * (e & 3) + 16 * z)) + 128 * (e >> 2) + 4 * z * ROW));
+          w[z] = __builtin_bit_cast(uint2, read_column(value_at[e & 1] + values + 256 * (e >> 1) + 4 * z * ROW));
         return (u32x4_v){w[0].x, w[0].y, w[1].x, w[1].y};
       };
       if constexpr (NO > 0) {
-        float f[RT];
+        float f[NR];
         bool raised = false;
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
+        for (int r = 0; r < NR; r++) {
           f[r] = *from_lds<float>(factor_at + 64 * r);
           p[r] = *from_lds<u32x4_v>(weight_at + 16 * r * PROW);
           raised |= f[r] != 1.f;
         }
         if (__any(raised)) {
 #pragma unroll
-          for (int r = 0; r < RT; r++)
+          for (int r = 0; r < NR; r++)
 #pragma unroll
             for (int e = 0; e < DB; e++) o[r][e] *= f[r];
         }
@@ -558,12 +568,11 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
         if (NO && (j + 1) * NO / N > e) {
           if (e + AHEAD_V < NO) vw[(e + AHEAD_V) % (AHEAD_V + 1)] = read_value(e + AHEAD_V);
 #pragma unroll
-          for (int r = 0; r < RT; r++) o[r][e] = H::mul32(vw[e % (AHEAD_V + 1)], p[r], o[r][e]);
+          for (int r = 0; r < NR; r++) o[r][e] = H::mul32(vw[e % (AHEAD_V + 1)], p[r], o[r][e]);
         } else {
           const int k = j - e;
           if (k + AHEAD_K < NI) kw[(k + AHEAD_K) % (AHEAD_K + 1)] = read_key(k + AHEAD_K);
-#pragma unroll
-          for (int r = 0; r < NR; r++) s[r] = H::mul32(kw[k % (AHEAD_K + 1)], q[r][k], s[r]);
+          s[k & 1] = H::mul32(kw[k % (AHEAD_K + 1)], q[k], s[k & 1]);
         }
       }
       __builtin_amdgcn_sched_group_barrier(0x100, AHEAD_K + 2 * AHEAD_V, 0);  // LDS reads
@@ -572,42 +581,40 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
         const int e = NO ? j * NO / N : 0;
         if (NO && (j + 1) * NO / N > e) {
           if (e + AHEAD_V < NO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-          __builtin_amdgcn_sched_group_barrier(0x8, RT, 0);  // products
+          __builtin_amdgcn_sched_group_barrier(0x8, NR, 0);  // products
         } else {
           if (j - e + AHEAD_K < NI) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x8, NR, 0);
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         }
       }
-      if constexpr (NI > 0) {
+      if constexpr (NI > 0) *to_lds_at<f32x4_v>(score_to) = s[0] + s[1];
+    };
+    // What some row does not see has a weight of 0 there; infinities and NaN would
+    // still reach its outputs.  (Rows that see them have them in their scores.)
+    auto clean = [&](int i, uint32_t slot) {
+      const int first = u.kv0 + TK * i, r0 = known >> (i & 31) & 1 ? max(0, min(TK, all_hi - first)) : 0;
+      for (int j = r0 * (KD / 8) + (tid & 255); j < TK * (KD / 8); j += 256) {
+        const uint32_t at = tiles_at + slot + 16 * j;
+        u32x4_v w = *from_lds<u32x4_v>(at);
 #pragma unroll
-        for (int r = 0; r < NR; r++)
-          *to_lds_at<f32x4_v>(score_to + 16 * r * SROW) = s[r];
+        for (int k = 0; k < 4; k++) w[k] = only_finite<BF16>(w[k]);
+        *to_lds_at<u32x4_v>(at) = w;
       }
     };
-    auto softmax = [&](int i) {
+    auto softmax = [&](int i, bool all) {
       const int first = u.kv0 + TK * i;
-      const bool there = known >> (i % RING) & 1, whole = there && first + TK <= all_hi;
       typedef float vec __attribute__((ext_vector_type(KEYS)));
-      vec x = *from_lds<vec>(score_at) + *from_lds<vec>(score_at + R * SROW);
-      if (!whole) {
-        // What some row does not see has a weight of 0 there; infinities and NaN
-        // would still reach its outputs.  (Rows that see them have them in their scores.)
-        const int r0 = there ? max(0, min(TK, all_hi - first)) : 0;
-        for (int j = r0 * (KD / 8) + tid; j < TK * (KD / 8); j += 64 * NW) {
-          u32x4_v *p = (u32x4_v *)(smem + i % RING * TILE + 16 * j);
-          u32x4_v w = *p;
+      vec x = *from_lds<vec>(score_at);
+      if constexpr (S::HALVES) x += *from_lds<vec>(score_at + R * SROW);
+      x *= mult;
+      if (!all) {
+        const int seen = known >> (i & 31) & 1 ? hi - first - KEYS * part : 0;
 #pragma unroll
-          for (int k = 0; k < 4; k++) w[k] = only_finite<BF16>(w[k]);
-          *p = w;
-        }
+        for (int k = 0; k < KEYS; k++) x[k] = k < seen ? x[k] : -INFINITY;
       }
-      float best = -INFINITY;
+      float best = x[0];
 #pragma unroll
-      for (int k = 0; k < KEYS; k++) {
-        x[k] *= mult;
-        if (!whole) x[k] = there && first + KEYS * part + k < hi ? x[k] : -INFINITY;
-        best = fmaxf(best, x[k]);
-      }
+      for (int k = 1; k < KEYS; k++) best = fmaxf(best, x[k]);
       best = row_max<LANES>(best);
       float factor = 1.f;
       if (best - m > kTop) {
@@ -628,59 +635,75 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
       if (part == 0) *to_lds_at<float>(factors + 4 * mine) = factor;
     };
 
+    uint32_t slot = 0;  // of tile i
     if (n > 0) {
-      wait_tiles(loaded - 1);
+      typedef std::integral_constant<int, RING - 2> Issued;          // tiles behind the one that is waited for
+      typedef std::integral_constant<int, RING - 1 - RG> Issued_late;  // (the late group has not loaded in this step)
+      wait_tile(Issued{}, 0);
       __syncthreads();
-      products(std::false_type{}, std::true_type{}, 0);
-      for (int i = 0;;) {
+      // a step apart
+      if (late) {
+        wait_tile(Issued{}, 0);
         __syncthreads();
+      }
+      products(std::false_type{}, std::true_type{}, 0, 0);
+      for (int i = 0;; i++) {
+        if (late && i + 1 < n) wait_tile(Issued_late{}, i + 1);
+        __syncthreads();
+        const bool all = whole(i);
+        if (late && !all) {
+          clean(i, slot);
+          __syncthreads();
+        }
         if (loaded < n) load();  // where the tile before this one was
-        softmax(i);
-        const bool last = ++i == n;
-        if (!last) wait_tiles(loaded - 1 - i);
+        softmax(i, all);
+        if (RG == 1) {
+          if (!all) clean(i, slot);
+          if (i + 1 < n) wait_tile(Issued{}, i + 1);
+        }
         __syncthreads();
-        if (last) break;
-        products(std::true_type{}, std::true_type{}, i);
+        if (RG == 2 && !late && !all) __syncthreads();  // the other group cleans the tile
+        if (i + 1 == n) break;
+        const uint32_t following_slot = after_slot(slot);
+        products(std::true_type{}, std::true_type{}, slot, following_slot);
+        slot = following_slot;
       }
     }
-    // the next unit's first tiles load beside the last products
+    // the next unit's first tiles load while this one's outputs leave
     const Unit done = u;
     const int last = n;
+    if (last > 0) products(std::true_type{}, std::false_type{}, slot, 0);
+    if (RG == 2 && !late && last > 0) __syncthreads();
+    __syncthreads();
     u = following, next = after;
-    if (unit_at + 1 < unit1) {
-      // (not where the last tile is)
-      if (last > 0) products(std::true_type{}, std::false_type{}, last);
-      __syncthreads();
-      begin();
-    } else if (last > 0) {
-      products(std::true_type{}, std::false_type{}, last);
-    }
+    if (unit_at + 1 < unit1) begin();
     // rows' units and sums, by way of LDS
     l = row_sum<LANES>(l);
     if (part == 0) {
-      *to_lds_at<float>(scores + 4 * mine) = m;
-      *to_lds_at<float>(scores + 4 * (R + mine)) = l;
+      *to_lds_at<float>(weights + 4 * mine) = m;
+      *to_lds_at<float>(weights + 4 * (R + mine)) = l;
     }
     __syncthreads();
+    const int fresh_o = anew(lane), go = fresh_o >> 4;
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-      const int row = 16 * r + c, d = wave * (W / NW) + 4 * g;
-      const float unit = *from_lds<float>(scores + 4 * row), all = *from_lds<float>(scores + 4 * (R + row));
+    for (int r = 0; r < NR; r++) {
+      const int row = row0 + 16 * r + (fresh_o & 15), d = 16 * share + 4 * go;
+      const float unit = *from_lds<float>(weights + 4 * row), all = *from_lds<float>(weights + 4 * (R + row));
       if (row >= done.rows) continue;
       if (done.part < 0) {
         const float f = all == 0.f ? 0.f : 1.f / all;
         uint16_t *dst = a.out + (done.q0 * (int64_t)G + done.f0 + row) * W + d;
 #pragma unroll
-        for (int e = 0; e < DB; e++) store4<BF16>(dst + 16 * e, o[r][e] * f);
+        for (int e = 0; e < DB; e++) store4<BF16>(dst + 64 * e, o[r][e] * f);
       } else {
         const int64_t slot = (int64_t)done.part * a.unit_rows + at_row + row;
 #pragma unroll
-        for (int e = 0; e < DB; e++) *(f32x4_v *)(a.ws + slot * W + d + 16 * e) = o[r][e];
-        if (wave == 0 && g == 0)
+        for (int e = 0; e < DB; e++) *(f32x4_v *)(a.ws + slot * W + d + 64 * e) = o[r][e];
+        if (share == 0 && go == 0)
           *(float2 *)(a.ws + (int64_t)a.max_partials * a.unit_rows * W + 2 * slot) = make_float2(unit, all);
       }
     }
-    __syncthreads();  // before the next unit's scores
+    __syncthreads();  // before the next unit's weights
   }
 }
 
@@ -946,10 +969,10 @@ int launch_absorbed(const AbsorbedDev &d, const sq_kv_schedule &s, hipStream_t s
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::threads), S::lds, st, d);
     return sq_internal_launched("latent_attend_kernel");
   };
-  typedef Absorbed<W, 1, 1, 4> S16;
-  typedef Absorbed<W, 2, 1, 4> S32;
-  typedef Absorbed<W, 2, 2, W == 512 ? 3 : 4> S64;
-  typedef Absorbed<W, 2, 2, W == 512 ? 3 : 4, true> S128;
+  typedef Absorbed<W, 1, 1> S16;
+  typedef Absorbed<W, 2, 1> S32;
+  typedef Absorbed<W, 2, 2> S64;
+  typedef Absorbed<W, 2, 2, true> S128;
   const int rc = s.rows == 16   ? go(latent_attend_kernel<S16, BF16>, 0, S16{})
                  : s.rows == 32 ? go(latent_attend_kernel<S32, BF16>, 1, S32{})
                  : s.rows == 64 ? go(latent_attend_kernel<S64, BF16>, 2, S64{})
