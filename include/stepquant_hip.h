@@ -718,11 +718,12 @@ int sq_latent_attend(const sq_latent_cache *cache, const sq_latent_attend_args *
  * over the keys of token t's request up to its own (causal) or all of them.
  *   q          [tokens, heads, dim + 64]; k, v [rows, heads, dim]; rope
  *              [rows, 64]; one type, SQ_BF16 or SQ_F16, strides multiples of 8,
- *              16-byte aligned; out [tokens, heads, dim] contiguous; dim 64 or 128
+ *              16-byte aligned (rows of keys and values below 2^24); out [tokens, heads, dim] contiguous; dim 64 or 128
  *   cu         [batch + 1] the plan's first packed rows of queries
  *   starts     [batch + 1] the requests' first rows of keys; request b has
  *              starts[b + 1] - starts[b], at least what its tokens see (rows that
  *              are not there are not seen)
+ *   workspace  max_partials * heads * 256 * (dim + 2) floats, 16-byte aligned
  *   schedule   of as many KV heads as query heads, rows 256, no window
  */
 typedef struct sq_expanded_attend_args {
@@ -731,6 +732,7 @@ typedef struct sq_expanded_attend_args {
     const void *v;
     const void *rope;
     void *out;
+    float *workspace;
     const int32_t *cu;
     const int32_t *starts;
     int64_t tokens;

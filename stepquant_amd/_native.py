@@ -153,7 +153,7 @@ class LatentAttend(ctypes.Structure):
 
 
 class ExpandedAttend(ctypes.Structure):
-    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("rope", _P), ("out", _P), ("cu", _P), ("starts", _P),
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("rope", _P), ("out", _P), ("workspace", _P), ("cu", _P), ("starts", _P),
                 ("tokens", ctypes.c_int64), ("rows", ctypes.c_int64), ("q_stride", ctypes.c_int64),
                 ("q_head_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
                 ("v_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("rope_stride", ctypes.c_int64),
@@ -293,7 +293,7 @@ ROTARY_ROWS = struct.Struct("=3Q5q4i")
 LATENT_APPEND = struct.Struct("=4Q3q")
 LATENT_GATHER = struct.Struct("=6Q2q4i")
 LATENT_ATTEND = struct.Struct(f"=5Q6qif{KV_SCHEDULE.size}s")
-EXPANDED_ATTEND = struct.Struct(f"=7Q9q3if{KV_SCHEDULE.size}s")
+EXPANDED_ATTEND = struct.Struct(f"=8Q9q3if{KV_SCHEDULE.size}s")
 _I32, _I64 = ctypes.c_int32, ctypes.c_int64
 _KV_ENTRIES = {"sq_kv_plan": [_P, ctypes.c_char_p, _P], "sq_kv_commit": [_P, ctypes.c_char_p, _P],
                "sq_kv_append": [_P, ctypes.c_char_p, _P], "sq_kv_attend": [_P, ctypes.c_char_p, _P],

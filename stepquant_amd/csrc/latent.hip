@@ -13,6 +13,9 @@
 #include "rotary.h"
 #include "stepquant_hip.h"
 
+// every fused multiply-add is written out
+#pragma clang fp contract(off)
+
 namespace {
 
 typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
@@ -31,6 +34,7 @@ constexpr int kRope = 64;
 constexpr int kTile = 64;        // keys of a plan's tile
 constexpr float kNone = -3e38f;  // below every score
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLarge = 0x1p19f;  // scores from here on (in log2) hold few fractions
 
 // Weights are in units of 2^m, m at most kTop and, once it is set, kBias below the
 // largest score that the row has seen: it is raised only where a score passes
@@ -61,8 +65,10 @@ struct Half<true> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_v){x, y}, bf16x2_v));
   }
-  // a pair's sum, as rounded
-  static __device__ __forceinline__ float sum(uint32_t w) { return __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u); }
+  // a pair's sum, as rounded, and l
+  static __device__ __forceinline__ float add(uint32_t w, float l) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, w), (bf16x2_v){(__bf16)1.f, (__bf16)1.f}, l, false);
+  }
 };
 
 template <>
@@ -80,8 +86,8 @@ struct Half<false> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_v){x, y}, half2_v));
   }
-  static __device__ __forceinline__ float sum(uint32_t w) {
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_v, w), (half2_v){(_Float16)1.f, (_Float16)1.f}, 0.f, false);
+  static __device__ __forceinline__ float add(uint32_t w, float l) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_v, w), (half2_v){(_Float16)1.f, (_Float16)1.f}, l, false);
   }
 };
 
@@ -253,8 +259,6 @@ __device__ __forceinline__ int place_of(int row, int at) {
 // rows of 32 scores (128 bytes) and of 32 weights (64)
 __device__ __forceinline__ int score_place(int row, int at) { return at ^ (row & 2) ^ (row >> 1 & 4); }
 __device__ __forceinline__ int weight_place(int row, int at) { return at ^ (row >> 2 & 2); }
-
-__device__ __forceinline__ int mix(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
 
 // 16 bytes a lane from memory to LDS at `lds` + 16 lane.  The compiler does not
 // count these loads: it would wait for all of them before any write to LDS; the
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
 #pragma unroll
       for (int k = 0; k < KEYS / 2; k++) {
         w[k] = H::pack(__builtin_amdgcn_exp2f(x[2 * k] - m), __builtin_amdgcn_exp2f(x[2 * k + 1] - m));
-        l += H::sum(w[k]);
+        l = H::add(w[k], l);
       }
       typedef uint32_t words __attribute__((ext_vector_type(2)));
       if constexpr (KEYS == 4) *to_lds_at<words>(weight_to) = (words){w[0], w[1]};
@@ -752,179 +756,351 @@ __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
 //
 // Every head has keys of its own, D dims beside the shared rope key, and values
 // of D dims, packed request after request.  A unit is up to 256 rows (tokens) of
-// one head, 32 a wave; the tiles of 64 keys pass through LDS.
+// one head, 32 for each of eight waves, against a range of keys; tiles of 64 keys pass through LDS.
+//
+// Two waves share a SIMD, one of each half of the workgroup, and the halves run a
+// step apart: while one issues its products (the tile before's values, this tile's
+// keys), the other one's vector instructions (the softmax) have the SIMD.  A barrier ends
+// each step.  The late half loads.
 
 struct ExpandedDev {
   const uint16_t *q, *k, *v, *rope;
   uint16_t *out;
-  const int32_t *cu, *starts, *units, *unit_starts;
+  float *ws;
+  const int32_t *cu, *starts, *units, *merges, *unit_starts;
   int64_t tokens, rows, q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, rope_stride;
-  int32_t batch, heads, causal, max_units, max_workers, unit_rows;
+  int32_t batch, heads, causal, max_partials, max_units, max_workers, unit_rows;
   float scale;
+};
+
+// Where 16-byte groups lie in LDS: rows of 128 dims of a key (256 bytes) and of 64 (128 bytes)
+// are read as 32 rows at one group, values as 64 bytes of four rows.
+template <int DIMS>
+__device__ __forceinline__ int key_place(int row, int at) { return at ^ (DIMS == 128 ? row & 15 : row >> 1 & 7); }
+template <int DIMS>
+__device__ __forceinline__ int value_place(int row, int at) { return at ^ (DIMS == 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2); }
+
+template <int D>
+struct Expanded {
+  static constexpr int KTILE = 64 * 2 * D, RTILE = 64 * 2 * kRope, VTILE = 64 * 2 * D, RING = 3;
+  static constexpr int KEYS = KTILE + RTILE;
+  static constexpr int OUT = 2 * D + 16;  // bytes from row to row of the outputs' way out
+  static constexpr size_t tiles = RING * (KEYS + VTILE), lds = tiles + 16;
+  static_assert(256 * OUT <= tiles, "outputs leave by way of the tiles' place");
 };
 
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) {
   typedef Half<BF16> H;
-  constexpr int KD = D + kRope, KROW = 2 * KD, VROW = 2 * D, KTILE = 64 * KROW, VTILE = 64 * VROW;
-  constexpr int KLOADS = KTILE / 8192, VLOADS = VTILE / 8192, KS = KD / 16, DT = D / 32;
-  extern __shared__ uint8_t smem[];
-  __shared__ unsigned long long bad_keys[2];
-  uint8_t *const kt = smem, *const vt = smem + 2 * KTILE;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  typedef Expanded<D> S;
+  constexpr int KS = (D + kRope) / 16, KK = D / 16, DT = D / 32, RING = S::RING;
+  constexpr int KL = S::KTILE / 4096, RL = S::RTILE / 4096, VL = S::VTILE / 4096, BATCH = KL + RL + VL;  // loads of a wave
+  constexpr int ROWS = 1024 / (2 * D);  // of keys or values that a load takes
+  extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), share = wave & 3;
   const int lane = tid & 63, c = lane & 31, hl = lane >> 5;
+  const bool late = wave >= 4;
   const int h = blockIdx.x % a.heads, worker = blockIdx.x / a.heads;
-  const int unit0 = max(0, a.unit_starts[worker]), unit1 = min(a.unit_starts[worker + 1], a.max_units);
-  const uint32_t kt_at = lds_address(kt), vt_at = lds_address(vt);
+  const int unit0 = max(0, uniform_word(a.unit_starts + worker)), unit1 = min(uniform_word(a.unit_starts + worker + 1), a.max_units);
+  const uint32_t at = lds_address(smem), keys_at = at, values_at = at + RING * S::KEYS;
+  const uint32_t bad_at = at + S::tiles;  // two masks of keys whose values are not numbers
+  // a lane's first operands: its key's groups (those of other steps flip bits 5 and on, or 4 and
+  // on of 64 dims), the rope key's, its four keys' values (other blocks of 32 dims flip bits 6 and on)
+  const uint32_t key_lane = c * (2 * D) + 16 * key_place<D>(c, hl), rope_lane = S::KTILE + c * 128 + 16 * key_place<64>(c, hl);
+  const int token = 4 * hl + (lane >> 2 & 3);
+  const uint32_t value_lane = token * (2 * D) + 16 * value_place<D>(token, 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) + 8 * (lane & 1);
 
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
     const int32_t *u = a.units + 8 * (int64_t)unit_at;
-    const int q0 = u[1], f0 = u[2], rows = u[3], pos0 = u[4];
-    if (rows <= 0 || rows > a.unit_rows || q0 < 0 || f0 < 0 || u[5] < 0 || (int64_t)q0 + f0 + rows > a.tokens) continue;
+    const int q0 = uniform_word(u + 1), f0 = uniform_word(u + 2), rows = uniform_word(u + 3), pos0 = uniform_word(u + 4);
+    const int kv0 = uniform_word(u + 5), unit_end = uniform_word(u + 6), part = uniform_word(u + 7);
+    if (rows <= 0 || rows > a.unit_rows || q0 < 0 || f0 < 0 || kv0 < 0 || (int64_t)q0 + f0 + rows > a.tokens) continue;
     // the request: the last one that starts at q0 or before
     int b = -1;
     for (int i = 0; i < a.batch && b < 0; i += 64) {
-      const unsigned long long past = __ballot(i + lane < a.batch && a.cu[i + lane + 1] > q0);
+      const unsigned long long past = __ballot(i + lane < a.batch && a.cu[min(i + lane, a.batch - 1) + 1] > q0);
       if (past) b = i + __builtin_ctzll(past);
     }
-    const int64_t start = b >= 0 ? max(a.starts[b], 0) : 0;
-    const int held = b >= 0 ? (int)max((int64_t)0, min((int64_t)a.starts[b + 1], a.rows) - start) : 0;
-    const int kv0 = u[5], kv1 = min(u[6], held), n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
+    const int64_t start = b >= 0 ? max(uniform_word(a.starts + b), 0) : 0;
+    const int held = b >= 0 ? (int)max((int64_t)0, min((int64_t)uniform_word(a.starts + b + 1), a.rows) - start) : 0;
+    const int kv1 = min(unit_end, held), n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
 
-    // (past the last key the last again; its scores are masked)
-    auto load = [&](int i) {
-      const int first = kv0 + kTile * i;
+    // Loads of tile i's keys, or values; past the last key the last again, whose scores are masked.
+    // Offsets from a tile's first row fit 32 bits (the host checks the strides).
+    auto load_rows = [&](auto COUNT, auto PLACE, const uint16_t *base, int64_t stride, int per, uint32_t to, int i) {
+      constexpr int count = decltype(COUNT)::value;
+      const int first = kv0 + kTile * i, last = kv1 - 1 - first, from = anew(lane);
+      const uint8_t *src = (const uint8_t *)(base + (start + first) * stride);
+      const int lanes = 64 / per, row_in = from / lanes, group = from % lanes;
 #pragma unroll
-      for (int k = 0; k < KLOADS; k++) {
-        const int j = 512 * k + tid, row = j / (KD / 8), at = j - row * (KD / 8);
-        const int g = (at & ~7) | ((at & 7) ^ mix(row & 7));
-        const int64_t key = start + min(first + row, kv1 - 1);
-        const uint16_t *src = g < D / 8 ? a.k + key * a.k_stride + h * a.k_head_stride + 8 * g : a.rope + key * a.rope_stride + 8 * g - D;
-        to_lds(kt_at + (i & 1) * KTILE + 8192 * k + 1024 * wave, src);
-      }
-#pragma unroll
-      for (int k = 0; k < VLOADS; k++) {
-        const int j = 512 * k + tid, row = j / (D / 8), at = j - row * (D / 8);
-        const int g = (at & ~7) | ((at & 7) ^ mix(row & 7));
-        const int64_t key = start + min(first + row, kv1 - 1);
-        to_lds(vt_at + (i & 1) * VTILE + 8192 * k + 1024 * wave, a.v + key * a.v_stride + h * a.v_head_stride + 8 * g);
+      for (int k = 0; k < count; k++) {
+        const int row = per * (count * share + k) + row_in;
+        const uint32_t offset = (uint32_t)min(row, last) * (uint32_t)(2 * stride) + 16 * PLACE(row, group);
+        to_lds(to + 1024 * (count * share + k), src, offset);
       }
     };
-    if (n > 0) load(0);
+    auto load_keys = [&](int i, uint32_t slot) {
+      if (i >= n) return;
+      load_rows(std::integral_constant<int, KL>{}, key_place<D>, a.k + h * a.k_head_stride, a.k_stride, ROWS, keys_at + slot, i);
+      load_rows(std::integral_constant<int, RL>{}, key_place<64>, a.rope, a.rope_stride, 8, keys_at + slot + S::KTILE, i);
+    };
+    auto load_values = [&](int i, uint32_t slot) {
+      if (i >= n) return;
+      load_rows(std::integral_constant<int, VL>{}, value_place<D>, a.v + h * a.v_head_stride, a.v_stride, ROWS, values_at + slot, i);
+    };
+    if (late) {
+      load_keys(0, 0);
+      load_values(0, 0);
+      load_keys(1, S::KEYS);
+      load_values(1, S::VTILE);
+      load_keys(2, 2 * S::KEYS);
+    }
     const int mine = 32 * wave + c;
     const bool live = mine < rows;
     u32x4_v q[KS];
     {
       const uint16_t *src = a.q + (int64_t)(q0 + f0 + (live ? mine : 0)) * a.q_stride + h * a.q_head_stride + 8 * hl;
+      // scores keep their order when they are scaled: the sign goes to the query
+      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-      for (int s = 0; s < KS; s++) q[s] = live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0};
+      for (int s = 0; s < KS; s++) q[s] = (live ? *(const u32x4_v *)(src + 16 * s) : (u32x4_v){0, 0, 0, 0}) ^ flip;
     }
+#pragma unroll
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     const int hi = live ? a.causal ? min(kv1, pos0 + f0 + mine + 1) : kv1 : 0;
     const int all_hi = a.causal ? min(kv1, pos0 + f0 + 1) : kv1;  // keys that every row of the unit sees
-    const float mult = a.scale * kLog2e;
-    float m = kNone, l = 0.f;
+    // (a factor of 0 would make NaN of masked scores)
+    const float mult = a.scale == 0.f ? 1e-37f : fabsf(a.scale) * kLog2e;
+    // (rows that see none of the unit's keys keep a unit that no branch below is taken for)
+    float m = hi > kv0 ? kNone : 0.f, l = 0.f;
     bool poisoned = false;
-    f32x16_v o[DT];
+    f32x16_v o[DT], s[2];
+    u32x4_v p[4];
 #pragma unroll
     for (int e = 0; e < DT; e++)
 #pragma unroll
       for (int k = 0; k < 16; k++) o[e][k] = 0.f;
+    auto whole = [&](int i) { return kv0 + kTile * (i + 1) <= all_hi; };
 
-    for (int i = 0; i < n; i++) {
-      const int first = kv0 + kTile * i;
-      const bool whole = first + kTile <= all_hi;
-      wait_loads<0>();
-      if (tid == 0) bad_keys[i & 1] = 0;
-      __syncthreads();
-      if (i + 1 < n) load(i + 1);
-      const uint8_t *keys = kt + (i & 1) * KTILE, *values = vt + (i & 1) * VTILE;
-      const uint32_t values_at = vt_at + (i & 1) * VTILE;
-      if (!whole) {
-        // Values that are not numbers would reach rows that do not see their key
-        // (0 times infinity); they are taken out, and rows that do see the key are NaN.
-#pragma unroll
-        for (int k = 0; k < VLOADS; k++) {
-          const int j = 512 * k + tid, row = j / (D / 8);
-          u32x4_v *p = (u32x4_v *)(values + 16 * j);
-          const u32x4_v w = *p;
-          u32x4_v x;
-          uint32_t off = 0;
-#pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = only_finite<BF16>(w[e]), off |= x[e] ^ w[e];
-          if (off) {
-            *p = x;
-            atomicOr(&bad_keys[i & 1], 1ull << row);
-          }
-        }
-        __syncthreads();
-        const int seen = hi - first;
-        const unsigned long long bad = bad_keys[i & 1];
-        poisoned |= seen > 0 && (bad & (seen >= 64 ? ~0ull : (1ull << seen) - 1));
-      }
-      f32x16_v s[2];
+    // Outputs with the values at `values` (OUT), then scores with the keys at `keys` (IN);
+    // operands are read DEEP products ahead.
+    auto products = [&](auto OUT, auto IN, uint32_t values, uint32_t keys) {
+      constexpr int NO = decltype(OUT)::value ? 4 * DT : 0, N = NO + (decltype(IN)::value ? 2 * KS : 0), DEEP = 4;
+      const uint32_t vat = values_at + values + value_lane, kat = keys_at + keys + key_lane, rat = keys_at + keys + rope_lane;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int k = 0; k < 16; k++) s[t][k] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; k++)
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const int row = 32 * t + c, g = 2 * k + hl;
-          const u32x4_v w = *(const u32x4_v *)(keys + row * KROW + 16 * ((g & ~7) | ((g & 7) ^ mix(row & 7))));
-          s[t] = H::mul(w, q[k], s[t]);
+      u32x4_v w[DEEP];
+      auto read = [&](int i) {
+        if (i < NO) {
+          const int e = i % DT, j = i / DT;
+          const uint2 x = __builtin_bit_cast(uint2, read_column((vat ^ 64 * e) + 16 * j * (2 * D)));
+          const uint2 y = __builtin_bit_cast(uint2, read_column((vat ^ 64 * e) + (16 * j + 8) * (2 * D)));
+          return (u32x4_v){x.x, x.y, y.x, y.y};
         }
-      float best = -INFINITY;
+        const int t = (i - NO) % 2, k = (i - NO) / 2;
+        return *from_lds<u32x4_v>(k < KK ? (kat ^ 32 * k) + 32 * t * (2 * D) : (rat ^ 32 * (k - KK)) + 32 * t * 128);
+      };
 #pragma unroll
-      for (int k = 0; k < 32; k++) {
-        float x = s[k >> 4][k & 15] * mult;
-        if (!whole) x = first + 32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hl + (k & 3) < hi ? x : -INFINITY;
-        s[k >> 4][k & 15] = x;
-        best = fmaxf(best, x);
+      for (int i = 0; i < DEEP; i++) w[i] = read(i);
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        if (i < NO) o[i % DT] = H::mul(w[i % DEEP], p[i / DT], o[i % DT]);
+        else s[(i - NO) % 2] = H::mul(w[i % DEEP], q[(i - NO) / 2], s[(i - NO) % 2]);
+        if (i + DEEP < N) w[i % DEEP] = read(i + DEEP);
       }
-      best = max2(best);
-      if (__any(best - m > kTop)) {
+      __builtin_amdgcn_sched_group_barrier(0x100, NO ? 2 * DEEP : DEEP, 0);  // LDS reads
+#pragma unroll
+      for (int i = 0; i < N - DEEP; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
+        if (i + DEEP < NO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, DEEP, 0);
+    };
+    // Values that are not numbers would reach rows that do not see their key (0 times
+    // infinity); they are taken out, and rows that do see the key are NaN.
+    auto clean = [&](int i, uint32_t slot) {
+      for (int j = tid & 255; j < S::VTILE / 16; j += 256) {
+        const uint32_t place = values_at + slot + 16 * j;
+        const u32x4_v w = *from_lds<u32x4_v>(place);
+        u32x4_v x;
+        uint32_t off = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = only_finite<BF16>(w[k]), off |= x[k] ^ w[k];
+        if (off) {
+          const int row = j / (D / 8);
+          *to_lds_at<u32x4_v>(place) = x;
+          __hip_atomic_fetch_or(to_lds_at<uint32_t>(bad_at + 8 * (i & 1) + 4 * (row >> 5)), 1u << (row & 31), __ATOMIC_RELAXED,
+                                __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      }
+    };
+    auto poison = [&](int i) {
+      const int seen = hi - (kv0 + kTile * i);
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const uint32_t bad = *from_lds<uint32_t>(bad_at + 8 * (i & 1) + 4 * k);
+        const int some = seen - 32 * k;
+        poisoned |= some > 0 && (bad & (some >= 32 ? ~0u : (1u << some) - 1)) != 0;
+      }
+    };
+    auto softmax = [&](int i, bool all) {
+      if (!all) {
+        const int above = hi - (kv0 + kTile * i) - 4 * hl;
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+          // all ones where the key is seen; as conditions, 32 of them would spill scalar registers
+          int seen = (32 * (k >> 4) + 8 * (k >> 2 & 3) + (k & 3) - above) >> 31;
+          asm("" : "+v"(seen));
+          const uint32_t x = __float_as_uint(s[k >> 4][k & 15]);
+          s[k >> 4][k & 15] = __uint_as_float((x & seen) | (0xff800000u & ~seen));
+        }
+      }
+      float best = s[0][0];
+#pragma unroll
+      for (int k = 1; k < 32; k++) best = fmaxf(best, s[k >> 4][k & 15]);
+      best = max2(best) * mult;
+      float f = mult, less = m;
+      if (__any(fmaxf(best - m, fabsf(m) * 0x1p-16f) > kTop)) {  // (or scores past 2^19, m of which hold no fine fractions)
         const float raised = best - m > kTop ? best - kBias : m, shrink = __builtin_amdgcn_exp2f(m - raised);
-        m = raised;
+        m = less = raised;
         l *= shrink;
 #pragma unroll
         for (int e = 0; e < DT; e++) o[e] *= shrink;
+        if (__any(fabsf(m) > kLarge)) {
+          // rounded before the difference, as the maximum is, so that no weight passes what a half holds
+#pragma unroll
+          for (int k = 0; k < 32; k++) s[k >> 4][k & 15] = s[k >> 4][k & 15] * mult - m;
+          f = 1.f, less = 0.f;
+        }
       }
-      u32x4_v p[4];
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const int at = 8 * j + 2 * k;
-          p[j][k] = H::pack(__builtin_amdgcn_exp2f(s[at >> 4][at & 15] - m), __builtin_amdgcn_exp2f(s[at >> 4][(at & 15) + 1] - m));
-          l += H::sum(p[j][k]);
+          const int x = 8 * j + 2 * k;
+          p[j][k] = H::pack(__builtin_amdgcn_exp2f(fmaf(s[x >> 4][x & 15], f, -less)), __builtin_amdgcn_exp2f(fmaf(s[x >> 4][(x & 15) + 1], f, -less)));
+          l = H::add(p[j][k], l);
         }
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int e = 0; e < DT; e++) {
-          uint2 w[2];
-#pragma unroll
-          for (int z = 0; z < 2; z++) {
-            const int row = 16 * j + 8 * z + 4 * hl + (lane >> 2 & 3), col = 32 * e + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-            const int g = col / 8;
-            w[z] = __builtin_bit_cast(uint2, read_column(values_at + row * VROW + 16 * ((g & ~7) | ((g & 7) ^ mix(row & 7))) + 2 * (col & 7)));
-          }
-          o[e] = H::mul((u32x4_v){w[0].x, w[0].y, w[1].x, w[1].y}, p[j], o[e]);
+    };
+
+    if (n > 0) {
+      auto next_keys = [](uint32_t x) { return x + S::KEYS == RING * S::KEYS ? 0u : x + S::KEYS; };
+      auto next_values = [](uint32_t x) { return x + S::VTILE == RING * S::VTILE ? 0u : x + S::VTILE; };
+      uint32_t keys = 0, values = 0;  // tile i's places
+      // (loads go in batches: a tile's keys and the values of the one before)
+      if (late) wait_loads<0>();
+      __syncthreads();
+      if (late) __syncthreads();
+      products(std::false_type{}, std::true_type{}, 0, 0);
+      for (int i = 0;; i++) {
+        const bool all = whole(i);
+        if (late) {
+          if (i >= 1 && i + 2 < n) wait_loads<BATCH>();
+          else wait_loads<0>();
+          if (!all && (tid & 255) < 2) *to_lds_at<uint32_t>(bad_at + 8 * (i & 1) + 4 * (tid & 1)) = 0;
         }
+        __syncthreads();
+        if (late && !all) {
+          clean(i, values);
+          __syncthreads();
+        }
+        if (late) {
+          const uint32_t k3 = keys, v2 = values >= S::VTILE ? values - S::VTILE : values + (RING - 1) * S::VTILE;
+          load_keys(i + 3, k3);
+          load_values(i + 2, v2);
+        }
+        softmax(i, all);
+        __syncthreads();
+        if (!late && !all) __syncthreads();  // the late half cleans the tile
+        if (!all) poison(i);
+        if (i + 1 == n) break;
+        const uint32_t k1 = next_keys(keys);
+        products(std::true_type{}, std::true_type{}, values, k1);
+        keys = k1, values = next_values(values);
+      }
+      products(std::true_type{}, std::false_type{}, values, 0);
+      if (!late) __syncthreads();
+      __syncthreads();  // the outputs go where the tiles were
     }
     l = sum2(l);
-    const float f = poisoned ? NAN : l == 0.f ? 0.f : 1.f / l;
-    if (live) {
-      uint16_t *dst = a.out + ((int64_t)(q0 + f0 + mine) * a.heads + h) * D + 4 * hl;
+    if (part < 0) {
+      // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
+      const float f = poisoned ? NAN : l == 0.f ? 0.f : 1.f / l;
+      const uint32_t mine_at = at + wave * (32 * S::OUT);
 #pragma unroll
       for (int e = 0; e < DT; e++)
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          store4<BF16>(dst + 32 * e + 8 * k, (f32x4_v){o[e][4 * k], o[e][4 * k + 1], o[e][4 * k + 2], o[e][4 * k + 3]} * f);
+        for (int k = 0; k < 4; k++) {
+          typedef uint32_t words __attribute__((ext_vector_type(2)));
+          *to_lds_at<words>(mine_at + c * S::OUT + 64 * e + 16 * k + 8 * hl) =
+              (words){H::pack(o[e][4 * k] * f, o[e][4 * k + 1] * f), H::pack(o[e][4 * k + 2] * f, o[e][4 * k + 3] * f)};
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      constexpr int LANES = D / 8;
+#pragma unroll
+      for (int i = 0; i < 32 * LANES / 64; i++) {
+        const int r = (64 * i + lane) / LANES, g = (64 * i + lane) % LANES;
+        const u32x4_v x = *from_lds<u32x4_v>(mine_at + r * S::OUT + 16 * g);
+        if (32 * wave + r < rows) *(u32x4_v *)(a.out + ((int64_t)(q0 + f0 + 32 * wave + r) * a.heads + h) * D + 8 * g) = x;
+      }
+    } else {
+      // as the registers hold them
+      typedef float vec __attribute__((ext_vector_type(DT)));
+      const int64_t slot = (int64_t)part * a.heads + h;
+      float *dst = a.ws + ((slot * 8 + wave) * (16 * 64) + lane) * DT;
+#pragma unroll
+      for (int k = 0; k < 16; k++) {
+        vec x;
+#pragma unroll
+        for (int e = 0; e < DT; e++) x[e] = o[e][k];
+        *(vec *)(dst + k * 64 * DT) = x;
+      }
+      if (live && hl == 0)
+        *(float2 *)(a.ws + (int64_t)a.max_partials * a.heads * a.unit_rows * D + 2 * (slot * a.unit_rows + mine)) =
+            make_float2(hi > kv0 ? m : kNone, poisoned ? NAN : l);
     }
     __syncthreads();  // before the next unit's tiles
   }
+}
+
+// Joins the parts of units whose keys were cut: one workgroup per (merge, head) and wave of 32 rows.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedDev a) {
+  constexpr int DT = D / 32;
+  typedef float vec __attribute__((ext_vector_type(DT)));
+  const int h = blockIdx.x % a.heads, wave = blockIdx.y;
+  const int32_t *u = a.merges + 8 * (int64_t)(blockIdx.x / a.heads);
+  const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4];
+  const int lane = threadIdx.x & 63, c = lane & 31, hl = lane >> 5, four = threadIdx.x >> 6, mine = 32 * wave + c;
+  if (32 * wave >= rows) return;
+  const float *ml = a.ws + (int64_t)a.max_partials * a.heads * a.unit_rows * D + 2 * (int64_t)min(mine, rows - 1);
+  vec x[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = (vec)(0.f);
+  float sum = 0, mm = kNone;
+#pragma unroll 2
+  for (int i = 0; i < n; i++) {
+    const int64_t slot = (int64_t)(p0 + i) * a.heads + h;
+    const float2 stat = *(const float2 *)(ml + 2 * slot * a.unit_rows);
+    vec y[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = *(const vec *)(a.ws + (((slot * 8 + wave) * 16 + 4 * four + k) * 64 + lane) * DT);
+    const float high = fmaxf(mm, stat.x), was = __builtin_amdgcn_exp2f(mm - high), w = __builtin_amdgcn_exp2f(stat.x - high);
+    mm = high;
+    sum = fmaf(sum, was, stat.y * w);
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[k] = x[k] * was + y[k] * w;
+  }
+  if (mine >= rows) return;
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t *dst = a.out + ((int64_t)(q0 + f0 + mine) * a.heads + h) * D;
+#pragma unroll
+  for (int e = 0; e < DT; e++)
+    store4<BF16>(dst + 32 * e + 8 * four + 4 * hl, (f32x4_v){x[0][e], x[1][e], x[2][e], x[3][e]} * f);
 }
 
 // ------------------------------------------------------------ host side
@@ -983,12 +1159,15 @@ int launch_absorbed(const AbsorbedDev &d, const sq_kv_schedule &s, hipStream_t s
 }
 
 template <int D, bool BF16>
-int launch_expanded(const ExpandedDev &d, hipStream_t st) {
-  constexpr size_t lds = 2 * 64 * 2 * (2 * D + kRope);
+int launch_expanded(const ExpandedDev &d, const sq_kv_schedule &s, hipStream_t st) {
+  constexpr size_t lds = Expanded<D>::lds;
   const int rc = dynamic_lds((const void *)expanded_attend_kernel<D, BF16>, 16 + 2 * (D == 128) + BF16, lds, "expanded attention: LDS attribute");
   if (rc) return rc;
   hipLaunchKernelGGL((expanded_attend_kernel<D, BF16>), dim3((unsigned)d.max_workers * d.heads), dim3(512), lds, st, d);
-  return sq_internal_launched("expanded_attend_kernel");
+  const int e = sq_internal_launched("expanded_attend_kernel");
+  if (e) return e;
+  hipLaunchKernelGGL((expanded_merge_kernel<D, BF16>), dim3((unsigned)s.max_merges * d.heads, (unsigned)(s.merge_rows + 31) / 32), dim3(256), 0, st, d);
+  return sq_internal_launched("expanded_merge_kernel");
 }
 
 }  // namespace
@@ -1082,6 +1261,7 @@ int sq_expanded_attend(const sq_expanded_attend_args *a, void *stream) {
   if (a->tokens == 0) return 0;
   if (!a->q || !a->k || !a->v || !a->rope || !a->out || !a->cu || !a->starts || a->tokens < 0 || a->rows < 0)
     return fail(SQ_EINVAL, "expanded attention: null pointer or size");
+  if (!a->workspace || ((uintptr_t)a->workspace & 15)) return fail(SQ_EINVAL, "expanded attention: null or misaligned workspace");
   if (a->dim != 64 && a->dim != 128) return fail(SQ_ESHAPE, "expanded attention: heads have 64 or 128 dims");
   if (a->dtype != SQ_BF16 && a->dtype != SQ_F16) return fail(SQ_EINVAL, "expanded attention: operands are bf16 or fp16");
   if (a->batch <= 0 || a->batch > SQ_KV_MAX_REQUESTS) return fail(SQ_EINVAL, "expanded attention: batch must be in [1, 4096]");
@@ -1091,6 +1271,8 @@ int sq_expanded_attend(const sq_expanded_attend_args *a, void *stream) {
   if (a->q_stride < 0 || a->q_head_stride < 0 || a->k_stride < 0 || a->k_head_stride < 0 || a->v_stride < 0 ||
       a->v_head_stride < 0 || a->rope_stride < 0)
     return fail(SQ_EINVAL, "expanded attention: negative stride");
+  if (a->k_stride >= 1 << 24 || a->v_stride >= 1 << 24 || a->rope_stride >= 1 << 24)
+    return fail(SQ_EINVAL, "expanded attention: rows of keys and values must be fewer than 2^24 elements apart");
   if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(SQ_EINVAL, "expanded attention: scale must be finite");
   const sq_kv_schedule &s = a->schedule;
   const int rc = sq_internal_check_schedule(&s, a->tokens, a->batch);
@@ -1098,13 +1280,13 @@ int sq_expanded_attend(const sq_expanded_attend_args *a, void *stream) {
   if (s.kv_heads != s.q_heads || s.window || s.few_work || s.rows != 256)
     return fail(SQ_ESHAPE, "expanded attention: the schedule is for another kind of attention");
   const ExpandedDev d = {(const uint16_t *)a->q, (const uint16_t *)a->k, (const uint16_t *)a->v, (const uint16_t *)a->rope,
-                         (uint16_t *)a->out, a->cu, a->starts, s.units, s.starts, a->tokens, a->rows, a->q_stride,
-                         a->q_head_stride, a->k_stride, a->k_head_stride, a->v_stride, a->v_head_stride, a->rope_stride,
-                         a->batch, s.q_heads, s.causal, s.max_units, s.max_workers, s.rows, a->scale};
+                         (uint16_t *)a->out, a->workspace, a->cu, a->starts, s.units, s.merges, s.starts, a->tokens, a->rows,
+                         a->q_stride, a->q_head_stride, a->k_stride, a->k_head_stride, a->v_stride, a->v_head_stride,
+                         a->rope_stride, a->batch, s.q_heads, s.causal, s.max_partials, s.max_units, s.max_workers, s.rows, a->scale};
   hipStream_t st = (hipStream_t)stream;
   const bool bf16 = a->dtype == SQ_BF16;
-  if (a->dim == 64) return bf16 ? launch_expanded<64, true>(d, st) : launch_expanded<64, false>(d, st);
-  return bf16 ? launch_expanded<128, true>(d, st) : launch_expanded<128, false>(d, st);
+  if (a->dim == 64) return bf16 ? launch_expanded<64, true>(d, s, st) : launch_expanded<64, false>(d, s, st);
+  return bf16 ? launch_expanded<128, true>(d, s, st) : launch_expanded<128, false>(d, s, st);
 }
 
 }  // extern "C"

@@ -249,6 +249,7 @@ class BlockTables:
 
     # Latent attention.  Absorbed, every head shares the one key: a set is rows of all heads.
     latent_min_tiles, latent_cut_tiles = 2, 4
+    expanded_min_tiles, expanded_cut_tiles = 4, 16
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows, absorbed=None, expanded=None):
         """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all
@@ -302,7 +303,7 @@ class BlockTables:
                 # (one workgroup on a CU; sets of 128 have two)
                 add(form, 0, n, 1, rows, self._cus // (2 if rows == 128 else 1), self.latent_min_tiles, self.latent_cut_tiles)
             else:
-                add(form, 0, n, n, 256, self._cus, 1, 1 << 28)
+                add(form, 0, n, n, 256, self._cus, self.expanded_min_tiles, self.expanded_cut_tiles)
         offsets = [4 * sum(sizes[:i]) for i in range(7)]
         return sizes, sum(sizes), offsets, most, schedules
 

@@ -48,6 +48,11 @@ def _whole(x):
     return x
 
 
+def _near(x):
+    """The same, with rows fewer than 2^24 elements apart."""
+    return _whole(x) if x.stride(0) < 1 << 24 else x.clone(memory_format=torch.contiguous_format)
+
+
 def _scale(scale):
     scale = float(scale)
     if not abs(scale) < 3e38:
@@ -251,8 +256,9 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
         return out
     if not rows:
         return out.zero_()
-    q, k, v, rope = _whole(q), _whole(k), _whole(v), _whole(rope)
-    args = N.EXPANDED_ATTEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), out.data_ptr(), plan._cu,
+    q, k, v, rope = _whole(q), _near(k), _near(v), _near(rope)
+    ws = torch.empty(s.floats * (dim + 2), dtype=torch.float32, device=v.device)
+    args = N.EXPANDED_ATTEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), out.data_ptr(), ws.data_ptr(), plan._cu,
                                   starts_at, plan.tokens, rows, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
                                   rope.stride(0), plan.batch, dim, _HALVES[v.dtype], scale, s.packed)
     rc = N.kv_entry("sq_expanded_attend")(args, N.raw_stream())

@@ -111,11 +111,12 @@ def test_absorbed_attention_is_checked_before_any_launch(kw):
 @pytest.mark.parametrize("kw", [dict(q=None), dict(k=8), dict(v=None), dict(rope=24), dict(out=8), dict(cu=None),
                                 dict(starts=None), dict(tokens=-1), dict(rows=-1), dict(dim=96), dict(dtype=N.F32),
                                 dict(batch=0), dict(batch=4097), dict(q_stride=12), dict(k_head_stride=-128),
-                                dict(v_stride=4), dict(rope_stride=-64), dict(scale=math.inf)] +
+                                dict(v_stride=4), dict(rope_stride=-64), dict(scale=math.inf), dict(workspace=None), dict(workspace=8),
+                                dict(k_stride=1 << 24)] +
                          [dict(schedule=_schedule(**{**dict(kv_heads=8, rows=256), **s})) for s in (
                              dict(kv_heads=4), dict(rows=16), dict(window=5), dict(units=None), dict(max_units=3))])
 def test_expanded_attention_is_checked_before_any_launch(kw):
-    a = dict(q=16, k=16, v=16, rope=16, out=16, cu=16, starts=16, tokens=16, rows=16, q_stride=1536, q_head_stride=192,
+    a = dict(q=16, k=16, v=16, rope=16, out=16, workspace=16, cu=16, starts=16, tokens=16, rows=16, q_stride=1536, q_head_stride=192,
              k_stride=1024, k_head_stride=128, v_stride=1024, v_head_stride=128, rope_stride=64, batch=2, dim=128,
              dtype=N.F16, scale=1., schedule=_schedule(kv_heads=8, rows=256))
     assert N.lib().sq_expanded_attend(N.ExpandedAttend(**{**a, **kw}), None) in (-22, -23)
