@@ -810,19 +810,32 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
   const int token = 4 * hl + (lane >> 2 & 3);
   const uint32_t value_lane = token * (2 * D) + 16 * value_place<D>(token, 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) + 8 * (lane & 1);
 
+  // the lanes hold where the first 64 requests' queries end and their keys begin
+  const int ends = a.cu[min(lane, a.batch - 1) + 1];
+  const int2 keys_of = make_int2(a.starts[min(lane, a.batch - 1)], a.starts[min(lane, a.batch - 1) + 1]);
+
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
     const int32_t *u = a.units + 8 * (int64_t)unit_at;
     const int q0 = uniform_word(u + 1), f0 = uniform_word(u + 2), rows = uniform_word(u + 3), pos0 = uniform_word(u + 4);
     const int kv0 = uniform_word(u + 5), unit_end = uniform_word(u + 6), part = uniform_word(u + 7);
     if (rows <= 0 || rows > a.unit_rows || q0 < 0 || f0 < 0 || kv0 < 0 || (int64_t)q0 + f0 + rows > a.tokens) continue;
     // the request: the last one that starts at q0 or before
-    int b = -1;
-    for (int i = 0; i < a.batch && b < 0; i += 64) {
-      const unsigned long long past = __ballot(i + lane < a.batch && a.cu[min(i + lane, a.batch - 1) + 1] > q0);
-      if (past) b = i + __builtin_ctzll(past);
+    int64_t start = 0, end = 0;
+    const unsigned long long past = __ballot(lane < a.batch && ends > q0);
+    if (past) {
+      const int b = __builtin_ctzll(past);
+      start = __builtin_amdgcn_readlane(keys_of.x, b), end = __builtin_amdgcn_readlane(keys_of.y, b);
+    } else {
+      for (int i = 64; i < a.batch; i += 64) {
+        const unsigned long long there = __ballot(i + lane < a.batch && a.cu[min(i + lane, a.batch - 1) + 1] > q0);
+        if (!there) continue;
+        const int b = i + __builtin_ctzll(there);
+        start = uniform_word(a.starts + b), end = uniform_word(a.starts + b + 1);
+        break;
+      }
     }
-    const int64_t start = b >= 0 ? max(uniform_word(a.starts + b), 0) : 0;
-    const int held = b >= 0 ? (int)max((int64_t)0, min((int64_t)uniform_word(a.starts + b + 1), a.rows) - start) : 0;
+    start = max(start, (int64_t)0);
+    const int held = (int)max((int64_t)0, min(end, a.rows) - start);
     const int kv1 = min(unit_end, held), n = max(0, (kv1 - kv0 + kTile - 1) / kTile);
 
     // Loads of tile i's keys, or values; past the last key the last again, whose scores are masked.
@@ -990,15 +1003,18 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
       auto next_keys = [](uint32_t x) { return x + S::KEYS == RING * S::KEYS ? 0u : x + S::KEYS; };
       auto next_values = [](uint32_t x) { return x + S::VTILE == RING * S::VTILE ? 0u : x + S::VTILE; };
       uint32_t keys = 0, values = 0;  // tile i's places
-      // (loads go in batches: a tile's keys and the values of the one before)
-      if (late) wait_loads<0>();
+      // loads go in batches, a tile's keys and the values of the one before; the first keys by themselves
+      if (late) {
+        if (n > 2) wait_loads<2 * BATCH>();
+        else wait_loads<0>();
+      }
       __syncthreads();
       if (late) __syncthreads();
       products(std::false_type{}, std::true_type{}, 0, 0);
       for (int i = 0;; i++) {
         const bool all = whole(i);
         if (late) {
-          if (i >= 1 && i + 2 < n) wait_loads<BATCH>();
+          if (i + 2 < n) wait_loads<BATCH>();
           else wait_loads<0>();
           if (!all && (tid & 255) < 2) *to_lds_at<uint32_t>(bad_at + 8 * (i & 1) + 4 * (tid & 1)) = 0;
         }
