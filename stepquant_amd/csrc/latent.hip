@@ -501,8 +501,6 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   };
   begin();
   for (int unit_at = unit0; unit_at < unit1; unit_at++) {
-    const Unit following = read_unit(a, min(unit_at + 1, unit1 - 1), at_row, R);
-    const Place after = place(following);
     u32x4_v q[KS];
     f32x4_v o[NR][DB];
     {
@@ -517,6 +515,8 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
         q[s] = live ? *(const u32x4_v *)(32 * (step0 + s) < W ? src + d : rope + d - W) : (u32x4_v){0, 0, 0, 0};
       }
     }
+    const Unit following = read_unit(a, min(unit_at + 1, unit1 - 1), at_row, R);
+    const Place after = place(following);
 #pragma unroll
     for (int r = 0; r < NR; r++)
 #pragma unroll
@@ -711,45 +711,45 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   }
 }
 
-// Joins the parts of query rows whose keys were cut: one workgroup per merge and row.
-template <int W, bool BF16>
+// Joins the parts of query rows whose keys were cut: one workgroup per merge, row and
+// 4 * L dims; L lanes read a part, 512 / L parts at a time.
+template <int W, int L, bool BF16>
 __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
-  constexpr int LANES = W / 4, GROUPS = 512 / LANES;
-  __shared__ f32x4_v part_o[GROUPS][LANES];
-  __shared__ float part_l[GROUPS], part_m[GROUPS];
-  const int tid = threadIdx.x, j = blockIdx.y;
+  constexpr int GR = 512 / L;
+  __shared__ f32x4_v part_o[GR][L];
+  __shared__ float2 part_s[GR];
+  const int tid = threadIdx.x, j = blockIdx.y, lane = tid % L, grp = tid / L, d = 4 * (L * (int)blockIdx.z + lane);
   const int32_t *u = a.merges + 8 * (int64_t)blockIdx.x;
   const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4];
   if (j >= rows) return;
-  const int lane = tid % LANES, grp = tid / LANES;
   const float *ml = a.ws + (int64_t)a.max_partials * a.unit_rows * W;
   f32x4_v x = {0, 0, 0, 0};
   float sum = 0, mm = kNone;
-#pragma unroll 2
-  for (int i = grp; i < n; i += GROUPS) {
+#pragma unroll 4
+  for (int i = grp; i < n; i += GR) {
     const int64_t slot = (int64_t)(p0 + i) * a.unit_rows + j;
     const float2 stat = *(const float2 *)(ml + 2 * slot);
-    const f32x4_v y = *(const f32x4_v *)(a.ws + slot * W + 4 * lane);
+    const f32x4_v y = *(const f32x4_v *)(a.ws + slot * W + d);
     const float high = fmaxf(mm, stat.x), was = __builtin_amdgcn_exp2f(mm - high), w = __builtin_amdgcn_exp2f(stat.x - high);
     mm = high;
     sum = fmaf(sum, was, stat.y * w);
     x = x * was + y * w;
   }
   part_o[grp][lane] = x;
-  if (lane == 0) part_l[grp] = sum, part_m[grp] = mm;
+  if (lane == 0) part_s[grp] = make_float2(mm, sum);
   __syncthreads();
   if (grp) return;
 #pragma unroll
-  for (int i = 1; i < GROUPS; i++) mm = fmaxf(mm, part_m[i]);
+  for (int i = 1; i < GR; i++) mm = fmaxf(mm, part_s[i].x);
   sum = 0;
   x = (f32x4_v){0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < GROUPS; i++) {
-    const float w = __builtin_amdgcn_exp2f(part_m[i] - mm);
+  for (int i = 0; i < GR; i++) {
+    const float w = __builtin_amdgcn_exp2f(part_s[i].x - mm);
     x += part_o[i][lane] * w;
-    sum = fmaf(part_l[i], w, sum);
+    sum = fmaf(part_s[i].y, w, sum);
   }
-  store4<BF16>(a.out + (q0 * (int64_t)a.heads + f0 + j) * W + 4 * lane, x * (sum == 0.f ? 0.f : 1.f / sum));
+  store4<BF16>(a.out + (q0 * (int64_t)a.heads + f0 + j) * W + d, x * (sum == 0.f ? 0.f : 1.f / sum));
 }
 
 // ------------------------------------------------------------ expanded
@@ -1170,7 +1170,10 @@ int launch_absorbed(const AbsorbedDev &d, const sq_kv_schedule &s, hipStream_t s
                  : s.rows == 64 ? go(latent_attend_kernel<S64, BF16>, 2, S64{})
                                 : go(latent_attend_kernel<S128, BF16>, 3, S128{});
   if (rc) return rc;
-  hipLaunchKernelGGL((latent_merge_kernel<W, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
+  if ((int64_t)s.max_merges * s.merge_rows <= 256)
+    hipLaunchKernelGGL((latent_merge_kernel<W, 32, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows, W / 128), dim3(512), 0, st, d);
+  else
+    hipLaunchKernelGGL((latent_merge_kernel<W, W / 4, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
   return sq_internal_launched("latent_merge_kernel");
 }
 
