@@ -2,13 +2,15 @@
 softmax-attention layers over an 8-bit KV cache.
 
 Random weights of a small model: blocks of three gated-delta layers
-(``PackedStatePool``) and one attention layer (``KVCache``), residual
+(``PackedStatePool``) and one attention layer (``KVCache``, its queries and keys
+turned by their positions with --rotary; or ``LatentCache`` with --latent), residual
 connections, no MLP and no vocabulary.  Prompts of unequal lengths are
 prefilled in one call; then every request grows by one position a step, in a
 HIP graph that plans its pages, runs the layers and commits the plan without
 returning to the host.
 
     python examples/hybrid_serving.py --requests 16 --prompt 700 --steps 64
+    python examples/hybrid_serving.py --latent 512
 """
 import argparse
 import os
@@ -20,7 +22,9 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from stepquant_amd.kernels.kv_cache import BlockTables, KVCache  # noqa: E402
+from stepquant_amd.kernels.latent_cache import ROPE, LatentCache, expanded_attention  # noqa: E402
 from stepquant_amd.kernels.pool import PackedStatePool  # noqa: E402
+from stepquant_amd.kernels.rotary import Rotary  # noqa: E402
 from stepquant_amd.quantization import QuantizationPlan  # noqa: E402
 
 DIM, PAGE = 128, 64
@@ -59,24 +63,59 @@ class Recurrent:
 class Attention:
     """One softmax-attention layer with grouped heads over its own 8-bit pages."""
 
-    def __init__(self, width, q_heads, kv_heads, pages, storage, rng, dev):
-        self.q_heads, self.kv_heads = q_heads, kv_heads
+    def __init__(self, width, q_heads, kv_heads, pages, storage, rng, dev, rotary=None):
+        self.q_heads, self.kv_heads, self.rotary = q_heads, kv_heads, rotary
         self.cache = KVCache(pages, kv_heads, DIM, page_tokens=PAGE, storage=storage, device=dev)
         draw = lambda *s: (torch.randn(*s, generator=rng, device=dev) * s[0] ** -.5).to(torch.bfloat16)
         self.qkv, self.out = draw(width, (q_heads + 2 * kv_heads) * DIM), draw(q_heads * DIM, width)
 
     def __call__(self, x, plan):
         q, k, v = (normed(x) @ self.qkv).split([n * DIM for n in (self.q_heads, self.kv_heads, self.kv_heads)], -1)
-        self.cache.append(k, v, plan)
+        if self.rotary is None:
+            self.cache.append(k, v, plan)
+        else:
+            q = self.cache.append(k, v, plan, rotary=self.rotary, q=q)
         return x + self.cache.attend(q, plan).flatten(1) @ self.out
 
 
+class Latent:
+    """One softmax-attention layer whose heads share one latent a token: prompts
+    with keys and values expanded from the latents, single tokens with the
+    projections absorbed into queries and outputs."""
+
+    def __init__(self, width, heads, latent, pages, rng, dev):
+        self.heads, self.latent, self.rotary = heads, latent, Rotary(ROPE, layout="interleaved", device=dev)
+        self.cache = LatentCache(pages, latent, page_tokens=PAGE, device=dev)
+        draw = lambda *s: (torch.randn(*s, generator=rng, device=dev) * s[-2] ** -.5).to(torch.bfloat16)
+        self.q, self.down, self.out = draw(width, heads * (DIM + ROPE)), draw(width, latent + ROPE), draw(heads * DIM, width)
+        # [latent, heads * DIM] expand; [heads, DIM, latent] and [heads, latent, DIM] are the same for single tokens
+        self.keys, self.values = draw(latent, heads * DIM), draw(latent, heads * DIM)
+        self.into_q = self.keys.unflatten(1, (heads, DIM)).permute(1, 2, 0).contiguous()
+        self.from_y = self.values.unflatten(1, (heads, DIM)).transpose(0, 1).contiguous()
+
+    def __call__(self, x, plan, held=None):
+        h = normed(x)
+        q = (h @ self.q).unflatten(1, (self.heads, DIM + ROPE))
+        c, r = (h @ self.down).split([self.latent, ROPE], -1)
+        turned = self.cache.append(c, r, plan, rotary=self.rotary, q=q[..., DIM:], out=None if held is None else q[..., DIM:])
+        if held is None:
+            q = torch.bmm(q[..., :DIM].transpose(0, 1).contiguous(), self.into_q)
+            y = self.cache.attend(q.transpose(0, 1), turned, plan, scale=(DIM + ROPE) ** -.5)
+            y = torch.bmm(y.transpose(0, 1).contiguous(), self.from_y).transpose(0, 1)
+        else:
+            c, r, starts = self.cache.gather(plan, held)
+            k, v = ((c @ w).unflatten(1, (self.heads, DIM)) for w in (self.keys, self.values))
+            y = expanded_attention(q, k, v, r, plan, starts)
+        return x + y.flatten(1) @ self.out
+
+
 class Hybrid:
-    def __init__(self, requests, tokens, blocks=2, width=1024, heads=8, q_heads=8, kv_heads=2, storage="int8", seed=0):
+    def __init__(self, requests, tokens, blocks=2, width=1024, heads=8, q_heads=8, kv_heads=2, storage="int8", seed=0,
+                 rotary=False, latent=0):
         dev = torch.device("cuda", torch.cuda.current_device())
         rng = torch.Generator(device=dev).manual_seed(seed)
         rows = -(-tokens // PAGE)
-        self.heads = (q_heads, kv_heads)
+        self.heads, self.latent = (q_heads, kv_heads), latent
         self.tables = BlockTables(requests, 1 + requests * rows, rows, page_tokens=PAGE, device=dev)
         # slot 0 of a state pool is the padding slot: request r has slot r + 1
         self.rows = torch.arange(requests, device=dev, dtype=torch.int32)
@@ -84,7 +123,11 @@ class Hybrid:
         self.layers = []
         for _ in range(blocks):
             self.layers += [Recurrent(width, heads, requests + 1, rng, dev) for _ in range(3)]
-            self.layers.append(Attention(width, q_heads, kv_heads, self.tables.pages, storage, rng, dev))
+            if latent:
+                self.layers.append(Latent(width, q_heads, latent, self.tables.pages, rng, dev))
+            else:
+                self.layers.append(Attention(width, q_heads, kv_heads, self.tables.pages, storage, rng, dev,
+                                             Rotary(DIM, device=dev) if rotary else None))
         for layer in self.layers:
             if isinstance(layer, Recurrent):
                 layer.pool.clear(self.slots)
@@ -92,17 +135,22 @@ class Hybrid:
     def prefill(self, x, lengths):
         """``x`` [sum(lengths), width]: every request's prompt."""
         cu = torch.tensor([0] + lengths).cumsum(0)
-        plan = self.tables.plan(lengths, self.rows, heads=self.heads)
+        kind = dict(expanded=self.heads[0]) if self.latent else dict(heads=self.heads)
+        plan = self.tables.plan(lengths, self.rows, **kind)
         for layer in self.layers:
-            x = layer(x, plan) if isinstance(layer, Attention) else layer(x, self.slots, cu)
+            if isinstance(layer, Recurrent):
+                x = layer(x, self.slots, cu)
+            else:
+                x = layer(x, plan, x.shape[0]) if self.latent else layer(x, plan)
         self.tables.commit(plan)
         return x
 
     def step(self, x, counts):
         """``x`` [requests, width]: one position of every request (``counts`` ones on the GPU)."""
-        plan = self.tables.plan(counts, self.rows, tokens=x.shape[0], max_new=1, heads=self.heads)
+        kind = dict(absorbed=self.heads[0]) if self.latent else dict(heads=self.heads)
+        plan = self.tables.plan(counts, self.rows, tokens=x.shape[0], max_new=1, **kind)
         for layer in self.layers:
-            x = layer(x, plan) if isinstance(layer, Attention) else layer(x, self.slots)
+            x = layer(x, self.slots) if isinstance(layer, Recurrent) else layer(x, plan)
         self.tables.commit(plan)
         return x
 
@@ -147,9 +195,11 @@ if __name__ == "__main__":
     p.add_argument("--prompt", type=int, default=700, help="longest prompt")
     p.add_argument("--steps", type=int, default=64)
     p.add_argument("--storage", choices=["int8", "fp8"], default="int8")
+    p.add_argument("--rotary", action="store_true", help="turn the attention layers' queries and keys by their positions")
+    p.add_argument("--latent", type=int, default=0, choices=[0, 256, 512], help="dims of a latent that attention layers' heads share")
     p.add_argument("--eager", action="store_true", help="launch every step instead of replaying a graph")
     a = p.parse_args()
-    _, out, seconds, model = serve(a.requests, a.prompt, a.steps, a.storage, not a.eager)
+    _, out, seconds, model = serve(a.requests, a.prompt, a.steps, a.storage, not a.eager, rotary=a.rotary, latent=a.latent)
     layers = len(model.layers)
     print(f"{a.requests} requests, {layers} layers: {seconds * 1e6:.0f} us a step, "
           f"{a.requests / seconds:.0f} tokens/s, outputs finite: {bool(torch.isfinite(out).all())}")

@@ -424,7 +424,7 @@ class KVCache:
                 q = q.unflatten(1, (-1, self.dim))
             if q.dim() != 3 or q.shape[0] != plan.tokens or q.shape[2] != self.dim:
                 raise ValueError(f"queries must be [{plan.tokens}, heads, {self.dim}], the plan's tokens")
-            rows, out = rotary._rows(q, plan._positions, N.I32, out)
+            rows, out, q = rotary._rows(q, plan._positions, N.I32, out)
         elif out is not None:
             raise ValueError("out is where queries go")
         if not plan.tokens:

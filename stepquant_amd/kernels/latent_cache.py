@@ -145,7 +145,7 @@ class LatentCache:
         if q is not None:
             if q.dim() != 3 or q.shape[0] != plan.tokens or q.dtype != self.dtype:
                 raise ValueError(f"queries must be [{plan.tokens}, heads, dim], the plan's tokens, of the cache's type")
-            rows, out = rotary._rows(q, plan._positions, N.I32, out)
+            rows, out, q = rotary._rows(q, plan._positions, N.I32, out)
         elif out is not None:
             raise ValueError("out is where queries go")
         if not plan.tokens:

@@ -105,7 +105,7 @@ class Rotary:
         self._at = ctypes.addressof(self._desc)
 
     def _rows(self, x, positions, positions_dtype, out):
-        """(packed sq_rotary_rows, out) of ``x`` [tokens, heads, head_dim]."""
+        """(packed sq_rotary_rows, out, the rows that are read) of ``x`` [tokens, heads, head_dim]."""
         if x.dtype not in N.FLOATS:
             raise ValueError("rows must be fp32, bf16 or fp16")
         if x.device != self.device:
@@ -129,7 +129,7 @@ class Rotary:
             x = x.clone(memory_format=torch.contiguous_format)
         (xs, xh, _), (os, oh, _) = x.stride(), out.stride()
         return N.ROTARY_ROWS.pack(x.data_ptr(), out.data_ptr(), positions, tokens, xs, xh, os, oh, heads, dim,
-                                  N.FLOATS[x.dtype], positions_dtype), out
+                                  N.FLOATS[x.dtype], positions_dtype), out, x
 
     def apply(self, x, positions, *, out=None):
         """``x`` [tokens, heads, head_dim] (fp32, bf16 or fp16) turned to
@@ -146,7 +146,7 @@ class Rotary:
             raise ValueError("positions must be int32 or int64, one a token, on the rotary's device")
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        rows, out = self._rows(x, positions.data_ptr(), N.INTS[positions.dtype], out)
+        rows, out, x = self._rows(x, positions.data_ptr(), N.INTS[positions.dtype], out)
         if x.shape[0]:
             rc = N.kv_entry("sq_rotary_apply")(self._at, rows, N.raw_stream())
             if rc:
