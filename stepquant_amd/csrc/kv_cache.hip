@@ -607,7 +607,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(sq_kv_cache c, sq_kv_app
 // The same with the keys turned on the way, in 32 bits: they are rounded once, to
 // their codes (rounded to bfloat16 first, 3% of int8 codes would be others).  A
 // thread holds N pairs of groups of 8 dims, which are turned together.  The
-// workgroups from z = 2 on turn the queries of the same tokens.
+// workgroups from z = 2 on turn the queries of the same tokens, a head a thread: four,
+// which share their angles where queries are turned alone, would take registers that the
+// pages' workgroups wait for (5 prompts of up to 3777 tokens, 16 heads of 256 dims, 2 of
+// keys: 46 us and 54).  HBM bounds it there, 5 TB/s with the queries' way; a decode step of
+// 64 requests and 32 + 8 heads of 128 dims takes 6 us.
 template <bool FP8, int N>
 __global__ __launch_bounds__(256) void kv_append_rotary_kernel(sq_kv_cache c, sq_kv_append_args a, int log_dim,
                                                                const int32_t *positions, sq_rotary r, sq_rotary_rows q,
@@ -615,8 +619,9 @@ __global__ __launch_bounds__(256) void kv_append_rotary_kernel(sq_kv_cache c, sq
   __shared__ uint32_t peaks[4];
   const int tid = threadIdx.x, tile = blockIdx.x, h = blockIdx.y, part = blockIdx.z;
   if (part >= 2) {
-    const uint32_t block = ((part - 2) * gridDim.y + h) * gridDim.x + tile;
-    rotary::rotate_rows<1>(r, q, q_lanes, block * 256 + tid);
+    const uint64_t id = (((uint64_t)(part - 2) * gridDim.y + h) * gridDim.x + tile) * 256 + tid;
+    if (id >> 31) return;  // (the rows have fewer threads; the grid can have more)
+    rotary::rotate_rows<1>(r, q, q_lanes, (uint32_t)id);
     return;
   }
   const int64_t page = a.pages[tile];
@@ -1987,7 +1992,8 @@ int sq_kv_append(const sq_kv_cache *c, const sq_kv_append_args *a, void *stream)
 int sq_kv_append_rotary(const sq_kv_cache *c, const sq_kv_append_args *a, const int32_t *positions, const sq_rotary *r,
                         const sq_rotary_rows *rows, void *stream) {
   int rc = check_append(c, a);
-  if (rc || a->max_tiles == 0) return rc;
+  if (rc) return rc;
+  if (a->max_tiles == 0) return rows && rows->tokens ? sq_rotary_apply(r, rows, stream) : 0;
   rc = rotary::check(r);
   if (rc) return rc;
   if (!positions) return fail(SQ_EINVAL, "kv append: null positions");
@@ -2000,7 +2006,7 @@ int sq_kv_append_rotary(const sq_kv_cache *c, const sq_kv_append_args *a, const 
     if (rc) return rc;
     q = *rows;
     lanes = q.heads;
-    const int64_t threads = q.tokens * q.heads * (r->dim / 16), plane = (int64_t)a->max_tiles * c->heads;
+    const int64_t threads = q.tokens * lanes * (r->dim / 16), plane = (int64_t)a->max_tiles * c->heads;
     if (threads >= (int64_t)1 << 31) return fail(SQ_EINVAL, "kv append: too many queries for one call");
     z += ((threads + 255) / 256 + plane - 1) / plane;
     if (z > 65535) return fail(SQ_EINVAL, "kv append: too many queries for one call");

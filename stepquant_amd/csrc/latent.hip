@@ -21,7 +21,6 @@ namespace {
 typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_v __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
-typedef _Float16 half4_v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_v __attribute__((ext_vector_type(8)));
 typedef short short4_v __attribute__((ext_vector_type(4)));
 typedef float f32x2_v __attribute__((ext_vector_type(2)));
@@ -31,7 +30,7 @@ typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void *lds_t;
 
 constexpr int kRope = 64;
-constexpr int kTile = 64;        // keys of a plan's tile
+constexpr int kTile = 64;        // keys of a plan's tile, and of the expanded form's
 constexpr float kNone = -3e38f;  // below every score
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLarge = 0x1p19f;  // scores from here on (in log2) hold few fractions
@@ -56,9 +55,6 @@ struct Half<true> {
   static __device__ __forceinline__ f32x4_v mul32(u32x4_v a, u32x4_v b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ f32x4_v mul16(short4_v a, uint2 b, f32x4_v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, __builtin_bit_cast(short4_v, b), c, 0, 0, 0);
-  }
   static __device__ __forceinline__ f32x16_v mul(u32x4_v a, u32x4_v b, f32x16_v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0, 0, 0);
   }
@@ -76,9 +72,6 @@ struct Half<false> {
   static constexpr uint32_t exponent = 0x7c00u;
   static __device__ __forceinline__ f32x4_v mul32(u32x4_v a, u32x4_v b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_v, a), __builtin_bit_cast(half8_v, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x4_v mul16(short4_v a, uint2 b, f32x4_v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4_v, a), __builtin_bit_cast(half4_v, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ f32x16_v mul(u32x4_v a, u32x4_v b, f32x16_v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_v, a), __builtin_bit_cast(half8_v, b), c, 0, 0, 0);
@@ -99,17 +92,6 @@ __device__ __forceinline__ float sum2(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-__device__ __forceinline__ float max4(float x) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
-  x = max2(x);
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float sum4(float x) {
-  x = sum2(x);
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
@@ -141,7 +123,9 @@ struct LatentAppend {
 };
 
 // A thread moves 16 bytes of a token's latent, or turns 16 dims of its rope
-// key; the workgroups behind turn the queries.
+// key; the workgroups behind turn the queries.  It moves memory and nothing else bounds
+// it; a decode step's is smaller than a launch (256 requests, 32 heads: 10 us with the
+// host's share, 300 as five calls of the library with the rotation written out).
 template <int T>
 __global__ __launch_bounds__(256) void latent_append_kernel(LatentAppend d) {
   const uint32_t block = blockIdx.x;
@@ -179,7 +163,10 @@ __global__ __launch_bounds__(256) void latent_append_kernel(LatentAppend d) {
 }
 
 // Rows of all requests, request after request, 64 of them a workgroup, which
-// sums the requests' lengths for itself.
+// sums the requests' lengths for itself, so that nothing is read back and one launch does:
+// a workgroup reads up to 16 KB of lengths from its L2 beside 72 KB of rows.  Each row
+// is read and written once (6 requests of up to 9100, 32,000 rows in all: 19 us,
+// 4 TB/s; a copy of as much 15).
 constexpr int kGatherRows = 64;
 
 __global__ __launch_bounds__(256) void latent_gather_kernel(sq_latent_cache c, sq_latent_gather_args a) {
@@ -272,10 +259,6 @@ __device__ __forceinline__ void to_lds_once(uint32_t lds, const uint8_t *base, u
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-__device__ __forceinline__ void to_lds(uint32_t lds, const void *lane_at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(lane_at) : "memory");
-}
-
 // a word that the whole wave reads and no kernel running beside writes, by the scalar cache
 __device__ __forceinline__ int uniform_word(const int32_t *p) {
   return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p;
@@ -284,13 +267,6 @@ __device__ __forceinline__ int uniform_word(const int32_t *p) {
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // until at most N are under way
   asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
-}
-
-// until at most N are under way, or none where fewer may be
-template <int N>
-__device__ __forceinline__ void wait_ring(bool some) {
-  if (N && some) wait_loads<N>();
-  else wait_loads<0>();
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) {
@@ -340,9 +316,19 @@ __device__ __forceinline__ void store4(uint16_t *dst, f32x4_v x) {
 // out[t, h] = sum_j softmax_j(scale (q[t, h] . c_j + q_rope[t, h] . r_j)) c_j: one
 // key and value for all heads, so a row is a token's head and the rows of a
 // token share every key that is read.  S^T = K Q^T and O^T = C^T P^T run as matrix
-// products whose columns are rows of queries: a lane keeps scores, statistics
-// and outputs of one row, and the rounded weights of the first product are the
-// operand of the second without leaving their registers.
+// products whose columns are rows of queries, and the softmax by rows between them.
+//
+// Weights are rounded to the cache's type for the second product, by 2^-8 (bf16) or
+// 2^-11 of each at most, and their sum is that of the rounded ones, so that the error is
+// of the spread of the values alone; scores, sums and outputs are held in 32 bits.
+//
+// What bounds it: with up to 32 rows (a decode step of 32 heads) the pages, 1152 bytes a token
+// that are read once.  64 requests of up to 8191 take 69 us, 4.9 TB/s; of equal lengths
+// it is 5.9 (16 heads 6.5; a large copy reaches 5, reading alone 6.5).  What is missing are
+// units' starts, which wait for queries and first tiles.  With 128 rows (32 requests of up to
+// 16,383: 144 us) it is the two steps below, 0.7 us each of a tile of 32 keys, in
+// which the matrix cores are busy for a third of the time: each waits for the barrier,
+// for its weights and first operands from LDS, and for its last scores.
 
 struct AbsorbedDev {
   sq_latent_cache c;
@@ -762,6 +748,12 @@ __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
 // step apart: while one issues its products (the tile before's values, this tile's
 // keys), the other one's vector instructions (the softmax) have the SIMD.  A barrier ends
 // each step.  The late half loads.
+//
+// It is bound by the products: a prompt of 8192 tokens and 16 heads of 128 + 64 dims takes
+// 353 us, 974 TFLOP/s (16,384 tokens of 8 heads 645 us, 1066; a large matrix product of the
+// library reaches 1364); less is reached where rows do not fill sets of 256 or
+// see few tiles, whose starts nothing covers (2048 tokens 59 us, 733; 700 and 1100
+// tokens behind 12,000 176 us).
 
 struct ExpandedDev {
   const uint16_t *q, *k, *v, *rope;

@@ -191,3 +191,20 @@ def test_keys_turned_from_rows_that_are_copied():
     assert torch.equal(rotary.apply(q, plan.positions), want)
     assert torch.equal(cache.append(x[:, :256], x[:, 256:], plan, rotary=rotary, q=q), want)
     assert torch.equal(kv.append(x[:, :128], x[:, 128:256], plan, rotary=rotary, q=q), want)
+
+
+def test_queries_beside_more_workgroups_than_they_need():
+    """2048 KV heads and 8200 rows of padding launch over 2^24 workgroups for keys, and as
+    many for the queries, which are turned once all the same."""
+    heads, tokens = 2048, 8200
+    tables, kv, rotary = BlockTables(4096, 4, 1), KVCache(4, heads, 64), Rotary(16)
+    counts = torch.zeros(4096, dtype=torch.int32, device=dev())
+    counts[5] = 3
+    plan = tables.plan(counts, tokens=tokens, max_new=3)
+    assert plan.max_tiles * heads >= 1 << 24
+    k = torch.ones(tokens, 1, 64, dtype=torch.bfloat16, device=dev()).expand(tokens, heads, 64)
+    q = randn(gen(1), tokens, 9, 64)
+    want = rotary.apply(q, plan.positions)
+    assert not torch.equal(want, q)
+    assert kv.append(k, k, plan, rotary=rotary, q=q, out=q) is not None
+    assert torch.equal(q, want)
