@@ -4,8 +4,9 @@ Mirrors the reference package's operator surface: ``stepquant_amd.kernels.pool``
 ``stepquant_amd.kernels.format_pool``, ``stepquant_amd.kernels.writeback``,
 ``stepquant_amd.formats``, ``stepquant_amd.packing``, ``stepquant_amd.quantization``
 and ``stepquant_amd.cli.fingerprint``, plus two serving hooks of its own in
-``stepquant_amd.sglang`` and ``stepquant_amd.kernels.kv_cache`` for the attention
-layers between the recurrent ones.  ``install_alias()`` binds the reference's
+``stepquant_amd.sglang`` and, for the attention layers between the recurrent ones,
+``stepquant_amd.kernels.kv_cache``, ``stepquant_amd.kernels.rotary`` and
+``stepquant_amd.kernels.latent_cache``.  ``install_alias()`` binds the reference's
 ``stepquant.*`` operator modules to these, so the reference's serving adapter
 imports them unchanged.
 """
