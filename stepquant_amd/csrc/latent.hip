@@ -752,8 +752,8 @@ __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
 // It is bound by the products: a prompt of 8192 tokens and 16 heads of 128 + 64 dims takes
 // 353 us, 974 TFLOP/s (16,384 tokens of 8 heads 645 us, 1066; a large matrix product of the
 // library reaches 1364); less is reached where rows do not fill sets of 256 or
-// see few tiles, whose starts nothing covers (2048 tokens 59 us, 733; 700 and 1100
-// tokens behind 12,000 176 us).
+// see few tiles, whose starts and partial results nothing covers (2048 tokens 60 us, 357
+// TFLOP/s; 4 chunks of up to 701 tokens over 12,000 175 us, 600).
 
 struct ExpandedDev {
   const uint16_t *q, *k, *v, *rope;

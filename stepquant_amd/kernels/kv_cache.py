@@ -249,14 +249,18 @@ class BlockTables:
     few_rows, few_work = 1 << 14, 3 << 16
 
     # Latent attention.  Absorbed, every head shares the one key: a set is rows of
-    # all heads of a few tokens, 16, 32, 64 or 128 as one request's new tokens fill them (the
-    # smallest that holds them; past 128 the keys are read once for every 128).  Expanded, a
-    # set is 256 tokens of one head.  One workgroup on a CU in all of them.  Where keys are
-    # cut matters little: absorbed, 1 to 4 least tiles and 2 to 16 for the parts are within 3%
-    # (one request of 1000 tokens 15 us, 64 of up to 8191 77 us, 32 of 128 heads 144 us);
-    # expanded, 2 to 8 and 8 to 24 as well (4 chunks over 12,000 tokens 176 us; not cut 594).
+    # all heads of a few tokens, the smallest of 16, 32, 64 and 128 that one request's new
+    # tokens fit (past 128 the keys are read once for every 128).  Requests of thousands of
+    # tokens with 16 heads take 68 us in sets of 16 (84 in sets of 64, 116 of 128), with
+    # 32 heads 80 of 32 (130 of 16, 84 of 64, 122 of 128), with 64 heads 96 of 64 (143 of
+    # 32, 137 of 128), with 128 heads 144 of 128 (162 of 64, 262 of 32); a request of 1000
+    # tokens 16 us in all.  Expanded, a set is 256 tokens of one head.  One workgroup on a CU.
+    # Cut keys: absorbed, 1 to 4 least tiles are alike, and 2 and 4 for the parts (one request
+    # of 1000 tokens 15.5 us, with 16 not cut 39); expanded, 4 to 16 for the parts (prompts of
+    # 8192 tokens 350 us, with 2, cut, 417; of 2048 60 us, with 24, not cut, 80; with 16 one of 1024
+    # 48 us, with 8 30) and least tiles of 4 (of 1024 30 us, with 2 33).
     latent_min_tiles, latent_cut_tiles = 2, 4
-    expanded_min_tiles, expanded_cut_tiles = 4, 16
+    expanded_min_tiles, expanded_cut_tiles = 4, 8
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows, absorbed=None, expanded=None):
         """Where a plan's parts lie in its 32-bit words: (sizes of the parts, all

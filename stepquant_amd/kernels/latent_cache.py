@@ -40,10 +40,7 @@ ROPE = 64
 def _whole(x):
     """``x`` with a last dim that is contiguous and other strides and a start of whole 16 bytes (a copy where it has not)."""
     s = x.stride()
-    bits = 0
-    for n in s[:-1]:
-        bits |= n
-    if s[-1] != 1 or bits & 7 or min(s) < 0 or x.data_ptr() % 16:
+    if s[-1] != 1 or (s[0] | s[-2]) & 7 or x.data_ptr() % 16:  # (of two or three dims)
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -62,7 +59,7 @@ def _scale(scale):
 
 def _output(out, shape, like):
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(shape)
     if out.shape != shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous {list(shape)} of the queries' type")
@@ -94,6 +91,7 @@ class LatentCache:
         self._latent = N.LatentCache(data=self.data.data_ptr(), num_pages=pages, latent=latent_dim, rope=rope_dim,
                                      page_tokens=page_tokens, dtype=_HALVES[dtype])
         self._at = ctypes.addressof(self._latent)
+        self._words = torch.empty(0, dtype=torch.float32, device=self.device)  # workspaces are made like it
         # page copies read only these
         self.page_bytes = 2 * page_tokens * (latent_dim + rope_dim)
         self._desc = N.Pool(data=self.data.data_ptr(), page_bytes=self.page_bytes, num_slots=pages)
@@ -172,9 +170,9 @@ class LatentCache:
         tokens = int(tokens)
         if not 0 <= tokens <= 0x7fffffff:
             raise ValueError("tokens must be a non-negative 32-bit number")
-        latent = torch.empty((tokens, self.latent_dim), dtype=self.dtype, device=self.device)
-        rope = torch.empty((tokens, self.rope_dim), dtype=self.dtype, device=self.device)
-        starts = torch.empty(plan.batch + 1, dtype=torch.int32, device=self.device)
+        latent = self.data.new_empty((tokens, self.latent_dim))
+        rope = self.data.new_empty((tokens, self.rope_dim))
+        starts = plan._ints.new_empty((plan.batch + 1,))
         t = plan.tables
         args = N.LATENT_GATHER.pack(plan.rows.data_ptr(), plan._lens, t.table.data_ptr(), latent.data_ptr(),
                                     rope.data_ptr(), starts.data_ptr(), t.requests, tokens, plan.batch, t.max_blocks,
@@ -205,7 +203,7 @@ class LatentCache:
         q = self._like(q, (plan.tokens, s.q_heads, self.latent_dim), "queries")
         q_rope = self._like(q_rope, (plan.tokens, s.q_heads, self.rope_dim), "rope queries")
         scale, out = _scale(scale), _output(out, q.shape, q)
-        ws = torch.empty(s.floats * (self.latent_dim + 2), dtype=torch.float32, device=self.device)
+        ws = self._words.new_empty((s.floats * (self.latent_dim + 2),))
         t = plan.tables
         args = N.LATENT_ATTEND.pack(q.data_ptr(), q_rope.data_ptr(), out.data_ptr(), ws.data_ptr(), t.table.data_ptr(),
                                     t.requests, plan.tokens, *q.stride()[:2], *q_rope.stride()[:2], t.max_blocks, scale,

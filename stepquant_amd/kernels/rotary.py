@@ -106,30 +106,34 @@ class Rotary:
 
     def _rows(self, x, positions, positions_dtype, out):
         """(packed sq_rotary_rows, out, the rows that are read) of ``x`` [tokens, heads, head_dim]."""
-        if x.dtype not in N.FLOATS:
+        dtype = N.FLOATS.get(x.dtype)
+        if dtype is None:
             raise ValueError("rows must be fp32, bf16 or fp16")
         if x.device != self.device:
             raise ValueError("rows must be on the rotary's device")
         tokens, heads, dim = x.shape
         if dim < self.dim or dim % 8 or not 0 < heads <= 65536 or dim > 65536:
             raise ValueError(f"rows must have heads of at least {self.dim} dims, a multiple of 8")
-        whole = 3 if x.dtype == torch.float32 else 7
-        off = lambda y: (y.stride(2) != 1 or (y.stride(0) | y.stride(1)) & whole or y.stride(0) < 0 or y.stride(1) < 0
-                         or y.data_ptr() % 16)
+        whole = 3 if dtype == N.F32 else 7
+        off = lambda y, s: s[2] != 1 or (s[0] | s[1]) & whole or y.data_ptr() % 16
+        strides = x.stride()
+        copied = tokens and off(x, strides)
         if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=self.device)
+            out = x.new_empty((tokens, heads, dim)) if copied or not x.is_contiguous() else torch.empty_like(x)
+            os, oh = heads * dim, dim
         else:
             if out.dim() == 2 and out.shape == (tokens, heads * dim) and out.stride(1) == 1:
                 out = out.unflatten(1, (heads, dim))
             if out.shape != x.shape or out.dtype != x.dtype or out.device != self.device:
                 raise ValueError("out must be like the rows")
-            if tokens and (off(out) or (tokens > 1 and out.stride(0) == 0) or (heads > 1 and out.stride(1) == 0)):
+            os, oh, _ = out.stride()
+            if tokens and (off(out, out.stride()) or (tokens > 1 and os == 0) or (heads > 1 and oh == 0)):
                 raise ValueError("out must have heads that are contiguous inside, and strides and a start of whole 16 bytes")
-        if tokens and off(x):
+        if copied:
             x = x.clone(memory_format=torch.contiguous_format)
-        (xs, xh, _), (os, oh, _) = x.stride(), out.stride()
-        return N.ROTARY_ROWS.pack(x.data_ptr(), out.data_ptr(), positions, tokens, xs, xh, os, oh, heads, dim,
-                                  N.FLOATS[x.dtype], positions_dtype), out, x
+            strides = x.stride()
+        return N.ROTARY_ROWS.pack(x.data_ptr(), out.data_ptr(), positions, tokens, strides[0], strides[1], os, oh, heads,
+                                  dim, dtype, positions_dtype), out, x
 
     def apply(self, x, positions, *, out=None):
         """``x`` [tokens, heads, head_dim] (fp32, bf16 or fp16) turned to
