@@ -486,15 +486,16 @@ typedef struct sq_kv_schedule {
     int32_t max_partials;
     int32_t q_heads;
     int32_t kv_heads;
-    int32_t rows;         /* 16, 32 or 256 (latent attention: see there) */
+    int32_t rows;         /* 16, 32 or 256 (latent attention: 16 to 128, expanded 256) */
     int32_t causal;
     int32_t window;       /* 0: none; else the last `window` keys (causal only) */
     int32_t slots;        /* workers times KV heads that the device holds at once, at most 4096 */
     int32_t min_tiles;    /* least 64-key tiles of a worker, at least 1 */
     int32_t cut_tiles;    /* what a cut costs, in tiles of work */
     int32_t merge_rows;   /* most rows of a unit: min(rows, max_count * G) */
-    int32_t few_work;     /* 0, or for 256 rows: a plan of at most so many query rows (of all
-                             heads) times tiles that they see takes 32 (sets as of 32) */
+    int32_t few_work;     /* 0, or for 64 rows and more: a plan of at most so many query rows (of all
+                             heads) times tiles that they see takes 32 (sets as of 32, and
+                             twice the slots of 128 rows) */
     int32_t few_min_tiles;  /* min_tiles and cut_tiles then */
     int32_t few_cut_tiles;
 } sq_kv_schedule;

@@ -190,7 +190,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   uint32_t sum = 0;
   const int items = (NB + kPlanThreads - 1) / kPlanThreads;
   Scan scan;
-  int rows = s.rows, min_tiles = s.min_tiles, cut_tiles = s.cut_tiles;
+  int rows = s.rows, min_tiles = s.min_tiles, cut_tiles = s.cut_tiles, all_slots = s.slots;
   if (s.few_work > 0) {
     // query rows times the tiles that they see, about: little work goes to sets of 32
 #pragma unroll 1
@@ -204,7 +204,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
       }
     }
     scan = block_scan(sum);
-    if (scan.all <= (uint32_t)s.few_work) rows = 32, min_tiles = s.few_min_tiles, cut_tiles = s.few_cut_tiles;
+    if (scan.all <= (uint32_t)s.few_work) rows = 32, min_tiles = s.few_min_tiles, cut_tiles = s.few_cut_tiles, all_slots <<= s.rows == 128;
     sum = 0;
   }
 #pragma unroll 1
@@ -241,7 +241,7 @@ __device__ void plan_schedule(const sq_kv_schedule &s, const sq_kv_plan_args &p,
   const uint32_t tiles = block_scan(sum).all;  // (its barriers stand behind the atomics, too)
   most = bounds[0], least = bounds[1];
   // worker w has the tiles from w * share on
-  const uint32_t slots = max(1, s.slots / s.kv_heads), share = max((uint32_t)min_tiles, (tiles + slots - 1) / slots);
+  const uint32_t slots = max(1, all_slots / s.kv_heads), share = max((uint32_t)min_tiles, (tiles + slots - 1) / slots);
   // tiles until the last slot is done, either way
   const uint32_t whole = (uint32_t)sets <= slots ? most : max(most, (tiles + slots - 1) / slots + least);
   const bool dealt = share + cut_tiles < whole && tiles < kMost;
@@ -1829,10 +1829,13 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
     return fail(SQ_EINVAL, "kv schedule: min_tiles, cut_tiles or merge_rows");
   const int64_t G = s->q_heads / s->kv_heads;
   if (tokens * G > 0x3fffffff) return fail(SQ_EINVAL, "kv schedule: tokens * heads of a group too large");
-  if (s->few_work < 0 || (s->few_work > 0 && (s->rows != 256 || s->few_min_tiles <= 0 || s->few_cut_tiles < 0)))
+  if (s->few_work < 0 || (s->few_work > 0 && (s->rows < 64 || s->few_min_tiles <= 0 || s->few_cut_tiles < 0)))
     return fail(SQ_EINVAL, "kv schedule: few_work, few_min_tiles or few_cut_tiles");
+  // (two workgroups of sets of 128 rows become one each of sets of 32)
+  const int twice = s->few_work > 0 && s->rows == 128 ? 2 : 1;
+  if (s->slots * twice > kMaxSlots) return fail(SQ_EINVAL, "kv schedule: slots must be in [1, 4096]");
   const int64_t least = s->few_work > 0 ? 32 : s->rows, sets = (tokens * G + least - 1) / least + batch + 1;
-  const int64_t slots = s->slots / s->kv_heads > 1 ? s->slots / s->kv_heads : 1;
+  const int64_t slots = s->slots * twice / s->kv_heads > 1 ? s->slots * twice / s->kv_heads : 1;
   const int64_t larger = sets > slots ? sets : slots, smaller = sets < slots ? sets : slots;
   if (s->max_workers < larger || s->max_units < sets + slots || s->max_merges < smaller ||
       s->max_partials < 2 * slots || s->max_units >= 1 << 24)

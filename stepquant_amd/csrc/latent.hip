@@ -386,7 +386,7 @@ struct Absorbed {
 };
 
 template <typename S, bool BF16>
-__global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(AbsorbedDev a) {
+__device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
   typedef Half<BF16> H;
   constexpr int W = S::W, TK = S::TK, RG = S::RG, NR = S::NR, NW = S::NW, RING = S::RING, TILE = S::TILE, R = S::R;
   constexpr int KD = W + kRope, ROW = 2 * KD, KS = KD / (S::HALVES ? 64 : 32), DB = W / 64;
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int rg = wave >> 2, share = wave & 3, kg = wave & 1, half = wave >> 1 & 1;
   const bool late = RG == 2 && rg == 1, loads = rg == RG - 1;
-  const int worker = S::PAIR ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x;
+  const int worker = S::PAIR ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : (int)blockIdx.x;
   const int at_row = S::PAIR ? R * (blockIdx.x >> 3 & 1) : 0;
   if (worker >= a.max_workers) return;
   const int unit0 = max(0, uniform_word(a.starts + worker)), unit1 = min(uniform_word(a.starts + worker + 1), a.max_units);
@@ -695,6 +695,17 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
     }
     __syncthreads();  // before the next unit's weights
   }
+}
+
+// Plans of sets of 64 and 128 may hold sets of 32 instead, where there is little work.
+template <typename S, bool BF16>
+__global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(AbsorbedDev a) {
+  if constexpr (S::NR > 1) {
+    typedef Absorbed<S::W, 2, 1> Few;
+    static_assert(Few::threads == S::threads && Few::lds <= S::lds, "one launch for both");
+    if (uniform_word(a.starts + a.max_workers + 1) == Few::R) return absorbed_attend<Few, BF16>(a);
+  }
+  absorbed_attend<S, BF16>(a);
 }
 
 // Joins the parts of query rows whose keys were cut: one workgroup per merge, row and
@@ -1255,7 +1266,7 @@ int sq_latent_attend(const sq_latent_cache *c, const sq_latent_attend_args *a, v
   const sq_kv_schedule &s = a->schedule;
   rc = sq_internal_check_schedule(&s, a->tokens, 1);
   if (rc) return rc;
-  if (s.kv_heads != 1 || s.window || s.few_work || (s.rows != 16 && s.rows != 32 && s.rows != 64 && s.rows != 128))
+  if (s.kv_heads != 1 || s.window || (s.rows != 16 && s.rows != 32 && s.rows != 64 && s.rows != 128))
     return fail(SQ_ESHAPE, "latent attend: the schedule is for another kind of attention");
   if (!a->workspace || ((uintptr_t)a->workspace & 15)) return fail(SQ_EINVAL, "latent attend: null or misaligned workspace");
   const AbsorbedDev d = {*c, (const uint16_t *)a->q, (const uint16_t *)a->q_rope, (uint16_t *)a->out, a->workspace, a->table,

@@ -249,17 +249,23 @@ class BlockTables:
     few_rows, few_work = 1 << 14, 3 << 16
 
     # Latent attention.  Absorbed, every head shares the one key: a set is rows of
-    # all heads of a few tokens, the smallest of 16, 32, 64 and 128 that one request's new
-    # tokens fit (past 128 the keys are read once for every 128).  Requests of thousands of
+    # all heads of a few tokens, the smallest of 16, 32 and 64 that one request's new
+    # tokens fit, 64 past it, and 128 where one token has more than 96 heads, so that such sets
+    # are full.  Requests of thousands of
     # tokens with 16 heads take 68 us in sets of 16 (84 in sets of 64, 116 of 128), with
     # 32 heads 80 of 32 (130 of 16, 84 of 64, 122 of 128), with 64 heads 96 of 64 (143 of
-    # 32, 137 of 128), with 128 heads 144 of 128 (162 of 64, 262 of 32); a request of 1000
-    # tokens 16 us in all.  Expanded, a set is 256 tokens of one head.  One workgroup on a CU.
+    # 32, 137 of 128), with 128 heads 144 of 128 (162 of 64, 262 of 32); drafts of up to
+    # 4 and 32 heads 81 of 64 (100 of 128).  Little work ends sooner in sets of 32,
+    # all at a time; the plan kernel, which knows the lengths, takes them for at most
+    # `latent_few_work` query rows times the tiles that they see.  In sets of 32 and of
+    # 64 or 128: 2^11 17 and 22 us, 2^14 34 and 36, 2^15.4 27.5 and 30.4 (256 dims), 2^16.1
+    # 53 and 49, 2^17 108 and 79.  Expanded, a set is 256 tokens of one head.  One
+    # workgroup on a CU; a set of 128 has two.
     # Cut keys: absorbed, 1 to 4 least tiles are alike, and 2 and 4 for the parts (one request
     # of 1000 tokens 15.5 us, with 16 not cut 39); expanded, 4 to 16 for the parts (prompts of
     # 8192 tokens 350 us, with 2, cut, 417; of 2048 60 us, with 24, not cut, 80; with 16 one of 1024
     # 48 us, with 8 30) and least tiles of 4 (of 1024 30 us, with 2 33).
-    latent_min_tiles, latent_cut_tiles = 2, 4
+    latent_min_tiles, latent_cut_tiles, latent_few_work = 2, 4, 3 << 14
     expanded_min_tiles, expanded_cut_tiles = 4, 8
 
     def _layout(self, batch, tokens, max_new, heads, causal, windows, absorbed=None, expanded=None):
@@ -271,9 +277,11 @@ class BlockTables:
         sizes = [2 * most, batch + 1, tokens, batch, -(-batch // 4), most, most]
         schedules = []
 
-        def add(key, window, q_heads, kv_heads, rows, slots, min_tiles, cut_tiles, few=False):
+        def add(key, window, q_heads, kv_heads, rows, slots, min_tiles, cut_tiles, few=0, few_min=0, few_cut=0):
             group = q_heads // kv_heads
             sets, cuts = -(-tokens * group // (32 if few else rows)) + batch + 1, max(1, slots // kv_heads)
+            if few and rows == 128:  # (two workgroups a set, or one a set of 32)
+                cuts = max(1, 2 * slots // kv_heads)
             workers, joins = max(sets, cuts), min(sets, cuts)
             if not schedules:
                 sizes.append(-sum(sizes) % 8)  # units and merges start on a boundary of their 32 bytes
@@ -281,7 +289,7 @@ class BlockTables:
             merges = units + 32 * (sets + cuts)
             numbers = (sets + cuts, joins, workers, 2 * cuts, q_heads, kv_heads, rows, causal, window, slots,
                        min_tiles, cut_tiles, max(1, min(rows, max_new * group)),
-                       self.few_work if few else 0, self.min_tiles[32], self.cut_tiles[32])
+                       few, few_min, few_cut)
             schedules.append((key, q_heads, kv_heads, 2 * cuts * kv_heads * rows, units, merges, merges + 32 * joins,
                               numbers))
             sizes.append(8 * (sets + cuts + joins) + (workers + 9) // 8 * 8)
@@ -298,9 +306,10 @@ class BlockTables:
             rows = max_new * group
             rows = 16 if rows <= 16 else 32 if rows <= 64 else 256
             slots = 2 * self._cus if rows == 16 else self._cus
-            few = rows == 256 and tokens * q_heads <= self.few_rows
+            few = self.few_work if rows == 256 and tokens * q_heads <= self.few_rows else 0
             for w in windows if tokens else ():
-                add(int(w), int(w), q_heads, kv_heads, rows, slots, self.min_tiles[rows], self.cut_tiles[rows], few)
+                add(int(w), int(w), q_heads, kv_heads, rows, slots, self.min_tiles[rows], self.cut_tiles[rows], few,
+                    self.min_tiles[32], self.cut_tiles[32])
         for form, n in ("absorbed", absorbed), ("expanded", expanded):
             if n is None:
                 continue
@@ -310,9 +319,11 @@ class BlockTables:
                 continue
             if form == "absorbed":
                 rows = max_new * n
-                rows = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
+                rows = 16 if rows <= 16 else 32 if rows <= 32 else 64 if n <= 96 else 128
+                few = self.latent_few_work if rows > 32 and tokens * n <= self.few_rows else 0
                 # (one workgroup on a CU; sets of 128 have two)
-                add(form, 0, n, 1, rows, self._cus // (2 if rows == 128 else 1), self.latent_min_tiles, self.latent_cut_tiles)
+                add(form, 0, n, 1, rows, self._cus // (2 if rows == 128 else 1), self.latent_min_tiles, self.latent_cut_tiles,
+                    few, self.latent_min_tiles, self.latent_cut_tiles)
             else:
                 add(form, 0, n, n, 256, self._cus, self.expanded_min_tiles, self.expanded_cut_tiles)
         offsets = [4 * sum(sizes[:i]) for i in range(7)]

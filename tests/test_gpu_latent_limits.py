@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from stepquant_amd import _native as N
 from stepquant_amd.kernels.kv_cache import BlockTables, KVCache
 from stepquant_amd.kernels.latent_cache import LatentCache, expanded_attention
 from stepquant_amd.kernels.rotary import Rotary
@@ -15,10 +16,13 @@ from tests.test_gpu_latent import U, Batch, Prompts, attention64, gen, randn
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("heads", [4, 24, 40, 128])
+@pytest.mark.parametrize("heads,few", [(4, None), (24, None), (24, 1), (40, None), (40, 1), (128, None), (128, 1)])
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
-def test_cut_keys_with_numbers_that_are_none(heads, value):
-    """The last of a draft's tokens holds them: one part of its rows' keys is not finite."""
+def test_cut_keys_with_numbers_that_are_none(heads, few, value, monkeypatch):
+    """The last of a draft's tokens holds them: one part of its rows' keys is not finite.
+    ``few``: sets of 64 and 128 rows where plans would take 32."""
+    if few:
+        monkeypatch.setattr(BlockTables, "latent_few_work", few)
     b = Batch([(3000, 4), (900, 2)], heads=heads)
     clean = b.attend()
     b.check(clean)
@@ -43,6 +47,22 @@ def test_expanded_cut_keys_with_numbers_that_are_none(value):
     y = p.attend()
     assert torch.equal(y[:50, 0], clean[:50, 0]) and torch.equal(y[:70, 1], clean[:70, 1]) and torch.equal(y[100:], clean[100:])
     assert not torch.isfinite(y[50:100, 0, 9]).any() and torch.isnan(y[70:100, 1]).all()
+
+
+@pytest.mark.parametrize("heads,sizes", [(64, [(70, 1), (0, 2), (3, 1)]), (128, [(200, 1), (0, 1)]), (20, [(300, 4), (61, 3)]),
+                                         (128, [(3000, 1)]), (110, [(5, 1), (64, 2)])])
+def test_sets_that_the_work_decides(heads, sizes, monkeypatch):
+    """Little work runs in sets of 32 rows, the same work in others where the choice is
+    taken away: both are right, and of masks and padding alike."""
+    few = BlockTables.latent_few_work
+    for most in (few, 1):
+        monkeypatch.setattr(BlockTables, "latent_few_work", most)
+        for causal in (True, False):
+            b = Batch(sizes, heads=heads, padding=2, causal=causal, latent=256 if heads == 64 else 512)
+            fields = N.KV_SCHEDULE.unpack(b.plan.latent["absorbed"].packed)
+            starts, workers = (fields[2] - b.plan._ints.data_ptr()) // 4, fields[5]
+            assert int(b.plan._ints[starts + workers + 1]) == (32 if most == few else 128 if heads > 96 else 64)
+            b.check(b.attend())
 
 
 def test_more_requests_than_lanes():
@@ -135,9 +155,12 @@ def test_other_streams():
         del b
 
 
-def test_two_graphs_in_turn():
+@pytest.mark.parametrize("few", [None, 1])
+def test_two_graphs_in_turn(few, monkeypatch):
     """Two graphs of one pool, whose workspaces share memory, replayed in turn and beside eager calls."""
-    a, b = Batch([(2000, 1), (700, 1)], heads=16, seed=1), Batch([(1500, 3)], heads=40, seed=2)
+    if few:
+        monkeypatch.setattr(BlockTables, "latent_few_work", few)
+    a, b = Batch([(2000, 1), (700, 1)], heads=16, seed=1), Batch([(1500, 3)], heads=128, seed=2)
     want = a.attend(), b.attend()
     pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
     side = torch.cuda.Stream()
