@@ -708,11 +708,12 @@ __global__ __launch_bounds__(S::threads, S::RG) void latent_attend_kernel(Absorb
   absorbed_attend<S, BF16>(a);
 }
 
-// Joins the parts of query rows whose keys were cut: one workgroup per merge, row and
-// 4 * L dims; L lanes read a part, 512 / L parts at a time.
-template <int W, int L, bool BF16>
+// Joins the parts of query rows whose keys were cut.  Few rows (a long sequence by itself,
+// hundreds of parts): one workgroup per merge, row and 128 dims; 32 lanes read a part,
+// 16 parts at a time.
+template <int W, bool BF16>
 __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
-  constexpr int GR = 512 / L;
+  constexpr int L = 32, GR = 512 / L;
   __shared__ f32x4_v part_o[GR][L];
   __shared__ float2 part_s[GR];
   const int tid = threadIdx.x, j = blockIdx.y, lane = tid % L, grp = tid / L, d = 4 * (L * (int)blockIdx.z + lane);
@@ -747,6 +748,38 @@ __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
     sum = fmaf(part_s[i].y, w, sum);
   }
   store4<BF16>(a.out + (q0 * (int64_t)a.heads + f0 + j) * W + d, x * (sum == 0.f ? 0.f : 1.f / sum));
+}
+
+// The same of many rows, with a few parts each: a wave a row, so that a plan's merges that there
+// are none of cost little (4608 of 128 rows: 10 us with a workgroup a row, 3 so).
+template <int W, bool BF16>
+__global__ __launch_bounds__(512) void latent_merge_rows_kernel(AbsorbedDev a) {
+  constexpr int N = W / 256;
+  const int j = 8 * blockIdx.y + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int32_t *u = a.merges + 8 * (int64_t)blockIdx.x;
+  const int q0 = u[0], f0 = u[1], rows = u[2], p0 = u[3], n = u[4];
+  if (j >= rows) return;
+  const float *ml = a.ws + (int64_t)a.max_partials * a.unit_rows * W;
+  f32x4_v x[N];
+#pragma unroll
+  for (int k = 0; k < N; k++) x[k] = (f32x4_v){0, 0, 0, 0};
+  float sum = 0, mm = kNone;
+#pragma unroll 4
+  for (int i = 0; i < n; i++) {
+    const int64_t slot = (int64_t)(p0 + i) * a.unit_rows + j;
+    const float2 stat = *(const float2 *)(ml + 2 * slot);
+    f32x4_v y[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) y[k] = *(const f32x4_v *)(a.ws + slot * W + 4 * lane + 256 * k);
+    const float high = fmaxf(mm, stat.x), was = __builtin_amdgcn_exp2f(mm - high), w = __builtin_amdgcn_exp2f(stat.x - high);
+    mm = high;
+    sum = fmaf(sum, was, stat.y * w);
+#pragma unroll
+    for (int k = 0; k < N; k++) x[k] = x[k] * was + y[k] * w;
+  }
+  uint16_t *dst = a.out + (q0 * (int64_t)a.heads + f0 + j) * W + 4 * lane;
+#pragma unroll
+  for (int k = 0; k < N; k++) store4<BF16>(dst + 256 * k, x[k] * (sum == 0.f ? 0.f : 1.f / sum));
 }
 
 // ------------------------------------------------------------ expanded
@@ -1174,9 +1207,9 @@ int launch_absorbed(const AbsorbedDev &d, const sq_kv_schedule &s, hipStream_t s
                                 : go(latent_attend_kernel<S128, BF16>, 3, S128{});
   if (rc) return rc;
   if ((int64_t)s.max_merges * s.merge_rows <= 256)
-    hipLaunchKernelGGL((latent_merge_kernel<W, 32, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows, W / 128), dim3(512), 0, st, d);
+    hipLaunchKernelGGL((latent_merge_kernel<W, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows, W / 128), dim3(512), 0, st, d);
   else
-    hipLaunchKernelGGL((latent_merge_kernel<W, W / 4, BF16>), dim3((unsigned)s.max_merges, (unsigned)s.merge_rows), dim3(512), 0, st, d);
+    hipLaunchKernelGGL((latent_merge_rows_kernel<W, BF16>), dim3((unsigned)s.max_merges, (unsigned)(s.merge_rows + 7) / 8), dim3(512), 0, st, d);
   return sq_internal_launched("latent_merge_kernel");
 }
 

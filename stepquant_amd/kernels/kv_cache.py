@@ -257,7 +257,8 @@ class BlockTables:
     # 32, 137 of 128), with 128 heads 144 of 128 (162 of 64, 262 of 32); drafts of up to
     # 4 and 32 heads 81 of 64 (100 of 128).  Little work ends sooner in sets of 32,
     # all at a time; the plan kernel, which knows the lengths, takes them for at most
-    # `latent_few_work` query rows times the tiles that they see.  In sets of 32 and of
+    # `latent_few_work` query rows times the tiles that they see, unless there are more
+    # sets than CUs (108 requests of 80 tokens, 128 heads: 44 us, 36 in sets of 128).  In sets of 32 and of
     # 64 or 128: 2^11 17 and 22 us, 2^14 34 and 36, 2^15.4 27.5 and 30.4 (256 dims), 2^16.1
     # 53 and 49, 2^17 108 and 79.  Expanded, a set is 256 tokens of one head.  One
     # workgroup on a CU; a set of 128 has two.
@@ -320,7 +321,7 @@ class BlockTables:
             if form == "absorbed":
                 rows = max_new * n
                 rows = 16 if rows <= 16 else 32 if rows <= 32 else 64 if n <= 96 else 128
-                few = self.latent_few_work if rows > 32 and tokens * n <= self.few_rows else 0
+                few = self.latent_few_work if rows > 32 and tokens * n <= 32 * self._cus else 0
                 # (one workgroup on a CU; sets of 128 have two)
                 add(form, 0, n, 1, rows, self._cus // (2 if rows == 128 else 1), self.latent_min_tiles, self.latent_cut_tiles,
                     few, self.latent_min_tiles, self.latent_cut_tiles)
