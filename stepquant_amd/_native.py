@@ -322,6 +322,15 @@ def raw_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def stream_on(device: torch.device) -> int:
+    """The current stream as a number; ``device`` has to be the current one: a
+    kernel would run on another one than its operands'."""
+    current = torch._C._cuda_getDevice()
+    if current != device.index:
+        raise ValueError(f"the operands are on {device}, the current device is cuda:{current}")
+    return torch._C._cuda_getCurrentRawStream(current)
+
+
 def stream_handle(stream=None) -> ctypes.c_void_p:
     s = torch.cuda.current_stream() if stream is None else stream
     return ctypes.c_void_p(s.cuda_stream)

@@ -458,7 +458,8 @@ class KVCache:
         if rotary is None:
             rc = N.kv_entry("sq_kv_append")(self._at, args, N.raw_stream())
         else:
-            rc = N.kv_entry("sq_kv_append_rotary")(self._at, args, plan._positions, rotary._at, rows, N.raw_stream())
+            rc = N.kv_entry("sq_kv_append_rotary")(self._at, args, plan._positions, rotary._at, rows,
+                                                   N.stream_on(self.device))
         if rc:
             N.check(rc, "kv append")
         return out

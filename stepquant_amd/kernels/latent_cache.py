@@ -150,7 +150,7 @@ class LatentCache:
             return out
         args = N.LATENT_APPEND.pack(latent.data_ptr(), rope.data_ptr(), plan._slots, plan._positions, plan.tokens,
                                     latent.stride(0), rope.stride(0))
-        rc = N.kv_entry("sq_latent_append")(self._at, args, None if rotary is None else rotary._at, rows, N.raw_stream())
+        rc = N.kv_entry("sq_latent_append")(self._at, args, None if rotary is None else rotary._at, rows, N.stream_on(self.device))
         if rc:
             N.check(rc, "latent append")
         return out
@@ -177,7 +177,7 @@ class LatentCache:
         args = N.LATENT_GATHER.pack(plan.rows.data_ptr(), plan._lens, t.table.data_ptr(), latent.data_ptr(),
                                     rope.data_ptr(), starts.data_ptr(), t.requests, tokens, plan.batch, t.max_blocks,
                                     N.INTS[plan.rows.dtype], 0)
-        rc = N.kv_entry("sq_latent_gather")(self._at, args, N.raw_stream())
+        rc = N.kv_entry("sq_latent_gather")(self._at, args, N.stream_on(self.device))
         if rc:
             N.check(rc, "latent gather")
         return latent, rope, starts
@@ -208,7 +208,7 @@ class LatentCache:
         args = N.LATENT_ATTEND.pack(q.data_ptr(), q_rope.data_ptr(), out.data_ptr(), ws.data_ptr(), t.table.data_ptr(),
                                     t.requests, plan.tokens, *q.stride()[:2], *q_rope.stride()[:2], t.max_blocks, scale,
                                     s.packed)
-        rc = N.kv_entry("sq_latent_attend")(self._at, args, N.raw_stream())
+        rc = N.kv_entry("sq_latent_attend")(self._at, args, N.stream_on(self.device))
         if rc:
             N.check(rc, "latent attend")
         return out
@@ -259,7 +259,7 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
     args = N.EXPANDED_ATTEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), out.data_ptr(), ws.data_ptr(), plan._cu,
                                   starts_at, plan.tokens, rows, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
                                   rope.stride(0), plan.batch, dim, _HALVES[v.dtype], scale, s.packed)
-    rc = N.kv_entry("sq_expanded_attend")(args, N.raw_stream())
+    rc = N.kv_entry("sq_expanded_attend")(args, N.stream_on(v.device))
     if rc:
         N.check(rc, "expanded attention")
     return out

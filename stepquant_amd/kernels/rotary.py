@@ -152,7 +152,7 @@ class Rotary:
             positions = positions.contiguous()
         rows, out, x = self._rows(x, positions.data_ptr(), N.INTS[positions.dtype], out)
         if x.shape[0]:
-            rc = N.kv_entry("sq_rotary_apply")(self._at, rows, N.raw_stream())
+            rc = N.kv_entry("sq_rotary_apply")(self._at, rows, N.stream_on(self.device))
             if rc:
                 N.check(rc, "rotary")
         return out

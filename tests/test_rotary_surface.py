@@ -98,6 +98,14 @@ def test_calls_are_checked_before_any_launch(rotary, rows):
     assert L.sq_kv_append_rotary(cache, a, 16, _rotary(**rotary), _rows(**rows), None) in (-22, -23)
 
 
+def test_launches_on_another_device_are_refused(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 40 + device, raising=False)
+    assert N.stream_on(torch.device("cuda", 1)) == 41
+    with pytest.raises(ValueError, match="cuda:0.*cuda:1"):
+        N.stream_on(torch.device("cuda", 0))
+
+
 def test_appends_refuse_rotations_that_do_not_fit():
     L = N.lib()
     cache = N.KVCache(data=4096, page_bytes=16512, num_pages=4, heads=2, dim=64, page_tokens=64, storage=N.KV_INT8)
