@@ -162,13 +162,14 @@ __global__ __launch_bounds__(256) void latent_append_kernel(LatentAppend d) {
   xa.store(dst, 8 * ga), xb.store(dst, 8 * gb);
 }
 
-// Rows of all requests, request after request, 64 of them a workgroup, which
+// Rows of all requests, request after request, 32 of them a workgroup, which
 // sums the requests' lengths for itself, so that nothing is read back and one launch does:
-// a workgroup reads up to 16 KB of lengths from its L2 beside 72 KB of rows.  Each row
-// is read and written once (6 requests of up to 9100, 32,000 rows in all: 19 us,
-// 4 TB/s; a copy of as much 15).
-constexpr int kGatherRows = 64;
+// a workgroup reads up to 16 KB of lengths from its L2 beside 36 KB of rows.  Each row
+// is read and written once, all of a thread's loads before its stores (6 requests of up to 9100, 32,000 rows
+// in all: 20 us, 3.7 TB/s with pages in any order; 25 with 64 rows a workgroup and four loads at a time).
+constexpr int kGatherRows = 32;
 
+template <int W>
 __global__ __launch_bounds__(256) void latent_gather_kernel(sq_latent_cache c, sq_latent_gather_args a) {
   extern __shared__ int64_t ends[];  // of the requests' rows, [batch]
   __shared__ int64_t waves[4];
@@ -214,15 +215,21 @@ __global__ __launch_bounds__(256) void latent_gather_kernel(sq_latent_cache c, s
     source[tid] = from;
   }
   __syncthreads();
-  const int W = c.latent, groups = (W + kRope) / 8;
+  constexpr int groups = (W + kRope) / 8, N = (kGatherRows * groups + 255) / 256;
   const int rows = (int)min((int64_t)kGatherRows, a.rows_out - first);
-#pragma unroll 4
-  for (int i = tid; i < rows * groups; i += 256) {
-    const int r = i / groups, g = i - r * groups;
-    const int64_t from = source[r];
-    const u32x4_v x = from < 0 ? (u32x4_v){0, 0, 0, 0} : *(const u32x4_v *)((const uint16_t *)c.data + from * (W + kRope) + 8 * g);
-    if (8 * g < W) *(u32x4_v *)((uint16_t *)a.latent + (first + r) * W + 8 * g) = x;
-    else *(u32x4_v *)((uint16_t *)a.rope + (first + r) * kRope + 8 * g - W) = x;
+  u32x4_v x[N];
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    const int i = 256 * k + tid, r = i / groups, g = i - r * groups;
+    const int64_t from = r < rows ? source[r] : -1;
+    x[k] = from < 0 ? (u32x4_v){0, 0, 0, 0} : *(const u32x4_v *)((const uint16_t *)c.data + from * (W + kRope) + 8 * g);
+  }
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    const int i = 256 * k + tid, r = i / groups, g = i - r * groups;
+    if (r >= rows) break;
+    if (8 * g < W) *(u32x4_v *)((uint16_t *)a.latent + (first + r) * W + 8 * g) = x[k];
+    else *(u32x4_v *)((uint16_t *)a.rope + (first + r) * kRope + 8 * g - W) = x[k];
   }
 }
 
@@ -1281,7 +1288,10 @@ int sq_latent_gather(const sq_latent_cache *c, const sq_latent_gather_args *a, v
   int64_t blocks = (a->rows_out + kGatherRows - 1) / kGatherRows;
   if (blocks < 1) blocks = 1;  // (starts)
   if (blocks >= 1 << 24) return fail(SQ_EINVAL, "latent gather: too many rows for one call");
-  hipLaunchKernelGGL(latent_gather_kernel, dim3((unsigned)blocks), dim3(256), sizeof(int64_t) * (size_t)a->batch, (hipStream_t)stream, *c, *a);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), sizeof(int64_t) * (size_t)a->batch, (hipStream_t)stream, *c, *a);
+  };
+  c->latent == 512 ? go(latent_gather_kernel<512>) : go(latent_gather_kernel<256>);
   return sq_internal_launched("latent_gather_kernel");
 }
 
