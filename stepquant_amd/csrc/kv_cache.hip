@@ -2009,7 +2009,7 @@ int sq_kv_append_rotary(const sq_kv_cache *c, const sq_kv_append_args *a, const 
     if (rc) return rc;
     q = *rows;
     lanes = q.heads;
-    const int64_t threads = q.tokens * lanes * (r->dim / 16), plane = (int64_t)a->max_tiles * c->heads;
+    const int64_t threads = q.tokens * lanes * rotary::row_items(*r, q, false), plane = (int64_t)a->max_tiles * c->heads;
     if (threads >= (int64_t)1 << 31) return fail(SQ_EINVAL, "kv append: too many queries for one call");
     z += ((threads + 255) / 256 + plane - 1) / plane;
     if (z > 65535) return fail(SQ_EINVAL, "kv append: too many queries for one call");

@@ -1266,7 +1266,7 @@ int sq_latent_append(const sq_latent_cache *c, const sq_latent_append_args *a, c
     if (rows->dtype != c->dtype) return fail(SQ_EINVAL, "latent append: queries have the cache's type");
     d.q = *rows;
     d.q_lanes = rows->heads;
-    const int64_t more = rows->tokens * rows->heads * (r->dim / 16);
+    const int64_t more = rows->tokens * rows->heads * rotary::row_items(*r, *rows, false);
     if (more >= (int64_t)1 << 31) return fail(SQ_EINVAL, "latent append: too many queries for one call");
     blocks += (more + 255) / 256;
   }

@@ -121,17 +121,28 @@ __device__ __forceinline__ int64_t position_of(const void *p, int dtype, int64_t
   return dtype == SQ_I64 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
 }
 
-// Thread `id` of the rows' `lanes * items` threads a token (lanes * PER >= heads):
-// 16 dims of PER heads, whose angles it computes once, and their share of the
-// dims that do not turn.
-template <int T, int PER>
+// Items of 16 dims of a head that threads of its own kernel take: those that turn and, unless rows
+// are turned in place, those that are copied, so that these have as many loads under way
+// (11,000 tokens of 16 heads of 256 dims, 64 of them turned: 40.7 us; 49.6 where threads that
+// turn copy what is left).  Beside appends they do, whose kernels have room for fewer
+// waves (those tokens with their keys 51.7 us, 55.8 with threads that copy).
+__host__ __device__ __forceinline__ int row_items(const sq_rotary &r, const sq_rotary_rows &a, bool copiers) {
+  return copiers && a.x != a.out ? (a.head_dim + 15) / 16 : r.dim / 16;
+}
+
+// Thread `id` of the rows' `lanes * row_items` threads a token (lanes * PER >= heads):
+// 16 dims of PER heads, whose angles it computes once, and without COPIERS its share of
+// the dims that do not turn.
+template <int T, int PER, bool COPIERS = false>
 __device__ __forceinline__ void rotate_rows_typed(const sq_rotary &r, const sq_rotary_rows &a, int lanes, uint32_t id) {
-  const uint32_t items = r.dim / 16, threads = lanes * items;
+  const uint32_t items = row_items(r, a, COPIERS), threads = lanes * items;
   const uint32_t token = id / threads, rest = id - token * threads, lane = rest / items, item = rest - lane * items;
   if (token >= a.tokens) return;
-  const int64_t position = position_of(a.positions, a.positions_dtype, token);
+  const bool turns = !COPIERS || item < (uint32_t)r.dim / 16;
+  const int64_t position = turns ? position_of(a.positions, a.positions_dtype, token) : -1;
   int ga, gb;
   groups(r, item, ga, gb);
+  const bool two = !COPIERS || 8 * gb < a.head_dim;  // (heads have whole groups of 8 dims)
   const int64_t from = token * a.x_stride, to = token * a.out_stride;
   Eight<T> xa[PER], xb[PER];
 #pragma unroll
@@ -139,7 +150,7 @@ __device__ __forceinline__ void rotate_rows_typed(const sq_rotary &r, const sq_r
     const int h = lane + k * lanes;
     if (h < a.heads) {
       xa[k].load(a.x, from + h * a.x_head_stride + 8 * ga);
-      xb[k].load(a.x, from + h * a.x_head_stride + 8 * gb);
+      if (two) xb[k].load(a.x, from + h * a.x_head_stride + 8 * gb);
     }
   }
   Angles t;
@@ -155,9 +166,9 @@ __device__ __forceinline__ void rotate_rows_typed(const sq_rotary &r, const sq_r
       xa[k].narrow(x), xb[k].narrow(x + 8);
     }
     xa[k].store(a.out, to + h * a.out_head_stride + 8 * ga);
-    xb[k].store(a.out, to + h * a.out_head_stride + 8 * gb);
+    if (two) xb[k].store(a.out, to + h * a.out_head_stride + 8 * gb);
   }
-  if (a.x == a.out) return;
+  if (COPIERS || a.x == a.out) return;
   const int n = a.head_dim / 8;
 #pragma unroll
   for (int k = 0; k < PER; k++) {
@@ -183,7 +194,7 @@ __device__ __forceinline__ void rotate_rows(const sq_rotary &r, const sq_rotary_
 // GPU all the same: 2^17 of 128 dims take 3.9 us so and 3.7 one by one, 2^18
 // 5.7 and 6.5, 2^20 12.0 and 16.4, 2^22 50 and 59 (5.4 TB/s; a copy reaches 5).
 inline int heads_per_thread(const sq_rotary *r, const sq_rotary_rows *a) {
-  return a->tokens * a->heads * (r->dim / 16) >= (int64_t)1 << 18 ? 4 : 1;
+  return a->tokens * a->heads * row_items(*r, *a, true) >= (int64_t)1 << 18 ? 4 : 1;
 }
 // threads that a token's heads are dealt out to, PER heads each
 inline int head_lanes(int heads, int per) { return (heads + per - 1) / per; }

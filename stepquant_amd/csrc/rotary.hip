@@ -9,7 +9,7 @@ namespace {
 // 5.4 TB/s); a decode step's rows take less than the launch (64 tokens: 2.8 us in a graph).
 template <int T, int PER>
 __global__ __launch_bounds__(256) void rotary_kernel(sq_rotary r, sq_rotary_rows a, int lanes) {
-  rotary::rotate_rows_typed<T, PER>(r, a, lanes, blockIdx.x * 256 + threadIdx.x);
+  rotary::rotate_rows_typed<T, PER, true>(r, a, lanes, blockIdx.x * 256 + threadIdx.x);
 }
 
 int fail(int code, const char *msg) { return sq_internal_fail(code, msg); }
@@ -36,6 +36,8 @@ int check_rows(const sq_rotary *r, const sq_rotary_rows *a) {
     return fail(SQ_EINVAL, "rotary: strides must be whole 16 bytes and starts 16-byte aligned");
   if (a->x_stride < 0 || a->x_head_stride < 0 || a->out_stride < 0 || a->out_head_stride < 0)
     return fail(SQ_EINVAL, "rotary: negative stride");
+  if (a->x == a->out && ((a->tokens > 1 && a->x_stride != a->out_stride) || (a->heads > 1 && a->x_head_stride != a->out_head_stride)))
+    return fail(SQ_EINVAL, "rotary: rows that are turned in place have one layout");
   return 0;
 }
 
@@ -48,7 +50,7 @@ extern "C" int sq_rotary_apply(const sq_rotary *r, const sq_rotary_rows *rows, v
   rc = rotary::check_rows(r, rows);
   if (rc) return rc;
   sq_rotary_rows a = *rows;
-  const int64_t items = r->dim / 16;
+  const int64_t items = rotary::row_items(*r, a, true);
   const bool many = rotary::heads_per_thread(r, rows) > 1;
   const int lanes = rotary::head_lanes(a.heads, rotary::heads_per_thread(r, rows));
   const int64_t threads = lanes * items, size = a.dtype == SQ_F32 ? 4 : 2;

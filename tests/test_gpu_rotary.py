@@ -261,3 +261,29 @@ def test_a_step_that_turns_replays():
         torch.cuda.synchronize()
         assert torch.equal(y[0], w[0]) and torch.equal(y[1], w[1])
     assert torch.equal(a[1].data, b[1].data) and a[0].lens.tolist() == b[0].lens.tolist()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("dim,n,layout", [(72, 16, "half"), (256, 64, "half"), (200, 128, "interleaved"), (64, 64, "half")])
+@pytest.mark.parametrize("tokens,heads", [(3, 2), (600, 9), (5000, 11)])
+def test_dims_that_do_not_turn_are_copied(tokens, heads, dim, n, layout, dtype):
+    """By threads of their own; the same rows in place, where they stay, and by the cache's launch."""
+    g = torch.Generator(device=dev()).manual_seed(dim + tokens)
+    x = torch.randn(tokens, heads, dim, generator=g, device=dev()).to(TYPES[dtype])
+    pos = torch.randint(-2, 70000, (tokens,), generator=g, device=dev())
+    rotary = Rotary(n, layout=layout, base=3e4)
+    y, z = rotary.apply(x, pos), x.clone()
+    assert torch.equal(y[..., n:], x[..., n:]) and torch.equal(y[pos < 0], x[pos < 0])
+    assert rotary.apply(z, pos, out=z) is z and torch.equal(y, z)
+    wide = torch.zeros(tokens, heads + 1, dim + 8, dtype=x.dtype, device=dev())
+    out = wide[:, :heads, 8:]
+    rotary.apply(x, pos, out=out)
+    assert torch.equal(out, y) and not wide[:, heads].any() and not wide[..., :8].any()
+
+
+def test_rows_in_place_have_one_layout():
+    rotary = Rotary(16)
+    x = torch.zeros(64, dtype=torch.bfloat16, device=dev())
+    a, b = x.as_strided((2, 2, 16), (32, 16, 1)), x.as_strided((2, 2, 16), (16, 32, 1))
+    with pytest.raises((ValueError, RuntimeError)):
+        rotary.apply(a, torch.zeros(2, dtype=torch.int64, device=dev()), out=b)

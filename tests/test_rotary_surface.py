@@ -84,7 +84,7 @@ BAD_ROTARY = [dict(turns=None), dict(turns=12), dict(dim=8), dict(dim=0), dict(d
               dict(magnitude=math.nan)]
 BAD_ROWS = [dict(x=None), dict(out=None), dict(positions=None), dict(tokens=-1), dict(x=24), dict(out=24), dict(heads=0),
             dict(head_dim=56), dict(head_dim=132), dict(dtype=N.I32), dict(positions_dtype=N.F32), dict(x_stride=508),
-            dict(x_head_stride=-128), dict(out_stride=-512), dict(out_head_stride=12)]
+            dict(x_head_stride=-128), dict(out_stride=-512), dict(out_head_stride=12), dict(x=16, out=16, out_stride=1024)]
 
 
 @pytest.mark.parametrize("rotary,rows", [(r, {}) for r in BAD_ROTARY] + [({}, r) for r in BAD_ROWS])
