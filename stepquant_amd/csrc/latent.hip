@@ -801,10 +801,10 @@ __global__ __launch_bounds__(512) void latent_merge_rows_kernel(AbsorbedDev a) {
 // each step.  The late half loads.
 //
 // It is bound by the products: a prompt of 8192 tokens and 16 heads of 128 + 64 dims takes
-// 353 us, 974 TFLOP/s (16,384 tokens of 8 heads 645 us, 1066; a large matrix product of the
+// 347 us, 990 TFLOP/s (16,384 tokens of 8 heads 645 to 663 us, 1036 to 1066; a large matrix product of the
 // library reaches 1364); less is reached where rows do not fill sets of 256 or
-// see few tiles, whose starts and partial results nothing covers (2048 tokens 60 us, 357
-// TFLOP/s; 4 chunks of up to 701 tokens over 12,000 175 us, 600).
+// see few tiles, whose starts and partial results nothing covers (2048 tokens 54 us, 394
+// TFLOP/s; 4 chunks of up to 701 tokens over 12,000 171 us, 614).
 
 struct ExpandedDev {
   const uint16_t *q, *k, *v, *rope;
@@ -906,11 +906,12 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
     };
     if (late) {
       load_keys(0, 0);
-      load_values(0, 0);
       load_keys(1, S::KEYS);
-      load_values(1, S::VTILE);
+      load_values(0, 0);
       load_keys(2, 2 * S::KEYS);
+      load_values(1, S::VTILE);
     }
+    if (tid < 2) *to_lds_at<uint32_t>(bad_at + 4 * tid) = 0;
     const int mine = 32 * wave + c;
     const bool live = mine < rows;
     u32x4_v q[KS];
@@ -1046,35 +1047,38 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
       auto next_keys = [](uint32_t x) { return x + S::KEYS == RING * S::KEYS ? 0u : x + S::KEYS; };
       auto next_values = [](uint32_t x) { return x + S::VTILE == RING * S::VTILE ? 0u : x + S::VTILE; };
       uint32_t keys = 0, values = 0;  // tile i's places
-      // loads go in batches, a tile's keys and the values of the one before; the first keys by themselves
+      // Loads go in batches, a tile's keys and the values of the one before; the first keys by themselves.
+      // The early half cleans a tile's values beside its softmax, so they are waited for a step
+      // before their products (prompts of 2048 and 4096 tokens 54 and 134 us; with a step of its own 59 and 144).
       if (late) {
         if (n > 2) wait_loads<2 * BATCH>();
         else wait_loads<0>();
       }
       __syncthreads();
-      if (late) __syncthreads();
+      if (late) {
+        if (n > 2) wait_loads<BATCH>();
+        else wait_loads<0>();
+        __syncthreads();
+      }
       products(std::false_type{}, std::true_type{}, 0, 0);
       for (int i = 0;; i++) {
         const bool all = whole(i);
-        if (late) {
-          if (i + 2 < n) wait_loads<BATCH>();
-          else wait_loads<0>();
-          if (!all && (tid & 255) < 2) *to_lds_at<uint32_t>(bad_at + 8 * (i & 1) + 4 * (tid & 1)) = 0;
-        }
         __syncthreads();
-        if (late && !all) {
-          clean(i, values);
-          __syncthreads();
-        }
         if (late) {
           const uint32_t k3 = keys, v2 = values >= S::VTILE ? values - S::VTILE : values + (RING - 1) * S::VTILE;
           load_keys(i + 3, k3);
           load_values(i + 2, v2);
         }
         softmax(i, all);
+        if (late) {
+          if (i + 3 < n) wait_loads<BATCH>();
+          else wait_loads<0>();
+        } else if (!all) {
+          clean(i, values);
+        }
         __syncthreads();
-        if (!late && !all) __syncthreads();  // the late half cleans the tile
         if (!all) poison(i);
+        if (tid < 2) *to_lds_at<uint32_t>(bad_at + 8 * (~i & 1) + 4 * tid) = 0;  // of the next tile
         if (i + 1 == n) break;
         const uint32_t k1 = next_keys(keys);
         products(std::true_type{}, std::true_type{}, values, k1);

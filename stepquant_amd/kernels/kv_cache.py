@@ -264,8 +264,8 @@ class BlockTables:
     # workgroup on a CU; a set of 128 has two.
     # Cut keys: absorbed, 1 to 4 least tiles are alike, and 2 and 4 for the parts (one request
     # of 1000 tokens 15.5 us, with 16 not cut 39); expanded, 4 to 16 for the parts (prompts of
-    # 8192 tokens 350 us, with 2, cut, 417; of 2048 60 us, with 24, not cut, 80; with 16 one of 1024
-    # 48 us, with 8 30) and least tiles of 4 (of 1024 30 us, with 2 33).
+    # 8192 tokens 348 us, with 2, cut, 405; of 2048 54 us, with 24, not cut, 77; with 16 one of 1024
+    # 44 us, with 8 28) and least tiles of 4 (of 1024 28 us, with 2 32).
     latent_min_tiles, latent_cut_tiles, latent_few_work = 2, 4, 3 << 14
     expanded_min_tiles, expanded_cut_tiles = 4, 8
 
