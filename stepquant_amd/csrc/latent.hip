@@ -388,7 +388,7 @@ struct Absorbed {
   static constexpr int W = W_, TK = 32, RG = RG_, NR = NR_, NW = 4 * RG, threads = 64 * NW, RING = W == 512 ? 4 : 6;
   static constexpr bool PAIR = PAIR_, HALVES = NR == 1;  // two waves share 16 rows' scores: half of the dims each
   static constexpr int R = 16 * RG * NR, TILE = TK * 2 * (W + kRope), SROW = 4 * TK, PROW = 2 * TK;
-  static constexpr size_t lds = RING * TILE + R * ((HALVES ? 2 : 1) * SROW + PROW + 4);
+  static constexpr size_t lds = RING * TILE + R * ((HALVES ? 2 : 1) * SROW + PROW + 4) + 16;
   static_assert(lds <= 163840, "LDS of a CU");
 };
 
@@ -414,6 +414,7 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
   const uint32_t scores = tiles_at + RING * TILE;  // [HALVES ? 2 : 1][R] rows of TK
   const uint32_t weights = scores + (S::HALVES ? 2 : 1) * R * SROW;  // [R] rows of TK
   const uint32_t factors = weights + R * PROW;     // [R]
+  const uint32_t bad_at = factors + 4 * R;         // [4] keys of a tile that the waves cleaned
   // Where a lane's operands lie: its key's steps of 32 dims (four of them 256 bytes;
   // the last two may be the rope key's), and its four keys of the wave's 16 dims of
   // every 64 (two of them 256 bytes, and four keys on a constant way).
@@ -587,16 +588,33 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
       if constexpr (NI > 0) *to_lds_at<f32x4_v>(score_to) = s[0] + s[1];
     };
     // What some row does not see has a weight of 0 there; infinities and NaN would
-    // still reach its outputs.  (Rows that see them have them in their scores.)
+    // still reach its outputs.  They are taken out, and rows that do see such a latent are
+    // NaN (its score may be -infinity, of which neither sum nor outputs would tell).
     auto clean = [&](int i, uint32_t slot) {
       const int first = u.kv0 + TK * i, r0 = known >> (i & 31) & 1 ? max(0, min(TK, all_hi - first)) : 0;
-      for (int j = r0 * (KD / 8) + (tid & 255); j < TK * (KD / 8); j += 256) {
-        const uint32_t at = tiles_at + slot + 16 * j;
+      uint32_t bad = 0;
+      for (int j = r0 * (W / 8) + (tid & 255); j < TK * (W / 8); j += 256) {
+        const int row = j / (W / 8);
+        const uint32_t at = tiles_at + slot + row * ROW + 16 * (j % (W / 8));
         u32x4_v w = *from_lds<u32x4_v>(at);
 #pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = only_finite<BF16>(w[k]);
+        for (int k = 0; k < 4; k++) {
+          const uint32_t x = only_finite<BF16>(w[k]);
+          bad |= x != w[k] ? 1u << row : 0u;
+          w[k] = x;
+        }
         *to_lds_at<u32x4_v>(at) = w;
       }
+      if (__any(bad != 0))
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) bad |= (uint32_t)__shfl_xor((int)bad, k, 64);
+      *to_lds_at<uint32_t>(bad_at + 4 * share) = bad;
+    };
+    auto poison = [&](int i) {
+      const int seen = known >> (i & 31) & 1 ? hi - (u.kv0 + TK * i) : 0;
+      const u32x4_v w = *from_lds<u32x4_v>(bad_at);
+      const uint32_t bad = w[0] | w[1] | w[2] | w[3];
+      if (seen > 0 && (bad & (seen >= TK ? ~0u : (1u << seen) - 1))) l = NAN;
     };
     auto softmax = [&](int i, bool all) {
       const int first = u.kv0 + TK * i;
@@ -660,6 +678,7 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
         }
         __syncthreads();
         if (RG == 2 && !late && !all) __syncthreads();  // the other group cleans the tile
+        if (!all) poison(i);
         if (i + 1 == n) break;
         const uint32_t following_slot = after_slot(slot);
         products(std::true_type{}, std::true_type{}, slot, following_slot);

@@ -191,6 +191,9 @@ class LatentCache:
         like ``q``, each row the weighted mean of the latents that its token sees (as
         the plan's ``causal`` says), zero where it sees none.  ``scale`` is that of
         the heads' own dims, which the latents do not tell.
+
+        What a token does not see does not reach it.  One that sees a latent that is
+        infinite or NaN has NaN in that dim, or, near where some token's sight ends, in all.
         """
         self._check_plan(plan)
         s = plan.latent.get("absorbed")
