@@ -35,11 +35,12 @@ constexpr float kNone = -3e38f;  // below every score
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLarge = 0x1p19f;  // scores from here on (in log2) hold few fractions
 
-// Weights are in units of 2^m, m at most kTop and, once it is set, kBias below the
+// Weights are in units of 2^m, m at most `top` and, once it is set, `bias` below the
 // largest score that the row has seen: it is raised only where a score passes
-// kTop, so that outputs are seldom rescaled.  A half then holds all bits of a
-// weight down to 2^-21 of the row's largest.
-constexpr float kBias = 7.f, kTop = 15.f;
+// `top`, so that outputs are seldom rescaled.  A half then holds all bits of a
+// weight down to 2^-21 of the row's largest.  Weights in bfloat16, whose range is that
+// of 32 bits, are 2^-36 of those: sums over a million of the largest values stay within
+// 32 bits, and products with values down to 2^-97 normal numbers.
 
 __device__ __forceinline__ int64_t load_index(const void *p, int dtype, int64_t i) {
   return dtype == SQ_I64 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
@@ -52,6 +53,7 @@ struct Half;
 template <>
 struct Half<true> {
   static constexpr uint32_t exponent = 0x7f80u;
+  static constexpr float bias = -29.f, top = -21.f;
   static __device__ __forceinline__ f32x4_v mul32(u32x4_v a, u32x4_v b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0, 0, 0);
   }
@@ -70,6 +72,7 @@ struct Half<true> {
 template <>
 struct Half<false> {
   static constexpr uint32_t exponent = 0x7c00u;
+  static constexpr float bias = 7.f, top = 15.f;
   static __device__ __forceinline__ f32x4_v mul32(u32x4_v a, u32x4_v b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_v, a), __builtin_bit_cast(half8_v, b), c, 0, 0, 0);
   }
@@ -632,8 +635,8 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
       for (int k = 1; k < KEYS; k++) best = fmaxf(best, x[k]);
       best = row_max<LANES>(best);
       float factor = 1.f;
-      if (best - m > kTop) {
-        const float raised = best - kBias;
+      if (best - m > H::top) {
+        const float raised = best - H::bias;
         factor = __builtin_amdgcn_exp2f(m - raised);
         m = raised;
         l *= factor;
@@ -948,7 +951,7 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
     // (a factor of 0 would make NaN of masked scores)
     const float mult = a.scale == 0.f ? 1e-37f : fabsf(a.scale) * kLog2e;
     // (rows that see none of the unit's keys keep a unit that no branch below is taken for)
-    float m = hi > kv0 ? kNone : 0.f, l = 0.f;
+    float m = hi > kv0 ? kNone : -H::bias, l = 0.f;
     bool poisoned = false;
     f32x16_v o[DT], s[2];
     u32x4_v p[4];
@@ -1039,8 +1042,9 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
       for (int k = 1; k < 32; k++) best = fmaxf(best, s[k >> 4][k & 15]);
       best = max2(best) * mult;
       float f = mult, less = m;
-      if (__any(fmaxf(best - m, fabsf(m) * 0x1p-16f) > kTop)) {  // (or scores past 2^19, m of which hold no fine fractions)
-        const float raised = best - m > kTop ? best - kBias : m, shrink = __builtin_amdgcn_exp2f(m - raised);
+      // (or scores past 2^19, m of which hold no fine fractions)
+      if (__any(fmaxf(best - m, fmaf(fabsf(m), 15.f / kLarge, H::top - 15.f)) > H::top)) {
+        const float raised = best - m > H::top ? best - H::bias : m, shrink = __builtin_amdgcn_exp2f(m - raised);
         m = less = raised;
         l *= shrink;
 #pragma unroll

@@ -85,3 +85,44 @@ def test_infinite_rope_keys_whose_scores_are_minus_infinity_weigh_nothing(heads,
         x = torch.where(keep[:, None], b.dense[0], 0.)
         out, bound = attention64(q, x, x[:, :512], seen, .05, U["bf16"])
         assert ((y[t].double() - out).abs() <= bound).all(), t
+
+
+# ---------------------------------------------------------------- large and small values
+def large(x, size):
+    """Values of ``size`` with one sign a dim."""
+    g = torch.Generator(device=dev()).manual_seed(3)
+    sign = torch.where(torch.rand(x.shape[-1], generator=g, device=dev()) < .5, -1., 1.)
+    return ((.3 + .7 * torch.rand(x.shape, generator=g, device=dev())) * sign * size).to(x.dtype)
+
+
+@pytest.mark.parametrize("heads,sizes,few", [(16, [(2000, 1), (3, 1)], None), (24, [(2000, 1)], None), (40, [(2000, 2)], 1),
+                                             (128, [(2000, 1), (0, 1)], 1), (128, [(200, 1)], None)])
+@pytest.mark.parametrize("size", [3.3e38, 1e33, 1e-25])
+@pytest.mark.parametrize("workgroups", [None, 2])
+def test_sums_of_latents_of_any_size(workgroups, size, heads, sizes, few, monkeypatch):
+    """Outputs are finite where latents are; queries that are 0 leave scores to the rope keys."""
+    if few:
+        monkeypatch.setattr(BlockTables, "latent_few_work", few)
+    b = Batch(sizes, heads=heads)
+    for d, i in zip(b.dense, b.plan.rows.tolist()):
+        d[:, :512] = large(d[:, :512], size)
+        n = torch.arange(len(d), device=dev())
+        b.cache.data.view(-1, 576)[b.tables.table[i, n // 64].long() * 64 + n % 64] = d
+    b.q.zero_()
+    if workgroups:  # few, so that each of them has many keys
+        b.tables._cus = workgroups
+        b.plan = b.tables.plan(b.new, b.plan.rows, absorbed=heads)
+    y = b.attend(scale=.3)
+    assert (y[0] != 0).all()
+    b.check(y, scale=.3)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sizes", [[(0, 300)], [(3000, 40), (0, 7)], [(2000, 700)]])
+@pytest.mark.parametrize("size", [3.3e38, 1e33, 1e-25])
+def test_sums_of_expanded_values_of_any_size(D, sizes, size):
+    p = Prompts(sizes, heads=2, D=D, shared=False)
+    p.v = large(p.v, size)
+    y = p.attend()
+    assert (y[:1] != 0).all()
+    p.check(y)
