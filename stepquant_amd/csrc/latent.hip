@@ -31,7 +31,8 @@ typedef __attribute__((address_space(3))) void *lds_t;
 
 constexpr int kRope = 64;
 constexpr int kTile = 64;        // keys of a plan's tile, and of the expanded form's
-constexpr float kNone = -3e38f;  // below every score
+constexpr float kNone = -3e38f;    // a row's unit before it has seen a finite score
+constexpr float kUnseen = -3.2e38f;  // before it has seen a key
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLarge = 0x1p19f;  // scores from here on (in log2) hold few fractions
 
@@ -86,6 +87,10 @@ struct Half<false> {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_v, w), (half2_v){(_Float16)1.f, (_Float16)1.f}, l, false);
   }
 };
+
+// What a row's outputs are multiplied by.  A row that sees nothing is zero; where it sees
+// keys and every weight is 0, all scores are -infinity and it is no number.
+__device__ __forceinline__ float inverse_sum(float sum, float m) { return sum != 0.f ? 1.f / sum : m < kNone ? 0.f : NAN; }
 
 __device__ __forceinline__ float max2(float x) {  // over the lanes l and l ^ 32
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -525,8 +530,8 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
     // the keys that the lane's row sees, and those that every row of the unit sees
     const int hi = mine >= u.rows ? 0 : a.causal ? min(u.kv1, u.pos0 + (u.f0 + mine) / G + 1) : u.kv1;
     const int all_hi = u.rows <= 0 ? 0 : a.causal ? min(u.kv1, u.pos0 + u.f0 / G + 1) : u.kv1;
-    float m = kNone, l = 0.f;
     auto whole = [&](int i) { return (known >> (i & 31) & 1) && u.kv0 + TK * (i + 1) <= all_hi; };
+    float m = whole(0) ? kNone : kUnseen, l = 0.f;
 
     // Outputs with the tile at `values` (OUT) and scores with the one at `keys` (IN), their products in turn;
     // operands are read some products ahead.
@@ -626,9 +631,10 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
       if constexpr (S::HALVES) x += *from_lds<vec>(score_at + R * SROW);
       x *= mult;
       if (!all) {
-        const int seen = known >> (i & 31) & 1 ? hi - first - KEYS * part : 0;
+        const int held = known >> (i & 31) & 1 ? hi - first : 0, seen = held - KEYS * part;
 #pragma unroll
         for (int k = 0; k < KEYS; k++) x[k] = k < seen ? x[k] : -INFINITY;
+        m = fmaxf(m, held > 0 ? kNone : kUnseen);
       }
       float best = x[0];
 #pragma unroll
@@ -710,7 +716,7 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
       const float unit = *from_lds<float>(weights + 4 * row), all = *from_lds<float>(weights + 4 * (R + row));
       if (row >= done.rows) continue;
       if (done.part < 0) {
-        const float f = all == 0.f ? 0.f : 1.f / all;
+        const float f = inverse_sum(all, unit);
         uint16_t *dst = a.out + (done.q0 * (int64_t)G + done.f0 + row) * W + d;
 #pragma unroll
         for (int e = 0; e < DB; e++) store4<BF16>(dst + 64 * e, o[r][e] * f);
@@ -751,7 +757,7 @@ __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
   if (j >= rows) return;
   const float *ml = a.ws + (int64_t)a.max_partials * a.unit_rows * W;
   f32x4_v x = {0, 0, 0, 0};
-  float sum = 0, mm = kNone;
+  float sum = 0, mm = kUnseen;
 #pragma unroll 4
   for (int i = grp; i < n; i += GR) {
     const int64_t slot = (int64_t)(p0 + i) * a.unit_rows + j;
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(512) void latent_merge_kernel(AbsorbedDev a) {
     x += part_o[i][lane] * w;
     sum = fmaf(part_s[i].y, w, sum);
   }
-  store4<BF16>(a.out + (q0 * (int64_t)a.heads + f0 + j) * W + d, x * (sum == 0.f ? 0.f : 1.f / sum));
+  store4<BF16>(a.out + (q0 * (int64_t)a.heads + f0 + j) * W + d, x * inverse_sum(sum, mm));
 }
 
 // The same of many rows, with a few parts each: a wave a row, so that a plan's merges that there
@@ -792,7 +798,7 @@ __global__ __launch_bounds__(512) void latent_merge_rows_kernel(AbsorbedDev a) {
   f32x4_v x[N];
 #pragma unroll
   for (int k = 0; k < N; k++) x[k] = (f32x4_v){0, 0, 0, 0};
-  float sum = 0, mm = kNone;
+  float sum = 0, mm = kUnseen;
 #pragma unroll 4
   for (int i = 0; i < n; i++) {
     const int64_t slot = (int64_t)(p0 + i) * a.unit_rows + j;
@@ -808,7 +814,7 @@ __global__ __launch_bounds__(512) void latent_merge_rows_kernel(AbsorbedDev a) {
   }
   uint16_t *dst = a.out + (q0 * (int64_t)a.heads + f0 + j) * W + 4 * lane;
 #pragma unroll
-  for (int k = 0; k < N; k++) store4<BF16>(dst + 256 * k, x[k] * (sum == 0.f ? 0.f : 1.f / sum));
+  for (int k = 0; k < N; k++) store4<BF16>(dst + 256 * k, x[k] * inverse_sum(sum, mm));
 }
 
 // ------------------------------------------------------------ expanded
@@ -1049,8 +1055,9 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
         l *= shrink;
 #pragma unroll
         for (int e = 0; e < DT; e++) o[e] *= shrink;
-        if (__any(fabsf(m) > kLarge)) {
+        if (__any(fabsf(m) > kLarge && m > kNone)) {
           // rounded before the difference, as the maximum is, so that no weight passes what a half holds
+          // (rows without a finite score need no such care, and leave the others' rounding as it is)
 #pragma unroll
           for (int k = 0; k < 32; k++) s[k >> 4][k & 15] = s[k >> 4][k & 15] * mult - m;
           f = 1.f, less = 0.f;
@@ -1114,7 +1121,7 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
     l = sum2(l);
     if (part < 0) {
       // through LDS, by the wave alone, so that whole rows go out 16 bytes a lane
-      const float f = poisoned ? NAN : l == 0.f ? 0.f : 1.f / l;
+      const float f = poisoned ? NAN : inverse_sum(l, hi > kv0 ? m : kUnseen);
       const uint32_t mine_at = at + wave * (32 * S::OUT);
 #pragma unroll
       for (int e = 0; e < DT; e++)
@@ -1147,7 +1154,7 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
       }
       if (live && hl == 0)
         *(float2 *)(a.ws + (int64_t)a.max_partials * a.heads * a.unit_rows * D + 2 * (slot * a.unit_rows + mine)) =
-            make_float2(hi > kv0 ? m : kNone, poisoned ? NAN : l);
+            make_float2(hi > kv0 ? m : kUnseen, poisoned ? NAN : l);
     }
     __syncthreads();  // before the next unit's tiles
   }
@@ -1167,7 +1174,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedDev a) {
   vec x[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = (vec)(0.f);
-  float sum = 0, mm = kNone;
+  float sum = 0, mm = kUnseen;
 #pragma unroll 2
   for (int i = 0; i < n; i++) {
     const int64_t slot = (int64_t)(p0 + i) * a.heads + h;
@@ -1182,7 +1189,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedDev a) {
     for (int k = 0; k < 4; k++) x[k] = x[k] * was + y[k] * w;
   }
   if (mine >= rows) return;
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  const float f = inverse_sum(sum, mm);
   uint16_t *dst = a.out + ((int64_t)(q0 + f0 + mine) * a.heads + h) * D;
 #pragma unroll
   for (int e = 0; e < DT; e++)

@@ -194,6 +194,8 @@ class LatentCache:
 
         What a token does not see does not reach it.  One that sees a latent that is
         infinite or NaN has NaN in that dim, or, near where some token's sight ends, in all.
+        Scores are held in 32 bits: a head with one above their range, or with none but
+        -infinity, is NaN.
         """
         self._check_plan(plan)
         s = plan.latent.get("absorbed")
@@ -231,7 +233,8 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
 
     What a token does not see does not reach it.  One that sees a value that is
     infinite or NaN has NaN in that dim, or, within 64 keys of where some token's
-    sight ends, in all.
+    sight ends, in all.  Scores are held in 32 bits: a head with one above their range,
+    or with none but -infinity, is NaN.
     """
     tables = plan.tables
     if v.dim() != 3 or v.shape[2] not in (64, 128) or v.dtype not in _HALVES or v.device != tables.device:

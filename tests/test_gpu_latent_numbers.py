@@ -126,3 +126,53 @@ def test_sums_of_expanded_values_of_any_size(D, sizes, size):
     y = p.attend()
     assert (y[:1] != 0).all()
     p.check(y)
+
+
+# ---------------------------------------------------------------- scores
+@pytest.mark.parametrize("heads,sizes,few", [(1, [(61, 4), (0, 1)], None), (16, [(61, 2), (0, 1)], None), (40, [(61, 2), (0, 1)], 1),
+                                             (16, [(3000, 4), (0, 2)], None), (128, [(3000, 1), (5, 1)], 1), (128, [(3000, 1)], None)])
+def test_rows_whose_scores_are_all_minus_infinity(heads, sizes, few, monkeypatch):
+    """Not a number, as the definition has it: only rows that see nothing are zero."""
+    if few:
+        monkeypatch.setattr(BlockTables, "latent_few_work", few)
+    b = Batch(sizes, heads=heads, padding=2)
+    for d, i in zip(b.dense, b.plan.rows.tolist()):
+        d[:, 512] = -1
+        n = torch.arange(len(d), device=dev())
+        b.cache.data.view(-1, 576)[b.tables.table[i, n // 64].long() * 64 + n % 64] = d
+    y = b.attend()
+    b.check(y)
+    clean = y.clone()
+    b.q_rope[0, 0, 0] = math.inf
+    b.q_rope[-2:, :, 0] = math.inf
+    y = b.attend()
+    assert torch.isnan(y[0, 0]).all() and not y[-2:].any()
+    assert torch.equal(y[0, 1:], clean[0, 1:]) and torch.equal(y[1:], clean[1:])
+
+
+@pytest.mark.parametrize("sizes", [[(0, 70)], [(6000, 100)], [(0, 1000)]])
+def test_expanded_rows_whose_scores_are_all_minus_infinity(sizes):
+    p = Prompts(sizes, heads=2, padding=3)
+    p.rope[:, 5] = -1
+    clean = p.attend()
+    p.check(clean)
+    p.q[[0, 40, 69], 1, 128 + 5] = math.inf
+    p.q[-3:, :, 128 + 5] = math.inf
+    y = p.attend()
+    keep = torch.ones(len(y), 2, dtype=torch.bool, device=dev())
+    keep[[0, 40, 69], 1] = False
+    assert torch.isnan(y[~keep]).all() and torch.equal(y[keep], clean[keep]) and not y[-3:].any()
+
+
+@pytest.mark.parametrize("heads", [1, 16, 128])
+def test_parts_whose_scores_are_all_minus_infinity(heads):
+    """Keys cut between workgroups, some of which see no finite score."""
+    b = Batch([(3000, 1)], heads=heads)
+    b.q_rope[..., 0] = 1
+    d, n = b.dense[0], torch.arange(3001, device=dev())
+    d[:2000, 512] = -math.inf
+    b.cache.data.view(-1, 576)[b.tables.table[b.plan.rows[0], n // 64].long() * 64 + n % 64] = d
+    y = b.attend()
+    out, bound = attention64(torch.cat([b.q[0], b.q_rope[0]], -1), d[2000:], d[2000:, :512],
+                             torch.ones(heads, 1001, dtype=torch.bool, device=dev()), .05, U["bf16"])
+    assert ((y[0].double() - out).abs() <= bound).all()
