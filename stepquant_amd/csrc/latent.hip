@@ -954,8 +954,8 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     const int hi = live ? a.causal ? min(kv1, pos0 + f0 + mine + 1) : kv1 : 0;
     const int all_hi = a.causal ? min(kv1, pos0 + f0 + 1) : kv1;  // keys that every row of the unit sees
-    // (a factor of 0 would make NaN of masked scores)
-    const float mult = a.scale == 0.f ? 1e-37f : fabsf(a.scale) * kLog2e;
+    // (a factor of 0 would make NaN of masked scores; the least number leaves no score past 2^-21)
+    const float mult = a.scale == 0.f ? 0x1p-149f : fabsf(a.scale) * kLog2e;
     // (rows that see none of the unit's keys keep a unit that no branch below is taken for)
     float m = hi > kv0 ? kNone : -H::bias, l = 0.f;
     bool poisoned = false;

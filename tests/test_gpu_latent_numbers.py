@@ -176,3 +176,11 @@ def test_parts_whose_scores_are_all_minus_infinity(heads):
     out, bound = attention64(torch.cat([b.q[0], b.q_rope[0]], -1), d[2000:], d[2000:, :512],
                              torch.ones(heads, 1001, dtype=torch.bool, device=dev()), .05, U["bf16"])
     assert ((y[0].double() - out).abs() <= bound).all()
+
+
+def test_a_scale_of_nothing_takes_the_mean_of_scores_of_any_size():
+    for sizes in ([(0, 100)], [(3000, 60)]):
+        p = Prompts(sizes, heads=2)
+        p.q = (p.q.float() * 1e18).to(torch.bfloat16)
+        p.k, p.rope = (p.k.float() * 1e18).to(torch.bfloat16), (p.rope.float() * 1e18).to(torch.bfloat16)
+        p.check(p.attend(scale=0.), 0.)
