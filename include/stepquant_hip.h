@@ -694,6 +694,7 @@ int sq_latent_gather(const sq_latent_cache *cache, const sq_latent_gather_args *
  *              type, strides multiples of 8, 16-byte aligned; out contiguous
  *   workspace  max_partials * rows * (latent + 2) floats, 16-byte aligned
  *   schedule   of one KV head (q_heads of them share it), rows 16, 32, 64 or 128, no window
+ *   scale      below 2e38 in size (times log2 e it stays within 32 bits)
  */
 typedef struct sq_latent_attend_args {
     const void *q;
@@ -726,6 +727,7 @@ int sq_latent_attend(const sq_latent_cache *cache, const sq_latent_attend_args *
  *              are not there are not seen)
  *   workspace  max_partials * heads * 256 * (dim + 2) floats, 16-byte aligned
  *   schedule   of as many KV heads as query heads, rows 256, no window
+ *   scale      below 2e38 in size
  */
 typedef struct sq_expanded_attend_args {
     const void *q;

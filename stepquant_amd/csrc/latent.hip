@@ -1341,7 +1341,7 @@ int sq_latent_attend(const sq_latent_cache *c, const sq_latent_attend_args *a, v
     return fail(SQ_EINVAL, "latent attend: strides must be multiples of 8 and starts 16-byte aligned");
   if (a->q_stride < 0 || a->q_head_stride < 0 || a->rope_stride < 0 || a->rope_head_stride < 0)
     return fail(SQ_EINVAL, "latent attend: negative stride");
-  if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(SQ_EINVAL, "latent attend: scale must be finite");
+  if (!(a->scale > -2e38f && a->scale < 2e38f)) return fail(SQ_EINVAL, "latent attend: scale must be finite, below 2e38");
   const sq_kv_schedule &s = a->schedule;
   rc = sq_internal_check_schedule(&s, a->tokens, 1);
   if (rc) return rc;
@@ -1374,7 +1374,7 @@ int sq_expanded_attend(const sq_expanded_attend_args *a, void *stream) {
     return fail(SQ_EINVAL, "expanded attention: negative stride");
   if (a->k_stride >= 1 << 24 || a->v_stride >= 1 << 24 || a->rope_stride >= 1 << 24)
     return fail(SQ_EINVAL, "expanded attention: rows of keys and values must be fewer than 2^24 elements apart");
-  if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(SQ_EINVAL, "expanded attention: scale must be finite");
+  if (!(a->scale > -2e38f && a->scale < 2e38f)) return fail(SQ_EINVAL, "expanded attention: scale must be finite, below 2e38");
   const sq_kv_schedule &s = a->schedule;
   const int rc = sq_internal_check_schedule(&s, a->tokens, a->batch);
   if (rc) return rc;

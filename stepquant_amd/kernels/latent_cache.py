@@ -52,8 +52,8 @@ def _near(x):
 
 def _scale(scale):
     scale = float(scale)
-    if not abs(scale) < 3e38:
-        raise ValueError("scale must be finite, below 3e38")
+    if not abs(scale) < 2e38:  # (kernels multiply it by log2 e)
+        raise ValueError("scale must be finite, below 2e38")
     return scale
 
 

@@ -184,3 +184,13 @@ def test_a_scale_of_nothing_takes_the_mean_of_scores_of_any_size():
         p.q = (p.q.float() * 1e18).to(torch.bfloat16)
         p.k, p.rope = (p.k.float() * 1e18).to(torch.bfloat16), (p.rope.float() * 1e18).to(torch.bfloat16)
         p.check(p.attend(scale=0.), 0.)
+
+
+@pytest.mark.parametrize("scale", [1.9e38, -1.9e38])
+def test_the_largest_scales_of_queries_of_nothing(scale):
+    b = Batch([(100, 2), (0, 1)], heads=20)
+    b.q.zero_(), b.q_rope.zero_()
+    b.check(b.attend(scale=scale), scale=scale)
+    p = Prompts([(0, 100)], heads=2)
+    p.q.zero_()
+    p.check(p.attend(scale=scale), scale)

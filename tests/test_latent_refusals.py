@@ -1,0 +1,24 @@
+"""Calls of latent attention that are refused before any launch, without a GPU."""
+import pytest
+
+from stepquant_amd import _native as N
+from stepquant_amd.kernels.latent_cache import _scale
+from tests.test_latent_surface import _cache, _schedule
+
+ABSORBED = dict(q=16, q_rope=16, out=16, workspace=16, table=16, requests=2, tokens=16, q_stride=4096, q_head_stride=512,
+                rope_stride=512, rope_head_stride=64, width=4, scale=1.)
+EXPANDED = dict(q=16, k=16, v=16, rope=16, out=16, workspace=16, cu=16, starts=16, tokens=16, rows=16, q_stride=1536,
+                q_head_stride=192, k_stride=1024, k_head_stride=128, v_stride=1024, v_head_stride=128, rope_stride=64, batch=2,
+                dim=128, dtype=N.F16, scale=1.)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -2.9e38])
+def test_scales_that_pass_32_bits_times_log2_e_are_refused(scale):
+    """Scores are powers of two: scale * log2(e) would be infinite, and no number where a score is 0."""
+    a = N.LatentAttend(**{**ABSORBED, "scale": scale}, schedule=_schedule())
+    assert N.lib().sq_latent_attend(_cache(), a, None) == -22 and b"scale" in N.lib().sq_last_error()
+    a = N.ExpandedAttend(**{**EXPANDED, "scale": scale}, schedule=_schedule(kv_heads=8, rows=256))
+    assert N.lib().sq_expanded_attend(a, None) == -22 and b"scale" in N.lib().sq_last_error()
+    with pytest.raises(ValueError, match="scale"):
+        _scale(scale)
+    assert _scale(1.9e38) == 1.9e38
