@@ -724,7 +724,8 @@ int sq_latent_attend(const sq_latent_cache *cache, const sq_latent_attend_args *
  *   cu         [batch + 1] the plan's first packed rows of queries
  *   starts     [batch + 1] the requests' first rows of keys; request b has
  *              starts[b + 1] - starts[b], at least what its tokens see (rows that
- *              are not there are not seen)
+ *              are not there are not seen); cu itself where keys are those of the
+ *              new tokens alone (requests that held others before are NaN)
  *   workspace  max_partials * heads * 256 * (dim + 2) floats, 16-byte aligned
  *   schedule   of as many KV heads as query heads, rows 256, no window
  *   scale      below 2e38 in size

@@ -958,7 +958,8 @@ __global__ __launch_bounds__(512, 2) void expanded_attend_kernel(ExpandedDev a) 
     const float mult = a.scale == 0.f ? 0x1p-149f : fabsf(a.scale) * kLog2e;
     // (rows that see none of the unit's keys keep a unit that no branch below is taken for)
     float m = hi > kv0 ? kNone : -H::bias, l = 0.f;
-    bool poisoned = false;
+    // (keys that are the plan's own new rows are not all that a request sees that held others before)
+    bool poisoned = a.starts == a.cu && pos0 > 0;
     f32x16_v o[DT], s[2];
     u32x4_v p[4];
 #pragma unroll

@@ -226,7 +226,8 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
     [rows, heads, dim] with ``dim`` 64 or 128, ``rope`` [rows, 64], one type
     (bf16 or fp16); the plan was made with ``expanded=heads``.  ``starts`` [B + 1]
     (int32) says where each request's rows begin, as ``LatentCache.gather``
-    returns it; default: the plan's ``cu``, where no request held tokens before.
+    returns it; default: the plan's ``cu``, keys and values of the new tokens alone, for
+    requests that held none before (others are NaN: they would see keys that are not there).
     Each token sees its request's rows up to its own position (all of them in a
     plan that is not ``causal``); the result is [tokens, heads, dim], zero where a
     token sees none.  ``scale`` defaults to ``(dim + 64) ** -0.5``.
@@ -258,8 +259,9 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
         if plan.tokens:
             raise ValueError(f"the plan was made without expanded={heads}")
         return out
-    if not rows:
-        return out.zero_()
+    if not rows:  # (none is read)
+        k = v = v.new_empty((1, heads, dim))
+        rope = rope.new_empty((1, ROPE))
     q, k, v, rope = _whole(q), _near(k), _near(v), _near(rope)
     ws = torch.empty(s.floats * (dim + 2), dtype=torch.float32, device=v.device)
     args = N.EXPANDED_ATTEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), out.data_ptr(), ws.data_ptr(), plan._cu,

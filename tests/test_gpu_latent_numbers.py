@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from stepquant_amd.kernels.kv_cache import BlockTables
+from stepquant_amd.kernels.latent_cache import expanded_attention
 from tests.helpers import dev
 from tests.test_gpu_latent import U, Batch, Prompts, attention64
 
@@ -194,3 +195,31 @@ def test_the_largest_scales_of_queries_of_nothing(scale):
     p = Prompts([(0, 100)], heads=2)
     p.q.zero_()
     p.check(p.attend(scale=scale), scale)
+
+
+# ---------------------------------------------------------------- keys that are not there
+@pytest.mark.parametrize("causal", [True, False])
+def test_requests_that_held_tokens_need_starts(causal):
+    """Without starts keys are the new tokens' alone: no numbers for requests that held
+    others before, the plan's own answer for the rest, zero past them."""
+    p = Prompts([(0, 100), (5, 70), (0, 300), (3000, 1), (1, 40)], heads=3, padding=2, causal=causal)
+    fresh = torch.cat([torch.arange(int(s) + o, int(s) + o + n) for s, o, n in zip(p.starts, p.old, p.new)]).to(dev())
+    p.k, p.v, p.rope = p.k[fresh], p.v[fresh], p.rope[fresh]
+    # (by the same plan: another may cut keys elsewhere and round otherwise)
+    alone = expanded_attention(p.q, p.k, p.v, p.rope, p.plan, p.plan.cu.clone())
+    y = expanded_attention(p.q, p.k, p.v, p.rope, p.plan)
+    at = 0
+    for o, n in zip(p.old, p.new):
+        if o:
+            assert torch.isnan(y[at:at + n]).all(), (o, n)
+        else:
+            assert torch.equal(y[at:at + n], alone[at:at + n]), (o, n)
+        at += n
+    assert not y[at:].any()
+
+
+def test_requests_that_held_tokens_without_any_rows():
+    p = Prompts([(0, 4), (9, 3)], heads=2, padding=1)
+    y = expanded_attention(p.q, p.k[:0], p.v[:0], p.rope[:0], p.plan)
+    assert not y[:4].any() and torch.isnan(y[4:7]).all() and not y[7:].any()
+    assert not expanded_attention(p.q, p.k[:0], p.v[:0], p.rope[:0], p.plan, p.starts).any()
