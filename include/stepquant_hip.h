@@ -649,6 +649,7 @@ typedef struct sq_latent_cache {
  * aligned) to `slots`; -1 and slots that the cache does not have are passed
  * over.  With `rotary` rope keys are turned to `positions` on the way; `rows`
  * (NULL: none; the cache's type) are turned in the same launch, the tokens' queries as a rule.
+ * They have a number of their own, and are turned beside no tokens too.
  */
 typedef struct sq_latent_append_args {
     const void *latent;

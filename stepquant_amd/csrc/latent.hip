@@ -1278,7 +1278,11 @@ int sq_latent_append(const sq_latent_cache *c, const sq_latent_append_args *a, c
   int rc = check_cache(c);
   if (rc) return rc;
   if (!a) return fail(SQ_EINVAL, "latent append: null arguments");
-  if (a->tokens == 0) return 0;
+  const bool turned = rows && rows->tokens;
+  if (turned && !r) return fail(SQ_EINVAL, "latent append: queries are turned by a rotary");
+  if (turned && rows->dtype != c->dtype) return fail(SQ_EINVAL, "latent append: queries have the cache's type");
+  if (r && r->dim > kRope) return fail(SQ_ESHAPE, "latent append: the rotation turns more dims than a rope key has");
+  if (a->tokens == 0) return turned ? sq_rotary_apply(r, rows, stream) : 0;
   if (!a->latent || !a->rope || !a->slots || a->tokens < 0) return fail(SQ_EINVAL, "latent append: null pointer or size");
   if ((a->latent_stride | a->rope_stride) & 7 || (((uintptr_t)a->latent | (uintptr_t)a->rope) & 15))
     return fail(SQ_EINVAL, "latent append: strides must be multiples of 8 and starts 16-byte aligned");
@@ -1291,14 +1295,11 @@ int sq_latent_append(const sq_latent_cache *c, const sq_latent_append_args *a, c
     rc = rotary::check(r);
     if (rc) return rc;
     if (!a->positions) return fail(SQ_EINVAL, "latent append: null positions");
-    if (r->dim > kRope) return fail(SQ_ESHAPE, "latent append: the rotation turns more dims than a rope key has");
     d.r = *r;
   }
-  if (rows && rows->tokens) {
-    if (!r) return fail(SQ_EINVAL, "latent append: queries are turned by a rotary");
+  if (turned) {
     rc = rotary::check_rows(r, rows);
     if (rc) return rc;
-    if (rows->dtype != c->dtype) return fail(SQ_EINVAL, "latent append: queries have the cache's type");
     d.q = *rows;
     d.q_lanes = rows->heads;
     const int64_t more = rows->tokens * rows->heads * rotary::row_items(*r, *rows, false);

@@ -1,12 +1,14 @@
 """Latent attention where latents, values or scores are infinite, or next to what
-their types hold (MI355X).  Tolerances as in ``test_gpu_latent``."""
+their types hold, and where operands are missing (MI355X).  Tolerances as in ``test_gpu_latent``."""
 import math
 
 import pytest
 import torch
 
+from stepquant_amd import _native as N
 from stepquant_amd.kernels.kv_cache import BlockTables
-from stepquant_amd.kernels.latent_cache import expanded_attention
+from stepquant_amd.kernels.latent_cache import LatentCache, expanded_attention
+from stepquant_amd.kernels.rotary import Rotary
 from tests.helpers import dev
 from tests.test_gpu_latent import U, Batch, Prompts, attention64
 
@@ -223,3 +225,17 @@ def test_requests_that_held_tokens_without_any_rows():
     y = expanded_attention(p.q, p.k[:0], p.v[:0], p.rope[:0], p.plan)
     assert not y[:4].any() and torch.isnan(y[4:7]).all() and not y[7:].any()
     assert not expanded_attention(p.q, p.k[:0], p.v[:0], p.rope[:0], p.plan, p.starts).any()
+
+
+def test_rows_beside_an_append_of_no_tokens():
+    """Rows that the C entry is given are turned, whatever it appends."""
+    rotary, cache = Rotary(64), LatentCache(4, 256)
+    x = torch.randn(7, 3, 64, device=dev()).to(torch.bfloat16)
+    positions = torch.arange(5, 12, device=dev(), dtype=torch.int32)
+    out = torch.zeros_like(x)
+    rows = N.RotaryRows(x=x.data_ptr(), out=out.data_ptr(), positions=positions.data_ptr(), tokens=7, x_stride=192,
+                        x_head_stride=64, out_stride=192, out_head_stride=64, heads=3, head_dim=64, dtype=N.BF16,
+                        positions_dtype=N.I32)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert N.lib().sq_latent_append(cache._latent, N.LatentAppend(tokens=0), rotary._desc, rows, stream) == 0
+    assert torch.equal(out, rotary.apply(x, positions)) and not cache.data.any()

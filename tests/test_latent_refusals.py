@@ -22,3 +22,16 @@ def test_scales_that_pass_32_bits_times_log2_e_are_refused(scale):
     with pytest.raises(ValueError, match="scale"):
         _scale(scale)
     assert _scale(1.9e38) == 1.9e38
+
+
+def test_appends_of_no_tokens_check_the_rows_that_they_turn():
+    """Rows may be turned beside an empty append, as beside the 8-bit cache's."""
+    L = N.lib()
+    rotary = lambda **kw: N.Rotary(**{**dict(turns=16, dim=64, magnitude=1.), **kw})
+    rows = lambda **kw: N.RotaryRows(**{**dict(x=16, out=16, positions=16, tokens=4, x_stride=512, x_head_stride=64,
+                                               out_stride=512, out_head_stride=64, heads=8, head_dim=64, dtype=N.BF16,
+                                               positions_dtype=N.I32), **kw})
+    call = lambda r, q: L.sq_latent_append(_cache(), N.LatentAppend(tokens=0), r, q, None)
+    assert call(None, rows()) == -22 and call(rotary(turns=None), rows()) == -22 and call(rotary(dim=80), rows(head_dim=80)) == -23
+    assert call(rotary(), rows(dtype=N.F16)) == -22 and call(rotary(), rows(x=None)) == -22 and call(rotary(), rows(tokens=-1)) == -22
+    assert call(rotary(), rows(tokens=0)) == 0 and call(rotary(), None) == 0 and call(None, None) == 0
