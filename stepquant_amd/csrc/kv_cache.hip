@@ -1840,8 +1840,9 @@ int check_schedule(const sq_kv_schedule *s, int64_t tokens, int64_t batch) {
   if (s->max_workers < larger || s->max_units < sets + slots || s->max_merges < smaller ||
       s->max_partials < 2 * slots || s->max_units >= 1 << 24)
     return fail(SQ_EINVAL, "kv schedule: room for workers, units, merges or partials");
-  // (a launch has fewer than 2^32 threads, 512 a workgroup)
-  if ((int64_t)s->max_workers * s->kv_heads >= 1 << 23 || (int64_t)s->max_merges * s->kv_heads >= 1 << 23)
+  // (a launch has fewer than 2^32 threads, 512 a workgroup; sets of 128 rows have two workgroups a worker, in eights)
+  const int64_t workgroups = s->rows == 128 ? 2 * ((int64_t)s->max_workers + 8) : s->max_workers;
+  if (workgroups * s->kv_heads >= 1 << 23 || (int64_t)s->max_merges * s->kv_heads >= 1 << 23)
     return fail(SQ_EINVAL, "kv schedule: workers * heads too large");
   return 0;
 }

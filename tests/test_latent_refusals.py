@@ -35,3 +35,10 @@ def test_appends_of_no_tokens_check_the_rows_that_they_turn():
     assert call(None, rows()) == -22 and call(rotary(turns=None), rows()) == -22 and call(rotary(dim=80), rows(head_dim=80)) == -23
     assert call(rotary(), rows(dtype=N.F16)) == -22 and call(rotary(), rows(x=None)) == -22 and call(rotary(), rows(tokens=-1)) == -22
     assert call(rotary(), rows(tokens=0)) == 0 and call(rotary(), None) == 0 and call(None, None) == 0
+
+
+def test_sets_of_128_rows_have_two_workgroups_to_count():
+    """A launch has fewer than 2^32 threads: 512 a workgroup, two workgroups a worker."""
+    fits = dict(rows=128, slots=128, max_workers=1 << 22, max_units=600, max_merges=256, max_partials=512, merge_rows=128)
+    a = N.LatentAttend(**ABSORBED, schedule=_schedule(**fits))
+    assert N.lib().sq_latent_attend(_cache(), a, None) == -22 and b"workers" in N.lib().sq_last_error()
