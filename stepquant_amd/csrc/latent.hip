@@ -264,14 +264,14 @@ __device__ __forceinline__ int weight_place(int row, int at) { return at ^ (row 
 
 // 16 bytes a lane from memory to LDS at `lds` + 16 lane.  The compiler does not
 // count these loads: it would wait for all of them before any write to LDS; the
-// waits are written out.  M0, which holds the place in LDS, has no other use in these kernels.
+// waits are written out.  M0 holds the place in LDS, and is to be there an instruction before.
 __device__ __forceinline__ void to_lds(uint32_t lds, const uint8_t *base, uint32_t offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // the same, of what nothing else will read (64 requests of up to 8192: 8% faster)
 __device__ __forceinline__ void to_lds_once(uint32_t lds, const uint8_t *base, uint32_t offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // a word that the whole wave reads and no kernel running beside writes, by the scalar cache
