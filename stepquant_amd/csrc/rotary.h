@@ -2,11 +2,12 @@
 //
 // Pair i of a head's first `dim` dims turns by position * f_i.  A frequency is
 // held as turns a position, a 64-bit fraction: its product with the position,
-// modulo 2^64, is the fraction of a turn that is left, exact to 2^-44 of a turn
-// at position 2^20, with no table of angles and no limit to the positions
-// (an angle in 32-bit floats is off by 0.004 rad at position 2^17).  Sine and
-// cosine are Taylor polynomials on an eighth of a turn either side, off by at
-// most 2.4e-7.
+// modulo 2^64, is the fraction of a turn that is left, off by position * 2^-65 of a
+// turn, with no table of angles and no longest position (position times frequency in
+// 32-bit floats is off by 0.004 rad at position 2^17).  The upper 32 bits of
+// the product, 2^-32 of a turn, become the angle, a float on an eighth of a turn either
+// side: 1.2e-7 rad off at most.  Sine and cosine are Taylor polynomials there, off by at most
+// 2.4e-7 with the angle's error.
 //
 // A thread takes 16 dims, 8 pairs: two 16-byte groups `dim / 2` apart in the
 // half layout, two adjacent ones in the interleaved layout.

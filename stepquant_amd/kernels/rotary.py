@@ -138,7 +138,8 @@ class Rotary:
     def apply(self, x, positions, *, out=None):
         """``x`` [tokens, heads, head_dim] (fp32, bf16 or fp16) turned to
         ``positions`` [tokens] (int32 or int64), of any size; rows at negative
-        positions stay as they are, and so do dims past the first ``dim``.
+        positions stay as they are, and so do dims past the first ``dim``.  Angles are off
+        by 1.2e-7 rad at most, and by position * 2^-65 of a turn more.
 
         The result is new and contiguous, or ``out`` (like ``x``, which it may be;
         otherwise they do not overlap).  Heads are contiguous inside; rows and heads
