@@ -340,9 +340,10 @@ __device__ __forceinline__ void store4(uint16_t *dst, f32x4_v x) {
 // What bounds it: with up to 32 rows (a decode step of 32 heads) the pages, 1152 bytes a token
 // that are read once.  64 requests of up to 8191 take 69 us, 4.9 TB/s; of equal lengths
 // it is 5.9 (16 heads 6.5; a large copy reaches 5, reading alone 6.5).  What is missing are
-// units' starts, which wait for queries and first tiles.  With 128 rows (32 requests of up to
+// units' starts, which wait for queries and all tiles under way, and the parts of cut keys, 20 MB
+// written and read again (311 of 314 units).  With 128 rows (32 requests of up to
 // 16,383: 144 us) it is the two steps below, 0.7 us each of a tile of 32 keys, in
-// which the matrix cores are busy for a third of the time: each waits for the barrier,
+// which the matrix cores are busy for a quarter of the time: each waits for the barrier,
 // for its weights and first operands from LDS, and for its last scores.
 
 struct AbsorbedDev {
@@ -390,7 +391,8 @@ __device__ __forceinline__ Unit read_unit(const AbsorbedDev &a, int i, int at_ro
 // the other waits for scores and exponentials; a barrier ends each step.  The
 // late group loads.  PAIR: units of 128 rows have two workgroups, which run
 // side by side on one XCD (8 apart, blocks go to the 8 in turn) so that its L2 gives one
-// of them the keys; others are read past the caches' later use.
+// of them the keys (349 MB of pages: half of the reads hit, 364 MB come from memory); others
+// are read past the caches' later use.
 template <int W_, int RG_, int NR_, bool PAIR_ = false>
 struct Absorbed {
   static constexpr int W = W_, TK = 32, RG = RG_, NR = NR_, NW = 4 * RG, threads = 64 * NW, RING = W == 512 ? 4 : 6;
@@ -523,7 +525,8 @@ __device__ __forceinline__ void absorbed_attend(const AbsorbedDev &a) {
     for (int r = 0; r < NR; r++)
 #pragma unroll
       for (int e = 0; e < DB; e++) o[r][e] = (f32x4_v){0, 0, 0, 0};
-    // (the queries' loads are waited for here, not by a wait for all loads in the loop)
+    // (the queries' loads are waited for here, and the tiles' that were issued before them, as loads
+    // return in order, but not those of later tiles by a wait in the loop)
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     const float mult = a.scale * kLog2e;
@@ -832,7 +835,9 @@ __global__ __launch_bounds__(512) void latent_merge_rows_kernel(AbsorbedDev a) {
 // 347 us, 990 TFLOP/s (16,384 tokens of 8 heads 645 to 663 us, 1036 to 1066; a large matrix product of the
 // library reaches 1364); less is reached where rows do not fill sets of 256 or
 // see few tiles, whose starts and partial results nothing covers (2048 tokens 54 us, 394
-// TFLOP/s; 4 chunks of up to 701 tokens over 12,000 171 us, 614).
+// TFLOP/s; 4 chunks of up to 701 tokens over 12,000 171 us, 614).  Heads of 64 dims are
+// bound by the softmax, which is as long for them (8192 tokens 241 us, 857 TFLOP/s; vector
+// instructions 47% of the cycles, products 37%).
 
 struct ExpandedDev {
   const uint16_t *q, *k, *v, *rope;

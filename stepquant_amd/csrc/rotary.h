@@ -193,7 +193,8 @@ __device__ __forceinline__ void rotate_rows(const sq_rotary &r, const sq_rotary_
 
 // Heads of a thread.  Four share their angles where there are enough items of 16 dims to fill the
 // GPU all the same: 2^17 of 128 dims take 3.9 us so and 3.7 one by one, 2^18
-// 5.7 and 6.5, 2^20 12.0 and 16.4, 2^22 50 and 59 (5.4 TB/s; a copy reaches 5).
+// 5.7 and 6.5, 2^20 12.0 and 16.4, 2^22 50 and 59 (5.4 TB/s; a copy reaches 5), in 16 bits.  Rows
+// of 32 bits follow the same rule: 2^18 items 9.2 us with the host's share, 2^20 27, 2^22 103 (5.2 TB/s).
 inline int heads_per_thread(const sq_rotary *r, const sq_rotary_rows *a) {
   return a->tokens * a->heads * row_items(*r, *a, true) >= (int64_t)1 << 18 ? 4 : 1;
 }
