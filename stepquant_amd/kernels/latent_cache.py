@@ -57,12 +57,25 @@ def _scale(scale):
     return scale
 
 
-def _output(out, shape, like):
+def _range(x):
+    at = x.data_ptr()
+    return at, at + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size() if x.numel() else at
+
+
+def _output(out, shape, like, *operands, in_place=None):
+    """``out``, or a new tensor; it lies over no operand, but may be ``in_place``."""
     if out is None:
         return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(shape)
     if out.shape != shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous {list(shape)} of the queries' type")
+    if in_place is not None and (in_place.data_ptr() != out.data_ptr() or not in_place.is_contiguous()):
+        operands += in_place,
+    start, end = _range(out)
+    for x in operands:
+        first, last = _range(x)
+        if first < last and first < end and start < last:
+            raise ValueError("out overlaps an operand")
     return out
 
 
@@ -190,7 +203,7 @@ class LatentCache:
         ``append`` of the same plan (made with ``absorbed=heads``); the result is
         like ``q``, each row the weighted mean of the latents that its token sees (as
         the plan's ``causal`` says), zero where it sees none.  ``scale`` is that of
-        the heads' own dims, which the latents do not tell.
+        the heads' own dims, which the latents do not tell.  ``out`` may be ``q``.
 
         What a token does not see does not reach it.  One that sees a latent that is
         infinite or NaN has NaN in that dim, or, near where some token's sight ends, in all.
@@ -207,7 +220,7 @@ class LatentCache:
             return _output(out, q.shape, q)
         q = self._like(q, (plan.tokens, s.q_heads, self.latent_dim), "queries")
         q_rope = self._like(q_rope, (plan.tokens, s.q_heads, self.rope_dim), "rope queries")
-        scale, out = _scale(scale), _output(out, q.shape, q)
+        scale, out = _scale(scale), _output(out, q.shape, q, q_rope, in_place=q)
         ws = self._words.new_empty((s.floats * (self.latent_dim + 2),))
         t = plan.tables
         args = N.LATENT_ATTEND.pack(q.data_ptr(), q_rope.data_ptr(), out.data_ptr(), ws.data_ptr(), t.table.data_ptr(),
@@ -230,7 +243,7 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
     requests that held none before (others are NaN: they would see keys that are not there).
     Each token sees its request's rows up to its own position (all of them in a
     plan that is not ``causal``); the result is [tokens, heads, dim], zero where a
-    token sees none.  ``scale`` defaults to ``(dim + 64) ** -0.5``.
+    token sees none.  ``scale`` defaults to ``(dim + 64) ** -0.5``.  ``out`` lies over no operand.
 
     What a token does not see does not reach it.  One that sees a value that is
     infinite or NaN has NaN in that dim, or, within 64 keys of where some token's
@@ -253,7 +266,7 @@ def expanded_attention(q, k, v, rope, plan, starts=None, *, scale=None, out=None
     else:
         starts_at = starts.data_ptr()
     scale = _scale((dim + ROPE) ** -.5 if scale is None else scale)
-    out = _output(out, (plan.tokens, heads, dim), q)
+    out = _output(out, (plan.tokens, heads, dim), q, q, k, v, rope)
     s = plan.latent.get("expanded")
     if s is None or s.q_heads != heads:
         if plan.tokens:

@@ -239,3 +239,20 @@ def test_rows_beside_an_append_of_no_tokens():
     stream = torch.cuda.current_stream().cuda_stream
     assert N.lib().sq_latent_append(cache._latent, N.LatentAppend(tokens=0), rotary._desc, rows, stream) == 0
     assert torch.equal(out, rotary.apply(x, positions)) and not cache.data.any()
+
+
+@pytest.mark.parametrize("heads,sizes,few", [(16, [(300, 1), (0, 2)], None), (40, [(300, 2), (5, 1)], 1), (128, [(300, 1)], 1), (24, [(5000, 3)], None),
+                                             (128, [(5000, 1), (70, 1)], 1)])
+def test_absorbed_outputs_may_take_the_place_of_queries(heads, sizes, few, monkeypatch):
+    if few:
+        monkeypatch.setattr(BlockTables, "latent_few_work", few)
+    b = Batch(sizes, heads=heads, padding=1)
+    want = b.attend()
+    assert torch.equal(b.attend(out=b.q), want) and torch.equal(b.q, want)
+
+
+def test_expanded_outputs_over_values_are_refused():
+    p = Prompts([(0, 100)], heads=2, shared=False)
+    for out in (p.v, p.k):
+        with pytest.raises(ValueError, match="overlap"):
+            p.attend(out=out)

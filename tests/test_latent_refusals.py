@@ -1,8 +1,9 @@
 """Calls of latent attention that are refused before any launch, without a GPU."""
 import pytest
+import torch
 
 from stepquant_amd import _native as N
-from stepquant_amd.kernels.latent_cache import _scale
+from stepquant_amd.kernels.latent_cache import _output, _scale
 from tests.test_latent_surface import _cache, _schedule
 
 ABSORBED = dict(q=16, q_rope=16, out=16, workspace=16, table=16, requests=2, tokens=16, q_stride=4096, q_head_stride=512,
@@ -42,3 +43,20 @@ def test_sets_of_128_rows_have_two_workgroups_to_count():
     fits = dict(rows=128, slots=128, max_workers=1 << 22, max_units=600, max_merges=256, max_partials=512, merge_rows=128)
     a = N.LatentAttend(**ABSORBED, schedule=_schedule(**fits))
     assert N.lib().sq_latent_attend(_cache(), a, None) == -22 and b"workers" in N.lib().sq_last_error()
+
+
+def test_outputs_that_lie_over_operands_are_refused():
+    """Workgroups still read the operands while others write; only absorbed queries, a row of
+    which no other row's workgroups read, may be where their outputs go."""
+    x = torch.zeros(6, 4, 192, dtype=torch.bfloat16)
+    out = x.view(-1)[:6 * 4 * 128].view(6, 4, 128)
+    other = torch.zeros(6, 4, 128, dtype=torch.bfloat16)
+    assert _output(other, (6, 4, 128), x, x, out) is other
+    for y in (x, x[..., 64:], x[3:], out, x[2:3, :, :8]):
+        with pytest.raises(ValueError, match="overlap"):
+            _output(out, (6, 4, 128), x, other, y)
+    assert _output(out, (6, 4, 128), x, x[:0], x[1:1]) is out and _output(out, (6, 4, 128), x, x.view(-1)[6 * 4 * 128:]) is out
+    assert _output(out, (6, 4, 128), x, in_place=out) is out
+    for y in (x.view(-1)[8:8 + 6 * 4 * 128].view(6, 4, 128), x[..., :128]):
+        with pytest.raises(ValueError, match="overlap"):
+            _output(out, (6, 4, 128), x, in_place=y)
