@@ -425,8 +425,8 @@ class KVCache:
         ``rotary`` (a ``Rotary`` of at most ``head_dim`` dims) turns the keys to the
         plan's positions on the way, in 32 bits; then ``q``, the same tokens'
         queries [tokens, q_heads, head_dim] (or [tokens, q_heads * head_dim]), are turned in the
-        same launch and returned, in ``out`` where it is given (which may be ``q``).
-        Rows without a slot come back as they are.
+        same launch and returned, in ``out`` where it is given (which may be ``q``, and lies
+        over no key or value: they are read meanwhile).  Rows without a slot come back as they are.
 
         Every page belongs to one request, as ``BlockTables`` gives them out: two
         requests that wrote to one page would race for its peaks.

@@ -141,8 +141,8 @@ class LatentCache:
         ``rotary`` (a ``Rotary`` of at most 64 dims) turns the rope keys to the
         plan's positions on the way; then ``q``, rows [tokens, heads, dim] such as the same
         tokens' rope queries, are turned in the same launch and returned, in ``out``
-        where it is given (which may be ``q``).  Rows without a slot come back as
-        they are.
+        where it is given (which may be ``q``, and lies over no latent or rope key: they
+        are read meanwhile).  Rows without a slot come back as they are.
         """
         self._check_plan(plan)
         latent = self._like(latent, (plan.tokens, self.latent_dim), "latents")
